@@ -961,6 +961,71 @@ int lp_moe_align(const int* idx, int n_pairs, int top, int E, int tile_rows, int
 int lp_moe_combine(const float* y, long long ldy, const int* pair_row, const float* w, int top, const float* shared, long long lds,
                    const float* gate, float* out, long long ldo, int T, int D, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Drafting: a tree of drafted tokens is attended over the cache in one step, verified against the target's probabilities, and the accepted
+ * nodes' rows become the cache's last ones; a draft model is trained on a teacher's top logits.  (The reference decodes one token a step.)
+ *
+ * Node 0 of a tree is the last certain token; a node's parent lies before it (parents[0] = -1), so children follow their parents.
+ * `nodes` (NULL: all T) gives each sequence's number of nodes: what lies behind is not read, nor written but where a call says so.
+ * ------------------------------------------------------------------------------------------------------------------ */
+#define LP_TREE_MAX_NODES 256
+/* mask[b][i][w], w < ceil(T / 64): bit j of the words of row i is set for node j = i and its ancestors; depth[b][i] (NULL: not wanted) is the number of
+ * these.  A parent that does not lie before its child ends the walk there.  parents int32 [B][ld]. */
+int lp_tree_mask(const int* parents, long long ld, int B, int T, unsigned long long* mask, int* depth, void* stream);
+
+/* out[b][i][h] = softmax_j(scale q[b][i][h] . k[j][g]) v[j][g] over the rows j < lengths[b] of the cache and, of the rows lengths[b] + n that hold the step's own
+ * nodes n < nodes[b], those whose bit is set in node i's words; g = h / (H / KVH).  All bf16, sums in fp32.  D = 64, 96 or 128.
+ * k, v: [n_pages][page_size][KVH][D] with the strides given in elements (multiples of 8, the last dimension contiguous, 16-byte aligned bases); row r of
+ * sequence b lies in page page_table[b][r / page_size] of `max_pages` a sequence (ld_table between sequences).  page_table NULL: page b (max_pages 1).  A page
+ * that is not in [0, n_pages) is not there: its rows are not seen.  Nor are rows past max_pages * page_size.  A row that sees nothing is zeros.
+ * What a row does not see has no effect on it, NaN and infinities among it.  Rows i >= nodes[b] of out are not written.
+ * workspace: lp_tree_attention_workspace_bytes(desc) bytes, 16-byte aligned, for this call alone until it has ended. */
+typedef struct lp_tree_attn_desc {
+  const void* q; long long q_batch, q_node, q_head;
+  const void* k; long long k_page, k_row, k_head;
+  const void* v; long long v_page, v_row, v_head;
+  void* out; long long o_batch, o_node, o_head;
+  const int* page_table; long long ld_table; int max_pages, n_pages, page_size;
+  const int* lengths; const int* nodes;
+  const unsigned long long* mask; long long mask_batch, mask_node; /* in words */
+  int B, T, H, KVH, D;
+  float scale;
+} lp_tree_attn_desc;
+size_t lp_tree_attention_workspace_bytes(const lp_tree_attn_desc* desc);
+int lp_tree_attention(const lp_tree_attn_desc* desc, void* workspace, size_t ws_bytes, void* stream);
+
+/* Speculative sampling over a tree, from given random numbers u in [0, 1): the walk starts at node 0 with P = target row 0.  The children c of the node where it
+ * stands are tried in their order: c is accepted when u[b][c] * q(x) < P(x), x = tokens[b][c] and q the draft's row of that node (draft NULL: drafts that
+ * were not drawn, q(x) = 1); the walk goes there with P = target row c.  A refused child takes P = max(P - q, 0) / its sum (draft NULL: P without x), unless
+ * nothing would be left.  Where no child is accepted the next token is the first v with P(0) + ... + P(v) > u[b][0] sum(P).
+ * path[b][T]: the accepted nodes, node 0 first, -1 behind them; count[b] their number (0 where nodes[b] is 0); next[b] the token (-1 where P has no
+ * sum).  Row i of target and draft, fp32 [V], is the distribution after node i; negative and NaN probabilities count as 0.  A token outside [0, V) is
+ * refused and takes nothing away.  Choices are made in 64 bits.  uniform fp32, tokens, parents [B][T] contiguous; T <= 1024. */
+int lp_verify_draft(const float* target, long long target_batch, long long target_row, const float* draft, long long draft_batch,
+                    long long draft_row, const long long* tokens, const int* parents, const float* uniform, const int* nodes, int B, int T,
+                    int V, int* path, int* count, long long* next, void* stream);
+
+/* Rows lengths[b] + path[b][j] of every pool move to rows lengths[b] + j, j < count[b], in place (path as lp_verify_draft gives it: rising; a list that does not
+ * rise leaves unspecified rows at those places).  pools: HOST array of n_pools device pointers, each [n_pages][page_size] rows of row_bytes
+ * bytes, strides in bytes; page table as in lp_tree_attention.  Entries and rows that are not there move nothing. */
+int lp_cache_compact(const void* const* pools, int n_pools, long long page_stride, long long row_stride, long long row_bytes, int n_pages,
+                     int page_size, const int* page_table, long long ld_table, int max_pages, const int* lengths, const int* path,
+                     long long ld_path, const int* count, int B, int T, void* stream);
+/* Page src[i] of every pool is copied to page dst[i], i < n (device lists; no page may be among both, nor twice among dst).  Entries that are not
+ * pages copy nothing. */
+int lp_cache_copy_pages(const void* const* pools, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
+                        const int* dst, int n, void* stream);
+
+/* Distillation from a teacher's K top logits a row (K <= 1024), beside lp_ce_fwd_bwd: with t = softmax(teacher / temperature) over the entries whose id lies in [0, V)
+ * and p = softmax(logits / temperature),
+ *   loss[r] = (1 - hard) temperature^2 sum_k t_k (log t_k - log p[id_k]) + hard * (cross entropy of target[r]),
+ *   dlogits[r] = weight[r] * its gradient, bf16; columns V..Vp-1 receive 0.
+ * Rows of weight 0 are zeros and their logits are not read.  A row without such entries has no first term, one whose target lies outside [0, V) no second (target
+ * NULL with hard 0).  ids int32 or int64 (ids_64), an id may come twice; teacher and logits fp32 or bf16. */
+int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long ld, const void* ids, int ids_64, long long ld_ids,
+                       const void* teacher, int teacher_fp32, long long ld_teacher, int K, const float* weight, const long long* target,
+                       float temperature, float hard, float* loss, void* dlogits, long long ldd, int rows, int V, int Vp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,7 @@ RETENTION_CHUNK = 32
 LATENT_SPLIT_ROWS = 16
 GEMM_SPLIT_BF16, GEMM_SPLIT_F32, GEMM_SPLIT_PLANES = 0, 1, 2
 LINEAR_W_CONSTANT = 0x100      # lp_linear: with an epilogue, for weights that nothing on the stream writes
+TREE_MAX_NODES = 256
 LINEAR_ROWS_MAX, LINEAR_ROWS_COLS = 8, 8      # lp_linear: up to this many rows stream the weights, a CTA to so many columns
 
 
@@ -131,6 +132,14 @@ class LatentDesc(C.Structure):
                 ("c_gain", _vp), ("eps", _f), ("inv_freq", _vp), ("rot_dims", _i), ("rot_layout", _i), ("rot_mscale", _f),
                 ("cache", _vp), ("page_size", _i), ("page_table", _vp), ("max_pages", _i), ("window", _i), ("scale", _f),
                 ("sink", _vp), ("gate", _vp), ("ldg", _ll)]
+
+
+class TreeAttnDesc(C.Structure):
+    """lp_tree_attn_desc (include/leopard_b200.h)."""
+    _fields_ = [("q", _vp), ("q_batch", _ll), ("q_node", _ll), ("q_head", _ll), ("k", _vp), ("k_page", _ll), ("k_row", _ll), ("k_head", _ll),
+                ("v", _vp), ("v_page", _ll), ("v_row", _ll), ("v_head", _ll), ("out", _vp), ("o_batch", _ll), ("o_node", _ll), ("o_head", _ll),
+                ("page_table", _vp), ("ld_table", _ll), ("max_pages", _i), ("n_pages", _i), ("page_size", _i), ("lengths", _vp), ("nodes", _vp),
+                ("mask", _vp), ("mask_batch", _ll), ("mask_node", _ll), ("B", _i), ("T", _i), ("H", _i), ("KVH", _i), ("D", _i), ("scale", _f)]
 
 
 class MLSTMDesc(C.Structure):
@@ -305,6 +314,13 @@ _SIGS = {
     "lp_moe_max_tiles": (_i, [_i, _i, _i]),
     "lp_moe_align": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "lp_moe_combine": (_i, [_vp, _ll, _vp, _vp, _i, _vp, _ll, _vp, _vp, _ll, _i, _i, _vp]),
+    "lp_tree_mask": (_i, [_vp, _ll, _i, _i, _vp, _vp, _vp]),
+    "lp_tree_attention_workspace_bytes": (_sz, [_P(TreeAttnDesc)]),
+    "lp_tree_attention": (_i, [_P(TreeAttnDesc), _vp, _sz, _vp]),
+    "lp_verify_draft": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "lp_cache_compact": (_i, [_vp, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _vp, _ll, _vp, _i, _i, _vp]),
+    "lp_cache_copy_pages": (_i, [_vp, _i, _ll, _ll, _i, _vp, _vp, _i, _vp]),
+    "lp_distill_fwd_bwd": (_i, [_vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _i, _vp, _vp, _f, _f, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "lp_profile_enable": (_i, [_i]),
     "lp_profile_read": (_i, [_vp, _i]),
 }
@@ -359,7 +375,8 @@ STREAM32_SYMBOLS = ("lp_last_error", "lp_abi_version", "lp_launch_count", "lp_li
                     "lp_moe_route_group_softmax")
 STREAM32_OPTIONAL = ("lp_gemm_bf16", "lp_split_rows", "lp_gemm_split", "lp_latent_expanded_workspace_bytes", "lp_latent_attend_expanded",
                      "lp_latent_route", "lp_window_prompt_count", "lp_gather_rows",
-                     "lp_window_prompt_workspace_bytes", "lp_window_attn_prompt", "lp_gemm_grouped", "lp_linear_split", "lp_gemm_linear")      # present in the native libraries, absent from the CPU-emulated build
+                     "lp_window_prompt_workspace_bytes", "lp_window_attn_prompt", "lp_gemm_grouped", "lp_linear_split", "lp_gemm_linear",
+                     "lp_cache_compact", "lp_cache_copy_pages")      # present in the native libraries, absent from the CPU-emulated build
 _stream32 = None
 
 

@@ -1,0 +1,320 @@
+// leopard_b200 — what drafting needs beside the attention of a tree (lp_treeattn.cu): which nodes of a tree see which, verification of the drafts against
+// the target's probabilities, and rows and pages of a cache moved in all layers at once.
+#include "lp_host.h"
+#include "../../include/leopard_b200.h"
+
+namespace lp {
+
+// ---- trees ---------------------------------------------------------------------------------------------------------
+// A node's word mask holds itself and its ancestors; its depth is the number of its ancestors.  A thread walks one node up to its root: parents lie before
+// their children (an entry that does not ends the walk), so a walk takes at most T steps.
+__global__ void __launch_bounds__(128)
+tree_mask_kernel(const int* __restrict__ parents, long long ldp, int T, int words, unsigned long long* __restrict__ mask, int* __restrict__ depth) {
+  const int b = blockIdx.y, i = blockIdx.x * 128 + threadIdx.x;
+  if (i >= T) return;
+  const int* p = parents + b * ldp;
+  unsigned long long* m = mask + ((long long)b * T + i) * words;
+  for (int w = 0; w < words; ++w) {
+    unsigned long long bits = 0;
+    for (int at = i; at >= 0;) {
+      if ((at >> 6) == w) bits |= 1ull << (at & 63);
+      const int up = p[at];
+      at = up < at ? up : -1;
+    }
+    m[w] = bits;
+  }
+  if (depth) {
+    int n = 0;
+    for (int at = i; at >= 0; ++n) {
+      const int up = p[at];
+      at = up < at ? up : -1;
+    }
+    depth[(long long)b * T + i] = n - 1;
+  }
+}
+
+// ---- verification --------------------------------------------------------------------------------------------------
+constexpr int VERIFY_MAX_NODES = 1024;
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+struct VerifyArgs {
+  const float* target; long long target_batch, target_row;
+  const float* draft; long long draft_batch, draft_row;
+  const long long* tokens; const int* parents; const float* uniform; const int* nodes;
+  int T, V;
+  int* path; int* count; long long* next;
+};
+
+// One sequence a CTA.  The walk over the nodes in their order is the walk down the tree, since children come after their parents: node c is tried when its
+// parent is where the walk stands, and accepted when u[c] q(x) < P(x), P the target's distribution there less what was refused before.  A refusal
+// takes P = max(P - q, 0) / sum.  P is not stored: a value of it is taken again from p, q and the sums of the refusals.
+// Everything is computed in 64 bits, so that the choices are those of the definition.
+__global__ void __launch_bounds__(1024)
+verify_kernel(const VerifyArgs a) {
+  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n = min(a.nodes ? a.nodes[b] : a.T, a.T);
+  int* path = a.path + (long long)b * a.T;
+  for (int i = tid; i < a.T; i += 1024) path[i] = -1;
+  if (n <= 0) {
+    if (tid == 0) { a.count[b] = 0; a.next[b] = -1; }
+    return;
+  }
+  __shared__ double red[32], inv[VERIFY_MAX_NODES];     // sums by warp; 1 / sum of each refusal at the node where the walk stands
+  __shared__ int tok[VERIFY_MAX_NODES];                 // ... and the token that was refused
+  __shared__ int s_pick;
+  const long long* tokens = a.tokens + (long long)b * a.T;
+  const int* parents = a.parents + (long long)b * a.T;
+  const float* u = a.uniform + (long long)b * a.T;
+  const float* p = a.target + b * a.target_batch;
+  const float* q = a.draft ? a.draft + b * a.draft_batch : nullptr;
+  int cur = 0, refused = 0, count = 1;
+  auto left = [&](long long v) {                        // P(v)
+    double x = (double)p[v];
+    x = x > 0.0 ? x : 0.0;
+    const double d = q && refused ? (double)q[v] : 0.0;
+    for (int k = 0; k < refused; ++k) {
+      x -= q ? d : (v == tok[k] ? 1.0 : 0.0);
+      x = x > 0.0 ? x * inv[k] : 0.0;
+    }
+    return x;
+  };
+  const int part = ((a.V + 31) / 32 + 31) & ~31;        // a warp's range of the vocabulary
+  const int v0 = min(a.V, warp * part), v1 = min(a.V, v0 + part);
+  auto mass = [&]() {                                   // sum of P; red[] holds the warps' shares
+    double s = 0.0;
+    for (int v = v0 + lane; v < v1; v += 32) s += left(v);
+    s = warp_sum_f64(s);
+    __syncthreads();
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < 32; ++w) t += red[w];
+    return t;
+  };
+  __syncthreads();
+  if (tid == 0) path[0] = 0;
+  for (int c = 1; c < n; ++c) {
+    if (parents[c] != cur) continue;
+    const long long x = tokens[c];
+    const bool in = x >= 0 && x < a.V;
+    const double qx = !in ? 1.0 : q ? (double)q[x] : 1.0;
+    if (in && (double)u[c] * qx < left(x)) {
+      cur = c;
+      refused = 0;
+      p = a.target + b * a.target_batch + c * a.target_row;
+      if (q) q = a.draft + b * a.draft_batch + c * a.draft_row;
+      if (tid == 0) path[count] = c;
+      ++count;
+      continue;
+    }
+    if (!in) continue;                                  // no token of the vocabulary: nothing to take away
+    __syncthreads();
+    if (tid == 0) { tok[refused] = (int)x; inv[refused] = 1.0; }
+    __syncthreads();
+    ++refused;
+    const double s = mass();
+    if (s > 0.0) {
+      if (tid == 0) inv[refused - 1] = 1.0 / s;
+    } else {
+      --refused;                                        // nothing would be left: P stays
+    }
+    __syncthreads();
+  }
+  // the next token: the first whose running sum is above u[0] of the whole
+  const double total = mass(), goal = (double)u[0] * total;
+  if (tid == 0) s_pick = 0x7fffffff;
+  double before = 0.0;
+  for (int w = 0; w < warp; ++w) before += red[w];
+  __syncthreads();
+  const bool mine = before + red[warp] > goal && !(before > goal);
+  int last = -1;                                        // of a warp's range: its last token that has any probability
+  if (mine) {
+    int found = -1;
+    double run = before;
+    for (int v = v0; v < v1 && found < 0; v += 32) {
+      const double x = v + lane < v1 ? left(v + lane) : 0.0;
+      double s = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && run + s > goal), any = __ballot_sync(0xffffffffu, x > 0.0);
+      if (hit) found = v + __ffs(hit) - 1;
+      if (any) last = v + 31 - __clz(any);
+      run += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (found < 0) found = last;                        // the sums' last bits: the range's own total was above the goal
+    if (lane == 0 && found >= 0) atomicMin(&s_pick, found);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    a.count[b] = count;
+    a.next[b] = s_pick == 0x7fffffff ? -1 : s_pick;
+  }
+}
+
+// ---- rows of a cache -----------------------------------------------------------------------------------------------
+// where the pools of a call start, by value
+constexpr int POOLS_MAX = 256;
+struct Pools {
+  unsigned long long base[POOLS_MAX];
+};
+
+// Accepted row path[j] of a sequence moves to place j behind its cached rows.  A thread takes one piece of the row through all moves in their order, ROWS_DEEP loads
+// ahead of the stores: path rises, so path[j] >= j and a store never hits a row that a later move still has to read.
+constexpr int ROWS_DEEP = 8;
+template <typename U>
+__global__ void __launch_bounds__(128)
+cache_compact_kernel(const __grid_constant__ Pools pools, long long page_stride, long long row_stride, int units, int n_pages, int page_size,
+                     const int* __restrict__ table, long long ld_table, int max_pages, const int* __restrict__ lengths,
+                     const int* __restrict__ path, long long ld_path, const int* __restrict__ count, int T) {
+  const int b = blockIdx.z;
+  const int n = min(count[b], T), len = lengths[b];
+  if (len < 0) return;
+  char* base = reinterpret_cast<char*>(pools.base[blockIdx.y]);
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= units) return;
+  const int* order = path + b * ld_path;
+  auto place = [&](int i) -> char* {
+    const long long row = (long long)len + i;
+    const long long logical = row / page_size;
+    if (i < 0 || logical >= max_pages) return nullptr;
+    const int page = table ? table[b * ld_table + logical] : b;
+    if (page < 0 || page >= n_pages) return nullptr;
+    return base + page * page_stride + (row - logical * page_size) * row_stride + (long long)c * sizeof(U);
+  };
+  for (int j0 = 0; j0 < n; j0 += ROWS_DEEP) {
+    U held[ROWS_DEEP];
+    char* to[ROWS_DEEP];
+#pragma unroll
+    for (int k = 0; k < ROWS_DEEP; ++k) {
+      to[k] = nullptr;
+      const int j = j0 + k;
+      if (j >= n) continue;
+      const int i = order[j];
+      if (i == j || i < 0) continue;
+      const char* from = place(i);
+      to[k] = place(j);
+      if (from == nullptr) to[k] = nullptr;
+      if (to[k]) held[k] = *reinterpret_cast<const U*>(from);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS_DEEP; ++k)
+      if (to[k]) *reinterpret_cast<U*>(to[k]) = held[k];
+  }
+}
+
+// Pages src[i] -> dst[i] of every pool: a CTA copies up to PAGE_PIECES pieces of one page.
+constexpr int PAGE_PIECES = 1024;
+template <typename U>
+__global__ void __launch_bounds__(256)
+cache_pages_kernel(const __grid_constant__ Pools pools, long long page_stride, long long units, int n_pages, const int* __restrict__ src,
+                   const int* __restrict__ dst) {
+  const int s = src[blockIdx.z], d = dst[blockIdx.z];
+  if (s < 0 || s >= n_pages || d < 0 || d >= n_pages || s == d) return;
+  char* base = reinterpret_cast<char*>(pools.base[blockIdx.y]);
+  const U* from = reinterpret_cast<const U*>(base + s * page_stride);
+  U* to = reinterpret_cast<U*>(base + d * page_stride);
+  const long long at = (long long)blockIdx.x * PAGE_PIECES + threadIdx.x;
+  U held[PAGE_PIECES / 256];
+#pragma unroll
+  for (int k = 0; k < PAGE_PIECES / 256; ++k)
+    if (at + k * 256 < units) held[k] = from[at + k * 256];
+#pragma unroll
+  for (int k = 0; k < PAGE_PIECES / 256; ++k)
+    if (at + k * 256 < units) to[at + k * 256] = held[k];
+}
+
+// the widest piece that a list of addresses and sizes is a multiple of
+static int piece_bytes(const void* const* pools, int n, long long a, long long b, long long c) {
+  unsigned long long all = (unsigned long long)a | (unsigned long long)b | (unsigned long long)c;
+  for (int i = 0; i < n; ++i) all |= reinterpret_cast<unsigned long long>(pools[i]);
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+}
+
+}  // namespace lp
+
+extern "C" int lp_tree_mask(const int* parents, long long ld, int B, int T, unsigned long long* mask, int* depth, void* stream_) {
+  using namespace lp;
+  LP_REQUIRE(parents && mask && B > 0 && B <= 65535 && T > 0 && T <= LP_TREE_MAX_NODES && ld >= T,
+             "lp_tree_mask: bad arguments B=%d T=%d (at most %d nodes) ld=%lld", B, T, LP_TREE_MAX_NODES, ld);
+  note_launch();
+  tree_mask_kernel<<<dim3((T + 127) / 128, B), 128, 0, reinterpret_cast<cudaStream_t>(stream_)>>>(parents, ld, T, (T + 63) / 64, mask, depth);
+  LP_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int lp_verify_draft(const float* target, long long target_batch, long long target_row, const float* draft, long long draft_batch,
+                               long long draft_row, const long long* tokens, const int* parents, const float* uniform, const int* nodes, int B, int T,
+                               int V, int* path, int* count, long long* next, void* stream_) {
+  using namespace lp;
+  LP_REQUIRE(target && tokens && parents && uniform && path && count && next, "lp_verify_draft: null argument");
+  LP_REQUIRE(B > 0 && T > 0 && T <= VERIFY_MAX_NODES && V > 0, "lp_verify_draft: bad sizes B=%d T=%d (at most %d nodes) V=%d", B, T, VERIFY_MAX_NODES, V);
+  VerifyArgs a = {target, target_batch, target_row, draft, draft_batch, draft_row, tokens, parents, uniform, nodes, T, V, path, count, next};
+  note_launch();
+  verify_kernel<<<B, 1024, 0, reinterpret_cast<cudaStream_t>(stream_)>>>(a);
+  LP_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int lp_cache_compact(const void* const* pools, int n_pools, long long page_stride, long long row_stride, long long row_bytes, int n_pages,
+                                int page_size, const int* table, long long ld_table, int max_pages, const int* lengths, const int* path,
+                                long long ld_path, const int* count, int B, int T, void* stream_) {
+  using namespace lp;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  LP_REQUIRE(pools && lengths && path && count && n_pools > 0 && B > 0 && B <= 65535 && T > 0, "lp_cache_compact: bad arguments n_pools=%d B=%d T=%d", n_pools, B, T);
+  LP_REQUIRE(n_pages > 0 && page_size > 0 && row_bytes > 0 && row_stride >= row_bytes && ld_path >= T && max_pages > 0 && (table == nullptr || ld_table >= max_pages),
+             "lp_cache_compact: bad layout n_pages=%d page_size=%d row %lld of %lld bytes, %d pages a sequence", n_pages, page_size, row_bytes, row_stride, max_pages);
+  LP_REQUIRE(table != nullptr || (max_pages == 1 && B <= n_pages), "lp_cache_compact: %d sequences without a page table need a page each, there are %d", B, n_pages);
+  const int u = piece_bytes(pools, n_pools, page_stride, row_stride, row_bytes);
+  const long long units = row_bytes / u;
+  LP_REQUIRE(units < (1 << 30), "lp_cache_compact: rows of %lld bytes are too wide", row_bytes);
+  for (int at = 0; at < n_pools; at += POOLS_MAX) {
+    const int m = n_pools - at < POOLS_MAX ? n_pools - at : POOLS_MAX;
+    Pools list;
+    for (int i = 0; i < m; ++i) list.base[i] = reinterpret_cast<unsigned long long>(pools[at + i]);
+    const dim3 grid((unsigned)((units + 127) / 128), m, B);
+    note_launch();
+#define LP_COMPACT(U) cache_compact_kernel<U><<<grid, 128, 0, stream>>>(list, page_stride, row_stride, (int)units, n_pages, page_size, table, ld_table, max_pages, lengths, path, ld_path, count, T)
+    if (u == 16) LP_COMPACT(uint4);
+    else if (u == 4) LP_COMPACT(unsigned);
+    else if (u == 2) LP_COMPACT(unsigned short);
+    else LP_COMPACT(unsigned char);
+#undef LP_COMPACT
+    LP_CHECK_CUDA(cudaGetLastError());
+  }
+  return 0;
+}
+
+extern "C" int lp_cache_copy_pages(const void* const* pools, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
+                                   const int* dst, int n, void* stream_) {
+  using namespace lp;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  LP_REQUIRE(pools && src && dst && n_pools > 0 && n_pages > 0 && n >= 0 && n <= 65535, "lp_cache_copy_pages: bad arguments n_pools=%d n_pages=%d n=%d", n_pools, n_pages, n);
+  LP_REQUIRE(page_bytes > 0 && page_stride >= page_bytes, "lp_cache_copy_pages: pages of %lld bytes, %lld apart", page_bytes, page_stride);
+  if (n == 0) return 0;
+  const int u = piece_bytes(pools, n_pools, page_stride, page_bytes, 0);
+  const long long units = page_bytes / u, ctas = (units + PAGE_PIECES - 1) / PAGE_PIECES;
+  LP_REQUIRE(ctas < (1LL << 31), "lp_cache_copy_pages: pages of %lld bytes are too large", page_bytes);
+  for (int at = 0; at < n_pools; at += POOLS_MAX) {
+    const int m = n_pools - at < POOLS_MAX ? n_pools - at : POOLS_MAX;
+    Pools list;
+    for (int i = 0; i < m; ++i) list.base[i] = reinterpret_cast<unsigned long long>(pools[at + i]);
+    const dim3 grid((unsigned)ctas, m, n);
+    note_launch();
+#define LP_PAGES(U) cache_pages_kernel<U><<<grid, 256, 0, stream>>>(list, page_stride, units, n_pages, src, dst)
+    if (u == 16) LP_PAGES(uint4);
+    else if (u == 4) LP_PAGES(unsigned);
+    else if (u == 2) LP_PAGES(unsigned short);
+    else LP_PAGES(unsigned char);
+#undef LP_PAGES
+    LP_CHECK_CUDA(cudaGetLastError());
+  }
+  return 0;
+}

@@ -522,3 +522,239 @@ def parity_softmax_(scores, Tk, scale, causal):
     _lib.check(_lib.lib().lp_parity_softmax(_lib.ptr(scores), scores.stride(0), scores.shape[0], Tk, float(scale),
                                             1 if causal else 0, _lib.stream_ptr()), "lp_parity_softmax")
     return scores
+
+
+# ---- drafting (csrc/lp_treeattn.cu, lp_draft.cu, lp_distill.cu): trees of drafted tokens over a cache, their verification, the accepted rows, and the loss
+# that trains a draft model.  Calls run on the current stream of the tensors' device. ---------------------------------------------------------------------------
+def _chk_cuda(t, name, dtypes, dim=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
+        what = "/".join(str(d).replace("torch.", "") for d in dtypes)
+        raise TypeError(f"{name} must be a CUDA {what} tensor, got " + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
+    if dim is not None and t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
+
+
+def _chk_int32(t, name, shape, device, contiguous=True):
+    _chk_cuda(t, name, (torch.int32,))
+    if tuple(t.shape) != tuple(shape) or t.device != device or (contiguous and not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+
+
+def _overlaps(a, b):
+    """whether two tensors' spans of memory meet"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def tree_mask(parents):
+    """parents int32 [B, T] (node 0 the last certain token, parents[b, 0] = -1, a parent lies before its children) -> (mask int64 [B, T, ceil(T / 64)], the
+    bits of each node and its ancestors; depth int32 [B, T], its position behind the cached rows) (lp_tree_mask).  T <= 256."""
+    _chk_cuda(parents, "parents", (torch.int32,), 2)
+    if parents.stride(1) != 1 and parents.shape[1] > 1:
+        raise ValueError("parents must have a contiguous last dimension")
+    B, T = parents.shape
+    mask = torch.empty((B, T, -(-T // 64)), dtype=torch.int64, device=parents.device)
+    depth = torch.empty((B, T), dtype=torch.int32, device=parents.device)
+    if B == 0 or T == 0:
+        return mask, depth
+    with torch.cuda.device(parents.device):
+        _lib.check(_lib.lib().lp_tree_mask(_lib.ptr(parents), max(parents.stride(0), T), B, T, _lib.ptr(mask), _lib.ptr(depth), _lib.stream_ptr()), "lp_tree_mask")
+    return mask, depth
+
+
+def tree_attention(q, k, v, lengths, mask, nodes=None, page_table=None, scale=None, out=None):
+    """Attention of the step's nodes over a cache that holds their keys and values behind the rows of the past (lp_tree_attention):
+    q bf16 [B, T, H, D]; k, v bf16 [pages, page_size, KVH, D] (page_table int32 [B, max_pages]; -1: not there) or [B, rows, KVH, D]; lengths int32 [B], rows
+    of the past, seen by every node; mask int64 [B, T, ceil(T / 64)] (tree_mask), the nodes that a node sees: node n is row lengths[b] + n; nodes
+    int32 [B] or None, nodes of each sequence.  Strides are free but for a contiguous last dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of nodes
+    that a sequence does not have stay as they were (`out` given) or are unspecified.  A node that sees nothing is zeros."""
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        _chk_cuda(t, n, (torch.bfloat16,), 4)
+    B, T, H, D = q.shape
+    P, S, KVH, Dk = k.shape
+    dev = q.device
+    if Dk != D or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if out is None:
+        out = torch.empty((B, T, H, D), dtype=torch.bfloat16, device=dev)
+    _chk_cuda(out, "out", (torch.bfloat16,), 4)
+    if out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    _chk_cuda(mask, "mask", (torch.int64,), 3)
+    if tuple(mask.shape) != (B, T, -(-T // 64)):
+        raise ValueError(f"mask must be [B, T, ceil(T / 64)] = {(B, T, -(-T // 64))}, got {tuple(mask.shape)}")
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out"), (mask, "mask")):
+        if t.device != dev:
+            raise ValueError(f"{n} is on {t.device}, q on {dev}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{n} must have a contiguous last dimension")
+    _chk_int32(lengths, "lengths", (B,), dev)
+    if nodes is not None:
+        _chk_int32(nodes, "nodes", (B,), dev)
+    if page_table is not None:
+        _chk_cuda(page_table, "page_table", (torch.int32,), 2)
+        if page_table.shape[0] != B or page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"page_table must be int32 [{B}, max_pages] with contiguous rows on {dev}, got {tuple(page_table.shape)} on {page_table.device}")
+    elif P < B:
+        raise ValueError(f"{B} sequences need a page table or a cache of their own each, k holds {P}")
+    if B == 0 or T == 0:
+        return out
+    if any(_overlaps(out, t) for t in (q, k, v)):
+        raise ValueError("out must not share memory with q, k or v")
+    max_pages = 1 if page_table is None else page_table.shape[1]
+
+    def strides(t):      # of a dimension of one any number may stand there
+        return [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride())]
+    d = _lib.TreeAttnDesc(q.data_ptr(), *strides(q), k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), out.data_ptr(), *strides(out),
+                          None if page_table is None else page_table.data_ptr(), 0 if page_table is None else max(page_table.stride(0), max_pages), max_pages, P, S,
+                          lengths.data_ptr(), None if nodes is None else nodes.data_ptr(), mask.data_ptr(), mask.stride(0), mask.stride(1), B, T, H, KVH, D,
+                          D ** -0.5 if scale is None else float(scale))
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        ws = torch.empty(max(L.lp_tree_attention_workspace_bytes(C.byref(d)), 16), dtype=torch.uint8, device=dev)
+        _lib.check(L.lp_tree_attention(C.byref(d), _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "lp_tree_attention")
+    return out
+
+
+def verify_draft(target, tokens, parents, uniform, draft=None, nodes=None):
+    """Which drafted nodes the target accepts, and the token after them (lp_verify_draft): target fp32 [B, T, V], row i the target's probabilities after node i;
+    draft of the same shape, what the children of node i were drawn from (None: drafts that were not drawn, such as the best of a list); tokens
+    int64, parents int32, uniform fp32 (numbers in [0, 1): [b, c] tries node c, [b, 0] takes the next token) [B, T]; nodes int32 [B] or None.
+    -> (path int32 [B, T]: the accepted nodes from node 0 on, then -1; count int32 [B]; next token int64 [B])."""
+    _chk_cuda(target, "target", (torch.float32,), 3)
+    B, T, V = target.shape
+    dev = target.device
+    for t, n, kinds in ((tokens, "tokens", (torch.int64,)), (parents, "parents", (torch.int32,)), (uniform, "uniform", (torch.float32,))):
+        _chk_cuda(t, n, kinds)
+        if tuple(t.shape) != (B, T) or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous [{B}, {T}] on {dev}, got {tuple(t.shape)} on {t.device}")
+    if draft is not None:
+        _chk_cuda(draft, "draft", (torch.float32,), 3)
+        if draft.shape != target.shape or draft.device != dev:
+            raise ValueError(f"draft must be {tuple(target.shape)} on {dev}, got {tuple(draft.shape)} on {draft.device}")
+    for t, n in ((target, "target"), (draft, "draft")):
+        if t is not None and V > 1 and t.stride(2) != 1:
+            raise ValueError(f"{n} must have a contiguous last dimension")
+    if nodes is not None:
+        _chk_int32(nodes, "nodes", (B,), dev)
+    path = torch.empty((B, T), dtype=torch.int32, device=dev)
+    count = torch.empty((B,), dtype=torch.int32, device=dev)
+    token = torch.empty((B,), dtype=torch.int64, device=dev)
+    if B == 0:
+        return path, count, token
+    with torch.cuda.device(dev):
+        rc = _lib.lib().lp_verify_draft(target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(),
+                                        0 if draft is None else draft.stride(0), 0 if draft is None else draft.stride(1), tokens.data_ptr(), parents.data_ptr(),
+                                        uniform.data_ptr(), None if nodes is None else nodes.data_ptr(), B, T, V, path.data_ptr(), count.data_ptr(),
+                                        token.data_ptr(), _lib.stream_ptr())
+        _lib.check(rc, "lp_verify_draft")
+    return path, count, token
+
+
+def _pools(pools):
+    """one tensor [n, pages, page_size, width] or a list of [pages, page_size, width] alike -> (a tensor of the list, pointers, their number, device)"""
+    if isinstance(pools, torch.Tensor):
+        _chk_cuda(pools, "pools", (pools.dtype,), 4)
+        n, step, at = pools.shape[0], pools.stride(0) * pools.element_size(), pools.data_ptr()
+        if n > 1 and step == 0:
+            raise ValueError("pools must not share their memory")
+        return (pools[0] if n else None), (C.c_void_p * max(n, 1))(*[at + i * step for i in range(n)]), n
+    pools = list(pools)
+    for i, t in enumerate(pools):
+        _chk_cuda(t, f"pools[{i}]", (pools[0].dtype if isinstance(pools[0], torch.Tensor) else torch.bfloat16,), 3)
+        if t.shape != pools[0].shape or t.stride() != pools[0].stride() or t.device != pools[0].device:
+            raise ValueError(f"pools[{i}] is {tuple(t.shape)} on {t.device}, pools[0] {tuple(pools[0].shape)} on {pools[0].device}: shapes and strides have to be alike")
+    return (pools[0] if pools else None), (C.c_void_p * max(len(pools), 1))(*[t.data_ptr() for t in pools]), len(pools)
+
+
+def cache_compact(pools, lengths, path, count, page_table=None):
+    """The accepted nodes' rows become the last rows of their sequences, in every pool, in place (lp_cache_compact): row lengths[b] + path[b, j] moves to row
+    lengths[b] + j, j < count[b] (path and count as verify_draft gives them; path rises).  pools: one tensor [n, pages, page_size, width] or a list of [pages, page_size,
+    width] of equal shapes, any type (the decoder's cache [layers, 2, rows, width]: kv.flatten(0, 1).unsqueeze(1)); page_table int32 [B, max_pages], or None: sequence b
+    is page b.  lengths, count int32 [B], path int32 [B, T].  Rows that are not there move nothing.  Returns pools."""
+    t, ptrs, n = _pools(pools)
+    _chk_cuda(path, "path", (torch.int32,), 2)
+    B, T = path.shape
+    if n == 0 or B == 0 or T == 0:
+        return pools
+    dev = t.device
+    P, S, W = t.shape
+    _chk_int32(lengths, "lengths", (B,), dev)
+    _chk_int32(count, "count", (B,), dev)
+    if path.device != dev or (T > 1 and path.stride(1) != 1):
+        raise ValueError(f"path must have contiguous rows on {dev}")
+    if page_table is not None:
+        _chk_cuda(page_table, "page_table", (torch.int32,), 2)
+        if page_table.shape[0] != B or page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"page_table must be int32 [{B}, max_pages] with contiguous rows on {dev}, got {tuple(page_table.shape)} on {page_table.device}")
+    if W > 1 and t.stride(2) != 1:
+        raise ValueError("rows must be contiguous")
+    e = t.element_size()
+    max_pages = 1 if page_table is None else page_table.shape[1]
+    L = _lib.stream32_lib()
+    with torch.cuda.device(dev):
+        rc = L.lp_cache_compact(ptrs, n, t.stride(0) * e, (t.stride(1) if S > 1 else W) * e, W * e, P, S, None if page_table is None else page_table.data_ptr(),
+                                0 if page_table is None else max(page_table.stride(0), max_pages), max_pages, lengths.data_ptr(), path.data_ptr(),
+                                max(path.stride(0), T), count.data_ptr(), B, T, _lib.stream_ptr())
+        _lib.check_on(L, rc, "lp_cache_compact")
+    return pools
+
+
+def cache_copy_pages(pools, src, dst):
+    """Page src[i] of every pool is copied to page dst[i] (lp_cache_copy_pages): src, dst int32 [n] on the device; no page may be in both, nor twice in dst; entries
+    that are not pages copy nothing.  pools as in cache_compact, contiguous within a page.  Returns pools."""
+    t, ptrs, n = _pools(pools)
+    _chk_cuda(src, "src", (torch.int32,), 1)
+    if n == 0 or src.numel() == 0:
+        return pools
+    _chk_int32(src, "src", src.shape, t.device)
+    _chk_int32(dst, "dst", src.shape, t.device)
+    P, S, W = t.shape
+    if (W > 1 and t.stride(2) != 1) or (S > 1 and t.stride(1) != W):
+        raise ValueError("pages must be contiguous")
+    e = t.element_size()
+    L = _lib.stream32_lib()
+    with torch.cuda.device(t.device):
+        rc = L.lp_cache_copy_pages(ptrs, n, (t.stride(0) if P > 1 else S * W) * e, S * W * e, P, src.data_ptr(), dst.data_ptr(), src.numel(), _lib.stream_ptr())
+        _lib.check_on(L, rc, "lp_cache_copy_pages")
+    return pools
+
+
+def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target=None, hard=0.0):
+    """Loss against a teacher's top logits, and its gradient, beside ce_fwd_bwd (lp_distill_fwd_bwd): logits [R, Vp] (fp32 or bf16; columns >= vocab are padding), ids
+    int64 or int32 [R, K] and teacher fp32 or bf16 [R, K] the teacher's best tokens and their logits (ids outside [0, vocab): missing entries; K <= 1024), weight fp32
+    [R] (rows of weight 0 are skipped), target int64 [R] labels for the share `hard` of the loss.
+    loss = (1 - hard) temperature^2 KL(softmax(teacher / temperature) || softmax(logits / temperature)) + hard CE(target)
+    -> (loss [R] fp32, dlogits bf16 [R, Vp], weighted as in ce_fwd_bwd)."""
+    _chk_cuda(logits, "logits", (torch.float32, torch.bfloat16), 2)
+    _chk_cuda(ids, "ids", (torch.int64, torch.int32), 2)
+    _chk_cuda(teacher, "teacher", (torch.float32, torch.bfloat16), 2)
+    _chk_cuda(weight, "weight", (torch.float32,), 1)
+    R, Vp = logits.shape
+    K = ids.shape[1]
+    dev = logits.device
+    if not 0 < vocab <= Vp:
+        raise ValueError(f"vocab {vocab} must lie in [1, {Vp}], the logits' columns")
+    if ids.shape != teacher.shape or ids.shape[0] != R or weight.shape[0] != R:
+        raise ValueError(f"logits {tuple(logits.shape)}, ids {tuple(ids.shape)}, teacher {tuple(teacher.shape)} and weight {tuple(weight.shape)} do not fit together")
+    if target is not None:
+        _chk_cuda(target, "target", (torch.int64,), 1)
+        if target.shape[0] != R or not target.is_contiguous():
+            raise ValueError(f"target must be a contiguous int64 [{R}]")
+    for t, n in ((logits, "logits"), (ids, "ids"), (teacher, "teacher"), (weight, "weight"), (target, "target")):
+        if t is not None and (t.device != dev or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{n} must have contiguous rows on {dev}")
+    loss = torch.empty((R,), device=dev, dtype=torch.float32)
+    d = torch.empty((R, -(-Vp // 2) * 2), device=dev, dtype=torch.bfloat16)[:, :Vp]
+    if R == 0:
+        return loss, d
+    with torch.cuda.device(dev):
+        rc = _lib.lib().lp_distill_fwd_bwd(logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, max(logits.stride(0), Vp), ids.data_ptr(),
+                                           1 if ids.dtype == torch.int64 else 0, max(ids.stride(0), K), teacher.data_ptr(),
+                                           1 if teacher.dtype == torch.float32 else 0, max(teacher.stride(0), K), K, weight.data_ptr(),
+                                           None if target is None else target.data_ptr(), float(temperature), float(hard), loss.data_ptr(), d.data_ptr(),
+                                           d.stride(0), R, vocab, d.stride(0), _lib.stream_ptr())
+        _lib.check(rc, "lp_distill_fwd_bwd")
+    return loss, d
