@@ -318,8 +318,8 @@ _SIGS = {
     "lp_tree_attention_workspace_bytes": (_sz, [_P(TreeAttnDesc)]),
     "lp_tree_attention": (_i, [_P(TreeAttnDesc), _vp, _sz, _vp]),
     "lp_verify_draft": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
-    "lp_cache_compact": (_i, [_vp, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _vp, _ll, _vp, _i, _i, _vp]),
-    "lp_cache_copy_pages": (_i, [_vp, _i, _ll, _ll, _i, _vp, _vp, _i, _vp]),
+    "lp_cache_compact": (_i, [_vp, _ll, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _vp, _ll, _vp, _i, _i, _vp]),
+    "lp_cache_copy_pages": (_i, [_vp, _ll, _i, _ll, _ll, _i, _vp, _vp, _i, _vp]),
     "lp_distill_fwd_bwd": (_i, [_vp, _i, _ll, _vp, _i, _ll, _vp, _i, _ll, _i, _vp, _vp, _f, _f, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "lp_profile_enable": (_i, [_i]),
     "lp_profile_read": (_i, [_vp, _i]),

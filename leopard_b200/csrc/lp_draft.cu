@@ -232,9 +232,9 @@ cache_pages_kernel(const __grid_constant__ Pools pools, long long page_stride, l
 }
 
 // the widest piece that a list of addresses and sizes is a multiple of
-static int piece_bytes(const void* const* pools, int n, long long a, long long b, long long c) {
-  unsigned long long all = (unsigned long long)a | (unsigned long long)b | (unsigned long long)c;
-  for (int i = 0; i < n; ++i) all |= reinterpret_cast<unsigned long long>(pools[i]);
+static int piece_bytes(const void* const* pools, long long step, int n, long long a, long long b, long long c) {
+  unsigned long long all = (unsigned long long)a | (unsigned long long)b | (unsigned long long)c | (unsigned long long)step;
+  for (int i = 0; i < (step ? 1 : n); ++i) all |= reinterpret_cast<unsigned long long>(pools[i]);
   return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
 }
 
@@ -263,7 +263,7 @@ extern "C" int lp_verify_draft(const float* target, long long target_batch, long
   return 0;
 }
 
-extern "C" int lp_cache_compact(const void* const* pools, int n_pools, long long page_stride, long long row_stride, long long row_bytes, int n_pages,
+extern "C" int lp_cache_compact(const void* const* pools, long long pool_step, int n_pools, long long page_stride, long long row_stride, long long row_bytes, int n_pages,
                                 int page_size, const int* table, long long ld_table, int max_pages, const int* lengths, const int* path,
                                 long long ld_path, const int* count, int B, int T, void* stream_) {
   using namespace lp;
@@ -272,13 +272,14 @@ extern "C" int lp_cache_compact(const void* const* pools, int n_pools, long long
   LP_REQUIRE(n_pages > 0 && page_size > 0 && row_bytes > 0 && row_stride >= row_bytes && ld_path >= T && max_pages > 0 && (table == nullptr || ld_table >= max_pages),
              "lp_cache_compact: bad layout n_pages=%d page_size=%d row %lld of %lld bytes, %d pages a sequence", n_pages, page_size, row_bytes, row_stride, max_pages);
   LP_REQUIRE(table != nullptr || (max_pages == 1 && B <= n_pages), "lp_cache_compact: %d sequences without a page table need a page each, there are %d", B, n_pages);
-  const int u = piece_bytes(pools, n_pools, page_stride, row_stride, row_bytes);
+  const int u = piece_bytes(pools, pool_step, n_pools, page_stride, row_stride, row_bytes);
   const long long units = row_bytes / u;
   LP_REQUIRE(units < (1 << 30), "lp_cache_compact: rows of %lld bytes are too wide", row_bytes);
   for (int at = 0; at < n_pools; at += POOLS_MAX) {
     const int m = n_pools - at < POOLS_MAX ? n_pools - at : POOLS_MAX;
     Pools list;
-    for (int i = 0; i < m; ++i) list.base[i] = reinterpret_cast<unsigned long long>(pools[at + i]);
+    for (int i = 0; i < m; ++i)
+      list.base[i] = pool_step ? reinterpret_cast<unsigned long long>(pools[0]) + (unsigned long long)pool_step * (at + i) : reinterpret_cast<unsigned long long>(pools[at + i]);
     const dim3 grid((unsigned)((units + 127) / 128), m, B);
     note_launch();
 #define LP_COMPACT(U) cache_compact_kernel<U><<<grid, 128, 0, stream>>>(list, page_stride, row_stride, (int)units, n_pages, page_size, table, ld_table, max_pages, lengths, path, ld_path, count, T)
@@ -292,20 +293,21 @@ extern "C" int lp_cache_compact(const void* const* pools, int n_pools, long long
   return 0;
 }
 
-extern "C" int lp_cache_copy_pages(const void* const* pools, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
+extern "C" int lp_cache_copy_pages(const void* const* pools, long long pool_step, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
                                    const int* dst, int n, void* stream_) {
   using namespace lp;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LP_REQUIRE(pools && src && dst && n_pools > 0 && n_pages > 0 && n >= 0 && n <= 65535, "lp_cache_copy_pages: bad arguments n_pools=%d n_pages=%d n=%d", n_pools, n_pages, n);
   LP_REQUIRE(page_bytes > 0 && page_stride >= page_bytes, "lp_cache_copy_pages: pages of %lld bytes, %lld apart", page_bytes, page_stride);
   if (n == 0) return 0;
-  const int u = piece_bytes(pools, n_pools, page_stride, page_bytes, 0);
+  const int u = piece_bytes(pools, pool_step, n_pools, page_stride, page_bytes, 0);
   const long long units = page_bytes / u, ctas = (units + PAGE_PIECES - 1) / PAGE_PIECES;
   LP_REQUIRE(ctas < (1LL << 31), "lp_cache_copy_pages: pages of %lld bytes are too large", page_bytes);
   for (int at = 0; at < n_pools; at += POOLS_MAX) {
     const int m = n_pools - at < POOLS_MAX ? n_pools - at : POOLS_MAX;
     Pools list;
-    for (int i = 0; i < m; ++i) list.base[i] = reinterpret_cast<unsigned long long>(pools[at + i]);
+    for (int i = 0; i < m; ++i)
+      list.base[i] = pool_step ? reinterpret_cast<unsigned long long>(pools[0]) + (unsigned long long)pool_step * (at + i) : reinterpret_cast<unsigned long long>(pools[at + i]);
     const dim3 grid((unsigned)ctas, m, n);
     note_launch();
 #define LP_PAGES(U) cache_pages_kernel<U><<<grid, 256, 0, stream>>>(list, page_stride, units, n_pages, src, dst)

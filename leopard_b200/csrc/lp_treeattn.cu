@@ -371,7 +371,7 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
   if (c0 == c1) return;                                  // written whole
   float top = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[(2LL * c + (c == c0 && tree_cut(total, c, a.ctas) <= at ? 1 : 0)) * a.rows + r].x);
+  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[(2LL * c + (c == c0 ? 1 : 0)) * a.rows + r].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -438,13 +438,20 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   LP_REQUIRE(d->q && d->k && d->v && d->out && d->lengths && d->mask && workspace, "lp_tree_attention: null argument");
   LP_REQUIRE(d->page_table ? d->ld_table >= d->max_pages : (d->max_pages == 1 && d->B <= d->n_pages),
              "lp_tree_attention: %d sequences of %d pages: ld_table %lld, %d pages there", d->B, d->max_pages, d->ld_table, d->n_pages);
+  TreeArgs a;
+  a.d = *d;
+  d = &a.d;                               // of a dimension of one any stride may have come
+  if (d->B == 1) a.d.q_batch = a.d.o_batch = a.d.mask_batch = a.d.ld_table = 0;
+  if (d->T == 1) a.d.q_node = a.d.o_node = a.d.mask_node = 0;
+  if (d->H == 1) a.d.q_head = a.d.o_head = 0;
+  if (d->n_pages == 1) a.d.k_page = a.d.v_page = 0;
+  if (d->page_size == 1) a.d.k_row = a.d.v_row = 0;
+  if (d->KVH == 1) a.d.k_head = a.d.v_head = 0;
   const long long strides = d->q_batch | d->q_node | d->q_head | d->k_page | d->k_row | d->k_head | d->v_page | d->v_row | d->v_head | d->o_batch | d->o_node | d->o_head;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v) |
                           reinterpret_cast<uintptr_t>(d->out) | reinterpret_cast<uintptr_t>(workspace);
   LP_REQUIRE(strides % 8 == 0 && bases % 16 == 0, "lp_tree_attention: strides in multiples of 8 elements, 16-byte aligned bases");
   LP_REQUIRE(ws_bytes >= lp_tree_attention_workspace_bytes(d), "lp_tree_attention: workspace too small");
-  TreeArgs a;
-  a.d = *d;
   a.group = d->H / d->KVH;
   a.rows = tree_rows(d);
   a.scale_log2 = d->scale * 1.4426950408889634f;

@@ -525,43 +525,82 @@ def parity_softmax_(scores, Tk, scale, causal):
 
 
 # ---- drafting (csrc/lp_treeattn.cu, lp_draft.cu, lp_distill.cu): trees of drafted tokens over a cache, their verification, the accepted rows, and the loss
-# that trains a draft model.  Calls run on the current stream of the tensors' device. ---------------------------------------------------------------------------
-def _chk_cuda(t, name, dtypes, dim=None):
+# that trains a draft model.  Calls run on the current stream of the tensors' device.  A step makes these calls once a layer, so what is in order passes one
+# condition; only what does not pass is looked at piece by piece, to say what is wrong. ---------------------------------------------------------------------
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+
+
+def _need(t, name, dtypes, dim=None, shape=None, device=None, contiguous=False, rows=False):
+    """raises unless t is a CUDA tensor of one of these types, of this shape and device, contiguous (in its rows)"""
+    kinds = "/".join(str(d).replace("torch.", "") for d in dtypes)
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
-        what = "/".join(str(d).replace("torch.", "") for d in dtypes)
-        raise TypeError(f"{name} must be a CUDA {what} tensor, got " + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
-    if dim is not None and t.dim() != dim:
-        raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
-
-
-def _chk_int32(t, name, shape, device, contiguous=True):
-    _chk_cuda(t, name, (torch.int32,))
-    if tuple(t.shape) != tuple(shape) or t.device != device or (contiguous and not t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous int32 {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+        raise TypeError(f"{name} must be a CUDA {kinds} tensor, got " + (f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__))
+    if (dim is not None and t.dim() != dim) or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} must have {f'{dim} dimensions' if shape is None else f'the shape {tuple(shape)}'}, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call on {device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if rows and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
 
 
 def _overlaps(a, b):
     """whether two tensors' spans of memory meet"""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+
     def span(t):
         return t.data_ptr(), t.data_ptr() + (sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
 
 
+def _call(device, L, name, fn, *args):
+    """fn(*args, stream) on the current stream of `device`"""
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check_on(L, rc, name)
+
+
 def tree_mask(parents):
     """parents int32 [B, T] (node 0 the last certain token, parents[b, 0] = -1, a parent lies before its children) -> (mask int64 [B, T, ceil(T / 64)], the
     bits of each node and its ancestors; depth int32 [B, T], its position behind the cached rows) (lp_tree_mask).  T <= 256."""
-    _chk_cuda(parents, "parents", (torch.int32,), 2)
-    if parents.stride(1) != 1 and parents.shape[1] > 1:
-        raise ValueError("parents must have a contiguous last dimension")
+    _need(parents, "parents", (_I32,), 2, rows=True)
     B, T = parents.shape
-    mask = torch.empty((B, T, -(-T // 64)), dtype=torch.int64, device=parents.device)
-    depth = torch.empty((B, T), dtype=torch.int32, device=parents.device)
-    if B == 0 or T == 0:
-        return mask, depth
-    with torch.cuda.device(parents.device):
-        _lib.check(_lib.lib().lp_tree_mask(_lib.ptr(parents), max(parents.stride(0), T), B, T, _lib.ptr(mask), _lib.ptr(depth), _lib.stream_ptr()), "lp_tree_mask")
+    mask = torch.empty((B, T, -(-T // 64)), dtype=_I64, device=parents.device)
+    depth = torch.empty((B, T), dtype=_I32, device=parents.device)
+    if B and T:
+        L = _lib.lib()
+        _call(parents.device, L, "lp_tree_mask", L.lp_tree_mask, parents.data_ptr(), max(parents.stride(0), T), B, T, mask.data_ptr(), depth.data_ptr())
     return mask, depth
+
+
+def _tree_refusals(q, k, v, lengths, mask, nodes, page_table, out):
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        if t is not None:
+            _need(t, n, (_BF16,), 4, rows=True)
+    B, T, _, D = q.shape
+    dev = q.device
+    if k.shape[3] != D or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if out is not None and out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    for t, n in ((k, "k"), (v, "v")) + (((out, "out"),) if out is not None else ()):
+        _need(t, n, (_BF16,), device=dev)
+    _need(mask, "mask", (_I64,), 3, (B, T, -(-T // 64)), dev, rows=True)
+    _need(lengths, "lengths", (_I32,), 1, (B,), dev, contiguous=True)
+    if nodes is not None:
+        _need(nodes, "nodes", (_I32,), 1, (B,), dev, contiguous=True)
+    if page_table is not None:
+        _need(page_table, "page_table", (_I32,), 2, (B, page_table.shape[-1]), dev, rows=True)
+    elif k.shape[0] < B:
+        raise ValueError(f"{B} sequences need a page table or a cache of their own each, k holds {k.shape[0]}")
 
 
 def tree_attention(q, k, v, lengths, mask, nodes=None, page_table=None, scale=None, out=None):
@@ -570,52 +609,59 @@ def tree_attention(q, k, v, lengths, mask, nodes=None, page_table=None, scale=No
     of the past, seen by every node; mask int64 [B, T, ceil(T / 64)] (tree_mask), the nodes that a node sees: node n is row lengths[b] + n; nodes
     int32 [B] or None, nodes of each sequence.  Strides are free but for a contiguous last dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of nodes
     that a sequence does not have stay as they were (`out` given) or are unspecified.  A node that sees nothing is zeros."""
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        _chk_cuda(t, n, (torch.bfloat16,), 4)
-    B, T, H, D = q.shape
-    P, S, KVH, Dk = k.shape
-    dev = q.device
-    if Dk != D or v.shape != k.shape:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    try:
+        B, T, H, D = q.shape
+        P, S, KVH, Dk = k.shape
+        dev, words = q.device, (T + 63) >> 6
+        fine = (q.is_cuda and q.dtype is _BF16 and k.dtype is _BF16 and v.dtype is _BF16 and Dk == D and v.shape == k.shape and k.device == dev and v.device == dev
+                and mask.dtype is _I64 and mask.device == dev and mask.shape == (B, T, words) and lengths.dtype is _I32 and lengths.device == dev
+                and lengths.shape == (B,) and lengths.is_contiguous())
+        qs, ks, vs, ms = q.stride(), k.stride(), v.stride(), mask.stride()
+        fine = fine and qs[3] == ks[3] == vs[3] == 1 and (ms[2] == 1 or words == 1)
+        if nodes is not None:
+            fine = fine and nodes.dtype is _I32 and nodes.device == dev and nodes.shape == (B,) and nodes.is_contiguous()
+        if page_table is not None:
+            max_pages = page_table.shape[1]
+            fine = (fine and page_table.dtype is _I32 and page_table.device == dev and page_table.shape == (B, max_pages)
+                    and (page_table.stride(1) == 1 or max_pages <= 1))
+            table, ld = page_table.data_ptr(), max(page_table.stride(0), max_pages)
+        else:
+            fine, max_pages, table, ld = fine and P >= B, 1, None, 0
+        if out is not None:
+            fine = fine and out.dtype is _BF16 and out.device == dev and out.shape == q.shape and out.stride(3) == 1
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _tree_refusals(q, k, v, lengths, mask, nodes, page_table, out)
+        raise ValueError("tree_attention: heads must be contiguous")
     if out is None:
-        out = torch.empty((B, T, H, D), dtype=torch.bfloat16, device=dev)
-    _chk_cuda(out, "out", (torch.bfloat16,), 4)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    _chk_cuda(mask, "mask", (torch.int64,), 3)
-    if tuple(mask.shape) != (B, T, -(-T // 64)):
-        raise ValueError(f"mask must be [B, T, ceil(T / 64)] = {(B, T, -(-T // 64))}, got {tuple(mask.shape)}")
-    for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out"), (mask, "mask")):
-        if t.device != dev:
-            raise ValueError(f"{n} is on {t.device}, q on {dev}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{n} must have a contiguous last dimension")
-    _chk_int32(lengths, "lengths", (B,), dev)
-    if nodes is not None:
-        _chk_int32(nodes, "nodes", (B,), dev)
-    if page_table is not None:
-        _chk_cuda(page_table, "page_table", (torch.int32,), 2)
-        if page_table.shape[0] != B or page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError(f"page_table must be int32 [{B}, max_pages] with contiguous rows on {dev}, got {tuple(page_table.shape)} on {page_table.device}")
-    elif P < B:
-        raise ValueError(f"{B} sequences need a page table or a cache of their own each, k holds {P}")
+        out = torch.empty((B, T, H, D), dtype=_BF16, device=dev)
+    elif _overlaps(out, q) or _overlaps(out, k) or _overlaps(out, v):
+        raise ValueError("out must not share memory with q, k or v")
     if B == 0 or T == 0:
         return out
-    if any(_overlaps(out, t) for t in (q, k, v)):
-        raise ValueError("out must not share memory with q, k or v")
-    max_pages = 1 if page_table is None else page_table.shape[1]
-
-    def strides(t):      # of a dimension of one any number may stand there
-        return [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride())]
-    d = _lib.TreeAttnDesc(q.data_ptr(), *strides(q), k.data_ptr(), *strides(k), v.data_ptr(), *strides(v), out.data_ptr(), *strides(out),
-                          None if page_table is None else page_table.data_ptr(), 0 if page_table is None else max(page_table.stride(0), max_pages), max_pages, P, S,
-                          lengths.data_ptr(), None if nodes is None else nodes.data_ptr(), mask.data_ptr(), mask.stride(0), mask.stride(1), B, T, H, KVH, D,
+    os_ = out.stride()
+    d = _lib.TreeAttnDesc(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os_[0], os_[1], os_[2],
+                          table, ld, max_pages, P, S, lengths.data_ptr(), None if nodes is None else nodes.data_ptr(), mask.data_ptr(), ms[0], ms[1], B, T, H, KVH, D,
                           D ** -0.5 if scale is None else float(scale))
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        ws = torch.empty(max(L.lp_tree_attention_workspace_bytes(C.byref(d)), 16), dtype=torch.uint8, device=dev)
-        _lib.check(L.lp_tree_attention(C.byref(d), _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "lp_tree_attention")
+    L, ref = _lib.lib(), C.byref(d)
+    need = L.lp_tree_attention_workspace_bytes(ref)
+    if need == 0:
+        _lib.check(-1, "lp_tree_attention")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(dev, L, "lp_tree_attention", L.lp_tree_attention, ref, ws.data_ptr(), need)
     return out
+
+
+def _verify_refusals(target, tokens, parents, uniform, draft, nodes):
+    _need(target, "target", (_F32,), 3, rows=True)
+    B, T, _ = target.shape
+    for t, n, kind in ((tokens, "tokens", _I64), (parents, "parents", _I32), (uniform, "uniform", _F32)):
+        _need(t, n, (kind,), 2, (B, T), target.device, contiguous=True)
+    if draft is not None:
+        _need(draft, "draft", (_F32,), 3, target.shape, target.device, rows=True)
+    if nodes is not None:
+        _need(nodes, "nodes", (_I32,), 1, (B,), target.device, contiguous=True)
 
 
 def verify_draft(target, tokens, parents, uniform, draft=None, nodes=None):
@@ -623,50 +669,51 @@ def verify_draft(target, tokens, parents, uniform, draft=None, nodes=None):
     draft of the same shape, what the children of node i were drawn from (None: drafts that were not drawn, such as the best of a list); tokens
     int64, parents int32, uniform fp32 (numbers in [0, 1): [b, c] tries node c, [b, 0] takes the next token) [B, T]; nodes int32 [B] or None.
     -> (path int32 [B, T]: the accepted nodes from node 0 on, then -1; count int32 [B]; next token int64 [B])."""
-    _chk_cuda(target, "target", (torch.float32,), 3)
-    B, T, V = target.shape
-    dev = target.device
-    for t, n, kinds in ((tokens, "tokens", (torch.int64,)), (parents, "parents", (torch.int32,)), (uniform, "uniform", (torch.float32,))):
-        _chk_cuda(t, n, kinds)
-        if tuple(t.shape) != (B, T) or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{n} must be a contiguous [{B}, {T}] on {dev}, got {tuple(t.shape)} on {t.device}")
-    if draft is not None:
-        _chk_cuda(draft, "draft", (torch.float32,), 3)
-        if draft.shape != target.shape or draft.device != dev:
-            raise ValueError(f"draft must be {tuple(target.shape)} on {dev}, got {tuple(draft.shape)} on {draft.device}")
-    for t, n in ((target, "target"), (draft, "draft")):
-        if t is not None and V > 1 and t.stride(2) != 1:
-            raise ValueError(f"{n} must have a contiguous last dimension")
-    if nodes is not None:
-        _chk_int32(nodes, "nodes", (B,), dev)
-    path = torch.empty((B, T), dtype=torch.int32, device=dev)
-    count = torch.empty((B,), dtype=torch.int32, device=dev)
-    token = torch.empty((B,), dtype=torch.int64, device=dev)
-    if B == 0:
-        return path, count, token
-    with torch.cuda.device(dev):
-        rc = _lib.lib().lp_verify_draft(target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(),
-                                        0 if draft is None else draft.stride(0), 0 if draft is None else draft.stride(1), tokens.data_ptr(), parents.data_ptr(),
-                                        uniform.data_ptr(), None if nodes is None else nodes.data_ptr(), B, T, V, path.data_ptr(), count.data_ptr(),
-                                        token.data_ptr(), _lib.stream_ptr())
-        _lib.check(rc, "lp_verify_draft")
+    try:
+        B, T, V = target.shape
+        dev, shape, ts = target.device, (B, T), target.stride()
+        fine = (target.is_cuda and target.dtype is _F32 and ts[2] == 1 and tokens.dtype is _I64 and parents.dtype is _I32 and uniform.dtype is _F32
+                and tokens.shape == shape and parents.shape == shape and uniform.shape == shape and tokens.device == dev and parents.device == dev
+                and uniform.device == dev and tokens.is_contiguous() and parents.is_contiguous() and uniform.is_contiguous())
+        ds = (0, 0, 1) if draft is None else draft.stride()
+        fine = fine and (draft is None or (draft.dtype is _F32 and draft.shape == target.shape and draft.device == dev and ds[2] == 1))
+        fine = fine and (nodes is None or (nodes.dtype is _I32 and nodes.shape == (B,) and nodes.device == dev and nodes.is_contiguous()))
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _verify_refusals(target, tokens, parents, uniform, draft, nodes)
+        if target.shape[2] != 1:
+            raise ValueError("verify_draft: rows must be contiguous")
+        ts, ds = target.stride(), (0, 0, 1) if draft is None else draft.stride()
+    path = torch.empty((B, T), dtype=_I32, device=dev)
+    count = torch.empty((B,), dtype=_I32, device=dev)
+    token = torch.empty((B,), dtype=_I64, device=dev)
+    if B:
+        L = _lib.lib()
+        _call(dev, L, "lp_verify_draft", L.lp_verify_draft, target.data_ptr(), ts[0], ts[1], None if draft is None else draft.data_ptr(), ds[0], ds[1], tokens.data_ptr(),
+              parents.data_ptr(), uniform.data_ptr(), None if nodes is None else nodes.data_ptr(), B, T, V, path.data_ptr(), count.data_ptr(), token.data_ptr())
     return path, count, token
 
 
 def _pools(pools):
-    """one tensor [n, pages, page_size, width] or a list of [pages, page_size, width] alike -> (a tensor of the list, pointers, their number, device)"""
+    """one tensor [n, pages, page_size, width] or a list of [pages, page_size, width] alike -> (their pointers or the first one's, bytes between them, their number,
+    shape, strides, bytes of an element, device)"""
     if isinstance(pools, torch.Tensor):
-        _chk_cuda(pools, "pools", (pools.dtype,), 4)
-        n, step, at = pools.shape[0], pools.stride(0) * pools.element_size(), pools.data_ptr()
-        if n > 1 and step == 0:
+        if not pools.is_cuda or pools.dim() != 4:
+            _need(pools, "pools", (pools.dtype,), 4)
+        n, st, e = pools.shape[0], pools.stride(), pools.element_size()
+        if n > 1 and st[0] == 0:
             raise ValueError("pools must not share their memory")
-        return (pools[0] if n else None), (C.c_void_p * max(n, 1))(*[at + i * step for i in range(n)]), n
+        return (C.c_void_p * 1)(pools.data_ptr()), st[0] * e if n > 1 else 0, n, pools.shape[1:], st[1:], e, pools.device
     pools = list(pools)
+    if not pools:
+        return None, 0, 0, (0, 0, 0), (0, 0, 0), 0, None
+    first = pools[0]
+    _need(first, "pools[0]", (first.dtype if isinstance(first, torch.Tensor) else _BF16,), 3)
     for i, t in enumerate(pools):
-        _chk_cuda(t, f"pools[{i}]", (pools[0].dtype if isinstance(pools[0], torch.Tensor) else torch.bfloat16,), 3)
-        if t.shape != pools[0].shape or t.stride() != pools[0].stride() or t.device != pools[0].device:
-            raise ValueError(f"pools[{i}] is {tuple(t.shape)} on {t.device}, pools[0] {tuple(pools[0].shape)} on {pools[0].device}: shapes and strides have to be alike")
-    return (pools[0] if pools else None), (C.c_void_p * max(len(pools), 1))(*[t.data_ptr() for t in pools]), len(pools)
+        if not isinstance(t, torch.Tensor) or t.shape != first.shape or t.stride() != first.stride() or t.device != first.device or t.dtype != first.dtype:
+            raise ValueError(f"pools[{i}] is not like pools[0], {tuple(first.shape)} {first.dtype} on {first.device}: shapes, strides and types have to be the same")
+    return (C.c_void_p * len(pools))(*[t.data_ptr() for t in pools]), 0, len(pools), first.shape, first.stride(), first.element_size(), first.device
 
 
 def cache_compact(pools, lengths, path, count, page_table=None):
@@ -674,52 +721,66 @@ def cache_compact(pools, lengths, path, count, page_table=None):
     lengths[b] + j, j < count[b] (path and count as verify_draft gives them; path rises).  pools: one tensor [n, pages, page_size, width] or a list of [pages, page_size,
     width] of equal shapes, any type (the decoder's cache [layers, 2, rows, width]: kv.flatten(0, 1).unsqueeze(1)); page_table int32 [B, max_pages], or None: sequence b
     is page b.  lengths, count int32 [B], path int32 [B, T].  Rows that are not there move nothing.  Returns pools."""
-    t, ptrs, n = _pools(pools)
-    _chk_cuda(path, "path", (torch.int32,), 2)
-    B, T = path.shape
-    if n == 0 or B == 0 or T == 0:
+    ptrs, step, n, shape, st, e, dev = _pools(pools)
+    if not n or not path.numel():
         return pools
-    dev = t.device
-    P, S, W = t.shape
-    _chk_int32(lengths, "lengths", (B,), dev)
-    _chk_int32(count, "count", (B,), dev)
-    if path.device != dev or (T > 1 and path.stride(1) != 1):
-        raise ValueError(f"path must have contiguous rows on {dev}")
-    if page_table is not None:
-        _chk_cuda(page_table, "page_table", (torch.int32,), 2)
-        if page_table.shape[0] != B or page_table.device != dev or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError(f"page_table must be int32 [{B}, max_pages] with contiguous rows on {dev}, got {tuple(page_table.shape)} on {page_table.device}")
-    if W > 1 and t.stride(2) != 1:
+    P, S, W = shape
+    try:
+        B, T = path.shape
+        fine = (path.dtype is _I32 and path.device == dev and (path.stride(1) == 1 or T == 1) and lengths.dtype is _I32 and lengths.device == dev and lengths.shape == (B,)
+                and lengths.is_contiguous() and count.dtype is _I32 and count.device == dev and count.shape == (B,) and count.is_contiguous() and (st[2] == 1 or W == 1))
+        if page_table is not None:
+            max_pages = page_table.shape[1]
+            fine = (fine and page_table.dtype is _I32 and page_table.device == dev and page_table.shape == (B, max_pages)
+                    and (page_table.stride(1) == 1 or max_pages <= 1))
+            table, ld = page_table.data_ptr(), max(page_table.stride(0), max_pages)
+        else:
+            max_pages, table, ld = 1, None, 0
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _need(path, "path", (_I32,), 2, device=dev, rows=True)
+        _need(lengths, "lengths", (_I32,), 1, (path.shape[0],), dev, contiguous=True)
+        _need(count, "count", (_I32,), 1, (path.shape[0],), dev, contiguous=True)
+        if page_table is not None:
+            _need(page_table, "page_table", (_I32,), 2, (path.shape[0], page_table.shape[-1]), dev, rows=True)
         raise ValueError("rows must be contiguous")
-    e = t.element_size()
-    max_pages = 1 if page_table is None else page_table.shape[1]
     L = _lib.stream32_lib()
-    with torch.cuda.device(dev):
-        rc = L.lp_cache_compact(ptrs, n, t.stride(0) * e, (t.stride(1) if S > 1 else W) * e, W * e, P, S, None if page_table is None else page_table.data_ptr(),
-                                0 if page_table is None else max(page_table.stride(0), max_pages), max_pages, lengths.data_ptr(), path.data_ptr(),
-                                max(path.stride(0), T), count.data_ptr(), B, T, _lib.stream_ptr())
-        _lib.check_on(L, rc, "lp_cache_compact")
+    _call(dev, L, "lp_cache_compact", L.lp_cache_compact, ptrs, step, n, st[0] * e, (st[1] if S > 1 else W) * e, W * e, P, S, table, ld, max_pages, lengths.data_ptr(),
+          path.data_ptr(), max(path.stride(0), T), count.data_ptr(), B, T)
     return pools
 
 
 def cache_copy_pages(pools, src, dst):
     """Page src[i] of every pool is copied to page dst[i] (lp_cache_copy_pages): src, dst int32 [n] on the device; no page may be in both, nor twice in dst; entries
     that are not pages copy nothing.  pools as in cache_compact, contiguous within a page.  Returns pools."""
-    t, ptrs, n = _pools(pools)
-    _chk_cuda(src, "src", (torch.int32,), 1)
-    if n == 0 or src.numel() == 0:
+    ptrs, step, n, shape, st, e, dev = _pools(pools)
+    _need(src, "src", (_I32,), 1)
+    if not n or not src.numel():
         return pools
-    _chk_int32(src, "src", src.shape, t.device)
-    _chk_int32(dst, "dst", src.shape, t.device)
-    P, S, W = t.shape
-    if (W > 1 and t.stride(2) != 1) or (S > 1 and t.stride(1) != W):
+    _need(src, "src", (_I32,), device=dev, contiguous=True)
+    _need(dst, "dst", (_I32,), 1, src.shape, dev, contiguous=True)
+    P, S, W = shape
+    if (W > 1 and st[2] != 1) or (S > 1 and st[1] != W):
         raise ValueError("pages must be contiguous")
-    e = t.element_size()
     L = _lib.stream32_lib()
-    with torch.cuda.device(t.device):
-        rc = L.lp_cache_copy_pages(ptrs, n, (t.stride(0) if P > 1 else S * W) * e, S * W * e, P, src.data_ptr(), dst.data_ptr(), src.numel(), _lib.stream_ptr())
-        _lib.check_on(L, rc, "lp_cache_copy_pages")
+    _call(dev, L, "lp_cache_copy_pages", L.lp_cache_copy_pages, ptrs, step, n, (st[0] if P > 1 else S * W) * e, S * W * e, P, src.data_ptr(), dst.data_ptr(), src.numel())
     return pools
+
+
+def _distill_refusals(logits, ids, teacher, weight, vocab, target):
+    _need(logits, "logits", (_F32, _BF16), 2, rows=True)
+    R, Vp = logits.shape
+    dev = logits.device
+    _need(ids, "ids", (_I64, _I32), 2, device=dev, rows=True)
+    _need(teacher, "teacher", (_F32, _BF16), 2, ids.shape, dev, rows=True)
+    _need(weight, "weight", (_F32,), 1, (R,), dev, rows=True)
+    if ids.shape[0] != R:
+        raise ValueError(f"logits {tuple(logits.shape)} and ids {tuple(ids.shape)} do not fit together")
+    if target is not None:
+        _need(target, "target", (_I64,), 1, (R,), dev, rows=True)
+    if not 0 < vocab <= Vp:
+        raise ValueError(f"vocab {vocab} must lie in [1, {Vp}], the logits' columns")
 
 
 def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target=None, hard=0.0):
@@ -728,33 +789,25 @@ def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target
     [R] (rows of weight 0 are skipped), target int64 [R] labels for the share `hard` of the loss.
     loss = (1 - hard) temperature^2 KL(softmax(teacher / temperature) || softmax(logits / temperature)) + hard CE(target)
     -> (loss [R] fp32, dlogits bf16 [R, Vp], weighted as in ce_fwd_bwd)."""
-    _chk_cuda(logits, "logits", (torch.float32, torch.bfloat16), 2)
-    _chk_cuda(ids, "ids", (torch.int64, torch.int32), 2)
-    _chk_cuda(teacher, "teacher", (torch.float32, torch.bfloat16), 2)
-    _chk_cuda(weight, "weight", (torch.float32,), 1)
-    R, Vp = logits.shape
-    K = ids.shape[1]
-    dev = logits.device
-    if not 0 < vocab <= Vp:
-        raise ValueError(f"vocab {vocab} must lie in [1, {Vp}], the logits' columns")
-    if ids.shape != teacher.shape or ids.shape[0] != R or weight.shape[0] != R:
-        raise ValueError(f"logits {tuple(logits.shape)}, ids {tuple(ids.shape)}, teacher {tuple(teacher.shape)} and weight {tuple(weight.shape)} do not fit together")
-    if target is not None:
-        _chk_cuda(target, "target", (torch.int64,), 1)
-        if target.shape[0] != R or not target.is_contiguous():
-            raise ValueError(f"target must be a contiguous int64 [{R}]")
-    for t, n in ((logits, "logits"), (ids, "ids"), (teacher, "teacher"), (weight, "weight"), (target, "target")):
-        if t is not None and (t.device != dev or (t.shape[-1] > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"{n} must have contiguous rows on {dev}")
-    loss = torch.empty((R,), device=dev, dtype=torch.float32)
-    d = torch.empty((R, -(-Vp // 2) * 2), device=dev, dtype=torch.bfloat16)[:, :Vp]
-    if R == 0:
-        return loss, d
-    with torch.cuda.device(dev):
-        rc = _lib.lib().lp_distill_fwd_bwd(logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, max(logits.stride(0), Vp), ids.data_ptr(),
-                                           1 if ids.dtype == torch.int64 else 0, max(ids.stride(0), K), teacher.data_ptr(),
-                                           1 if teacher.dtype == torch.float32 else 0, max(teacher.stride(0), K), K, weight.data_ptr(),
-                                           None if target is None else target.data_ptr(), float(temperature), float(hard), loss.data_ptr(), d.data_ptr(),
-                                           d.stride(0), R, vocab, d.stride(0), _lib.stream_ptr())
-        _lib.check(rc, "lp_distill_fwd_bwd")
+    try:
+        R, Vp = logits.shape
+        K, dev = ids.shape[1], logits.device
+        fine = (logits.is_cuda and (logits.dtype is _F32 or logits.dtype is _BF16) and logits.stride(1) == 1 and (ids.dtype is _I64 or ids.dtype is _I32)
+                and (teacher.dtype is _F32 or teacher.dtype is _BF16) and ids.shape == (R, K) and teacher.shape == (R, K) and ids.device == dev and teacher.device == dev
+                and (K <= 1 or (ids.stride(1) == 1 and teacher.stride(1) == 1)) and weight.dtype is _F32 and weight.shape == (R,) and weight.device == dev
+                and weight.is_contiguous() and 0 < vocab <= Vp
+                and (target is None or (target.dtype is _I64 and target.shape == (R,) and target.device == dev and target.is_contiguous())))
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _distill_refusals(logits, ids, teacher, weight, vocab, target)
+        if logits.shape[1] != 1:
+            raise ValueError("distill_fwd_bwd: rows must be contiguous")
+    loss = torch.empty((R,), device=dev, dtype=_F32)
+    d = torch.empty((R, Vp), device=dev, dtype=_BF16) if Vp % 2 == 0 else torch.empty((R, Vp + 1), device=dev, dtype=_BF16)[:, :Vp]
+    if R:
+        L, ld = _lib.lib(), Vp + (Vp & 1)
+        _call(dev, L, "lp_distill_fwd_bwd", L.lp_distill_fwd_bwd, logits.data_ptr(), 1 if logits.dtype is _F32 else 0, max(logits.stride(0), Vp), ids.data_ptr(),
+              1 if ids.dtype is _I64 else 0, max(ids.stride(0), K), teacher.data_ptr(), 1 if teacher.dtype is _F32 else 0, max(teacher.stride(0), K), K, weight.data_ptr(),
+              None if target is None else target.data_ptr(), float(temperature), float(hard), loss.data_ptr(), d.data_ptr(), ld, R, vocab, ld)
     return loss, d

@@ -79,12 +79,12 @@ def test_other_refusals_are_status_codes(native_lib):
     assert L.lp_verify_draft(p, 0, 0, None, 0, 0, p, p, p, None, 1, 1025, 5, p, p, p, None) == -1
     assert L.lp_verify_draft(p, 0, 0, None, 0, 0, p, p, p, None, 1, 4, 0, p, p, p, None) == -1
     one = (C.c_void_p * 1)(1 << 20)
-    assert L.lp_cache_compact(one, 1, 4096, 64, 64, 8, 64, None, 0, 2, p, p, 4, p, 1, 4, None) == -1            # no table, two pages a sequence
-    assert L.lp_cache_compact(one, 1, 4096, 64, 64, 8, 64, None, 0, 1, p, p, 4, p, 9, 4, None) == -1            # nine sequences, eight pages
-    assert L.lp_cache_compact(one, 1, 4096, 32, 64, 8, 64, p, 2, 2, p, p, 4, p, 1, 4, None) == -1               # rows overlap
-    assert L.lp_cache_copy_pages(one, 1, 64, 4096, 8, p, p, 1, None) == -1                                      # pages overlap
-    assert L.lp_cache_copy_pages(one, 0, 4096, 4096, 8, p, p, 1, None) == -1
-    assert L.lp_cache_copy_pages(one, 1, 4096, 4096, 8, p, p, 0, None) == 0                                     # nothing to do
+    assert L.lp_cache_compact(one, 0, 1, 4096, 64, 64, 8, 64, None, 0, 2, p, p, 4, p, 1, 4, None) == -1            # no table, two pages a sequence
+    assert L.lp_cache_compact(one, 0, 1, 4096, 64, 64, 8, 64, None, 0, 1, p, p, 4, p, 9, 4, None) == -1            # nine sequences, eight pages
+    assert L.lp_cache_compact(one, 0, 1, 4096, 32, 64, 8, 64, p, 2, 2, p, p, 4, p, 1, 4, None) == -1               # rows overlap
+    assert L.lp_cache_copy_pages(one, 0, 1, 64, 4096, 8, p, p, 1, None) == -1                                      # pages overlap
+    assert L.lp_cache_copy_pages(one, 0, 0, 4096, 4096, 8, p, p, 1, None) == -1
+    assert L.lp_cache_copy_pages(one, 0, 1, 4096, 4096, 8, p, p, 0, None) == 0                                     # nothing to do
     args = dict(K=4, temp=1.0, hard=0.0, target=None, V=10, Vp=10, ldd=10)
 
     def distill(**kw):
