@@ -49,12 +49,235 @@ __device__ __forceinline__ float block_max_f32(float v, float* red) {
   return t;
 }
 
+// ---- pieces that the kernels share ---------------------------------------------------------------------------------
+// The teacher's entries of a row into shared memory: top[k] = t_k (0 where there is none), lt[k] = log t_k, id[k] (-1).  Returns whether there are any; the whole block.
+__device__ __forceinline__ bool teacher_side(const DistillArgs& a, int r, float* top, float* lt, int* id, float* red) {
+  const int tid = threadIdx.x;
+  float tm = -INFINITY;
+  for (int k = tid; k < a.K; k += 256) {
+    const long long at = (long long)r * a.ld_ids + k, at_t = (long long)r * a.ld_teacher + k;
+    const long long i = a.ids_64 ? reinterpret_cast<const long long*>(a.ids)[at] : reinterpret_cast<const int*>(a.ids)[at];
+    const bool in = i >= 0 && i < a.V;
+    id[k] = in ? (int)i : -1;
+    lt[k] = !in ? -INFINITY : a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at_t] : (float)reinterpret_cast<const bf16*>(a.teacher)[at_t];
+    if (in) tm = fmaxf(tm, lt[k]);
+  }
+  tm = block_max_f32(tm, red);
+  float ts = 0.f;
+  for (int k = tid; k < a.K; k += 256)
+    if (lt[k] != -INFINITY) ts += expf((lt[k] - tm) * a.inv_tau);
+  ts = block_sum_f32(ts, red);
+  const float log_ts = logf(ts);
+  for (int k = tid; k < a.K; k += 256) {
+    const bool in = lt[k] != -INFINITY;
+    lt[k] = in ? (lt[k] - tm) * a.inv_tau - log_ts : 0.f;
+    top[k] = in ? expf(lt[k]) : 0.f;
+  }
+  return !(ts == 0.f);                      // a NaN stays one
+}
+// 2^x in one instruction (2^-22 of the value)
+__device__ __forceinline__ float di_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// what a row's gradient is made of, once its maximum and sums are known
+struct RowGrad {
+  float m, c, ks, kh;                       // maximum; log2(e) / tau; w (1 - h) tau / sum, w h / sum1
+  float cs, ch;                             // the same without the sums: what the named entries lose of each t, and the label
+  __device__ __forceinline__ float at(float z) const {
+    const float d = z - m;
+    float g = 0.f;
+    if (ks != 0.f) g = di_ex2(d * c) * ks;
+    if (kh != 0.f) g += di_ex2(d * 1.4426950408889634f) * kh;
+    return g;
+  }
+};
+// The places of [v0, v1) that the teacher or the label names are written again with their whole value: by the first entry of each id, the sum of its entries taken off.
+// For after a barrier behind the row's other stores.
+template <typename T>
+__device__ __forceinline__ void named_places(const DistillArgs& a, const RowGrad& g, const T* row, bf16* drow, const float* top, const int* id, long long y, int v0, int v1) {
+  const bool label = y >= v0 && y < v1 && g.ch != 0.f;
+  for (int k = threadIdx.x; k < a.K; k += 256) {
+    if (id[k] < v0 || id[k] >= v1) continue;
+    float t = 0.f;
+    bool first = true;
+    for (int o = 0; o < a.K; ++o)
+      if (id[o] == id[k]) {
+        if (o < k) first = false;
+        t += top[o];
+      }
+    if (first) drow[id[k]] = __float2bfloat16_rn(g.at((float)row[id[k]]) - g.cs * t - (label && y == id[k] ? g.ch : 0.f));
+  }
+  if (label && threadIdx.x == 0) {
+    bool named = false;
+    for (int o = 0; o < a.K; ++o) named |= id[o] == y;
+    if (!named) drow[y] = __float2bfloat16_rn(g.at((float)row[y]) - g.ch);
+  }
+}
+// loss of a row (thread 0 writes it); the whole block
+template <typename T>
+__device__ __forceinline__ void row_loss(const DistillArgs& a, int r, bool soft, float m, float s, float s1, const T* row, const float* top, const float* lt, const int* id,
+                                         long long y, float* red) {
+  const float log_s = logf(s);
+  float kl = 0.f;
+  if (soft)
+    for (int k = threadIdx.x; k < a.K; k += 256)
+      if (id[k] >= 0 && top[k] != 0.f) kl += top[k] * (lt[k] - ((float)row[id[k]] - m) * a.inv_tau + log_s);
+  kl = block_sum_f32(kl, red);
+  if (threadIdx.x == 0) {
+    float l = soft ? (1.f - a.hard) * a.tau * a.tau * kl : 0.f;
+    if (y >= 0 && y < a.V && a.hard != 0.f) l += a.hard * (logf(s1) - ((float)row[y] - m));
+    a.loss[r] = l;
+  }
+}
+__device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, float w, bool soft, long long y, float m, float s, float s1) {
+  RowGrad g;
+  g.m = m;
+  g.c = a.inv_tau * 1.4426950408889634f;
+  g.cs = soft ? w * (1.f - a.hard) * a.tau : 0.f;
+  g.ch = y >= 0 && y < a.V ? w * a.hard : 0.f;
+  g.ks = g.cs / s;
+  g.kh = g.ch / s1;
+  return g;
+}
+
+// ---- rows that fit the registers of a cluster ------------------------------------------------------------------------
+// Bound by HBM: logits in, gradient out, once each.  A row is held by the registers of up to 8 CTAs (a cluster), 64 values a thread, between the sums and the gradient
+// that needs them; the CTAs tell one another their maximum and sums through their shared memory.  All loads of a row are in flight at once.
+// VEC values a load: 16 bytes where all rows start on 16 (and the gradient's on 8), else single values.  BOTH: a temperature and labels, two exponentials a value.
+constexpr int DISTILL_HELD = 64;
+template <typename T, int VEC, bool BOTH>
+__global__ void __launch_bounds__(256, 2)
+distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
+  constexpr int N = DISTILL_HELD / VEC;
+  extern __shared__ float top[];
+  __shared__ float red[8];
+  __shared__ float3 shared_sums;
+  float* lt = top + a.K;
+  int* id = reinterpret_cast<int*>(lt + a.K);
+  const int r = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x;
+  const T* row = reinterpret_cast<const T*>(a.logits) + (long long)r * a.ld;
+  bf16* drow = a.dlogits + (long long)r * a.ldd;
+  const int all = (a.V + VEC - 1) / VEC, each = (all + ctas - 1) / ctas;
+  const int i0 = min(all, rank * each), i1 = min(all, i0 + each);
+  const int v0 = min(a.V, i0 * VEC), v1 = min(a.V, i1 * VEC);
+  const float w = a.weight[r];
+  if (rank == ctas - 1)
+    for (int i = a.V + tid; i < a.Vp; i += 256) drow[i] = __float2bfloat16_rn(0.f);
+  if (w == 0.f) {
+    for (int i = i0 + tid; i < i1; i += 256) {
+      if (VEC > 1 && (i + 1) * VEC <= a.V) {
+        if (VEC == 8) *reinterpret_cast<uint4*>(drow + i * VEC) = make_uint4(0, 0, 0, 0);
+        else *reinterpret_cast<uint2*>(drow + i * VEC) = make_uint2(0, 0);
+      } else {
+        for (int e = i * VEC; e < min(a.V, (i + 1) * VEC); ++e) drow[e] = __float2bfloat16_rn(0.f);
+      }
+    }
+    if (tid == 0 && rank == 0) a.loss[r] = 0.f;
+    return;
+  }
+  float x[DISTILL_HELD];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = i0 + k * 256 + tid;
+    if (VEC > 1 && i < i1 && (i + 1) * VEC <= a.V) {
+      const uint4 u = ldg_once(row + (long long)i * VEC);
+      if (sizeof(T) == 4) {
+        x[k * VEC] = __uint_as_float(u.x); x[k * VEC + 1] = __uint_as_float(u.y); x[k * VEC + 2] = __uint_as_float(u.z); x[k * VEC + 3] = __uint_as_float(u.w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
+          x[k * VEC + (2 * e) % VEC] = __uint_as_float(h << 16);
+          x[k * VEC + (2 * e + 1) % VEC] = __uint_as_float(h & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[k * VEC + e] = i < i1 && i * VEC + e < a.V ? (float)row[(long long)i * VEC + e] : -INFINITY;
+    }
+  }
+  const bool soft = teacher_side(a, r, top, lt, id, red);
+  const long long y = a.target ? a.target[r] : -1;
+  float m = x[0];
+#pragma unroll
+  for (int k = 1; k < DISTILL_HELD; ++k) m = fmaxf(m, x[k]);
+  m = block_max_f32(m, red);
+  const float ref = m == -INFINITY ? 0.f : m, c = a.inv_tau * 1.4426950408889634f;
+  float s = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int k = 0; k < DISTILL_HELD; ++k) {
+    const float d = x[k] - ref, e = di_ex2(d * c);
+    s += e;
+    if (BOTH) s1 += di_ex2(d * 1.4426950408889634f);
+    else x[k] = e;                          // the gradient is this, scaled
+  }
+  s = block_sum_f32(s, red);
+  if (BOTH) s1 = block_sum_f32(s1, red);
+  float top_m = m;
+  if (ctas > 1) {
+    if (tid == 0) shared_sums = make_float3(m, s, s1);
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    float3 part[8];
+    const uint32_t here = smem_u32(&shared_sums);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      part[q] = make_float3(-INFINITY, 0.f, 0.f);
+      if (q < ctas) {
+        const uint32_t there = mapa_u32(here, q);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[q].x) : "r"(there) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[q].y) : "r"(there + 4) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[q].z) : "r"(there + 8) : "memory");
+      }
+      top_m = fmaxf(top_m, part[q].x);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA has read; it stays until the others have (below)
+    s = s1 = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < ctas) {
+        const float d = part[q].x == -INFINITY ? 0.f : part[q].x - top_m;      // sums of nothing are 0, or NaN
+        s += part[q].y * di_ex2(d * c);
+        if (BOTH) s1 += part[q].z * di_ex2(d * 1.4426950408889634f);
+      }
+  }
+  if (!BOTH) s1 = s;                        // no label, or no temperature: one sum does
+  const RowGrad g = row_grad(a, w, soft, y, top_m, s, s1);
+  const float down = !BOTH ? (g.ks + g.kh) * (ctas > 1 && m != -INFINITY ? di_ex2((m - top_m) * c) : 1.f) : 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = i0 + k * 256 + tid;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[k * VEC + e] = BOTH ? g.at(x[k * VEC + e]) : x[k * VEC + e] * down;
+    if (VEC > 1 && i < i1 && (i + 1) * VEC <= a.V) {
+      if (VEC == 8)
+        *reinterpret_cast<uint4*>(drow + (long long)i * VEC) =
+            make_uint4(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]),
+                       pack_bf16x2(x[k * VEC + 4 % VEC], x[k * VEC + 5 % VEC]), pack_bf16x2(x[k * VEC + 6 % VEC], x[k * VEC + 7 % VEC]));
+      else
+        *reinterpret_cast<uint2*>(drow + (long long)i * VEC) = make_uint2(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (i < i1 && i * VEC + e < a.V) drow[(long long)i * VEC + e] = __float2bfloat16_rn(x[k * VEC + e]);
+    }
+  }
+  __syncthreads();
+  named_places(a, g, row, drow, top, id, y, v0, v1);
+  if (rank == 0) row_loss(a, r, soft, top_m, s, s1, row, top, lt, id, y, red);
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- longer rows: a CTA reads its row twice, the second time from the L2 ----------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256)
-distill_kernel(const DistillArgs a) {
-  extern __shared__ float top[];            // t_k of the row's entries, then their ids
+distill_long_kernel(const __grid_constant__ DistillArgs a) {
+  extern __shared__ float top[];
   __shared__ float red[8];
-  int* id = reinterpret_cast<int*>(top + a.K);
+  float* lt = top + a.K;
+  int* id = reinterpret_cast<int*>(lt + a.K);
   const int r = blockIdx.x, tid = threadIdx.x;
   const T* row = reinterpret_cast<const T*>(a.logits) + (long long)r * a.ld;
   bf16* drow = a.dlogits + (long long)r * a.ldd;
@@ -64,84 +287,28 @@ distill_kernel(const DistillArgs a) {
     if (tid == 0) a.loss[r] = 0.f;
     return;
   }
-  // the teacher's side
-  float tm = -INFINITY;
-  for (int k = tid; k < a.K; k += 256) {
-    const long long at = (long long)r * a.ld_ids + k, at_t = (long long)r * a.ld_teacher + k;
-    const long long i = a.ids_64 ? reinterpret_cast<const long long*>(a.ids)[at] : reinterpret_cast<const int*>(a.ids)[at];
-    const bool in = i >= 0 && i < a.V;
-    id[k] = in ? (int)i : -1;
-    top[k] = !in ? -INFINITY : a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at_t] : (float)reinterpret_cast<const bf16*>(a.teacher)[at_t];
-    if (in) tm = fmaxf(tm, top[k]);
-  }
-  tm = block_max_f32(tm, red);
-  float ts = 0.f;
-  for (int k = tid; k < a.K; k += 256)
-    if (top[k] != -INFINITY) ts += expf((top[k] - tm) * a.inv_tau);
-  ts = block_sum_f32(ts, red);
-  const bool soft = !(ts == 0.f);           // a NaN stays one
-  // the student's
+  const bool soft = teacher_side(a, r, top, lt, id, red);
+  const long long y = a.target ? a.target[r] : -1;
   float m = -INFINITY;
   for (int i = tid; i < a.V; i += 256) m = fmaxf(m, (float)row[i]);
   m = block_max_f32(m, red);
+  const float c = a.inv_tau * 1.4426950408889634f;
   float s = 0.f, s1 = 0.f;
   for (int i = tid; i < a.V; i += 256) {
     const float d = (float)row[i] - m;
-    s += __expf(d * a.inv_tau);
-    s1 += __expf(d);
+    s += di_ex2(d * c);
+    s1 += di_ex2(d * 1.4426950408889634f);
   }
   s = block_sum_f32(s, red);
   s1 = block_sum_f32(s1, red);
-  const float log_s = logf(s), log_ts = logf(ts);
-  float kl = 0.f;
-  for (int k = tid; k < a.K; k += 256) {
-    float t = 0.f;
-    if (id[k] >= 0 && soft) {
-      const float lt = (top[k] - tm) * a.inv_tau - log_ts;
-      t = expf(lt);
-      if (t != 0.f) kl += t * (lt - ((float)row[id[k]] - m) * a.inv_tau + log_s);
-    }
-    top[k] = t;
-  }
-  kl = block_sum_f32(kl, red);              // ... and top[] is written
-  const long long y = a.target ? a.target[r] : -1;
-  const bool has_y = y >= 0 && y < a.V;
-  const float cs = soft ? w * (1.f - a.hard) * a.tau : 0.f, ch = has_y ? w * a.hard : 0.f;
-  if (tid == 0) {
-    float l = soft ? (1.f - a.hard) * a.tau * a.tau * kl : 0.f;
-    if (has_y && a.hard != 0.f) l += a.hard * (logf(s1) - ((float)row[y] - m));
-    a.loss[r] = l;
-  }
-  const float ks = cs / s, kh = ch / s1;
-  auto grad = [&](int i) {
-    const float d = (float)row[i] - m;
-    float g = 0.f;
-    if (cs != 0.f) g = __expf(d * a.inv_tau) * ks;
-    if (ch != 0.f) g += __expf(d) * kh;
-    return g;
-  };
+  const RowGrad g = row_grad(a, w, soft, y, m, s, s1);
   for (int i = tid * 2; i < a.Vp; i += 512) {
-    const float x = i < a.V ? grad(i) : 0.f, z = i + 1 < a.V ? grad(i + 1) : 0.f;
-    *reinterpret_cast<uint32_t*>(drow + i) = pack_bf16x2(x, z);
+    const float e = i < a.V ? g.at((float)row[i]) : 0.f, o = i + 1 < a.V ? g.at((float)row[i + 1]) : 0.f;
+    *reinterpret_cast<uint32_t*>(drow + i) = pack_bf16x2(e, o);
   }
   __syncthreads();
-  // the places that the teacher or the label names are written again with their whole value: by the first entry of each id, the sum of its entries taken off
-  for (int k = tid; k < a.K; k += 256) {
-    if (id[k] < 0) continue;
-    float t = 0.f;
-    bool first = true;
-    for (int o = 0; o < a.K; ++o)
-      if (id[o] == id[k]) {
-        if (o < k) first = false;
-        t += top[o];
-      }
-    if (first) drow[id[k]] = __float2bfloat16_rn(grad(id[k]) - cs * t - (has_y && y == id[k] ? ch : 0.f));
-  }
-  if (has_y && tid == 0 && ch != 0.f) {
-    bool named = false;
-    for (int o = 0; o < a.K; ++o) named |= id[o] == y;
-    if (!named) drow[y] = __float2bfloat16_rn(grad((int)y) - ch);
-  }
+  named_places(a, g, row, drow, top, id, y, 0, a.V);
+  row_loss(a, r, soft, m, s, s1, row, top, lt, id, y, red);
 }
 
 }  // namespace lp
@@ -160,9 +327,25 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
   LP_REQUIRE(hard >= 0.f && hard <= 1.f && (hard == 0.f || target), "lp_distill_fwd_bwd: a hard share of %g needs labels and lies in [0, 1]", (double)hard);
   DistillArgs a = {logits, ld, ids, ids_64, ld_ids, teacher, teacher_fp32, ld_teacher, K, weight, target, 1.f / temperature, temperature, hard, loss, reinterpret_cast<bf16*>(dlogits), ldd, V, Vp};
   note_launch();
-  const size_t smem = (size_t)K * 8;
-  if (logits_fp32) distill_kernel<float><<<rows, 256, smem, stream>>>(a);
-  else distill_kernel<bf16><<<rows, 256, smem, stream>>>(a);
+  const size_t smem = (size_t)K * 12;
+  const int ctas = (V + 256 * DISTILL_HELD - 1) / (256 * DISTILL_HELD);
+  const int size = logits_fp32 ? 4 : 2;
+  const bool wide = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld * size % 16 == 0 && reinterpret_cast<uintptr_t>(dlogits) % 16 == 0 && ldd * 2 % (logits_fp32 ? 8 : 16) == 0;
+  const bool both = hard != 0.f && temperature != 1.f;
+  if (ctas > 8) {                           // more than a cluster holds
+    if (logits_fp32) distill_long_kernel<float><<<rows, 256, smem, stream>>>(a);
+    else distill_long_kernel<bf16><<<rows, 256, smem, stream>>>(a);
+  } else {
+    LP_REQUIRE((long long)rows * ctas < (1LL << 31), "lp_distill_fwd_bwd: %d rows of %d columns are too many", rows, V);
+    cudaError_t rc;
+#define LP_HELD(T, VEC) \
+  rc = both ? launch_ex(distill_held_kernel<T, VEC, true>, dim3((unsigned)rows * ctas), dim3(256), smem, stream, ctas, false, a, ctas) \
+            : launch_ex(distill_held_kernel<T, VEC, false>, dim3((unsigned)rows * ctas), dim3(256), smem, stream, ctas, false, a, ctas)
+    if (logits_fp32) { if (wide) LP_HELD(float, 4); else LP_HELD(float, 1); }
+    else { if (wide) LP_HELD(bf16, 8); else LP_HELD(bf16, 1); }
+#undef LP_HELD
+    LP_CHECK_CUDA(rc);
+  }
   LP_CHECK_CUDA(cudaGetLastError());
   return 0;
 }
