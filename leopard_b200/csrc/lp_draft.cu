@@ -50,113 +50,196 @@ struct VerifyArgs {
   int* path; int* count; long long* next;
 };
 
-// One sequence a CTA.  The walk over the nodes in their order is the walk down the tree, since children come after their parents: node c is tried when its
-// parent is where the walk stands, and accepted when u[c] q(x) < P(x), P the target's distribution there less what was refused before.  A refusal
-// takes P = max(P - q, 0) / sum.  P is not stored: a value of it is taken again from p, q and the sums of the refusals.
-// Everything is computed in 64 bits, so that the choices are those of the definition.
-__global__ void __launch_bounds__(1024)
-verify_kernel(const VerifyArgs a) {
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// A cluster of up to 8 CTAs takes a sequence, a CTA an equal part of the vocabulary.  The walk over the nodes in their order is the walk down the tree, since children come after
+// their parents: node c is tried when its parent is where the walk stands, and accepted when u[c] q(x) < P(x), P the target's distribution there less what was
+// refused before.  A refusal takes P = max(P - q, 0) / sum.  P is not stored: a value of it is taken again from p, q and the sums of the refusals.  What the tests need of a node,
+// p and q at its token, is fetched for all nodes at once; the vocabulary is passed over once a refusal and once for the next token, and the CTAs add up their sums in the
+// order of their ranks.  All CTAs go the same way.  Everything is computed in 64 bits, so that the choices are those of the definition.
+// Bound by latency: a pass is 2 us (loads from the L2 or HBM, a barrier of the cluster).
+constexpr int VERIFY_THREADS = 512;
+constexpr int VERIFY_PART = 4096;                       // of the vocabulary, a CTA at least
+
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ double cluster_read_f64(const double* p, int rank) {      // the same place of another CTA's shared memory
+  uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+  double v;
+  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(VERIFY_THREADS)
+verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
+  constexpr int WARPS = VERIFY_THREADS / 32;
+  __shared__ double red[WARPS], sums[2];                // by warp; this CTA's, of the passes in turn
+  extern __shared__ double inv[];                       // [T] 1 / sum of each refusal at the node where the walk stands
+  float* px = reinterpret_cast<float*>(inv + a.T);      // [T] p and q of a node's token, after its parent
+  float* qx = px + a.T;
+  float* us = qx + a.T;
+  int* up = reinterpret_cast<int*>(us + a.T);           // [T] parents; -1 where the walk never comes
+  int* tok = up + a.T;                                  // [T] tokens (-1: none of the vocabulary)
+  int* gone = tok + a.T;                                // [T] the tokens that were refused at this node
+  const int b = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = min(a.nodes ? a.nodes[b] : a.T, a.T);
   int* path = a.path + (long long)b * a.T;
-  for (int i = tid; i < a.T; i += 1024) path[i] = -1;
   if (n <= 0) {
-    if (tid == 0) { a.count[b] = 0; a.next[b] = -1; }
+    if (rank == 0) {
+      for (int i = tid; i < a.T; i += VERIFY_THREADS) path[i] = -1;
+      if (tid == 0) { a.count[b] = 0; a.next[b] = -1; }
+    }
     return;
   }
-  __shared__ double red[32], inv[VERIFY_MAX_NODES];     // sums by warp; 1 / sum of each refusal at the node where the walk stands
-  __shared__ int tok[VERIFY_MAX_NODES];                 // ... and the token that was refused
-  __shared__ int s_pick;
-  const long long* tokens = a.tokens + (long long)b * a.T;
-  const int* parents = a.parents + (long long)b * a.T;
-  const float* u = a.uniform + (long long)b * a.T;
-  const float* p = a.target + b * a.target_batch;
-  const float* q = a.draft ? a.draft + b * a.draft_batch : nullptr;
-  int cur = 0, refused = 0, count = 1;
-  auto left = [&](long long v) {                        // P(v)
-    double x = (double)p[v];
+  const float* target = a.target + b * a.target_batch;
+  const float* draft = a.draft ? a.draft + b * a.draft_batch : nullptr;
+  for (int c = tid; c < n; c += VERIFY_THREADS) {
+    const int at = a.parents[(long long)b * a.T + c];
+    const long long x = a.tokens[(long long)b * a.T + c];
+    const bool in = x >= 0 && x < a.V, comes = c > 0 && at >= 0 && at < c;
+    up[c] = comes ? at : -1;
+    tok[c] = in ? (int)x : -1;
+    us[c] = a.uniform[(long long)b * a.T + c];
+    px[c] = comes && in ? target[at * a.target_row + x] : 0.f;
+    qx[c] = comes && in && draft ? draft[at * a.draft_row + x] : 1.f;
+  }
+  __syncthreads();
+  const int part = (a.V + ctas - 1) / ctas, v0 = min(a.V, rank * part), v1 = min(a.V, v0 + part);
+  const int each = ((v1 - v0 + WARPS - 1) / WARPS + 31) & ~31, w0 = min(v1, v0 + warp * each), w1 = min(v1, w0 + each);      // a warp's part, whole 32s
+  int cur = 0, refused = 0, count = 1, passes = 0;
+  const float* p = target;
+  const float* q = draft;
+  auto take = [&](double x, double d, int v) {          // P(v) of p(v), q(v)
     x = x > 0.0 ? x : 0.0;
-    const double d = q && refused ? (double)q[v] : 0.0;
     for (int k = 0; k < refused; ++k) {
-      x -= q ? d : (v == tok[k] ? 1.0 : 0.0);
+      x -= draft ? d : (v == gone[k] ? 1.0 : 0.0);
       x = x > 0.0 ? x * inv[k] : 0.0;
     }
     return x;
   };
-  const int part = ((a.V + 31) / 32 + 31) & ~31;        // a warp's range of the vocabulary
-  const int v0 = min(a.V, warp * part), v1 = min(a.V, v0 + part);
-  auto mass = [&]() {                                   // sum of P; red[] holds the warps' shares
+  const bool draws = draft != nullptr;
+  auto mass = [&](double* before) {                     // sum of P; red[] holds the warps' shares, `before` what the lower ranks have
     double s = 0.0;
-    for (int v = v0 + lane; v < v1; v += 32) s += left(v);
+    const bool less = draws && refused > 0;
+    constexpr int DEEP = 8;                             // loads under way
+    for (int v = w0 + lane; v < w1; v += 32 * DEEP) {
+      float x[DEEP], d[DEEP];
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) x[k] = v + 32 * k < w1 ? p[v + 32 * k] : 0.f;
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) d[k] = less && v + 32 * k < w1 ? q[v + 32 * k] : 0.f;
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) s += take((double)x[k], (double)d[k], v + 32 * k);
+    }
     s = warp_sum_f64(s);
-    __syncthreads();
     if (lane == 0) red[warp] = s;
     __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < 32; ++w) t += red[w];
-    return t;
+    double mine = 0.0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) mine += red[w];
+    double all = mine;
+    *before = 0.0;
+    if (ctas > 1) {
+      double* slot = &sums[passes & 1];                 // two in turn: who writes the first again has passed the barrier after its last reading
+      if (tid == 0) *slot = mine;
+      cluster_barrier();
+      all = 0.0;
+      for (int r = 0; r < ctas; ++r) {
+        if (r == rank) *before = all;
+        all += cluster_read_f64(slot, r);
+      }
+    }
+    ++passes;
+    return all;
   };
-  __syncthreads();
-  if (tid == 0) path[0] = 0;
+  double before;
+  if (rank == 0 && tid == 0) path[0] = 0;
   for (int c = 1; c < n; ++c) {
-    if (parents[c] != cur) continue;
-    const long long x = tokens[c];
-    const bool in = x >= 0 && x < a.V;
-    const double qx = !in ? 1.0 : q ? (double)q[x] : 1.0;
-    if (in && (double)u[c] * qx < left(x)) {
+    if (up[c] != cur || tok[c] < 0) continue;           // a token of no vocabulary takes nothing away
+    if ((double)us[c] * (double)qx[c] < take((double)px[c], (double)qx[c], tok[c])) {
       cur = c;
       refused = 0;
-      p = a.target + b * a.target_batch + c * a.target_row;
-      if (q) q = a.draft + b * a.draft_batch + c * a.draft_row;
-      if (tid == 0) path[count] = c;
+      p = target + c * a.target_row;
+      if (draws) q = draft + c * a.draft_row;
+      if (rank == 0 && tid == 0) path[count] = c;
       ++count;
       continue;
     }
-    if (!in) continue;                                  // no token of the vocabulary: nothing to take away
-    __syncthreads();
-    if (tid == 0) { tok[refused] = (int)x; inv[refused] = 1.0; }
+    __syncthreads();                                    // all have made the test
+    if (tid == 0) { gone[refused] = tok[c]; inv[refused] = 1.0; }
     __syncthreads();
     ++refused;
-    const double s = mass();
+    const double s = mass(&before);
     if (s > 0.0) {
-      if (tid == 0) inv[refused - 1] = 1.0 / s;
+      if (tid == 0) inv[refused - 1] = 1.0 / s;         // (mass ends behind a barrier after its last look at it)
     } else {
       --refused;                                        // nothing would be left: P stays
     }
     __syncthreads();
   }
-  // the next token: the first whose running sum is above u[0] of the whole
-  const double total = mass(), goal = (double)u[0] * total;
-  if (tid == 0) s_pick = 0x7fffffff;
-  double before = 0.0;
-  for (int w = 0; w < warp; ++w) before += red[w];
-  __syncthreads();
-  const bool mine = before + red[warp] > goal && !(before > goal);
-  int last = -1;                                        // of a warp's range: its last token that has any probability
-  if (mine) {
-    int found = -1;
-    double run = before;
-    for (int v = v0; v < v1 && found < 0; v += 32) {
-      const double x = v + lane < v1 ? left(v + lane) : 0.0;
-      double s = x;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && run + s > goal), any = __ballot_sync(0xffffffffu, x > 0.0);
-      if (hit) found = v + __ffs(hit) - 1;
-      if (any) last = v + 31 - __clz(any);
-      run += __shfl_sync(0xffffffffu, s, 31);
+  // the next token: the first whose running sum is above u[0] of the whole.  Its CTA, its warp there, its place in the warp's part.
+  const double total = mass(&before), goal = (double)us[0] * total;
+  if (rank == 0) {
+    for (int i = count + tid; i < a.T; i += VERIFY_THREADS) path[i] = -1;
+    if (tid == 0) {
+      a.count[b] = count;
+      if (!(total > goal)) a.next[b] = -1;
     }
-    if (found < 0) found = last;                        // the sums' last bits: the range's own total was above the goal
-    if (lane == 0 && found >= 0) atomicMin(&s_pick, found);
   }
-  __syncthreads();
-  if (tid == 0) {
-    a.count[b] = count;
-    a.next[b] = s_pick == 0x7fffffff ? -1 : s_pick;
+  double mine = 0.0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) mine += red[w];
+  if (before + mine > goal && !(before > goal)) {
+    int w_of = -1, w_any = -1;
+    double run = before, at = before;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (red[w] > 0.0 && w_of < 0) { w_any = w; at = run; }
+      if (run + red[w] > goal && w_of < 0) w_of = w;
+      run += red[w];
+    }
+    if (w_of < 0) w_of = w_any;                         // the sums' last bits: then the last warp that has any
+    if (warp == w_of) {
+      // 32 runs of the warp's part, then the 32s of the run
+      const int len = (w1 - w0 + 31) / 32;
+      auto value = [&](int v) { return take((double)p[v], draws && refused ? (double)q[v] : 0.0, v); };
+      auto pick = [&](double x, double base, double* start) {      // the lane where base + the running sum passes the goal, else the last that has any
+        double s = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, x > 0.0 && base + s > goal), any = __ballot_sync(0xffffffffu, x > 0.0);
+        const int l = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+        *start = base + __shfl_sync(0xffffffffu, s - x, l);
+        return l;
+      };
+      double x = 0.0, start;
+      for (int i = 0; i < len; ++i) {
+        const int v = w0 + lane * len + i;
+        if (v < w1) x += value(v);
+      }
+      int from = w0 + pick(x, at, &start) * len, found = -1;
+      const int end = min(w1, from + len);
+      for (; from < end; from += 32) {                  // one round for parts of up to 1,024
+        const int v = from + lane;
+        const double y = v < end ? value(v) : 0.0;
+        if (!__any_sync(0xffffffffu, y > 0.0)) continue;
+        double s = y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        double next;
+        found = from + pick(y, start, &next);
+        if (start + s > goal) break;
+        start += s;
+      }
+      if (lane == 0) a.next[b] = found;
+    }
   }
+  if (ctas > 1) cluster_barrier();                      // no CTA ends while another reads its sum
 }
 
 // ---- rows of a cache -----------------------------------------------------------------------------------------------
@@ -257,9 +340,10 @@ extern "C" int lp_verify_draft(const float* target, long long target_batch, long
   LP_REQUIRE(target && tokens && parents && uniform && path && count && next, "lp_verify_draft: null argument");
   LP_REQUIRE(B > 0 && T > 0 && T <= VERIFY_MAX_NODES && V > 0, "lp_verify_draft: bad sizes B=%d T=%d (at most %d nodes) V=%d", B, T, VERIFY_MAX_NODES, V);
   VerifyArgs a = {target, target_batch, target_row, draft, draft_batch, draft_row, tokens, parents, uniform, nodes, T, V, path, count, next};
+  const int parts = (V + VERIFY_PART - 1) / VERIFY_PART, ctas = parts < 8 ? parts : 8;
+  LP_REQUIRE(B <= (1 << 27), "lp_verify_draft: %d sequences are too many", B);
   note_launch();
-  verify_kernel<<<B, 1024, 0, reinterpret_cast<cudaStream_t>(stream_)>>>(a);
-  LP_CHECK_CUDA(cudaGetLastError());
+  LP_CHECK_CUDA(launch_ex(verify_kernel, dim3((unsigned)B * ctas), dim3(VERIFY_THREADS), (size_t)T * 32, reinterpret_cast<cudaStream_t>(stream_), ctas, false, a, ctas));
   return 0;
 }
 
