@@ -52,12 +52,15 @@ struct VerifyArgs {
 
 // A cluster of up to 8 CTAs takes a sequence, a CTA an equal part of the vocabulary.  The walk over the nodes in their order is the walk down the tree, since children come after
 // their parents: node c is tried when its parent is where the walk stands, and accepted when u[c] q(x) < P(x), P the target's distribution there less what was
-// refused before.  A refusal takes P = max(P - q, 0) / sum.  P is not stored: a value of it is taken again from p, q and the sums of the refusals.  What the tests need of a node,
-// p and q at its token, is fetched for all nodes at once; the vocabulary is passed over once a refusal and once for the next token, and the CTAs add up their sums in the
-// order of their ranks.  All CTAs go the same way.  Everything is computed in 64 bits, so that the choices are those of the definition.
-// Bound by latency: a pass is 2 us (loads from the L2 or HBM, a barrier of the cluster).
+// refused before.  A refusal takes P = max(P - q, 0) / sum.  What the tests need of a node, p and q at its token, is fetched for all nodes at once; the vocabulary is passed over
+// once a refusal and once for the next token, and the CTAs add up their sums in the order of their ranks.  All CTAs go the same way.  Everything is computed in 64
+// bits, so that the choices are those of the definition.
+// HELD: vocabularies of up to 8 x 16,384 words stay in registers, 32 values of P (but for a factor) and q a thread, from a node's first pass to its last; of longer ones a value of P is taken
+// again from p, q and the sums of the refusals.
+// Bound by latency, not by the rows that are read: barriers of the cluster and dependent loads.
 constexpr int VERIFY_THREADS = 512;
 constexpr int VERIFY_PART = 4096;                       // of the vocabulary, a CTA at least
+constexpr int VERIFY_HELD = 32;                         // values of a thread
 
 __device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
@@ -72,10 +75,12 @@ __device__ __forceinline__ double cluster_read_f64(const double* p, int rank) { 
   return v;
 }
 
-__global__ void __launch_bounds__(VERIFY_THREADS)
+template <bool HELD>
+__global__ void __launch_bounds__(VERIFY_THREADS, 1)
 verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
   constexpr int WARPS = VERIFY_THREADS / 32;
-  __shared__ double red[WARPS], sums[2];                // by warp; this CTA's, of the passes in turn
+  __shared__ double red[WARPS], sums[2], joined[2];     // by warp; this CTA's, of the passes in turn; all CTAs' and those of lower rank
+  __shared__ double rows[32][33];                       // the part of the vocabulary that the next token lies in
   extern __shared__ double inv[];                       // [T] 1 / sum of each refusal at the node where the walk stands
   float* px = reinterpret_cast<float*>(inv + a.T);      // [T] p and q of a node's token, after its parent
   float* qx = px + a.T;
@@ -120,18 +125,48 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     return x;
   };
   const bool draws = draft != nullptr;
-  auto mass = [&](double* before) {                     // sum of P; red[] holds the warps' shares, `before` what the lower ranks have
+  double xs[HELD ? VERIFY_HELD : 1], unit = 1.0;        // P of this thread's words w0 + lane + 32 i is xs[i] x unit
+  float ds[HELD ? VERIFY_HELD : 1];                     // q
+  bool have_p = false, have_q = false;
+  constexpr int DEEP = 8;                               // loads under way, of long vocabularies
+  // sum of P, or of max(P - q, 0) when a token x has just been refused; red[] holds the warps' shares, `before` what the lower ranks have
+  auto mass = [&](bool refusal, int x, double* before) {
     double s = 0.0;
-    const bool less = draws && refused > 0;
-    constexpr int DEEP = 8;                             // loads under way
-    for (int v = w0 + lane; v < w1; v += 32 * DEEP) {
-      float x[DEEP], d[DEEP];
+    if (HELD) {
+      if (!have_p) {
 #pragma unroll
-      for (int k = 0; k < DEEP; ++k) x[k] = v + 32 * k < w1 ? p[v + 32 * k] : 0.f;
+        for (int i = 0; i < VERIFY_HELD; ++i) ds[i] = w0 + lane + 32 * i < w1 ? p[w0 + lane + 32 * i] : 0.f;
 #pragma unroll
-      for (int k = 0; k < DEEP; ++k) d[k] = less && v + 32 * k < w1 ? q[v + 32 * k] : 0.f;
+        for (int i = 0; i < VERIFY_HELD; ++i) xs[i] = ds[i] > 0.f ? (double)ds[i] : 0.0;
+        have_p = true;
+        unit = 1.0;
+      }
+      if (refusal && draws && !have_q) {
 #pragma unroll
-      for (int k = 0; k < DEEP; ++k) s += take((double)x[k], (double)d[k], v + 32 * k);
+        for (int i = 0; i < VERIFY_HELD; ++i) ds[i] = w0 + lane + 32 * i < w1 ? q[w0 + lane + 32 * i] : 0.f;
+        have_q = true;
+      }
+      if (refusal) {
+#pragma unroll
+        for (int i = 0; i < VERIFY_HELD; ++i) {
+          const float d = draws ? ds[i] : w0 + lane + 32 * i == x ? 1.f : 0.f;
+          const double y = xs[i] * unit - (double)d;
+          xs[i] = y > 0.0 ? y : 0.0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VERIFY_HELD; ++i) s += xs[i];
+    } else {
+      const bool less = draws && refused > 0;
+      for (int v = w0 + lane; v < w1; v += 32 * DEEP) {
+        float f[DEEP], d[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) f[k] = v + 32 * k < w1 ? p[v + 32 * k] : 0.f;
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) d[k] = less && v + 32 * k < w1 ? q[v + 32 * k] : 0.f;
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) s += take((double)f[k], (double)d[k], v + 32 * k);
+      }
     }
     s = warp_sum_f64(s);
     if (lane == 0) red[warp] = s;
@@ -139,20 +174,24 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     double mine = 0.0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) mine += red[w];
-    double all = mine;
     *before = 0.0;
-    if (ctas > 1) {
-      double* slot = &sums[passes & 1];                 // two in turn: who writes the first again has passed the barrier after its last reading
-      if (tid == 0) *slot = mine;
-      cluster_barrier();
-      all = 0.0;
-      for (int r = 0; r < ctas; ++r) {
-        if (r == rank) *before = all;
-        all += cluster_read_f64(slot, r);
-      }
-    }
+    if (ctas == 1) return mine;
+    double* slot = &sums[passes & 1];                   // two in turn: who writes the first again has passed the barrier after its last reading
     ++passes;
-    return all;
+    if (tid == 0) *slot = mine;
+    cluster_barrier();
+    if (warp == 0) {
+      const double other = lane < ctas ? cluster_read_f64(slot, lane) : 0.0;
+      double run = 0.0, mark = 0.0;
+      for (int r = 0; r < ctas; ++r) {
+        if (r == rank) mark = run;
+        run += __shfl_sync(0xffffffffu, other, r);
+      }
+      if (lane == 0) { joined[0] = run; joined[1] = mark; }
+    }
+    __syncthreads();
+    *before = joined[1];
+    return joined[0];
   };
   double before;
   if (rank == 0 && tid == 0) path[0] = 0;
@@ -161,6 +200,7 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     if ((double)us[c] * (double)qx[c] < take((double)px[c], (double)qx[c], tok[c])) {
       cur = c;
       refused = 0;
+      have_p = have_q = false;
       p = target + c * a.target_row;
       if (draws) q = draft + c * a.draft_row;
       if (rank == 0 && tid == 0) path[count] = c;
@@ -171,16 +211,28 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     if (tid == 0) { gone[refused] = tok[c]; inv[refused] = 1.0; }
     __syncthreads();
     ++refused;
-    const double s = mass(&before);
+    const double s = mass(true, tok[c], &before);
     if (s > 0.0) {
-      if (tid == 0) inv[refused - 1] = 1.0 / s;         // (mass ends behind a barrier after its last look at it)
-    } else {
-      --refused;                                        // nothing would be left: P stays
+      const double f = 1.0 / s;
+      if (tid == 0) inv[refused - 1] = f;               // (mass ends behind a barrier after its last look at it)
+      unit = f;
+    } else {                                            // nothing would be left: P stays
+      --refused;
+      if (HELD) {                                       // (rare: taken again from what came before)
+        for (int i = 0; i < VERIFY_HELD; ++i) {
+          const int v = w0 + lane + 32 * i;
+          const double y = v < w1 ? take((double)p[v], draws && refused ? (double)q[v] : 0.0, v) : 0.0;
+#pragma unroll
+          for (int k = 0; k < VERIFY_HELD; ++k)
+            if (k == i) xs[k] = y;
+        }
+        unit = 1.0;
+      }
     }
     __syncthreads();
   }
   // the next token: the first whose running sum is above u[0] of the whole.  Its CTA, its warp there, its place in the warp's part.
-  const double total = mass(&before), goal = (double)us[0] * total;
+  const double total = mass(false, -1, &before), goal = (double)us[0] * total;
   if (rank == 0) {
     for (int i = count + tid; i < a.T; i += VERIFY_THREADS) path[i] = -1;
     if (tid == 0) {
@@ -202,9 +254,6 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
     }
     if (w_of < 0) w_of = w_any;                         // the sums' last bits: then the last warp that has any
     if (warp == w_of) {
-      // 32 runs of the warp's part, then the 32s of the run
-      const int len = (w1 - w0 + 31) / 32;
-      auto value = [&](int v) { return take((double)p[v], draws && refused ? (double)q[v] : 0.0, v); };
       auto pick = [&](double x, double base, double* start) {      // the lane where base + the running sum passes the goal, else the last that has any
         double s = x;
 #pragma unroll
@@ -217,24 +266,29 @@ verify_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
         *start = base + __shfl_sync(0xffffffffu, s - x, l);
         return l;
       };
-      double x = 0.0, start;
-      for (int i = 0; i < len; ++i) {
-        const int v = w0 + lane * len + i;
-        if (v < w1) x += value(v);
-      }
-      int from = w0 + pick(x, at, &start) * len, found = -1;
-      const int end = min(w1, from + len);
-      for (; from < end; from += 32) {                  // one round for parts of up to 1,024
-        const int v = from + lane;
-        const double y = v < end ? value(v) : 0.0;
-        if (!__any_sync(0xffffffffu, y > 0.0)) continue;
-        double s = y;
+      int found = -1;
+      double start = at;
+      if (HELD) {                                       // the 32s of the warp's part, then the words of one
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        double next;
-        found = from + pick(y, start, &next);
-        if (start + s > goal) break;
-        start += s;
+        for (int i = 0; i < VERIFY_HELD; ++i) rows[i][lane] = xs[i];
+        __syncwarp();
+        double x = 0.0;
+        for (int k = 0; k < 32; ++k) x += rows[lane][k];
+        const int i = pick(x, at, &start);
+        double end;
+        found = w0 + 32 * i + pick(rows[i][lane], start, &end);
+      } else {
+        for (int from = w0; from < w1; from += 32) {
+          const int v = from + lane;
+          const double y = v < w1 ? take((double)p[v], draws && refused ? (double)q[v] : 0.0, v) : 0.0;
+          if (!__any_sync(0xffffffffu, y > 0.0)) continue;
+          double s = y, end;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          found = from + pick(y, start, &end);
+          if (start + s > goal) break;
+          start += s;
+        }
       }
       if (lane == 0) a.next[b] = found;
     }
@@ -343,7 +397,7 @@ extern "C" int lp_verify_draft(const float* target, long long target_batch, long
   const int parts = (V + VERIFY_PART - 1) / VERIFY_PART, ctas = parts < 8 ? parts : 8;
   LP_REQUIRE(B <= (1 << 27), "lp_verify_draft: %d sequences are too many", B);
   note_launch();
-  LP_CHECK_CUDA(launch_ex(verify_kernel, dim3((unsigned)B * ctas), dim3(VERIFY_THREADS), (size_t)T * 32, reinterpret_cast<cudaStream_t>(stream_), ctas, false, a, ctas));
+  LP_CHECK_CUDA(launch_ex(V <= ctas * VERIFY_THREADS * VERIFY_HELD ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)B * ctas), dim3(VERIFY_THREADS), (size_t)T * 32, reinterpret_cast<cudaStream_t>(stream_), ctas, false, a, ctas));
   return 0;
 }
 

@@ -339,7 +339,8 @@ def same(got, want):
 
 
 @gpu
-@pytest.mark.parametrize("B, T, V", [(1, 1, 1), (1, 1, 32003), (2, 2, 5), (5, 6, 33), (3, 17, 1000), (2, 32, 32000), (40, 4, 100), (1, 64, 128256), (2, 200, 77)])
+@pytest.mark.parametrize("B, T, V", [(1, 1, 1), (1, 1, 32003), (2, 2, 5), (5, 6, 33), (3, 17, 1000), (2, 32, 32000), (40, 4, 100), (1, 64, 128256), (2, 200, 77), (2, 12, 131072), (2, 12, 131073), (3, 9, 4097),
+                                     (1, 5, 400007)])
 @pytest.mark.parametrize("drawn", [True, False])
 @pytest.mark.parametrize("chain", [True, False])
 def test_verify_draft(B, T, V, drawn, chain):
