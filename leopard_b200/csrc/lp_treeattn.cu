@@ -2,13 +2,9 @@
 //
 //   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, g]) v[j, g],   j < len (every cached row) or j = len + n with node n in node i's mask
 //
-// The T nodes and the G = H / KVH query heads of a key head are the rows of one product, row r = i G + g, so that a key is read once for all of them.  The
-// keys of an item (sequence, key head, block of R rows) are cut into tiles of 64; the tiles of all items stand in one line, of which every CTA takes an equal
-// piece: sequences of any lengths load all SMs alike, and where a CTA's piece ends inside an item its rows' running maximum, sum and weighted values
-// go to the workspace, to be joined by combine_kernel.  Which pieces an item lies in follows from the lengths alone, in both kernels.
-#include "lp_common.cuh"
-#include "lp_host.h"
-#include "../../include/leopard_b200.h"
+// The T nodes and the G = H / KVH query heads of a key head are the rows of one product, row r = i G + g, so that a key is read once for all of them.  This file has the
+// entry point, the kernel for few rows and any cache (mma.sync), and the one that joins the pieces; lp_treeattn_tc.cu has the kernel for many rows (tcgen05).
+#include "lp_treeattn.cuh"
 
 namespace lp {
 
@@ -17,19 +13,6 @@ constexpr int TA_STAGES = 3;
 constexpr int TA_RING = TA_STAGES + 1;    // tiles whose rows' places are known
 constexpr int TA_MAX_BATCH = 4096;
 
-struct TreeArgs {
-  lp_tree_attn_desc d;
-  int group, rows;                        // query heads of a key head; rows of a block
-  float scale_log2;
-  float* part_o; float2* part_ml;         // [2 x CTAs][rows][D], [2 x CTAs][rows]: maximum (log2 units) and sum
-  int ctas;
-};
-
-__device__ __forceinline__ float ta_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ta_ldmatrix(uint32_t* r, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)) : "memory");
 }
@@ -43,58 +26,6 @@ __device__ __forceinline__ void ta_copy16(void* dst, const void* src, bool there
 __device__ __forceinline__ void ta_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void ta_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// a sequence's part of the line of tiles
-struct TreeSeq {
-  int len, n, tiles, blocks;              // cached rows; nodes; tiles of an item; blocks of rows
-  long long keys;                         // rows that are there: cached and nodes', as far as the page table reaches
-};
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
-  TreeSeq s;
-  s.n = a.d.nodes ? min(max(a.d.nodes[b], 0), a.d.T) : a.d.T;
-  s.len = max(a.d.lengths[b], 0);
-  s.keys = min((long long)s.len + s.n, (long long)a.d.max_pages * a.d.page_size);
-  s.tiles = s.n ? (int)((s.keys + TA_KEYS - 1) / TA_KEYS) : 0;
-  s.blocks = (s.n * a.group + a.rows - 1) / a.rows;
-  return s;
-}
-// first[b] = tiles of all items of the sequences before b; by one warp, in shared memory
-__device__ __forceinline__ void tree_line(const TreeArgs& a, long long* first) {
-  if (threadIdx.x < 32) {
-    long long run = 0;
-    for (int b0 = 0; b0 < a.d.B; b0 += 32) {
-      const int b = b0 + threadIdx.x;
-      long long mine = 0;
-      if (b < a.d.B) {
-        const TreeSeq s = tree_seq(a, b);
-        mine = (long long)a.d.KVH * s.blocks * s.tiles;
-      }
-      long long sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-        if ((int)threadIdx.x >= o) sum += up;
-      }
-      if (b < a.d.B) first[b] = run + sum - mine;
-      run += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (threadIdx.x == 0) first[a.d.B] = run;
-  }
-  __syncthreads();
-}
-__device__ __forceinline__ long long tree_cut(long long total, int cta, int ctas) { return total / ctas * cta + min((long long)cta, total % ctas); }
-__device__ __forceinline__ int tree_cta_of(long long total, long long unit, int ctas) {
-  const long long each = total / ctas, more = total % ctas;      // the first `more` CTAs have one tile more
-  return unit < (each + 1) * more ? (int)(unit / (each + 1)) : (int)(more + (unit - (each + 1) * more) / each);
-}
-__device__ __forceinline__ int tree_find(const long long* first, int B, long long unit) {      // the sequence that `unit` belongs to
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first[mid] <= unit) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
 
 // WM x WN warps: 16 WM rows, the 64 keys of a tile dealt to WN warps
 template <int D, int WM, int WN>
@@ -394,17 +325,22 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-// rows of a block: what the widest tree needs, 64 at most
+// which kernel: tcgen05 for more rows than TREE_TC_ROWS where it takes the cache
+constexpr int TREE_TC_ROWS = 32;
+static bool tree_tc(const lp_tree_attn_desc* d) { return (long long)d->T * (d->H / d->KVH) > TREE_TC_ROWS && tree_tc_takes(d); }
+// rows of a block: what the widest tree needs, 64 (256) at most
 static int tree_rows(const lp_tree_attn_desc* d) {
   const long long rows = (long long)d->T * (d->H / d->KVH);
+  if (tree_tc(d)) return rows <= 128 ? 128 : 256;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
-// two CTAs on each SM, no more than there can be tiles
+static int tree_keys(const lp_tree_attn_desc* d) { return tree_tc(d) ? 128 : TA_KEYS; }
+// two CTAs on each SM (tcgen05: one), no more than there can be tiles
 static int tree_ctas(const lp_tree_attn_desc* d) {
-  const int R = tree_rows(d);
+  const int R = tree_rows(d), keys = tree_keys(d);
   const long long blocks = ((long long)d->T * (d->H / d->KVH) + R - 1) / R;
-  const long long tiles = ((long long)d->max_pages * d->page_size + TA_KEYS - 1) / TA_KEYS;
-  const long long most = 2LL * sm_count();
+  const long long tiles = ((long long)d->max_pages * d->page_size + keys - 1) / keys;
+  const long long most = (tree_tc(d) ? 1LL : 2LL) * sm_count();
   if (tiles > most || blocks > most) return (int)most;
   const long long all = tiles * blocks * d->KVH;
   return (int)(all > most / d->B ? most : all * d->B);
@@ -454,11 +390,13 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   LP_REQUIRE(ws_bytes >= lp_tree_attention_workspace_bytes(d), "lp_tree_attention: workspace too small");
   a.group = d->H / d->KVH;
   a.rows = tree_rows(d);
+  a.keys = tree_keys(d);
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.ctas = tree_ctas(d);
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * a.rows * d->D);
-  const int wm = a.rows / 16, wn = 4 / wm;
+  const bool tc = tree_tc(d);
+  const int wm = tc ? 1 : a.rows / 16, wn = 4 / wm;
   const size_t smem = tree_smem(d->D, wm, wn, d->B);
   note_launch(2);
 #define LP_TREE(DD, WM, WN)                                                                                                                    \
@@ -467,7 +405,8 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
     tree_attn_kernel<DD, WM, WN><<<a.ctas, 128, smem, stream>>>(a);                                                                            \
   }
 #define LP_TREE_D(DD)                                                                                                                          \
-  if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
+  if (tc) { if (const int rc = launch_tree_tc(a, stream)) return rc; }                                                                          \
+  else if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
   LP_CHECK_CUDA(cudaGetLastError());                                                                                                           \
   LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + TA_JOIN_WARPS - 1) / TA_JOIN_WARPS), d->KVH, d->B), \
                           dim3(32 * TA_JOIN_WARPS), (size_t)(d->B + 1) * 8, stream, 1, true, a));

@@ -1,0 +1,84 @@
+// leopard_b200 — attention of a tree of drafted tokens over a cache: what the kernels of lp_treeattn.cu and lp_treeattn_tc.cu share.
+//
+// The keys of an item (sequence, key head, block of rows) are cut into tiles; the tiles of all items stand in one line, of which every CTA takes an equal piece: sequences
+// of any lengths load all SMs alike.  Where a CTA's piece ends inside an item its rows' running maximum, sum and weighted values go to the workspace, to be joined.
+// Which pieces an item lies in follows from the lengths alone, in every kernel.
+#pragma once
+#include "lp_common.cuh"
+#include "lp_host.h"
+#include "../../include/leopard_b200.h"
+
+namespace lp {
+
+struct TreeArgs {
+  lp_tree_attn_desc d;
+  int group, rows, keys;                  // query heads of a key head; rows of a block; keys of a tile
+  float scale_log2;
+  float* part_o; float2* part_ml;         // [2 x CTAs][rows][D], [2 x CTAs][rows]: maximum (log2 units) and sum
+  int ctas;
+};
+// the tcgen05 kernel (lp_treeattn_tc.cu): whether it takes this cache, and its launch
+bool tree_tc_takes(const lp_tree_attn_desc* d);
+int launch_tree_tc(const TreeArgs& a, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ta_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// a sequence's part of the line of tiles
+struct TreeSeq {
+  int len, n, tiles, blocks;              // cached rows; nodes; tiles of an item; blocks of rows
+  long long keys;                         // rows that are there: cached and nodes', as far as the page table reaches
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+  TreeSeq s;
+  s.n = a.d.nodes ? min(max(a.d.nodes[b], 0), a.d.T) : a.d.T;
+  s.len = max(a.d.lengths[b], 0);
+  s.keys = min((long long)s.len + s.n, (long long)a.d.max_pages * a.d.page_size);
+  s.tiles = s.n ? (int)((s.keys + a.keys - 1) / a.keys) : 0;
+  s.blocks = (s.n * a.group + a.rows - 1) / a.rows;
+  return s;
+}
+// first[b] = tiles of all items of the sequences before b; by one warp, in shared memory
+__device__ __forceinline__ void tree_line(const TreeArgs& a, long long* first) {
+  if (threadIdx.x < 32) {
+    long long run = 0;
+    for (int b0 = 0; b0 < a.d.B; b0 += 32) {
+      const int b = b0 + threadIdx.x;
+      long long mine = 0;
+      if (b < a.d.B) {
+        const TreeSeq s = tree_seq(a, b);
+        mine = (long long)a.d.KVH * s.blocks * s.tiles;
+      }
+      long long sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((int)threadIdx.x >= o) sum += up;
+      }
+      if (b < a.d.B) first[b] = run + sum - mine;
+      run += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) first[a.d.B] = run;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ long long tree_cut(long long total, int cta, int ctas) { return total / ctas * cta + min((long long)cta, total % ctas); }
+__device__ __forceinline__ int tree_cta_of(long long total, long long unit, int ctas) {
+  const long long each = total / ctas, more = total % ctas;      // the first `more` CTAs have one tile more
+  return unit < (each + 1) * more ? (int)(unit / (each + 1)) : (int)(more + (unit - (each + 1) * more) / each);
+}
+__device__ __forceinline__ int tree_find(const long long* first, int B, long long unit) {      // the sequence that `unit` belongs to
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= unit) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+#endif
+
+}  // namespace lp

@@ -1,0 +1,518 @@
+// leopard_b200 — attention of a tree of drafted tokens over a cache, for many rows: tcgen05 products, keys and values by TMA from the cache's pages.
+//
+// One persistent CTA an SM takes its piece of the line of tiles (lp_treeattn.cuh), tile after tile of 128 keys.  Up to 256 rows (node x query head of a key head) are two
+// 128-row streams on the same keys, each with its own MMA issuer and softmax warps, as in the prefill's kernel (lp_attn3.cu): S of a tile comes in two halves of 64
+// keys with their own TMEM columns, so that the product for the next half runs while the softmax is at this one.
+//   warp 0       TMA producer: K_j, V_j into rings of two, a box a page or part of one; pages that are not there come as zeros
+//   warp 1 / 2   MMA issuer of stream 0 / 1:  S(j).h = Q K_j[h]^T,  O += P(j).h V_j[h] (P in TMEM)
+//   warp 3       TMEM
+//   warps 4-7, 8-11   softmax of stream 0 / 1: a thread a row; they also bring the row's queries (rows of a product are G heads of each node) and take O out
+// TMEM: S0 [0, 128) S1 [128, 256) O0 [256, 384) O1 [384, 512).
+// Only the last tiles of an item, which hold nodes or reach past them, look at masks; there V is searched before its product: rows behind the keys become zeros (a
+// cache's unwritten memory may hold anything), and values that are not finite are taken out and reach the rows that see them when O is taken out.
+#include "lp_treeattn.cuh"
+
+namespace lp {
+
+constexpr int TT_BOX = 128 * 128;      // 128 rows x 64 bf16
+constexpr int TT_THREADS = 384;
+constexpr int TT_KEYS = 128;
+
+#define LP_TT_TMEM_ST_16(regs, taddr)                                                                               \
+  asm volatile(                                                                                                     \
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, " \
+      "%15, %16};" ::"r"(taddr),                                                                                    \
+      "r"(regs[0]), "r"(regs[1]), "r"(regs[2]), "r"(regs[3]), "r"(regs[4]), "r"(regs[5]), "r"(regs[6]),             \
+      "r"(regs[7]), "r"(regs[8]), "r"(regs[9]), "r"(regs[10]), "r"(regs[11]), "r"(regs[12]), "r"(regs[13]),         \
+      "r"(regs[14]), "r"(regs[15])                                                                                  \
+      : "memory")
+
+__device__ __forceinline__ uint64_t tt_pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void tt_upk2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t tt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t tt_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void tt_bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+struct TreeTc {
+  TreeArgs a;
+  int box;                             // rows of a TMA box: of one page
+};
+
+// a CTA's piece of an item
+struct TreePiece {
+  int b, kvh, r0, t0, n;               // sequence, key head, first row, first tile, tiles
+  TreeSeq s;
+};
+__device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const long long* first, long long u, long long u_end) {
+  TreePiece p;
+  p.b = tree_find(first, a.d.B, u);
+  p.s = tree_seq(a, p.b);
+  const long long local = u - first[p.b];
+  const int item = (int)(local / p.s.tiles);
+  p.t0 = (int)(local % p.s.tiles);
+  p.n = (int)min((long long)(p.s.tiles - p.t0), u_end - u);
+  p.kvh = item / p.s.blocks;
+  p.r0 = (item % p.s.blocks) * a.rows;
+  return p;
+}
+// the page that holds row `key` of sequence b (-1: none)
+__device__ __forceinline__ int tree_page(const TreeArgs& a, int b, long long key) {
+  const long long logical = key / a.d.page_size;
+  if (logical >= a.d.max_pages) return -1;
+  const int page = a.d.page_table ? a.d.page_table[b * a.d.ld_table + logical] : b;
+  return page >= 0 && page < a.d.n_pages ? page : -1;
+}
+
+template <int DH>
+__global__ void __launch_bounds__(TT_THREADS, 1)
+tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeTc tc) {
+  constexpr int NB = (DH + 63) / 64, KS_QK = DH / 16, HEAD_BYTES = NB * TT_BOX;
+  constexpr int Q_OFF = 0, K_OFF = Q_OFF + 2 * HEAD_BYTES, V_OFF = K_OFF + 2 * HEAD_BYTES, BAR_OFF = V_OFF + 2 * HEAD_BYTES;
+  constexpr uint32_t TM_S = 0, TM_O = 256;
+  const TreeArgs& a = tc.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream, a phase a piece
+  uint64_t* k_full = q_full + 2;                                       // [2] by stage
+  uint64_t* v_full = k_full + 2;                                       // [2]
+  uint64_t* k_empty = v_full + 2;                                      // [2] both streams' issuers
+  uint64_t* v_empty = k_empty + 2;                                     // [2]
+  uint64_t* s_full = v_empty + 2;                                      // [4] stream x half
+  uint64_t* p_full = s_full + 4;                                       // [4]
+  uint64_t* pv_done = p_full + 4;                                      // [4]
+  uint64_t* o_done = pv_done + 4;                                      // [2]
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(o_done + 2);
+  int* odd = reinterpret_cast<int*>(tmem_at + 1);                      // [4] piece whose V had values that are not finite, by its number mod 4
+  long long* first = reinterpret_cast<long long*>(smem + BAR_OFF + 256);
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  tree_line(a, first);
+  const long long total = first[a.d.B];
+  const long long u_begin = tree_cut(total, blockIdx.x, a.ctas), u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&k_empty[i], 2);
+      mbar_init(&v_empty[i], 2);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+      odd[i] = -1;
+    }
+    fence_barrier_init();
+  }
+  if (warp == 3) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_at;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer: the lanes know the pages of a tile's boxes, the first issues
+    const int boxes = TT_KEYS / tc.box;
+    int g = 0;
+    for (long long u = u_begin; u < u_end;) {
+      const TreePiece p = tree_piece(a, first, u, u_end);
+      u += p.n;
+      auto pages_of = [&](int j) {
+        const long long key = (long long)(p.t0 + j) * TT_KEYS + lane * tc.box;
+        return lane < boxes && key < p.s.keys ? tree_page(a, p.b, key) : -1;
+      };
+      int page = pages_of(0);
+      for (int j = 0; j < p.n; ++j, ++g) {
+        const int st = g & 1, next = j + 1 < p.n ? pages_of(j + 1) : -1;
+        const long long key = (long long)(p.t0 + j) * TT_KEYS;
+        const uint32_t ph = (g >> 1) & 1;
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t* full = kv ? &v_full[st] : &k_full[st];
+          if (g >= 2) mbar_wait_warp(kv ? &v_empty[st] : &k_empty[st], ph ^ 1);
+          if (lane == 0) mbar_arrive_expect_tx(full, HEAD_BYTES);
+          uint8_t* at = smem + (kv ? V_OFF : K_OFF) + st * HEAD_BYTES;
+          for (int i = 0; i < boxes; ++i) {
+            const int pg = __shfl_sync(0xffffffffu, page, i);
+            const int row = (int)((key + i * tc.box) % a.d.page_size);
+            if (lane == 0) {
+#pragma unroll
+              for (int c = 0; c < NB; ++c) tma_load_4d(at + c * TT_BOX + i * tc.box * 128, kv ? &tmV : &tmK, full, c * 64, p.kvh, row, pg);
+            }
+          }
+        }
+        page = next;
+      }
+    }
+  } else if (warp == 1 || warp == 2) {
+    // ---------------------------------------------------------------- MMA issuer of a stream
+    const int q = warp - 1;
+    const bool issue = elect_one();
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0, 0), idesc_o = umma_idesc_bf16(128, DH, 0, 1);
+    const uint32_t q_addr = smem_u32(smem + Q_OFF + q * HEAD_BYTES), s_tm = tmem_base + TM_S + (uint32_t)q * 128, d_o = tmem_base + TM_O + (uint32_t)q * 128;
+    int g = 0, nt = 0, pieces = 0;      // tiles so far; tiles and pieces of this stream
+    for (long long u = u_begin; u < u_end;) {
+      const TreePiece p = tree_piece(a, first, u, u_end);
+      u += p.n;
+      if (p.r0 + q * 128 >= p.s.n * a.group) {      // no rows here: the stages are passed on
+        for (int j = 0; j < p.n; ++j, ++g) {
+          mbar_wait_warp(&k_full[g & 1], (g >> 1) & 1);
+          if (issue) mbar_arrive(&k_empty[g & 1]);
+          mbar_wait_warp(&v_full[g & 1], (g >> 1) & 1);
+          if (issue) mbar_arrive(&v_empty[g & 1]);
+        }
+        continue;
+      }
+      auto issue_S = [&](int gt, int h) {
+        const uint32_t k_addr = smem_u32(smem + K_OFF + (gt & 1) * HEAD_BYTES) + (uint32_t)h * 64 * 128;
+        if (issue) {
+#pragma unroll
+          for (int ks = 0; ks < KS_QK; ++ks) {
+            const uint32_t off = (ks >> 2) * TT_BOX + (ks & 3) * 32;
+            umma_ss(s_tm + (uint32_t)h * 64, umma_desc_sw128(q_addr + off, 0, 1024), umma_desc_sw128(k_addr + off, 0, 1024), idesc_s, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[q * 2 + h]);
+        }
+      };
+      auto issue_PV = [&](int gt, int j, int h) {
+        const uint32_t v_addr = smem_u32(smem + V_OFF + (gt & 1) * HEAD_BYTES);
+        mbar_wait_warp(&p_full[q * 2 + h], (nt + j) & 1);
+        tc_fence_after();
+        if (issue) {
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const int ks = h * 4 + k4;
+            umma_ts(d_o, s_tm + (uint32_t)h * 64 + k4 * 8, umma_desc_sw128(v_addr + ks * 2048, TT_BOX, 1024), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+          }
+          umma_commit(&pv_done[q * 2 + h]);
+        }
+      };
+      mbar_wait_warp(&q_full[q], pieces & 1);
+      mbar_wait_warp(&k_full[g & 1], (g >> 1) & 1);
+      tc_fence_after();
+      issue_S(g, 0);
+      issue_S(g, 1);
+      if (issue) umma_commit(&k_empty[g & 1]);
+      for (int j = 0; j < p.n; ++j) {
+        const int gt = g + j;
+        const bool more = j + 1 < p.n;
+        mbar_wait_warp(&v_full[gt & 1], (gt >> 1) & 1);
+        issue_PV(gt, j, 0);
+        if (more) {
+          mbar_wait_warp(&k_full[(gt + 1) & 1], ((gt + 1) >> 1) & 1);
+          tc_fence_after();
+          issue_S(gt + 1, 0);
+        }
+        issue_PV(gt, j, 1);
+        if (issue) umma_commit(&v_empty[gt & 1]);
+        if (more) {
+          issue_S(gt + 1, 1);
+          if (issue) umma_commit(&k_empty[(gt + 1) & 1]);
+        } else if (issue) {
+          umma_commit(&o_done[q]);
+        }
+      }
+      g += p.n;
+      nt += p.n;
+      ++pieces;
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- softmax: thread = row
+    const int q = (warp - 4) >> 2, lg = warp & 3, r = lg * 32 + lane;
+    const uint32_t lane_addr = tmem_base + ((uint32_t)(lg * 32) << 16);
+    const uint32_t s_addr = lane_addr + TM_S + (uint32_t)q * 128, o_addr = lane_addr + TM_O + (uint32_t)q * 128;
+    int g = 0, nt = 0, pieces = 0, seg = 0;
+    for (long long u = u_begin; u < u_end; ++seg) {
+      const TreePiece p = tree_piece(a, first, u, u_end);
+      u += p.n;
+      const int rows = p.s.n * a.group;
+      if (p.r0 + q * 128 >= rows) { g += p.n; continue; }
+      const bool both = p.r0 + 128 < rows && a.rows > 128;             // the other stream is at the same tiles
+      const int row = p.r0 + q * 128 + r;
+      const bool row_ok = row < rows;
+      const int node = row_ok ? row / a.group : 0, head = p.kvh * a.group + (row_ok ? row % a.group : 0);
+      // the row's queries, in the swizzled layout that TMA writes
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + p.b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head);
+        uint8_t* at = smem + Q_OFF + q * HEAD_BYTES + r * 128;
+#pragma unroll
+        for (int c = 0; c < NB * 8; ++c) {
+          const uint4 x = row_ok && c < DH / 8 ? src[c] : make_uint4(0, 0, 0, 0);
+          sts_u4(at + (c >> 3) * TT_BOX + (((c & 7) ^ (r & 7)) << 4), x);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[q]);
+      }
+      const unsigned long long* words = a.d.mask + p.b * a.d.mask_batch + node * a.d.mask_node;
+      // which of a half's 64 keys there are, by their pages (known a step ahead)
+      const int box = min(tc.box, 64), n_box = 64 / box;
+      const bool paged = a.d.page_table != nullptr;
+      auto page_there = [&](long long key0) {
+        const long long key = key0 + lane * box;
+        return !paged || lane >= n_box || key >= p.s.keys || tree_page(a, p.b, key) >= 0;
+      };
+      bool there_next = page_there((long long)p.t0 * TT_KEYS);
+      float m_used = -INFINITY, l_sum = 0.f;
+      uint32_t v[64];
+      mbar_wait(&s_full[q * 2], nt & 1);
+      tc_fence_after();
+      LP_TMEM_LD_32((v + 0), s_addr + 0);
+      LP_TMEM_LD_32((v + 32), s_addr + 32);
+#pragma unroll 1
+      for (int t = 0; t < 2 * p.n; ++t) {
+        const int j = t >> 1, h = t & 1;
+        const long long key0 = (long long)(p.t0 + j) * TT_KEYS + h * 64;
+        const bool tail = (long long)(p.t0 + j + 1) * TT_KEYS > p.s.len;
+        const unsigned pages = __ballot_sync(0xffffffffu, there_next);
+        if (t + 1 < 2 * p.n) there_next = page_there(key0 + 64);
+        if (tail && h == 0) {
+          // V of this tile before its product: rows that are not keys, values that are not finite
+          mbar_wait(&v_full[(g + j) & 1], ((g + j) >> 1) & 1);
+          const bool key_ok = key0 + r < p.s.keys;
+          uint8_t* at = smem + V_OFF + ((g + j) & 1) * HEAD_BYTES + r * 128;
+#pragma unroll 1
+          for (int c = 0; c < NB; ++c) {
+            if (both && NB == 2 && c != q) continue;                   // each stream searches its half of the columns
+            if (both && NB == 1 && q == 1) continue;
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              uint8_t* x_at = at + c * TT_BOX + ((i ^ (r & 7)) << 4);
+              if (!key_ok) { sts_u4(x_at, make_uint4(0, 0, 0, 0)); continue; }
+              uint4 x = lds_u4(x_at);
+              bool bad = false;
+              auto clean = [&](uint32_t& w) {
+                if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; bad = true; }
+                if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; bad = true; }
+              };
+              clean(x.x); clean(x.y); clean(x.z); clean(x.w);
+              if (bad) {
+                sts_u4(x_at, x);
+                *reinterpret_cast<volatile int*>(&odd[seg & 3]) = seg;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          if (both) tt_bar_sync(1, 256);
+        }
+        tmem_wait_ld();
+        unsigned long long sees = ~0ull;
+        if (pages != 0xffffffffu)
+          for (int i = 0; i < n_box; ++i)
+            if (!((pages >> i) & 1)) sees &= ~((box == 64 ? ~0ull : (1ull << box) - 1) << (i * box));
+        if (key0 + 64 > p.s.len) {
+          const long long behind = p.s.keys - key0;                    // keys of this half
+          if (behind < 64) sees &= behind <= 0 ? 0ull : (1ull << (int)behind) - 1;
+          const long long j0 = key0 - p.s.len;                         // the node of the half's first key
+          const int nw = (a.d.T + 63) >> 6;
+          unsigned long long bits;
+          if (j0 < 0) bits = (words[0] << (int)-j0) | ((1ull << (int)-j0) - 1);
+          else {
+            const int w = (int)min(j0 >> 6, (long long)nw), sh = (int)(j0 & 63);
+            bits = w < nw ? words[w] >> sh : 0ull;
+            if (sh && w + 1 < nw) bits |= words[w + 1] << (64 - sh);
+          }
+          sees &= bits;
+        }
+        if (__any_sync(0xffffffffu, sees != ~0ull)) {
+          const uint32_t lo = (uint32_t)sees, hi = (uint32_t)(sees >> 32);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!((lo >> i) & 1)) v[i] = 0xff800000u;
+            if (!((hi >> i) & 1)) v[32 + i] = 0xff800000u;
+          }
+        }
+        const uint64_t sc2 = tt_pk2(a.scale_log2, a.scale_log2);
+        float mx;      // of scores, not scaled yet: scales are not negative here
+        {
+          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 64; i += 8) {
+            m0 = fmaxf(m0, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+            m1 = fmaxf(m1, fmaxf(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])));
+            m2 = fmaxf(m2, fmaxf(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5])));
+            m3 = fmaxf(m3, fmaxf(__uint_as_float(v[i + 6]), __uint_as_float(v[i + 7])));
+          }
+          mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        }
+        const float m_new = fmaxf(m_used, mx * a.scale_log2);
+        const bool grow = (m_new - m_used) > 8.0f;
+        if (t == 0) {
+          m_used = m_new;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          // every product issued so far has to be done before O is scaled in place
+          mbar_wait(&pv_done[q * 2 + (h ^ 1)], (nt + ((t - 1) >> 1)) & 1);
+          tc_fence_after();
+          float alpha = 1.0f;
+          if (grow) {
+            alpha = ta_ex2(m_used - m_new);
+            m_used = m_new;
+            l_sum *= alpha;
+          }
+#pragma unroll 1
+          for (int c = 0; c < DH / 16; ++c) {
+            uint32_t o[16];
+            LP_TMEM_LD_16(o, o_addr + c * 16);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            LP_TT_TMEM_ST_16(o, o_addr + c * 16);
+          }
+          tmem_wait_st();
+        }
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        const uint64_t nm2 = tt_pk2(neg_m, neg_m);
+        uint64_t acc2 = tt_pk2(0.f, 0.f);
+        const int jn = (t + 1) >> 1, hn = (t + 1) & 1;
+        const bool has_next = t + 1 < 2 * p.n;
+        const bool s_ready = has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + jn) & 1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            tt_upk2(tt_fma2(tt_pk2(__uint_as_float(v[c * 32 + i]), __uint_as_float(v[c * 32 + i + 1])), sc2, nm2), x0, x1);
+            const float p0 = ta_ex2(x0), p1 = ta_ex2(x1);
+            acc2 = tt_add2(acc2, tt_pk2(p0, p1));
+            pk[i >> 1] = pack_bf16x2(p0, p1);      // half a step is 2^-8 of a weight; their sum is taken in fp32 before
+          }
+          LP_TT_TMEM_ST_16(pk, s_addr + h * 64 + c * 16);
+        }
+        bool loaded = false;
+        if (s_ready || (has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + jn) & 1))) {
+          tc_fence_after();
+          LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
+          LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
+          loaded = true;
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[q * 2 + h]);
+        {
+          float a0, a1;
+          tt_upk2(acc2, a0, a1);
+          l_sum += a0 + a1;
+        }
+        if (has_next && !loaded) {
+          mbar_wait(&s_full[q * 2 + hn], (nt + jn) & 1);
+          tc_fence_after();
+          LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
+          LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
+        }
+      }
+      // ---- O of this piece
+      mbar_wait(&o_done[q], pieces & 1);
+      tc_fence_after();
+      const bool whole = p.t0 == 0 && p.n == p.s.tiles;
+      const bool fix = *reinterpret_cast<volatile int*>(&odd[seg & 3]) == seg;
+      const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;
+      const long long slot = ((2LL * blockIdx.x + (p.t0 == 0 ? 1 : 0)) * a.rows + q * 128 + r);
+      bf16* out = reinterpret_cast<bf16*>(a.d.out) + p.b * a.d.o_batch + node * a.d.o_node + head * a.d.o_head;
+      float* part = a.part_o + slot * DH;
+      if (!whole && row_ok) a.part_ml[slot] = make_float2(m_used, l_sum);
+#pragma unroll 1
+      for (int c = 0; c < DH / 16; ++c) {
+        uint32_t o[16];
+        LP_TMEM_LD_16(o, o_addr + c * 16);
+        tmem_wait_ld();
+        if (fix) {
+          const long long k1 = min(p.s.keys, (long long)(p.t0 + p.n) * TT_KEYS);
+          for (long long key = max((long long)p.t0, (long long)(p.s.len / TT_KEYS)) * TT_KEYS; key < k1; ++key) {
+            const int page = tree_page(a, p.b, key), nd = (int)max(0LL, key - p.s.len);
+            if (page < 0 || (key >= p.s.len && !((words[nd >> 6] >> (nd & 63)) & 1))) continue;
+            const bf16* vr = reinterpret_cast<const bf16*>(a.d.v) + page * a.d.v_page + (key % a.d.page_size) * a.d.v_row + p.kvh * a.d.v_head + c * 16;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = __bfloat162float(vr[i]);
+              if (not_finite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+            }
+          }
+        }
+        if (!row_ok) continue;
+        if (whole) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
+          *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(out + c * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(part + c * 16 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();
+      g += p.n;
+      nt += p.n;
+      ++pieces;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 3) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// rows of a TMA box: a cache of one page a sequence takes whole tiles, else the largest part of a tile that pages are multiples of
+static int tree_box(const lp_tree_attn_desc* d) {
+  if (d->max_pages == 1) return 128;
+  for (int box = 128; box >= 8; box /= 2)
+    if (d->page_size % box == 0) return box;
+  return 0;
+}
+bool tree_tc_takes(const lp_tree_attn_desc* d) {
+  const bool strides = (d->n_pages == 1 || (d->k_page > 0 && d->v_page > 0)) && (d->page_size == 1 || (d->k_row > 0 && d->v_row > 0)) &&
+                       (d->KVH == 1 || (d->k_head > 0 && d->v_head > 0));
+  return tree_box(d) != 0 && strides && d->scale > 0.f;      // (0 x -inf is not -inf)
+}
+
+template <int DH>
+static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
+  constexpr int NB = (DH + 63) / 64;
+  const lp_tree_attn_desc& d = tc.a.d;
+  CUtensorMap tm[2];
+  const void* base[2] = {d.k, d.v};
+  const long long page[2] = {d.k_page, d.v_page}, row[2] = {d.k_row, d.v_row}, head[2] = {d.k_head, d.v_head};
+  const uint32_t box[4] = {64, 1, (uint32_t)tc.box, 1};
+  for (int i = 0; i < 2; ++i) {      // of a dimension of one the distance is any
+    const uint64_t dims[4] = {(uint64_t)d.D, (uint64_t)d.KVH, (uint64_t)d.page_size, (uint64_t)d.n_pages};
+    const uint64_t strides[3] = {d.KVH == 1 ? (uint64_t)d.D : (uint64_t)head[i], d.page_size == 1 ? (uint64_t)d.D : (uint64_t)row[i], d.n_pages == 1 ? (uint64_t)d.D : (uint64_t)page[i]};
+    if (const int rc = make_tmap_bf16_4d(&tm[i], base[i], dims, strides, box)) return rc;
+  }
+  const size_t smem = 6 * NB * TT_BOX + 256 + (size_t)(d.B + 1) * 8 + 1024;
+  LP_CHECK_CUDA(cudaFuncSetAttribute(tree_tc_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  tree_tc_kernel<DH><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+  LP_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int launch_tree_tc(const TreeArgs& a, cudaStream_t stream) {
+  TreeTc tc;
+  tc.a = a;
+  tc.box = tree_box(&a.d);
+  if (a.d.D == 128) return launch_tc<128>(tc, stream);
+  if (a.d.D == 96) return launch_tc<96>(tc, stream);
+  return launch_tc<64>(tc, stream);
+}
+
+}  // namespace lp
