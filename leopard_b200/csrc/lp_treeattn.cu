@@ -285,7 +285,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 }
 
 // Rows whose tiles lie in several CTAs: a warp joins a row.
-constexpr int TA_JOIN_WARPS = 4;
+constexpr int TA_JOIN_WARPS = 4, TA_JOIN_DEEP = 8;
 template <int D>
 __global__ void __launch_bounds__(32 * TA_JOIN_WARPS)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
@@ -301,20 +301,33 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   const long long at = join_first[b] + ((long long)kvh * s.blocks + blk) * s.tiles;
   const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
   if (c0 == c1) return;                                  // written whole
+  // the first piece begins with the item (slot 2 c + 1), the others begin inside it; TA_JOIN_DEEP rows of values are under way at once
   float top = -INFINITY;
   for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[(2LL * c + (c == c0 ? 1 : 0)) * a.rows + r].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const long long slot = 2LL * c + (c == c0 ? 1 : 0);  // the first piece begins with the item, the others begin inside it
-    const float2 p = a.part_ml[slot * a.rows + r];
-    const float f = p.x == -INFINITY ? 1.f : ta_ex2(p.x - top);
-    sum += p.y * f;
-    if (lane < D / 4) {
-      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (slot * a.rows + r) * D + lane * 4);
-      x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
+  const float* from = a.part_o + (size_t)r * D + lane * 4;
+  for (int base = c0; base <= c1; base += TA_JOIN_DEEP) {
+    float4 y[TA_JOIN_DEEP];
+    float2 p = make_float2(-INFINITY, 0.f);
+    if (lane < TA_JOIN_DEEP && base + lane <= c1) {
+      const int c = base + lane;
+      p = a.part_ml[(2LL * c + (c == c0 ? 1 : 0)) * a.rows + r];
+    }
+#pragma unroll
+    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
+      const int c = base + k;
+      y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c <= c1 && lane < D / 4) y[k] = *reinterpret_cast<const float4*>(from + (2LL * c + (c == c0 ? 1 : 0)) * a.rows * D);
+    }
+    const float weight = p.x == -INFINITY ? 1.f : ta_ex2(p.x - top);      // of a piece that saw nothing: its values are zeros, or NaN
+#pragma unroll
+    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
+      const float f = __shfl_sync(0xffffffffu, weight, k);
+      sum += __shfl_sync(0xffffffffu, p.y, k) * f;
+      x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
     }
   }
   if (lane < D / 4) {

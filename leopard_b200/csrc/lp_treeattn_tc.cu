@@ -67,13 +67,19 @@ __device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const long lo
   p.r0 = (item % p.s.blocks) * a.rows;
   return p;
 }
-// the page that holds row `key` of sequence b (-1: none)
-__device__ __forceinline__ int tree_page(const TreeArgs& a, int b, long long key) {
-  const long long logical = key / a.d.page_size;
-  if (logical >= a.d.max_pages) return -1;
-  const int page = a.d.page_table ? a.d.page_table[b * a.d.ld_table + logical] : b;
-  return page >= 0 && page < a.d.n_pages ? page : -1;
-}
+// where row `key` of a sequence lies: its place in the page table and in the page.  A sequence's rows are fewer than 2^31 (the entry point sees to it).
+struct TreePlace {
+  int index, row;
+  __device__ __forceinline__ TreePlace(const TreeArgs& a, int key) : index(key / a.d.page_size), row(key - index * a.d.page_size) {}
+  __device__ __forceinline__ void forward(const TreeArgs& a, int keys) {
+    for (row += keys; row >= a.d.page_size; ++index) row -= a.d.page_size;
+  }
+  __device__ __forceinline__ int page(const TreeArgs& a, int b) const {      // -1: none
+    if (index >= a.d.max_pages) return -1;
+    const int page = a.d.page_table ? a.d.page_table[b * a.d.ld_table + index] : b;
+    return page >= 0 && page < a.d.n_pages ? page : -1;
+  }
+};
 
 template <int DH>
 __global__ void __launch_bounds__(TT_THREADS, 1)
@@ -137,26 +143,30 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     for (long long u = u_begin; u < u_end;) {
       const TreePiece p = tree_piece(a, first, u, u_end);
       u += p.n;
-      auto pages_of = [&](int j) {
-        const long long key = (long long)(p.t0 + j) * TT_KEYS + lane * tc.box;
-        return lane < boxes && key < p.s.keys ? tree_page(a, p.b, key) : -1;
-      };
-      int page = pages_of(0);
+      const int n_keys = (int)p.s.keys;
+      int key = p.t0 * TT_KEYS + lane * tc.box;      // this lane's box of the tile
+      TreePlace at(a, lane < boxes ? key : 0);
+      auto page_of = [&]() { return lane < boxes && key < n_keys ? at.page(a, p.b) : -1; };
+      int page = page_of();
       for (int j = 0; j < p.n; ++j, ++g) {
-        const int st = g & 1, next = j + 1 < p.n ? pages_of(j + 1) : -1;
-        const long long key = (long long)(p.t0 + j) * TT_KEYS;
+        const int st = g & 1, row = at.row;
+        int next = -1;
+        if (j + 1 < p.n) {
+          key += TT_KEYS;
+          if (lane < boxes) at.forward(a, TT_KEYS);
+          next = page_of();
+        }
         const uint32_t ph = (g >> 1) & 1;
         for (int kv = 0; kv < 2; ++kv) {
           uint64_t* full = kv ? &v_full[st] : &k_full[st];
           if (g >= 2) mbar_wait_warp(kv ? &v_empty[st] : &k_empty[st], ph ^ 1);
           if (lane == 0) mbar_arrive_expect_tx(full, HEAD_BYTES);
-          uint8_t* at = smem + (kv ? V_OFF : K_OFF) + st * HEAD_BYTES;
+          uint8_t* to = smem + (kv ? V_OFF : K_OFF) + st * HEAD_BYTES;
           for (int i = 0; i < boxes; ++i) {
-            const int pg = __shfl_sync(0xffffffffu, page, i);
-            const int row = (int)((key + i * tc.box) % a.d.page_size);
+            const int pg = __shfl_sync(0xffffffffu, page, i), r = __shfl_sync(0xffffffffu, row, i);
             if (lane == 0) {
 #pragma unroll
-              for (int c = 0; c < NB; ++c) tma_load_4d(at + c * TT_BOX + i * tc.box * 128, kv ? &tmV : &tmK, full, c * 64, p.kvh, row, pg);
+              for (int c = 0; c < NB; ++c) tma_load_4d(to + c * TT_BOX + i * tc.box * 128, kv ? &tmV : &tmK, full, c * 64, p.kvh, r, pg);
             }
           }
         }
@@ -266,11 +276,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       // which of a half's 64 keys there are, by their pages (known a step ahead)
       const int box = min(tc.box, 64), n_box = 64 / box;
       const bool paged = a.d.page_table != nullptr;
-      auto page_there = [&](long long key0) {
-        const long long key = key0 + lane * box;
-        return !paged || lane >= n_box || key >= p.s.keys || tree_page(a, p.b, key) >= 0;
-      };
-      bool there_next = page_there((long long)p.t0 * TT_KEYS);
+      const int n_keys = (int)p.s.keys, len = p.s.len;
+      int box_key = p.t0 * TT_KEYS + lane * box;
+      TreePlace box_at(a, paged && lane < n_box ? box_key : 0);
+      auto page_there = [&]() { return !paged || lane >= n_box || box_key >= n_keys || box_at.page(a, p.b) >= 0; };
+      bool there_next = page_there();
       float m_used = -INFINITY, l_sum = 0.f;
       uint32_t v[64];
       mbar_wait(&s_full[q * 2], nt & 1);
@@ -280,14 +290,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll 1
       for (int t = 0; t < 2 * p.n; ++t) {
         const int j = t >> 1, h = t & 1;
-        const long long key0 = (long long)(p.t0 + j) * TT_KEYS + h * 64;
-        const bool tail = (long long)(p.t0 + j + 1) * TT_KEYS > p.s.len;
-        const unsigned pages = __ballot_sync(0xffffffffu, there_next);
-        if (t + 1 < 2 * p.n) there_next = page_there(key0 + 64);
+        const int key0 = (p.t0 + j) * TT_KEYS + h * 64;
+        const bool tail = key0 - h * 64 + TT_KEYS > len;
+        const unsigned pages = paged ? __ballot_sync(0xffffffffu, there_next) : 0xffffffffu;
+        if (paged && t + 1 < 2 * p.n) {
+          box_key += 64;
+          if (lane < n_box) box_at.forward(a, 64);
+          there_next = page_there();
+        }
         if (tail && h == 0) {
           // V of this tile before its product: rows that are not keys, values that are not finite
           mbar_wait(&v_full[(g + j) & 1], ((g + j) >> 1) & 1);
-          const bool key_ok = key0 + r < p.s.keys;
+          const bool key_ok = key0 + r < n_keys;
           uint8_t* at = smem + V_OFF + ((g + j) & 1) * HEAD_BYTES + r * 128;
 #pragma unroll 1
           for (int c = 0; c < NB; ++c) {
@@ -318,15 +332,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (pages != 0xffffffffu)
           for (int i = 0; i < n_box; ++i)
             if (!((pages >> i) & 1)) sees &= ~((box == 64 ? ~0ull : (1ull << box) - 1) << (i * box));
-        if (key0 + 64 > p.s.len) {
-          const long long behind = p.s.keys - key0;                    // keys of this half
-          if (behind < 64) sees &= behind <= 0 ? 0ull : (1ull << (int)behind) - 1;
-          const long long j0 = key0 - p.s.len;                         // the node of the half's first key
-          const int nw = (a.d.T + 63) >> 6;
+        if (key0 + 64 > len) {
+          const int behind = n_keys - key0;                            // keys of this half
+          if (behind < 64) sees &= behind <= 0 ? 0ull : (1ull << behind) - 1;
+          const int j0 = key0 - len, nw = (a.d.T + 63) >> 6;           // the node of the half's first key
           unsigned long long bits;
-          if (j0 < 0) bits = (words[0] << (int)-j0) | ((1ull << (int)-j0) - 1);
+          if (j0 < 0) bits = (words[0] << -j0) | ((1ull << -j0) - 1);
           else {
-            const int w = (int)min(j0 >> 6, (long long)nw), sh = (int)(j0 & 63);
+            const int w = min(j0 >> 6, nw), sh = j0 & 63;
             bits = w < nw ? words[w] >> sh : 0ull;
             if (sh && w + 1 < nw) bits |= words[w + 1] << (64 - sh);
           }
@@ -435,11 +448,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         LP_TMEM_LD_16(o, o_addr + c * 16);
         tmem_wait_ld();
         if (fix) {
-          const long long k1 = min(p.s.keys, (long long)(p.t0 + p.n) * TT_KEYS);
-          for (long long key = max((long long)p.t0, (long long)(p.s.len / TT_KEYS)) * TT_KEYS; key < k1; ++key) {
-            const int page = tree_page(a, p.b, key), nd = (int)max(0LL, key - p.s.len);
-            if (page < 0 || (key >= p.s.len && !((words[nd >> 6] >> (nd & 63)) & 1))) continue;
-            const bf16* vr = reinterpret_cast<const bf16*>(a.d.v) + page * a.d.v_page + (key % a.d.page_size) * a.d.v_row + p.kvh * a.d.v_head + c * 16;
+          const int k1 = min(n_keys, (p.t0 + p.n) * TT_KEYS);
+          for (int key = max(p.t0, len / TT_KEYS) * TT_KEYS; key < k1; ++key) {
+            const TreePlace at(a, key);
+            const int page = at.page(a, p.b), nd = max(0, key - len);
+            if (page < 0 || (key >= len && !((words[nd >> 6] >> (nd & 63)) & 1))) continue;
+            const bf16* vr = reinterpret_cast<const bf16*>(a.d.v) + page * a.d.v_page + at.row * a.d.v_row + p.kvh * a.d.v_head + c * 16;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float x = __bfloat162float(vr[i]);
