@@ -39,7 +39,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   uint32_t* present = reinterpret_cast<uint32_t*>(place + TA_RING * TA_KEYS);       // [ring][2]
   float2* ml = reinterpret_cast<float2*>(present + TA_RING * 2);                    // [WN][R]
   long long* first = reinterpret_cast<long long*>(ml + WN * R);                     // [B + 1]
-  float* obuf = reinterpret_cast<float*>(ta_smem);                                  // [R][D], when the tiles are done with
+  constexpr int LDO = D + 4;
+  float* obuf = reinterpret_cast<float*>(ta_smem);                                  // [R][LDO], when the tiles are done with
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM, g = lane >> 2, t4 = lane & 3;
   pdl_launch_dependents();
   tree_line(a, first);
@@ -254,7 +255,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
           for (int d = 0; d < D / 8; ++d)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              float* at = obuf + r * D + d * 8 + 2 * t4 + k;
+              float* at = obuf + r * LDO + d * 8 + 2 * t4 + k;
               *at = w == 0 ? o[d][2 * h + k] * f : *at + o[d][2 * h + k] * f;
             }
         if (WN > 1) __syncthreads();
@@ -263,77 +264,94 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     if (WN == 1) __syncthreads();
     const bool whole = t0 == 0 && t1 == s.tiles;
     const long long slot = 2LL * blockIdx.x + (t0 == 0 ? 1 : 0);
-    for (int c = tid; c < n_rows * (D / 4); c += NT) {
-      const int r = c / (D / 4), col = (c % (D / 4)) * 4;
-      float4 x = *reinterpret_cast<const float4*>(obuf + r * D + col);
-      float top = -INFINITY, sum = 0.f;
+    auto row_ml = [&](int r) {                             // of all warps' keys
+      float2 x = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int w = 0; w < WN; ++w) top = fmaxf(top, ml[w * R + r].x);
+      for (int w = 0; w < WN; ++w) x.x = fmaxf(x.x, ml[w * R + r].x);
 #pragma unroll
-      for (int w = 0; w < WN; ++w) sum += ml[w * R + r].y * (ml[w * R + r].x == -INFINITY ? 1.f : ta_ex2(ml[w * R + r].x - top));
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      for (int w = 0; w < WN; ++w) x.y += ml[w * R + r].y * (ml[w * R + r].x == -INFINITY ? 1.f : ta_ex2(ml[w * R + r].x - x.x));
+      return x;
+    };
+    if (whole) {
+      for (int c = tid; c < n_rows * (D / 4); c += NT) {
+        const int r = c / (D / 4), col = (c % (D / 4)) * 4;
+        const float4 x = *reinterpret_cast<const float4*>(obuf + r * LDO + col);
+        const float sum = row_ml(r).y, inv = sum == 0.f ? 0.f : 1.f / sum;
         bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + ((r0 + r) / a.group) * a.d.o_node + (kvh * a.group + (r0 + r) % a.group) * a.d.o_head;
         *reinterpret_cast<uint2*>(out + col) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(a.part_o + (slot * R + r) * D + col) = x;
-        if (col == 0) a.part_ml[slot * R + r] = make_float2(top, sum);
+      }
+    } else {
+      for (int c = tid; c < R * (D / 4); c += NT) {
+        const int r = c % R, c4 = c / R;
+        if (r >= n_rows) continue;
+        *reinterpret_cast<float4*>(a.part_o + ((slot * (D / 4) + c4) * R + r) * 4) = *reinterpret_cast<const float4*>(obuf + r * LDO + c4 * 4);
+        if (c4 == 0) a.part_ml[slot * R + r] = row_ml(r);
       }
     }
     __syncthreads();
   }
 }
 
-// Rows whose tiles lie in several CTAs: a warp joins a row.
-constexpr int TA_JOIN_WARPS = 4, TA_JOIN_DEEP = 8;
+// Rows whose tiles lie in several CTAs: a CTA joins 32 rows of a key head, a lane a row, a warp every eighth four columns; TA_JOIN_DEEP pieces are under way at once.
+constexpr int TA_JOIN_WARPS = 8, TA_JOIN_DEEP = 4;
 template <int D>
 __global__ void __launch_bounds__(32 * TA_JOIN_WARPS)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
+  constexpr int COLS = D / 4 / TA_JOIN_WARPS;
   extern __shared__ long long join_first[];
+  __shared__ __align__(16) bf16 done[32][D + 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * 32;
   tree_line(a, join_first);
-  const int lane = threadIdx.x & 31, b = blockIdx.z, kvh = blockIdx.y;
   const TreeSeq s = tree_seq(a, b);
   const long long total = join_first[a.d.B];
-  const int row = blockIdx.x * TA_JOIN_WARPS + (threadIdx.x >> 5);      // of the sequence and key head
+  const int rows = s.n * a.group;
   pdl_wait();
-  if (row >= s.n * a.group) return;
-  const int blk = row / a.rows, r = row % a.rows;
+  if (row0 >= rows) return;
+  const int blk = row0 / a.rows, r = row0 % a.rows + lane;      // (a block is whole 32s, or 16 rows and all there is)
   const long long at = join_first[b] + ((long long)kvh * s.blocks + blk) * s.tiles;
   const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
   if (c0 == c1) return;                                  // written whole
-  // the first piece begins with the item (slot 2 c + 1), the others begin inside it; TA_JOIN_DEEP rows of values are under way at once
+  const bool there = row0 + lane < rows && r < a.rows;
+  // the first piece begins with the item (slot 2 c + 1), the others begin inside it
+  auto slot = [&](int c) { return 2LL * c + (c == c0 ? 1 : 0); };
   float top = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[(2LL * c + (c == c0 ? 1 : 0)) * a.rows + r].x);
+#pragma unroll 8
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, there ? a.part_ml[slot(c) * a.rows + r].x : -INFINITY);
+  float4 x[COLS];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < COLS; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  const float* from = a.part_o + (size_t)r * D + lane * 4;
   for (int base = c0; base <= c1; base += TA_JOIN_DEEP) {
-    float4 y[TA_JOIN_DEEP];
-    float2 p = make_float2(-INFINITY, 0.f);
-    if (lane < TA_JOIN_DEEP && base + lane <= c1) {
-      const int c = base + lane;
-      p = a.part_ml[(2LL * c + (c == c0 ? 1 : 0)) * a.rows + r];
+    float4 y[TA_JOIN_DEEP][COLS];
+    float2 p[TA_JOIN_DEEP];
+#pragma unroll
+    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
+      const bool on = there && base + k <= c1;
+      p[k] = on ? a.part_ml[slot(base + k) * a.rows + r] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int i = 0; i < COLS; ++i)
+        y[k][i] = on ? *reinterpret_cast<const float4*>(a.part_o + ((slot(base + k) * (D / 4) + i * TA_JOIN_WARPS + warp) * a.rows + r) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int k = 0; k < TA_JOIN_DEEP; ++k) {
-      const int c = base + k;
-      y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (c <= c1 && lane < D / 4) y[k] = *reinterpret_cast<const float4*>(from + (2LL * c + (c == c0 ? 1 : 0)) * a.rows * D);
-    }
-    const float weight = p.x == -INFINITY ? 1.f : ta_ex2(p.x - top);      // of a piece that saw nothing: its values are zeros, or NaN
+      const float f = p[k].x == -INFINITY ? 1.f : ta_ex2(p[k].x - top);      // of a piece that saw nothing: its values are zeros, or NaN
+      sum += p[k].y * f;
 #pragma unroll
-    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
-      const float f = __shfl_sync(0xffffffffu, weight, k);
-      sum += __shfl_sync(0xffffffffu, p.y, k) * f;
-      x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
+      for (int i = 0; i < COLS; ++i) {
+        x[i].x += y[k][i].x * f; x[i].y += y[k][i].y * f; x[i].z += y[k][i].z * f; x[i].w += y[k][i].w * f;
+      }
     }
   }
-  if (lane < D / 4) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < COLS; ++i)
+    *reinterpret_cast<uint2*>(&done[lane][(i * TA_JOIN_WARPS + warp) * 4]) = make_uint2(pack_bf16x2(x[i].x * inv, x[i].y * inv), pack_bf16x2(x[i].z * inv, x[i].w * inv));
+  __syncthreads();
+  const int n = min(min(32, rows - row0), a.rows);
+  for (int c = threadIdx.x; c < n * (D / 8); c += 32 * TA_JOIN_WARPS) {
+    const int row = row0 + c / (D / 8), col = (c % (D / 8)) * 8;
     bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + (row / a.group) * a.d.o_node + (kvh * a.group + row % a.group) * a.d.o_head;
-    *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+    *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(&done[c / (D / 8)][col]);
   }
 }
 
@@ -421,7 +439,7 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   if (tc) { if (const int rc = launch_tree_tc(a, stream)) return rc; }                                                                          \
   else if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
   LP_CHECK_CUDA(cudaGetLastError());                                                                                                           \
-  LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + TA_JOIN_WARPS - 1) / TA_JOIN_WARPS), d->KVH, d->B), \
+  LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + 31) / 32), d->KVH, d->B), \
                           dim3(32 * TA_JOIN_WARPS), (size_t)(d->B + 1) * 8, stream, 1, true, a));
   if (d->D == 128) { LP_TREE_D(128) } else if (d->D == 96) { LP_TREE_D(96) } else { LP_TREE_D(64) }
 #undef LP_TREE_D

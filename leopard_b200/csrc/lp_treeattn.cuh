@@ -14,7 +14,7 @@ struct TreeArgs {
   lp_tree_attn_desc d;
   int group, rows, keys;                  // query heads of a key head; rows of a block; keys of a tile
   float scale_log2;
-  float* part_o; float2* part_ml;         // [2 x CTAs][rows][D], [2 x CTAs][rows]: maximum (log2 units) and sum
+  float* part_o; float2* part_ml;         // [2 x CTAs][D / 4][rows][4] (a warp writes and reads 32 rows of 4 values side by side), [2 x CTAs][rows]: maximum (log2 units), sum
   int ctas;
 };
 // the tcgen05 kernel (lp_treeattn_tc.cu): whether it takes this cache, and its launch

@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeTc tc) {
   constexpr int NB = (DH + 63) / 64, KS_QK = DH / 16, HEAD_BYTES = NB * TT_BOX;
   constexpr int Q_OFF = 0, K_OFF = Q_OFF + 2 * HEAD_BYTES, V_OFF = K_OFF + 2 * HEAD_BYTES, BAR_OFF = V_OFF + 2 * HEAD_BYTES;
+  constexpr int CH = DH / 8, MAX_WORDS = LP_TREE_MAX_NODES / 64;
   constexpr uint32_t TM_S = 0, TM_O = 256;
   const TreeArgs& a = tc.a;
   extern __shared__ uint8_t smem_raw[];
@@ -101,7 +102,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   uint64_t* o_done = pv_done + 4;                                      // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(o_done + 2);
   int* odd = reinterpret_cast<int*>(tmem_at + 1);                      // [4] piece whose V had values that are not finite, by its number mod 4
-  long long* first = reinterpret_cast<long long*>(smem + BAR_OFF + 256);
+  unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + 256);      // [256][MAX_WORDS] of this thread's row
+  long long* first = reinterpret_cast<long long*>(mask_words + 256 * MAX_WORDS);
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -260,19 +262,29 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const int row = p.r0 + q * 128 + r;
       const bool row_ok = row < rows;
       const int node = row_ok ? row / a.group : 0, head = p.kvh * a.group + (row_ok ? row % a.group : 0);
-      // the row's queries, in the swizzled layout that TMA writes
+      // the warp's rows' queries, in the swizzled layout that TMA writes; 32 lanes take neighbouring pieces of 16 bytes
       {
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + p.b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head);
-        uint8_t* at = smem + Q_OFF + q * HEAD_BYTES + r * 128;
+        const long long from = p.b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head;
+        uint8_t* at = smem + Q_OFF + q * HEAD_BYTES + lg * 32 * 128;
 #pragma unroll
-        for (int c = 0; c < NB * 8; ++c) {
-          const uint4 x = row_ok && c < DH / 8 ? src[c] : make_uint4(0, 0, 0, 0);
-          sts_u4(at + (c >> 3) * TT_BOX + (((c & 7) ^ (r & 7)) << 4), x);
+        for (int i = 0; i < CH; ++i) {
+          const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
+          const long long src = __shfl_sync(0xffffffffu, from, rr);
+          const uint4 x = p.r0 + q * 128 + lg * 32 + rr < rows ? *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + src + c * 8) : make_uint4(0, 0, 0, 0);
+          sts_u4(at + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), x);
         }
+        if (DH % 64 != 0)
+          for (int c = CH; c < NB * 8; ++c) sts_u4(at + (c >> 3) * TT_BOX + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), make_uint4(0, 0, 0, 0));
         fence_proxy_async_smem();
         mbar_arrive(&q_full[q]);
       }
-      const unsigned long long* words = a.d.mask + p.b * a.d.mask_batch + node * a.d.mask_node;
+      // its node's mask, when this piece gets there
+      const int nw = (a.d.T + 63) >> 6;
+      unsigned long long* words = mask_words + (q * 128 + r) * MAX_WORDS;
+      if ((p.t0 + p.n) * TT_KEYS > p.s.len) {
+        const unsigned long long* src = a.d.mask + p.b * a.d.mask_batch + node * a.d.mask_node;
+        for (int w = 0; w < nw; ++w) words[w] = src[w];
+      }
       // which of a half's 64 keys there are, by their pages (known a step ahead)
       const int box = min(tc.box, 64), n_box = 64 / box;
       const bool paged = a.d.page_table != nullptr;
@@ -335,7 +347,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (key0 + 64 > len) {
           const int behind = n_keys - key0;                            // keys of this half
           if (behind < 64) sees &= behind <= 0 ? 0ull : (1ull << behind) - 1;
-          const int j0 = key0 - len, nw = (a.d.T + 63) >> 6;           // the node of the half's first key
+          const int j0 = key0 - len;                                   // the node of the half's first key
           unsigned long long bits;
           if (j0 < 0) bits = (words[0] << -j0) | ((1ull << -j0) - 1);
           else {
@@ -438,10 +450,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const bool whole = p.t0 == 0 && p.n == p.s.tiles;
       const bool fix = *reinterpret_cast<volatile int*>(&odd[seg & 3]) == seg;
       const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;
-      const long long slot = ((2LL * blockIdx.x + (p.t0 == 0 ? 1 : 0)) * a.rows + q * 128 + r);
-      bf16* out = reinterpret_cast<bf16*>(a.d.out) + p.b * a.d.o_batch + node * a.d.o_node + head * a.d.o_head;
-      float* part = a.part_o + slot * DH;
-      if (!whole && row_ok) a.part_ml[slot] = make_float2(m_used, l_sum);
+      const long long slot = 2LL * blockIdx.x + (p.t0 == 0 ? 1 : 0);
+      const int in_block = q * 128 + r;
+      float* part = a.part_o + (slot * (DH / 4) * a.rows + in_block) * 4;
+      uint8_t* stage = smem + Q_OFF + q * HEAD_BYTES + lg * 32 * 128;      // the queries are done with
+      if (!whole && row_ok) a.part_ml[slot * a.rows + in_block] = make_float2(m_used, l_sum);
 #pragma unroll 1
       for (int c = 0; c < DH / 16; ++c) {
         uint32_t o[16];
@@ -461,17 +474,29 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
         }
-        if (!row_ok) continue;
         if (whole) {
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
-          *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(out + c * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
+          uint8_t* at = stage + (c >> 2) * TT_BOX + lane * 128;
+          sts_u4(at + ((((2 * c) & 7) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+          sts_u4(at + ((((2 * c + 1) & 7) ^ (lane & 7)) << 4), make_uint4(w[4], w[5], w[6], w[7]));
+        } else if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(part + c * 16 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(part + (c * 4 + i) * a.rows * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
+      }
+      if (whole) {
+        __syncwarp();
+        const long long to = p.b * a.d.o_batch + node * a.d.o_node + head * a.d.o_head;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
+          const long long dst = __shfl_sync(0xffffffffu, to, rr);
+          const uint4 x = lds_u4(stage + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+          if (p.r0 + q * 128 + lg * 32 + rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.d.out) + dst + c * 8) = x;
+        }
+        __syncwarp();
       }
       tc_fence_before();
       g += p.n;
@@ -513,7 +538,7 @@ static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
     const uint64_t strides[3] = {d.KVH == 1 ? (uint64_t)d.D : (uint64_t)head[i], d.page_size == 1 ? (uint64_t)d.D : (uint64_t)row[i], d.n_pages == 1 ? (uint64_t)d.D : (uint64_t)page[i]};
     if (const int rc = make_tmap_bf16_4d(&tm[i], base[i], dims, strides, box)) return rc;
   }
-  const size_t smem = 6 * NB * TT_BOX + 256 + (size_t)(d.B + 1) * 8 + 1024;
+  const size_t smem = 6 * NB * TT_BOX + 256 + 256 * (LP_TREE_MAX_NODES / 64) * 8 + (size_t)(d.B + 1) * 8 + 1024;
   LP_CHECK_CUDA(cudaFuncSetAttribute(tree_tc_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   tree_tc_kernel<DH><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
   LP_CHECK_CUDA(cudaGetLastError());

@@ -62,7 +62,7 @@ def joined(c, out, part, ml, ctas, rows, want):
             f = torch.where(m == -torch.inf, 1.0, torch.exp2(m - m.max()))
             s = (l * f).sum()
             row = blk * rows + r
-            out[b, row // group, g * group + row % group] = ((part[slots, r].double() * f[:, None]).sum(0) / s if s != 0 else torch.zeros(D, dtype=torch.float64)).to(BF16)
+            out[b, row // group, g * group + row % group] = ((part[slots, :, r].reshape(len(slots), D).double() * f[:, None]).sum(0) / s if s != 0 else torch.zeros(D, dtype=torch.float64)).to(BF16)
     return out
 
 
@@ -96,7 +96,7 @@ def run(emu, c, ctas):
     box = 128 if c["page_table"] is None else next(x for x in (128, 64, 32, 16, 8) if S % x == 0)
     words = O.tree_words(c["sees"])
     out = torch.full((B, T, H, D), 7.0).to(BF16)
-    part, ml = torch.full((2 * ctas, rows, D), float("nan")), torch.full((2 * ctas, rows, 2), float("nan"))
+    part, ml = torch.full((2 * ctas, D // 4, rows, 4), float("nan")), torch.full((2 * ctas, rows, 2), float("nan"))
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     d = _lib.TreeAttnDesc(ptr(c["q"]), *c["q"].stride()[:3], ptr(c["k"]), *c["k"].stride()[:3], ptr(c["v"]), *c["v"].stride()[:3], ptr(out), *out.stride()[:3],
                           ptr(c["page_table"]), 0 if c["page_table"] is None else c["page_table"].shape[1], 1 if c["page_table"] is None else c["page_table"].shape[1], P, S,
