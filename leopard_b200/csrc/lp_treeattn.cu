@@ -52,7 +52,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     const int b = tree_find(first, a.d.B, u);
     const TreeSeq s = tree_seq(a, b);
     const long long local = u - first[b];
-    const int item = (int)(local / s.tiles), t0 = (int)(local % s.tiles), t1 = (int)min((long long)s.tiles, t0 + (u_end - u));
+    const int item = (int)tree_div(local, s.tiles), t0 = (int)(local - (long long)item * s.tiles), t1 = (int)min((long long)s.tiles, t0 + (u_end - u));
     const int kvh = item / s.blocks, r0 = (item % s.blocks) * R;
     u += t1 - t0;
     const int n_rows = min(R, s.n * a.group - r0);
@@ -292,66 +292,61 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   }
 }
 
-// Rows whose tiles lie in several CTAs: a CTA joins 32 rows of a key head, a lane a row, a warp every eighth four columns; TA_JOIN_DEEP pieces are under way at once.
-constexpr int TA_JOIN_WARPS = 8, TA_JOIN_DEEP = 4;
+// Rows whose tiles lie in several CTAs: a CTA joins 8 rows of a key head, a thread four columns of a row over all pieces.  Bound by latency: TA_JOIN_DEEP pieces are under way
+// at once, and their weights follow a running maximum, so that each is read once.
+constexpr int TA_JOIN_ROWS = 8, TA_JOIN_DEEP = 10;
 template <int D>
-__global__ void __launch_bounds__(32 * TA_JOIN_WARPS)
+__global__ void __launch_bounds__(TA_JOIN_ROWS * D / 4)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
-  constexpr int COLS = D / 4 / TA_JOIN_WARPS;
   extern __shared__ long long join_first[];
-  __shared__ __align__(16) bf16 done[32][D + 8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * 32;
+  __shared__ __align__(16) bf16 done[TA_JOIN_ROWS][D + 8];
+  const int b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * TA_JOIN_ROWS, in = threadIdx.x % TA_JOIN_ROWS, c4 = threadIdx.x / TA_JOIN_ROWS;
   tree_line(a, join_first);
   const TreeSeq s = tree_seq(a, b);
   const long long total = join_first[a.d.B];
   const int rows = s.n * a.group;
-  pdl_wait();
   if (row0 >= rows) return;
-  const int blk = row0 / a.rows, r = row0 % a.rows + lane;      // (a block is whole 32s, or 16 rows and all there is)
+  const int blk = row0 / a.rows, r = row0 - blk * a.rows + in;      // (blocks are multiples of 16 rows)
   const long long at = join_first[b] + ((long long)kvh * s.blocks + blk) * s.tiles;
   const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
   if (c0 == c1) return;                                  // written whole
-  const bool there = row0 + lane < rows && r < a.rows;
-  // the first piece begins with the item (slot 2 c + 1), the others begin inside it
-  auto slot = [&](int c) { return 2LL * c + (c == c0 ? 1 : 0); };
-  float top = -INFINITY;
-#pragma unroll 8
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, there ? a.part_ml[slot(c) * a.rows + r].x : -INFINITY);
-  float4 x[COLS];
-#pragma unroll
-  for (int i = 0; i < COLS; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  const bool there = row0 + in < rows;
+  pdl_wait();
+  float top = -INFINITY, sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int base = c0; base <= c1; base += TA_JOIN_DEEP) {
-    float4 y[TA_JOIN_DEEP][COLS];
+    float4 y[TA_JOIN_DEEP];
     float2 p[TA_JOIN_DEEP];
 #pragma unroll
     for (int k = 0; k < TA_JOIN_DEEP; ++k) {
       const bool on = there && base + k <= c1;
-      p[k] = on ? a.part_ml[slot(base + k) * a.rows + r] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int i = 0; i < COLS; ++i)
-        y[k][i] = on ? *reinterpret_cast<const float4*>(a.part_o + ((slot(base + k) * (D / 4) + i * TA_JOIN_WARPS + warp) * a.rows + r) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const long long slot = 2LL * (base + k) + (base + k == c0 ? 1 : 0);      // the first piece begins with the item, the others begin inside it
+      p[k] = on ? a.part_ml[slot * a.rows + r] : make_float2(-INFINITY, 0.f);
+      y[k] = on ? *reinterpret_cast<const float4*>(a.part_o + ((slot * (D / 4) + c4) * a.rows + r) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    float m = top;
+#pragma unroll
+    for (int k = 0; k < TA_JOIN_DEEP; ++k) m = fmaxf(m, p[k].x);
+    const float old = top == -INFINITY ? 1.f : ta_ex2(top - m);      // sums and values of pieces that saw nothing are zeros, or NaN
+    top = m;
+    sum *= old;
+    x.x *= old; x.y *= old; x.z *= old; x.w *= old;
 #pragma unroll
     for (int k = 0; k < TA_JOIN_DEEP; ++k) {
-      const float f = p[k].x == -INFINITY ? 1.f : ta_ex2(p[k].x - top);      // of a piece that saw nothing: its values are zeros, or NaN
+      const float f = p[k].x == -INFINITY ? 1.f : ta_ex2(p[k].x - m);
       sum += p[k].y * f;
-#pragma unroll
-      for (int i = 0; i < COLS; ++i) {
-        x[i].x += y[k][i].x * f; x[i].y += y[k][i].y * f; x[i].z += y[k][i].z * f; x[i].w += y[k][i].w * f;
-      }
+      x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int i = 0; i < COLS; ++i)
-    *reinterpret_cast<uint2*>(&done[lane][(i * TA_JOIN_WARPS + warp) * 4]) = make_uint2(pack_bf16x2(x[i].x * inv, x[i].y * inv), pack_bf16x2(x[i].z * inv, x[i].w * inv));
+  *reinterpret_cast<uint2*>(&done[in][c4 * 4]) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
   __syncthreads();
-  const int n = min(min(32, rows - row0), a.rows);
-  for (int c = threadIdx.x; c < n * (D / 8); c += 32 * TA_JOIN_WARPS) {
-    const int row = row0 + c / (D / 8), col = (c % (D / 8)) * 8;
-    bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + (row / a.group) * a.d.o_node + (kvh * a.group + row % a.group) * a.d.o_head;
-    *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(&done[c / (D / 8)][col]);
+  if (threadIdx.x < TA_JOIN_ROWS * (D / 8)) {
+    const int row = row0 + threadIdx.x / (D / 8), col = (threadIdx.x % (D / 8)) * 8;
+    if (row < rows) {
+      bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + (row / a.group) * a.d.o_node + (kvh * a.group + row % a.group) * a.d.o_head;
+      *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(&done[threadIdx.x / (D / 8)][col]);
+    }
   }
 }
 
@@ -439,8 +434,8 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   if (tc) { if (const int rc = launch_tree_tc(a, stream)) return rc; }                                                                          \
   else if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
   LP_CHECK_CUDA(cudaGetLastError());                                                                                                           \
-  LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + 31) / 32), d->KVH, d->B), \
-                          dim3(32 * TA_JOIN_WARPS), (size_t)(d->B + 1) * 8, stream, 1, true, a));
+  LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + TA_JOIN_ROWS - 1) / TA_JOIN_ROWS), d->KVH, d->B), \
+                          dim3(TA_JOIN_ROWS * DD / 4), (size_t)(d->B + 1) * 8, stream, 1, true, a));
   if (d->D == 128) { LP_TREE_D(128) } else if (d->D == 96) { LP_TREE_D(96) } else { LP_TREE_D(64) }
 #undef LP_TREE_D
 #undef LP_TREE

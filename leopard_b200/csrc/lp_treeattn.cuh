@@ -37,7 +37,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   s.n = a.d.nodes ? min(max(a.d.nodes[b], 0), a.d.T) : a.d.T;
   s.len = max(a.d.lengths[b], 0);
   s.keys = min((long long)s.len + s.n, (long long)a.d.max_pages * a.d.page_size);
-  s.tiles = s.n ? (int)((s.keys + a.keys - 1) / a.keys) : 0;
+  s.tiles = s.n ? (int)((unsigned)(s.keys + a.keys - 1) / (unsigned)a.keys) : 0;
   s.blocks = (s.n * a.group + a.rows - 1) / a.rows;
   return s;
 }
@@ -65,10 +65,15 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, long long* first) {
   }
   __syncthreads();
 }
-__device__ __forceinline__ long long tree_cut(long long total, int cta, int ctas) { return total / ctas * cta + min((long long)cta, total % ctas); }
+// a / b of numbers that seldom need 64 bits (whose division takes 0.3 us)
+__device__ __forceinline__ long long tree_div(long long a, long long b) { return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b; }
+__device__ __forceinline__ long long tree_cut(long long total, int cta, int ctas) {
+  const long long each = tree_div(total, ctas);
+  return each * cta + min((long long)cta, total - each * ctas);
+}
 __device__ __forceinline__ int tree_cta_of(long long total, long long unit, int ctas) {
-  const long long each = total / ctas, more = total % ctas;      // the first `more` CTAs have one tile more
-  return unit < (each + 1) * more ? (int)(unit / (each + 1)) : (int)(more + (unit - (each + 1) * more) / each);
+  const long long each = tree_div(total, ctas), more = total - each * ctas;      // the first `more` CTAs have one tile more
+  return unit < (each + 1) * more ? (int)tree_div(unit, each + 1) : (int)(more + tree_div(unit - (each + 1) * more, each));
 }
 __device__ __forceinline__ int tree_find(const long long* first, int B, long long unit) {      // the sequence that `unit` belongs to
   int lo = 0, hi = B - 1;

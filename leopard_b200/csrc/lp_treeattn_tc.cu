@@ -1,12 +1,14 @@
 // leopard_b200 — attention of a tree of drafted tokens over a cache, for many rows: tcgen05 products, keys and values by TMA from the cache's pages.
 //
-// One persistent CTA an SM takes its piece of the line of tiles (lp_treeattn.cuh), tile after tile of 128 keys.  Up to 256 rows (node x query head of a key head) are two
-// 128-row streams on the same keys, each with its own MMA issuer and softmax warps, as in the prefill's kernel (lp_attn3.cu): S of a tile comes in two halves of 64
-// keys with their own TMEM columns, so that the product for the next half runs while the softmax is at this one.
-//   warp 0       TMA producer: K_j, V_j into rings of two, a box a page or part of one; pages that are not there come as zeros
+// One persistent CTA an SM takes its piece of the line of tiles (lp_treeattn.cuh), tile after tile of 128 keys.  Two 128-row streams, each with its own MMA issuer and softmax
+// warps as in the prefill's kernel (lp_attn3.cu): S of a tile comes in two halves of 64 keys with their own TMEM columns, so that the product for the next half runs
+// while the softmax is at this one.  Of up to 256 rows (node x query head of a key head) each stream has a half, on the same keys; up to 128 rows (SPLIT) are
+// the rows of both streams, which take the tiles in turn and join their sums at the end of a piece: alone, a stream is bound by the latency of its chain
+// S -> softmax -> P V (1.8 us a tile, where reading 64 KB at an SM's share of HBM takes 1.5).
+//   warp 0       TMA producer: K_j, V_j into rings of two (SPLIT: three), a box a page or part of one; pages that are not there come as zeros
 //   warp 1 / 2   MMA issuer of stream 0 / 1:  S(j).h = Q K_j[h]^T,  O += P(j).h V_j[h] (P in TMEM)
 //   warp 3       TMEM
-//   warps 4-7, 8-11   softmax of stream 0 / 1: a thread a row; they also bring the row's queries (rows of a product are G heads of each node) and take O out
+//   warps 4-7, 8-11   softmax of stream 0 / 1: a thread a row; they also bring the rows' queries (rows of a product are G heads of each node) and take O out
 // TMEM: S0 [0, 128) S1 [128, 256) O0 [256, 384) O1 [384, 512).
 // Only the last tiles of an item, which hold nodes or reach past them, look at masks; there V is searched before its product: rows behind the keys become zeros (a
 // cache's unwritten memory may hold anything), and values that are not finite are taken out and reach the rows that see them when O is taken out.
@@ -17,6 +19,7 @@ namespace lp {
 constexpr int TT_BOX = 128 * 128;      // 128 rows x 64 bf16
 constexpr int TT_THREADS = 384;
 constexpr int TT_KEYS = 128;
+constexpr int TT_SPLIT_BATCH = 64;     // sequences whose line of tiles leaves room for three stages
 
 #define LP_TT_TMEM_ST_16(regs, taddr)                                                                               \
   asm volatile(                                                                                                     \
@@ -44,6 +47,7 @@ __device__ __forceinline__ uint64_t tt_add2(uint64_t a, uint64_t b) {
   return d;
 }
 __device__ __forceinline__ void tt_bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void tt_bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 struct TreeTc {
   TreeArgs a;
@@ -60,8 +64,8 @@ __device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const long lo
   p.b = tree_find(first, a.d.B, u);
   p.s = tree_seq(a, p.b);
   const long long local = u - first[p.b];
-  const int item = (int)(local / p.s.tiles);
-  p.t0 = (int)(local % p.s.tiles);
+  const int item = (int)tree_div(local, p.s.tiles);
+  p.t0 = (int)(local - (long long)item * p.s.tiles);
   p.n = (int)min((long long)(p.s.tiles - p.t0), u_end - u);
   p.kvh = item / p.s.blocks;
   p.r0 = (item % p.s.blocks) * a.rows;
@@ -81,45 +85,45 @@ struct TreePlace {
   }
 };
 
-template <int DH>
+template <int DH, bool SPLIT>
 __global__ void __launch_bounds__(TT_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeTc tc) {
-  constexpr int NB = (DH + 63) / 64, KS_QK = DH / 16, HEAD_BYTES = NB * TT_BOX;
-  constexpr int Q_OFF = 0, K_OFF = Q_OFF + 2 * HEAD_BYTES, V_OFF = K_OFF + 2 * HEAD_BYTES, BAR_OFF = V_OFF + 2 * HEAD_BYTES;
-  constexpr int CH = DH / 8, MAX_WORDS = LP_TREE_MAX_NODES / 64;
+  constexpr int NB = (DH + 63) / 64, KS_QK = DH / 16, HEAD_BYTES = NB * TT_BOX, STAGES = SPLIT ? 3 : 2;
+  constexpr int Q_OFF = 0, K_OFF = Q_OFF + (SPLIT ? 1 : 2) * HEAD_BYTES, V_OFF = K_OFF + STAGES * HEAD_BYTES, BAR_OFF = V_OFF + STAGES * HEAD_BYTES;
+  constexpr int CH = DH / 8, MAX_WORDS = SPLIT ? 2 : LP_TREE_MAX_NODES / 64;
   constexpr uint32_t TM_S = 0, TM_O = 256;
   const TreeArgs& a = tc.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream, a phase a piece
-  uint64_t* k_full = q_full + 2;                                       // [2] by stage
-  uint64_t* v_full = k_full + 2;                                       // [2]
-  uint64_t* k_empty = v_full + 2;                                      // [2] both streams' issuers
-  uint64_t* v_empty = k_empty + 2;                                     // [2]
-  uint64_t* s_full = v_empty + 2;                                      // [4] stream x half
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream (SPLIT: one), a phase a piece
+  uint64_t* k_full = q_full + 2;                                       // [3] by stage
+  uint64_t* v_full = k_full + 3;                                       // [3]
+  uint64_t* k_empty = v_full + 3;                                      // [3] both streams' issuers, or that of the tile's stream
+  uint64_t* v_empty = k_empty + 3;                                     // [3]
+  uint64_t* s_full = v_empty + 3;                                      // [4] stream x half
   uint64_t* p_full = s_full + 4;                                       // [4]
   uint64_t* pv_done = p_full + 4;                                      // [4]
   uint64_t* o_done = pv_done + 4;                                      // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(o_done + 2);
   int* odd = reinterpret_cast<int*>(tmem_at + 1);                      // [4] piece whose V had values that are not finite, by its number mod 4
-  unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + 256);      // [256][MAX_WORDS] of this thread's row
-  long long* first = reinterpret_cast<long long*>(mask_words + 256 * MAX_WORDS);
+  float2* other = reinterpret_cast<float2*>(smem + BAR_OFF + 256);     // [128] SPLIT: maximum and sum of stream 1's rows
+  unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + 256);      // [256][MAX_WORDS] else: of this thread's row
+  long long* first = reinterpret_cast<long long*>(smem + BAR_OFF + 256 + (SPLIT ? 128 * 8 : 256 * MAX_WORDS * 8));
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  tree_line(a, first);
-  const long long total = first[a.d.B];
-  const long long u_begin = tree_cut(total, blockIdx.x, a.ctas), u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
-  if (warp == 0 && lane == 0) {
+  if (warp == 1 && lane == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&k_empty[i], 2);
-      mbar_init(&v_empty[i], 2);
-      mbar_init(&o_done[i], 1);
+      mbar_init(&k_empty[i], SPLIT ? 1 : 2);
+      mbar_init(&v_empty[i], SPLIT ? 1 : 2);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -134,8 +138,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  tree_line(a, first);                 // (ends in the block's barrier)
   tc_fence_after();
+  const long long total = first[a.d.B];
+  const long long u_begin = tree_cut(total, blockIdx.x, a.ctas), u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
   const uint32_t tmem_base = *tmem_at;
 
   if (warp == 0) {
@@ -151,17 +157,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       auto page_of = [&]() { return lane < boxes && key < n_keys ? at.page(a, p.b) : -1; };
       int page = page_of();
       for (int j = 0; j < p.n; ++j, ++g) {
-        const int st = g & 1, row = at.row;
+        const int st = g % STAGES, row = at.row;
         int next = -1;
         if (j + 1 < p.n) {
           key += TT_KEYS;
           if (lane < boxes) at.forward(a, TT_KEYS);
           next = page_of();
         }
-        const uint32_t ph = (g >> 1) & 1;
+        const uint32_t ph = (g / STAGES) & 1;
         for (int kv = 0; kv < 2; ++kv) {
           uint64_t* full = kv ? &v_full[st] : &k_full[st];
-          if (g >= 2) mbar_wait_warp(kv ? &v_empty[st] : &k_empty[st], ph ^ 1);
+          if (g >= STAGES) mbar_wait_warp(kv ? &v_empty[st] : &k_empty[st], ph ^ 1);
           if (lane == 0) mbar_arrive_expect_tx(full, HEAD_BYTES);
           uint8_t* to = smem + (kv ? V_OFF : K_OFF) + st * HEAD_BYTES;
           for (int i = 0; i < boxes; ++i) {
@@ -180,22 +186,30 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     const int q = warp - 1;
     const bool issue = elect_one();
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0, 0), idesc_o = umma_idesc_bf16(128, DH, 0, 1);
-    const uint32_t q_addr = smem_u32(smem + Q_OFF + q * HEAD_BYTES), s_tm = tmem_base + TM_S + (uint32_t)q * 128, d_o = tmem_base + TM_O + (uint32_t)q * 128;
-    int g = 0, nt = 0, pieces = 0;      // tiles so far; tiles and pieces of this stream
+    const uint32_t q_addr = smem_u32(smem + Q_OFF + (SPLIT ? 0 : q) * HEAD_BYTES), s_tm = tmem_base + TM_S + (uint32_t)q * 128, d_o = tmem_base + TM_O + (uint32_t)q * 128;
+    constexpr int STEP = SPLIT ? 2 : 1;
+    int g = 0, nt = 0, pieces = 0;      // tiles of the CTA so far; tiles of this stream; pieces whose queries it has waited for
     for (long long u = u_begin; u < u_end;) {
       const TreePiece p = tree_piece(a, first, u, u_end);
       u += p.n;
-      if (p.r0 + q * 128 >= p.s.n * a.group) {      // no rows here: the stages are passed on
+      const int j0 = SPLIT ? q : 0;
+      if (SPLIT && j0 >= p.n) {         // one tile: the other stream's (whose phases of the queries are counted all the same)
+        mbar_wait_warp(&q_full[0], pieces & 1);
+        g += p.n;
+        ++pieces;
+        continue;
+      }
+      if (!SPLIT && p.r0 + q * 128 >= p.s.n * a.group) {      // no rows here: the stages are passed on
         for (int j = 0; j < p.n; ++j, ++g) {
-          mbar_wait_warp(&k_full[g & 1], (g >> 1) & 1);
-          if (issue) mbar_arrive(&k_empty[g & 1]);
-          mbar_wait_warp(&v_full[g & 1], (g >> 1) & 1);
-          if (issue) mbar_arrive(&v_empty[g & 1]);
+          mbar_wait_warp(&k_full[g % STAGES], (g / STAGES) & 1);
+          if (issue) mbar_arrive(&k_empty[g % STAGES]);
+          mbar_wait_warp(&v_full[g % STAGES], (g / STAGES) & 1);
+          if (issue) mbar_arrive(&v_empty[g % STAGES]);
         }
         continue;
       }
       auto issue_S = [&](int gt, int h) {
-        const uint32_t k_addr = smem_u32(smem + K_OFF + (gt & 1) * HEAD_BYTES) + (uint32_t)h * 64 * 128;
+        const uint32_t k_addr = smem_u32(smem + K_OFF + (gt % STAGES) * HEAD_BYTES) + (uint32_t)h * 64 * 128;
         if (issue) {
 #pragma unroll
           for (int ks = 0; ks < KS_QK; ++ks) {
@@ -205,135 +219,157 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           umma_commit(&s_full[q * 2 + h]);
         }
       };
-      auto issue_PV = [&](int gt, int j, int h) {
-        const uint32_t v_addr = smem_u32(smem + V_OFF + (gt & 1) * HEAD_BYTES);
-        mbar_wait_warp(&p_full[q * 2 + h], (nt + j) & 1);
+      auto issue_PV = [&](int gt, bool start, int h) {
+        const uint32_t v_addr = smem_u32(smem + V_OFF + (gt % STAGES) * HEAD_BYTES);
+        mbar_wait_warp(&p_full[q * 2 + h], nt & 1);
         tc_fence_after();
         if (issue) {
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) {
             const int ks = h * 4 + k4;
-            umma_ts(d_o, s_tm + (uint32_t)h * 64 + k4 * 8, umma_desc_sw128(v_addr + ks * 2048, TT_BOX, 1024), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+            umma_ts(d_o, s_tm + (uint32_t)h * 64 + k4 * 8, umma_desc_sw128(v_addr + ks * 2048, TT_BOX, 1024), idesc_o, (!start || ks > 0) ? 1u : 0u);
           }
           umma_commit(&pv_done[q * 2 + h]);
         }
       };
-      mbar_wait_warp(&q_full[q], pieces & 1);
-      mbar_wait_warp(&k_full[g & 1], (g >> 1) & 1);
+      mbar_wait_warp(&q_full[SPLIT ? 0 : q], pieces & 1);
+      ++pieces;
+      int gt = g + j0;
+      mbar_wait_warp(&k_full[gt % STAGES], (gt / STAGES) & 1);
       tc_fence_after();
-      issue_S(g, 0);
-      issue_S(g, 1);
-      if (issue) umma_commit(&k_empty[g & 1]);
-      for (int j = 0; j < p.n; ++j) {
-        const int gt = g + j;
-        const bool more = j + 1 < p.n;
-        mbar_wait_warp(&v_full[gt & 1], (gt >> 1) & 1);
-        issue_PV(gt, j, 0);
+      issue_S(gt, 0);
+      issue_S(gt, 1);
+      if (issue) umma_commit(&k_empty[gt % STAGES]);
+      for (int j = j0; j < p.n; j += STEP, gt += STEP, ++nt) {
+        const bool more = j + STEP < p.n;
+        const int gn = gt + STEP;
+        mbar_wait_warp(&v_full[gt % STAGES], (gt / STAGES) & 1);
+        issue_PV(gt, j == j0, 0);
         if (more) {
-          mbar_wait_warp(&k_full[(gt + 1) & 1], ((gt + 1) >> 1) & 1);
+          mbar_wait_warp(&k_full[gn % STAGES], (gn / STAGES) & 1);
           tc_fence_after();
-          issue_S(gt + 1, 0);
+          issue_S(gn, 0);
         }
-        issue_PV(gt, j, 1);
-        if (issue) umma_commit(&v_empty[gt & 1]);
+        issue_PV(gt, j == j0, 1);
+        if (issue) umma_commit(&v_empty[gt % STAGES]);
         if (more) {
-          issue_S(gt + 1, 1);
-          if (issue) umma_commit(&k_empty[(gt + 1) & 1]);
+          issue_S(gn, 1);
+          if (issue) umma_commit(&k_empty[gn % STAGES]);
         } else if (issue) {
           umma_commit(&o_done[q]);
         }
       }
       g += p.n;
-      nt += p.n;
-      ++pieces;
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax: thread = row
     const int q = (warp - 4) >> 2, lg = warp & 3, r = lg * 32 + lane;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(lg * 32) << 16);
     const uint32_t s_addr = lane_addr + TM_S + (uint32_t)q * 128, o_addr = lane_addr + TM_O + (uint32_t)q * 128;
-    int g = 0, nt = 0, pieces = 0, seg = 0;
+    constexpr int STEP = SPLIT ? 2 : 1;
+    int g = 0, nt = 0, pieces = 0, joins = 0, seg = 0;      // tiles of the CTA and of this stream so far; pieces that it had tiles of; SPLIT: pieces of both streams
     for (long long u = u_begin; u < u_end; ++seg) {
       const TreePiece p = tree_piece(a, first, u, u_end);
       u += p.n;
-      const int rows = p.s.n * a.group;
-      if (p.r0 + q * 128 >= rows) { g += p.n; continue; }
-      const bool both = p.r0 + 128 < rows && a.rows > 128;             // the other stream is at the same tiles
-      const int row = p.r0 + q * 128 + r;
+      const int rows = p.s.n * a.group, row_base = p.r0 + (SPLIT ? 0 : q * 128), j0 = SPLIT ? q : 0;
+      if (SPLIT ? j0 >= p.n : row_base >= rows) { g += p.n; continue; }
+      const bool both = !SPLIT && p.r0 + 128 < rows;                   // the other stream is at the same tiles
+      const int row = row_base + r;
       const bool row_ok = row < rows;
-      const int node = row_ok ? row / a.group : 0, head = p.kvh * a.group + (row_ok ? row % a.group : 0);
+      const int node = row_ok ? row / a.group : 0, head = p.kvh * a.group + (row_ok ? row - node * a.group : 0);
       // the warp's rows' queries, in the swizzled layout that TMA writes; 32 lanes take neighbouring pieces of 16 bytes
-      {
+      if (!SPLIT || q == 0) {
         const long long from = p.b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head;
-        uint8_t* at = smem + Q_OFF + q * HEAD_BYTES + lg * 32 * 128;
+        uint8_t* at = smem + Q_OFF + (SPLIT ? 0 : q) * HEAD_BYTES + lg * 32 * 128;
+        uint4 x[CH];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
           const long long src = __shfl_sync(0xffffffffu, from, rr);
-          const uint4 x = p.r0 + q * 128 + lg * 32 + rr < rows ? *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + src + c * 8) : make_uint4(0, 0, 0, 0);
-          sts_u4(at + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), x);
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (row_base + lg * 32 + rr < rows) x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + src + c * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
+          sts_u4(at + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), x[i]);
         }
         if (DH % 64 != 0)
           for (int c = CH; c < NB * 8; ++c) sts_u4(at + (c >> 3) * TT_BOX + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), make_uint4(0, 0, 0, 0));
         fence_proxy_async_smem();
-        mbar_arrive(&q_full[q]);
+        mbar_arrive(&q_full[SPLIT ? 0 : q]);
       }
       // its node's mask, when this piece gets there
       const int nw = (a.d.T + 63) >> 6;
-      unsigned long long* words = mask_words + (q * 128 + r) * MAX_WORDS;
+      unsigned long long word[2] = {0, 0};                             // SPLIT: two at most
+      unsigned long long* words = SPLIT ? word : mask_words + (q * 128 + r) * MAX_WORDS;
       if ((p.t0 + p.n) * TT_KEYS > p.s.len) {
         const unsigned long long* src = a.d.mask + p.b * a.d.mask_batch + node * a.d.mask_node;
-        for (int w = 0; w < nw; ++w) words[w] = src[w];
+#pragma unroll
+        for (int w = 0; w < MAX_WORDS; ++w)
+          if (w < nw) words[w] = src[w];
       }
+      auto word_at = [&](int w) -> unsigned long long { return w >= nw ? 0ull : SPLIT ? (w == 0 ? word[0] : word[1]) : words[w]; };
       // which of a half's 64 keys there are, by their pages (known a step ahead)
       const int box = min(tc.box, 64), n_box = 64 / box;
       const bool paged = a.d.page_table != nullptr;
       const int n_keys = (int)p.s.keys, len = p.s.len;
-      int box_key = p.t0 * TT_KEYS + lane * box;
+      int box_key = (p.t0 + j0) * TT_KEYS + lane * box;
       TreePlace box_at(a, paged && lane < n_box ? box_key : 0);
       auto page_there = [&]() { return !paged || lane >= n_box || box_key >= n_keys || box_at.page(a, p.b) >= 0; };
       bool there_next = page_there();
+      if (SPLIT && q == 1 && joins > 0) tt_bar_sync(3, 256);           // stream 0 has taken out what this one had of its last piece
       float m_used = -INFINITY, l_sum = 0.f;
       uint32_t v[64];
       mbar_wait(&s_full[q * 2], nt & 1);
       tc_fence_after();
       LP_TMEM_LD_32((v + 0), s_addr + 0);
       LP_TMEM_LD_32((v + 32), s_addr + 32);
+      const int mine = (p.n - j0 + STEP - 1) / STEP;                   // tiles of this stream
 #pragma unroll 1
-      for (int t = 0; t < 2 * p.n; ++t) {
-        const int j = t >> 1, h = t & 1;
+      for (int t = 0; t < 2 * mine; ++t) {
+        const int j = j0 + (t >> 1) * STEP, h = t & 1;
         const int key0 = (p.t0 + j) * TT_KEYS + h * 64;
         const bool tail = key0 - h * 64 + TT_KEYS > len;
         const unsigned pages = paged ? __ballot_sync(0xffffffffu, there_next) : 0xffffffffu;
-        if (paged && t + 1 < 2 * p.n) {
-          box_key += 64;
-          if (lane < n_box) box_at.forward(a, 64);
+        if (paged && t + 1 < 2 * mine) {
+          const int on = h == 0 || STEP == 1 ? 64 : 64 + TT_KEYS;
+          box_key += on;
+          if (lane < n_box) box_at.forward(a, on);
           there_next = page_there();
         }
         if (tail && h == 0) {
           // V of this tile before its product: rows that are not keys, values that are not finite
-          mbar_wait(&v_full[(g + j) & 1], ((g + j) >> 1) & 1);
+          mbar_wait(&v_full[(g + j) % STAGES], ((g + j) / STAGES) & 1);
           const bool key_ok = key0 + r < n_keys;
-          uint8_t* at = smem + V_OFF + ((g + j) & 1) * HEAD_BYTES + r * 128;
+          uint8_t* at = smem + V_OFF + ((g + j) % STAGES) * HEAD_BYTES + r * 128;
 #pragma unroll 1
           for (int c = 0; c < NB; ++c) {
             if (both && NB == 2 && c != q) continue;                   // each stream searches its half of the columns
             if (both && NB == 1 && q == 1) continue;
-#pragma unroll 1
+            at += c * TT_BOX;
+            if (!key_ok) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) sts_u4(at + (i << 4), make_uint4(0, 0, 0, 0));
+              continue;
+            }
+            uint4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = lds_u4(at + ((i ^ (r & 7)) << 4));
+            uint32_t any = 0;                                          // a carry into bit 15 (31): an exponent of all ones
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
-              uint8_t* x_at = at + c * TT_BOX + ((i ^ (r & 7)) << 4);
-              if (!key_ok) { sts_u4(x_at, make_uint4(0, 0, 0, 0)); continue; }
-              uint4 x = lds_u4(x_at);
-              bool bad = false;
-              auto clean = [&](uint32_t& w) {
-                if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; bad = true; }
-                if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; bad = true; }
-              };
-              clean(x.x); clean(x.y); clean(x.z); clean(x.w);
-              if (bad) {
-                sts_u4(x_at, x);
-                *reinterpret_cast<volatile int*>(&odd[seg & 3]) = seg;
+              auto look = [&](uint32_t w) { any |= ((w & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; };
+              look(x[i].x); look(x[i].y); look(x[i].z); look(x[i].w);
+            }
+            if (any) {
+#pragma unroll 1
+              for (int i = 0; i < 32; ++i) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(at) + i;
+                const uint32_t b = ((*w & 0x7fff7fffu) + 0x00800080u) & 0x80008000u;
+                if (b) *w &= (b & 0x8000u ? 0u : 0xffffu) | (b & 0x80000000u ? 0u : 0xffff0000u);
               }
+              *reinterpret_cast<volatile int*>(&odd[seg & 3]) = seg;
             }
           }
           fence_proxy_async_smem();
@@ -347,13 +383,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (key0 + 64 > len) {
           const int behind = n_keys - key0;                            // keys of this half
           if (behind < 64) sees &= behind <= 0 ? 0ull : (1ull << behind) - 1;
-          const int j0 = key0 - len;                                   // the node of the half's first key
+          const int first_node = key0 - len;
           unsigned long long bits;
-          if (j0 < 0) bits = (words[0] << -j0) | ((1ull << -j0) - 1);
+          if (first_node < 0) bits = (word_at(0) << -first_node) | ((1ull << -first_node) - 1);
           else {
-            const int w = min(j0 >> 6, nw), sh = j0 & 63;
-            bits = w < nw ? words[w] >> sh : 0ull;
-            if (sh && w + 1 < nw) bits |= words[w + 1] << (64 - sh);
+            const int w = first_node >> 6, sh = first_node & 63;
+            bits = word_at(w) >> sh;
+            if (sh) bits |= word_at(w + 1) << (64 - sh);
           }
           sees &= bits;
         }
@@ -406,9 +442,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
         const uint64_t nm2 = tt_pk2(neg_m, neg_m);
         uint64_t acc2 = tt_pk2(0.f, 0.f);
-        const int jn = (t + 1) >> 1, hn = (t + 1) & 1;
-        const bool has_next = t + 1 < 2 * p.n;
-        const bool s_ready = has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + jn) & 1);
+        const int tn = (t + 1) >> 1, hn = (t + 1) & 1;
+        const bool has_next = t + 1 < 2 * mine;
+        const bool s_ready = has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
@@ -423,7 +459,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           LP_TT_TMEM_ST_16(pk, s_addr + h * 64 + c * 16);
         }
         bool loaded = false;
-        if (s_ready || (has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + jn) & 1))) {
+        if (s_ready || (has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1))) {
           tc_fence_after();
           LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
           LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
@@ -438,54 +474,85 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           l_sum += a0 + a1;
         }
         if (has_next && !loaded) {
-          mbar_wait(&s_full[q * 2 + hn], (nt + jn) & 1);
+          mbar_wait(&s_full[q * 2 + hn], (nt + tn) & 1);
           tc_fence_after();
           LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
           LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
         }
       }
+      g += p.n;
+      nt += mine;
       // ---- O of this piece
+      const bool two = SPLIT && p.n > 1;                               // both streams had tiles
+      if (SPLIT && q == 1) {                                           // stream 0 takes it out
+        other[r] = make_float2(m_used, l_sum);
+        tt_bar_arrive(2, 256);
+        ++pieces;
+        ++joins;
+        continue;
+      }
       mbar_wait(&o_done[q], pieces & 1);
+      ++pieces;
+      float f0 = 1.f, f1 = 0.f;
+      if (two) {
+        tt_bar_sync(2, 256);
+        mbar_wait(&o_done[1], joins & 1);
+        ++joins;
+        const float2 x = other[r];
+        const float m = fmaxf(m_used, x.x);
+        f0 = m_used == -INFINITY ? 1.f : ta_ex2(m_used - m);           // sums and values of a stream that saw nothing are zeros, or NaN
+        f1 = x.x == -INFINITY ? 1.f : ta_ex2(x.x - m);
+        l_sum = l_sum * f0 + x.y * f1;
+        m_used = m;
+      }
       tc_fence_after();
       const bool whole = p.t0 == 0 && p.n == p.s.tiles;
       const bool fix = *reinterpret_cast<volatile int*>(&odd[seg & 3]) == seg;
       const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;
       const long long slot = 2LL * blockIdx.x + (p.t0 == 0 ? 1 : 0);
-      const int in_block = q * 128 + r;
+      const int in_block = (SPLIT ? 0 : q * 128) + r;
       float* part = a.part_o + (slot * (DH / 4) * a.rows + in_block) * 4;
-      uint8_t* stage = smem + Q_OFF + q * HEAD_BYTES + lg * 32 * 128;      // the queries are done with
+      uint8_t* stage = smem + Q_OFF + (SPLIT ? 0 : q) * HEAD_BYTES + lg * 32 * 128;      // the queries are done with
       if (!whole && row_ok) a.part_ml[slot * a.rows + in_block] = make_float2(m_used, l_sum);
 #pragma unroll 1
-      for (int c = 0; c < DH / 16; ++c) {
-        uint32_t o[16];
-        LP_TMEM_LD_16(o, o_addr + c * 16);
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t o[32], y[32];
+        LP_TMEM_LD_32(o, o_addr + c * 32);
+        if (two) LP_TMEM_LD_32(y, o_addr + 128 + c * 32);
         tmem_wait_ld();
+        if (two)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(y[i]) * f1);
         if (fix) {
           const int k1 = min(n_keys, (p.t0 + p.n) * TT_KEYS);
           for (int key = max(p.t0, len / TT_KEYS) * TT_KEYS; key < k1; ++key) {
             const TreePlace at(a, key);
             const int page = at.page(a, p.b), nd = max(0, key - len);
-            if (page < 0 || (key >= len && !((words[nd >> 6] >> (nd & 63)) & 1))) continue;
-            const bf16* vr = reinterpret_cast<const bf16*>(a.d.v) + page * a.d.v_page + at.row * a.d.v_row + p.kvh * a.d.v_head + c * 16;
+            if (page < 0 || (key >= len && !((word_at(nd >> 6) >> (nd & 63)) & 1))) continue;
+            const bf16* vr = reinterpret_cast<const bf16*>(a.d.v) + page * a.d.v_page + at.row * a.d.v_row + p.kvh * a.d.v_head + c * 32;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 32; ++i) {
               const float x = __bfloat162float(vr[i]);
               if (not_finite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
             }
           }
         }
         if (whole) {
-          uint32_t w[8];
+          uint8_t* at = stage + (c >> 1) * TT_BOX + lane * 128;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
-          uint8_t* at = stage + (c >> 2) * TT_BOX + lane * 128;
-          sts_u4(at + ((((2 * c) & 7) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
-          sts_u4(at + ((((2 * c + 1) & 7) ^ (lane & 7)) << 4), make_uint4(w[4], w[5], w[6], w[7]));
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(o[k * 8 + 2 * i]) * inv_l, __uint_as_float(o[k * 8 + 2 * i + 1]) * inv_l);
+            sts_u4(at + ((((c & 1) * 4 + k) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+          }
         } else if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(part + (c * 4 + i) * a.rows * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(part + (c * 8 + i) * a.rows * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
+      tc_fence_before();
+      if (two) tt_bar_arrive(3, 256);
       if (whole) {
         __syncwarp();
         const long long to = p.b * a.d.o_batch + node * a.d.o_node + head * a.d.o_head;
@@ -494,15 +561,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
           const long long dst = __shfl_sync(0xffffffffu, to, rr);
           const uint4 x = lds_u4(stage + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
-          if (p.r0 + q * 128 + lg * 32 + rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.d.out) + dst + c * 8) = x;
+          if (row_base + lg * 32 + rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.d.out) + dst + c * 8) = x;
         }
         __syncwarp();
       }
-      tc_fence_before();
-      g += p.n;
-      nt += p.n;
-      ++pieces;
     }
+    if (SPLIT && q == 1 && joins > 0) tt_bar_sync(3, 256);             // (what stream 0 has arrived at)
   }
   tc_fence_before();
   __syncthreads();
@@ -538,9 +602,11 @@ static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
     const uint64_t strides[3] = {d.KVH == 1 ? (uint64_t)d.D : (uint64_t)head[i], d.page_size == 1 ? (uint64_t)d.D : (uint64_t)row[i], d.n_pages == 1 ? (uint64_t)d.D : (uint64_t)page[i]};
     if (const int rc = make_tmap_bf16_4d(&tm[i], base[i], dims, strides, box)) return rc;
   }
-  const size_t smem = 6 * NB * TT_BOX + 256 + 256 * (LP_TREE_MAX_NODES / 64) * 8 + (size_t)(d.B + 1) * 8 + 1024;
-  LP_CHECK_CUDA(cudaFuncSetAttribute(tree_tc_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  tree_tc_kernel<DH><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+  const bool split = d.B <= TT_SPLIT_BATCH && tc.a.rows <= 128;
+  const size_t smem = (split ? 7 : 6) * NB * TT_BOX + 256 + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * 8 + 1024;
+  auto kernel = split ? tree_tc_kernel<DH, true> : tree_tc_kernel<DH, false>;
+  LP_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
   LP_CHECK_CUDA(cudaGetLastError());
   return 0;
 }

@@ -62,6 +62,7 @@ inline uint64_t tt_add2(uint64_t a, uint64_t b) {
   return tt_pk2(a0 + b0, a1 + b1);
 }
 inline void tt_bar_sync(int id, int n) { named_bar(id, n, true); }
+inline void tt_bar_arrive(int id, int n) { named_bar(id, n, false); }
 #define LP_TT_TMEM_ST_16(regs, taddr) lp::tmem_st(regs, taddr, 16)
 #define CUtensorMap Map4
 #include "tree_tc_kernel.inc"
@@ -70,7 +71,7 @@ inline void tt_bar_sync(int id, int n) { named_bar(id, n, true); }
 
 using namespace lp;
 
-extern "C" void emu_tree_tc(const lp_tree_attn_desc* d, int ctas, int rows, int box, float* part_o, float* part_ml) {
+extern "C" void emu_tree_tc(const lp_tree_attn_desc* d, int ctas, int rows, int box, int split, float* part_o, float* part_ml) {
   TreeTc tc;
   tc.a.d = *d;
   tc.a.group = d->H / d->KVH;
@@ -92,9 +93,15 @@ extern "C" void emu_tree_tc(const lp_tree_attn_desc* d, int ctas, int rows, int 
   }
   emu::g_block_hook = [] { emu_tc::reset(); };
   emu::launch(dim3(ctas), dim3(TT_THREADS), [&] {
-    if (d->D == 128) tree_tc_kernel<128>(tm[0], tm[1], tc);
-    else if (d->D == 96) tree_tc_kernel<96>(tm[0], tm[1], tc);
-    else tree_tc_kernel<64>(tm[0], tm[1], tc);
+    if (split) {
+      if (d->D == 128) tree_tc_kernel<128, true>(tm[0], tm[1], tc);
+      else if (d->D == 96) tree_tc_kernel<96, true>(tm[0], tm[1], tc);
+      else tree_tc_kernel<64, true>(tm[0], tm[1], tc);
+    } else {
+      if (d->D == 128) tree_tc_kernel<128, false>(tm[0], tm[1], tc);
+      else if (d->D == 96) tree_tc_kernel<96, false>(tm[0], tm[1], tc);
+      else tree_tc_kernel<64, false>(tm[0], tm[1], tc);
+    }
   });
   emu::g_block_hook = nullptr;
 }

@@ -89,7 +89,7 @@ def case(B, T, H, G, D, lengths, nodes, page, seed, shared_tree=False):
     return c
 
 
-def run(emu, c, ctas):
+def run(emu, c, ctas, split):
     B, T, H, D = c["q"].shape
     P, S, G, _ = c["k"].shape
     rows = 128 if T * (H // G) <= 128 else 256
@@ -101,7 +101,7 @@ def run(emu, c, ctas):
     d = _lib.TreeAttnDesc(ptr(c["q"]), *c["q"].stride()[:3], ptr(c["k"]), *c["k"].stride()[:3], ptr(c["v"]), *c["v"].stride()[:3], ptr(out), *out.stride()[:3],
                           ptr(c["page_table"]), 0 if c["page_table"] is None else c["page_table"].shape[1], 1 if c["page_table"] is None else c["page_table"].shape[1], P, S,
                           ptr(c["lengths"]), ptr(c["nodes"]), ptr(words), words.stride(0), words.stride(1), B, T, H, G, D, D ** -0.5)
-    emu.emu_tree_tc(C.byref(d), ctas, rows, box, C.c_void_p(part.data_ptr()), C.c_void_p(ml.data_ptr()))
+    emu.emu_tree_tc(C.byref(d), ctas, rows, box, int(split and rows <= 128), C.c_void_p(part.data_ptr()), C.c_void_p(ml.data_ptr()))
     want, weight = O.tree_attention(c["q"], c["k"], c["v"], c["lengths"], c["sees"], c["nodes"], c["page_table"])
     return joined(c, out, part, ml, ctas, rows, want), want, weight
 
@@ -116,6 +116,7 @@ def check(got, c, want, weight):
         assert bool((got[b, t:] == 7.0).all())
 
 
+@pytest.mark.parametrize("split", [True, False])
 @pytest.mark.parametrize("B, T, H, G, D, lengths, nodes, page, ctas", [
     (1, 40, 4, 4, 128, [100], None, 0, 1),                      # one stream, several items a CTA
     (1, 40, 4, 4, 128, [600], None, 64, 3),                     # items cut between CTAs
@@ -124,15 +125,16 @@ def check(got, c, want, weight):
     (1, 36, 4, 1, 96, [0], None, 32, 1),                        # nodes only, columns beyond a head
     (1, 150, 4, 2, 64, [127], None, 8, 4),                      # two blocks of rows, pages of eight
     (3, 34, 1, 1, 128, [1, 0, 255], [1, 0, 34], 0, 2),          # a sequence without nodes
+    (2, 33, 2, 2, 64, [1100, 90], None, 64, 2),                 # many tiles a piece, rings that wrap
 ])
-def test_the_kernel_is_green_under_the_emulator(emu, B, T, H, G, D, lengths, nodes, page, ctas):
+def test_the_kernel_is_green_under_the_emulator(emu, B, T, H, G, D, lengths, nodes, page, ctas, split):
     c = case(B, T, H, G, D, lengths, nodes, page, T + D)
-    got, want, weight = run(emu, c, ctas)
+    got, want, weight = run(emu, c, ctas, split)
     check(got, c, want, weight)
 
 
-@pytest.mark.parametrize("H, G", [(4, 4), (4, 1)])
-def test_masks_pages_and_values_that_are_not_finite(emu, H, G):
+@pytest.mark.parametrize("H, G, split", [(4, 4, True), (4, 4, False), (4, 1, False)])
+def test_masks_pages_and_values_that_are_not_finite(emu, H, G, split):
     c = case(1, 40, H, G, 64, [200], None, 32, 5)
     c["sees"][0, 7] = False
     c["page_table"][0, 1] = -1
@@ -147,13 +149,14 @@ def test_masks_pages_and_values_that_are_not_finite(emu, H, G):
     at = 200 + 3
     c["v"][int(c["page_table"][0, at // 32]), at % 32, 0, 5] = float("inf")
     c["v"][int(c["page_table"][0, at // 32]), at % 32, 0, 40] = float("nan")
-    got, want, weight = run(emu, c, 2)
+    got, want, weight = run(emu, c, 2, split)
     check(got, c, want, weight.nan_to_num(0, 0))
 
 
-def test_a_row_that_sees_nothing_is_zeros(emu):
+@pytest.mark.parametrize("split", [True, False])
+def test_a_row_that_sees_nothing_is_zeros(emu, split):
     c = case(1, 40, 4, 4, 64, [0], None, 0, 6)
     c["sees"][0, 5] = False
-    got, want, weight = run(emu, c, 1)
+    got, want, weight = run(emu, c, 1, split)
     check(got, c, want, weight)
     assert bool((got[0, 5] == 0).all())
