@@ -11,7 +11,7 @@ namespace lp {
 constexpr int TA_KEYS = 64;               // keys of a tile
 constexpr int TA_STAGES = 3;
 constexpr int TA_RING = TA_STAGES + 1;    // tiles whose rows' places are known
-constexpr int TA_MAX_BATCH = 4096;
+constexpr int TA_MAX_BATCH = 2048;        // the line of the sequences is in shared memory
 
 __device__ __forceinline__ void ta_ldmatrix(uint32_t* r, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)) : "memory");
@@ -38,22 +38,22 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   int2* place = reinterpret_cast<int2*>(tiles + TA_STAGES * 2 * TA_KEYS * LD);      // [ring][64]: page (-1: not there) and row in it
   uint32_t* present = reinterpret_cast<uint32_t*>(place + TA_RING * TA_KEYS);       // [ring][2]
   float2* ml = reinterpret_cast<float2*>(present + TA_RING * 2);                    // [WN][R]
-  long long* first = reinterpret_cast<long long*>(ml + WN * R);                     // [B + 1]
+  TreeLine* line = reinterpret_cast<TreeLine*>(ml + WN * R);                        // [B + 1]
   constexpr int LDO = D + 4;
   float* obuf = reinterpret_cast<float*>(ta_smem);                                  // [R][LDO], when the tiles are done with
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM, g = lane >> 2, t4 = lane & 3;
   pdl_launch_dependents();
-  tree_line(a, first);
-  const long long total = first[a.d.B];
+  tree_line(a, line);
+  const long long total = line[a.d.B].first;
   long long u = tree_cut(total, blockIdx.x, a.ctas);
   const long long u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
 
   while (u < u_end) {
-    const int b = tree_find(first, a.d.B, u);
-    const TreeSeq s = tree_seq(a, b);
-    const long long local = u - first[b];
+    const int b = tree_find(line, a.d.B, u);
+    const TreeSeq s = tree_seq(a, line[b].len, line[b].n);
+    const long long local = u - line[b].first;
     const int item = (int)tree_div(local, s.tiles), t0 = (int)(local - (long long)item * s.tiles), t1 = (int)min((long long)s.tiles, t0 + (u_end - u));
-    const int kvh = item / s.blocks, r0 = (item % s.blocks) * R;
+    const int kvh = item / s.blocks, r0 = (item - kvh * s.blocks) * R;
     u += t1 - t0;
     const int n_rows = min(R, s.n * a.group - r0);
     const bf16* kb = reinterpret_cast<const bf16*>(a.d.k) + kvh * a.d.k_head;
@@ -298,16 +298,16 @@ constexpr int TA_JOIN_ROWS = 8, TA_JOIN_DEEP = 10;
 template <int D>
 __global__ void __launch_bounds__(TA_JOIN_ROWS * D / 4)
 tree_join_kernel(const __grid_constant__ TreeArgs a) {
-  extern __shared__ long long join_first[];
+  extern __shared__ TreeLine join_line[];
   __shared__ __align__(16) bf16 done[TA_JOIN_ROWS][D + 8];
   const int b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * TA_JOIN_ROWS, in = threadIdx.x % TA_JOIN_ROWS, c4 = threadIdx.x / TA_JOIN_ROWS;
-  tree_line(a, join_first);
-  const TreeSeq s = tree_seq(a, b);
-  const long long total = join_first[a.d.B];
+  tree_line(a, join_line);
+  const TreeSeq s = tree_seq(a, join_line[b].len, join_line[b].n);
+  const long long total = join_line[a.d.B].first;
   const int rows = s.n * a.group;
   if (row0 >= rows) return;
-  const int blk = row0 / a.rows, r = row0 - blk * a.rows + in;      // (blocks are multiples of 16 rows)
-  const long long at = join_first[b] + ((long long)kvh * s.blocks + blk) * s.tiles;
+  const int blk = row0 >> a.row_bits, r = row0 - (blk << a.row_bits) + in;      // (blocks are multiples of 16 rows)
+  const long long at = join_line[b].first + ((long long)kvh * s.blocks + blk) * s.tiles;
   const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
   if (c0 == c1) return;                                  // written whole
   const bool there = row0 + in < rows;
@@ -372,7 +372,7 @@ static int tree_ctas(const lp_tree_attn_desc* d) {
   return (int)(all > most / d->B ? most : all * d->B);
 }
 static size_t tree_smem(int D, int wm, int wn, int B) {
-  return (size_t)TA_STAGES * 2 * TA_KEYS * (D + 8) * 2 + TA_RING * TA_KEYS * 8 + TA_RING * 8 + (size_t)wn * wm * 16 * 8 + (size_t)(B + 1) * 8;
+  return (size_t)TA_STAGES * 2 * TA_KEYS * (D + 8) * 2 + TA_RING * TA_KEYS * 8 + TA_RING * 8 + (size_t)wn * wm * 16 * 8 + (size_t)(B + 1) * sizeof(TreeLine);
 }
 static int tree_check(const lp_tree_attn_desc* d) {
   LP_REQUIRE(d != nullptr, "lp_tree_attention: null descriptor");
@@ -416,7 +416,8 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   LP_REQUIRE(ws_bytes >= lp_tree_attention_workspace_bytes(d), "lp_tree_attention: workspace too small");
   a.group = d->H / d->KVH;
   a.rows = tree_rows(d);
-  a.keys = tree_keys(d);
+  for (a.row_bits = 0; 1 << a.row_bits < a.rows;) ++a.row_bits;
+  a.key_bits = tree_keys(d) == 128 ? 7 : 6;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.ctas = tree_ctas(d);
   a.part_o = reinterpret_cast<float*>(workspace);
@@ -435,7 +436,7 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   else if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
   LP_CHECK_CUDA(cudaGetLastError());                                                                                                           \
   LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + TA_JOIN_ROWS - 1) / TA_JOIN_ROWS), d->KVH, d->B), \
-                          dim3(TA_JOIN_ROWS * DD / 4), (size_t)(d->B + 1) * 8, stream, 1, true, a));
+                          dim3(TA_JOIN_ROWS * DD / 4), (size_t)(d->B + 1) * sizeof(TreeLine), stream, 1, true, a));
   if (d->D == 128) { LP_TREE_D(128) } else if (d->D == 96) { LP_TREE_D(96) } else { LP_TREE_D(64) }
 #undef LP_TREE_D
 #undef LP_TREE

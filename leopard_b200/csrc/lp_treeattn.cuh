@@ -12,7 +12,7 @@ namespace lp {
 
 struct TreeArgs {
   lp_tree_attn_desc d;
-  int group, rows, keys;                  // query heads of a key head; rows of a block; keys of a tile
+  int group, rows, row_bits, key_bits;    // query heads of a key head; rows of a block and their power of two; that of a tile's keys
   float scale_log2;
   float* part_o; float2* part_ml;         // [2 x CTAs][D / 4][rows][4] (a warp writes and reads 32 rows of 4 values side by side), [2 x CTAs][rows]: maximum (log2 units), sum
   int ctas;
@@ -32,24 +32,31 @@ struct TreeSeq {
   int len, n, tiles, blocks;              // cached rows; nodes; tiles of an item; blocks of rows
   long long keys;                         // rows that are there: cached and nodes', as far as the page table reaches
 };
-__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+// what the line knows of a sequence: the tiles before it, its length and nodes
+struct __align__(16) TreeLine {
+  long long first;
+  int len, n;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int len, int n) {
   TreeSeq s;
-  s.n = a.d.nodes ? min(max(a.d.nodes[b], 0), a.d.T) : a.d.T;
-  s.len = max(a.d.lengths[b], 0);
-  s.keys = min((long long)s.len + s.n, (long long)a.d.max_pages * a.d.page_size);
-  s.tiles = s.n ? (int)((unsigned)(s.keys + a.keys - 1) / (unsigned)a.keys) : 0;
-  s.blocks = (s.n * a.group + a.rows - 1) / a.rows;
+  s.n = n;
+  s.len = len;
+  s.keys = min((long long)len + n, (long long)a.d.max_pages * a.d.page_size);
+  s.tiles = n ? (int)((unsigned)(s.keys + (1 << a.key_bits) - 1) >> a.key_bits) : 0;
+  s.blocks = (n * a.group + a.rows - 1) >> a.row_bits;
   return s;
 }
-// first[b] = tiles of all items of the sequences before b; by one warp, in shared memory
-__device__ __forceinline__ void tree_line(const TreeArgs& a, long long* first) {
+// by one warp, in shared memory: line[b] of the sequences, line[B].first all tiles.  Ends in the block's barrier.
+__device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
   if (threadIdx.x < 32) {
     long long run = 0;
     for (int b0 = 0; b0 < a.d.B; b0 += 32) {
       const int b = b0 + threadIdx.x;
       long long mine = 0;
       if (b < a.d.B) {
-        const TreeSeq s = tree_seq(a, b);
+        line[b].len = max(a.d.lengths[b], 0);
+        line[b].n = a.d.nodes ? min(max(a.d.nodes[b], 0), a.d.T) : a.d.T;
+        const TreeSeq s = tree_seq(a, line[b].len, line[b].n);
         mine = (long long)a.d.KVH * s.blocks * s.tiles;
       }
       long long sum = mine;
@@ -58,10 +65,10 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, long long* first) {
         const long long up = __shfl_up_sync(0xffffffffu, sum, o);
         if ((int)threadIdx.x >= o) sum += up;
       }
-      if (b < a.d.B) first[b] = run + sum - mine;
+      if (b < a.d.B) line[b].first = run + sum - mine;
       run += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (threadIdx.x == 0) first[a.d.B] = run;
+    if (threadIdx.x == 0) line[a.d.B].first = run;
   }
   __syncthreads();
 }
@@ -75,11 +82,11 @@ __device__ __forceinline__ int tree_cta_of(long long total, long long unit, int 
   const long long each = tree_div(total, ctas), more = total - each * ctas;      // the first `more` CTAs have one tile more
   return unit < (each + 1) * more ? (int)tree_div(unit, each + 1) : (int)(more + tree_div(unit - (each + 1) * more, each));
 }
-__device__ __forceinline__ int tree_find(const long long* first, int B, long long unit) {      // the sequence that `unit` belongs to
+__device__ __forceinline__ int tree_find(const TreeLine* line, int B, long long unit) {      // the sequence that `unit` belongs to
   int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (first[mid] <= unit) lo = mid; else hi = mid - 1;
+    if (line[mid].first <= unit) lo = mid; else hi = mid - 1;
   }
   return lo;
 }

@@ -19,7 +19,8 @@ namespace lp {
 constexpr int TT_BOX = 128 * 128;      // 128 rows x 64 bf16
 constexpr int TT_THREADS = 384;
 constexpr int TT_KEYS = 128;
-constexpr int TT_SPLIT_BATCH = 64;     // sequences whose line of tiles leaves room for three stages
+constexpr int TT_MAX_BATCH = 1024;      // sequences whose line of tiles fits beside the tiles
+constexpr int TT_SPLIT_BATCH = 32;      // sequences whose line of tiles leaves room for three stages
 
 #define LP_TT_TMEM_ST_16(regs, taddr)                                                                               \
   asm volatile(                                                                                                     \
@@ -59,16 +60,16 @@ struct TreePiece {
   int b, kvh, r0, t0, n;               // sequence, key head, first row, first tile, tiles
   TreeSeq s;
 };
-__device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const long long* first, long long u, long long u_end) {
+__device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const TreeLine* line, long long u, long long u_end) {
   TreePiece p;
-  p.b = tree_find(first, a.d.B, u);
-  p.s = tree_seq(a, p.b);
-  const long long local = u - first[p.b];
+  p.b = tree_find(line, a.d.B, u);
+  p.s = tree_seq(a, line[p.b].len, line[p.b].n);
+  const long long local = u - line[p.b].first;
   const int item = (int)tree_div(local, p.s.tiles);
   p.t0 = (int)(local - (long long)item * p.s.tiles);
   p.n = (int)min((long long)(p.s.tiles - p.t0), u_end - u);
   p.kvh = item / p.s.blocks;
-  p.r0 = (item % p.s.blocks) * a.rows;
+  p.r0 = (item - p.kvh * p.s.blocks) * a.rows;
   return p;
 }
 // where row `key` of a sequence lies: its place in the page table and in the page.  A sequence's rows are fewer than 2^31 (the entry point sees to it).
@@ -108,7 +109,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   int* odd = reinterpret_cast<int*>(tmem_at + 1);                      // [4] piece whose V had values that are not finite, by its number mod 4
   float2* other = reinterpret_cast<float2*>(smem + BAR_OFF + 256);     // [128] SPLIT: maximum and sum of stream 1's rows
   unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + 256);      // [256][MAX_WORDS] else: of this thread's row
-  long long* first = reinterpret_cast<long long*>(smem + BAR_OFF + 256 + (SPLIT ? 128 * 8 : 256 * MAX_WORDS * 8));
+  TreeLine* line = reinterpret_cast<TreeLine*>(smem + BAR_OFF + 256 + (SPLIT ? 128 * 8 : 256 * MAX_WORDS * 8));
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -138,9 +139,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     tmem_relinquish();
   }
   tc_fence_before();
-  tree_line(a, first);                 // (ends in the block's barrier)
+  tree_line(a, line);                 // (ends in the block's barrier)
   tc_fence_after();
-  const long long total = first[a.d.B];
+  const long long total = line[a.d.B].first;
   const long long u_begin = tree_cut(total, blockIdx.x, a.ctas), u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
   const uint32_t tmem_base = *tmem_at;
 
@@ -149,7 +150,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     const int boxes = TT_KEYS / tc.box;
     int g = 0;
     for (long long u = u_begin; u < u_end;) {
-      const TreePiece p = tree_piece(a, first, u, u_end);
+      const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
       const int n_keys = (int)p.s.keys;
       int key = p.t0 * TT_KEYS + lane * tc.box;      // this lane's box of the tile
@@ -190,7 +191,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     constexpr int STEP = SPLIT ? 2 : 1;
     int g = 0, nt = 0, pieces = 0;      // tiles of the CTA so far; tiles of this stream; pieces whose queries it has waited for
     for (long long u = u_begin; u < u_end;) {
-      const TreePiece p = tree_piece(a, first, u, u_end);
+      const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
       const int j0 = SPLIT ? q : 0;
       if (SPLIT && j0 >= p.n) {         // one tile: the other stream's (whose phases of the queries are counted all the same)
@@ -269,7 +270,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     constexpr int STEP = SPLIT ? 2 : 1;
     int g = 0, nt = 0, pieces = 0, joins = 0, seg = 0;      // tiles of the CTA and of this stream so far; pieces that it had tiles of; SPLIT: pieces of both streams
     for (long long u = u_begin; u < u_end; ++seg) {
-      const TreePiece p = tree_piece(a, first, u, u_end);
+      const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
       const int rows = p.s.n * a.group, row_base = p.r0 + (SPLIT ? 0 : q * 128), j0 = SPLIT ? q : 0;
       if (SPLIT ? j0 >= p.n : row_base >= rows) { g += p.n; continue; }
@@ -586,7 +587,7 @@ static int tree_box(const lp_tree_attn_desc* d) {
 bool tree_tc_takes(const lp_tree_attn_desc* d) {
   const bool strides = (d->n_pages == 1 || (d->k_page > 0 && d->v_page > 0)) && (d->page_size == 1 || (d->k_row > 0 && d->v_row > 0)) &&
                        (d->KVH == 1 || (d->k_head > 0 && d->v_head > 0));
-  return tree_box(d) != 0 && strides && d->scale > 0.f;      // (0 x -inf is not -inf)
+  return tree_box(d) != 0 && strides && d->scale > 0.f && d->B <= TT_MAX_BATCH;      // (0 x -inf is not -inf)
 }
 
 template <int DH>
@@ -603,7 +604,7 @@ static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
     if (const int rc = make_tmap_bf16_4d(&tm[i], base[i], dims, strides, box)) return rc;
   }
   const bool split = d.B <= TT_SPLIT_BATCH && tc.a.rows <= 128;
-  const size_t smem = (split ? 7 : 6) * NB * TT_BOX + 256 + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * 8 + 1024;
+  const size_t smem = (split ? 7 : 6) * NB * TT_BOX + 256 + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * sizeof(TreeLine) + 1024;
   auto kernel = split ? tree_tc_kernel<DH, true> : tree_tc_kernel<DH, false>;
   LP_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);

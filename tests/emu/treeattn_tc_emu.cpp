@@ -47,6 +47,7 @@ inline void tma_load_4d(void* dst, const Map4* m, uint64_t* bar, int c0, int c1,
     }
   mbar_complete_tx_addr(smem_u32(bar), 64 * m->box[2] * 2);
 }
+#define __align__(n) alignas(n)
 #include "tree_shared.inc"
 constexpr int TT_BOX = 128 * 128, TT_THREADS = 384, TT_KEYS = 128;
 inline uint64_t tt_pk2(float a, float b) { return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32); }
@@ -76,7 +77,8 @@ extern "C" void emu_tree_tc(const lp_tree_attn_desc* d, int ctas, int rows, int 
   tc.a.d = *d;
   tc.a.group = d->H / d->KVH;
   tc.a.rows = rows;
-  tc.a.keys = 128;
+  for (tc.a.row_bits = 0; 1 << tc.a.row_bits < rows;) ++tc.a.row_bits;
+  tc.a.key_bits = 7;
   tc.a.scale_log2 = d->scale * 1.4426950408889634f;
   tc.a.part_o = part_o;
   tc.a.part_ml = reinterpret_cast<float2*>(part_ml);
