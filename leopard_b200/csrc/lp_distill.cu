@@ -270,6 +270,276 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
   if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ---- the same, persistent: while a row is worked on, the next one's values are on their way into shared memory ----------------
+// What the kernel above waits for between a row's loads and its stores (loads 4 us under load, two block reductions, a barrier of the cluster) this one overlaps: a cluster
+// takes every n-th row, a CTA's part of the next row (64 KB of fp32) comes by one bulk copy, the next row's teacher entries into registers.  For rows that start on 16
+// bytes and K <= 255: a thread an entry, the label being one more.
+// Two block reductions a row: (maximum, teacher's maximum), then the sums, the teacher's among them: with u = (T - max T) / tau, t = e^u / sum e^u,
+//   sum t (log t - log p) = (sum e^u u - sum e^u (z - m) / tau) / sum e^u - log sum e^u + log sum e^((z - m) / tau)
+// where each CTA adds up e^u (z - m) of the entries in its part, against its own maximum.
+constexpr int RING_TOP = 255;
+struct RingSums {                            // of a CTA: maximum, sums, sums over its entries of e^u (z - m) and e^u, the label's z - m (0: not here)
+  float m, s, s1, ez, e, zy;
+};
+template <typename T, bool BOTH>
+__global__ void __launch_bounds__(256, 2)
+distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
+  constexpr int VEC = 16 / sizeof(T), N = DISTILL_HELD / VEC;
+  extern __shared__ __align__(128) unsigned char ring_smem[];
+  T* part = reinterpret_cast<T*>(ring_smem);                                       // [256 x DISTILL_HELD]
+  __shared__ __align__(8) uint64_t full;
+  __shared__ float2 tops[8];
+  __shared__ float sums[8][8];
+  __shared__ RingSums all[2][8];                                                   // by rank, in turn: written by the others before a barrier, read after it
+  __shared__ int ids_of[2][256];                                                   // of the rows in turn: a warp may be at the next row's while another looks for its place
+  __shared__ float es[256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % ctas;
+  const int n_clusters = gridDim.x / ctas;
+  const int vecs = (a.V + VEC - 1) / VEC, each = (vecs + ctas - 1) / ctas, i0 = min(vecs, rank * each), i1 = min(vecs, i0 + each);
+  const int v0 = min(a.V, i0 * VEC), v1 = min(a.V, i1 * VEC), whole = min(i1, a.V / VEC) - i0;      // (whole: pieces of 16 bytes that the row has)
+  const float c = a.inv_tau * 1.4426950408889634f;
+  auto row_of = [&](int r) { return reinterpret_cast<const T*>(a.logits) + (long long)r * a.ld; };
+  auto fetch = [&](int r) {                                                         // one thread
+    const uint32_t bytes = (uint32_t)max(whole, 0) * 16;
+    mbar_arrive_expect_tx(&full, bytes);
+    if (bytes) bulk_load(part, row_of(r) + (long long)i0 * VEC, bytes, &full);
+  };
+  // an entry of the next row: its id (-1: none), the teacher's value; the label is entry K
+  auto entry_id = [&](int r) {
+    long long i = -1;
+    if (tid < a.K) {
+      const long long at = (long long)r * a.ld_ids + tid;
+      i = a.ids_64 ? reinterpret_cast<const long long*>(a.ids)[at] : reinterpret_cast<const int*>(a.ids)[at];
+    } else if (tid == a.K && a.target) {
+      i = a.target[r];
+    }
+    return i >= 0 && i < a.V ? (int)i : -1;
+  };
+  auto entry_value = [&](int r) {
+    if (tid >= a.K) return -INFINITY;
+    const long long at = (long long)r * a.ld_teacher + tid;
+    return a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at] : (float)reinterpret_cast<const bf16*>(a.teacher)[at];
+  };
+  if (tid == 0) {
+    mbar_init(&full, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  int r = blockIdx.x / ctas;
+  float w = r < rows ? a.weight[r] : 0.f;
+  int id = -1;
+  float value = -INFINITY;
+  if (w != 0.f) {
+    id = entry_id(r);
+    value = entry_value(r);
+    if (tid == 0) fetch(r);
+  }
+  uint32_t loads = 0, steps = 0;
+  bf16* late_at = nullptr;                                                          // a named place of the row before, for after that row's other stores
+  float late = 0.f;
+  if (ctas > 1) {                                                                   // no CTA writes to one that has not started
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  for (; r < rows; r += n_clusters) {
+    const int next = r + n_clusters;
+    const float w_next = next < rows ? a.weight[next] : 0.f;
+    bf16* drow = a.dlogits + (long long)r * a.ldd;
+    if (rank == ctas - 1)
+      for (int i = a.V + tid; i < a.Vp; i += 256) drow[i] = __float2bfloat16_rn(0.f);
+    if (w == 0.f) {
+      if (w_next != 0.f) {
+        id = entry_id(next);
+        value = entry_value(next);
+        if (tid == 0) fetch(next);                                                  // (the part is free: its last row has been read behind a barrier)
+      }
+      for (int i = i0 + tid; i < i0 + whole; i += 256) {
+        if (VEC == 8) *reinterpret_cast<uint4*>(drow + (long long)i * VEC) = make_uint4(0, 0, 0, 0);
+        else *reinterpret_cast<uint2*>(drow + (long long)i * VEC) = make_uint2(0, 0);
+      }
+      for (int i = max(v0, (i0 + whole) * VEC) + tid; i < v1; i += 256) drow[i] = __float2bfloat16_rn(0.f);
+      if (tid == 0 && rank == 0) a.loss[r] = 0.f;
+      w = w_next;
+      continue;
+    }
+    const T* row = row_of(r);
+    mbar_wait(&full, loads & 1);
+    ++loads;
+    float x[DISTILL_HELD];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = k * 256 + tid;
+      if (i < whole) {
+        const uint4 u = lds_u4(part + (long long)i * VEC);
+        if (sizeof(T) == 4) {
+          x[k * VEC] = __uint_as_float(u.x); x[k * VEC + 1] = __uint_as_float(u.y); x[k * VEC + 2] = __uint_as_float(u.z); x[k * VEC + 3] = __uint_as_float(u.w);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
+            x[k * VEC + (2 * e) % VEC] = __uint_as_float(h << 16);
+            x[k * VEC + (2 * e + 1) % VEC] = __uint_as_float(h & 0xffff0000u);
+          }
+        }
+      } else {
+        const int v = (i0 + i) * VEC;                                               // the row's last values, fewer than 16 bytes; else nothing
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[k * VEC + e] = i0 + i < i1 && v + e < a.V ? (float)row[v + e] : -INFINITY;
+      }
+    }
+    const bool here = id >= v0 && id < v1;
+    const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
+    float m = x[0];
+#pragma unroll
+    for (int k = 1; k < DISTILL_HELD; ++k) m = fmaxf(m, x[k]);
+    float tm = id >= 0 && tid < a.K ? value : -INFINITY;
+    const float mine = tm;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+    }
+    if (lane == 0) tops[warp] = make_float2(m, tm);
+    int* ids = ids_of[steps & 1];
+    ids[tid] = id;
+    __syncthreads();                                                                // the part has been read; the row before is stored
+    if (w_next != 0.f && tid == 0) fetch(next);
+    if (late_at) *late_at = __float2bfloat16_rn(late);
+    late_at = nullptr;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      m = fmaxf(m, tops[q].x);
+      tm = fmaxf(tm, tops[q].y);
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < DISTILL_HELD; ++k) {
+      const float d = x[k] - ref, e = di_ex2(d * c);
+      s += e;
+      if (BOTH) s1 += di_ex2(d * 1.4426950408889634f);
+      else x[k] = e;                                                                // the gradient is this, scaled
+    }
+    // this thread's entry; a NaN stays one
+    const float u = mine == -INFINITY ? 0.f : (mine - tm) * a.inv_tau, e = mine == -INFINITY ? 0.f : expf(u);
+    es[tid] = e;
+    float sum[7] = {s, s1, here && e != 0.f ? e * (z - ref) : 0.f, here ? e : 0.f, here && tid == a.K ? z - ref : 0.f, e, e != 0.f ? e * u : 0.f};
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {
+      if (k == 1 && !BOTH) continue;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+      if (lane == 0) sums[warp][k] = sum[k];
+    }
+    __syncthreads();
+    RingSums* now = all[steps & 1];
+    ++steps;
+    if (warp == 0) {
+      float v = lane == 7 ? m : 0.f;
+      if (lane < 5 && (BOTH || lane != 1))
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += sums[q][lane];
+      // lanes 0 to 4 hold s, s1, ez, e, zy and lane 7 m: to the ranks' places of this CTA
+      RingSums own;
+      own.m = __shfl_sync(0xffffffffu, v, 7);
+      own.s = __shfl_sync(0xffffffffu, v, 0);
+      own.s1 = __shfl_sync(0xffffffffu, v, 1);
+      own.ez = __shfl_sync(0xffffffffu, v, 2);
+      own.e = __shfl_sync(0xffffffffu, v, 3);
+      own.zy = __shfl_sync(0xffffffffu, v, 4);
+      if (lane < ctas) {
+        const uint32_t at = mapa_u32(smem_u32(now + rank), lane);
+        const float f[6] = {own.m, own.s, own.s1, own.ez, own.e, own.zy};
+#pragma unroll
+        for (int k = 0; k < 6; ++k) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + k * 4), "f"(f[k]) : "memory");
+      }
+    }
+    __syncwarp();
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    float ts = 0.f, eu = 0.f;                                                       // the teacher's whole sums
+#pragma unroll
+    for (int q = 0; q < 8; ++q) { ts += sums[q][5]; eu += sums[q][6]; }
+    // of the entries with one id the first writes: the teacher's share of all of them, the label
+    float share = 0.f;
+    bool first = here, label = false;
+    if (here)
+      for (int o = 0; o <= a.K; ++o)
+        if (ids[o] == id) {
+          if (o < tid) first = false;
+          if (o == a.K) label = true;
+          share += es[o];
+        }
+    int id_next = -1;
+    float value_next = -INFINITY;
+    if (w_next != 0.f) {
+      id_next = entry_id(next);
+      value_next = entry_value(next);
+    }
+    const bool has_label = ids[a.K] >= 0;
+    __syncwarp();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
+    float top = -INFINITY;
+    for (int q = 0; q < ctas; ++q) top = fmaxf(top, now[q].m);
+    s = s1 = 0.f;
+    float ez = 0.f, zy = 0.f;
+    for (int q = 0; q < ctas; ++q) {
+      const RingSums o = now[q];
+      const float d = (o.m == -INFINITY ? 0.f : o.m) - top, f = o.m == -INFINITY ? 1.f : di_ex2(d * c);      // sums of a part that has nothing are 0, or NaN
+      s += o.s * f;
+      if (BOTH) s1 += o.s1 * (o.m == -INFINITY ? 1.f : di_ex2(d * 1.4426950408889634f));
+      if (o.e != 0.f) ez += o.ez + o.e * d;
+      zy += o.zy;
+    }
+    if (!BOTH) s1 = s;
+    const bool soft = !(ts == 0.f);
+    RowGrad g;
+    g.m = top;
+    g.c = c;
+    g.cs = soft ? w * (1.f - a.hard) * a.tau : 0.f;
+    g.ch = has_label ? w * a.hard : 0.f;
+    g.ks = g.cs / s;
+    g.kh = g.ch / s1;
+    if (rank == 0 && tid == 0) {
+      float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / ts - logf(ts) + logf(s)) : 0.f;
+      if (has_label && a.hard != 0.f) {
+        const int y = ids[a.K];
+        const int q = min(y / VEC / each, ctas - 1);                                // whose part it lies in: z - that part's maximum
+        l += a.hard * (logf(s1) - (zy + ((now[q].m == -INFINITY ? 0.f : now[q].m) - top)));
+      }
+      a.loss[r] = l;
+    }
+    const float down = !BOTH ? (g.ks + g.kh) * (m != -INFINITY ? di_ex2((m - top) * c) : 1.f) : 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = k * 256 + tid;
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) x[k * VEC + q] = BOTH ? g.at(x[k * VEC + q]) : x[k * VEC + q] * down;
+      const long long v = (long long)(i0 + i) * VEC;
+      if (i < whole) {
+        if (VEC == 8)
+          *reinterpret_cast<uint4*>(drow + v) = make_uint4(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]),
+                                                           pack_bf16x2(x[k * VEC + 4 % VEC], x[k * VEC + 5 % VEC]), pack_bf16x2(x[k * VEC + 6 % VEC], x[k * VEC + 7 % VEC]));
+        else
+          *reinterpret_cast<uint2*>(drow + v) = make_uint2(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]));
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q)
+          if (i0 + i < i1 && v + q < a.V) drow[v + q] = __float2bfloat16_rn(x[k * VEC + q]);
+      }
+    }
+    if (first && (share != 0.f || (label && g.ch != 0.f))) {
+      late_at = drow + id;
+      late = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
+    }
+    w = w_next;
+    id = id_next;
+    value = value_next;
+  }
+  __syncthreads();
+  if (late_at) *late_at = __float2bfloat16_rn(late);
+}
+
 // ---- longer rows: a CTA reads its row twice, the second time from the L2 ----------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -311,6 +581,27 @@ distill_long_kernel(const __grid_constant__ DistillArgs a) {
   row_loss(a, r, soft, m, s, s1, row, top, lt, id, y, red);
 }
 
+// clusters that run at once: two CTAs an SM, as far as clusters fit the GPU's groups of SMs
+template <typename Kernel>
+static cudaError_t launch_ring(Kernel kernel, const DistillArgs& a, int rows, int ctas, size_t smem, cudaStream_t stream) {
+  if (cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaError_t rc = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return rc;
+  if (n < 1) n = 1;
+  if (n > rows) n = rows;
+  return launch_ex(kernel, dim3((unsigned)(n * ctas)), dim3(256), smem, stream, ctas, false, a, ctas, rows);
+}
+
 }  // namespace lp
 
 extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long ld, const void* ids, int ids_64, long long ld_ids,
@@ -338,6 +629,15 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
   } else {
     LP_REQUIRE((long long)rows * ctas < (1LL << 31), "lp_distill_fwd_bwd: %d rows of %d columns are too many", rows, V);
     cudaError_t rc;
+    if (wide && K <= RING_TOP) {
+      const size_t part = (size_t)256 * DISTILL_HELD * size;
+#define LP_RING(T) rc = both ? launch_ring(distill_ring_kernel<T, true>, a, rows, ctas, part, stream) : launch_ring(distill_ring_kernel<T, false>, a, rows, ctas, part, stream)
+      if (logits_fp32) LP_RING(float);
+      else LP_RING(bf16);
+#undef LP_RING
+      LP_CHECK_CUDA(rc);
+      return 0;
+    }
 #define LP_HELD(T, VEC) \
   rc = both ? launch_ex(distill_held_kernel<T, VEC, true>, dim3((unsigned)rows * ctas), dim3(256), smem, stream, ctas, false, a, ctas) \
             : launch_ex(distill_held_kernel<T, VEC, false>, dim3((unsigned)rows * ctas), dim3(256), smem, stream, ctas, false, a, ctas)
