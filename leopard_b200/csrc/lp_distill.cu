@@ -271,38 +271,45 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 }
 
 // ---- the same, persistent: while a row is worked on, the next one's values are on their way into shared memory ----------------
-// What the kernel above waits for between a row's loads and its stores (loads 4 us under load, two block reductions, a barrier of the cluster) this one overlaps: a cluster
-// takes every n-th row, a CTA's part of the next row (64 KB of fp32) comes by one bulk copy, the next row's teacher entries into registers.  For rows that start on 16
-// bytes and K <= 255: a thread an entry, the label being one more.
-// Two block reductions a row: (maximum, teacher's maximum), then the sums, the teacher's among them: with u = (T - max T) / tau, t = e^u / sum e^u,
+// A cluster takes every n-th row; a CTA's part of the next row (64 KB of fp32) comes by one bulk copy, the next row's teacher entries into registers, a thread an entry and
+// the label as one more (K <= 255), for rows that start on 16 bytes.  What is left is the chain of a row: values -> maximum -> exponentials -> sums -> gradient.
+// It has one wait: every WARP sends its maximum and sums, against its own maximum, to all CTAs of the cluster (st.async on a barrier of the receiver), and takes the
+// row's from the 8 x CTAs entries that arrive.  (Block sums, a barrier of the cluster and sums of sums took 4 of 7 us a row; the barrier alone 0.7, since it waits for the
+// row before to be stored.)  The teacher's sums go along: with u = (T - max T) / tau, t = e^u / sum e^u,
 //   sum t (log t - log p) = (sum e^u u - sum e^u (z - m) / tau) / sum e^u - log sum e^u + log sum e^((z - m) / tau)
-// where each CTA adds up e^u (z - m) of the entries in its part, against its own maximum.
+// where the CTA that holds an entry's z adds up e^u (z - m) and e^u.
 constexpr int RING_TOP = 255;
-struct RingSums {                            // of a CTA: maximum, sums, sums over its entries of e^u (z - m) and e^u, the label's z - m (0: not here)
-  float m, s, s1, ez, e, zy;
+struct __align__(16) RingEntry {             // of a warp: maximum and sums of the row; the teacher's maximum
+  float m, s, s1, tm;
+  float ez, e, zy, ts;                       // over the entries in this CTA's part: e^u (z - m), e^u, the label's z - m; over all entries: e^u
+  float eu, x, y, z;                         // e^u u
 };
+__device__ __forceinline__ void ring_send(uint32_t at, uint32_t bar, float a, float b, float c, float d) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(__float_as_uint(a)), "r"(__float_as_uint(b)),
+               "r"(__float_as_uint(c)), "r"(__float_as_uint(d)), "r"(bar)
+               : "memory");
+}
 template <typename T, bool BOTH>
 __global__ void __launch_bounds__(256, 2)
 distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   constexpr int VEC = 16 / sizeof(T), N = DISTILL_HELD / VEC;
+  constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(128) unsigned char ring_smem[];
   T* part = reinterpret_cast<T*>(ring_smem);                                       // [256 x DISTILL_HELD]
-  __shared__ __align__(8) uint64_t full;
-  __shared__ float2 tops[8];
-  __shared__ float sums[8][8];
-  __shared__ RingSums all[2][8];                                                   // by rank, in turn: written by the others before a barrier, read after it
-  __shared__ int ids_of[2][256];                                                   // of the rows in turn: a warp may be at the next row's while another looks for its place
-  __shared__ float es[256];
+  // (what the rows write in turn: a warp that is at the next row but one has seen that all have sent for the next one, and so are done with this one)
+  __shared__ RingEntry all[2][64];                                                 // [rank x 8 + warp]
+  __shared__ __align__(8) uint64_t full, got[2];
+  __shared__ int ids_of[2][256];
+  __shared__ float es_of[2][256];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % ctas;
   const int n_clusters = gridDim.x / ctas;
   const int vecs = (a.V + VEC - 1) / VEC, each = (vecs + ctas - 1) / ctas, i0 = min(vecs, rank * each), i1 = min(vecs, i0 + each);
-  const int v0 = min(a.V, i0 * VEC), v1 = min(a.V, i1 * VEC), whole = min(i1, a.V / VEC) - i0;      // (whole: pieces of 16 bytes that the row has)
-  const float c = a.inv_tau * 1.4426950408889634f;
+  const int v0 = min(a.V, i0 * VEC), v1 = min(a.V, i1 * VEC), whole = max(0, min(i1, a.V / VEC) - i0);      // (whole: pieces of 16 bytes that the row has)
+  const float c = a.inv_tau * LOG2E;
   auto row_of = [&](int r) { return reinterpret_cast<const T*>(a.logits) + (long long)r * a.ld; };
   auto fetch = [&](int r) {                                                         // one thread
-    const uint32_t bytes = (uint32_t)max(whole, 0) * 16;
-    mbar_arrive_expect_tx(&full, bytes);
-    if (bytes) bulk_load(part, row_of(r) + (long long)i0 * VEC, bytes, &full);
+    mbar_arrive_expect_tx(&full, (uint32_t)whole * 16);
+    if (whole) bulk_load(part, row_of(r) + (long long)i0 * VEC, (uint32_t)whole * 16, &full);
   };
   // an entry of the next row: its id (-1: none), the teacher's value; the label is entry K
   auto entry_id = [&](int r) {
@@ -322,6 +329,8 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   };
   if (tid == 0) {
     mbar_init(&full, 1);
+    mbar_init(&got[0], 8);
+    mbar_init(&got[1], 8);
     fence_barrier_init();
   }
   __syncthreads();
@@ -334,13 +343,10 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     value = entry_value(r);
     if (tid == 0) fetch(r);
   }
-  uint32_t loads = 0, steps = 0;
+  uint32_t steps = 0;                                                               // rows of a weight so far
   bf16* late_at = nullptr;                                                          // a named place of the row before, for after that row's other stores
   float late = 0.f;
-  if (ctas > 1) {                                                                   // no CTA writes to one that has not started
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
+  if (ctas > 1) cluster_sync_all();                                                 // no CTA sends to one that has not started
   for (; r < rows; r += n_clusters) {
     const int next = r + n_clusters;
     const float w_next = next < rows ? a.weight[next] : 0.f;
@@ -351,7 +357,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       if (w_next != 0.f) {
         id = entry_id(next);
         value = entry_value(next);
-        if (tid == 0) fetch(next);                                                  // (the part is free: its last row has been read behind a barrier)
+        if (tid == 0) fetch(next);                                                  // (the part is free: thread 0 has waited for the row before it)
       }
       for (int i = i0 + tid; i < i0 + whole; i += 256) {
         if (VEC == 8) *reinterpret_cast<uint4*>(drow + (long long)i * VEC) = make_uint4(0, 0, 0, 0);
@@ -363,8 +369,9 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       continue;
     }
     const T* row = row_of(r);
-    mbar_wait(&full, loads & 1);
-    ++loads;
+    const uint32_t turn = steps & 1, phase = (steps >> 1) & 1;
+    mbar_wait(&full, steps & 1);
+    ++steps;
     float x[DISTILL_HELD];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -389,127 +396,103 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     }
     const bool here = id >= v0 && id < v1;
     const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
-    float m = x[0];
+    float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-    for (int k = 1; k < DISTILL_HELD; ++k) m = fmaxf(m, x[k]);
-    float tm = id >= 0 && tid < a.K ? value : -INFINITY;
-    const float mine = tm;
+    for (int k = 4; k < DISTILL_HELD; ++k) m4[k & 3] = fmaxf(m4[k & 3], x[k]);
+    float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    const float mine = id >= 0 && tid < a.K ? value : -INFINITY;
+    float tm = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
     }
-    if (lane == 0) tops[warp] = make_float2(m, tm);
-    int* ids = ids_of[steps & 1];
-    ids[tid] = id;
-    __syncthreads();                                                                // the part has been read; the row before is stored
-    if (w_next != 0.f && tid == 0) fetch(next);
-    if (late_at) *late_at = __float2bfloat16_rn(late);
-    late_at = nullptr;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      m = fmaxf(m, tops[q].x);
-      tm = fmaxf(tm, tops[q].y);
-    }
     const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, s1 = 0.f;
+    float s4[4] = {0.f, 0.f, 0.f, 0.f}, s1 = 0.f;
 #pragma unroll
     for (int k = 0; k < DISTILL_HELD; ++k) {
       const float d = x[k] - ref, e = di_ex2(d * c);
-      s += e;
-      if (BOTH) s1 += di_ex2(d * 1.4426950408889634f);
+      s4[k & 3] += e;
+      if (BOTH) s1 += di_ex2(d * LOG2E);
       else x[k] = e;                                                                // the gradient is this, scaled
     }
     // this thread's entry; a NaN stays one
     const float u = mine == -INFINITY ? 0.f : (mine - tm) * a.inv_tau, e = mine == -INFINITY ? 0.f : expf(u);
-    es[tid] = e;
-    float sum[7] = {s, s1, here && e != 0.f ? e * (z - ref) : 0.f, here ? e : 0.f, here && tid == a.K ? z - ref : 0.f, e, e != 0.f ? e * u : 0.f};
+    ids_of[turn][tid] = id;
+    es_of[turn][tid] = e;
+    RingEntry me;
+    {
+      float sum[7] = {(s4[0] + s4[1]) + (s4[2] + s4[3]), s1, here && e != 0.f ? e * (z - ref) : 0.f, here ? e : 0.f, here && tid == a.K ? z - ref : 0.f, e, e != 0.f ? e * u : 0.f};
+      const bool entries = warp * 32 <= a.K;                                        // this warp has some
 #pragma unroll
-    for (int k = 0; k < 7; ++k) {
-      if (k == 1 && !BOTH) continue;
+      for (int k = 0; k < 7; ++k) {
+        if ((k == 1 && !BOTH) || (k > 1 && !entries)) continue;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
-      if (lane == 0) sums[warp][k] = sum[k];
-    }
-    __syncthreads();
-    RingSums* now = all[steps & 1];
-    ++steps;
-    if (warp == 0) {
-      float v = lane == 7 ? m : 0.f;
-      if (lane < 5 && (BOTH || lane != 1))
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v += sums[q][lane];
-      // lanes 0 to 4 hold s, s1, ez, e, zy and lane 7 m: to the ranks' places of this CTA
-      RingSums own;
-      own.m = __shfl_sync(0xffffffffu, v, 7);
-      own.s = __shfl_sync(0xffffffffu, v, 0);
-      own.s1 = __shfl_sync(0xffffffffu, v, 1);
-      own.ez = __shfl_sync(0xffffffffu, v, 2);
-      own.e = __shfl_sync(0xffffffffu, v, 3);
-      own.zy = __shfl_sync(0xffffffffu, v, 4);
-      if (lane < ctas) {
-        const uint32_t at = mapa_u32(smem_u32(now + rank), lane);
-        const float f[6] = {own.m, own.s, own.s1, own.ez, own.e, own.zy};
-#pragma unroll
-        for (int k = 0; k < 6; ++k) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + k * 4), "f"(f[k]) : "memory");
+        for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
       }
+      me = {m, sum[0], sum[1], tm, sum[2], sum[3], sum[4], sum[5], sum[6], 0.f, 0.f, 0.f};
     }
     __syncwarp();
-    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    float ts = 0.f, eu = 0.f;                                                       // the teacher's whole sums
-#pragma unroll
-    for (int q = 0; q < 8; ++q) { ts += sums[q][5]; eu += sums[q][6]; }
-    // of the entries with one id the first writes: the teacher's share of all of them, the label
-    float share = 0.f;
-    bool first = here, label = false;
-    if (here)
-      for (int o = 0; o <= a.K; ++o)
-        if (ids[o] == id) {
-          if (o < tid) first = false;
-          if (o == a.K) label = true;
-          share += es[o];
-        }
+    if (ctas == 1) {                                                                // (not launched as a cluster: st.async is for clusters)
+      if (lane == 0) {
+        all[turn][warp] = me;
+        mbar_arrive(&got[turn]);
+      }
+    } else if (lane == 0) {
+      mbar_arrive_expect_tx(&got[turn], (uint32_t)ctas * sizeof(RingEntry));
+    }
+    if (ctas > 1 && lane < ctas) {
+      const uint32_t at = mapa_u32(smem_u32(&all[turn][rank * 8 + warp]), lane), bar = mapa_u32(smem_u32(&got[turn]), lane);
+      ring_send(at, bar, me.m, me.s, me.s1, me.tm);
+      ring_send(at + 16, bar, me.ez, me.e, me.zy, me.ts);
+      ring_send(at + 32, bar, me.eu, 0.f, 0.f, 0.f);
+    }
     int id_next = -1;
     float value_next = -INFINITY;
     if (w_next != 0.f) {
       id_next = entry_id(next);
       value_next = entry_value(next);
     }
-    const bool has_label = ids[a.K] >= 0;
-    __syncwarp();
-    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else __syncthreads();
-    float top = -INFINITY;
-    for (int q = 0; q < ctas; ++q) top = fmaxf(top, now[q].m);
-    s = s1 = 0.f;
-    float ez = 0.f, zy = 0.f;
-    for (int q = 0; q < ctas; ++q) {
-      const RingSums o = now[q];
-      const float d = (o.m == -INFINITY ? 0.f : o.m) - top, f = o.m == -INFINITY ? 1.f : di_ex2(d * c);      // sums of a part that has nothing are 0, or NaN
-      s += o.s * f;
-      if (BOTH) s1 += o.s1 * (o.m == -INFINITY ? 1.f : di_ex2(d * 1.4426950408889634f));
-      if (o.e != 0.f) ez += o.ez + o.e * d;
-      zy += o.zy;
+    mbar_wait(&got[turn], phase);
+    if (w_next != 0.f && tid == 0) fetch(next);                                     // all warps have read the part
+    if (late_at) *late_at = __float2bfloat16_rn(late);                              // ... and stored the row before
+    late_at = nullptr;
+    // the row's maximum and sums, from all warps of the cluster: two entries a lane
+    const RingEntry* from = all[turn];
+    const int n_from = 8 * ctas;
+    float4 f0 = make_float4(-INFINITY, 0.f, 0.f, 0.f), f1 = f0;
+    if (lane < n_from) f0 = *reinterpret_cast<const float4*>(from + lane);
+    if (lane + 32 < n_from) f1 = *reinterpret_cast<const float4*>(from + lane + 32);
+    float top = fmaxf(f0.x, f1.x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    auto against = [&](float mw, float scale) { return mw == -INFINITY ? 1.f : di_ex2((mw - top) * scale); };      // sums of a warp that has nothing are 0, or NaN
+    float S = f0.y * against(f0.x, c) + f1.y * against(f1.x, c), S1 = BOTH ? f0.z * against(f0.x, LOG2E) + f1.z * against(f1.x, LOG2E) : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      S += __shfl_xor_sync(0xffffffffu, S, o);
+      if (BOTH) S1 += __shfl_xor_sync(0xffffffffu, S1, o);
     }
-    if (!BOTH) s1 = s;
+    if (!BOTH) S1 = S;
+    const int* ids = ids_of[turn];
+    const bool has_label = ids[a.K] >= 0;
+    // the teacher's: of this CTA's warps, all of which have all entries' sums between them
+    float t_top = -INFINITY, ts = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) t_top = fmaxf(t_top, from[rank * 8 + q].tm);
+    auto teacher_scale = [&](float tmw) { return tmw == -INFINITY ? 1.f : di_ex2((tmw - t_top) * c); };
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q * 32 < a.K) ts += from[rank * 8 + q].ts * teacher_scale(from[rank * 8 + q].tm);
     const bool soft = !(ts == 0.f);
     RowGrad g;
     g.m = top;
     g.c = c;
     g.cs = soft ? w * (1.f - a.hard) * a.tau : 0.f;
     g.ch = has_label ? w * a.hard : 0.f;
-    g.ks = g.cs / s;
-    g.kh = g.ch / s1;
-    if (rank == 0 && tid == 0) {
-      float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / ts - logf(ts) + logf(s)) : 0.f;
-      if (has_label && a.hard != 0.f) {
-        const int y = ids[a.K];
-        const int q = min(y / VEC / each, ctas - 1);                                // whose part it lies in: z - that part's maximum
-        l += a.hard * (logf(s1) - (zy + ((now[q].m == -INFINITY ? 0.f : now[q].m) - top)));
-      }
-      a.loss[r] = l;
-    }
-    const float down = !BOTH ? (g.ks + g.kh) * (m != -INFINITY ? di_ex2((m - top) * c) : 1.f) : 0.f;
+    g.ks = g.cs / S;
+    g.kh = g.ch / S1;
+    const float down = !BOTH ? (g.ks + g.kh) * against(m, c) : 0.f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int i = k * 256 + tid;
@@ -528,9 +511,43 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
           if (i0 + i < i1 && v + q < a.V) drow[v + q] = __float2bfloat16_rn(x[k * VEC + q]);
       }
     }
-    if (first && (share != 0.f || (label && g.ch != 0.f))) {
-      late_at = drow + id;
-      late = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
+    // of the entries with one id the first writes: the teacher's share of all of them, the label
+    if (here) {
+      float share = 0.f;
+      bool first = true, label = false;
+      for (int o = 0; o <= a.K; ++o)
+        if (ids[o] == id) {
+          if (o < tid) first = false;
+          if (o == a.K) label = true;
+          share += es_of[turn][o] * teacher_scale(from[rank * 8 + (o >> 5)].tm);
+        }
+      if (first && (share != 0.f || (label && g.ch != 0.f))) {
+        late_at = drow + id;
+        late = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
+      }
+    }
+    __syncwarp();
+    if (rank == 0 && warp == 7) {                                                   // (the warp that has the fewest entries)
+      float ez = 0.f, zy = 0.f, eu = 0.f;
+      for (int q = lane; q < n_from; q += 32) {
+        const RingEntry o = from[q];
+        // o.e, o.ez are against o's teacher maximum and its own maximum: e^u (z - m)
+        const float t = teacher_scale(o.tm), d = (o.m == -INFINITY ? 0.f : o.m) - top;
+        if (o.e != 0.f) ez += t * (o.ez + o.e * d);
+        if (has_label && q / 8 == min(ids[a.K] / VEC / each, ctas - 1) && q % 8 == a.K >> 5) zy = o.zy + d;      // of the CTA that holds the label's z, the warp of entry K
+        if (q < 8 && o.ts != 0.f) eu += t * (o.eu + o.ts * (o.tm == -INFINITY ? 0.f : (o.tm - t_top) * a.inv_tau));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        ez += __shfl_xor_sync(0xffffffffu, ez, o);
+        zy += __shfl_xor_sync(0xffffffffu, zy, o);
+        eu += __shfl_xor_sync(0xffffffffu, eu, o);
+      }
+      if (lane == 0) {
+        float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / ts - logf(ts) + logf(S)) : 0.f;
+        if (has_label && a.hard != 0.f) l += a.hard * (logf(S1) - zy);
+        a.loss[r] = l;
+      }
     }
     w = w_next;
     id = id_next;
