@@ -301,6 +301,9 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   __shared__ __align__(8) uint64_t full, got[2];
   __shared__ int ids_of[2][256];
   __shared__ float es_of[2][256];
+  __shared__ uint32_t bits_of[3][256 * DISTILL_HELD / 32];                          // the places of this part that an entry names (three: cleared while the next row is done) ...
+  __shared__ uint32_t twice[2];                                                     // ... and the last row that named one twice
+  __shared__ struct { float S, S1, top, ts, t_top; int y; } done;                   // what the loss of a row needs, besides the warps' entries
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % ctas;
   const int n_clusters = gridDim.x / ctas;
   const int vecs = (a.V + VEC - 1) / VEC, each = (vecs + ctas - 1) / ctas, i0 = min(vecs, rank * each), i1 = min(vecs, i0 + each);
@@ -311,23 +314,26 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     mbar_arrive_expect_tx(&full, (uint32_t)whole * 16);
     if (whole) bulk_load(part, row_of(r) + (long long)i0 * VEC, (uint32_t)whole * 16, &full);
   };
-  // an entry of the next row: its id (-1: none), the teacher's value; the label is entry K
+  // an entry of a row: its id (-1: none), the teacher's value; the label is entry K
   auto entry_id = [&](int r) {
     long long i = -1;
-    if (tid < a.K) {
+    if (r < rows && tid < a.K) {
       const long long at = (long long)r * a.ld_ids + tid;
       i = a.ids_64 ? reinterpret_cast<const long long*>(a.ids)[at] : reinterpret_cast<const int*>(a.ids)[at];
-    } else if (tid == a.K && a.target) {
+    } else if (r < rows && tid == a.K && a.target) {
       i = a.target[r];
     }
-    return i >= 0 && i < a.V ? (int)i : -1;
+    return i;
   };
   auto entry_value = [&](int r) {
-    if (tid >= a.K) return -INFINITY;
+    if (r >= rows || tid >= a.K) return -INFINITY;
     const long long at = (long long)r * a.ld_teacher + tid;
     return a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at] : (float)reinterpret_cast<const bf16*>(a.teacher)[at];
   };
+  auto weight_of = [&](int r) { return r < rows ? a.weight[r] : 0.f; };
+  for (int i = tid; i < 3 * 256 * DISTILL_HELD / 32; i += 256) (&bits_of[0][0])[i] = 0;
   if (tid == 0) {
+    twice[0] = twice[1] = 0;
     mbar_init(&full, 1);
     mbar_init(&got[0], 8);
     mbar_init(&got[1], 8);
@@ -335,42 +341,67 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   }
   __syncthreads();
   int r = blockIdx.x / ctas;
-  float w = r < rows ? a.weight[r] : 0.f;
-  int id = -1;
-  float value = -INFINITY;
-  if (w != 0.f) {
-    id = entry_id(r);
-    value = entry_value(r);
-    if (tid == 0) fetch(r);
-  }
+  // this row's and, under way for a whole row (loads take 2 us and more while the memory is busy), the next one's
+  float w = weight_of(r), w_next = weight_of(r + n_clusters);
+  long long id_now = entry_id(r), id_next = entry_id(r + n_clusters);
+  float value = entry_value(r), value_next = entry_value(r + n_clusters);
+  if (w != 0.f && tid == 0) fetch(r);
   uint32_t steps = 0;                                                               // rows of a weight so far
   bf16* late_at = nullptr;                                                          // a named place of the row before, for after that row's other stores
   float late = 0.f;
   if (ctas > 1) cluster_sync_all();                                                 // no CTA sends to one that has not started
+  // the loss of the last row, by a warp of the first CTA while it would wait for the next one's sums (0.6 us that all would wait for)
+  int row_done = -1;
+  auto loss_of = [&](const RingEntry* from) {
+    __syncwarp();
+    const bool has_label = done.y >= 0, soft = !(done.ts == 0.f);
+    const int holder = has_label ? min(done.y / VEC / each, ctas - 1) * 8 + (a.K >> 5) : -1;      // of the CTA that holds the label's z, the warp of entry K
+    float ez = 0.f, zy = 0.f, eu = 0.f;
+    for (int q = lane; q < 8 * ctas; q += 32) {
+      const RingEntry o = from[q];
+      // o.e, o.ez are against o's teacher maximum and its own maximum: e^u (z - m)
+      const float t = o.tm == -INFINITY ? 1.f : di_ex2((o.tm - done.t_top) * c), d = (o.m == -INFINITY ? 0.f : o.m) - done.top;
+      if (o.e != 0.f) ez += t * (o.ez + o.e * d);
+      if (q == holder) zy = o.zy + d;
+      if (q < 8 && o.ts != 0.f) eu += t * (o.eu + o.ts * (o.tm == -INFINITY ? 0.f : (o.tm - done.t_top) * a.inv_tau));      // (every CTA has all entries' e^u)
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ez += __shfl_xor_sync(0xffffffffu, ez, o);
+      zy += __shfl_xor_sync(0xffffffffu, zy, o);
+      eu += __shfl_xor_sync(0xffffffffu, eu, o);
+    }
+    if (lane == 0) {
+      float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / done.ts - logf(done.ts) + logf(done.S)) : 0.f;
+      if (has_label && a.hard != 0.f) l += a.hard * (logf(done.S1) - zy);
+      a.loss[row_done] = l;
+    }
+    __syncwarp();
+    row_done = -1;
+  };
   for (; r < rows; r += n_clusters) {
     const int next = r + n_clusters;
-    const float w_next = next < rows ? a.weight[next] : 0.f;
+    const float w_then = weight_of(next + n_clusters), value_then = entry_value(next + n_clusters);
+    const long long id_then = entry_id(next + n_clusters);
     bf16* drow = a.dlogits + (long long)r * a.ldd;
     if (rank == ctas - 1)
       for (int i = a.V + tid; i < a.Vp; i += 256) drow[i] = __float2bfloat16_rn(0.f);
     if (w == 0.f) {
-      if (w_next != 0.f) {
-        id = entry_id(next);
-        value = entry_value(next);
-        if (tid == 0) fetch(next);                                                  // (the part is free: thread 0 has waited for the row before it)
-      }
+      if (w_next != 0.f && tid == 0) fetch(next);                                   // (the part is free: thread 0 has waited for the row before it)
       for (int i = i0 + tid; i < i0 + whole; i += 256) {
         if (VEC == 8) *reinterpret_cast<uint4*>(drow + (long long)i * VEC) = make_uint4(0, 0, 0, 0);
         else *reinterpret_cast<uint2*>(drow + (long long)i * VEC) = make_uint2(0, 0);
       }
       for (int i = max(v0, (i0 + whole) * VEC) + tid; i < v1; i += 256) drow[i] = __float2bfloat16_rn(0.f);
       if (tid == 0 && rank == 0) a.loss[r] = 0.f;
-      w = w_next;
+      w = w_next, w_next = w_then, id_now = id_next, id_next = id_then, value = value_next, value_next = value_then;
       continue;
     }
     const T* row = row_of(r);
     const uint32_t turn = steps & 1, phase = (steps >> 1) & 1;
     mbar_wait(&full, steps & 1);
+    uint32_t* bits = bits_of[steps % 3];
+    uint32_t* bits_before = bits_of[(steps + 2) % 3];
     ++steps;
     float x[DISTILL_HELD];
 #pragma unroll
@@ -394,6 +425,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
         for (int e = 0; e < VEC; ++e) x[k * VEC + e] = i0 + i < i1 && v + e < a.V ? (float)row[v + e] : -INFINITY;
       }
     }
+    const int id = id_now >= 0 && id_now < a.V ? (int)id_now : -1;
     const bool here = id >= v0 && id < v1;
     const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
     float m4[4] = {x[0], x[1], x[2], x[3]};
@@ -420,6 +452,10 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     const float u = mine == -INFINITY ? 0.f : (mine - tm) * a.inv_tau, e = mine == -INFINITY ? 0.f : expf(u);
     ids_of[turn][tid] = id;
     es_of[turn][tid] = e;
+    if (here && tid < a.K) {
+      const uint32_t bit = 1u << ((id - v0) & 31);
+      if (atomicOr(&bits[(id - v0) >> 5], bit) & bit) twice[turn] = steps;
+    }
     RingEntry me;
     {
       float sum[7] = {(s4[0] + s4[1]) + (s4[2] + s4[3]), s1, here && e != 0.f ? e * (z - ref) : 0.f, here ? e : 0.f, here && tid == a.K ? z - ref : 0.f, e, e != 0.f ? e * u : 0.f};
@@ -447,16 +483,15 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       ring_send(at + 16, bar, me.ez, me.e, me.zy, me.ts);
       ring_send(at + 32, bar, me.eu, 0.f, 0.f, 0.f);
     }
-    int id_next = -1;
-    float value_next = -INFINITY;
-    if (w_next != 0.f) {
-      id_next = entry_id(next);
-      value_next = entry_value(next);
-    }
+    if (row_done >= 0) loss_of(all[turn ^ 1]);
     mbar_wait(&got[turn], phase);
     if (w_next != 0.f && tid == 0) fetch(next);                                     // all warps have read the part
     if (late_at) *late_at = __float2bfloat16_rn(late);                              // ... and stored the row before
     late_at = nullptr;
+    if (steps > 1 && tid < a.K) {
+      const int old = ids_of[turn ^ 1][tid];
+      if (old >= v0 && old < v1) bits_before[(old - v0) >> 5] = 0;
+    }
     // the row's maximum and sums, from all warps of the cluster: two entries a lane
     const RingEntry* from = all[turn];
     const int n_from = 8 * ctas;
@@ -511,48 +546,33 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
           if (i0 + i < i1 && v + q < a.V) drow[v + q] = __float2bfloat16_rn(x[k * VEC + q]);
       }
     }
-    // of the entries with one id the first writes: the teacher's share of all of them, the label
+    // the places that entries name lose the teacher's share, the label's its own.  Of entries with one id the first writes, of the label and entries these.
     if (here) {
-      float share = 0.f;
-      bool first = true, label = false;
-      for (int o = 0; o <= a.K; ++o)
-        if (ids[o] == id) {
-          if (o < tid) first = false;
-          if (o == a.K) label = true;
-          share += es_of[turn][o] * teacher_scale(from[rank * 8 + (o >> 5)].tm);
-        }
-      if (first && (share != 0.f || (label && g.ch != 0.f))) {
+      const uint32_t word = (id - v0) >> 5, bit = 1u << ((id - v0) & 31);
+      const bool label = ids[a.K] == id;
+      float share = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm);
+      bool writes = tid < a.K || !(bits[word] & bit);
+      if (writes && tid < a.K && twice[turn] == steps) {
+        share = 0.f;
+        for (int o = 0; o < a.K; ++o)
+          if (ids[o] == id) {
+            if (o < tid) writes = false;
+            share += es_of[turn][o] * teacher_scale(from[rank * 8 + (o >> 5)].tm);
+          }
+      }
+      if (writes && (share != 0.f || (label && g.ch != 0.f))) {
         late_at = drow + id;
         late = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
       }
     }
     __syncwarp();
-    if (rank == 0 && warp == 7) {                                                   // (the warp that has the fewest entries)
-      float ez = 0.f, zy = 0.f, eu = 0.f;
-      for (int q = lane; q < n_from; q += 32) {
-        const RingEntry o = from[q];
-        // o.e, o.ez are against o's teacher maximum and its own maximum: e^u (z - m)
-        const float t = teacher_scale(o.tm), d = (o.m == -INFINITY ? 0.f : o.m) - top;
-        if (o.e != 0.f) ez += t * (o.ez + o.e * d);
-        if (has_label && q / 8 == min(ids[a.K] / VEC / each, ctas - 1) && q % 8 == a.K >> 5) zy = o.zy + d;      // of the CTA that holds the label's z, the warp of entry K
-        if (q < 8 && o.ts != 0.f) eu += t * (o.eu + o.ts * (o.tm == -INFINITY ? 0.f : (o.tm - t_top) * a.inv_tau));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        ez += __shfl_xor_sync(0xffffffffu, ez, o);
-        zy += __shfl_xor_sync(0xffffffffu, zy, o);
-        eu += __shfl_xor_sync(0xffffffffu, eu, o);
-      }
-      if (lane == 0) {
-        float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / ts - logf(ts) + logf(S)) : 0.f;
-        if (has_label && a.hard != 0.f) l += a.hard * (logf(S1) - zy);
-        a.loss[r] = l;
-      }
+    if (rank == 0 && warp == 7) {
+      if (lane == 0) done = {S, S1, top, ts, t_top, ids[a.K]};
+      row_done = r;
     }
-    w = w_next;
-    id = id_next;
-    value = value_next;
+    w = w_next, w_next = w_then, id_now = id_next, id_next = id_then, value = value_next, value_next = value_then;
   }
+  if (row_done >= 0) loss_of(all[(steps & 1) ^ 1]);
   __syncthreads();
   if (late_at) *late_at = __float2bfloat16_rn(late);
 }
