@@ -271,18 +271,17 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 }
 
 // ---- the same, persistent: while a row is worked on, the next one's values are on their way into shared memory ----------------
-// A cluster takes every n-th row; a CTA's part of the next row (64 KB of fp32) comes by one bulk copy, the next row's teacher entries into registers, a thread an entry and
+// A cluster takes every n-th row that has a weight (and zeroes every n-th that has none): in a batch where the answers alone count it matters that all have as many.
+// A CTA's part of the next row (64 KB of fp32) comes by one bulk copy, the next row's teacher entries into registers, a thread an entry and
 // the label as one more (K <= 255), for rows that start on 16 bytes.  What is left is the chain of a row: values -> maximum -> exponentials -> sums -> gradient.
 // It has one wait: every WARP sends its maximum and sums, against its own maximum, to all CTAs of the cluster (st.async on a barrier of the receiver), and takes the
 // row's from the 8 x CTAs entries that arrive.  (Block sums, a barrier of the cluster and sums of sums took 4 of 7 us a row; the barrier alone 0.7, since it waits for the
-// row before to be stored.)  The teacher's sums go along: with u = (T - max T) / tau, t = e^u / sum e^u,
-//   sum t (log t - log p) = (sum e^u u - sum e^u (z - m) / tau) / sum e^u - log sum e^u + log sum e^((z - m) / tau)
-// where the CTA that holds an entry's z adds up e^u (z - m) and e^u.
+// row before to be stored.)  A warp's part of the row's loss, which needs the row's sums, goes along with the next row's.
 constexpr int RING_TOP = 255;
+constexpr int RING_LIST = 1536, RING_LOOK = 1024;      // rows that a cluster knows to be its own; weights that are looked at at once
 struct __align__(16) RingEntry {             // of a warp: maximum and sums of the row; the teacher's maximum
   float m, s, s1, tm;
-  float ez, e, zy, ts;                       // over the entries in this CTA's part: e^u (z - m), e^u, the label's z - m; over all entries: e^u
-  float eu, x, y, z;                         // e^u u
+  float ts, loss, x, y;                      // sum over the teacher's entries of e^((T - tm) / tau); the warp's part of the loss of the row before
 };
 __device__ __forceinline__ void ring_send(uint32_t at, uint32_t bar, float a, float b, float c, float d) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at), "r"(__float_as_uint(a)), "r"(__float_as_uint(b)),
@@ -303,7 +302,12 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   __shared__ float es_of[2][256];
   __shared__ uint32_t bits_of[3][256 * DISTILL_HELD / 32];                          // the places of this part that an entry names (three: cleared while the next row is done) ...
   __shared__ uint32_t twice[2];                                                     // ... and the last row that named one twice
-  __shared__ struct { float S, S1, top, ts, t_top; int y; } done;                   // what the loss of a row needs, besides the warps' entries
+  __shared__ int list[RING_LIST], empty_rows[RING_LIST];                            // this cluster's rows of a weight, and of none
+  __shared__ float list_weight[RING_LIST];
+  __shared__ int counts[8];
+  // what a thread or warp needs between rows: not in registers, which the row's values take
+  __shared__ int late_id[256], state[4];                                            // a named place of the row before, for after that row's other stores; the list's numbers
+  __shared__ float late_value[256], warp_loss[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % ctas;
   const int n_clusters = gridDim.x / ctas;
   const int vecs = (a.V + VEC - 1) / VEC, each = (vecs + ctas - 1) / ctas, i0 = min(vecs, rank * each), i1 = min(vecs, i0 + each);
@@ -330,7 +334,6 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     const long long at = (long long)r * a.ld_teacher + tid;
     return a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at] : (float)reinterpret_cast<const bf16*>(a.teacher)[at];
   };
-  auto weight_of = [&](int r) { return r < rows ? a.weight[r] : 0.f; };
   for (int i = tid; i < 3 * 256 * DISTILL_HELD / 32; i += 256) (&bits_of[0][0])[i] = 0;
   if (tid == 0) {
     twice[0] = twice[1] = 0;
@@ -340,63 +343,117 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     fence_barrier_init();
   }
   __syncthreads();
-  int r = blockIdx.x / ctas;
-  // this row's and, under way for a whole row (loads take 2 us and more while the memory is busy), the next one's
-  float w = weight_of(r), w_next = weight_of(r + n_clusters);
-  long long id_now = entry_id(r), id_next = entry_id(r + n_clusters);
-  float value = entry_value(r), value_next = entry_value(r + n_clusters);
-  if (w != 0.f && tid == 0) fetch(r);
-  uint32_t steps = 0;                                                               // rows of a weight so far
-  bf16* late_at = nullptr;                                                          // a named place of the row before, for after that row's other stores
-  float late = 0.f;
-  if (ctas > 1) cluster_sync_all();                                                 // no CTA sends to one that has not started
-  // the loss of the last row, by a warp of the first CTA while it would wait for the next one's sums (0.6 us that all would wait for)
-  int row_done = -1;
-  auto loss_of = [&](const RingEntry* from) {
-    __syncwarp();
-    const bool has_label = done.y >= 0, soft = !(done.ts == 0.f);
-    const int holder = has_label ? min(done.y / VEC / each, ctas - 1) * 8 + (a.K >> 5) : -1;      // of the CTA that holds the label's z, the warp of entry K
-    float ez = 0.f, zy = 0.f, eu = 0.f;
-    for (int q = lane; q < 8 * ctas; q += 32) {
-      const RingEntry o = from[q];
-      // o.e, o.ez are against o's teacher maximum and its own maximum: e^u (z - m)
-      const float t = o.tm == -INFINITY ? 1.f : di_ex2((o.tm - done.t_top) * c), d = (o.m == -INFINITY ? 0.f : o.m) - done.top;
-      if (o.e != 0.f) ez += t * (o.ez + o.e * d);
-      if (q == holder) zy = o.zy + d;
-      if (q < 8 && o.ts != 0.f) eu += t * (o.eu + o.ts * (o.tm == -INFINITY ? 0.f : (o.tm - done.t_top) * a.inv_tau));      // (every CTA has all entries' e^u)
-    }
+  // which rows: of those of a weight the cluster's is every n_clusters-th, likewise of the others; the block looks at RING_LOOK weights at a time
+  const int cluster = blockIdx.x / ctas;
+  if (tid < 4) state[tid] = 0;                                                      // rows looked at, those of a weight among them, list, empty_rows
+  auto look = [&]() {
+    __syncthreads();
+    int looked = state[0], some_before = state[1], n_list = 0, n_empty = 0;
+    int list_from = (some_before - cluster + n_clusters - 1) / n_clusters, empty_from = (looked - some_before - cluster + n_clusters - 1) / n_clusters;      // (what came before)
+    list_from = max(list_from, 0), empty_from = max(empty_from, 0);
+    const int most = RING_LOOK / n_clusters + 2;
+    while (looked < rows && n_list + most <= RING_LIST && n_empty + most <= RING_LIST) {
+      float w[4];
+      int mine = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      ez += __shfl_xor_sync(0xffffffffu, ez, o);
-      zy += __shfl_xor_sync(0xffffffffu, zy, o);
-      eu += __shfl_xor_sync(0xffffffffu, eu, o);
+      for (int k = 0; k < 4; ++k) {
+        const int i = looked + tid * 4 + k;
+        w[k] = i < rows ? a.weight[i] : 0.f;
+        mine += w[k] != 0.f;
+      }
+      int before = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+      }
+      __syncthreads();                                                              // (counts of the last round, and the lists, have been read)
+      if (lane == 31) counts[warp] = before;
+      __syncthreads();
+      int some = 0;
+      before -= mine;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (q < warp) before += counts[q];
+        some += counts[q];
+      }
+      const int here = min(RING_LOOK, rows - looked);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool on = w[k] != 0.f;
+        const int i = tid * 4 + k, nth = on ? some_before + before : looked - some_before + i - before;
+        if (i < here && nth % n_clusters == cluster) {
+          if (on) {
+            list[nth / n_clusters - list_from] = looked + i;
+            list_weight[nth / n_clusters - list_from] = w[k];
+          } else empty_rows[nth / n_clusters - empty_from] = looked + i;
+        }
+        before += on;
+      }
+      looked += here;
+      some_before += some;
+      n_list = max(0, (some_before - cluster + n_clusters - 1) / n_clusters - list_from);
+      n_empty = max(0, (looked - some_before - cluster + n_clusters - 1) / n_clusters - empty_from);
     }
-    if (lane == 0) {
-      float l = soft ? (1.f - a.hard) * a.tau * a.tau * ((eu - ez * a.inv_tau) / done.ts - logf(done.ts) + logf(done.S)) : 0.f;
-      if (has_label && a.hard != 0.f) l += a.hard * (logf(done.S1) - zy);
-      a.loss[row_done] = l;
-    }
-    __syncwarp();
-    row_done = -1;
+    __syncthreads();
+    if (tid == 0) { state[0] = looked; state[1] = some_before; state[2] = n_list; state[3] = n_empty; }
+    __syncthreads();
+    return n_list + n_empty > 0;
   };
-  for (; r < rows; r += n_clusters) {
-    const int next = r + n_clusters;
-    const float w_then = weight_of(next + n_clusters), value_then = entry_value(next + n_clusters);
-    const long long id_then = entry_id(next + n_clusters);
+  uint32_t steps = 0;                                                               // rows of a weight so far
+  late_id[tid] = -1;
+  if (lane == 0) warp_loss[warp] = 0.f;
+  int row_before = -1;
+  auto store_late = [&]() {
+    if (late_id[tid] >= 0) a.dlogits[(long long)row_before * a.ldd + late_id[tid]] = __float2bfloat16_rn(late_value[tid]);
+    late_id[tid] = -1;
+  };
+  if (ctas > 1) cluster_sync_all();                                                 // no CTA sends to one that has not started
+  auto send = [&](uint32_t turn, float m, float s, float s1, float tm, float ts) {
+    __syncwarp();
+    if (ctas == 1) {                                                                // (not launched as a cluster: st.async is for clusters)
+      if (lane == 0) {
+        all[turn][warp] = {m, s, s1, tm, ts, warp_loss[warp], 0.f, 0.f};
+        mbar_arrive(&got[turn]);
+      }
+    } else {
+      if (lane == 0) mbar_arrive_expect_tx(&got[turn], (uint32_t)ctas * sizeof(RingEntry));
+      if (lane < ctas) {
+        const uint32_t at = mapa_u32(smem_u32(&all[turn][rank * 8 + warp]), lane), bar = mapa_u32(smem_u32(&got[turn]), lane);
+        ring_send(at, bar, m, s, s1, tm);
+        ring_send(at + 16, bar, ts, warp_loss[warp], 0.f, 0.f);
+      }
+    }
+  };
+  auto write_loss = [&](const RingEntry* from) {                                    // of the row before, by one warp: in the order of the warps
+    float l = (lane < 8 * ctas ? from[lane].loss : 0.f) + (lane + 32 < 8 * ctas ? from[lane + 32].loss : 0.f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) a.loss[row_before] = l;
+  };
+  while (look()) {
+  long long id_now = -1;
+  float value = -INFINITY;
+  if (state[2] > 0) {
+    if (tid == 0) fetch(list[0]);      // (the part is free: thread 0 has waited for the row before)
+    id_now = entry_id(list[0]);
+    value = entry_value(list[0]);
+  }
+  for (int k = 0; k < state[3]; ++k) {
+    const int r = empty_rows[k];
+    bf16* drow = a.dlogits + (long long)r * a.ldd;
+    for (int i = i0 + tid; i < i0 + whole; i += 256) {
+      if (VEC == 8) *reinterpret_cast<uint4*>(drow + (long long)i * VEC) = make_uint4(0, 0, 0, 0);
+      else *reinterpret_cast<uint2*>(drow + (long long)i * VEC) = make_uint2(0, 0);
+    }
+    for (int i = max(v0, (i0 + whole) * VEC) + tid; i < (rank == ctas - 1 ? a.Vp : v1); i += 256) drow[i] = __float2bfloat16_rn(0.f);
+    if (tid == 0 && rank == 0) a.loss[r] = 0.f;
+  }
+  for (int at_row = 0; at_row < state[2]; ++at_row) {
+    const int r = list[at_row];
     bf16* drow = a.dlogits + (long long)r * a.ldd;
     if (rank == ctas - 1)
       for (int i = a.V + tid; i < a.Vp; i += 256) drow[i] = __float2bfloat16_rn(0.f);
-    if (w == 0.f) {
-      if (w_next != 0.f && tid == 0) fetch(next);                                   // (the part is free: thread 0 has waited for the row before it)
-      for (int i = i0 + tid; i < i0 + whole; i += 256) {
-        if (VEC == 8) *reinterpret_cast<uint4*>(drow + (long long)i * VEC) = make_uint4(0, 0, 0, 0);
-        else *reinterpret_cast<uint2*>(drow + (long long)i * VEC) = make_uint2(0, 0);
-      }
-      for (int i = max(v0, (i0 + whole) * VEC) + tid; i < v1; i += 256) drow[i] = __float2bfloat16_rn(0.f);
-      if (tid == 0 && rank == 0) a.loss[r] = 0.f;
-      w = w_next, w_next = w_then, id_now = id_next, id_next = id_then, value = value_next, value_next = value_then;
-      continue;
-    }
     const T* row = row_of(r);
     const uint32_t turn = steps & 1, phase = (steps >> 1) & 1;
     mbar_wait(&full, steps & 1);
@@ -449,45 +506,29 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       else x[k] = e;                                                                // the gradient is this, scaled
     }
     // this thread's entry; a NaN stays one
-    const float u = mine == -INFINITY ? 0.f : (mine - tm) * a.inv_tau, e = mine == -INFINITY ? 0.f : expf(u);
+    const float e = mine == -INFINITY ? 0.f : expf((mine - tm) * a.inv_tau);
     ids_of[turn][tid] = id;
     es_of[turn][tid] = e;
     if (here && tid < a.K) {
       const uint32_t bit = 1u << ((id - v0) & 31);
       if (atomicOr(&bits[(id - v0) >> 5], bit) & bit) twice[turn] = steps;
     }
-    RingEntry me;
-    {
-      float sum[7] = {(s4[0] + s4[1]) + (s4[2] + s4[3]), s1, here && e != 0.f ? e * (z - ref) : 0.f, here ? e : 0.f, here && tid == a.K ? z - ref : 0.f, e, e != 0.f ? e * u : 0.f};
-      const bool entries = warp * 32 <= a.K;                                        // this warp has some
+    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]), ts_mine = e;
 #pragma unroll
-      for (int k = 0; k < 7; ++k) {
-        if ((k == 1 && !BOTH) || (k > 1 && !entries)) continue;
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (BOTH) s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    }
+    if (warp * 32 < a.K)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
-      }
-      me = {m, sum[0], sum[1], tm, sum[2], sum[3], sum[4], sum[5], sum[6], 0.f, 0.f, 0.f};
-    }
-    __syncwarp();
-    if (ctas == 1) {                                                                // (not launched as a cluster: st.async is for clusters)
-      if (lane == 0) {
-        all[turn][warp] = me;
-        mbar_arrive(&got[turn]);
-      }
-    } else if (lane == 0) {
-      mbar_arrive_expect_tx(&got[turn], (uint32_t)ctas * sizeof(RingEntry));
-    }
-    if (ctas > 1 && lane < ctas) {
-      const uint32_t at = mapa_u32(smem_u32(&all[turn][rank * 8 + warp]), lane), bar = mapa_u32(smem_u32(&got[turn]), lane);
-      ring_send(at, bar, me.m, me.s, me.s1, me.tm);
-      ring_send(at + 16, bar, me.ez, me.e, me.zy, me.ts);
-      ring_send(at + 32, bar, me.eu, 0.f, 0.f, 0.f);
-    }
-    if (row_done >= 0) loss_of(all[turn ^ 1]);
+      for (int o = 16; o > 0; o >>= 1) ts_mine += __shfl_xor_sync(0xffffffffu, ts_mine, o);
+    send(turn, m, s, s1, tm, ts_mine);
+    const int next = at_row + 1 < state[2] ? list[at_row + 1] : rows;
+    const long long id_next = entry_id(next);
+    const float value_next = entry_value(next);
     mbar_wait(&got[turn], phase);
-    if (w_next != 0.f && tid == 0) fetch(next);                                     // all warps have read the part
-    if (late_at) *late_at = __float2bfloat16_rn(late);                              // ... and stored the row before
-    late_at = nullptr;
+    if (next < rows && tid == 0) fetch(next);                                       // all warps have read the part
+    store_late();                                                                   // ... and stored the row before
     if (steps > 1 && tid < a.K) {
       const int old = ids_of[turn ^ 1][tid];
       if (old >= v0 && old < v1) bits_before[(old - v0) >> 5] = 0;
@@ -495,6 +536,8 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     // the row's maximum and sums, from all warps of the cluster: two entries a lane
     const RingEntry* from = all[turn];
     const int n_from = 8 * ctas;
+    if (rank == 0 && warp == 7 && row_before >= 0) write_loss(from);
+    row_before = r;
     float4 f0 = make_float4(-INFINITY, 0.f, 0.f, 0.f), f1 = f0;
     if (lane < n_from) f0 = *reinterpret_cast<const float4*>(from + lane);
     if (lane + 32 < n_from) f1 = *reinterpret_cast<const float4*>(from + lane + 32);
@@ -514,12 +557,14 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     // the teacher's: of this CTA's warps, all of which have all entries' sums between them
     float t_top = -INFINITY, ts = 0.f;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) t_top = fmaxf(t_top, from[rank * 8 + q].tm);
+    for (int q = 0; q < 8; ++q)
+      if (q * 32 < a.K) t_top = fmaxf(t_top, from[rank * 8 + q].tm);
     auto teacher_scale = [&](float tmw) { return tmw == -INFINITY ? 1.f : di_ex2((tmw - t_top) * c); };
 #pragma unroll
     for (int q = 0; q < 8; ++q)
       if (q * 32 < a.K) ts += from[rank * 8 + q].ts * teacher_scale(from[rank * 8 + q].tm);
     const bool soft = !(ts == 0.f);
+    const float w = list_weight[at_row];
     RowGrad g;
     g.m = top;
     g.c = c;
@@ -561,20 +606,32 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
           }
       }
       if (writes && (share != 0.f || (label && g.ch != 0.f))) {
-        late_at = drow + id;
-        late = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
+        late_id[tid] = id;
+        late_value[tid] = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
       }
     }
-    __syncwarp();
-    if (rank == 0 && warp == 7) {
-      if (lane == 0) done = {S, S1, top, ts, t_top, ids[a.K]};
-      row_done = r;
+    if (warp * 32 <= a.K) {
+      float loss = 0.f;
+      if (here && tid < a.K && soft) {
+        const float lt = (value - t_top) * a.inv_tau - logf(ts), t = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm) / ts;
+        if (t != 0.f) loss = (1.f - a.hard) * a.tau * a.tau * t * (lt - (z - top) * a.inv_tau + logf(S));
+      }
+      if (here && tid == a.K && a.hard != 0.f) loss = a.hard * (logf(S1) - (z - top));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+      if (lane == 0) warp_loss[warp] = loss;
     }
-    w = w_next, w_next = w_then, id_now = id_next, id_next = id_then, value = value_next, value_next = value_then;
+    id_now = id_next, value = value_next;
   }
-  if (row_done >= 0) loss_of(all[(steps & 1) ^ 1]);
+  }
+  if (row_before >= 0) {                                                            // the last row's loss
+    const uint32_t turn = steps & 1;
+    send(turn, 0.f, 0.f, 0.f, 0.f, 0.f);
+    mbar_wait(&got[turn], (steps >> 1) & 1);
+    if (rank == 0 && warp == 7) write_loss(all[turn]);
+  }
   __syncthreads();
-  if (late_at) *late_at = __float2bfloat16_rn(late);
+  store_late();
 }
 
 // ---- longer rows: a CTA reads its row twice, the second time from the L2 ----------------------------------------------
