@@ -81,6 +81,12 @@ __device__ __forceinline__ float di_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// the largest of a warp's values (one that is not a number does not count)
+__device__ __forceinline__ float warp_top(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 // what a row's gradient is made of, once its maximum and sums are known
 struct RowGrad {
   float m, c, ks, kh;                       // maximum; log2(e) / tau; w (1 - h) tau / sum, w h / sum1
@@ -491,11 +497,8 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
     const float mine = id >= 0 && tid < a.K ? value : -INFINITY;
     float tm = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-    }
+    m = warp_top(m);
+    tm = warp * 32 < a.K ? warp_top(tm) : -INFINITY;
     const float ref = m == -INFINITY ? 0.f : m;
     float s4[4] = {0.f, 0.f, 0.f, 0.f}, s1 = 0.f;
 #pragma unroll
@@ -541,9 +544,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     float4 f0 = make_float4(-INFINITY, 0.f, 0.f, 0.f), f1 = f0;
     if (lane < n_from) f0 = *reinterpret_cast<const float4*>(from + lane);
     if (lane + 32 < n_from) f1 = *reinterpret_cast<const float4*>(from + lane + 32);
-    float top = fmaxf(f0.x, f1.x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float top = warp_top(fmaxf(f0.x, f1.x));
     auto against = [&](float mw, float scale) { return mw == -INFINITY ? 1.f : di_ex2((mw - top) * scale); };      // sums of a warp that has nothing are 0, or NaN
     float S = f0.y * against(f0.x, c) + f1.y * against(f1.x, c), S1 = BOTH ? f0.z * against(f0.x, LOG2E) + f1.z * against(f1.x, LOG2E) : 0.f;
 #pragma unroll
