@@ -15,6 +15,10 @@ Two kinds of per-request memory, both owned here and handed to the kernels as po
   (layer, slot).  A slot is not cleared when it is handed
   out again: the kernels start a request at position 0 from a zero state without reading the slot.
 
+A request may be FORKED: the new one shares the pages of the old one, each page counted, and has a slot of its own with a copy of the states.  A page that
+several requests hold is copied, in all pools at once, before one of them writes to it, and goes back to the pool when the last of them has given it back.
+A request may be TRUNCATED to fewer tokens, where it has no recurrent state and its window has not given back what the next token would see.
+
 Pools grow (by reallocation) when a batch needs more than the configured size; `max_tokens` only sizes the first allocation.
 """
 from __future__ import annotations
@@ -54,6 +58,7 @@ class SequenceCache:
         self.free_pages: List[int] = []
         self.free_slots: List[int] = []
         self.seqs: Dict[Hashable, Sequence] = {}
+        self.held: Dict[int, int] = {}     # pages that more than one request holds: by how many
         self.generation = 0                # bumped whenever a pool is reallocated (captured pointers become stale)
         self.keep_first = int(keep_first)
         # summary streams: one per distinct block size; summary pool k is pool summary_index[k][1] of stream summary_index[k][0]
@@ -70,6 +75,7 @@ class SequenceCache:
                                                          for w in ws] for ws in self.summary_widths]
         self.summary_n_pages: List[int] = [0] * len(self.summary_every)
         self.summary_free: List[List[int]] = [[] for _ in self.summary_every]
+        self.summary_held: List[Dict[int, int]] = [{} for _ in self.summary_every]
         for k, e in enumerate(self.summary_every):
             self._grow_summary(k, -(-max(int(max_tokens) // e, 1) // self.page_size) + max_seqs)
         if self.row_widths:
@@ -129,9 +135,10 @@ class SequenceCache:
         return self.seqs.get(key)
 
     def reserve(self, seq: Sequence, n_tokens: int) -> None:
-        """Make sure pages exist for positions [seq.length, seq.length + n_tokens) and for the blocks they complete."""
-        if not self.row_widths or (n_tokens == 1 and not self.summary_every and len(seq.pages) * self.page_size > seq.length):
+        """Make sure pages exist for positions [seq.length, seq.length + n_tokens) and for the blocks they complete, and that nobody else holds those pages."""
+        if not self.row_widths or (n_tokens == 1 and not self.summary_every and not self.held and len(seq.pages) * self.page_size > seq.length):
             return
+        self._own(seq, n_tokens)
         need = -(-(seq.length + n_tokens) // self.page_size)
         while len(seq.pages) < need:
             if not self.free_pages:
@@ -155,15 +162,109 @@ class SequenceCache:
         kept = -(-self.keep_first // self.page_size)           # pages that hold a token some layer keeps for ever
         for b in range(kept, min(len(seq.pages), max(first_needed, 0) // self.page_size)):
             if seq.pages[b] >= 0:
-                self.free_pages.append(seq.pages[b])
+                self._give_back(self.held, self.free_pages, seq.pages[b])
                 seq.pages[b] = -1
 
     def close(self, key: Hashable) -> None:
         seq = self.seqs.pop(key)
-        self.free_pages.extend(p for p in seq.pages if p >= 0)
+        for p in seq.pages:
+            if p >= 0:
+                self._give_back(self.held, self.free_pages, p)
         for k, pages in enumerate(seq.summary_pages):
-            self.summary_free[k].extend(pages)
+            for p in pages:
+                self._give_back(self.summary_held[k], self.summary_free[k], p)
         self.free_slots.append(seq.slot)
+
+    # ------------------------------------------------------------------ shared pages
+    @staticmethod
+    def _give_back(held: Dict[int, int], free: List[int], page: int) -> None:
+        n = held.get(page, 1)
+        if n == 1:
+            free.append(page)
+        elif n == 2:
+            del held[page]
+        else:
+            held[page] = n - 1
+
+    @staticmethod
+    def _copy_pages(pools: Seq[torch.Tensor], src: Seq[int], dst: Seq[int]) -> None:
+        """page src[i] of every pool to page dst[i]: pools of one width in one launch (on the CPU, where there are no kernels, by indexing)"""
+        for shape in {tuple(p.shape) for p in pools}:
+            alike = [p for p in pools if tuple(p.shape) == shape]
+            if alike[0].is_cuda:
+                from . import ops
+                s, d = (torch.tensor(list(x), dtype=torch.int32).pin_memory().to(alike[0].device, non_blocking=True) for x in (src, dst))
+                ops.cache_copy_pages(alike, s, d)
+            else:
+                for p in alike:
+                    p[list(dst)] = p[list(src)]
+
+    def _own(self, seq: Sequence, n_tokens: int) -> None:
+        """pages that the next n_tokens write to and that others hold too: copied, the copies are this request's"""
+        if self.held:
+            first, last = seq.length // self.page_size, (seq.length + n_tokens - 1) // self.page_size
+            shared = [b for b in range(first, min(last + 1, len(seq.pages))) if seq.pages[b] in self.held]
+            while len(self.free_pages) < len(shared):
+                self._grow_pages(max(8, self.n_pages // 2))
+            copies = [self.free_pages.pop() for _ in shared]
+            if shared:
+                self._copy_pages(self.pools, [seq.pages[b] for b in shared], copies)
+            for b, p in zip(shared, copies):
+                self._give_back(self.held, self.free_pages, seq.pages[b])
+                seq.pages[b] = p
+        for k, e in enumerate(self.summary_every):
+            pages, held = seq.summary_pages[k], self.summary_held[k]
+            first, end = seq.length // e, (seq.length + n_tokens) // e      # block rows that these tokens complete
+            shared = [b for b in range(first // self.page_size, min(-(-end // self.page_size), len(pages))) if pages[b] in held] if held and end > first else []
+            while len(self.summary_free[k]) < len(shared):
+                self._grow_summary(k, max(8, self.summary_n_pages[k] // 2))
+            copies = [self.summary_free[k].pop() for _ in shared]
+            if shared:
+                self._copy_pages(self.summary_pools[k], [pages[b] for b in shared], copies)
+            for b, p in zip(shared, copies):
+                self._give_back(held, self.summary_free[k], pages[b])
+                pages[b] = p
+
+    def fork(self, key: Hashable, new_key: Hashable) -> Sequence:
+        """A new request that continues from where `key` is: its pages are shared until one of the two writes to them, its states are copied."""
+        seq = self.seqs[key]
+        new = self.open(new_key)
+        new.length, new.pages, new.summary_pages = seq.length, list(seq.pages), [list(p) for p in seq.summary_pages]
+        for p in seq.pages:
+            if p >= 0:
+                self.held[p] = self.held.get(p, 1) + 1
+        for held, pages in zip(self.summary_held, seq.summary_pages):
+            for p in pages:
+                held[p] = held.get(p, 1) + 1
+        if seq.length and self.states:      # (a request at position 0 starts from a state of zeros, whatever its slot holds)
+            self._copy_pages([s.view(s.shape[0], 1, -1) for s in self.states], [seq.slot], [new.slot])
+        return new
+
+    def truncate(self, key: Hashable, length: int) -> None:
+        """The request keeps its first `length` tokens; pages behind them go back to the pools."""
+        seq = self.seqs[key]
+        if not 0 <= length <= seq.length:
+            raise ValueError(f"request {key!r} has {seq.length} tokens and cannot keep {length}")
+        if length == seq.length:
+            return
+        if length and self.states:
+            raise ValueError(f"request {key!r} has recurrent states, which cannot go back")
+        if length and self.window is not None:
+            kept = -(-self.keep_first // self.page_size)
+            for b in range(max(length - self.window + 1, 0) // self.page_size, (length - 1) // self.page_size + 1):
+                if b >= kept and seq.pages[b] < 0:
+                    raise ValueError(f"request {key!r}: tokens that position {length} would see have left the window and are gone")
+        need = -(-length // self.page_size)
+        for p in seq.pages[need:]:
+            if p >= 0:
+                self._give_back(self.held, self.free_pages, p)
+        del seq.pages[need:]
+        for k, e in enumerate(self.summary_every):
+            need = -(-(length // e) // self.page_size)
+            for p in seq.summary_pages[k][need:]:
+                self._give_back(self.summary_held[k], self.summary_free[k], p)
+            del seq.summary_pages[k][need:]
+        seq.length = length
 
     def live_tokens(self) -> int:
         return sum(s.length for s in self.seqs.values())

@@ -1849,3 +1849,12 @@ class SeqLMEngine:
     def finish(self, key: Hashable) -> None:
         """The request is over: its pages and its slot go back to the pools."""
         self.cache.close(key)
+
+    def fork(self, key: Hashable, new_key: Hashable) -> None:
+        """A new request that continues from the tokens of `key` (another sample of the same prompt, a branch of a search): the cache pages are shared until one of
+        the two writes to them, recurrent states are copied."""
+        self.cache.fork(key, new_key)
+
+    def truncate(self, key: Hashable, length: int) -> None:
+        """The request keeps its first `length` tokens (drafts that were refused are dropped); models with recurrent states cannot."""
+        self.cache.truncate(key, length)

@@ -115,12 +115,16 @@ class SFTTrainer:
 
     tokens / labels / loss_mask: [b, s] in the Megatron convention of mm_collate_fn (one -200 per image feature row,
     labels not shifted, loss_mask = the dataset's 'weights'); every sequence of the micro-batch has the same length s,
-    s % 8 == 0.  images: [N, 3, 364, 364] crops of the whole micro-batch in slot order."""
+    s % 8 == 0.  images: [N, 3, 364, 364] crops of the whole micro-batch in slot order.
+
+    Distillation: `tr.step(tokens, labels, loss_mask, images, teacher=(ids, logits))` trains on a teacher's K best tokens and their logits [b, s, K] at each position
+    (row (b, t): for token t + 1, weighted as that token's label is; ids outside the vocabulary are missing entries) instead of the labels, which keep the share
+    `distill_hard` of the loss; `distill_temperature` divides both sides' logits (ops.distill_fwd_bwd)."""
 
     def __init__(self, engine, lr: float = 1e-5, min_lr: float = 0.0, warmup_iters: int = 0, decay_iters: int = 0,
                  beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, weight_decay: float = 0.0,
                  clip_grad: float = 1.0, freeze_llm: bool = False, freeze_vision_tower: bool = True, process_group=None,
-                 attn_bwd: Optional[str] = None, recompute: str = "full"):
+                 attn_bwd: Optional[str] = None, recompute: str = "full", distill_temperature: float = 1.0, distill_hard: float = 0.0):
         if not torch.cuda.is_available():
             raise _lib.NativeError("leopard_b200 needs a CUDA device (sm_100a); there is no CPU fallback")
         _lib.lib()
@@ -128,6 +132,9 @@ class SFTTrainer:
         self.dev = engine.device
         self.hp = dict(lr=lr, min_lr=min_lr, warmup=warmup_iters, decay=decay_iters, beta1=beta1, beta2=beta2, eps=eps,
                        wd=weight_decay, clip=clip_grad)
+        if not distill_temperature > 0 or not 0 <= distill_hard <= 1:
+            raise ValueError(f"distill_temperature must be positive and distill_hard in [0, 1], got {distill_temperature} and {distill_hard}")
+        self.distill = (distill_temperature, distill_hard)
         self.freeze_llm = freeze_llm
         self.pg = process_group
         self.world = 1
@@ -507,15 +514,18 @@ class SFTTrainer:
 
     # ------------------------------------------------------------------ the step
     @torch.no_grad()
-    def step(self, tokens, labels, loss_mask, images):
+    def step(self, tokens, labels, loss_mask, images, teacher=None):
         """One iteration.  Each argument is a tensor (one micro-batch) or a list of them (gradient accumulation over
         get_num_microbatches() micro-batches, as Megatron's forward_backward_func does: every micro-batch loss is its own
         masked mean, divided by the number of micro-batches).  Returns (loss, grad_norm) as Python floats — the mean of the
-        micro-batch losses of this rank, and the global gradient norm before clipping; one device -> host read."""
+        micro-batch losses of this rank, and the global gradient norm before clipping; one device -> host read.
+        teacher: (ids, logits) [b, s, K] each, a list of such pairs with micro-batches, or None."""
         if isinstance(tokens, (list, tuple)):
-            micro = list(zip(tokens, labels, loss_mask, images))
+            if teacher is not None and len(teacher) != len(tokens):
+                raise ValueError(f"{len(tokens)} micro-batches need as many teachers, got {len(teacher)}")
+            micro = list(zip(tokens, labels, loss_mask, images, teacher if teacher is not None else [None] * len(tokens)))
         else:
-            micro = [(tokens, labels, loss_mask, images)]
+            micro = [(tokens, labels, loss_mask, images, teacher)]
         self.iteration += 1
         # the decoder's gradients are overwritten by the first micro-batch; the embedding's are added to, and the projector's and the
         # tower's stay zero in a step without images
@@ -566,7 +576,7 @@ class SFTTrainer:
             self.iteration -= 1      # (Megatron's found-inf path: the step does not count, optimizer.py:313-340)
         return out[0], out[1]
 
-    def _forward_backward(self, tokens, labels, loss_mask, images, n_micro: int, last: bool, handles: list):
+    def _forward_backward(self, tokens, labels, loss_mask, images, teacher, n_micro: int, last: bool, handles: list):
         """Forward, loss and backward of one micro-batch; gradients are written (first micro-batch) or added (later ones)
         into the flat buffer; on the last micro-batch every bucket's all-reduce is issued as soon as it is complete."""
         cfg, d, w = self.cfg, self.cfg.dec, self.w.named
@@ -575,6 +585,8 @@ class SFTTrainer:
         if s % 8:
             raise ValueError(f"sequence length {s} must be a multiple of 8")
         R = b * s
+        if teacher is not None and (len(teacher) != 2 or any(t.dim() != 3 or tuple(t.shape[:2]) != (b, s) for t in teacher) or teacher[0].shape != teacher[1].shape):
+            raise ValueError(f"teacher must be (ids, logits), each [{b}, {s}, K]")
         n_img_rows = int((tokens == cfg.megatron_image_index).sum())      # counted where the batch lives (the host): no device sync
         ids = tokens.reshape(-1).to(self.dev, torch.long).contiguous()
 
@@ -619,7 +631,12 @@ class SFTTrainer:
 
         # ---- loss and its gradient
         tgt, wt = shifted_targets(labels.to(self.dev), loss_mask.to(self.dev), self.world * n_micro)
-        loss_rows, dlogits = ops.ce_fwd_bwd(logits, tgt, wt, d.vocab)
+        if teacher is None:
+            loss_rows, dlogits = ops.ce_fwd_bwd(logits, tgt, wt, d.vocab)
+        else:
+            ids_t, logits_t = (t.to(self.dev).reshape(R, t.shape[-1]) for t in teacher)
+            temperature, hard = self.distill
+            loss_rows, dlogits = ops.distill_fwd_bwd(logits, ids_t, logits_t, wt, d.vocab, temperature=temperature, target=tgt if hard else None, hard=hard)
         del logits
         loss = torch.dot(loss_rows, wt) * (self.world * n_micro)     # this micro-batch's masked mean (what is reported)
 
