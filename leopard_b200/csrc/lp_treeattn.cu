@@ -44,9 +44,8 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM, g = lane >> 2, t4 = lane & 3;
   pdl_launch_dependents();
   tree_line(a, line);
-  const long long total = line[a.d.B].first;
-  long long u = tree_cut(total, blockIdx.x, a.ctas);
-  const long long u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
+  long long u, u_end;
+  tree_range(a, line, blockIdx.x, u, u_end);
 
   while (u < u_end) {
     const int b = tree_find(line, a.d.B, u);
@@ -303,12 +302,11 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
   const int b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * TA_JOIN_ROWS, in = threadIdx.x % TA_JOIN_ROWS, c4 = threadIdx.x / TA_JOIN_ROWS;
   tree_line(a, join_line);
   const TreeSeq s = tree_seq(a, join_line[b].len, join_line[b].n);
-  const long long total = join_line[a.d.B].first;
   const int rows = s.n * a.group;
   if (row0 >= rows) return;
   const int blk = row0 >> a.row_bits, r = row0 - (blk << a.row_bits) + in;      // (blocks are multiples of 16 rows)
-  const long long at = join_line[b].first + ((long long)kvh * s.blocks + blk) * s.tiles;
-  const int c0 = tree_cta_of(total, at, a.ctas), c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
+  int c0, c1;
+  tree_ctas_of(a, join_line, b, s, kvh * s.blocks + blk, c0, c1);
   if (c0 == c1) return;                                  // written whole
   const bool there = row0 + in < rows;
   pdl_wait();

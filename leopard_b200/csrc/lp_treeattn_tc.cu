@@ -20,7 +20,7 @@ constexpr int TT_BOX = 128 * 128;      // 128 rows x 64 bf16
 constexpr int TT_THREADS = 384;
 constexpr int TT_KEYS = 128;
 constexpr int TT_MAX_BATCH = 1024;      // sequences whose line of tiles fits beside the tiles
-constexpr int TT_SPLIT_BATCH = 32;      // sequences whose line of tiles leaves room for three stages
+constexpr int TT_SPLIT_BATCH = 24;      // sequences whose line of tiles leaves room for three stages
 
 #define LP_TT_TMEM_ST_16(regs, taddr)                                                                               \
   asm volatile(                                                                                                     \
@@ -141,8 +141,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   tc_fence_before();
   tree_line(a, line);                 // (ends in the block's barrier)
   tc_fence_after();
-  const long long total = line[a.d.B].first;
-  const long long u_begin = tree_cut(total, blockIdx.x, a.ctas), u_end = tree_cut(total, blockIdx.x + 1, a.ctas);
+  long long u_begin, u_end;
+  tree_range(a, line, blockIdx.x, u_begin, u_end);
   const uint32_t tmem_base = *tmem_at;
 
   if (warp == 0) {

@@ -19,7 +19,9 @@ inline T emu_shuffle(T v, int from) {
 }
 template <typename T>
 inline T emu_shfl(unsigned, T v, int lane) { return emu_shuffle(v, lane); }
-inline long long __shfl_up_sync(unsigned, long long v, int d) { return emu_shuffle(v, (int)(emu::linear_tid() & 31) - d); }
+template <typename T>
+inline T __shfl_up_sync(unsigned, T v, int d) { return emu_shuffle(v, (int)(emu::linear_tid() & 31) - d); }
+inline long long __shfl_xor_sync(unsigned, long long v, int m) { return emu_shuffle(v, (int)(emu::linear_tid() & 31) ^ m); }
 inline unsigned __ballot_sync(unsigned, bool p) {
   unsigned bits = 0;
   const unsigned t = emu::linear_tid(), w = t >> 5, l = t & 31;

@@ -52,12 +52,20 @@ def joined(c, out, part, ml, ctas, rows, want):
                 items.append((b, g, blk, n, first, tiles))
                 first += tiles
     cuts = [cut(first, i, ctas) for i in range(ctas + 1)]
-    for b, g, blk, n, at, tiles in items:
+    real = [it for it in items if it[5]]
+    owned = len(real) * 8 <= ctas                                # few items have CTAs of their own
+    next_cta = 0
+    for b, g, blk, n, at, tiles in real:
         mine = [i for i in range(ctas) if cuts[i] < at + tiles and cuts[i + 1] > at]
+        starts = [cuts[i] <= at for i in mine]
+        if owned:
+            own = min(tiles, 1 + tiles * (ctas - len(real)) // first)
+            mine, starts = list(range(next_cta, next_cta + own)), [i == 0 for i in range(own)]
+            next_cta += own
         if len(mine) < 2:
             continue
         for r in range(min(rows, n * group - blk * rows)):
-            slots = [2 * i + (1 if cuts[i] <= at else 0) for i in mine]
+            slots = [2 * i + int(x) for i, x in zip(mine, starts)]
             m, l = ml[slots, r, 0].double(), ml[slots, r, 1].double()
             f = torch.where(m == -torch.inf, 1.0, torch.exp2(m - m.max()))
             s = (l * f).sum()
@@ -126,6 +134,9 @@ def check(got, c, want, weight):
     (1, 150, 4, 2, 64, [127], None, 8, 4),                      # two blocks of rows, pages of eight
     (3, 34, 1, 1, 128, [1, 0, 255], [1, 0, 34], 0, 2),          # a sequence without nodes
     (2, 33, 2, 2, 64, [1100, 90], None, 64, 2),                 # many tiles a piece, rings that wrap
+    (1, 33, 2, 1, 64, [700], None, 64, 9),                      # an item with CTAs of its own
+    (2, 40, 1, 1, 64, [500, 20], [40, 0], 0, 20),               # ... beside a sequence without nodes
+    (3, 40, 1, 1, 64, [0, 260, 20], [0, 40, 33], 0, 17),
 ])
 def test_the_kernel_is_green_under_the_emulator(emu, B, T, H, G, D, lengths, nodes, page, ctas, split):
     c = case(B, T, H, G, D, lengths, nodes, page, T + D)
