@@ -31,7 +31,7 @@ __device__ __forceinline__ float ta_ex2(float x) {
 // a sequence's part of the line of tiles
 struct TreeSeq {
   int len, n, tiles, blocks;              // cached rows; nodes; tiles of an item; blocks of rows
-  long long keys;                         // rows that are there: cached and nodes', as far as the page table reaches
+  int keys;                               // rows that are there: cached and nodes', as far as the page table reaches (fewer than 2^31)
 };
 // what the line knows of a sequence: the tiles before it, its length and nodes, and its first CTA where items have CTAs of their own.
 // line[B]: all tiles; whether items have.
@@ -43,8 +43,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int len, int n) {
   TreeSeq s;
   s.n = n;
   s.len = len;
-  s.keys = min((long long)len + n, (long long)a.d.max_pages * a.d.page_size);
-  s.tiles = n ? (int)((unsigned)(s.keys + (1 << a.key_bits) - 1) >> a.key_bits) : 0;
+  s.keys = (int)min((long long)len + n, (long long)a.d.max_pages * a.d.page_size);
+  s.tiles = n ? (int)(((unsigned)s.keys + (1u << a.key_bits) - 1) >> a.key_bits) : 0;
   s.blocks = (n * a.group + a.rows - 1) >> a.row_bits;
   return s;
 }
@@ -65,7 +65,17 @@ __device__ __forceinline__ int tree_own(int tiles, long long total, int items, i
 constexpr int TREE_OWN = 8;               // CTAs an item from which on each has its own
 // by one warp, in shared memory.  Ends in the block's barrier.
 __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
-  if (threadIdx.x < 32) {
+  if (a.d.B == 1) {                       // one sequence: nothing to add up
+    if (threadIdx.x == 0) {
+      const int len = max(a.d.lengths[0], 0), n = a.d.nodes ? min(max(a.d.nodes[0], 0), a.d.T) : a.d.T;
+      const TreeSeq s = tree_seq(a, len, n);
+      const int items = s.tiles ? a.d.KVH * s.blocks : 0;
+      const long long all = (long long)items * s.tiles;
+      const bool owned = items * TREE_OWN <= a.ctas;
+      line[0] = {0, len, n, 0};
+      line[1] = {all, items, owned, owned && items ? items * tree_own(s.tiles, all, items, a.ctas) : 0};
+    }
+  } else if (threadIdx.x < 32) {
     long long run = 0, items = 0;
     for (int b0 = 0; b0 < a.d.B; b0 += 32) {
       const int b = b0 + threadIdx.x;

@@ -152,7 +152,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     for (long long u = u_begin; u < u_end;) {
       const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
-      const int n_keys = (int)p.s.keys;
+      const int n_keys = p.s.keys;
       int key = p.t0 * TT_KEYS + lane * tc.box;      // this lane's box of the tile
       TreePlace at(a, lane < boxes ? key : 0);
       auto page_of = [&]() { return lane < boxes && key < n_keys ? at.page(a, p.b) : -1; };
@@ -302,19 +302,31 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
       // its node's mask, when this piece gets there
       const int nw = (a.d.T + 63) >> 6;
-      unsigned long long word[2] = {0, 0};                             // SPLIT: two at most
-      unsigned long long* words = SPLIT ? word : mask_words + (q * 128 + r) * MAX_WORDS;
+      unsigned long long word0 = 0, word1 = 0;                         // SPLIT: two at most
+      unsigned long long* words = mask_words + (q * 128 + r) * MAX_WORDS;
       if ((p.t0 + p.n) * TT_KEYS > p.s.len) {
         const unsigned long long* src = a.d.mask + p.b * a.d.mask_batch + node * a.d.mask_node;
-#pragma unroll
-        for (int w = 0; w < MAX_WORDS; ++w)
-          if (w < nw) words[w] = src[w];
+        if (SPLIT) {
+          word0 = src[0];
+          if (nw > 1) word1 = src[1];
+        } else {
+          for (int w = 0; w < nw; ++w) words[w] = src[w];
+        }
       }
-      auto word_at = [&](int w) -> unsigned long long { return w >= nw ? 0ull : SPLIT ? (w == 0 ? word[0] : word[1]) : words[w]; };
+      auto word_at = [&](int w) -> unsigned long long { return w >= nw ? 0ull : SPLIT ? (w == 0 ? word0 : word1) : words[w]; };
       // which of a half's 64 keys there are, by their pages (known a step ahead)
       const int box = min(tc.box, 64), n_box = 64 / box;
-      const bool paged = a.d.page_table != nullptr;
-      const int n_keys = (int)p.s.keys, len = p.s.len;
+      const int n_keys = p.s.keys, len = p.s.len;
+      bool paged = a.d.page_table != nullptr;
+      if (paged) {                                                     // (all of the piece's pages there: no more looks)
+        const int from = p.t0 * TT_KEYS / a.d.page_size, to = (min((p.t0 + p.n) * TT_KEYS, n_keys) - 1) / a.d.page_size;
+        bool there = true;
+        for (int i = from + lane; i <= to; i += 32) {
+          const int page = a.d.page_table[p.b * a.d.ld_table + i];
+          there &= page >= 0 && page < a.d.n_pages;
+        }
+        paged = !__all_sync(0xffffffffu, there);
+      }
       int box_key = (p.t0 + j0) * TT_KEYS + lane * box;
       TreePlace box_at(a, paged && lane < n_box ? box_key : 0);
       auto page_there = [&]() { return !paged || lane >= n_box || box_key >= n_keys || box_at.page(a, p.b) >= 0; };
@@ -446,6 +458,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int tn = (t + 1) >> 1, hn = (t + 1) & 1;
         const bool has_next = t + 1 < 2 * mine;
         const bool s_ready = has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1);
+        if (both) {                                                    // the streams' exponentials in turns: one's loads and stores run beside the other's
+          if (q == 1) tt_bar_sync(5, 256);
+          else if (t > 0) tt_bar_sync(4, 256);
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
@@ -458,6 +474,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             pk[i >> 1] = pack_bf16x2(p0, p1);      // half a step is 2^-8 of a weight; their sum is taken in fp32 before
           }
           LP_TT_TMEM_ST_16(pk, s_addr + h * 64 + c * 16);
+        }
+        if (both) {
+          if (q == 0) tt_bar_arrive(5, 256);
+          else if (has_next) tt_bar_arrive(4, 256);
         }
         bool loaded = false;
         if (s_ready || (has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1))) {

@@ -31,6 +31,7 @@ inline unsigned __ballot_sync(unsigned, bool p) {
   __syncwarp();
   return bits;
 }
+inline bool __all_sync(unsigned m, bool p) { return __ballot_sync(m, p) == 0xffffffffu; }
 #define __shfl_sync emu_shfl
 inline float __bfloat162float(bf16 v) { return (float)v; }
 inline bool not_finite(float v) { return !(fabsf(v) <= 3.402823466e38f); }
