@@ -52,7 +52,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     const TreeSeq s = tree_seq(a, line[b].len, line[b].n);
     const long long local = u - line[b].first;
     const int item = (int)tree_div(local, s.tiles), t0 = (int)(local - (long long)item * s.tiles), t1 = (int)min((long long)s.tiles, t0 + (u_end - u));
-    const int kvh = item / s.blocks, r0 = (item - kvh * s.blocks) * R;
+    const int kvh = tree_div32(item, s.blocks), r0 = (item - kvh * s.blocks) * R;
     u += t1 - t0;
     const int n_rows = min(R, s.n * a.group - r0);
     const bf16* kb = reinterpret_cast<const bf16*>(a.d.k) + kvh * a.d.k_head;
@@ -64,9 +64,9 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
         const long long key = (long long)(t0 + i) * TA_KEYS + tid;
         int2 p = make_int2(-1, 0);
         if (key < s.keys) {
-          const long long logical = key / a.d.page_size;
+          const int logical = tree_div32((int)key, a.d.page_size);
           p.x = table ? table[logical] : b;
-          p.y = (int)(key - logical * a.d.page_size);
+          p.y = (int)key - logical * a.d.page_size;
           if (p.x >= a.d.n_pages) p.x = -1;
         }
         place[(i % TA_RING) * TA_KEYS + tid] = p;
@@ -104,7 +104,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
     for (int h = 0; h < 2; ++h) {
       const int r = r0 + wm * 16 + g + 8 * h;
       const bool there = r < s.n * a.group;
-      const int node = there ? r / a.group : 0, head = kvh * a.group + (there ? r % a.group : 0);
+      const int node = there ? tree_div32(r, a.group) : 0, head = kvh * a.group + (there ? r - node * a.group : 0);
       const bf16* q = reinterpret_cast<const bf16*>(a.d.q) + b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head;
       words[h] = a.d.mask + b * a.d.mask_batch + node * a.d.mask_node;
 #pragma unroll

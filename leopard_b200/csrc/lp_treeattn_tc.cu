@@ -68,14 +68,14 @@ __device__ __forceinline__ TreePiece tree_piece(const TreeArgs& a, const TreeLin
   const int item = (int)tree_div(local, p.s.tiles);
   p.t0 = (int)(local - (long long)item * p.s.tiles);
   p.n = (int)min((long long)(p.s.tiles - p.t0), u_end - u);
-  p.kvh = item / p.s.blocks;
+  p.kvh = tree_div32(item, p.s.blocks);
   p.r0 = (item - p.kvh * p.s.blocks) * a.rows;
   return p;
 }
 // where row `key` of a sequence lies: its place in the page table and in the page.  A sequence's rows are fewer than 2^31 (the entry point sees to it).
 struct TreePlace {
   int index, row;
-  __device__ __forceinline__ TreePlace(const TreeArgs& a, int key) : index(key / a.d.page_size), row(key - index * a.d.page_size) {}
+  __device__ __forceinline__ TreePlace(const TreeArgs& a, int key) : index(tree_div32(key, a.d.page_size)), row(key - index * a.d.page_size) {}
   __device__ __forceinline__ void forward(const TreeArgs& a, int keys) {
     for (row += keys; row >= a.d.page_size; ++index) row -= a.d.page_size;
   }
@@ -277,7 +277,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const bool both = !SPLIT && p.r0 + 128 < rows;                   // the other stream is at the same tiles
       const int row = row_base + r;
       const bool row_ok = row < rows;
-      const int node = row_ok ? row / a.group : 0, head = p.kvh * a.group + (row_ok ? row - node * a.group : 0);
+      const int node = row_ok ? tree_div32(row, a.group) : 0, head = p.kvh * a.group + (row_ok ? row - node * a.group : 0);
       // the warp's rows' queries, in the swizzled layout that TMA writes; 32 lanes take neighbouring pieces of 16 bytes
       if (!SPLIT || q == 0) {
         const long long from = p.b * a.d.q_batch + node * a.d.q_node + head * a.d.q_head;
@@ -286,14 +286,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
-          const long long src = __shfl_sync(0xffffffffu, from, rr);
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (row_base + lg * 32 + rr < rows) x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + src + c * 8);
+          const long long src = __shfl_sync(0xffffffffu, from, rr);      // (of a row that is not there the first node's: loads without branches go out together)
+          x[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.d.q) + src + c * 8);
         }
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const int rr = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
-          sts_u4(at + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), x[i]);
+          sts_u4(at + (c >> 3) * TT_BOX + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), row_base + lg * 32 + rr < rows ? x[i] : make_uint4(0, 0, 0, 0));
         }
         if (DH % 64 != 0)
           for (int c = CH; c < NB * 8; ++c) sts_u4(at + (c >> 3) * TT_BOX + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), make_uint4(0, 0, 0, 0));
@@ -319,7 +318,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const int n_keys = p.s.keys, len = p.s.len;
       bool paged = a.d.page_table != nullptr;
       if (paged) {                                                     // (all of the piece's pages there: no more looks)
-        const int from = p.t0 * TT_KEYS / a.d.page_size, to = (min((p.t0 + p.n) * TT_KEYS, n_keys) - 1) / a.d.page_size;
+        const int from = tree_div32(p.t0 * TT_KEYS, a.d.page_size), to = tree_div32(min((p.t0 + p.n) * TT_KEYS, n_keys) - 1, a.d.page_size);
         bool there = true;
         for (int i = from + lane; i <= to; i += 32) {
           const int page = a.d.page_table[p.b * a.d.ld_table + i];
