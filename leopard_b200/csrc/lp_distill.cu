@@ -676,25 +676,31 @@ distill_long_kernel(const __grid_constant__ DistillArgs a) {
   row_loss(a, r, soft, m, s, s1, row, top, lt, id, y, red);
 }
 
-// clusters that run at once: two CTAs an SM, as far as clusters fit the GPU's groups of SMs
-template <typename Kernel>
-static cudaError_t launch_ring(Kernel kernel, const DistillArgs& a, int rows, int ctas, size_t smem, cudaStream_t stream) {
-  if (cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaError_t rc = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg)) return rc;
-  if (n < 1) n = 1;
+// clusters that run at once: two CTAs an SM, as far as clusters fit the GPU's groups of SMs (asked once a kernel, device and size of cluster: 7 us)
+template <auto Kernel>
+static cudaError_t launch_ring(const DistillArgs& a, int rows, int ctas, size_t smem, cudaStream_t stream) {
+  static std::atomic<int> fit[64][9];
+  int dev = 0, n = 0;
+  if (const cudaError_t rc = cudaGetDevice(&dev)) return rc;
+  if (const cudaError_t rc = allow_smem<Kernel>((int)smem)) return rc;
+  if (dev < 64) n = fit[dev][ctas].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (const cudaError_t rc = cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg)) return rc;
+    if (n < 1) n = 1;
+    if (dev < 64) fit[dev][ctas].store(n, std::memory_order_relaxed);
+  }
   if (n > rows) n = rows;
-  return launch_ex(kernel, dim3((unsigned)(n * ctas)), dim3(256), smem, stream, ctas, false, a, ctas, rows);
+  return launch_ex(Kernel, dim3((unsigned)(n * ctas)), dim3(256), smem, stream, ctas, false, a, ctas, rows);
 }
 
 }  // namespace lp
@@ -726,7 +732,7 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
     cudaError_t rc;
     if (wide && K <= RING_TOP) {
       const size_t part = (size_t)256 * DISTILL_HELD * size;
-#define LP_RING(T) rc = both ? launch_ring(distill_ring_kernel<T, true>, a, rows, ctas, part, stream) : launch_ring(distill_ring_kernel<T, false>, a, rows, ctas, part, stream)
+#define LP_RING(T) rc = both ? launch_ring<distill_ring_kernel<T, true>>(a, rows, ctas, part, stream) : launch_ring<distill_ring_kernel<T, false>>(a, rows, ctas, part, stream)
       if (logits_fp32) LP_RING(float);
       else LP_RING(bf16);
 #undef LP_RING

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <atomic>
 #include "lp_pdl.cuh"
 
 namespace lp {
@@ -131,6 +132,21 @@ inline cudaError_t launch_next(void (*kern)(KArgs...), dim3 grid, dim3 block, si
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_attention(long long work, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
   return work < 50000 ? launch_next(kern, grid, block, smem, stream, args...) : launch_ex(kern, grid, block, smem, stream, 1, false, args...);
+}
+
+// lets a kernel have `bytes` of dynamic shared memory; asked of the driver once a kernel, device and size (0.7 us)
+template <auto Kernel>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<int> have[64];
+  int dev = 0;
+  if (const cudaError_t rc = cudaGetDevice(&dev)) return rc;
+  if (dev < 64 && have[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  const cudaError_t rc = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc == cudaSuccess && dev < 64) {
+    int old = have[dev].load(std::memory_order_relaxed);
+    while (old < bytes && !have[dev].compare_exchange_weak(old, bytes)) {}
+  }
+  return rc;
 }
 
 // launch accounting + optional per-launch CUDA-event timing (off by default; see lp_profile_* in the public header)

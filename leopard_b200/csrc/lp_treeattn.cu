@@ -426,7 +426,7 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   note_launch(2);
 #define LP_TREE(DD, WM, WN)                                                                                                                    \
   {                                                                                                                                            \
-    LP_CHECK_CUDA(cudaFuncSetAttribute(tree_attn_kernel<DD, WM, WN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                 \
+    LP_CHECK_CUDA((allow_smem<tree_attn_kernel<DD, WM, WN>>((int)smem)));                                                                      \
     tree_attn_kernel<DD, WM, WN><<<a.ctas, 128, smem, stream>>>(a);                                                                            \
   }
 #define LP_TREE_D(DD)                                                                                                                          \

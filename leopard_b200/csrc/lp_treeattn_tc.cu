@@ -624,9 +624,13 @@ static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
   }
   const bool split = d.B <= TT_SPLIT_BATCH && tc.a.rows <= 128;
   const size_t smem = (split ? 7 : 6) * NB * TT_BOX + 256 + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * sizeof(TreeLine) + 1024;
-  auto kernel = split ? tree_tc_kernel<DH, true> : tree_tc_kernel<DH, false>;
-  LP_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+  if (split) {
+    LP_CHECK_CUDA((allow_smem<tree_tc_kernel<DH, true>>((int)smem)));
+    tree_tc_kernel<DH, true><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+  } else {
+    LP_CHECK_CUDA((allow_smem<tree_tc_kernel<DH, false>>((int)smem)));
+    tree_tc_kernel<DH, false><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+  }
   LP_CHECK_CUDA(cudaGetLastError());
   return 0;
 }
