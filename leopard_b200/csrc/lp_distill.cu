@@ -87,6 +87,14 @@ __device__ __forceinline__ float warp_top(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+// Exponents in the exponent's own units: z c - m c in one fma, where m c is rounded once and cancels out of every quotient: its rounding shifts the exponents by 2^-25 |m c|, 64 at most
+// up to 2^31.  Beyond that (a mask of -1e10, say) unequal logits are 64 apart at least after a factor c, and only those equal to the maximum count: a factor of a power of two above c
+// (far below it where the product would overflow) says as much, and its product is exact.
+__device__ __forceinline__ float factor_at(float m, float c) {
+  return fabsf(m * c) <= 2147483648.f || m == -INFINITY ? c : fabsf(m) > 1e30f ? 0x1p-40f : __uint_as_float((__float_as_uint(c) & 0x7f800000u) + 0x00800000u);
+}
+// minus a maximum in those units; 0 of nothing
+__device__ __forceinline__ float in_units(float m, float c) { return m == -INFINITY ? 0.f : -__fmul_rn(m, c); }      // (not to be contracted: all uses have one rounding)
 // what a row's gradient is made of, once its maximum and sums are known
 struct RowGrad {
   float m, c, ks, kh;                       // maximum; log2(e) / tau; w (1 - h) tau / sum, w h / sum1
@@ -283,6 +291,8 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 // It has one wait: every WARP sends its maximum and sums, against its own maximum, to all CTAs of the cluster (st.async on a barrier of the receiver), and takes the
 // row's from the 8 x CTAs entries that arrive.  (Block sums, a barrier of the cluster and sums of sums took 4 of 7 us a row; the barrier alone 0.7, since it waits for the
 // row before to be stored.)  A warp's part of the row's loss, which needs the row's sums, goes along with the next row's.
+// Measured: 4,096 rows of 128,256 fp32 logits, 64 entries, 518 us, 6.1 TB/s of logits read and gradient written (a copy's rate would be 489); 2,048 x 32,000, the label too, 70.7
+// (60.9); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
 constexpr int RING_TOP = 255;
 constexpr int RING_LIST = 1536, RING_LOOK = 1024;      // rows that a cluster knows to be its own; weights that are looked at at once
 struct __align__(16) RingEntry {             // of a warp: maximum and sums of the row; the teacher's maximum
@@ -298,7 +308,7 @@ template <typename T, bool BOTH>
 __global__ void __launch_bounds__(256, 2)
 distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   constexpr int VEC = 16 / sizeof(T), N = DISTILL_HELD / VEC;
-  constexpr float LOG2E = 1.4426950408889634f;
+  constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   extern __shared__ __align__(128) unsigned char ring_smem[];
   T* part = reinterpret_cast<T*>(ring_smem);                                       // [256 x DISTILL_HELD]
   // (what the rows write in turn: a warp that is at the next row but one has seen that all have sent for the next one, and so are done with this one)
@@ -341,6 +351,10 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     return a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at] : (float)reinterpret_cast<const bf16*>(a.teacher)[at];
   };
   for (int i = tid; i < 3 * 256 * DISTILL_HELD / 32; i += 256) (&bits_of[0][0])[i] = 0;
+  for (int v = whole * VEC + tid; v < 256 * DISTILL_HELD; v += 256) part[v] = (T)-INFINITY;      // copies never reach there
+  // the row's last values, where they are fewer than 16 bytes, are brought by the thread that their piece falls to
+  const int tail = v1 - min(v1, (i0 + whole) * VEC);
+  const bool tail_here = tail > 0 && tid == whole % 256;
   if (tid == 0) {
     twice[0] = twice[1] = 0;
     mbar_init(&full, 1);
@@ -466,47 +480,53 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     uint32_t* bits = bits_of[steps % 3];
     uint32_t* bits_before = bits_of[(steps + 2) % 3];
     ++steps;
-    float x[DISTILL_HELD];
+    if (tail_here)
+      for (int e = 0; e < tail; ++e) part[whole * VEC + e] = row[(i0 + whole) * VEC + e];
+    // pairs of values, in two-wide arithmetic, loads and stores at fixed offsets: what bounds a row is the instructions of its 64 values a thread (1,180 a warp and row with single
+    // values, a branch a load and z - max taken before the factor: 699 us instead of 518 for 4,096 x 128,256 of fp32)
+    float2 x[DISTILL_HELD / 2];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int i = k * 256 + tid;
-      if (i < whole) {
-        const uint4 u = lds_u4(part + (long long)i * VEC);
-        if (sizeof(T) == 4) {
-          x[k * VEC] = __uint_as_float(u.x); x[k * VEC + 1] = __uint_as_float(u.y); x[k * VEC + 2] = __uint_as_float(u.z); x[k * VEC + 3] = __uint_as_float(u.w);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
-            x[k * VEC + (2 * e) % VEC] = __uint_as_float(h << 16);
-            x[k * VEC + (2 * e + 1) % VEC] = __uint_as_float(h & 0xffff0000u);
-          }
-        }
+      const uint4 u = lds_u4(part + (k * 256 + tid) * VEC);
+      if (sizeof(T) == 4) {
+        x[k * VEC / 2] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+        x[k * VEC / 2 + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
       } else {
-        const int v = (i0 + i) * VEC;                                               // the row's last values, fewer than 16 bytes; else nothing
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[k * VEC + e] = i0 + i < i1 && v + e < a.V ? (float)row[v + e] : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
+          x[(k * VEC / 2 + e) % (DISTILL_HELD / 2)] = make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+        }
       }
     }
     const int id = id_now >= 0 && id_now < a.V ? (int)id_now : -1;
     const bool here = id >= v0 && id < v1;
     const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
-    float m4[4] = {x[0], x[1], x[2], x[3]};
+    float m4[4] = {x[0].x, x[0].y, x[1].x, x[1].y};
 #pragma unroll
-    for (int k = 4; k < DISTILL_HELD; ++k) m4[k & 3] = fmaxf(m4[k & 3], x[k]);
+    for (int k = 2; k < DISTILL_HELD / 2; ++k) {
+      m4[(k & 1) * 2] = fmaxf(m4[(k & 1) * 2], x[k].x);
+      m4[(k & 1) * 2 + 1] = fmaxf(m4[(k & 1) * 2 + 1], x[k].y);
+    }
     float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
     const float mine = id >= 0 && tid < a.K ? value : -INFINITY;
     float tm = mine;
     m = warp_top(m);
     tm = warp * 32 < a.K ? warp_top(tm) : -INFINITY;
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s4[4] = {0.f, 0.f, 0.f, 0.f}, s1 = 0.f;
+    // exponents against the maximum in the exponent's own units, rounded once: c m here and wherever the warp's sums are used
+    const float cm = factor_at(m, c), lm = factor_at(m, LOG2E), ref = in_units(m, cm), lref = in_units(m, lm);
+    const float2 cm2 = make_float2(cm, cm), ref2 = make_float2(ref, ref), one = make_float2(1.f, 1.f), lm2 = make_float2(lm, lm), lref2 = make_float2(lref, lref);
+    float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < DISTILL_HELD; ++k) {
-      const float d = x[k] - ref, e = di_ex2(d * c);
-      s4[k & 3] += e;
-      if (BOTH) s1 += di_ex2(d * LOG2E);
-      else x[k] = e;                                                                // the gradient is this, scaled
+    for (int k = 0; k < DISTILL_HELD / 2; ++k) {
+      const float2 y = fma2(x[k], cm2, ref2), e = make_float2(di_ex2(y.x), di_ex2(y.y));
+      s2[k & 1] = fma2(e, one, s2[k & 1]);
+      if (BOTH) {
+        const float2 y1 = fma2(x[k], lm2, lref2);
+        t2 = fma2(make_float2(di_ex2(y1.x), di_ex2(y1.y)), one, t2);
+      } else {
+        x[k] = e;                                                                   // the gradient is this, scaled
+      }
     }
     // this thread's entry; a NaN stays one
     const float e = mine == -INFINITY ? 0.f : expf((mine - tm) * a.inv_tau);
@@ -516,7 +536,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       const uint32_t bit = 1u << ((id - v0) & 31);
       if (atomicOr(&bits[(id - v0) >> 5], bit) & bit) twice[turn] = steps;
     }
-    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]), ts_mine = e;
+    float s = (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y), s1 = t2.x + t2.y, ts_mine = e;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -545,8 +565,9 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     if (lane < n_from) f0 = *reinterpret_cast<const float4*>(from + lane);
     if (lane + 32 < n_from) f1 = *reinterpret_cast<const float4*>(from + lane + 32);
     const float top = warp_top(fmaxf(f0.x, f1.x));
-    auto against = [&](float mw, float scale) { return mw == -INFINITY ? 1.f : di_ex2((mw - top) * scale); };      // sums of a warp that has nothing are 0, or NaN
-    float S = f0.y * against(f0.x, c) + f1.y * against(f1.x, c), S1 = BOTH ? f0.z * against(f0.x, LOG2E) + f1.z * against(f1.x, LOG2E) : 0.f;
+    const float ct = factor_at(top, c), lt = factor_at(top, LOG2E), up = in_units(top, ct), lup = in_units(top, lt);
+    auto against = [&](float mw, float f, float u) { return mw == -INFINITY ? 1.f : di_ex2(u - in_units(mw, f)); };      // (sums of a warp that has nothing are 0, or NaN)
+    float S = f0.y * against(f0.x, ct, up) + f1.y * against(f1.x, ct, up), S1 = BOTH ? f0.z * against(f0.x, lt, lup) + f1.z * against(f1.x, lt, lup) : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       S += __shfl_xor_sync(0xffffffffu, S, o);
@@ -566,32 +587,38 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       if (q * 32 < a.K) ts += from[rank * 8 + q].ts * teacher_scale(from[rank * 8 + q].tm);
     const bool soft = !(ts == 0.f);
     const float w = list_weight[at_row];
-    RowGrad g;
-    g.m = top;
-    g.c = c;
-    g.cs = soft ? w * (1.f - a.hard) * a.tau : 0.f;
-    g.ch = has_label ? w * a.hard : 0.f;
-    g.ks = g.cs / S;
-    g.kh = g.ch / S1;
-    const float down = !BOTH ? (g.ks + g.kh) * against(m, c) : 0.f;
+    const float cs = soft ? w * (1.f - a.hard) * a.tau : 0.f, ch = has_label ? w * a.hard : 0.f;
+    const float ks = __fdividef(cs, S), kh = __fdividef(ch, S1);                    // (2^-22 of the value; S lies in [1, V])
+    auto grad = [&](float z) {
+      float g = ks != 0.f ? di_ex2(fmaf(z, ct, up)) * ks : 0.f;
+      if (kh != 0.f) g += di_ex2(fmaf(z, lt, lup)) * kh;
+      return g;
+    };
+    const float down = !BOTH ? (ks + kh) * against(m, ct, up) : 0.f;
+    const float2 down2 = make_float2(down, down), c2 = make_float2(ct, ct), l2 = make_float2(lt, lt), up2 = make_float2(up, up), lup2 = make_float2(lup, lup);
+    const float2 ks2 = make_float2(ks, ks), kh2 = make_float2(kh, kh);
+    bf16* out = drow + (long long)(i0 + tid) * VEC;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int i = k * 256 + tid;
+      uint32_t p[VEC / 2];
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) x[k * VEC + q] = BOTH ? g.at(x[k * VEC + q]) : x[k * VEC + q] * down;
-      const long long v = (long long)(i0 + i) * VEC;
-      if (i < whole) {
-        if (VEC == 8)
-          *reinterpret_cast<uint4*>(drow + v) = make_uint4(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]),
-                                                           pack_bf16x2(x[k * VEC + 4 % VEC], x[k * VEC + 5 % VEC]), pack_bf16x2(x[k * VEC + 6 % VEC], x[k * VEC + 7 % VEC]));
-        else
-          *reinterpret_cast<uint2*>(drow + v) = make_uint2(pack_bf16x2(x[k * VEC], x[k * VEC + 1 % VEC]), pack_bf16x2(x[k * VEC + 2 % VEC], x[k * VEC + 3 % VEC]));
-      } else {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q)
-          if (i0 + i < i1 && v + q < a.V) drow[v + q] = __float2bfloat16_rn(x[k * VEC + q]);
+      for (int q = 0; q < VEC / 2; ++q) {
+        float2 y = x[k * VEC / 2 + q];
+        if (BOTH) {
+          const float2 e = fma2(y, c2, up2), e1 = fma2(y, l2, lup2);
+          y = fma2(make_float2(di_ex2(e.x), di_ex2(e.y)), ks2, mul2(make_float2(di_ex2(e1.x), di_ex2(e1.y)), kh2));
+        } else {
+          y = mul2(y, down2);
+        }
+        p[q] = pack_bf16x2(y.x, y.y);
+      }
+      if (k * 256 + tid < whole) {
+        if (VEC == 8) *reinterpret_cast<uint4*>(out + k * 256 * VEC) = make_uint4(p[0], p[1], p[2 % (VEC / 2)], p[3 % (VEC / 2)]);
+        else *reinterpret_cast<uint2*>(out + k * 256 * VEC) = make_uint2(p[0], p[1]);
       }
     }
+    if (tail_here)
+      for (int e = 0; e < tail; ++e) drow[(i0 + whole) * VEC + e] = __float2bfloat16_rn(grad((float)part[whole * VEC + e]));
     // the places that entries name lose the teacher's share, the label's its own.  Of entries with one id the first writes, of the label and entries these.
     if (here) {
       const uint32_t word = (id - v0) >> 5, bit = 1u << ((id - v0) & 31);
@@ -606,18 +633,18 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
             share += es_of[turn][o] * teacher_scale(from[rank * 8 + (o >> 5)].tm);
           }
       }
-      if (writes && (share != 0.f || (label && g.ch != 0.f))) {
+      if (writes && (share != 0.f || (label && ch != 0.f))) {
         late_id[tid] = id;
-        late_value[tid] = g.at(z) - (soft ? g.cs * (share / ts) : 0.f) - (label ? g.ch : 0.f);
+        late_value[tid] = grad(z) - (soft ? cs * (share / ts) : 0.f) - (label ? ch : 0.f);
       }
     }
     if (warp * 32 <= a.K) {
       float loss = 0.f;
       if (here && tid < a.K && soft) {
-        const float lt = (value - t_top) * a.inv_tau - logf(ts), t = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm) / ts;
-        if (t != 0.f) loss = (1.f - a.hard) * a.tau * a.tau * t * (lt - (z - top) * a.inv_tau + logf(S));
+        const float log_t = (value - t_top) * a.inv_tau - logf(ts), t = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm) / ts;
+        if (t != 0.f) loss = (1.f - a.hard) * a.tau * a.tau * t * (log_t - (ct == c ? fmaf(z, c, up) * LN2 : (z - top) * a.inv_tau) + logf(S));
       }
-      if (here && tid == a.K && a.hard != 0.f) loss = a.hard * (logf(S1) - (z - top));
+      if (here && tid == a.K && a.hard != 0.f) loss = a.hard * (logf(S1) - (lt == LOG2E ? fmaf(z, lt, lup) * LN2 : z - top));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
       if (lane == 0) warp_loss[warp] = loss;

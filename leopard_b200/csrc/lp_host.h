@@ -136,7 +136,7 @@ inline cudaError_t launch_attention(long long work, void (*kern)(KArgs...), dim3
 
 // lets a kernel have `bytes` of dynamic shared memory; asked of the driver once a kernel, device and size (0.7 us)
 template <auto Kernel>
-inline cudaError_t allow_smem(int bytes) {
+static cudaError_t allow_smem(int bytes) {      // (static: two libraries of these sources in one process each have their own kernels to ask for)
   static std::atomic<int> have[64];
   int dev = 0;
   if (const cudaError_t rc = cudaGetDevice(&dev)) return rc;

@@ -596,6 +596,29 @@ def test_distill_of_logits_that_are_not_finite():
 
 
 @gpu
+@pytest.mark.parametrize("V, dtype, kw", [(40000, torch.float32, dict()), (40000, BF16, dict(hard=0.4, temperature=1.5)), (3001, torch.float32, dict(hard=1.0)),
+                                          (140000, BF16, dict(hard=0.3, temperature=0.5)), (128256, torch.float32, dict(temperature=0.01))])
+def test_distill_of_tokens_masked_by_large_values(V, dtype, kw):
+    """Whole stretches at a mask's value, down to the type's lowest: as if they were -inf.  A row that is all mask is a row of equal logits."""
+    c = distill_case(4, V, 6, V, dtype, share=2.0)
+    c["ids"] %= 100
+    c["target"] %= 100
+    kept = torch.arange(V, device="cuda") < 2000
+    want = ops.distill_fwd_bwd(vocab=V, **{**c, "logits": c["logits"].masked_fill(~kept, -float("inf"))}, **kw)
+    assert bool(want[0].isfinite().all() and want[1].isfinite().all())
+    for mask in (-1e6, -1e10, -1e30, torch.finfo(dtype).min):
+        got = ops.distill_fwd_bwd(vocab=V, **{**c, "logits": c["logits"].masked_fill(~kept, mask)}, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), mask
+        d = ops.distill_fwd_bwd(vocab=V, **{**c, "logits": torch.full_like(c["logits"], mask)}, **kw)
+        equal = ops.distill_fwd_bwd(vocab=V, **{**c, "logits": torch.zeros_like(c["logits"])}, **kw)
+        # equal logits z have equal exponents s, which need not be 0: z / tau ln^-1 2 is rounded once, |s| <= 2^-25 of it and <= 64.  2^s cancels out of p but for the roundings
+        # of a sum and a quotient, so a gradient is the same before its rounding to bf16 within 2^-20: one step after it.  The loss has -s ln 2 + log(V 2^s): a rounding each of
+        # 2^-23 (64 + log V), and 2^s is off by 2^-21.
+        assert bool(((d[0] - equal[0]).abs() <= 2.0 ** -15 + 2.0 ** -22 * equal[0].abs()).all()), mask
+        assert bool(((d[1].double() - equal[1].double()).abs() <= 2.0 ** -7 * equal[1].double().abs()).all()), mask
+
+
+@gpu
 @pytest.mark.parametrize("temperature, hard", [(1.0, 0.0), (1.7, 0.35)])
 def test_distill_gradient_against_differences(temperature, hard):
     """central differences of the 64-bit loss over whole directions (the loss is smooth: their error is of the step's square)"""
