@@ -291,65 +291,91 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   }
 }
 
-// Rows whose tiles lie in several CTAs: a CTA joins 8 rows of a key head, a thread four columns of a row over all pieces.  Bound by latency: TA_JOIN_DEEP pieces are under way
-// at once, and their weights follow a running maximum, so that each is read once.
-constexpr int TA_JOIN_ROWS = 8, TA_JOIN_DEEP = 10;
-template <int D>
-__global__ void __launch_bounds__(TA_JOIN_ROWS * D / 4)
-tree_join_kernel(const __grid_constant__ TreeArgs a) {
-  extern __shared__ TreeLine join_line[];
-  __shared__ __align__(16) bf16 done[TA_JOIN_ROWS][D + 8];
-  const int b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * TA_JOIN_ROWS, in = threadIdx.x % TA_JOIN_ROWS, c4 = threadIdx.x / TA_JOIN_ROWS;
-  tree_line(a, join_line);
-  const TreeSeq s = tree_seq(a, join_line[b].len, join_line[b].n);
-  const int rows = s.n * a.group;
-  if (row0 >= rows) return;
-  const int blk = row0 >> a.row_bits, r = row0 - (blk << a.row_bits) + in;      // (blocks are multiples of 16 rows)
-  int c0, c1;
-  tree_ctas_of(a, join_line, b, s, kvh * s.blocks + blk, c0, c1);
-  if (c0 == c1) return;                                  // written whole
-  const bool there = row0 + in < rows;
-  pdl_wait();
+// Rows whose tiles lie in several CTAs: a CTA joins groups of 8 rows of a key head, a thread four columns of a row over all pieces.  Bound by latency: ten pieces of a group, two
+// of each of four or five of each of two are under way at once; weights follow a running maximum, so that each is read once.  A CTA takes 1 to 2 us for the line of tiles before it can
+// join.  Few CTAs have done so when the pieces' kernel ends; of more than run at once (8 an SM) each takes four groups (64 nodes of 48 sequences of 1,000 rows 121 us in all, 161
+// with one; 26 nodes of 6 sequences, 624 CTAs with one group, 44.8 with one and 50.9 with four).
+constexpr int TA_JOIN_ROWS = 8, TA_JOIN_GROUPS = 4;
+template <int N>
+struct TreeN { static constexpr int value = N; };
+struct TreeSum {
   float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = c0; base <= c1; base += TA_JOIN_DEEP) {
-    float4 y[TA_JOIN_DEEP];
-    float2 p[TA_JOIN_DEEP];
-#pragma unroll
-    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
-      const bool on = there && base + k <= c1;
-      const long long slot = 2LL * (base + k) + (base + k == c0 ? 1 : 0);      // the first piece begins with the item, the others begin inside it
-      p[k] = on ? a.part_ml[slot * a.rows + r] : make_float2(-INFINITY, 0.f);
-      y[k] = on ? *reinterpret_cast<const float4*>(a.part_o + ((slot * (D / 4) + c4) * a.rows + r) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+  template <int N>
+  __device__ __forceinline__ void add(const float2* p, const float4* y) {
     float m = top;
 #pragma unroll
-    for (int k = 0; k < TA_JOIN_DEEP; ++k) m = fmaxf(m, p[k].x);
+    for (int k = 0; k < N; ++k) m = fmaxf(m, p[k].x);
     const float old = top == -INFINITY ? 1.f : ta_ex2(top - m);      // sums and values of pieces that saw nothing are zeros, or NaN
     top = m;
     sum *= old;
     x.x *= old; x.y *= old; x.z *= old; x.w *= old;
 #pragma unroll
-    for (int k = 0; k < TA_JOIN_DEEP; ++k) {
+    for (int k = 0; k < N; ++k) {
       const float f = p[k].x == -INFINITY ? 1.f : ta_ex2(p[k].x - m);
       sum += p[k].y * f;
       x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint2*>(&done[in][c4 * 4]) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-  __syncthreads();
-  if (threadIdx.x < TA_JOIN_ROWS * (D / 8)) {
-    const int row = row0 + threadIdx.x / (D / 8), col = (threadIdx.x % (D / 8)) * 8;
-    if (row < rows) {
-      bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + (row / a.group) * a.d.o_node + (kvh * a.group + row % a.group) * a.d.o_head;
-      *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(&done[threadIdx.x / (D / 8)][col]);
+  __device__ __forceinline__ uint2 result() const {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    return make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  }
+};
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(TA_JOIN_ROWS * D / 4)
+tree_join_kernel(const __grid_constant__ TreeArgs a) {
+  extern __shared__ TreeLine join_line[];
+  __shared__ __align__(16) bf16 done[GROUPS * TA_JOIN_ROWS][D + 8];
+  const int b = blockIdx.z, kvh = blockIdx.y, row0 = blockIdx.x * TA_JOIN_ROWS * GROUPS, in = threadIdx.x % TA_JOIN_ROWS, c4 = threadIdx.x / TA_JOIN_ROWS;
+  tree_line(a, join_line);
+  const TreeSeq s = tree_seq(a, join_line[b].len, join_line[b].n);
+  const int rows = min(s.n * a.group, row0 + TA_JOIN_ROWS * GROUPS);
+  const int blk = row0 >> a.row_bits, r0 = row0 - (blk << a.row_bits) + in;      // (blocks are multiples of a CTA's rows, or there is one)
+  int c0 = 0, c1 = 0;
+  if (row0 < rows) tree_ctas_of(a, join_line, b, s, kvh * s.blocks + blk, c0, c1);
+  if (c0 != c1 || blockIdx.x + blockIdx.y + blockIdx.z == 0) pdl_wait();      // (the first in any case: the join may not be over before the pieces' kernel is)
+  if (c0 == c1) return;                                  // nothing, or written whole
+  auto load = [&](int row, int c, float2& p, float4& y) {
+    const bool on = row + in < rows && c <= c1;
+    const long long slot = 2LL * c + (c == c0 ? 1 : 0);  // the first piece begins with the item, the others begin inside it
+    const int r = r0 + row - row0;
+    p = on ? a.part_ml[slot * a.rows + r] : make_float2(-INFINITY, 0.f);
+    y = on ? *reinterpret_cast<const float4*>(a.part_o + ((slot * (D / 4) + c4) * a.rows + r) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  auto join = [&](auto groups, auto pieces) {             // so many at once
+    constexpr int NG = decltype(groups)::value, NP = decltype(pieces)::value;
+    for (int row = row0; row < rows; row += NG * TA_JOIN_ROWS) {
+      TreeSum t[NG];
+      for (int c = c0; c <= c1; c += NP) {
+        float2 p[NG][NP];
+        float4 y[NG][NP];
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int k = 0; k < NP; ++k) load(row + i * TA_JOIN_ROWS, c + k, p[i][k], y[i][k]);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) t[i].template add<NP>(p[i], y[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) *reinterpret_cast<uint2*>(&done[row - row0 + i * TA_JOIN_ROWS + in][c4 * 4]) = t[i].result();
     }
+  };
+  if constexpr (GROUPS == 1) join(TreeN<1>(), TreeN<10>());
+  else if (c1 - c0 < 2) join(TreeN<4>(), TreeN<2>());
+  else join(TreeN<2>(), TreeN<5>());
+  __syncthreads();
+  for (int i = threadIdx.x; i < (rows - row0) * (D / 8); i += TA_JOIN_ROWS * D / 4) {
+    const int row = row0 + i / (D / 8), col = (i % (D / 8)) * 8;
+    bf16* out = reinterpret_cast<bf16*>(a.d.out) + b * a.d.o_batch + (row / a.group) * a.d.o_node + (kvh * a.group + row % a.group) * a.d.o_head;
+    *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(&done[row - row0][col]);
   }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-// which kernel: tcgen05 for more rows than TREE_TC_ROWS where it takes the cache
+// which kernel: tcgen05 for more rows than TREE_TC_ROWS where it takes the cache.  mma.sync and tcgen05 (us, 32 heads over 8, nodes x 4 rows): 16 rows of one sequence of 512 rows
+// 9.7 and 12.2, 8 of 1,000 18.6 and 20.3, 48 of 1,000 56 and 69, 48 of 4,000 152 and 170; 32 rows 10.1 and 12.1, 20.1 and 20.6, 71 and 74, 197 and 176; 36 rows 11.5 and 12.1, 24.7
+// and 20.7, 97 and 76, 274 and 179; 128 rows 12.4 and 12.7, 48 and 31, 207 and 111, 542 and 208.
 constexpr int TREE_TC_ROWS = 32;
 static bool tree_tc(const lp_tree_attn_desc* d) { return (long long)d->T * (d->H / d->KVH) > TREE_TC_ROWS && tree_tc_takes(d); }
 // rows of a block: what the widest tree needs, 64 (256) at most
@@ -422,21 +448,29 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * a.rows * d->D);
   const bool tc = tree_tc(d);
   const int wm = tc ? 1 : a.rows / 16, wn = 4 / wm;
-  const size_t smem = tree_smem(d->D, wm, wn, d->B);
+  const size_t smem = tree_smem(d->D, wm, wn, d->B), line = (size_t)(d->B + 1) * sizeof(TreeLine);
+  dim3 join((unsigned)(((long long)d->T * a.group + TA_JOIN_ROWS - 1) / TA_JOIN_ROWS), d->KVH, d->B);
+  const int groups = (long long)join.x * join.y * join.z <= 8LL * sm_count() ? 1 : TA_JOIN_GROUPS;
+  join.x = (join.x + groups - 1) / groups;
   note_launch(2);
 #define LP_TREE(DD, WM, WN)                                                                                                                    \
   {                                                                                                                                            \
     LP_CHECK_CUDA((allow_smem<tree_attn_kernel<DD, WM, WN>>((int)smem)));                                                                      \
     tree_attn_kernel<DD, WM, WN><<<a.ctas, 128, smem, stream>>>(a);                                                                            \
   }
+#define LP_JOIN(DD, GG)                                                                                                                        \
+  {                                                                                                                                            \
+    LP_CHECK_CUDA((allow_smem<tree_join_kernel<DD, GG>>((int)line)));                                                                          \
+    LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD, GG>, join, dim3(TA_JOIN_ROWS * DD / 4), line, stream, 1, true, a));                           \
+  }
 #define LP_TREE_D(DD)                                                                                                                          \
   if (tc) { if (const int rc = launch_tree_tc(a, stream)) return rc; }                                                                          \
   else if (wm == 1) LP_TREE(DD, 1, 4) else if (wm == 2) LP_TREE(DD, 2, 2) else LP_TREE(DD, 4, 1)                                                    \
   LP_CHECK_CUDA(cudaGetLastError());                                                                                                           \
-  LP_CHECK_CUDA(launch_ex(tree_join_kernel<DD>, dim3((unsigned)(((long long)d->T * a.group + TA_JOIN_ROWS - 1) / TA_JOIN_ROWS), d->KVH, d->B), \
-                          dim3(TA_JOIN_ROWS * DD / 4), (size_t)(d->B + 1) * sizeof(TreeLine), stream, 1, true, a));
+  if (groups == 1) LP_JOIN(DD, 1) else LP_JOIN(DD, TA_JOIN_GROUPS)
   if (d->D == 128) { LP_TREE_D(128) } else if (d->D == 96) { LP_TREE_D(96) } else { LP_TREE_D(64) }
 #undef LP_TREE_D
+#undef LP_JOIN
 #undef LP_TREE
   return 0;
 }

@@ -1,9 +1,10 @@
 // leopard_b200 — attention of a tree of drafted tokens over a cache: what the kernels of lp_treeattn.cu and lp_treeattn_tc.cu share.
 //
 // The keys of an item (sequence, key head, block of rows) are cut into tiles; the tiles of all items stand in one line, of which every CTA takes an equal range: sequences
-// of any lengths load all SMs alike.  Few items are dealt out whole: each has CTAs of its own, as many as its tiles are a share of all, since a range that goes on in another
-// item costs the ends of two pieces (6 us; 26 nodes after 4,796 rows, 8 items on 148 CTAs, 19.7 and TREEALIGNED).  Where a CTA's range ends inside an item its rows' running
-// maximum, sum and weighted values go to the workspace, to be joined.  Which CTAs an item has follows from the lengths alone, in every kernel.
+// of any lengths load all SMs alike.  Few items are dealt out whole, each with CTAs of its own, where the longest range is then little above an equal share: a range that goes on
+// in another item costs the ends of two pieces, and a split item its join (26 nodes of 11 sequences of up to 5,000 rows 49.8 us and 53.7 without, 64 nodes of them 65 and 81; one
+// node after 4,796 rows 16.3 and 20.8).  Where a CTA's range ends inside an item its rows' running maximum, sum and weighted values go to the workspace, to be joined.  Which CTAs
+// an item has follows from the lengths alone, in every kernel.
 #pragma once
 #include "lp_common.cuh"
 #include "lp_host.h"
@@ -34,7 +35,7 @@ struct TreeSeq {
   int keys;                               // rows that are there: cached and nodes', as far as the page table reaches (fewer than 2^31)
 };
 // what the line knows of a sequence: the tiles before it, its length and nodes, and its first CTA where items have CTAs of their own.
-// line[B]: all tiles; whether items have.
+// line[B]: all tiles; how many an item's CTAs have at most (0: items have none of their own).
 struct TreeLine {
   long long first;
   int len, n, cta;
@@ -70,11 +71,13 @@ __device__ __forceinline__ int tree_cta_of(long long total, long long unit, int 
   const long long each = tree_div(total, ctas), more = total - each * ctas;      // the first `more` CTAs have one tile more
   return unit < (each + 1) * more ? (int)tree_div(unit, each + 1) : (int)(more + tree_div(unit - (each + 1) * more, each));
 }
-// CTAs of an item of `tiles` tiles, where there are `items` of them: one, and of the others as many as its share
-__device__ __forceinline__ int tree_own(int tiles, long long total, int items, int ctas) {
-  return (int)min((long long)tiles, 1 + tree_div((long long)tiles * (ctas - items), total));
-}
-constexpr int TREE_OWN = 8;               // CTAs an item from which on each has its own
+// CTAs of an item of `tiles` tiles, where items have CTAs of their own: `most` tiles each
+__device__ __forceinline__ int tree_own(int tiles, int most) { return tree_div32(tiles + most - 1, most); }
+// For items to have CTAs of their own the longest range may have this many tiles above an equal share: of 64 and of 128 keys, the latter looked for in steps of two.  A tile is 1 to
+// 2 us, the end of a piece and its join 6 to 12 (64 nodes of 12 sequences of 3,000 rows, 8.4 tiles above: 79.9 and 76.5 as a line; of 10, 11 above: 79.8 and 66.7; of 14 of 1,000
+// rows, 1.8 above: 41.6 and 65).
+constexpr int TREE_SLACK = 3, TREE_SLACK_TC = 6;
+__device__ __forceinline__ int tree_slack(const TreeArgs& a) { return a.key_bits == 7 ? TREE_SLACK_TC : TREE_SLACK; }
 // by one warp, in shared memory.  Ends in the block's barrier.
 __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
   if (a.d.B == 1) {                       // one sequence: nothing to add up
@@ -83,12 +86,17 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
       const TreeSeq s = tree_seq(a, len, n);
       const int items = s.tiles ? a.d.KVH * s.blocks : 0;
       const long long all = (long long)items * s.tiles;
-      const bool owned = items * TREE_OWN <= a.ctas;
+      int most = 0;
+      if (items <= a.ctas && all > a.ctas) {      // (of fewer tiles than CTAs each has its own in any case)
+        most = tree_own(s.tiles, tree_div32(a.ctas, items));
+        if (most > tree_div(all, a.ctas) + tree_slack(a)) most = 0;
+      }
       line[0] = {0, len, n, 0};
-      line[1] = {all, items, owned, owned && items ? items * tree_own(s.tiles, all, items, a.ctas) : 0};
+      line[1] = {all, 0, most, most ? items * tree_own(s.tiles, most) : 0};
     }
   } else if (threadIdx.x < 32) {
     long long run = 0, items = 0;
+    int my_items = 0, my_tiles = 0;       // of the first 32 sequences
     for (int b0 = 0; b0 < a.d.B; b0 += 32) {
       const int b = b0 + threadIdx.x;
       long long mine = 0, own = 0;
@@ -99,6 +107,7 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
         line[b].n = n;
         own = s.tiles ? (long long)a.d.KVH * s.blocks : 0;
         mine = own * s.tiles;
+        if (b0 == 0) my_items = (int)own, my_tiles = s.tiles;
       }
       long long sum = mine;
 #pragma unroll
@@ -112,15 +121,24 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
       for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
       items += own;
     }
-    const bool owned = items * TREE_OWN <= a.ctas;
-    if (owned) {                          // (then there are at most ctas / TREE_OWN sequences of any tiles)
+    int most = 0;
+    if (items <= a.ctas && run > a.ctas && a.d.B <= 32) {        // (a lane a sequence) the least number of tiles for which the CTAs are enough
+      const int share = (int)tree_div(run, a.ctas), step = a.key_bits == 7 ? 2 : 1;
+#pragma unroll
+      for (int k = 7; k >= 0; --k) {
+        const int m = share + 1 + k * step;
+        const int ctas = __reduce_add_sync(0xffffffffu, (unsigned)(my_items * tree_own(my_tiles, m)));
+        if (ctas <= a.ctas && m <= share + tree_slack(a)) most = m;
+      }
+    }
+    if (most) {
       int at = 0;
       for (int b0 = 0; b0 < a.d.B; b0 += 32) {
         const int b = b0 + threadIdx.x;
         int mine = 0;
         if (b < a.d.B) {
           const TreeSeq s = tree_seq(a, line[b].len, line[b].n);
-          if (s.tiles) mine = a.d.KVH * s.blocks * tree_own(s.tiles, run, (int)items, a.ctas);
+          if (s.tiles) mine = a.d.KVH * s.blocks * tree_own(s.tiles, most);
         }
         int sum = mine;
 #pragma unroll
@@ -135,8 +153,7 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
     }
     if (threadIdx.x == 0) {
       line[a.d.B].first = run;
-      line[a.d.B].len = (int)min(items, (long long)a.ctas);
-      line[a.d.B].n = owned;
+      line[a.d.B].n = most;
     }
   }
   __syncthreads();
@@ -154,22 +171,22 @@ __device__ __forceinline__ void tree_range(const TreeArgs& a, const TreeLine* li
   int b = a.d.B - 1;
   while (line[b].cta > cta) --b;          // (a sequence without tiles has no CTAs: its first one is the next sequence's)
   const TreeSeq s = tree_seq(a, line[b].len, line[b].n);
-  const int own = tree_own(s.tiles, total, line[a.d.B].len, a.ctas), item = tree_div32(cta - line[b].cta, own), k = cta - line[b].cta - item * own;
+  const int own = tree_own(s.tiles, line[a.d.B].n), item = tree_div32(cta - line[b].cta, own), k = cta - line[b].cta - item * own;
   const long long first = line[b].first + (long long)item * s.tiles;
   from = first + tree_cut(s.tiles, k, own);
   to = first + tree_cut(s.tiles, k + 1, own);
 }
 // the CTAs that an item of sequence b (its item-th) lies in
 __device__ __forceinline__ void tree_ctas_of(const TreeArgs& a, const TreeLine* line, int b, const TreeSeq& s, int item, int& c0, int& c1) {
-  const long long total = line[a.d.B].first;
-  if (!line[a.d.B].n) {
-    const long long at = line[b].first + (long long)item * s.tiles;
-    c0 = tree_cta_of(total, at, a.ctas);
-    c1 = tree_cta_of(total, at + s.tiles - 1, a.ctas);
+  const TreeLine &its = line[b], &all = line[a.d.B];
+  if (!all.n) {
+    const long long at = its.first + (long long)item * s.tiles;
+    c0 = tree_cta_of(all.first, at, a.ctas);
+    c1 = tree_cta_of(all.first, at + s.tiles - 1, a.ctas);
     return;
   }
-  const int own = tree_own(s.tiles, total, line[a.d.B].len, a.ctas);
-  c0 = line[b].cta + item * own;
+  const int own = tree_own(s.tiles, all.n);
+  c0 = its.cta + item * own;
   c1 = c0 + own - 1;
 }
 __device__ __forceinline__ int tree_find(const TreeLine* line, int B, long long unit) {      // the sequence that `unit` belongs to

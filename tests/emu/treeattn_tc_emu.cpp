@@ -31,6 +31,10 @@ inline unsigned __ballot_sync(unsigned, bool p) {
   __syncwarp();
   return bits;
 }
+inline unsigned __reduce_add_sync(unsigned, unsigned v) {
+  for (int m = 1; m < 32; m <<= 1) v += emu_shuffle(v, (int)(emu::linear_tid() & 31) ^ m);
+  return v;
+}
 inline bool __all_sync(unsigned m, bool p) { return __ballot_sync(m, p) == 0xffffffffu; }
 #define __shfl_sync emu_shfl
 inline float __bfloat162float(bf16 v) { return (float)v; }

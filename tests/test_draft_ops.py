@@ -291,6 +291,13 @@ def test_one_page_of_many_sequences():
 
 
 @gpu
+@pytest.mark.parametrize("B, T, H, G, D", [(2048, 1, 2, 1, 64), (1024, 20, 4, 2, 64), (1025, 33, 1, 1, 96)])
+def test_the_largest_batches(B, T, H, G, D):
+    c = attention_case(B, T, H, G, D, [(i * 37) % 90 for i in range(B)], page=16, seed=B)
+    close(attend(c), c)
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """a pool of 4.5 GB: its last pages lie past 2^32 bytes and 2^31 elements"""
     pages = 70000

@@ -53,13 +53,19 @@ def joined(c, out, part, ml, ctas, rows, want):
                 first += tiles
     cuts = [cut(first, i, ctas) for i in range(ctas + 1)]
     real = [it for it in items if it[5]]
-    owned = len(real) * 8 <= ctas                                # few items have CTAs of their own
+    most = 0                                                     # few items have CTAs of their own: of this many tiles, if that is little above an equal share
+    if real and len(real) <= ctas < first:
+        if B == 1:
+            most = -(-real[0][5] // (ctas // len(real)))
+            most = 0 if most > first // ctas + 6 else most
+        else:
+            most = next((m for m in range(first // ctas + 1, first // ctas + 7, 2) if sum(-(-it[5] // m) for it in real) <= ctas), 0)
     next_cta = 0
     for b, g, blk, n, at, tiles in real:
         mine = [i for i in range(ctas) if cuts[i] < at + tiles and cuts[i + 1] > at]
         starts = [cuts[i] <= at for i in mine]
-        if owned:
-            own = min(tiles, 1 + tiles * (ctas - len(real)) // first)
+        if most:
+            own = -(-tiles // most)
             mine, starts = list(range(next_cta, next_cta + own)), [i == 0 for i in range(own)]
             next_cta += own
         if len(mine) < 2:
