@@ -87,7 +87,8 @@ __device__ __forceinline__ void tree_line(const TreeArgs& a, TreeLine* line) {
       const int items = s.tiles ? a.d.KVH * s.blocks : 0;
       const long long all = (long long)items * s.tiles;
       int most = 0;
-      if (items <= a.ctas && all > a.ctas) {      // (of fewer tiles than CTAs each has its own in any case)
+      // (of fewer tiles than CTAs each has its own in any case; of few of 128 keys the sums take longer than they give: 26 nodes after 4,796 rows 21.5 us and 22, after 20,000 34.4 and 27)
+      if (items <= a.ctas && all > (a.key_bits == 7 ? 4LL : 1LL) * a.ctas) {
         most = tree_own(s.tiles, tree_div32(a.ctas, items));
         if (most > tree_div(all, a.ctas) + tree_slack(a)) most = 0;
       }

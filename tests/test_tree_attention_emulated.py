@@ -54,7 +54,7 @@ def joined(c, out, part, ml, ctas, rows, want):
     cuts = [cut(first, i, ctas) for i in range(ctas + 1)]
     real = [it for it in items if it[5]]
     most = 0                                                     # few items have CTAs of their own: of this many tiles, if that is little above an equal share
-    if real and len(real) <= ctas < first:
+    if real and len(real) <= ctas and first > (4 if B == 1 else 1) * ctas:
         if B == 1:
             most = -(-real[0][5] // (ctas // len(real)))
             most = 0 if most > first // ctas + 6 else most
@@ -140,7 +140,8 @@ def check(got, c, want, weight):
     (1, 150, 4, 2, 64, [127], None, 8, 4),                      # two blocks of rows, pages of eight
     (3, 34, 1, 1, 128, [1, 0, 255], [1, 0, 34], 0, 2),          # a sequence without nodes
     (2, 33, 2, 2, 64, [1100, 90], None, 64, 2),                 # many tiles a piece, rings that wrap
-    (1, 33, 2, 1, 64, [700], None, 64, 9),                      # an item with CTAs of its own
+    (1, 33, 2, 1, 64, [700], None, 64, 9),                      # few tiles a CTA
+    (1, 33, 1, 1, 64, [1400], None, 64, 2),                     # an item with CTAs of its own
     (2, 40, 1, 1, 64, [500, 20], [40, 0], 0, 20),               # ... beside a sequence without nodes
     (3, 40, 1, 1, 64, [0, 260, 20], [0, 40, 33], 0, 17),
 ])
