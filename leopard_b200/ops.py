@@ -543,6 +543,8 @@ def _need(t, name, dtypes, dim=None, shape=None, device=None, contiguous=False, 
         raise ValueError(f"{name} must be contiguous")
     if rows and t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
+    if rows and t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: its rows must not share their memory")
 
 
 def _overlaps(a, b):
@@ -623,7 +625,7 @@ def tree_attention(q, k, v, lengths, mask, nodes=None, page_table=None, scale=No
         if page_table is not None:
             max_pages = page_table.shape[1]
             fine = (fine and page_table.dtype is _I32 and page_table.device == dev and page_table.shape == (B, max_pages)
-                    and (page_table.stride(1) == 1 or max_pages <= 1))
+                    and (page_table.stride(1) == 1 or max_pages <= 1) and (page_table.stride(0) >= max_pages or B == 1))
             table, ld = page_table.data_ptr(), max(page_table.stride(0), max_pages)
         else:
             fine, max_pages, table, ld = fine and P >= B, 1, None, 0
@@ -727,12 +729,12 @@ def cache_compact(pools, lengths, path, count, page_table=None):
     P, S, W = shape
     try:
         B, T = path.shape
-        fine = (path.dtype is _I32 and path.device == dev and (path.stride(1) == 1 or T == 1) and lengths.dtype is _I32 and lengths.device == dev and lengths.shape == (B,)
+        fine = (path.dtype is _I32 and path.device == dev and (path.stride(1) == 1 or T == 1) and (path.stride(0) >= T or B == 1) and lengths.dtype is _I32 and lengths.device == dev and lengths.shape == (B,)
                 and lengths.is_contiguous() and count.dtype is _I32 and count.device == dev and count.shape == (B,) and count.is_contiguous() and (st[2] == 1 or W == 1))
         if page_table is not None:
             max_pages = page_table.shape[1]
             fine = (fine and page_table.dtype is _I32 and page_table.device == dev and page_table.shape == (B, max_pages)
-                    and (page_table.stride(1) == 1 or max_pages <= 1))
+                    and (page_table.stride(1) == 1 or max_pages <= 1) and (page_table.stride(0) >= max_pages or B == 1))
             table, ld = page_table.data_ptr(), max(page_table.stride(0), max_pages)
         else:
             max_pages, table, ld = 1, None, 0
@@ -794,7 +796,8 @@ def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target
         K, dev = ids.shape[1], logits.device
         fine = (logits.is_cuda and (logits.dtype is _F32 or logits.dtype is _BF16) and logits.stride(1) == 1 and (ids.dtype is _I64 or ids.dtype is _I32)
                 and (teacher.dtype is _F32 or teacher.dtype is _BF16) and ids.shape == (R, K) and teacher.shape == (R, K) and ids.device == dev and teacher.device == dev
-                and (K <= 1 or (ids.stride(1) == 1 and teacher.stride(1) == 1)) and weight.dtype is _F32 and weight.shape == (R,) and weight.device == dev
+                and (K <= 1 or (ids.stride(1) == 1 and teacher.stride(1) == 1))
+                and (R <= 1 or (logits.stride(0) >= Vp and ids.stride(0) >= K and teacher.stride(0) >= K)) and weight.dtype is _F32 and weight.shape == (R,) and weight.device == dev
                 and weight.is_contiguous() and 0 < vocab <= Vp
                 and (target is None or (target.dtype is _I64 and target.shape == (R,) and target.device == dev and target.is_contiguous())))
     except (AttributeError, ValueError, IndexError):

@@ -661,6 +661,27 @@ def test_distill_of_views_and_refusals():
     assert empty[0].shape == (0,) and empty[1].shape == (0, 90)
 
 
+@gpu
+def test_rows_that_share_their_memory():
+    """strides of zero are followed where the call takes a stride, and refused where a row's length is the least distance"""
+    c = attention_case(3, 5, 4, 2, 64, [40, 7, 22], page=16, seed=30)
+    same = dict(q=c["q"][:1].expand(3, -1, -1, -1), lengths=c["lengths"])
+    got = ops.tree_attention(same["q"], c["k"], c["v"], c["lengths"], O.tree_words(c["sees"])[:1].expand(3, -1, -1).cuda(), None, c["page_table"])
+    close(got, {**c, "q": same["q"], "sees": c["sees"][:1].expand(3, -1, -1)})
+    with pytest.raises(ValueError, match="page_table"):
+        attend(c, page_table=c["page_table"][:1].expand(3, -1))
+    with pytest.raises(ValueError, match="parents"):
+        ops.tree_mask(random_parents(1, 5, 1).cuda().expand(3, -1))
+    pools, lengths, path, count, table = compact_case(3, 5, 16, 8, BF16, 2, 3, [40, 7, 22])
+    for change in (dict(path=path[:1].expand(3, -1)), dict(page_table=table[:1].expand(3, -1))):
+        with pytest.raises(ValueError, match="share"):
+            ops.cache_compact(pools, **{**dict(lengths=lengths, path=path, count=count, page_table=table), **change})
+    d = distill_case(3, 40, 4, 1)
+    for name in ("logits", "ids", "teacher"):
+        with pytest.raises(ValueError, match=name):
+            ops.distill_fwd_bwd(vocab=40, **{**d, name: d[name][:1].expand(3, -1)})
+
+
 # ------------------------------------------------------------------------------------------------------------ streams, graphs
 @gpu
 def test_calls_on_other_streams_and_in_graphs():
