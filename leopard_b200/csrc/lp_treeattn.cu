@@ -198,7 +198,7 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
           l[h] += sc[j][2 * h] + sc[j][2 * h + 1];
         }
       }
-      // the weights go into the second product as bf16 (half a step is 2^-9 of a weight); their sum was taken before
+      // the weights go into the second product as bf16 (half a step is 2^-8 of a weight); their sum was taken before
       bool odd = false;
 #pragma unroll
       for (int j = 0; j < NK / 16; ++j) {
