@@ -721,3 +721,33 @@ def test_calls_on_other_streams_and_in_graphs():
     before = pools.clone()
     g.replay()
     assert torch.equal(pools, torch.stack([O.cache_compact(p, *rest) for p in before]))
+
+
+@gpu
+def test_calls_at_once_on_streams_and_from_threads():
+    """the same operators on two streams, launched by two threads, side by side: what each gives alone"""
+    import threading
+    work = []
+    for i in range(2):
+        a = attention_case(3, 40 if i else 5, 8, 2, 128, [900, 40, 2000], page=64, seed=40 + i)
+        v = verify_case(4, 9, 40000, 41 + i)
+        d = distill_case(60, 40000, 20, 42 + i)
+        words = O.tree_words(a["sees"]).cuda()
+        work.append(lambda a=a, v=v, d=d, words=words: [ops.tree_attention(a["q"], a["k"], a["v"], a["lengths"], words, a["nodes"], a["page_table"]), *ops.verify_draft(**v),
+                                                        *ops.distill_fwd_bwd(vocab=40000, **d)])
+    want = [w() for w in work]
+    torch.cuda.synchronize()
+    got, streams = [[], []], [torch.cuda.Stream() for _ in range(2)]
+
+    def run(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                got[i].append(work[i]())
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert len(g) == 20 and all(torch.equal(x, y) for one in g for x, y in zip(one, w))
