@@ -487,29 +487,26 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       for (int e = 0; e < tail; ++e) part[whole * VEC + e] = row[(i0 + whole) * VEC + e];
     // pairs of values, in two-wide arithmetic, loads and stores at fixed offsets: what bounds a row is the instructions of its 64 values a thread (1,180 a warp and row with single
     // values, a branch a load and z - max taken before the factor: 699 us instead of 518 for 4,096 x 128,256 of fp32)
-    float2 x[DISTILL_HELD / 2];
+    uint4 raw[N];                                                                   // (as they come: bf16 pairs are taken apart where they are used)
+    constexpr int HELD_PAIRS = !BOTH && sizeof(T) == 2 ? DISTILL_HELD / 2 : 1;
+    float2 held[HELD_PAIRS];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const uint4 u = lds_u4(part + (k * 256 + tid) * VEC);
-      if (sizeof(T) == 4) {
-        x[k * VEC / 2] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-        x[k * VEC / 2 + 1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
-          x[(k * VEC / 2 + e) % (DISTILL_HELD / 2)] = make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
-        }
-      }
-    }
+    for (int k = 0; k < N; ++k) raw[k] = lds_u4(part + (k * 256 + tid) * VEC);
+    auto pair = [&](int k) {                                                        // two neighbouring values
+      const uint4& u = raw[k * 2 / VEC];
+      const int e = k % (VEC / 2);
+      if (sizeof(T) == 4) return e == 0 ? make_float2(__uint_as_float(u.x), __uint_as_float(u.y)) : make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+      const uint32_t h = e == 0 ? u.x : e == 1 ? u.y : e == 2 ? u.z : u.w;
+      return make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+    };
     const int id = id_now >= 0 && id_now < a.V ? (int)id_now : -1;
     const bool here = id >= v0 && id < v1;
     const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
-    float m4[4] = {x[0].x, x[0].y, x[1].x, x[1].y};
+    float m4[4] = {pair(0).x, pair(0).y, pair(1).x, pair(1).y};
 #pragma unroll
     for (int k = 2; k < DISTILL_HELD / 2; ++k) {
-      m4[(k & 1) * 2] = fmaxf(m4[(k & 1) * 2], x[k].x);
-      m4[(k & 1) * 2 + 1] = fmaxf(m4[(k & 1) * 2 + 1], x[k].y);
+      m4[(k & 1) * 2] = fmaxf(m4[(k & 1) * 2], pair(k).x);
+      m4[(k & 1) * 2 + 1] = fmaxf(m4[(k & 1) * 2 + 1], pair(k).y);
     }
     float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
     const float mine = id >= 0 && tid < a.K ? value : -INFINITY;
@@ -522,13 +519,17 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < DISTILL_HELD / 2; ++k) {
-      const float2 y = fma2(x[k], cm2, ref2), e = make_float2(di_ex2(y.x), di_ex2(y.y));
+      const float2 x = pair(k), y = fma2(x, cm2, ref2), e = make_float2(di_ex2(y.x), di_ex2(y.y));
       s2[k & 1] = fma2(e, one, s2[k & 1]);
       if (BOTH) {
-        const float2 y1 = fma2(x[k], lm2, lref2);
+        const float2 y1 = fma2(x, lm2, lref2);
         t2 = fma2(make_float2(di_ex2(y1.x), di_ex2(y1.y)), one, t2);
+      } else if (sizeof(T) == 2) {                                                  // the gradient is this, scaled
+        held[k % HELD_PAIRS] = e;
       } else {
-        x[k] = e;                                                                   // the gradient is this, scaled
+        uint4& u = raw[k * 2 / VEC];
+        if (k % 2 == 0) u.x = __float_as_uint(e.x), u.y = __float_as_uint(e.y);
+        else u.z = __float_as_uint(e.x), u.w = __float_as_uint(e.y);
       }
     }
     // this thread's entry; a NaN stays one
@@ -606,7 +607,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       uint32_t p[VEC / 2];
 #pragma unroll
       for (int q = 0; q < VEC / 2; ++q) {
-        float2 y = x[k * VEC / 2 + q];
+        float2 y = !BOTH && sizeof(T) == 2 ? held[(k * VEC / 2 + q) % HELD_PAIRS] : pair(k * VEC / 2 + q);
         if (BOTH) {
           const float2 e = fma2(y, c2, up2), e1 = fma2(y, l2, lup2);
           y = fma2(make_float2(di_ex2(e.x), di_ex2(e.y)), ks2, mul2(make_float2(di_ex2(e1.x), di_ex2(e1.y)), kh2));
