@@ -292,7 +292,7 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 // It has one wait: every WARP sends its maximum and sums, against its own maximum, to all CTAs of the cluster (st.async on a barrier of the receiver), and takes the
 // row's from the 8 x CTAs entries that arrive.  (Block sums, a barrier of the cluster and sums of sums took 4 of 7 us a row; the barrier alone 0.7, since it waits for the
 // row before to be stored.)  A warp's part of the row's loss, which needs the row's sums, goes along with the next row's.
-// This kernel and the one above (us, 64 entries): 300 rows of 32,000 fp32 14.6 and 22.7, 2,048 68.8 and 140, of bf16 61.7 and 176; 4,096 of 1,000 56 and 91; 512 of 128,256 72 and
+// This kernel and the one above (us, 64 entries): 300 rows of 32,000 fp32 14.6 and 22.7, 2,048 68.8 and 140, of bf16 61.7 and 176; 4,096 of 1,000 38 and 91; 512 of 128,256 72 and
 // 145; one of 32,000 7.0 and 7.0.
 // Measured: 4,096 rows of 128,256 fp32 logits, 64 entries, 518 us, 6.1 TB/s of logits read and gradient written (a copy's rate would be 489); 2,048 x 32,000, the label too, 70.7
 // (60.9); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
@@ -307,19 +307,19 @@ __device__ __forceinline__ void ring_send(uint32_t at, uint32_t bar, float a, fl
                "r"(__float_as_uint(c)), "r"(__float_as_uint(d)), "r"(bar)
                : "memory");
 }
-template <typename T, bool BOTH>
-__global__ void __launch_bounds__(256, 2)
+template <typename T, bool BOTH, int HELD>
+__global__ void __launch_bounds__(256, HELD >= 64 ? 2 : HELD >= 32 ? 3 : 5)
 distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
-  constexpr int VEC = 16 / sizeof(T), N = DISTILL_HELD / VEC;
+  constexpr int VEC = 16 / sizeof(T), N = HELD / VEC;
   constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
   extern __shared__ __align__(128) unsigned char ring_smem[];
-  T* part = reinterpret_cast<T*>(ring_smem);                                       // [256 x DISTILL_HELD]
+  T* part = reinterpret_cast<T*>(ring_smem);                                       // [256 x HELD]
   // (what the rows write in turn: a warp that is at the next row but one has seen that all have sent for the next one, and so are done with this one)
   __shared__ RingEntry all[2][64];                                                 // [rank x 8 + warp]
   __shared__ __align__(8) uint64_t full, got[2];
   __shared__ int ids_of[2][256];
   __shared__ float es_of[2][256];
-  __shared__ uint32_t bits_of[3][256 * DISTILL_HELD / 32];                          // the places of this part that an entry names (three: cleared while the next row is done) ...
+  __shared__ uint32_t bits_of[3][256 * HELD / 32];                          // the places of this part that an entry names (three: cleared while the next row is done) ...
   __shared__ uint32_t twice[2];                                                     // ... and the last row that named one twice
   __shared__ int list[RING_LIST], empty_rows[RING_LIST];                            // this cluster's rows of a weight, and of none
   __shared__ float list_weight[RING_LIST];
@@ -353,8 +353,8 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     const long long at = (long long)r * a.ld_teacher + tid;
     return a.teacher_fp32 ? reinterpret_cast<const float*>(a.teacher)[at] : (float)reinterpret_cast<const bf16*>(a.teacher)[at];
   };
-  for (int i = tid; i < 3 * 256 * DISTILL_HELD / 32; i += 256) (&bits_of[0][0])[i] = 0;
-  for (int v = whole * VEC + tid; v < 256 * DISTILL_HELD; v += 256) part[v] = (T)-INFINITY;      // copies never reach there
+  for (int i = tid; i < 3 * 256 * HELD / 32; i += 256) (&bits_of[0][0])[i] = 0;
+  for (int v = whole * VEC + tid; v < 256 * HELD; v += 256) part[v] = (T)-INFINITY;      // copies never reach there
   // the row's last values, where they are fewer than 16 bytes, are brought by the thread that their piece falls to
   const int tail = v1 - min(v1, (i0 + whole) * VEC);
   const bool tail_here = tail > 0 && tid == whole % 256;
@@ -488,7 +488,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     // pairs of values, in two-wide arithmetic, loads and stores at fixed offsets: what bounds a row is the instructions of its 64 values a thread (1,180 a warp and row with single
     // values, a branch a load and z - max taken before the factor: 699 us instead of 518 for 4,096 x 128,256 of fp32)
     uint4 raw[N];                                                                   // (as they come: bf16 pairs are taken apart where they are used)
-    constexpr int HELD_PAIRS = !BOTH && sizeof(T) == 2 ? DISTILL_HELD / 2 : 1;
+    constexpr int HELD_PAIRS = !BOTH && sizeof(T) == 2 ? HELD / 2 : 1;
     float2 held[HELD_PAIRS];
 #pragma unroll
     for (int k = 0; k < N; ++k) raw[k] = lds_u4(part + (k * 256 + tid) * VEC);
@@ -504,7 +504,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     const float z = !here ? 0.f : id < (i0 + whole) * VEC ? (float)part[id - v0] : (float)row[id];
     float m4[4] = {pair(0).x, pair(0).y, pair(1).x, pair(1).y};
 #pragma unroll
-    for (int k = 2; k < DISTILL_HELD / 2; ++k) {
+    for (int k = 2; k < HELD / 2; ++k) {
       m4[(k & 1) * 2] = fmaxf(m4[(k & 1) * 2], pair(k).x);
       m4[(k & 1) * 2 + 1] = fmaxf(m4[(k & 1) * 2 + 1], pair(k).y);
     }
@@ -518,7 +518,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     const float2 cm2 = make_float2(cm, cm), ref2 = make_float2(ref, ref), one = make_float2(1.f, 1.f), lm2 = make_float2(lm, lm), lref2 = make_float2(lref, lref);
     float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, t2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < DISTILL_HELD / 2; ++k) {
+    for (int k = 0; k < HELD / 2; ++k) {
       const float2 x = pair(k), y = fma2(x, cm2, ref2), e = make_float2(di_ex2(y.x), di_ex2(y.y));
       s2[k & 1] = fma2(e, one, s2[k & 1]);
       if (BOTH) {
@@ -762,10 +762,14 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
     LP_REQUIRE((long long)rows * ctas < (1LL << 31), "lp_distill_fwd_bwd: %d rows of %d columns are too many", rows, V);
     cudaError_t rc;
     if (wide && K <= RING_TOP) {
-      const size_t part = (size_t)256 * DISTILL_HELD * size;
-#define LP_RING(T) rc = both ? launch_ring<distill_ring_kernel<T, true>>(a, rows, ctas, part, stream) : launch_ring<distill_ring_kernel<T, false>>(a, rows, ctas, part, stream)
-      if (logits_fp32) LP_RING(float);
-      else LP_RING(bf16);
+#define LP_RING(T, HELD)                                                                                    \
+  rc = both ? launch_ring<distill_ring_kernel<T, true, HELD>>(a, rows, ctas, (size_t)256 * HELD * size, stream) \
+            : launch_ring<distill_ring_kernel<T, false, HELD>>(a, rows, ctas, (size_t)256 * HELD * size, stream)
+      // few values a thread leave registers for more CTAs an SM, five and three: 4,096 rows of 1,000 fp32 37.5 us (57.9 with 64), 3,000 of 8,000 39 (50), of 4,000 with a
+      // temperature and labels 48 (71), of 2,048 bf16 34 (72); where a row has several CTAs either way their messages cost more (1,000 of 60,000 fp32 89 us with 32, 68 with 64)
+      if (V <= 256 * 8) { if (logits_fp32) LP_RING(float, 8); else LP_RING(bf16, 8); }
+      else if (V <= 256 * 32) { if (logits_fp32) LP_RING(float, 32); else LP_RING(bf16, 32); }
+      else { if (logits_fp32) LP_RING(float, DISTILL_HELD); else LP_RING(bf16, DISTILL_HELD); }
 #undef LP_RING
       LP_CHECK_CUDA(rc);
       return 0;

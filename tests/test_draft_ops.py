@@ -562,6 +562,20 @@ def test_distill(R, V, K, dtype, pad, temperature, hard):
 
 
 @gpu
+@pytest.mark.parametrize("R, V, share", [(1300000, 10, 0.9), (1300000, 10, 0.1), (70000, 600, 0.5)])
+def test_distill_of_many_rows(R, V, share):
+    """more rows than a cluster's list holds, most with a weight and most without: the same few rows over and over"""
+    c = distill_case(50, V, 3, R, share=2.0, labels=False)
+    c["weight"] = torch.ones(50, device="cuda")
+    loss, d = distill_close(c, V)
+    at = torch.arange(R, device="cuda") % 50
+    on = torch.rand(R, generator=gen(R), device="cuda") < share
+    got = ops.distill_fwd_bwd(vocab=V, **{**{k: v[at] if v is not None else None for k, v in c.items()}, "weight": on.float()})
+    assert torch.equal(got[0], torch.where(on, loss[at], 0.0))
+    assert torch.equal(got[1], torch.where(on[:, None], d[at], 0.0))
+
+
+@gpu
 @pytest.mark.parametrize("V, K", [(50, 6), (40000, 40)])
 def test_distill_of_missing_and_repeated_entries(V, K):
     c = distill_case(8, V, K, V, share=2.0)
