@@ -295,7 +295,7 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 // This kernel and the one above (us, 64 entries): 300 rows of 32,000 fp32 14.6 and 22.7, 2,048 68.8 and 140, of bf16 61.7 and 176; 4,096 of 1,000 38 and 91; 512 of 128,256 72 and
 // 145; one of 32,000 7.0 and 7.0.
 // Measured: 4,096 rows of 128,256 fp32 logits, 64 entries, 518 us, 6.1 TB/s of logits read and gradient written (a copy's rate would be 489); 2,048 x 32,000, the label too, 70.7
-// (60.9); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
+// (60.9), at another temperature and 60 % of the rows 68 (45); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
 constexpr int RING_TOP = 255;
 constexpr int RING_LIST = 1536, RING_LOOK = 1024;      // rows that a cluster knows to be its own; weights that are looked at at once
 struct __align__(16) RingEntry {             // of a warp: maximum and sums of the row; the teacher's maximum
