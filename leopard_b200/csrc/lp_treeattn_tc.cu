@@ -57,6 +57,7 @@ struct TreeTc {
   TreeArgs a;
   int box;                             // rows of a TMA box: of one page
 };
+constexpr int TT_BARS = 320;           // bytes of the barriers and what stands behind them
 
 // a CTA's piece of an item
 struct TreePiece {
@@ -93,6 +94,11 @@ template <int DH, bool SPLIT>
 __global__ void __launch_bounds__(TT_THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeTc tc) {
   constexpr int NB = (DH + 63) / 64, KS_QK = DH / 16, HEAD_BYTES = NB * TT_BOX, STAGES = SPLIT ? 3 : 2;
+  // A stage's loads have FULLS / STAGES barriers in turn.  SPLIT: three stages are dealt to two streams, and a stage's load before this one was the other stream's: a wait by parity for tile g on
+  // one barrier a stage would pass while the load of g - 3 is still under way.  With six, the phase before is that of g - 6, which has been consumed when anybody waits for g: before
+  // loads of g - 2, this stream's last tile, the producer sent those of g - 3, and for these it waited until g - 6 was free (a piece's first tiles: all before the piece has been consumed
+  // when its queries are there).
+  constexpr int FULLS = SPLIT ? 2 * STAGES : STAGES;
   constexpr int Q_OFF = 0, K_OFF = Q_OFF + (SPLIT ? 1 : 2) * HEAD_BYTES, V_OFF = K_OFF + STAGES * HEAD_BYTES, BAR_OFF = V_OFF + STAGES * HEAD_BYTES;
   constexpr int CH = DH / 8, MAX_WORDS = SPLIT ? 2 : LP_TREE_MAX_NODES / 64;
   constexpr uint32_t TM_S = 0, TM_O = 256;
@@ -100,9 +106,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream (SPLIT: one), a phase a piece
-  uint64_t* k_full = q_full + 2;                                       // [3] by stage
-  uint64_t* v_full = k_full + 3;                                       // [3]
-  uint64_t* k_empty = v_full + 3;                                      // [3] both streams' issuers, or that of the tile's stream
+  uint64_t* k_full = q_full + 2;                                       // [FULLS] by tile
+  uint64_t* v_full = k_full + FULLS;                                   // [FULLS]
+  uint64_t* k_empty = v_full + FULLS;                                  // [3] by stage: both streams' issuers, or that of the tile's stream
   uint64_t* v_empty = k_empty + 3;                                     // [3]
   uint64_t* s_full = v_empty + 3;                                      // [4] stream x half
   uint64_t* p_full = s_full + 4;                                       // [4]
@@ -110,9 +116,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   uint64_t* o_done = pv_done + 4;                                      // [2]
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(o_done + 2);
   int* odd = reinterpret_cast<int*>(tmem_at + 1);                      // [4] piece whose V had values that are not finite, by its number mod 4
-  float2* other = reinterpret_cast<float2*>(smem + BAR_OFF + 256);     // [128] SPLIT: maximum and sum of stream 1's rows
-  unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + 256);      // [256][MAX_WORDS] else: of this thread's row
-  TreeLine* line = reinterpret_cast<TreeLine*>(smem + BAR_OFF + 256 + (SPLIT ? 128 * 8 : 256 * MAX_WORDS * 8));
+  float2* other = reinterpret_cast<float2*>(smem + BAR_OFF + TT_BARS);     // [128] SPLIT: maximum and sum of stream 1's rows
+  unsigned long long* mask_words = reinterpret_cast<unsigned long long*>(smem + BAR_OFF + TT_BARS);      // [256][MAX_WORDS] else: of this thread's row
+  static_assert((2 + 2 * FULLS + 3 + 3 + 4 + 4 + 4 + 2) * 8 + 4 + 16 <= TT_BARS, "barriers");
+  TreeLine* line = reinterpret_cast<TreeLine*>(smem + BAR_OFF + TT_BARS + (SPLIT ? 128 * 8 : 256 * MAX_WORDS * 8));
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -123,9 +130,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mbar_init(&q_full[i], 128);
       mbar_init(&o_done[i], 1);
     }
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < FULLS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
+    }
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&k_empty[i], SPLIT ? 1 : 2);
       mbar_init(&v_empty[i], SPLIT ? 1 : 2);
     }
@@ -170,7 +179,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
         const uint32_t ph = (g / STAGES) & 1;
         for (int kv = 0; kv < 2; ++kv) {
-          uint64_t* full = kv ? &v_full[st] : &k_full[st];
+          uint64_t* full = kv ? &v_full[g % FULLS] : &k_full[g % FULLS];
           if (g >= STAGES) mbar_wait_warp(kv ? &v_empty[st] : &k_empty[st], ph ^ 1);
           if (lane == 0) mbar_arrive_expect_tx(full, HEAD_BYTES);
           uint8_t* to = smem + (kv ? V_OFF : K_OFF) + st * HEAD_BYTES;
@@ -205,9 +214,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
       if (!SPLIT && p.r0 + q * 128 >= p.s.n * a.group) {      // no rows here: the stages are passed on
         for (int j = 0; j < p.n; ++j, ++g) {
-          mbar_wait_warp(&k_full[g % STAGES], (g / STAGES) & 1);
+          mbar_wait_warp(&k_full[g % FULLS], (g / FULLS) & 1);
           if (issue) mbar_arrive(&k_empty[g % STAGES]);
-          mbar_wait_warp(&v_full[g % STAGES], (g / STAGES) & 1);
+          mbar_wait_warp(&v_full[g % FULLS], (g / FULLS) & 1);
           if (issue) mbar_arrive(&v_empty[g % STAGES]);
         }
         continue;
@@ -239,7 +248,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mbar_wait_warp(&q_full[SPLIT ? 0 : q], pieces & 1);
       ++pieces;
       int gt = g + j0;
-      mbar_wait_warp(&k_full[gt % STAGES], (gt / STAGES) & 1);
+      mbar_wait_warp(&k_full[gt % FULLS], (gt / FULLS) & 1);
       tc_fence_after();
       issue_S(gt, 0);
       issue_S(gt, 1);
@@ -247,10 +256,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       for (int j = j0; j < p.n; j += STEP, gt += STEP, ++nt) {
         const bool more = j + STEP < p.n;
         const int gn = gt + STEP;
-        mbar_wait_warp(&v_full[gt % STAGES], (gt / STAGES) & 1);
+        mbar_wait_warp(&v_full[gt % FULLS], (gt / FULLS) & 1);
         issue_PV(gt, j == j0, 0);
         if (more) {
-          mbar_wait_warp(&k_full[gn % STAGES], (gn / STAGES) & 1);
+          mbar_wait_warp(&k_full[gn % FULLS], (gn / FULLS) & 1);
           tc_fence_after();
           issue_S(gn, 0);
         }
@@ -355,7 +364,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
         if (tail && h == 0) {
           // V of this tile before its product: rows that are not keys, values that are not finite
-          mbar_wait(&v_full[(g + j) % STAGES], ((g + j) / STAGES) & 1);
+          mbar_wait(&v_full[(g + j) % FULLS], ((g + j) / FULLS) & 1);
           const bool key_ok = key0 + r < n_keys;
           uint8_t* at = smem + V_OFF + ((g + j) % STAGES) * HEAD_BYTES + r * 128;
 #pragma unroll 1
@@ -626,7 +635,7 @@ static int launch_tc(const TreeTc& tc, cudaStream_t stream) {
     if (const int rc = make_tmap_bf16_4d(&tm[i], base[i], dims, strides, box)) return rc;
   }
   const bool split = d.B <= TT_SPLIT_BATCH && tc.a.rows <= 128;
-  const size_t smem = (split ? 7 : 6) * NB * TT_BOX + 256 + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * sizeof(TreeLine) + 1024;
+  const size_t smem = (split ? 7 : 6) * NB * TT_BOX + TT_BARS + (split ? 128 * 8 : 256 * (LP_TREE_MAX_NODES / 64) * 8) + (size_t)(d.B + 1) * sizeof(TreeLine) + 1024;
   if (split) {
     LP_CHECK_CUDA((allow_smem<tree_tc_kernel<DH, true>>((int)smem)));
     tree_tc_kernel<DH, true><<<tc.a.ctas, TT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
