@@ -105,7 +105,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   const TreeArgs& a = tc.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream (SPLIT: one), a phase a piece
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);      // [2] by stream, a phase a piece that the stream has tiles of
   uint64_t* k_full = q_full + 2;                                       // [FULLS] by tile
   uint64_t* v_full = k_full + FULLS;                                   // [FULLS]
   uint64_t* k_empty = v_full + FULLS;                                  // [3] by stage: both streams' issuers, or that of the tile's stream
@@ -206,10 +206,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
       const int j0 = SPLIT ? q : 0;
-      if (SPLIT && j0 >= p.n) {         // one tile: the other stream's (whose phases of the queries are counted all the same)
-        mbar_wait_warp(&q_full[0], pieces & 1);
+      if (SPLIT && j0 >= p.n) {         // one tile: the other stream's, with nothing to wait for here (a wait that the other stream does not wait for in turn may miss its phase)
         g += p.n;
-        ++pieces;
         continue;
       }
       if (!SPLIT && p.r0 + q * 128 >= p.s.n * a.group) {      // no rows here: the stages are passed on
@@ -245,7 +243,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           umma_commit(&pv_done[q * 2 + h]);
         }
       };
-      mbar_wait_warp(&q_full[SPLIT ? 0 : q], pieces & 1);
+      mbar_wait_warp(&q_full[q], pieces & 1);
       ++pieces;
       int gt = g + j0;
       mbar_wait_warp(&k_full[gt % FULLS], (gt / FULLS) & 1);
@@ -309,7 +307,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (DH % 64 != 0)
           for (int c = CH; c < NB * 8; ++c) sts_u4(at + (c >> 3) * TT_BOX + lane * 128 + (((c & 7) ^ (lane & 7)) << 4), make_uint4(0, 0, 0, 0));
         fence_proxy_async_smem();
-        mbar_arrive(&q_full[SPLIT ? 0 : q]);
+        mbar_arrive(&q_full[q]);
+        if (SPLIT && p.n > 1) mbar_arrive(&q_full[1]);
       }
       // its node's mask, when this piece gets there
       const int nw = (a.d.T + 63) >> 6;

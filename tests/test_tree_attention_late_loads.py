@@ -77,3 +77,12 @@ def test_a_load_that_lands_late(library, load, split):
     apart(library, load, -1, split, [1100], [33])
 
 
+@pytest.mark.parametrize("warp", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("split", [True, False])
+def test_a_warp_that_comes_late(library, warp, split):
+    """... to pieces of one tile, which the first stream does alone, and to two that both have"""
+    apart(library, -1, warp, split, [60, 20, 90, 300, 10, 150], [33, 20, 33, 33, 5, 33])
+
+
+def test_a_warp_that_comes_late_to_pieces_that_are_not_its_own(library):
+    apart(library, -1, 2, True, [60, 20], [33, 20])
