@@ -31,7 +31,7 @@ __device__ __forceinline__ float ta_ex2(float x) {
 }
 // a sequence's part of the line of tiles
 struct TreeSeq {
-  int len, n, tiles, blocks;              // cached rows; nodes; tiles of an item; blocks of rows
+  int len, n, tiles, blocks;              // cached rows that are there; nodes; tiles of an item; blocks of rows
   int keys;                               // rows that are there: cached and nodes', as far as the page table reaches (fewer than 2^31)
 };
 // what the line knows of a sequence: the tiles before it, its length and nodes, and its first CTA where items have CTAs of their own.
@@ -42,9 +42,10 @@ struct TreeLine {
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int len, int n) {
   TreeSeq s;
+  const long long capacity = (long long)a.d.max_pages * a.d.page_size;
   s.n = n;
-  s.len = len;
-  s.keys = (int)min((long long)len + n, (long long)a.d.max_pages * a.d.page_size);
+  s.len = (int)min((long long)len, capacity);      // (a sequence that says it is longer than its pages: no row behind them is a cached one)
+  s.keys = (int)min((long long)len + n, capacity);
   s.tiles = n ? (int)(((unsigned)s.keys + (1u << a.key_bits) - 1) >> a.key_bits) : 0;
   s.blocks = (n * a.group + a.rows - 1) >> a.row_bits;
   return s;
