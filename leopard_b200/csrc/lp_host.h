@@ -32,6 +32,27 @@ const char* get_error();
 
 int sm_count();
 
+// Whether the places of a tensor share no memory, as far as strides say: sorted by size, each reaches past what lies within it.  `inner`: what lies side by side at a place, in the
+// strides' unit.  (Every slice and permutation of a contiguous tensor passes.)
+struct Dim { long long size, stride; };
+inline bool strides_nest(Dim* dims, int n, long long inner) {
+  for (int i = 0; i < n; ++i)
+    if (dims[i].stride < 0) dims[i].stride = -dims[i].stride;
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && dims[j].stride < dims[j - 1].stride; --j) {
+      const Dim d = dims[j];
+      dims[j] = dims[j - 1];
+      dims[j - 1] = d;
+    }
+  __int128 reach = inner;
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].size <= 1) continue;
+    if (dims[i].stride < reach) return false;
+    reach += (__int128)dims[i].stride * (dims[i].size - 1);
+  }
+  return true;
+}
+
 #ifdef __CUDACC__
 // two fp32 multiply-adds (products) in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {

@@ -438,6 +438,8 @@ extern "C" int lp_tree_attention(const lp_tree_attn_desc* d, void* workspace, si
   const uintptr_t bases = reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v) |
                           reinterpret_cast<uintptr_t>(d->out) | reinterpret_cast<uintptr_t>(workspace);
   LP_REQUIRE(strides % 8 == 0 && bases % 16 == 0, "lp_tree_attention: strides in multiples of 8 elements, 16-byte aligned bases");
+  Dim places[3] = {{d->B, d->o_batch}, {d->T, d->o_node}, {d->H, d->o_head}};
+  LP_REQUIRE(strides_nest(places, 3, d->D), "lp_tree_attention: rows of out share their memory (strides %lld, %lld, %lld)", d->o_batch, d->o_node, d->o_head);
   LP_REQUIRE(ws_bytes >= lp_tree_attention_workspace_bytes(d), "lp_tree_attention: workspace too small");
   a.group = d->H / d->KVH;
   a.rows = tree_rows(d);

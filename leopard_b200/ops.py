@@ -610,7 +610,7 @@ def tree_attention(q, k, v, lengths, mask, nodes=None, page_table=None, scale=No
     q bf16 [B, T, H, D]; k, v bf16 [pages, page_size, KVH, D] (page_table int32 [B, max_pages]; -1: not there) or [B, rows, KVH, D]; lengths int32 [B], rows
     of the past, seen by every node; mask int64 [B, T, ceil(T / 64)] (tree_mask), the nodes that a node sees: node n is row lengths[b] + n; nodes
     int32 [B] or None, nodes of each sequence.  Strides are free but for a contiguous last dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of nodes
-    that a sequence does not have stay as they were (`out` given) or are unspecified.  A node that sees nothing is zeros."""
+    that a sequence does not have stay as they were (`out` given; its rows share no memory, and its span meets none of q, k and v) or are unspecified.  A node that sees nothing is zeros."""
     try:
         B, T, H, D = q.shape
         P, S, KVH, Dk = k.shape
