@@ -1008,12 +1008,14 @@ int lp_verify_draft(const float* target, long long target_batch, long long targe
 
 /* Rows lengths[b] + path[b][j] of every pool move to rows lengths[b] + j, j < count[b], in place (path as lp_verify_draft gives it: rising; a list that does not
  * rise leaves unspecified rows at those places).  pools: HOST array of n_pools device pointers (pool_step not 0: of the first one, the
- * others pool_step bytes apart), each [n_pages][page_size] rows of row_bytes bytes, strides in bytes; page table as in lp_tree_attention.  Entries and rows that are not there move nothing. */
+ * others pool_step bytes apart), each [n_pages][page_size] rows of row_bytes bytes, strides in bytes; page table as in lp_tree_attention.  Entries and rows that are not there move nothing.
+ * Pools, pages and rows share no memory (strides reach past what lies within them; listed pools may lie between one another).  A page whose rows move stands in no other table,
+ * nor twice in one: what several sequences hold is copied first (lp_cache_copy_pages). */
 int lp_cache_compact(const void* const* pools, long long pool_step, int n_pools, long long page_stride, long long row_stride, long long row_bytes, int n_pages,
                      int page_size, const int* page_table, long long ld_table, int max_pages, const int* lengths, const int* path,
                      long long ld_path, const int* count, int B, int T, void* stream);
 /* Page src[i] of every pool is copied to page dst[i], i < n (device lists; no page may be among both, nor twice among dst).  Entries that are not
- * pages copy nothing. */
+ * pages copy nothing.  Pools and pages share no memory, as in lp_cache_compact. */
 int lp_cache_copy_pages(const void* const* pools, long long pool_step, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
                         const int* dst, int n, void* stream);
 

@@ -1,6 +1,8 @@
 // leopard_b200 — what drafting needs beside the attention of a tree (lp_treeattn.cu): which nodes of a tree see which, verification of the drafts against
 // the target's probabilities, and rows and pages of a cache moved in all layers at once.
 #include "lp_host.h"
+#include <stdlib.h>
+#include <algorithm>
 #include "../../include/leopard_b200.h"
 
 namespace lp {
@@ -378,6 +380,51 @@ static int piece_bytes(const void* const* pools, long long step, int n, long lon
   return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
 }
 
+// Pools are moved by CTAs of their own, in no order: none may share memory with another, nor places within one.  1: apart, 0: not, -1: no memory to find out.
+// `dims`, within a pool (nested afterwards: ascending); `inner`: bytes side by side.
+static bool pools_meet(long long diff, const Dim* dims, const __int128* extent, int level) {      // a place of one pool and one of another `diff` bytes on
+  if (level < 0) return diff < extent[0] && -diff < extent[0];
+  if (dims[level].size <= 1) return pools_meet(diff, dims, extent, level - 1);
+  // of the multiples of this stride only the two next to diff come nearer than what lies within it
+  long long k = diff / dims[level].stride;
+  if (diff % dims[level].stride < 0) --k;
+  for (int i = 0; i < 2; ++i, ++k)
+    if (k < dims[level].size && -k < dims[level].size && pools_meet(diff - k * dims[level].stride, dims, extent, level - 1)) return true;
+  return false;
+}
+static int pools_apart(const void* const* pools, long long step, int n_pools, Dim* dims, int n_dims, long long inner) {
+  if (step) {
+    Dim all[4];
+    for (int i = 0; i < n_dims; ++i) all[i] = dims[i];
+    all[n_dims] = {n_pools, step};
+    return strides_nest(all, n_dims + 1, inner);
+  }
+  if (!strides_nest(dims, n_dims, inner)) return 0;
+  if (n_pools == 1) return 1;
+  __int128 extent[4] = {inner};           // of a place, and with each dimension
+  for (int i = 0; i < n_dims; ++i) extent[i + 1] = extent[i] + (dims[i].size > 1 ? (__int128)dims[i].stride * (dims[i].size - 1) : 0);
+  unsigned long long* at = static_cast<unsigned long long*>(malloc(sizeof(unsigned long long) * (size_t)n_pools));
+  if (!at) return -1;
+  for (int i = 0; i < n_pools; ++i) at[i] = reinterpret_cast<unsigned long long>(pools[i]);
+  std::sort(at, at + n_pools);
+  unsigned long long least = ~0ull;
+  for (int i = 1; i < n_pools; ++i) least = std::min(least, at[i] - at[i - 1]);
+  bool apart = (__int128)least >= extent[n_dims];      // one behind the other
+  bool within = true;                                  // or all of them within one stride, of this dimension and those above, as layers side by side in a page are
+  for (int i = n_dims - 1; i >= 0 && !apart && within; --i) {
+    if (dims[i].size <= 1) continue;
+    within = (__int128)(at[n_pools - 1] - at[0]) + extent[i] <= dims[i].stride;
+    apart = within && (__int128)least >= extent[i];
+  }
+  if (!apart) {
+    apart = true;
+    for (int i = 0; i < n_pools && apart; ++i)
+      for (int j = i + 1; j < n_pools && apart && (__int128)(at[j] - at[i]) < extent[n_dims]; ++j) apart = !pools_meet((long long)(at[j] - at[i]), dims, extent, n_dims - 1);
+  }
+  free(at);
+  return apart;
+}
+
 }  // namespace lp
 
 extern "C" int lp_tree_mask(const int* parents, long long ld, int B, int T, unsigned long long* mask, int* depth, void* stream_) {
@@ -415,6 +462,9 @@ extern "C" int lp_cache_compact(const void* const* pools, long long pool_step, i
   LP_REQUIRE(table != nullptr || (max_pages == 1 && B <= n_pages), "lp_cache_compact: %d sequences without a page table need a page each, there are %d", B, n_pages);
   const int u = piece_bytes(pools, pool_step, n_pools, page_stride, row_stride, row_bytes);
   const long long units = row_bytes / u;
+  Dim within[2] = {{n_pages, page_stride}, {page_size, row_stride}};
+  const int apart = pools_apart(pools, pool_step, n_pools, within, 2, row_bytes);
+  LP_REQUIRE(apart == 1, apart == 0 ? "lp_cache_compact: pools, pages or rows share their memory" : "lp_cache_compact: out of host memory");
   LP_REQUIRE(units < (1 << 30), "lp_cache_compact: rows of %lld bytes are too wide", row_bytes);
   for (int at = 0; at < n_pools; at += POOLS_MAX) {
     const int m = n_pools - at < POOLS_MAX ? n_pools - at : POOLS_MAX;
@@ -441,6 +491,9 @@ extern "C" int lp_cache_copy_pages(const void* const* pools, long long pool_step
   LP_REQUIRE(pools && src && dst && n_pools > 0 && n_pages > 0 && n >= 0 && n <= 65535, "lp_cache_copy_pages: bad arguments n_pools=%d n_pages=%d n=%d", n_pools, n_pages, n);
   LP_REQUIRE(page_bytes > 0 && page_stride >= page_bytes, "lp_cache_copy_pages: pages of %lld bytes, %lld apart", page_bytes, page_stride);
   if (n == 0) return 0;
+  Dim within[1] = {{n_pages, page_stride}};
+  const int apart = pools_apart(pools, pool_step, n_pools, within, 1, page_bytes);
+  LP_REQUIRE(apart == 1, apart == 0 ? "lp_cache_copy_pages: pools or pages share their memory" : "lp_cache_copy_pages: out of host memory");
   const int u = piece_bytes(pools, pool_step, n_pools, page_stride, page_bytes, 0);
   const long long units = page_bytes / u, ctas = (units + PAGE_PIECES - 1) / PAGE_PIECES;
   LP_REQUIRE(ctas < (1LL << 31), "lp_cache_copy_pages: pages of %lld bytes are too large", page_bytes);

@@ -722,7 +722,8 @@ def cache_compact(pools, lengths, path, count, page_table=None):
     """The accepted nodes' rows become the last rows of their sequences, in every pool, in place (lp_cache_compact): row lengths[b] + path[b, j] moves to row
     lengths[b] + j, j < count[b] (path and count as verify_draft gives them; path rises).  pools: one tensor [n, pages, page_size, width] or a list of [pages, page_size,
     width] of equal shapes, any type (the decoder's cache [layers, 2, rows, width]: kv.flatten(0, 1).unsqueeze(1)); page_table int32 [B, max_pages], or None: sequence b
-    is page b.  lengths, count int32 [B], path int32 [B, T].  Rows that are not there move nothing.  Returns pools."""
+    is page b.  lengths, count int32 [B], path int32 [B, T].  Rows that are not there move nothing.  Pools, pages and rows share no memory, and a page whose rows move stands
+    in no other sequence's table (copy what several hold first: cache_copy_pages).  Returns pools."""
     ptrs, step, n, shape, st, e, dev = _pools(pools)
     if not n or not path.numel():
         return pools
