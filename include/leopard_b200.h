@@ -977,7 +977,7 @@ int lp_tree_mask(const int* parents, long long ld, int B, int T, unsigned long l
  * nodes n < nodes[b], those whose bit is set in node i's words; g = h / (H / KVH).  All bf16, sums in fp32.  D = 64, 96 or 128.
  * k, v: [n_pages][page_size][KVH][D] with the strides given in elements (multiples of 8, the last dimension contiguous, 16-byte aligned bases); row r of
  * sequence b lies in page page_table[b][r / page_size] of `max_pages` a sequence (ld_table between sequences).  page_table NULL: page b (max_pages 1).  A page
- * that is not in [0, n_pages) is not there: its rows are not seen.  Nor are rows past max_pages * page_size.  A row that sees nothing is zeros.
+ * that is not in [0, n_pages) is not there: its rows are not seen.  Nor are rows past max_pages * page_size (2^31 - 128 at most).  A row that sees nothing is zeros.
  * What a row does not see has no effect on it, NaN and infinities among it.  Rows i >= nodes[b] of out are not written;
  * its rows share no memory with one another (each stride reaches past what lies within it: slices and permutations of a contiguous tensor), nor with q, k and v.
  * workspace: lp_tree_attention_workspace_bytes(desc) bytes, 16-byte aligned, for this call alone until it has ended. */

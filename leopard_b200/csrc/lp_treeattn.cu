@@ -406,7 +406,7 @@ static int tree_check(const lp_tree_attn_desc* d) {
   LP_REQUIRE(d->KVH > 0 && d->KVH <= 65535 && d->H >= d->KVH && d->H % d->KVH == 0 && d->H <= 65535, "lp_tree_attention: %d query heads over %d key heads", d->H, d->KVH);
   LP_REQUIRE(d->D == 64 || d->D == 96 || d->D == 128, "lp_tree_attention: heads of %d are not built (64, 96, 128)", d->D);
   LP_REQUIRE(d->n_pages > 0 && d->page_size > 0 && d->max_pages > 0, "lp_tree_attention: %d pages of %d rows, %d a sequence", d->n_pages, d->page_size, d->max_pages);
-  LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 64, "lp_tree_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
+  LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 128 /* a row's place, and the end of its tile, in 32 bits */, "lp_tree_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
   return 0;
 }
 

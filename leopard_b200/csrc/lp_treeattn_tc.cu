@@ -165,16 +165,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const TreePiece p = tree_piece(a, line, u, u_end);
       u += p.n;
       const int n_keys = p.s.keys;
-      int key = p.t0 * TT_KEYS + lane * tc.box;      // this lane's box of the tile
-      TreePlace at(a, lane < boxes ? key : 0);
+      int key = lane < boxes ? p.t0 * TT_KEYS + lane * tc.box : 0;      // this lane's box of the tile
+      TreePlace at(a, key);
       auto page_of = [&]() { return lane < boxes && key < n_keys ? at.page(a, p.b) : -1; };
       int page = page_of();
       for (int j = 0; j < p.n; ++j, ++g) {
         const int st = g % STAGES, row = at.row;
         int next = -1;
         if (j + 1 < p.n) {
-          key += TT_KEYS;
-          if (lane < boxes) at.forward(a, TT_KEYS);
+          if (lane < boxes) {
+            key += TT_KEYS;
+            at.forward(a, TT_KEYS);
+          }
           next = page_of();
         }
         const uint32_t ph = (g / STAGES) & 1;
@@ -337,7 +339,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
         paged = !__all_sync(0xffffffffu, there);
       }
-      int box_key = (p.t0 + j0) * TT_KEYS + lane * box;
+      int box_key = lane < n_box ? (p.t0 + j0) * TT_KEYS + lane * box : 0;
       TreePlace box_at(a, paged && lane < n_box ? box_key : 0);
       auto page_there = [&]() { return !paged || lane >= n_box || box_key >= n_keys || box_at.page(a, p.b) >= 0; };
       bool there_next = page_there();
@@ -357,8 +359,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const unsigned pages = paged ? __ballot_sync(0xffffffffu, there_next) : 0xffffffffu;
         if (paged && t + 1 < 2 * mine) {
           const int on = h == 0 || STEP == 1 ? 64 : 64 + TT_KEYS;
-          box_key += on;
-          if (lane < n_box) box_at.forward(a, on);
+          if (lane < n_box) {
+            box_key += on;
+            box_at.forward(a, on);
+          }
           there_next = page_there();
         }
         if (tail && h == 0) {

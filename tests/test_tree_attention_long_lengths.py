@@ -1,7 +1,8 @@
 """Lengths beyond what a cache or a page table holds: what is there is seen, rows past it are not, nor the nodes that would stand there (tree attention; the tcgen05 kernel on the
 CPU, both kernels on a GPU)."""
+import ctypes as C
+
 import pytest
-import torch
 
 import test_draft_ops as D
 from test_tree_attention_emulated import case, check, emu, run  # noqa: F401 (emu: a fixture)
@@ -37,3 +38,10 @@ def test_both_kernels(B, T, H, G, rows, page, beyond):
     D.close(D.attend(c), c)
     c["lengths"][:] = c["lengths"][0].item()
     D.close(D.attend(c), c)
+
+
+def test_tables_end_where_a_tile_does_in_32_bits(native_lib):
+    most = (2 ** 31 - 128) // 64
+    for pages, word in ((most, b"workspace too small"), (most + 1, b"too many")):
+        d = D.tree_desc(max_pages=pages, ld_table=pages)
+        assert native_lib.lp_tree_attention(C.byref(d), C.c_void_p(1 << 20), 0, None) == -1 and word in native_lib.lp_last_error()
