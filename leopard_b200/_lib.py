@@ -88,6 +88,7 @@ LATENT_SPLIT_ROWS = 16
 GEMM_SPLIT_BF16, GEMM_SPLIT_F32, GEMM_SPLIT_PLANES = 0, 1, 2
 LINEAR_W_CONSTANT = 0x100      # lp_linear: with an epilogue, for weights that nothing on the stream writes
 TREE_MAX_NODES = 256
+DISTILL_MAX_TOP = 1024          # lp_distill_fwd_bwd: teacher entries a row
 LINEAR_ROWS_MAX, LINEAR_ROWS_COLS = 8, 8      # lp_linear: up to this many rows stream the weights, a CTA to so many columns
 
 

@@ -62,6 +62,18 @@ def shifted_targets(labels: torch.Tensor, loss_mask: torch.Tensor, dp_world: int
     return tgt.reshape(-1).contiguous(), w.reshape(-1).contiguous()
 
 
+def check_teacher(tokens: torch.Tensor, teacher) -> None:
+    """refuses what SFTTrainer.step does not take as a teacher of these tokens"""
+    if teacher is None:
+        return
+    b, s = tokens.shape
+    if (not isinstance(teacher, (list, tuple)) or len(teacher) != 2 or any(not isinstance(t, torch.Tensor) or t.dim() != 3 or tuple(t.shape[:2]) != (b, s) for t in teacher)
+            or teacher[0].shape != teacher[1].shape or not 0 < teacher[0].shape[2] <= _lib.DISTILL_MAX_TOP):
+        raise ValueError(f"teacher must be (ids, logits), each [{b}, {s}, K] with K from 1 to {_lib.DISTILL_MAX_TOP}")
+    if teacher[0].dtype not in (torch.int64, torch.int32) or teacher[1].dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"teacher must be ids of int64 or int32 and logits of float32 or bfloat16, got {teacher[0].dtype} and {teacher[1].dtype}")
+
+
 def layer_buckets(names: Sequence[str], layout: Dict[str, Tuple[int, int]], total: int) -> List[Tuple[int, int]]:
     """Contiguous [start, end) ranges of the flat gradient buffer, one per name prefix ('dec.31', ..., 'proj', ...) in
     the order the backward pass completes them (the order of `names`)."""
@@ -521,11 +533,13 @@ class SFTTrainer:
         micro-batch losses of this rank, and the global gradient norm before clipping; one device -> host read.
         teacher: (ids, logits) [b, s, K] each, a list of such pairs with micro-batches, or None."""
         if isinstance(tokens, (list, tuple)):
-            if teacher is not None and len(teacher) != len(tokens):
-                raise ValueError(f"{len(tokens)} micro-batches need as many teachers, got {len(teacher)}")
+            if teacher is not None and (not isinstance(teacher, (list, tuple)) or len(teacher) != len(tokens)):
+                raise ValueError(f"{len(tokens)} micro-batches need a list of as many teachers")
             micro = list(zip(tokens, labels, loss_mask, images, teacher if teacher is not None else [None] * len(tokens)))
         else:
             micro = [(tokens, labels, loss_mask, images, teacher)]
+        for mb in micro:
+            check_teacher(mb[0], mb[4])      # before anything of the step counts
         self.iteration += 1
         # the decoder's gradients are overwritten by the first micro-batch; the embedding's are added to, and the projector's and the
         # tower's stay zero in a step without images
@@ -585,8 +599,6 @@ class SFTTrainer:
         if s % 8:
             raise ValueError(f"sequence length {s} must be a multiple of 8")
         R = b * s
-        if teacher is not None and (len(teacher) != 2 or any(t.dim() != 3 or tuple(t.shape[:2]) != (b, s) for t in teacher) or teacher[0].shape != teacher[1].shape):
-            raise ValueError(f"teacher must be (ids, logits), each [{b}, {s}, K]")
         n_img_rows = int((tokens == cfg.megatron_image_index).sum())      # counted where the batch lives (the host): no device sync
         ids = tokens.reshape(-1).to(self.dev, torch.long).contiguous()
 
