@@ -151,8 +151,8 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, float w, bool 
   g.c = a.inv_tau * 1.4426950408889634f;
   g.cs = soft ? w * (1.f - a.hard) * a.tau : 0.f;
   g.ch = y >= 0 && y < a.V ? w * a.hard : 0.f;
-  g.ks = g.cs / s;
-  g.kh = g.ch / s1;
+  g.ks = g.cs == 0.f ? 0.f : g.cs / s;      // (a term that is not there has no part, whatever the sum is)
+  g.kh = g.ch == 0.f ? 0.f : g.ch / s1;
   return g;
 }
 
@@ -260,12 +260,13 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
   }
   if (!BOTH) s1 = s;                        // no label, or no temperature: one sum does
   const RowGrad g = row_grad(a, w, soft, y, top_m, s, s1);
+  const bool some = g.ks != 0.f || g.kh != 0.f;      // (a row without terms is zeros, whatever its logits are)
   const float down = !BOTH ? (g.ks + g.kh) * (ctas > 1 && m != -INFINITY ? di_ex2((m - top_m) * c) : 1.f) : 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int i = i0 + k * 256 + tid;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) x[k * VEC + e] = BOTH ? g.at(x[k * VEC + e]) : x[k * VEC + e] * down;
+    for (int e = 0; e < VEC; ++e) x[k * VEC + e] = BOTH ? g.at(x[k * VEC + e]) : some ? x[k * VEC + e] * down : 0.f;
     if (VEC > 1 && i < i1 && (i + 1) * VEC <= a.V) {
       if (VEC == 8)
         *reinterpret_cast<uint4*>(drow + (long long)i * VEC) =
@@ -598,7 +599,17 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       if (kh != 0.f) g += di_ex2(fmaf(z, lt, lup)) * kh;
       return g;
     };
-    const float down = !BOTH ? (ks + kh) * against(m, ct, up) : 0.f;
+    float down = !BOTH ? (ks + kh) * against(m, ct, up) : 0.f;
+    // a row without terms is zeros, whatever its logits are (0 x NaN otherwise; BOTH: the stores' bits, since values set to zero cost every row 5 %, these 3)
+    const bool none = cs == 0.f && ch == 0.f;
+    const uint32_t keep = BOTH && none ? 0u : ~0u;
+    if (!BOTH && none) {
+      down = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) raw[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < HELD_PAIRS; ++k) held[k] = make_float2(0.f, 0.f);
+    }
     const float2 down2 = make_float2(down, down), c2 = make_float2(ct, ct), l2 = make_float2(lt, lt), up2 = make_float2(up, up), lup2 = make_float2(lup, lup);
     const float2 ks2 = make_float2(ks, ks), kh2 = make_float2(kh, kh);
     bf16* out = drow + (long long)(i0 + tid) * VEC;
@@ -614,7 +625,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
         } else {
           y = mul2(y, down2);
         }
-        p[q] = pack_bf16x2(y.x, y.y);
+        p[q] = pack_bf16x2(y.x, y.y) & keep;
       }
       if (k * 256 + tid < whole) {
         if (VEC == 8) *reinterpret_cast<uint4*>(out + k * 256 * VEC) = make_uint4(p[0], p[1], p[2 % (VEC / 2)], p[3 % (VEC / 2)]);
@@ -622,9 +633,9 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
       }
     }
     if (tail_here)
-      for (int e = 0; e < tail; ++e) drow[(i0 + whole) * VEC + e] = __float2bfloat16_rn(grad((float)part[whole * VEC + e]));
+      for (int e = 0; e < tail; ++e) drow[(i0 + whole) * VEC + e] = __float2bfloat16_rn(none ? 0.f : grad((float)part[whole * VEC + e]));
     // the places that entries name lose the teacher's share, the label's its own.  Of entries with one id the first writes, of the label and entries these.
-    if (here) {
+        if (here) {
       const uint32_t word = (id - v0) >> 5, bit = 1u << ((id - v0) & 31);
       const bool label = ids[a.K] == id;
       float share = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm);
@@ -637,7 +648,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
             share += es_of[turn][o] * teacher_scale(from[rank * 8 + (o >> 5)].tm);
           }
       }
-      if (writes && (share != 0.f || (label && ch != 0.f))) {
+      if (writes && ((share != 0.f && cs != 0.f) || (label && ch != 0.f))) {
         late_id[tid] = id;
         late_value[tid] = grad(z) - (soft ? cs * (share / ts) : 0.f) - (label ? ch : 0.f);
       }
