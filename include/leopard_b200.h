@@ -998,7 +998,8 @@ int lp_tree_attention(const lp_tree_attn_desc* desc, void* workspace, size_t ws_
 /* Speculative sampling over a tree, from given random numbers u in [0, 1): the walk starts at node 0 with P = target row 0.  The children c of the node where it
  * stands are tried in their order: c is accepted when u[b][c] * q(x) < P(x), x = tokens[b][c] and q the draft's row of that node (draft NULL: drafts that
  * were not drawn, q(x) = 1); the walk goes there with P = target row c.  A refused child takes P = max(P - q, 0) / its sum (draft NULL: P without x), unless
- * nothing would be left.  Where no child is accepted the next token is the first v with P(0) + ... + P(v) > u[b][0] sum(P).
+ * nothing would be left.  The target's distribution is kept where the children of a node were drawn from q independently of one another, with replacement; children drawn without
+ * replacement, or a draft NULL for drafts that were drawn, give another distribution.  Where no child is accepted the next token is the first v with P(0) + ... + P(v) > u[b][0] sum(P).
  * path[b][T]: the accepted nodes, node 0 first, -1 behind them; count[b] their number (0 where nodes[b] is 0); next[b] the token (-1 where P has no
  * sum).  Row i of target and draft, fp32 [V], is the distribution after node i; negative and NaN probabilities count as 0.  A token outside [0, V) is
  * refused and takes nothing away.  Choices are made in 64 bits.  uniform fp32, tokens, parents [B][T] contiguous; T <= 1024. */

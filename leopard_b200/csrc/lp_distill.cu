@@ -635,7 +635,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     if (tail_here)
       for (int e = 0; e < tail; ++e) drow[(i0 + whole) * VEC + e] = __float2bfloat16_rn(none ? 0.f : grad((float)part[whole * VEC + e]));
     // the places that entries name lose the teacher's share, the label's its own.  Of entries with one id the first writes, of the label and entries these.
-        if (here) {
+    if (here) {
       const uint32_t word = (id - v0) >> 5, bit = 1u << ((id - v0) & 31);
       const bool label = ids[a.K] == id;
       float share = es_of[turn][tid] * teacher_scale(from[rank * 8 + warp].tm);

@@ -668,7 +668,8 @@ def _verify_refusals(target, tokens, parents, uniform, draft, nodes):
 
 def verify_draft(target, tokens, parents, uniform, draft=None, nodes=None):
     """Which drafted nodes the target accepts, and the token after them (lp_verify_draft): target fp32 [B, T, V], row i the target's probabilities after node i;
-    draft of the same shape, what the children of node i were drawn from (None: drafts that were not drawn, such as the best of a list); tokens
+    draft of the same shape, what the children of node i were drawn from, each independently of the others and with replacement, which is what keeps the target's distribution
+    (children drawn without replacement do not); None: drafts that were not drawn, such as the best of a list; tokens
     int64, parents int32, uniform fp32 (numbers in [0, 1): [b, c] tries node c, [b, 0] takes the next token) [B, T]; nodes int32 [B] or None.
     -> (path int32 [B, T]: the accepted nodes from node 0 on, then -1; count int32 [B]; next token int64 [B])."""
     try:
