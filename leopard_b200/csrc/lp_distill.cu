@@ -233,8 +233,8 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
   float top_m = m;
   if (ctas > 1) {
     if (tid == 0) shared_sums = make_float3(m, s, s1);
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncwarp();                           // (the cluster's barrier is for whole warps)
+    cluster_sync_all();
     float3 part[8];
     const uint32_t here = smem_u32(&shared_sums);
 #pragma unroll
@@ -248,6 +248,7 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
       }
       top_m = fmaxf(top_m, part[q].x);
     }
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA has read; it stays until the others have (below)
     s = s1 = 0.f;
 #pragma unroll
@@ -283,6 +284,7 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
   __syncthreads();
   named_places(a, g, row, drow, top, id, y, v0, v1);
   if (rank == 0) row_loss(a, r, soft, top_m, s, s1, row, top, lt, id, y, red);
+  __syncwarp();
   if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -432,6 +434,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     if (late_id[tid] >= 0) a.dlogits[(long long)row_before * a.ldd + late_id[tid]] = __float2bfloat16_rn(late_value[tid]);
     late_id[tid] = -1;
   };
+  __syncwarp();
   if (ctas > 1) cluster_sync_all();                                                 // no CTA sends to one that has not started
   auto send = [&](uint32_t turn, float m, float s, float s1, float tm, float ts) {
     __syncwarp();
