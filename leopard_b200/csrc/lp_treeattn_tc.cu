@@ -346,7 +346,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (SPLIT && q == 1 && joins > 0) tt_bar_sync(3, 256);           // stream 0 has taken out what this one had of its last piece
       float m_used = -INFINITY, l_sum = 0.f;
       uint32_t v[64];
-      mbar_wait(&s_full[q * 2], nt & 1);
+      mbar_wait_warp(&s_full[q * 2], nt & 1);                          // (loads from and stores to TMEM are for whole warps, here and below)
       tc_fence_after();
       LP_TMEM_LD_32((v + 0), s_addr + 0);
       LP_TMEM_LD_32((v + 32), s_addr + 32);
@@ -400,6 +400,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
           fence_proxy_async_smem();
+          __syncwarp();
           if (both) tt_bar_sync(1, 256);
         }
         tmem_wait_ld();
@@ -447,7 +448,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           m_used = m_new;
         } else if (__any_sync(0xffffffffu, grow)) {
           // every product issued so far has to be done before O is scaled in place
-          mbar_wait(&pv_done[q * 2 + (h ^ 1)], (nt + ((t - 1) >> 1)) & 1);
+          mbar_wait_warp(&pv_done[q * 2 + (h ^ 1)], (nt + ((t - 1) >> 1)) & 1);
           tc_fence_after();
           float alpha = 1.0f;
           if (grow) {
@@ -455,6 +456,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             m_used = m_new;
             l_sum *= alpha;
           }
+          __syncwarp();
 #pragma unroll 1
           for (int c = 0; c < DH / 16; ++c) {
             uint32_t o[16];
@@ -494,7 +496,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           else if (has_next) tt_bar_arrive(4, 256);
         }
         bool loaded = false;
-        if (s_ready || (has_next && mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1))) {
+        if (has_next && __all_sync(0xffffffffu, s_ready || mbar_test_wait(&s_full[q * 2 + hn], (nt + tn) & 1))) {
           tc_fence_after();
           LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
           LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
@@ -509,7 +511,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           l_sum += a0 + a1;
         }
         if (has_next && !loaded) {
-          mbar_wait(&s_full[q * 2 + hn], (nt + tn) & 1);
+          mbar_wait_warp(&s_full[q * 2 + hn], (nt + tn) & 1);
           tc_fence_after();
           LP_TMEM_LD_32((v + 0), s_addr + hn * 64 + 0);
           LP_TMEM_LD_32((v + 32), s_addr + hn * 64 + 32);
@@ -526,12 +528,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         ++joins;
         continue;
       }
-      mbar_wait(&o_done[q], pieces & 1);
+      mbar_wait_warp(&o_done[q], pieces & 1);
       ++pieces;
       float f0 = 1.f, f1 = 0.f;
       if (two) {
         tt_bar_sync(2, 256);
-        mbar_wait(&o_done[1], joins & 1);
+        mbar_wait_warp(&o_done[1], joins & 1);
         ++joins;
         const float2 x = other[r];
         const float m = fmaxf(m_used, x.x);
@@ -552,6 +554,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll 1
       for (int c = 0; c < DH / 32; ++c) {
         uint32_t o[32], y[32];
+        __syncwarp();
         LP_TMEM_LD_32(o, o_addr + c * 32);
         if (two) LP_TMEM_LD_32(y, o_addr + 128 + c * 32);
         tmem_wait_ld();
