@@ -160,7 +160,7 @@ __device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, float w, bool 
 // Bound by HBM: logits in, gradient out, once each.  A row is held by the registers of up to 8 CTAs (a cluster), 64 values a thread, between the sums and the gradient
 // that needs them; the CTAs tell one another their maximum and sums through their shared memory.  All loads of a row are in flight at once.
 // VEC values a load: 16 bytes where all rows start on 16 (and the gradient's on 8), else single values.  BOTH: a temperature and labels, two exponentials a value.
-// For rows that do not start on 16 bytes (2,048 x 32,003 fp32 192 us, 2 TB/s; bf16 291) and more than 255 entries (2,048 x 32,000 with 300 277 us): the next kernel takes what it can.
+// For rows that do not start on 16 bytes (2,048 x 32,003 fp32 194 us, 2 TB/s; bf16 295) and more than 255 entries (2,048 x 32,000 with 300 280 us, of bf16 318): the next kernel takes what it can.
 constexpr int DISTILL_HELD = 64;
 template <typename T, int VEC, bool BOTH>
 __global__ void __launch_bounds__(256, 2)
@@ -295,10 +295,10 @@ distill_held_kernel(const __grid_constant__ DistillArgs a, int ctas) {
 // It has one wait: every WARP sends its maximum and sums, against its own maximum, to all CTAs of the cluster (st.async on a barrier of the receiver), and takes the
 // row's from the 8 x CTAs entries that arrive.  (Block sums, a barrier of the cluster and sums of sums took 4 of 7 us a row; the barrier alone 0.7, since it waits for the
 // row before to be stored.)  A warp's part of the row's loss, which needs the row's sums, goes along with the next row's.
-// This kernel and the one above (us, 64 entries): 300 rows of 32,000 fp32 14.6 and 22.7, 2,048 68.8 and 140, of bf16 61.7 and 176; 4,096 of 1,000 38 and 91; 512 of 128,256 72 and
-// 145; one of 32,000 7.0 and 7.0.
-// Measured: 4,096 rows of 128,256 fp32 logits, 64 entries, 518 us, 6.1 TB/s of logits read and gradient written (a copy's rate would be 489); 2,048 x 32,000, the label too, 70.7
-// (60.9), at another temperature and 60 % of the rows 68 (45); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
+// This kernel and the one above (us, 64 entries): 300 rows of 32,000 fp32 15.3 and 22.8, 2,048 68.8 and 142, of bf16 62.6 and 177; 4,096 of 1,000 37 and 104; 512 of 128,256 73 and
+// 149; one of 32,000 7.4 and 7.6.
+// Measured: 4,096 rows of 128,256 fp32 logits, 64 entries, 519 us, 6.1 TB/s of logits read and gradient written (a copy's rate would be 489); 2,048 x 32,000, the label too, 69.0
+// (60.9), at another temperature and 60 % of the rows 71 (45), of all rows 99 (61); of bf16 logits 4,096 x 32,000 in 119 (81), where the exponentials and the chain of a row are longer than its bytes.
 constexpr int RING_TOP = 255;
 constexpr int RING_LIST = 1536, RING_LOOK = 1024;      // rows that a cluster knows to be its own; weights that are looked at at once
 struct __align__(16) RingEntry {             // of a warp: maximum and sums of the row; the teacher's maximum
@@ -490,7 +490,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
     if (tail_here)
       for (int e = 0; e < tail; ++e) part[whole * VEC + e] = row[(i0 + whole) * VEC + e];
     // pairs of values, in two-wide arithmetic, loads and stores at fixed offsets: what bounds a row is the instructions of its 64 values a thread (1,180 a warp and row with single
-    // values, a branch a load and z - max taken before the factor: 699 us instead of 518 for 4,096 x 128,256 of fp32)
+    // values, a branch a load and z - max taken before the factor: 699 us instead of 519 for 4,096 x 128,256 of fp32)
     uint4 raw[N];                                                                   // (as they come: bf16 pairs are taken apart where they are used)
     constexpr int HELD_PAIRS = !BOTH && sizeof(T) == 2 ? HELD / 2 : 1;
     float2 held[HELD_PAIRS];
@@ -680,7 +680,7 @@ distill_ring_kernel(const __grid_constant__ DistillArgs a, int ctas, int rows) {
   store_late();
 }
 
-// ---- longer rows: a CTA reads its row three times, mostly from the L2 (512 x 300,000 fp32 711 us, 1.3 TB/s of what has to be read and written) ---------------
+// ---- longer rows: a CTA reads its row three times, mostly from the L2 (512 x 300,000 fp32 710 - 725 us, 1.3 TB/s of what has to be read and written) ---------------
 template <typename T>
 __global__ void __launch_bounds__(256)
 distill_long_kernel(const __grid_constant__ DistillArgs a) {
@@ -780,7 +780,7 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
   rc = both ? launch_ring<distill_ring_kernel<T, true, HELD>>(a, rows, ctas, (size_t)256 * HELD * size, stream) \
             : launch_ring<distill_ring_kernel<T, false, HELD>>(a, rows, ctas, (size_t)256 * HELD * size, stream)
       // few values a thread leave registers for more CTAs an SM, five and three: 4,096 rows of 1,000 fp32 37.5 us (57.9 with 64), 3,000 of 8,000 39 (50), of 4,000 with a
-      // temperature and labels 48 (71), of 2,048 bf16 34 (72); where a row has several CTAs either way their messages cost more (1,000 of 60,000 fp32 89 us with 32, 68 with 64)
+      // temperature and labels 49.5 (71), of 2,048 bf16 35 (72); where a row has several CTAs either way their messages cost more (1,000 of 60,000 fp32 89 us with 32, 68 with 64)
       if (V <= 256 * 8) { if (logits_fp32) LP_RING(float, 8); else LP_RING(bf16, 8); }
       else if (V <= 256 * 32) { if (logits_fp32) LP_RING(float, 32); else LP_RING(bf16, 32); }
       else { if (logits_fp32) LP_RING(float, DISTILL_HELD); else LP_RING(bf16, DISTILL_HELD); }

@@ -28,7 +28,8 @@ template <int N>
 __device__ __forceinline__ void ta_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // WM x WN warps: 16 WM rows, the 64 keys of a tile dealt to WN warps.  Two CTAs an SM, each with three stages of keys and values on their way.  Bound by HBM for long caches: one node
-// of 64 sequences of 4,000 rows, 32 heads over 8, 187 us, 5.6 TB/s; of one after 100,000 rows 86, 4.8.  Short ones by latency: one node after 512 rows 9.3 us.
+// of 64 sequences of 4,000 rows, 32 heads over 8, 188 us, 5.6 TB/s; of one after 100,000 rows 87, 4.7.  Short ones by latency: one node after 512 rows 9.3 us.  Many short ones by the ends
+// of pieces: one node of 64 sequences of 512 rows, 512 items of 9 tiles on 296 CTAs, 44 us where their bytes take 21.
 template <int D, int WM, int WN>
 __global__ void __launch_bounds__(32 * WM * WN, 2)
 tree_attn_kernel(const __grid_constant__ TreeArgs a) {
@@ -294,8 +295,9 @@ tree_attn_kernel(const __grid_constant__ TreeArgs a) {
 
 // Rows whose tiles lie in several CTAs: a CTA joins groups of 8 rows of a key head, a thread four columns of a row over all pieces.  Bound by latency: ten pieces of a group, two
 // of each of four or five of each of two are under way at once; weights follow a running maximum, so that each is read once.  A CTA takes 1 to 2 us for the line of tiles before it can
-// join.  Few CTAs have done so when the pieces' kernel ends; of more than run at once (8 an SM) each takes four groups (64 nodes of 48 sequences of 1,000 rows 121 us in all, 161
-// with one; 26 nodes of 6 sequences, 624 CTAs with one group, 44.8 with one and 50.9 with four).
+// join.  Few CTAs have done so when the pieces' kernel ends; of more than run at once (8 an SM) each takes four groups (64 nodes of 48 sequences of 1,000 rows 122 us in all, 161
+// with one; 26 nodes of 6 sequences, 624 CTAs with one group, 44.8 with one and 50.9 with four).  Each CTA's line has all sequences, so the cost grows with the square of the batch: one
+// node after 64 rows of 64 sequences 20 us, of 256 76, of 512 258, of 1,024 612, of 2,048 1,617 (their bytes take 3, 11, 22, 45 and 90).
 constexpr int TA_JOIN_ROWS = 8, TA_JOIN_GROUPS = 4;
 template <int N>
 struct TreeN { static constexpr int value = N; };
@@ -374,9 +376,10 @@ tree_join_kernel(const __grid_constant__ TreeArgs a) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-// which kernel: tcgen05 for more rows than TREE_TC_ROWS where it takes the cache.  mma.sync and tcgen05 (us, 32 heads over 8, nodes x 4 rows): 16 rows of one sequence of 512 rows
-// 9.7 and 12.2, 8 of 1,000 18.6 and 20.3, 48 of 1,000 56 and 69, 48 of 4,000 152 and 170; 32 rows 10.1 and 12.1, 20.1 and 20.6, 71 and 74, 197 and 176; 36 rows 11.5 and 12.1, 24.7
-// and 20.7, 97 and 76, 274 and 179; 128 rows 12.4 and 12.7, 48 and 31, 207 and 111, 542 and 208.
+// which kernel: tcgen05 for more rows than TREE_TC_ROWS where it takes the cache.  mma.sync and tcgen05 (us, 32 heads over 8, nodes x 4 rows), of one sequence of 512 rows, one of 20,000, 8 of
+// 1,000, 8 of 4,000, 48 of 1,000, 48 of 4,000: 16 rows 9.3 and 12.6, 27.1 and 27.2, 18.5 and 21.4, 38 and 46, 57 and 74, 153 and 174; 32 rows 9.9 and 12.7, 34.2 and 27.7, 20.3 and 21.7,
+// 44.5 and 45.5, 64 and 74, 184 and 175; 36 rows 11.3 and 12.9, 43.5 and 28.3, 25.9 and 22.0, 63 and 46, 96 and 76, 272 and 178; 128 rows 12.1 and 13.6, 67 and 29, 47 and 31, 110 and 55, 188 and
+// 94, 525 and 189.  At 32 rows length decides as much as rows do: the rule loses a fifth after 20,000 rows and a twentieth at 48 of 4,000, and wins up to a seventh at the others.
 constexpr int TREE_TC_ROWS = 32;
 static bool tree_tc(const lp_tree_attn_desc* d) { return (long long)d->T * (d->H / d->KVH) > TREE_TC_ROWS && tree_tc_takes(d); }
 // rows of a block: what the widest tree needs, 64 (256) at most

@@ -2,8 +2,8 @@
 //
 // The keys of an item (sequence, key head, block of rows) are cut into tiles; the tiles of all items stand in one line, of which every CTA takes an equal range: sequences
 // of any lengths load all SMs alike.  Few items are dealt out whole, each with CTAs of its own, where the longest range is then little above an equal share: a range that goes on
-// in another item costs the ends of two pieces, and a split item its join (26 nodes of 11 sequences of up to 5,000 rows 49.8 us and 53.7 without, 64 nodes of them 65 and 81; one
-// node after 4,796 rows 16.3 and 20.8).  Where a CTA's range ends inside an item its rows' running maximum, sum and weighted values go to the workspace, to be joined.  Which CTAs
+// in another item costs the ends of two pieces, and a split item its join (26 nodes of 11 sequences of up to 5,000 rows 50.4 us and 60.3 without, 64 nodes of them 66 and 76; one
+// node after 4,796 rows 16.2 and 22.3).  Where a CTA's range ends inside an item its rows' running maximum, sum and weighted values go to the workspace, to be joined.  Which CTAs
 // an item has follows from the lengths alone, in every kernel.
 #pragma once
 #include "lp_common.cuh"
@@ -75,8 +75,9 @@ __device__ __forceinline__ int tree_cta_of(long long total, long long unit, int 
 // CTAs of an item of `tiles` tiles, where items have CTAs of their own: `most` tiles each
 __device__ __forceinline__ int tree_own(int tiles, int most) { return tree_div32(tiles + most - 1, most); }
 // For items to have CTAs of their own the longest range may have this many tiles above an equal share: of 64 and of 128 keys, the latter looked for in steps of two.  A tile is 1 to
-// 2 us, the end of a piece and its join 6 to 12 (64 nodes of 12 sequences of 3,000 rows, 8.4 tiles above: 79.9 and 76.5 as a line; of 10, 11 above: 79.8 and 66.7; of 14 of 1,000
-// rows, 1.8 above: 41.6 and 65).
+// 2 us, the end of a piece and its join 6 to 12 (CTAs of their own, and as a line: 64 nodes of 14 sequences of 1,000 rows, 1.8 tiles above: 37.4 us and 56.1; of 12 of 3,000, 8.4 above: 75.4
+// and 75.0; of 10 of 3,000, 11 above: 75.1 and 67.5).  The limits were found on such batches and are not the best for each: 26 nodes of 10 or 12 sequences of 3,000 rows stay a line, 53.1 and 56.6 us
+// where own CTAs take 49.2 and 51.9; 8 nodes of 10 have their own, 43.7 where a line takes 43.0.
 constexpr int TREE_SLACK = 3, TREE_SLACK_TC = 6;
 __device__ __forceinline__ int tree_slack(const TreeArgs& a) { return a.key_bits == 7 ? TREE_SLACK_TC : TREE_SLACK; }
 // by one warp, in shared memory.  Ends in the block's barrier.

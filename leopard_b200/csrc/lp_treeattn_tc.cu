@@ -5,13 +5,13 @@
 // while the softmax is at this one.  Of up to 256 rows (node x query head of a key head) each stream has a half, on the same keys; up to 128 rows (SPLIT) are
 // the rows of both streams, which take the tiles in turn and join their sums at the end of a piece: alone, a stream is bound by the latency of its chain
 // S -> softmax -> P V (1.8 us a tile, where reading 64 KB at an SM's share of HBM takes 1.5; 8 sequences of 8,000 rows, 9 to 32 nodes,
-// 61 to 70 us and 65 to 75 without; 24 of 4,000 90 to 108 and 100 to 118).
+// 67 to 77 us and 77 to 84 without; 24 of 4,000 90 to 99 and 99 to 108).
 //   warp 0       TMA producer: K_j, V_j into rings of two (SPLIT: three), a box a page or part of one; pages that are not there come as zeros
 //   warp 1 / 2   MMA issuer of stream 0 / 1:  S(j).h = Q K_j[h]^T,  O += P(j).h V_j[h] (P in TMEM)
 //   warp 3       TMEM
 //   warps 4-7, 8-11   softmax of stream 0 / 1: a thread a row; they also bring the rows' queries (rows of a product are G heads of each node) and take O out
-// Bound by HBM for few rows of long caches (13 nodes of two sequences of 100,003 rows 140 us, 5.8 TB/s), by the softmax's exponentials for many (64 nodes of 8 of 8,191 rows, 32
-// heads over 8, 103 us, 660 TFLOP/s); by the ends of pieces, 6 to 12 us each, in between (64 nodes of 8 sequences of 2,414 to 8,191 rows 71 us, where its bytes take 24).
+// Bound by HBM for few rows of long caches (13 nodes of two sequences of 100,003 rows 143 us, 5.7 TB/s), by the softmax's exponentials for many (64 nodes of 8 of 8,191 rows, 32
+// heads over 8, 103 us, 660 TFLOP/s); by the ends of pieces, 6 to 12 us each, in between (64 nodes of 8 sequences of 2,414 to 8,191 rows 72 us, where its bytes take 24).
 // TMEM: S0 [0, 128) S1 [128, 256) O0 [256, 384) O1 [384, 512).
 // Only the last tiles of an item, which hold nodes or reach past them, look at masks; there V is searched before its product: rows behind the keys become zeros (a
 // cache's unwritten memory may hold anything), and values that are not finite are taken out and reach the rows that see them when O is taken out.
@@ -23,7 +23,7 @@ constexpr int TT_BOX = 128 * 128;      // 128 rows x 64 bf16
 constexpr int TT_THREADS = 384;
 constexpr int TT_KEYS = 128;
 constexpr int TT_MAX_BATCH = 1024;      // sequences whose line of tiles fits beside the tiles
-constexpr int TT_SPLIT_BATCH = 24;      // sequences whose line of tiles leaves room for three stages
+constexpr int TT_SPLIT_BATCH = 24;      // sequences whose line of tiles leaves room for three stages (9 to 32 nodes of 24 of 4,000 rows 90 to 99 us, of 25 106 to 113)
 
 #define LP_TT_TMEM_ST_16(regs, taddr)                                                                               \
   asm volatile(                                                                                                     \
