@@ -1020,10 +1020,11 @@ int lp_cache_compact(const void* const* pools, long long pool_step, int n_pools,
 int lp_cache_copy_pages(const void* const* pools, long long pool_step, int n_pools, long long page_stride, long long page_bytes, int n_pages, const int* src,
                         const int* dst, int n, void* stream);
 
-/* Distillation from a teacher's K top logits a row (K <= 1024), beside lp_ce_fwd_bwd: with t = softmax(teacher / temperature) over the entries whose id lies in [0, V)
+/* Distillation from a teacher's K top logits a row (K <= 1024), beside lp_ce_fwd_bwd, at temperatures from 1e-6 to 1e6: with t = softmax(teacher / temperature) over the entries whose id lies in [0, V)
  * and p = softmax(logits / temperature),
  *   loss[r] = (1 - hard) temperature^2 sum_k t_k (log t_k - log p[id_k]) + hard * (cross entropy of target[r]),
  *   dlogits[r] = weight[r] * its gradient, bf16; columns V..Vp-1 receive 0.
+ * Logarithms are fp32: the loss is off by about 2^-22 temperature^2 (20 + the largest logit / temperature).
  * Rows of weight 0 are zeros and their logits are not read.  A row without such entries has no first term, one whose target lies outside [0, V) no second (target
  * NULL with hard 0).  ids int32 or int64 (ids_64), an id may come twice; teacher and logits fp32 or bf16. */
 int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long ld, const void* ids, int ids_64, long long ld_ids,

@@ -760,7 +760,8 @@ extern "C" int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long
              DISTILL_MAX_TOP, ld_ids, ld_teacher);
   LP_REQUIRE(Vp >= V && Vp % 2 == 0 && ldd % 2 == 0 && ldd >= Vp && ld >= V && (reinterpret_cast<uintptr_t>(dlogits) & 3) == 0,
              "lp_distill_fwd_bwd: Vp=%d must be even and >= V=%d, ldd=%lld even and >= Vp", Vp, V, ldd);
-  LP_REQUIRE(temperature > 0.f && temperature <= 3.0e38f, "lp_distill_fwd_bwd: temperature %g must be positive", (double)temperature);
+  // (the product of a maximum up to 1e30 and its factor, up to 2 log2(e) / temperature, is finite, and so is the square)
+  LP_REQUIRE(temperature >= 1e-6f && temperature <= 1e6f, "lp_distill_fwd_bwd: temperature %g must lie in [1e-6, 1e6]", (double)temperature);
   LP_REQUIRE(hard >= 0.f && hard <= 1.f && (hard == 0.f || target), "lp_distill_fwd_bwd: a hard share of %g needs labels and lies in [0, 1]", (double)hard);
   DistillArgs a = {logits, ld, ids, ids_64, ld_ids, teacher, teacher_fp32, ld_teacher, K, weight, target, 1.f / temperature, temperature, hard, loss, reinterpret_cast<bf16*>(dlogits), ldd, V, Vp};
   note_launch();

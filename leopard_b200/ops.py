@@ -790,7 +790,7 @@ def _distill_refusals(logits, ids, teacher, weight, vocab, target):
 def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target=None, hard=0.0):
     """Loss against a teacher's top logits, and its gradient, beside ce_fwd_bwd (lp_distill_fwd_bwd): logits [R, Vp] (fp32 or bf16; columns >= vocab are padding), ids
     int64 or int32 [R, K] and teacher fp32 or bf16 [R, K] the teacher's best tokens and their logits (ids outside [0, vocab): missing entries; K <= 1024), weight fp32
-    [R] (rows of weight 0 are skipped), target int64 [R] labels for the share `hard` of the loss.
+    [R] (rows of weight 0 are skipped), temperature from 1e-6 to 1e6, target int64 [R] labels for the share `hard` of the loss.
     loss = (1 - hard) temperature^2 KL(softmax(teacher / temperature) || softmax(logits / temperature)) + hard CE(target)
     -> (loss [R] fp32, dlogits bf16 [R, Vp], weighted as in ce_fwd_bwd)."""
     try:

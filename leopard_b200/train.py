@@ -144,8 +144,8 @@ class SFTTrainer:
         self.dev = engine.device
         self.hp = dict(lr=lr, min_lr=min_lr, warmup=warmup_iters, decay=decay_iters, beta1=beta1, beta2=beta2, eps=eps,
                        wd=weight_decay, clip=clip_grad)
-        if not distill_temperature > 0 or not 0 <= distill_hard <= 1:
-            raise ValueError(f"distill_temperature must be positive and distill_hard in [0, 1], got {distill_temperature} and {distill_hard}")
+        if not 1e-6 <= distill_temperature <= 1e6 or not 0 <= distill_hard <= 1:
+            raise ValueError(f"distill_temperature must lie in [1e-6, 1e6] and distill_hard in [0, 1], got {distill_temperature} and {distill_hard}")
         self.distill = (distill_temperature, distill_hard)
         self.freeze_llm = freeze_llm
         self.pg = process_group

@@ -1,4 +1,6 @@
 """A step whose teacher is refused is none: nothing of it counts, and the next one is as if it had not been asked for.  On the CPU with every native op restated (oracle)."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -31,3 +33,12 @@ def test_a_refused_teacher_is_no_step(cpu):  # noqa: F811
     for _ in range(3):
         assert tr.step(*both, teacher=[good, None]) == fresh.step(*both, teacher=[good, None])
     assert tr.iteration == 3
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 9e-7, 1.1e6, 1e20, float("inf"), float("nan"), -1.0])
+def test_temperatures_that_products_or_squares_do_not_hold(native_lib, cpu, temperature):  # noqa: F811
+    with pytest.raises(ValueError, match="distill_temperature"):
+        T.SFTTrainer(cpu[1](), distill_temperature=temperature)
+    L, p = native_lib, C.c_void_p(1 << 20)
+    assert L.lp_distill_fwd_bwd(p, 1, 16, p, 1, 2000, p, 1, 2000, 4, p, None, temperature, 0.0, p, p, 10, 2, 10, 10, None) == -1
+    assert b"temperature" in L.lp_last_error()
