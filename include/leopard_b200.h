@@ -1031,6 +1031,46 @@ int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long ld, const 
                        const void* teacher, int teacher_fp32, long long ld_teacher, int K, const float* weight, const long long* target,
                        float temperature, float hard, float* loss, void* dlogits, long long ldd, int rows, int V, int Vp, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Serving many continuations of one prompt: a step's index tables and cache pages, rotary positions and the cache rows that they end in, attention of a batch over the
+ * prefix that it shares, the next tokens.  (The reference decodes one request, one token a step.)
+ * ------------------------------------------------------------------------------------------------------------------ */
+/* Request b has lengths[b] cached rows and brings fresh[b] tokens (0: it waits; negative numbers count as 0), whose rows stand one request after the other: row0[b]
+ * [B + 1] is its first.  Entries of its new rows' pages in page_table [B][ld] (int32, max_pages a request) that are negative get free_pages[used[0]], free_pages[used[0] + 1], ... in the order of
+ * requests and pages, and used[0] grows by their number; when the list is over they stay as they were.  Row r < `rows`: row_seq[r] its request, row_pos[r] its position, slots[r] =
+ * page * page_size + row of the page, -1 where it has no page; all three -1 behind the last row.  Rows that do not fit into `rows` have pages but no entries. */
+int lp_step_tables(const int* lengths, const int* fresh, int* page_table, long long ld_table, int max_pages, int page_size, const int* free_pages, int n_free, int* used, int B, int rows,
+                   int* row_seq, int* row_pos, long long* slots, int* row0, void* stream);
+
+/* y = x with the first 2 n_freq dimensions of every head turned by its row's position: pair (i, i + n_freq), or (2i, 2i + 1) if interleaved, by the angle positions[row] * inv_freq[i], times
+ * `scale`; inverse: by minus the angle (the gradient of the turn).  Angles are formed in 64 bits.  x, y fp32 or bf16 [rows][heads][D] with strides in elements, the last dimension contiguous; y may be
+ * x, and shares no memory with it otherwise. */
+int lp_rotary(const void* x, long long x_row, long long x_head, void* y, long long y_row, long long y_head, int fp32, int rows, int heads, int D, const void* positions, int positions_64,
+              const float* inv_freq, int n_freq, int interleaved, float scale, int inverse, void* stream);
+
+/* A step's queries and keys are turned as in lp_rotary; q goes to q_out (which may be q), k and v to the rows `slots` of the cache [n_pages][page_size][KVH][D]: slot = page * page_size + row
+ * (lp_step_tables).  Slots outside the cache: nothing is written.  Two rows with the same slot leave either's values there, or some of both.  Pools, q_out and the inputs share no memory. */
+typedef struct lp_rotary_append_desc {
+  const void* q; long long q_row, q_head;
+  void* q_out; long long o_row, o_head;
+  const void* k; long long k_row, k_head;
+  const void* v; long long v_row, v_head;
+  void* k_pool; long long kp_page, kp_row, kp_head;
+  void* v_pool; long long vp_page, vp_row, vp_head;
+  const void* positions; const float* inv_freq; const long long* slots;
+  int positions_64, n_freq, interleaved, fp32, rows, H, KVH, D, n_pages, page_size;
+  float scale;
+} lp_rotary_append_desc;
+int lp_rotary_append(const lp_rotary_append_desc* desc, void* stream);
+
+/* The next token of each row of logits (fp32 or bf16 [rows][ld], V <= 393216 words), by uniform[row] in [0, 1).  With w = exp((z - max z) / temperature) and the words in the order of their logits, the
+ * largest first, equal ones by index: the first top_k are kept (0: all); of them those before which less than top_p of their mass lies, the first in any case; of them those with
+ * w >= min_p; out[row] is the first kept word, by index, up to which more than uniform of the kept mass lies.  temperature 0 (negative, NaN): the largest, the first of equal ones.
+ * Weights are held in units of 2^-43 of the largest.  Settings of each row, or (NULL) one for all.  -inf and NaN are never drawn; of a row with +inf entries only these are; a row with nothing
+ * to draw gives -1. */
+int lp_sample_tokens(const void* logits, int logits_fp32, long long ld, const float* uniform, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
+                     const float* top_p, float top_p_all, const float* min_p, float min_p_all, int rows, int V, long long* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

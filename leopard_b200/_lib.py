@@ -143,6 +143,14 @@ class TreeAttnDesc(C.Structure):
                 ("mask", _vp), ("mask_batch", _ll), ("mask_node", _ll), ("B", _i), ("T", _i), ("H", _i), ("KVH", _i), ("D", _i), ("scale", _f)]
 
 
+class RotaryAppendDesc(C.Structure):
+    """lp_rotary_append_desc (include/leopard_b200.h)."""
+    _fields_ = [("q", _vp), ("q_row", _ll), ("q_head", _ll), ("q_out", _vp), ("o_row", _ll), ("o_head", _ll), ("k", _vp), ("k_row", _ll), ("k_head", _ll),
+                ("v", _vp), ("v_row", _ll), ("v_head", _ll), ("k_pool", _vp), ("kp_page", _ll), ("kp_row", _ll), ("kp_head", _ll), ("v_pool", _vp), ("vp_page", _ll),
+                ("vp_row", _ll), ("vp_head", _ll), ("positions", _vp), ("inv_freq", _vp), ("slots", _vp), ("positions_64", _i), ("n_freq", _i), ("interleaved", _i),
+                ("fp32", _i), ("rows", _i), ("H", _i), ("KVH", _i), ("D", _i), ("n_pages", _i), ("page_size", _i), ("scale", _f)]
+
+
 class MLSTMDesc(C.Structure):
     """lp_mlstm_desc (include/leopard_b200.h)."""
     _fields_ = [("proj", _vp), ("ld", _ll), ("q_off", _i), ("k_off", _i), ("v_off", _i), ("g_off", _i), ("i_off", _i), ("f_off", _i),
@@ -318,6 +326,10 @@ _SIGS = {
     "lp_tree_mask": (_i, [_vp, _ll, _i, _i, _vp, _vp, _vp]),
     "lp_tree_attention_workspace_bytes": (_sz, [_P(TreeAttnDesc)]),
     "lp_tree_attention": (_i, [_P(TreeAttnDesc), _vp, _sz, _vp]),
+    "lp_step_tables": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "lp_rotary": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _f, _i, _vp]),
+    "lp_rotary_append": (_i, [_P(RotaryAppendDesc), _vp]),
+    "lp_sample_tokens": (_i, [_vp, _i, _ll, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _i, _i, _vp, _vp]),
     "lp_verify_draft": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "lp_cache_compact": (_i, [_vp, _ll, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _vp, _ll, _vp, _i, _i, _vp]),
     "lp_cache_copy_pages": (_i, [_vp, _ll, _i, _ll, _ll, _i, _vp, _vp, _i, _vp]),

@@ -816,3 +816,171 @@ def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target
               1 if ids.dtype is _I64 else 0, max(ids.stride(0), K), teacher.data_ptr(), 1 if teacher.dtype is _F32 else 0, max(teacher.stride(0), K), K, weight.data_ptr(),
               None if target is None else target.data_ptr(), float(temperature), float(hard), loss.data_ptr(), d.data_ptr(), ld, R, vocab, ld)
     return loss, d
+
+
+# ---- serving many continuations of one prompt (csrc/lp_serve.cu, lp_sample.cu, lp_prefixattn.cu): a step's tables and pages, rotary positions and cache rows, attention over a prefix
+# that the batch shares, the next tokens ----------------------------------------------------------------------------------------------------------------------------------------------
+def step_tables(lengths, new, page_table, free, used, page_size, rows):
+    """The index tables of a step whose requests bring tokens, and the cache pages that these need (lp_step_tables): lengths int32 [B], cached rows; new int32 [B], tokens that each
+    brings (0: none); page_table int32 [B, max_pages] (negative: no page yet), which gets pages for the new rows, in place, from free int32 [n], of which used int32 [1] have been given
+    before (it grows; when the list is over, entries stay negative); rows: how many rows the step has room for.
+    -> (row_seq int32 [rows], row_pos int32 [rows], slots int64 [rows] = page * page_size + row of the page; row0 int32 [B + 1], each request's first row).  Rows that no request has are -1 in all
+    three, rows without a page in slots."""
+    B = lengths.shape[0] if isinstance(lengths, torch.Tensor) and lengths.dim() == 1 else -1
+    dev = getattr(lengths, "device", None)
+    try:
+        max_pages = page_table.shape[1]
+        fine = (lengths.is_cuda and all(t.dtype is _I32 and t.device == dev for t in (lengths, new, page_table, free, used)) and B >= 0 and lengths.is_contiguous() and new.shape == (B,)
+                and new.is_contiguous() and page_table.shape == (B, max_pages) and (page_table.stride(1) == 1 or max_pages <= 1) and (page_table.stride(0) >= max_pages or B <= 1)
+                and free.dim() == 1 and free.is_contiguous() and used.shape == (1,))
+    except (AttributeError, IndexError):
+        fine = False
+    if not fine:
+        for t, n in ((lengths, "lengths"), (new, "new"), (used, "used"), (free, "free")):
+            _need(t, n, (_I32,), 1, None if n in ("free", "lengths") else (1,) if n == "used" else lengths.shape, lengths.device if n != "lengths" else None, contiguous=True)
+        _need(page_table, "page_table", (_I32,), 2, (B, page_table.shape[-1]), lengths.device, rows=True)
+    for t, n in ((lengths, "lengths"), (new, "new"), (free, "free"), (used, "used")):
+        if _overlaps(page_table, t) or (t is not used and _overlaps(used, t)):
+            raise ValueError(f"{n} must not share memory with what the call changes")
+    rows = int(rows)
+    if rows < 0:
+        raise ValueError(f"rows must not be negative, got {rows}")
+    both = torch.empty((2, rows), dtype=_I32, device=dev)
+    slots = torch.empty((rows,), dtype=_I64, device=dev)
+    if B == 0:
+        return both[0].fill_(-1), both[1].fill_(-1), slots.fill_(-1), torch.zeros((1,), dtype=_I32, device=dev)
+    row0 = torch.empty((B + 1,), dtype=_I32, device=dev)
+    L = _lib.lib()
+    at = both.data_ptr()
+    _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), page_table.stride(0), max_pages, int(page_size), free.data_ptr(), free.numel(),
+          used.data_ptr(), B, rows, at, at + 4 * rows, slots.data_ptr(), row0.data_ptr())
+    return both[0], both[1], slots, row0
+
+
+def _apart(a, b):
+    """whether two tensors of the same number of dimensions and the same strides share no element (the parts of one product or of one pool, whose spans of memory meet)"""
+    if a.dtype != b.dtype or a.dim() != b.dim() or any(p < 0 or (p != q and m > 1 and n > 1) for p, q, m, n in zip(a.stride(), b.stride(), a.shape, b.shape)):
+        return False
+    dims = sorted(((q if m == 1 else p, m, n) for p, q, m, n in zip(a.stride(), b.stride(), a.shape, b.shape) if m > 1 or n > 1), reverse=True)
+
+    def meet(delta, dims):                    # element i of a and element j of b, delta behind: i s = j s + the rest
+        if not dims:
+            return delta == 0
+        (s, m, n), inner = dims[0], dims[1:]
+        reach = sum(t * (max(x, y) - 1) for t, x, y in inner)
+        if s <= reach:
+            return True                       # not nested: not known
+        q, r = divmod(delta, s)
+        return (-n < q < m and meet(r, inner)) or (-n < q + 1 < m and meet(r - s, inner))
+    return not meet((b.data_ptr() - a.data_ptr()) // a.element_size(), dims)
+
+
+def _rotary_check(x, name, dtypes, dim, device=None):
+    _need(x, name, dtypes, dim, device=device)
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+
+
+def _rotary_layout(layout):
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    return layout == "interleaved"
+
+
+def _rotary_rows(positions, inv_freq, rows, D, dev):
+    _need(positions, "positions", (_I32, _I64), 1, (rows,), dev, contiguous=True)
+    _need(inv_freq, "inv_freq", (_F32,), 1, device=dev, contiguous=True)
+    if 2 * inv_freq.numel() > D:
+        raise ValueError(f"{inv_freq.numel()} frequencies turn {2 * inv_freq.numel()} dimensions, heads have {D}")
+
+
+def rotary(x, positions, inv_freq, layout="half", scale=1.0, inverse=False, out=None):
+    """Rotary positions (lp_rotary): x bf16 or fp32 [rows, heads, D]; positions int32 or int64 [rows]; inv_freq fp32 [n] (seqlm.rotary_table has the scaled ones and their `scale`): the first
+    2 n dimensions of each head are turned, pairs (i, i + n) for layout "half" and (2 i, 2 i + 1) for "interleaved", and multiplied by `scale`.  inverse: turned back, which takes the gradient of the result to
+    that of x.  Angles are formed in 64 bits from the position.  out: x itself, or memory apart from it.  -> out."""
+    inter = _rotary_layout(layout)
+    _rotary_check(x, "x", (_BF16, _F32), 3)
+    rows, heads, D = x.shape
+    dev = x.device
+    _rotary_rows(positions, inv_freq, rows, D, dev)
+    if out is None:
+        out = torch.empty((rows, heads, D), dtype=x.dtype, device=dev)
+    else:
+        _rotary_check(out, "out", (x.dtype,), 3, dev)
+        if out.shape != x.shape:
+            raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+        if _overlaps(out, x) and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()):
+            raise ValueError("out must be x itself or share no memory with it")
+        if _overlaps(out, positions) or _overlaps(out, inv_freq):
+            raise ValueError("out must not share memory with positions or inv_freq")
+    if x.numel() == 0:
+        return out
+    L = _lib.lib()
+    _call(dev, L, "lp_rotary", L.lp_rotary, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), 1 if x.dtype is _F32 else 0, rows, heads, D,
+          positions.data_ptr(), 1 if positions.dtype is _I64 else 0, inv_freq.data_ptr(), inv_freq.numel(), int(inter), float(scale), int(bool(inverse)))
+    return out
+
+
+def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="half", scale=1.0, q_out=None):
+    """A step's queries and keys turned as by `rotary`, keys and values written to their cache rows in the same pass (lp_rotary_append): q [rows, H, D], k, v [rows, KVH, D] bf16 or fp32 (views of
+    one product, say); k_pool, v_pool of the same type [pages, page_size, KVH, D]; slots int64 [rows] (step_tables): page * page_size + row of the page, rows whose slot is no row of the pool are
+    left out; no slot comes twice.  -> q_out (q itself, if given so)."""
+    inter = _rotary_layout(layout)
+    _rotary_check(q, "q", (_BF16, _F32), 3)
+    rows, H, D = q.shape
+    dev = q.device
+    for t, n, dim in ((k, "k", 3), (v, "v", 3), (k_pool, "k_pool", 4), (v_pool, "v_pool", 4)):
+        _rotary_check(t, n, (q.dtype,), dim, dev)
+    G = k.shape[1]
+    if k.shape != (rows, G, D) or v.shape != k.shape or k_pool.shape[2:] != (G, D) or v_pool.shape != k_pool.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, k_pool {tuple(k_pool.shape)} and v_pool {tuple(v_pool.shape)} do not fit together")
+    _rotary_rows(positions, inv_freq, rows, D, dev)
+    _need(slots, "slots", (_I64,), 1, (rows,), dev, contiguous=True)
+    if q_out is None:
+        q_out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
+    else:
+        _rotary_check(q_out, "q_out", (q.dtype,), 3, dev)
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+        if _overlaps(q_out, q) and (q_out.data_ptr() != q.data_ptr() or q_out.stride() != q.stride()):
+            raise ValueError("q_out must be q itself or share no memory with it")
+    written = (k_pool, v_pool, q_out)
+    for i, w in enumerate(written):
+        for t in (q, k, v, positions, inv_freq, slots) + written[:i]:
+            if t is q and w is q_out and q_out.data_ptr() == q.data_ptr():
+                continue
+            if _overlaps(w, t) and not _apart(w, t):
+                raise ValueError("k_pool, v_pool and q_out must share no memory with one another nor with what the call reads")
+    if rows == 0 or D == 0 or k_pool.numel() == 0:
+        return q_out
+    s, o, ks, vs, kp, vp = q.stride(), q_out.stride(), k.stride(), v.stride(), k_pool.stride(), v_pool.stride()
+    d = _lib.RotaryAppendDesc(q.data_ptr(), s[0], s[1], q_out.data_ptr(), o[0], o[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], k_pool.data_ptr(), kp[0], kp[1], kp[2],
+                              v_pool.data_ptr(), vp[0], vp[1], vp[2], positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), 1 if positions.dtype is _I64 else 0, inv_freq.numel(),
+                              int(inter), 1 if q.dtype is _F32 else 0, rows, H, G, D, k_pool.shape[0], k_pool.shape[1], float(scale))
+    L = _lib.lib()
+    _call(dev, L, "lp_rotary_append", L.lp_rotary_append, C.byref(d))
+    return q_out
+
+
+def _setting(x, name, dtype, rows, dev):
+    """a number for all rows, or a tensor of one each -> (its address or None, the number)"""
+    if isinstance(x, torch.Tensor):
+        _need(x, name, (dtype,), 1, (rows,), dev, contiguous=True)
+        return x.data_ptr(), 0
+    return None, int(x) if dtype is _I32 else float(x)
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of each row from given random numbers (lp_sample_tokens): logits fp32 or bf16 [rows, V]; uniform fp32 [rows] in [0, 1).  temperature, top_p, min_p (numbers or fp32 [rows]) and
+    top_k (a number or int32 [rows]): of the words in the order of their logits, equal ones by index, the first top_k are kept (0: all), of them those before which less than top_p of their mass
+    lies, of them those at least min_p times as likely as the likeliest; drawn is the first kept word, by index, up to which more than `uniform` of the kept mass lies.  temperature 0 takes the largest
+    logit, the first of equal ones.  -> int64 [rows]; -1 for a row of -inf and NaN alone, which are never drawn.  V <= 393216."""
+    _need(logits, "logits", (_F32, _BF16), 2, rows=True)
+    R, V = logits.shape
+    dev = logits.device
+    _need(uniform, "uniform", (_F32,), 1, (R,), dev, contiguous=True)
+    settings = [*_setting(temperature, "temperature", _F32, R, dev), *_setting(top_k, "top_k", _I32, R, dev), *_setting(top_p, "top_p", _F32, R, dev), *_setting(min_p, "min_p", _F32, R, dev)]
+    out = torch.empty((R,), dtype=_I64, device=dev)
+    L = _lib.lib()
+    _call(dev, L, "lp_sample_tokens", L.lp_sample_tokens, logits.data_ptr(), 1 if logits.dtype is _F32 else 0, max(logits.stride(0), V), uniform.data_ptr(), *settings, R, V, out.data_ptr())
+    return out
