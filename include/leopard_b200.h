@@ -1063,6 +1063,30 @@ typedef struct lp_rotary_append_desc {
 } lp_rotary_append_desc;
 int lp_rotary_append(const lp_rotary_append_desc* desc, void* stream);
 
+/* out[b][t][h] = softmax_j(scale q[b][t][h] . k[j][g]) v[j][g], g = h / (H / KVH), over the `prefix` rows that all requests share and the request's own rows up to its token t.
+ * lengths[b]: the request's rows before its new tokens, the prefix among them (what is shorter counts as the prefix); fresh[b] (NULL: T): its new tokens, whose keys and values are the cache's next rows.
+ * All bf16, sums in fp32.  D = 64, 96 or 128; T <= LP_PREFIX_MAX_NEW; B T H <= 2^24.  Two forms:
+ *   page_table given: k, v are pages as in lp_tree_attention, row j of request b (the prefix's rows counted) lies in its pages; the prefix is read from request 0's, prefix_k and prefix_v are NULL;
+ *   page_table NULL: the prefix is prefix_k, prefix_v [prefix][KVH][D], own rows lie in page b (max_pages 1) from its row 0 on.
+ * Strides in elements, multiples of 8, the last dimension contiguous, 16-byte aligned bases.  Rows of pages that are not in [0, n_pages) are not seen, nor are rows behind the request's pages.
+ * A row that sees nothing is zeros; what a row does not see has no effect on it, NaN and infinities among it.  Rows t >= fresh[b] of out are not written; its rows share
+ * no memory with one another nor with the inputs.  workspace: lp_prefix_attention_workspace_bytes(desc) bytes, 16-byte aligned, for this call alone until it has ended. */
+#define LP_PREFIX_MAX_NEW 256
+typedef struct lp_prefix_attn_desc {
+  const void* q; long long q_batch, q_token, q_head;
+  const void* k; long long k_page, k_row, k_head;
+  const void* v; long long v_page, v_row, v_head;
+  const void* prefix_k; long long pk_row, pk_head;
+  const void* prefix_v; long long pv_row, pv_head;
+  void* out; long long o_batch, o_token, o_head;
+  const int* page_table; long long ld_table; int max_pages, n_pages, page_size;
+  const int* lengths; const int* fresh;
+  int prefix, B, T, H, KVH, D;
+  float scale;
+} lp_prefix_attn_desc;
+size_t lp_prefix_attention_workspace_bytes(const lp_prefix_attn_desc* desc);
+int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* workspace, size_t ws_bytes, void* stream);
+
 /* The next token of each row of logits (fp32 or bf16 [rows][ld], V <= 393216 words), by uniform[row] in [0, 1).  With w = exp((z - max z) / temperature) and the words in the order of their logits, the
  * largest first, equal ones by index: the first top_k are kept (0: all); of them those before which less than top_p of their mass lies, the first in any case; of them those with
  * w >= min_p; out[row] is the first kept word, by index, up to which more than uniform of the kept mass lies.  temperature 0 (negative, NaN): the largest, the first of equal ones.

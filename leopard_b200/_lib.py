@@ -87,6 +87,7 @@ RETENTION_CHUNK = 32
 LATENT_SPLIT_ROWS = 16
 GEMM_SPLIT_BF16, GEMM_SPLIT_F32, GEMM_SPLIT_PLANES = 0, 1, 2
 LINEAR_W_CONSTANT = 0x100      # lp_linear: with an epilogue, for weights that nothing on the stream writes
+PREFIX_MAX_NEW = 256
 TREE_MAX_NODES = 256
 DISTILL_MAX_TOP = 1024          # lp_distill_fwd_bwd: teacher entries a row
 LINEAR_ROWS_MAX, LINEAR_ROWS_COLS = 8, 8      # lp_linear: up to this many rows stream the weights, a CTA to so many columns
@@ -149,6 +150,14 @@ class RotaryAppendDesc(C.Structure):
                 ("v", _vp), ("v_row", _ll), ("v_head", _ll), ("k_pool", _vp), ("kp_page", _ll), ("kp_row", _ll), ("kp_head", _ll), ("v_pool", _vp), ("vp_page", _ll),
                 ("vp_row", _ll), ("vp_head", _ll), ("positions", _vp), ("inv_freq", _vp), ("slots", _vp), ("positions_64", _i), ("n_freq", _i), ("interleaved", _i),
                 ("fp32", _i), ("rows", _i), ("H", _i), ("KVH", _i), ("D", _i), ("n_pages", _i), ("page_size", _i), ("scale", _f)]
+
+
+class PrefixAttnDesc(C.Structure):
+    """lp_prefix_attn_desc (include/leopard_b200.h)."""
+    _fields_ = [("q", _vp), ("q_batch", _ll), ("q_token", _ll), ("q_head", _ll), ("k", _vp), ("k_page", _ll), ("k_row", _ll), ("k_head", _ll),
+                ("v", _vp), ("v_page", _ll), ("v_row", _ll), ("v_head", _ll), ("prefix_k", _vp), ("pk_row", _ll), ("pk_head", _ll), ("prefix_v", _vp), ("pv_row", _ll), ("pv_head", _ll),
+                ("out", _vp), ("o_batch", _ll), ("o_token", _ll), ("o_head", _ll), ("page_table", _vp), ("ld_table", _ll), ("max_pages", _i), ("n_pages", _i), ("page_size", _i),
+                ("lengths", _vp), ("fresh", _vp), ("prefix", _i), ("B", _i), ("T", _i), ("H", _i), ("KVH", _i), ("D", _i), ("scale", _f)]
 
 
 class MLSTMDesc(C.Structure):
@@ -329,6 +338,8 @@ _SIGS = {
     "lp_step_tables": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "lp_rotary": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _f, _i, _vp]),
     "lp_rotary_append": (_i, [_P(RotaryAppendDesc), _vp]),
+    "lp_prefix_attention_workspace_bytes": (_sz, [_P(PrefixAttnDesc)]),
+    "lp_prefix_attention": (_i, [_P(PrefixAttnDesc), _vp, _sz, _vp]),
     "lp_sample_tokens": (_i, [_vp, _i, _ll, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _i, _i, _vp, _vp]),
     "lp_verify_draft": (_i, [_vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "lp_cache_compact": (_i, [_vp, _ll, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _vp, _ll, _vp, _i, _i, _vp]),

@@ -1,0 +1,76 @@
+// leopard_b200 — attention of a batch over a prefix that it shares and over each request's own rows: what lp_prefixattn.cu and lp_prefixattn_tc.cu share.
+//
+// The tokens that the requests bring stand in one list (request after request); for a key head, row r = token * G + g of that list are the rows of one product with the prefix's keys, which are
+// read once for all of them.  A request's own keys are read for its rows alone.  Keys are cut into pieces; each leaves its rows' maximum, sum and weighted values in the workspace, and a last
+// kernel joins them.
+#pragma once
+#include "lp_common.cuh"
+#include "lp_host.h"
+#include "../../include/leopard_b200.h"
+
+namespace lp {
+
+constexpr int PA_MAX_BATCH = 2048;
+constexpr int PA_KEYS = 64;               // keys of a tile of the requests' own rows (and of the prefix, where few rows look at it)
+constexpr int PA_ROWS = 16;               // rows of a block there
+
+struct PrefixArgs {
+  lp_prefix_attn_desc d;
+  int group;
+  float scale_log2;
+  int own_blocks, own_splits, own_rows;   // blocks of a request's rows, pieces of its keys (at most); keys that there may be
+  int pre_rows, pre_blocks, pre_splits;   // rows of a block (PA_ROWS, or the tcgen05 kernel's), blocks at most, pieces of the prefix's keys
+  int pre_tiles;                          // of PA_KEYS keys (tcgen05: of 128)
+  // partial results of the prefix's pieces [key head][block][piece] and of the own rows' [request][key head][block][piece]: values [D / 4][rows of a block][4], maximum (log2 units) and sum [rows]
+  float *pre_o, *own_o;
+  float2 *pre_ml, *own_ml;
+};
+// the tcgen05 kernel for many rows: whether it takes this call, its blocks' rows, its pieces; its launch
+bool prefix_tc_takes(const lp_prefix_attn_desc* d);
+int launch_prefix_tc(const PrefixArgs& a, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float pa_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ int pa_new(const PrefixArgs& a, int b) { return a.d.fresh ? min(max(a.d.fresh[b], 0), a.d.T) : a.d.T; }
+// first[b]: tokens of the requests before b; first[B]: of all.  By one warp; ends in the block's barrier.
+__device__ __forceinline__ void pa_tokens(const PrefixArgs& a, int* first) {
+  if (threadIdx.x < 32) {
+    int run = 0;
+    for (int b0 = 0; b0 < a.d.B; b0 += 32) {
+      const int b = b0 + threadIdx.x, mine = b < a.d.B ? pa_new(a, b) : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((int)threadIdx.x >= o) sum += up;
+      }
+      if (b < a.d.B) first[b] = run + sum - mine;
+      run += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) first[a.d.B] = run;
+  }
+  __syncthreads();
+}
+// the request that brings token i of the list
+__device__ __forceinline__ int pa_find(const int* first, int B, int i) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= i) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+// own rows of request b before its new tokens, and with them (as far as there is room for rows)
+__device__ __forceinline__ void pa_own(const PrefixArgs& a, int b, int fresh, int& past, int& keys) {
+  const int own = max(max(a.d.lengths[b], 0) - a.d.prefix, 0);
+  past = min(own, a.own_rows);
+  keys = (int)min((long long)own + fresh, (long long)a.own_rows);
+}
+__device__ __forceinline__ int pa_own_pieces(const PrefixArgs& a, int keys) { return min(a.own_splits, (keys + PA_KEYS - 1) / PA_KEYS); }
+#endif
+
+}  // namespace lp

@@ -962,6 +962,87 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
     return q_out
 
 
+def _prefix_refusals(q, k, v, lengths, prefix, new, page_table, prefix_k, prefix_v, out):
+    for t, n, dim in ((q, "q", 4), (k, "k", 4), (v, "v", 4), (out, "out", 4), (prefix_k, "prefix_k", 3), (prefix_v, "prefix_v", 3)):
+        if t is not None:
+            _rotary_check(t, n, (_BF16,), dim, q.device if t is not q else None)
+    B, T, H, D = q.shape
+    G, dev = k.shape[2], q.device
+    if k.shape[3] != D or v.shape != k.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if out is not None and out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    _need(lengths, "lengths", (_I32,), 1, (B,), dev, contiguous=True)
+    if new is not None:
+        _need(new, "new", (_I32,), 1, (B,), dev, contiguous=True)
+    if page_table is not None:
+        _need(page_table, "page_table", (_I32,), 2, (B, page_table.shape[-1]), dev, rows=True)
+        if prefix_k is not None or prefix_v is not None:
+            raise ValueError("the prefix lies in the pages of the table, or in prefix_k and prefix_v: not both")
+    else:
+        if k.shape[0] < B:
+            raise ValueError(f"{B} requests need a page table or a cache of their own each, k holds {k.shape[0]}")
+        if prefix and (prefix_k is None or prefix_v is None):
+            raise ValueError("without a page table the prefix is prefix_k and prefix_v")
+        for t, n in ((prefix_k, "prefix_k"), (prefix_v, "prefix_v")):
+            if prefix and t.shape != (prefix, G, D):
+                raise ValueError(f"{n} must be {(prefix, G, D)}, got {tuple(t.shape)}")
+    raise ValueError("prefix_attention: heads must be contiguous")
+
+
+def prefix_attention(q, k, v, lengths, prefix, new=None, page_table=None, prefix_k=None, prefix_v=None, scale=None, out=None):
+    """Attention of a batch whose requests share their first `prefix` rows, which are read once for all of them (lp_prefix_attention): q bf16 [B, T, H, D], the requests' new tokens; lengths int32 [B], rows
+    of each before these, the prefix among them; new int32 [B] or None (T), tokens that each brings, whose keys and values are the cache's next rows already (rotary_append): token t sees the prefix and its
+    request's rows up to its own.  With page_table int32 [B, max_pages]: k, v bf16 [pages, page_size, KVH, D] and each request's whole sequence in its pages (SequenceCache.fork shares them), the prefix
+    read from those of request 0.  Without: own rows in k, v [B, rows, KVH, D], from row 0 on, the prefix in prefix_k, prefix_v [prefix, KVH, D].  Strides are free but for a contiguous last
+    dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of tokens that a request does not bring stay as they were (`out` given; its rows share no memory, and its span meets none of the
+    inputs) or are unspecified.  A token that sees nothing is zeros.  T <= 256."""
+    try:
+        B, T, H, D = q.shape
+        P, S, G, Dk = k.shape
+        dev, prefix = q.device, int(prefix)
+        fine = (q.is_cuda and q.dtype is _BF16 and k.dtype is _BF16 and v.dtype is _BF16 and Dk == D and v.shape == k.shape and k.device == dev and v.device == dev
+                and lengths.dtype is _I32 and lengths.device == dev and lengths.shape == (B,) and lengths.is_contiguous())
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        fine = fine and qs[3] == ks[3] == vs[3] == 1 and (new is None or (new.dtype is _I32 and new.device == dev and new.shape == (B,) and new.is_contiguous()))
+        pk = pv = None
+        pks = pvs = (0, 0)
+        if page_table is not None:
+            max_pages = page_table.shape[1]
+            fine = (fine and page_table.dtype is _I32 and page_table.device == dev and page_table.shape == (B, max_pages) and (page_table.stride(1) == 1 or max_pages <= 1)
+                    and (page_table.stride(0) >= max_pages or B == 1) and prefix_k is None and prefix_v is None)
+            table, ld = page_table.data_ptr(), page_table.stride(0)
+        else:
+            fine, max_pages, table, ld = fine and P >= B, 1, None, 0
+            if prefix:
+                fine = (fine and prefix_k.dtype is _BF16 and prefix_v.dtype is _BF16 and prefix_k.shape == (prefix, G, D) and prefix_v.shape == (prefix, G, D) and prefix_k.device == dev
+                        and prefix_v.device == dev and prefix_k.stride(2) == 1 and prefix_v.stride(2) == 1)
+                pk, pv, pks, pvs = prefix_k.data_ptr(), prefix_v.data_ptr(), prefix_k.stride(), prefix_v.stride()
+        if out is not None:
+            fine = fine and out.dtype is _BF16 and out.device == dev and out.shape == q.shape and out.stride(3) == 1
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _prefix_refusals(q, k, v, lengths, prefix, new, page_table, prefix_k, prefix_v, out)
+    if out is None:
+        out = torch.empty((B, T, H, D), dtype=_BF16, device=dev)
+    elif any(t is not None and _overlaps(out, t) for t in (q, k, v, prefix_k, prefix_v, lengths, new, page_table)):
+        raise ValueError("out must not share memory with the inputs")
+    if B == 0 or T == 0:
+        return out
+    os_ = out.stride()
+    d = _lib.PrefixAttnDesc(q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], pk, pks[0], pks[1], pv, pvs[0], pvs[1],
+                            out.data_ptr(), os_[0], os_[1], os_[2], table, ld, max_pages, P, S, lengths.data_ptr(), None if new is None else new.data_ptr(), prefix, B, T, H, G, D,
+                            D ** -0.5 if scale is None else float(scale))
+    L, ref = _lib.lib(), C.byref(d)
+    need = L.lp_prefix_attention_workspace_bytes(ref)
+    if need == 0:
+        _lib.check(-1, "lp_prefix_attention")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(dev, L, "lp_prefix_attention", L.lp_prefix_attention, ref, ws.data_ptr(), need)
+    return out
+
+
 def _setting(x, name, dtype, rows, dev):
     """a number for all rows, or a tensor of one each -> (its address or None, the number)"""
     if isinstance(x, torch.Tensor):
