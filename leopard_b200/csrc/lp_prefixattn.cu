@@ -31,15 +31,18 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
   int page_size, n_pages, page_of, key_first;
   long long slot;
   if (pre) {
-    const int item = blockIdx.x / a.pre_splits, piece = blockIdx.x - item * a.pre_splits;
-    kvh = item / a.pre_blocks;
-    r0 = (item - kvh * a.pre_blocks) * PA_ROWS;
     rows = pa_first[a.d.B] * a.group;
-    n_keys = a.d.prefix;
-    past = n_keys;
-    t0 = (int)((long long)a.pre_tiles * piece / a.pre_splits);
-    t1 = (int)((long long)a.pre_tiles * (piece + 1) / a.pre_splits);
-    slot = blockIdx.x;
+    const PrefixLine line = pa_line(a, rows);
+    long long u, u_end;
+    pa_range(a, line, blockIdx.x, u, u_end);
+    if (u >= u_end) return;
+    const PrefixPiece p = pa_piece(a, line, u, u_end);            // (the only one: there are as many CTAs as items can be)
+    kvh = p.kvh;
+    r0 = p.r0;
+    t0 = p.t0;
+    t1 = p.t0 + p.n;
+    past = n_keys = a.d.prefix;
+    slot = (long long)p.item + blockIdx.x;
   } else {
     int i = blockIdx.x - pre_ctas;
     const int piece = i % a.own_splits;
@@ -319,9 +322,19 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
   const int r = min(r0 + in, rows - 1), i = r / a.group, g = r - i * a.group, b = pa_find(pa_first, a.d.B, i), t = i - pa_first[b];
   int past, keys;
   pa_own(a, b, pa_first[b + 1] - pa_first[b], past, keys);
-  const int own = t * a.group + g, n_own = pa_own_pieces(a, keys), n = a.pre_splits + n_own;
-  const int pre_blk = r / a.pre_rows, pre_in = r - pre_blk * a.pre_rows, own_blk = own / PA_ROWS, own_in = own - own_blk * PA_ROWS;
-  const long long pre_slot = ((long long)kvh * a.pre_blocks + pre_blk) * a.pre_splits, own_slot = (((long long)b * a.d.KVH + kvh) * a.own_blocks + own_blk) * a.own_splits;
+  int n_pre = 0, pre_in = 0;
+  long long pre_slot = 0;
+  if (a.pre_ctas) {
+    const PrefixLine line = pa_line(a, rows);
+    const int blk = r / a.pre_rows, item = kvh * line.blocks + blk;
+    int c0, c1;
+    pa_ctas_of(a, line, item, c0, c1);
+    pre_in = r - blk * a.pre_rows;
+    n_pre = c1 - c0 + 1;
+    pre_slot = (long long)item + c0;
+  }
+  const int own = t * a.group + g, n = n_pre + pa_own_pieces(a, keys), own_blk = own / PA_ROWS, own_in = own - own_blk * PA_ROWS;
+  const long long own_slot = (((long long)b * a.d.KVH + kvh) * a.own_blocks + own_blk) * a.own_splits;
   if (c4 == 0) to[in] = r0 + in < rows ? b * a.d.o_batch + t * a.d.o_token + (kvh * a.group + g) * a.d.o_head : -1;
   float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -333,11 +346,11 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
       const int p = p0 + k;
       ml[k] = make_float2(-INFINITY, 0.f);
       y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p < a.pre_splits) {
+      if (p < n_pre) {
         ml[k] = a.pre_ml[(pre_slot + p) * a.pre_rows + pre_in];
         y[k] = *reinterpret_cast<const float4*>(a.pre_o + (((pre_slot + p) * (D / 4) + c4) * a.pre_rows + pre_in) * 4);
       } else if (p < n) {
-        const long long s = own_slot + p - a.pre_splits;
+        const long long s = own_slot + p - n_pre;
         ml[k] = a.own_ml[s * PA_ROWS + own_in];
         y[k] = *reinterpret_cast<const float4*>(a.own_o + ((s * (D / 4) + c4) * PA_ROWS + own_in) * 4);
       }
@@ -380,6 +393,9 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   else LP_REQUIRE(d->prefix == 0, "lp_prefix_attention: a prefix of %d rows that is nowhere", d->prefix);
   return 0;
 }
+// whether the prefix goes to the tcgen05 kernel
+constexpr int PA_TC_ROWS = 16;
+static bool prefix_tc(const lp_prefix_attn_desc* d) { return (long long)d->B * d->T * (d->H / d->KVH) > PA_TC_ROWS && prefix_tc_takes(d); }
 // how a call is cut: what the descriptor's numbers alone decide
 static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
   a.d = *d;
@@ -391,17 +407,25 @@ static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
   long long splits = items >= room ? 1 : room / items;
   a.own_splits = (int)(splits < tiles ? splits : tiles > 0 ? tiles : 1);
   const long long rows = (long long)d->B * d->T * a.group;
-  a.pre_splits = a.pre_blocks = a.pre_tiles = 0;
-  a.pre_rows = PA_ROWS;
+  const bool tc = prefix_tc(d);
+  const int keys = tc ? 128 : PA_KEYS;
+  a.pre_rows = !tc ? PA_ROWS : rows <= 128 ? 128 : 256;
+  a.pre_tiles = (int)(((long long)d->prefix + keys - 1) / keys);
+  a.pre_ctas = 0;
+  a.pre_slots = 0;
   if (d->prefix > 0) {
-    a.pre_blocks = (int)((rows + PA_ROWS - 1) / PA_ROWS);
-    a.pre_tiles = (d->prefix + PA_KEYS - 1) / PA_KEYS;
-    const long long pre_items = (long long)d->KVH * a.pre_blocks;
-    splits = pre_items >= room ? 1 : room / pre_items;
-    a.pre_splits = (int)(splits < a.pre_tiles ? splits : a.pre_tiles);
+    const long long pre_items = (rows + a.pre_rows - 1) / a.pre_rows * d->KVH;
+    if (tc) {
+      const long long most = pre_items * a.pre_tiles;
+      a.pre_ctas = (int)(most < sm_count() ? most : sm_count());
+    } else {
+      splits = pre_items >= room ? 1 : room / pre_items;
+      a.pre_ctas = (int)((splits < a.pre_tiles ? splits : a.pre_tiles) * pre_items);
+    }
+    a.pre_slots = pre_items + a.pre_ctas;
   }
-  const size_t pre = (size_t)d->KVH * a.pre_blocks * a.pre_splits * a.pre_rows, mine = (size_t)items * a.own_splits * PA_ROWS;
-  return (pre + mine) * (d->D * 4 + 8);
+  a.own_slots = items * a.own_splits;
+  return ((size_t)a.pre_slots * a.pre_rows + (size_t)a.own_slots * PA_ROWS) * (d->D * 4 + 8);
 }
 
 }  // namespace lp
@@ -440,20 +464,22 @@ extern "C" int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* worksp
   LP_REQUIRE(strides_nest(places, 3, d->D), "lp_prefix_attention: rows of out share their memory (strides %lld, %lld, %lld)", d->o_batch, d->o_token, d->o_head);
   LP_REQUIRE(ws_bytes >= need, "lp_prefix_attention: workspace too small");
   a.scale_log2 = d->scale * 1.4426950408889634f;
-  const size_t pre = (size_t)d->KVH * a.pre_blocks * a.pre_splits * a.pre_rows, mine = (size_t)d->B * d->KVH * a.own_blocks * a.own_splits * PA_ROWS;
+  const size_t pre = (size_t)a.pre_slots * a.pre_rows, mine = (size_t)a.own_slots * PA_ROWS;
   a.pre_o = reinterpret_cast<float*>(workspace);
   a.own_o = a.pre_o + pre * d->D;
   a.pre_ml = reinterpret_cast<float2*>(a.own_o + mine * d->D);
   a.own_ml = a.pre_ml + pre;
-  const int pre_ctas = d->KVH * a.pre_blocks * a.pre_splits;
-  const long long ctas = pre_ctas + (long long)d->B * d->KVH * a.own_blocks * a.own_splits;
+  const bool tc = a.pre_ctas && a.pre_rows != PA_ROWS;
+  const int pre_ctas = tc ? 0 : a.pre_ctas;
+  const long long ctas = pre_ctas + a.own_slots;
   const size_t first = (size_t)(d->B + 1) * 4;
   const dim3 join((unsigned)(((long long)d->B * d->T * a.group + PJ_ROWS - 1) / PJ_ROWS), d->KVH);
-  note_launch(2);
+  note_launch(tc ? 3 : 2);
 #define LP_PREFIX(DD)                                                                                             \
   {                                                                                                               \
     prefix_rows_kernel<DD><<<(unsigned)ctas, 128, first, stream>>>(a, pre_ctas);                                  \
     LP_CHECK_CUDA(cudaGetLastError());                                                                            \
+    if (tc) { if (const int rc = launch_prefix_tc(a, stream)) return rc; }                                        \
     LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD>, join, dim3(PJ_ROWS * DD / 4), first, stream, 1, true, a));    \
   }
   if (d->D == 128) LP_PREFIX(128) else if (d->D == 96) LP_PREFIX(96) else LP_PREFIX(64)

@@ -19,9 +19,9 @@ struct PrefixArgs {
   int group;
   float scale_log2;
   int own_blocks, own_splits, own_rows;   // blocks of a request's rows, pieces of its keys (at most); keys that there may be
-  int pre_rows, pre_blocks, pre_splits;   // rows of a block (PA_ROWS, or the tcgen05 kernel's), blocks at most, pieces of the prefix's keys
-  int pre_tiles;                          // of PA_KEYS keys (tcgen05: of 128)
-  // partial results of the prefix's pieces [key head][block][piece] and of the own rows' [request][key head][block][piece]: values [D / 4][rows of a block][4], maximum (log2 units) and sum [rows]
+  int pre_rows, pre_tiles, pre_ctas;      // the prefix: rows of a block (PA_ROWS, or the tcgen05 kernel's), tiles of its keys (of PA_KEYS, or 128), CTAs (0: there is none)
+  long long pre_slots, own_slots;         // partial results' places
+  // partial results of the prefix's pieces [item + CTA] and of the own rows' [request][key head][block][piece]: values [D / 4][rows of a block][4], maximum (log2 units) and sum [rows]
   float *pre_o, *own_o;
   float2 *pre_ml, *own_ml;
 };
@@ -69,6 +69,60 @@ __device__ __forceinline__ void pa_own(const PrefixArgs& a, int b, int fresh, in
   const int own = max(max(a.d.lengths[b], 0) - a.d.prefix, 0);
   past = min(own, a.own_rows);
   keys = (int)min((long long)own + fresh, (long long)a.own_rows);
+}
+// The prefix's tiles of all items (key head, block of rows) stand in one line, of which every CTA takes an equal range; or each item has `own` CTAs, where the longest range is then little above an equal
+// share: a range that goes on in another item costs another piece's start and end.  How many rows there are, and so how many items, only the GPU knows.
+struct PrefixLine { int blocks, items, own; };
+constexpr int PA_SLACK = 4;
+__device__ __forceinline__ PrefixLine pa_line(const PrefixArgs& a, int rows) {
+  PrefixLine l;
+  l.blocks = (rows + a.pre_rows - 1) / a.pre_rows;
+  l.items = a.d.KVH * l.blocks;
+  l.own = 0;
+  if (l.items > 0 && l.items <= a.pre_ctas) {
+    l.own = min(a.pre_ctas / l.items, a.pre_tiles);
+    if (a.pre_rows != PA_ROWS && (a.pre_tiles + l.own - 1) / l.own > (long long)l.items * a.pre_tiles / a.pre_ctas + PA_SLACK) l.own = 0;
+  }
+  return l;
+}
+__device__ __forceinline__ long long pa_cut(long long total, int k, int n) {      // the k-th of n equal ranges begins here
+  const long long each = total / n;
+  return each * k + min((long long)k, total - each * n);
+}
+__device__ __forceinline__ void pa_range(const PrefixArgs& a, const PrefixLine& l, int cta, long long& from, long long& to) {
+  from = to = 0;
+  if (!l.own) {
+    const long long all = (long long)l.items * a.pre_tiles;
+    from = pa_cut(all, cta, a.pre_ctas);
+    to = pa_cut(all, cta + 1, a.pre_ctas);
+  } else if (cta < l.items * l.own) {
+    const int item = cta / l.own, k = cta - item * l.own;
+    from = (long long)item * a.pre_tiles + pa_cut(a.pre_tiles, k, l.own);
+    to = (long long)item * a.pre_tiles + pa_cut(a.pre_tiles, k + 1, l.own);
+  }
+}
+// the CTAs that an item's pieces are in
+__device__ __forceinline__ void pa_ctas_of(const PrefixArgs& a, const PrefixLine& l, int item, int& c0, int& c1) {
+  if (l.own) {
+    c0 = item * l.own;
+    c1 = c0 + l.own - 1;
+    return;
+  }
+  const long long all = (long long)l.items * a.pre_tiles, each = all / a.pre_ctas, more = all - each * a.pre_ctas;      // the first `more` CTAs have one tile more
+  auto cta = [&](long long u) { return (int)(u < (each + 1) * more ? u / (each + 1) : more + (u - (each + 1) * more) / max(each, 1LL)); };
+  c0 = cta((long long)item * a.pre_tiles);
+  c1 = cta((long long)(item + 1) * a.pre_tiles - 1);
+}
+// a CTA's piece of an item
+struct PrefixPiece { int item, kvh, r0, t0, n; };
+__device__ __forceinline__ PrefixPiece pa_piece(const PrefixArgs& a, const PrefixLine& l, long long u, long long u_end) {
+  PrefixPiece p;
+  p.item = (int)(u / a.pre_tiles);
+  p.t0 = (int)(u - (long long)p.item * a.pre_tiles);
+  p.n = (int)min((long long)(a.pre_tiles - p.t0), u_end - u);
+  p.kvh = p.item / l.blocks;
+  p.r0 = (p.item - p.kvh * l.blocks) * a.pre_rows;
+  return p;
 }
 __device__ __forceinline__ int pa_own_pieces(const PrefixArgs& a, int keys) { return min(a.own_splits, (keys + PA_KEYS - 1) / PA_KEYS); }
 #endif
