@@ -5,16 +5,17 @@
 // and drawn is the first kept word, by index, up to which more than u of the kept mass lies.  t = 0 takes the largest.
 //
 // Weights are integers in units of 2^-43 (from a 64-bit exponential): their sums do not depend on the order in which they are taken, and the draw is the one that 64 bits give.
-// A cluster of CTAs holds a row in shared memory, read once.  Nothing is sorted: what top_k and top_p keep ends at one word, which is found by counts and masses of 512 ranges of
-// logits, first of all of the row, then of the range where the limit lies, until the few words left in it are put in order one by one.
+// A cluster of CTAs holds a row in shared memory, read once.  Nothing is sorted: what top_k and top_p keep ends at one word, which is found by counts and masses of 1,024 ranges of
+// logits, first of all of the row, then of the range where the limit lies, until the few words left in it are put in order one by one.  Where the words down to the limit are few altogether (a top_k of
+// 50, a sure model's top_p), one CTA takes them all and is through.
 #include "lp_common.cuh"
 #include "lp_host.h"
 #include "../../include/leopard_b200.h"
 
 namespace lp {
 
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = SA_THREADS, SA_LIST = 256, SA_MAX_CTAS = 8;
-constexpr int SA_MAX_SLICE = 48 * 1024;      // words that a CTA can hold
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2 * SA_THREADS, SA_LIST = 256, SA_MAX_CTAS = 8;
+constexpr int SA_MAX_SLICE = 47 * 1024;      // words that a CTA can hold
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -26,22 +27,24 @@ struct SampleArgs {
   bool vec;
   long long* out;
 };
-struct SaHist { unsigned n[SA_BINS]; u64 w[SA_BINS]; };
-struct SaList { unsigned key[SA_LIST]; int at[SA_LIST]; u64 w[SA_LIST]; int n; };
+// of a range of logits: words, and their mass in two parts, since 64-bit sums in shared memory are ten times slower than 32-bit ones
+struct SaHist { unsigned n[SA_BINS], lo[SA_BINS], hi[SA_BINS]; };
+struct alignas(16) SaList { u64 word[SA_LIST]; };      // key and, below it, what is left of 2^32 - 1 behind the index: larger numbers stand before
 struct alignas(16) SaShared {
-  SaHist all, part[2];
-  SaList list[2];
-  SaList gathered;
+  SaHist hist[2];                         // in turns: others may read the one before until the next barrier
+  SaList list[2], gathered;
+  u64 sorted[SA_LIST], by_index[SA_LIST];      // masses or weights of what is gathered, in two orders
+  double root[64];                        // 2^(i / 64)
   u64 total[2][SA_MAX_CTAS];              // of each CTA of the cluster, written by it; in turns
   float2 top[SA_MAX_CTAS];                // largest and least logit of each CTA
-  int best[SA_MAX_CTAS];
+  int best[SA_MAX_CTAS], n_list[2];
   int tie;                                // a word's index, from the CTA that has it
   u64 warp_w[SA_WARPS];
   unsigned warp_n[SA_WARPS];
   float2 warp_top[SA_WARPS];
   // what all threads are told
-  int bin; unsigned bin_n; u64 bin_w, above_n, above_w;
-  unsigned last_rank; unsigned last_key; int last_at; u64 last_mass;
+  int bin; unsigned bin_n; u64 above_n, above_w;
+  unsigned last_rank; unsigned last_key; int last_at;
 };
 
 // a number whose order is that of the floats
@@ -50,24 +53,27 @@ __device__ __forceinline__ unsigned sa_key(float z) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float sa_of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-// 2^x for x <= 0 in units of 2^-43, rounded to nearest: 2^x = 2^n e^(f ln 2), |f| <= 1/2, the series of e^y to y^11 (the next term is below 2^-46)
-__device__ __forceinline__ u64 sa_weight(double x) {
-  if (!(x > -45.0)) return 0;
-  const double n = rint(x), y = (x - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, y, 1.0 / 3628800.0);
-  p = fma(p, y, 1.0 / 362880.0);
-  p = fma(p, y, 1.0 / 40320.0);
-  p = fma(p, y, 1.0 / 5040.0);
-  p = fma(p, y, 1.0 / 720.0);
-  p = fma(p, y, 1.0 / 120.0);
-  p = fma(p, y, 1.0 / 24.0);
-  p = fma(p, y, 1.0 / 6.0);
-  p = fma(p, y, 0.5);
-  p = fma(p, y, 1.0);
-  p = fma(p, y, 1.0);
-  p = __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
-  return (u64)__double_as_longlong(p + 512.0) - 0x4080000000000000ULL;      // (at 512 a step is 2^-43)
+__constant__ double SA_ROOT[64] = {      // 2^(i / 64)
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284, 1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418, 1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687, 1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303, 1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647, 1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267, 1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656, 1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+// 2^(x / 64), x <= 0, to nearest: x = 64 e + i + r, |r| <= 1/2; 2^(i / 64) from the table, e^y, y = r ln 2 / 64, by its series to y^4 (the next term is 2^-44.6).  Added to a power of two, it is a whole number
+// in the sum's low bits: 512 makes units of 2^-43, 131072 of 2^-35, 2^20 of 2^-32; that power's own bits are left in.  Below x = -2944 (-inf among it) the result is that of about there, less than half a unit.
+__device__ __forceinline__ u64 sa_weight_bits(double x, double power, const double* root) {
+  x = __hiloint2double((int)min((unsigned)__double2hiint(x), 0xc0a70000u), __double2loint(x));
+  const double m = x + 6755399441055744.0;                // 1.5 2^52: the whole number is in the low bits
+  const int n = __double2loint(m);
+  const double r = x - (m - 6755399441055744.0), c = 0.010830424696249145260;
+  double p = fma(r, c * c * c * c / 24.0, c * c * c / 6.0);
+  p = fma(p, r, c * c / 2.0);
+  p = fma(p, r, c) * r;
+  const double t = root[n & 63], w = fma(t, p, t);
+  return (u64)__double_as_longlong(__hiloint2double(__double2hiint(w) + ((n >> 6) << 20), __double2loint(w)) + power);
 }
 __device__ __forceinline__ u64 sa_warp_sum(u64 v) {
 #pragma unroll
@@ -81,74 +87,98 @@ __device__ __forceinline__ T* sa_at(T* mine, int rank) {
   asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(mine), "r"(rank));
   return reinterpret_cast<T*>(to);
 }
-__device__ __forceinline__ void sa_cluster(int ctas) {
-  if (ctas > 1) cluster_sync_all();
+struct SaByCount { static constexpr bool value = false; };
+struct SaByMass { static constexpr bool value = true; };
+template <int CTAS>
+__device__ __forceinline__ void sa_cluster() {
+  if (CTAS > 1) cluster_sync_all();
   else __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SA_THREADS)
-sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(SA_THREADS, 2)
+sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char sa_smem[];
   SaShared& s = *reinterpret_cast<SaShared*>(sa_smem);
   float* z = reinterpret_cast<float*>(sa_smem + sizeof(SaShared));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas;
+  const int row = blockIdx.x / CTAS, rank = blockIdx.x % CTAS;
   const int v0 = rank * a.slice, count = max(0, min(a.slice, a.V - v0));
-  const int part = a.slice / SA_WARPS, from = warp * part, to = min(from + part, count);      // a warp's words lie side by side
-
-  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (no CTA is written to before it has begun)
+  const int part = a.slice / SA_WARPS, from = warp * part;      // a warp's words lie side by side
+  if (CTAS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");         // (no CTA is written to before it has begun)
   const float t = a.temperature ? a.temperature[row] : a.temperature_all;
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all, u01 = a.uniform[row];
 
-  // ---- the row, its largest and least logit
+  // ---- the row (-inf behind its end), its largest and least logit
   const T* src = reinterpret_cast<const T*>(a.logits) + row * a.ld + v0;
   float hi = -INFINITY, lo = INFINITY;
-  auto take = [&](int i, float x) {
+  auto take = [&](float x) {
     x = x > -INFINITY ? x + 0.f : -INFINITY;              // (what is not a number is never drawn; the two zeros are equal)
-    z[i] = x;
     hi = fmaxf(hi, x);
     if (x > -INFINITY) lo = fminf(lo, x);
+    return x;
   };
+  int done = 0;
   if (a.vec) {
-    constexpr int N = 16 / (int)sizeof(T);
-    for (int i = tid * N; i < count; i += SA_THREADS * N) {
-      if (i + N <= count) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src + i);
-        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+    constexpr int N = 16 / (int)sizeof(T), AT_ONCE = 4;
+    const int whole = count / N;
+    done = whole * N;
+    for (int i0 = tid; i0 < whole; i0 += SA_THREADS * AT_ONCE) {
+      uint4 u[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (N == 4) take(i + k, __uint_as_float(w[k]));
-          else {
-            take(i + 2 * k, __uint_as_float(w[k] << 16));
-            take(i + 2 * k + 1, __uint_as_float(w[k] & 0xffff0000u));
-          }
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (i0 + k * SA_THREADS < whole) u[k] = ldg_once(src + (long long)(i0 + k * SA_THREADS) * N);
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int i = i0 + k * SA_THREADS;
+        if (i >= whole) continue;
+        if (N == 4) {
+          *reinterpret_cast<float4*>(z + i * 4) = make_float4(take(__uint_as_float(u[k].x)), take(__uint_as_float(u[k].y)), take(__uint_as_float(u[k].z)), take(__uint_as_float(u[k].w)));
+        } else {
+          const float2 a0 = unpack_bf16x2(u[k].x), a1 = unpack_bf16x2(u[k].y), a2 = unpack_bf16x2(u[k].z), a3 = unpack_bf16x2(u[k].w);
+          *reinterpret_cast<float4*>(z + i * 8) = make_float4(take(a0.x), take(a0.y), take(a1.x), take(a1.y));
+          *reinterpret_cast<float4*>(z + i * 8 + 4) = make_float4(take(a2.x), take(a2.y), take(a3.x), take(a3.y));
         }
-      } else {
-        for (int k = i; k < count; ++k) take(k, (float)src[k]);
       }
     }
   } else {
-    for (int i = tid; i < count; i += SA_THREADS) take(i, (float)src[i]);
-  }
+    constexpr int AT_ONCE = 8;
+    done = count;
+    for (int i0 = tid; i0 < count; i0 += SA_THREADS * AT_ONCE) {
+      float x[AT_ONCE];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (i0 + k * SA_THREADS < count) x[k] = (float)src[i0 + k * SA_THREADS];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (i0 + k * SA_THREADS < count) z[i0 + k * SA_THREADS] = take(x[k]);
+    }
   }
+  for (int i = done + tid; i < a.slice; i += SA_THREADS) z[i] = i < count ? take((float)src[i]) : -INFINITY;
+  auto top_of_warp = [&]() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+  };
+  top_of_warp();
   if (lane == 0) s.warp_top[warp] = make_float2(hi, lo);
-  for (int i = tid; i < SA_BINS; i += SA_THREADS) s.all.n[i] = 0, s.all.w[i] = 0;
-  if (tid < 2) s.list[tid].n = 0;
+  for (int i = tid; i < (int)(sizeof(s.hist) / 4); i += SA_THREADS) reinterpret_cast<unsigned*>(s.hist)[i] = 0;
+  if (tid < 2) s.n_list[tid] = 0;
+  if (tid < 64) s.root[tid] = SA_ROOT[tid];
   __syncthreads();
-  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (tid < ctas) {
-    for (int w = 0; w < SA_WARPS; ++w) hi = fmaxf(hi, s.warp_top[w].x), lo = fminf(lo, s.warp_top[w].y);
-    *sa_at(&s.top[rank], tid) = make_float2(hi, lo);
+  if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp == 0) {
+    hi = s.warp_top[lane % SA_WARPS].x, lo = s.warp_top[lane % SA_WARPS].y;
+    top_of_warp();
+    if (lane < CTAS) *sa_at(&s.top[rank], lane) = make_float2(hi, lo);
   }
-  sa_cluster(ctas);
+  sa_cluster<CTAS>();
   hi = -INFINITY, lo = INFINITY;
-  for (int c = 0; c < ctas; ++c) hi = fmaxf(hi, s.top[c].x), lo = fminf(lo, s.top[c].y);
+#pragma unroll
+  for (int c = 0; c < CTAS; ++c) hi = fmaxf(hi, s.top[c].x), lo = fminf(lo, s.top[c].y);
 
   // ---- nothing to draw; the largest
   if (hi == -INFINITY || !(t > 0.f)) {                    // (the same in all CTAs of the cluster)
@@ -163,9 +193,9 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
       for (int w = 0; w < SA_WARPS; ++w) best = min(best, (int)s.warp_n[w]);
       *sa_at(&s.best[rank], 0) = best;
     }
-    sa_cluster(ctas);
+    sa_cluster<CTAS>();
     if (rank == 0 && tid == 0) {
-      for (int c = 0; c < ctas; ++c) best = min(best, s.best[c]);
+      for (int c = 0; c < CTAS; ++c) best = min(best, s.best[c]);
       a.out[row] = best == 0x7fffffff ? -1 : best;
     }
     return;
@@ -175,28 +205,52 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
     hi = lo = 0.f;
     __syncthreads();
   }
-  const double unit = 1.4426950408889634074 / (double)t, top = (double)hi;
-  auto weight = [&](float x) { return sa_weight(((double)x - top) * unit); };
+  const double unit = fmax(1.4426950408889634074 * 64.0 / (double)t, 1e-300), top = (double)hi;
+  constexpr u64 AT_512 = 0x4080000000000000ULL, AT_2_17 = 0x4100000000000000ULL, AT_2_20 = 0x4130000000000000ULL;      // 512, 2^17, 2^20
+  auto weight_bits = [&](float x) { return sa_weight_bits(((double)x - top) * unit, 512.0, s.root); };
+  auto weight = [&](float x) { return weight_bits(x) - AT_512; };
+  // four of the warp's words a lane, at a time
+  auto each = [&](auto f) {
+#pragma unroll 2
+    for (int i = from + lane * 4; i < from + part; i += 128) f(i, *reinterpret_cast<const float4*>(z + i));
+  };
 
   // ---- what is kept: keys above last_key, and of those equal to it the ones up to last_at
   unsigned last_key = 0;
   int last_at = 0x7fffffff;
+  auto kept = [&](float x, int i) {
+    const unsigned key = sa_key(x);
+    return x > -INFINITY && (key > last_key || (key == last_key && v0 + i <= last_at));
+  };
   const bool by_count = top_k > 0 && top_k < a.V, by_mass = top_p < 1.f;
+  const float least = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+  const u64 w_min = least > 0.f ? (u64)ceil((double)least * 8796093022208.0) : 0;
+  const double u = (double)u01;
+  auto drawn = [&](u64 all) -> u64 {                      // the word up to which more than this lies
+    const double x = u > 0.0 ? floor(u * (double)all) : 0.0;
+    return x < (double)all ? min((u64)x, all - 1) : all - 1;
+  };
+  auto mass_limit = [&](u64 m) -> u64 {
+    const double x = ceil((double)top_p * (double)m);
+    return top_p > 0.f && x >= 1.0 ? (u64)x : 1ULL;
+  };
   int turn = 0;                                           // of s.total
-  // The word (by index) up to which more than `limit` of value(i) lies, by all CTAs; every CTA's sum is known to all when it returns.  `all`: of the sums, limit = choose(all).
-  // Returns its index in the one CTA that has it, -1 in the others.
-  auto locate = [&](auto value, auto choose) -> int {
+  // The word (by index) up to which more than `limit` of value(i, z_i) lies, by all CTAs; limit = choose(the sum of all).  Returns its index in the one CTA that has it, -1 in the others.
+  // value(...) is `base` too large.
+  auto locate = [&](auto value, u64 base, auto choose) -> int {
     u64 sum = 0;
-    for (int i = from + lane; i < to; i += 32) sum += value(i);
-    sum = sa_warp_sum(sum);
+    each([&](int i, const float4& x) { sum += (value(i, x.x) + value(i + 1, x.y)) + (value(i + 2, x.z) + value(i + 3, x.w)); });
+    sum = sa_warp_sum(sum) - base * part;
     if (lane == 0) s.warp_w[warp] = sum;
     __syncthreads();
     u64 mine = 0;
+#pragma unroll
     for (int w = 0; w < SA_WARPS; ++w) mine += s.warp_w[w];
-    if (tid < ctas) *sa_at(&s.total[turn][rank], tid) = mine;
-    sa_cluster(ctas);
+    if (tid < CTAS) *sa_at(&s.total[turn][rank], tid) = mine;
+    sa_cluster<CTAS>();
     u64 all = 0, before = 0;
-    for (int c = 0; c < ctas; ++c) {
+#pragma unroll
+    for (int c = 0; c < CTAS; ++c) {
       if (c == rank) before = all;
       all += s.total[turn][c];
     }
@@ -205,11 +259,14 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
     if (limit < before || limit >= before + mine) return -1;
     u64 at = before;
     int w = 0;
-    while (at + s.warp_w[w] <= limit) at += s.warp_w[w++];
+#pragma unroll
+    for (int k = 0; k < SA_WARPS; ++k)
+      if (k == w && at + s.warp_w[k] <= limit) at += s.warp_w[k], w = k + 1;
     // that warp's words, a thread some of them side by side
-    const int each = (part + SA_THREADS - 1) / SA_THREADS, i0 = w * part + tid * each, i1 = min(min(i0 + each, (w + 1) * part), count);
+    const int some = (part + SA_THREADS - 1) / SA_THREADS, i0 = min(tid * some, part) + w * part, i1 = min((tid + 1) * some, part) + w * part;
     u64 own = 0;
-    for (int i = i0; i < i1; ++i) own += value(i);
+#pragma unroll 2
+    for (int i = i0; i < i1; ++i) own += value(i, z[i]) - base;
     u64 run = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -220,10 +277,12 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
     if (lane == 31) s.warp_w[warp] = run;
     __syncthreads();
     at += run - own;
-    for (int k = 0; k < warp; ++k) at += s.warp_w[k];
+#pragma unroll
+    for (int k = 0; k < SA_WARPS; ++k)
+      if (k < warp) at += s.warp_w[k];
     if (limit >= at && limit < at + own)
       for (int i = i0; i < i1; ++i) {
-        const u64 v = value(i);
+        const u64 v = value(i, z[i]) - base;
         if (limit < at + v) { s.tie = i; break; }
         at += v;
       }
@@ -232,72 +291,220 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
   };
 
   if (by_count || by_mass) {
+    // masses are in units of 2^-35 (2^-32) here, so that the sums of their two parts over a CTA's words fit into 32 bits
+    const int low = a.slice <= 16384 ? 18 : 16;
+    const double power = a.slice <= 16384 ? 131072.0 : 1048576.0;
+    const u64 power_bits = a.slice <= 16384 ? AT_2_17 : AT_2_20;
+    auto mass = [&](float x) { return sa_weight_bits(((double)x - top) * unit, power, s.root) - power_bits; };
     // ranges of equal width below the largest logit, as far as weights reach (30 t) or a top_k may look
-    const float reach = fminf(fmaxf(30.f * t, 24.f), hi - lo), fine = reach > 0.f ? (float)SA_BINS / reach : 0.f;
-    auto bin_of = [&](float x) { return (int)fminf((hi - x) * fine, (float)(SA_BINS - 1)); };
-    for (int i = from + lane; i < to; i += 32)
-      if (z[i] > -INFINITY) {
-        const int b = bin_of(z[i]);
-        const u64 w = weight(z[i]);
-        atomicAdd(&s.all.n[b], 1u);
-        if (w) atomicAdd(&s.all.w[b], w);
-      }
-    sa_cluster(ctas);
-    u64 mass = 0;                                         // of what top_k has kept
-    int lists = 0, parts = 0;
-    // the last word before which fewer than k words or less than `limit` mass lies
-    auto cut = [&](bool count_them, u64 limit, auto limit_of_mass) {
-      unsigned key_lo = 0, key_hi = 0xffffffffu;
-      u64 above_n = 0, above_w = 0;
-      SaHist* h = &s.all;
-      unsigned shift = 0;
-      for (bool first = true;; first = false) {
-        // every CTA adds up all CTAs' ranges, a thread one, and finds the one where the limit lies
-        unsigned n = 0;
-        u64 w = 0;
-        for (int c = 0; c < ctas; ++c) {
-          const SaHist* o = sa_at(h, c);
-          n += o->n[tid];
-          w += o->w[tid];
+    const float reach = fminf(fmaxf(30.f * t, 24.f), hi - lo), fine = reach > 0.f ? (float)(SA_BINS - 1) / reach : 0.f;
+    auto bin_of = [&](float x) { return __float_as_int(fminf(__fmaf_rn(hi - x, fine, 12582912.f), 12582912.f + (SA_BINS - 1))) - 0x4b400000; };      // (1.5 2^23: the whole number is in the low bits)
+    int hists = 0;
+    // The last word before which fewer than `limit` words lie (MASS: less than top_p of the mass): last_key and last_at.  True: the word has been drawn.
+    auto cut = [&](auto by, u64 limit) -> bool {
+      constexpr bool MASS = decltype(by)::value;
+      SaHist* h;
+      auto count_in = [&](int b, u64 w) {
+        atomicAdd(&h->n[b], 1u);
+        if (MASS) {
+          const unsigned w_lo = (unsigned)w & ((1u << low) - 1), w_hi = (unsigned)(w >> low);
+          if (w_lo) atomicAdd(&h->lo[b], w_lo);
+          if (w_hi) atomicAdd(&h->hi[b], w_hi);
         }
-        u64 run_n = n, run_w = w;
+      };
+      auto next_hist = [&]() {
+        h = &s.hist[hists & 1];
+        if (hists++ > 1) {                                // (the first two are empty)
+          for (int i = tid; i < (int)(sizeof(SaHist) / 4); i += SA_THREADS) reinterpret_cast<unsigned*>(h)[i] = 0;
+          __syncthreads();
+        }
+      };
+      next_hist();
+      each([&](int i, const float4& x) {
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        bool on[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) on[k] = MASS && by_count ? kept(v[k], i + k) : v[k] > -INFINITY;      // (of the mass what top_k has kept)
+        if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+          u64 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = MASS ? mass(v[k]) : 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (on[k]) count_in(bin_of(v[k]), w[k]);
+        }
+      });
+      sa_cluster<CTAS>();
+      u64 above_n = 0, above_w = 0;
+      unsigned key_lo = 0, key_hi = 0;                    // of the range, from the second level on
+      int shift = 0;
+      for (bool first = true;; first = false) {
+        // every CTA adds up all CTAs' ranges, a thread two, and finds the one where the limit lies
+        uint2 n = make_uint2(0, 0);
+        u64 w0 = 0, w1 = 0;
+#pragma unroll
+        for (int c = 0; c < CTAS; ++c) {
+          const SaHist* o = sa_at(h, c);
+          const uint2 x = *reinterpret_cast<const uint2*>(&o->n[2 * tid]);
+          n.x += x.x, n.y += x.y;
+          if (MASS) {
+            const uint2 l = *reinterpret_cast<const uint2*>(&o->lo[2 * tid]), m = *reinterpret_cast<const uint2*>(&o->hi[2 * tid]);
+            w0 += ((u64)m.x << low) + l.x;
+            w1 += ((u64)m.y << low) + l.y;
+          }
+        }
+        unsigned run_n = n.x + n.y;
+        u64 run_w = w0 + w1;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const u64 up_n = __shfl_up_sync(0xffffffffu, run_n, o), up_w = __shfl_up_sync(0xffffffffu, run_w, o);
-          if (lane >= o) run_n += up_n, run_w += up_w;
+          const unsigned up_n = __shfl_up_sync(0xffffffffu, run_n, o);
+          if (lane >= o) run_n += up_n;
+          if (MASS) {
+            const u64 up_w = __shfl_up_sync(0xffffffffu, run_w, o);
+            if (lane >= o) run_w += up_w;
+          }
         }
-        __syncthreads();
-        if (lane == 31) s.warp_n[warp] = (unsigned)run_n, s.warp_w[warp] = run_w;
+        if (lane == 31) s.warp_n[warp] = run_n, s.warp_w[warp] = run_w;      // (the last reads of these lie before a barrier)
         if (tid == 0) s.bin = -1;
         __syncthreads();
-        u64 all_w = 0, all_n = 0;
+        u64 all_w = 0, upto_n = above_n + run_n, upto_w = above_w + run_w;
+#pragma unroll
         for (int k = 0; k < SA_WARPS; ++k) {
-          if (k < warp) run_n += s.warp_n[k], run_w += s.warp_w[k];
-          all_n += s.warp_n[k];
+          if (k < warp) upto_n += s.warp_n[k], upto_w += s.warp_w[k];
           all_w += s.warp_w[k];
         }
-        if (first && !count_them) limit = limit_of_mass(all_w);
-        run_n += above_n;
-        run_w += above_w;
-        const u64 upto = count_them ? run_n : run_w, before = upto - (count_them ? (u64)n : w);
-        if (before < limit && upto >= limit) {
-          s.bin = tid;
-          s.bin_n = n;
-          s.bin_w = w;
-          s.above_n = run_n - n;
-          s.above_w = run_w - w;
-        }
+        if (first && MASS) limit = mass_limit(all_w);
+        auto look = [&](int b, unsigned in, u64 mass, u64 n_end, u64 w_end) {
+          const u64 end = MASS ? w_end : n_end, begin = end - (MASS ? mass : in);
+          if (begin < limit && end >= limit) s.bin = b, s.bin_n = in, s.above_n = n_end - in, s.above_w = w_end - mass;
+        };
+        look(2 * tid, n.x, w0, upto_n - n.y, upto_w - w1);
+        look(2 * tid + 1, n.y, w1, upto_n, upto_w);
         __syncthreads();
         const int bin = s.bin;
-        if (bin < 0) {                                    // the limit is not reached: everything stays
-          mass = all_w;
-          return;
-        }
+        if (bin < 0) return false;                        // fewer words than the limit: all stay
         above_n = s.above_n;
         above_w = s.above_w;
         const unsigned in_bin = s.bin_n;
-        // its keys
-        if (first) {
+        if (!first) {
+          const unsigned lo_of = key_hi - ((unsigned)bin << shift), width = (1u << shift) - 1;
+          key_hi = lo_of;
+          key_lo = lo_of - key_lo > width ? lo_of - width : key_lo;
+        }
+        const bool finish = first && !(MASS && by_count) && above_n + in_bin <= SA_LIST;      // few words down to the limit: all of them are listed
+        auto inside = [&](float x, int i) {
+          if (MASS && by_count ? !kept(x, i) : !(x > -INFINITY)) return false;
+          if (first) {
+            const int b = bin_of(x);
+            return finish ? b <= bin : b == bin;
+          }
+          const unsigned k = sa_key(x);
+          return k >= key_lo && k <= key_hi;
+        };
+        if (finish || in_bin <= SA_LIST) {
+          auto list = [&](int i, float x) {
+            const int at = atomicAdd(&s.n_list[MASS], 1);      // (below SA_LIST: there are no more words)
+            s.list[MASS].word[at] = (u64)sa_key(x) << 32 | ~(unsigned)(v0 + i);
+          };
+          each([&](int i, const float4& x) {
+            const bool a0 = inside(x.x, i), a1 = inside(x.y, i + 1), a2 = inside(x.z, i + 2), a3 = inside(x.w, i + 3);
+            if (a0) list(i, x.x);
+            if (a1) list(i + 1, x.y);
+            if (a2) list(i + 2, x.z);
+            if (a3) list(i + 3, x.w);
+          });
+          sa_cluster<CTAS>();
+          if (finish && rank != 0) return true;
+          int n_all = 0;
+          u64 word = 0;
+          {
+            int sizes[CTAS];
+#pragma unroll
+            for (int c = 0; c < CTAS; ++c) sizes[c] = *sa_at(&s.n_list[MASS], c);
+#pragma unroll
+            for (int c = 0; c < CTAS; ++c) {
+              if (tid >= n_all && tid < n_all + sizes[c]) word = sa_at(&s.list[MASS], c)->word[tid - n_all];
+              n_all += sizes[c];
+            }
+          }
+          if (tid < SA_LIST) s.gathered.word[tid] = word;      // (0 stands behind all words)
+          __syncthreads();
+          // each word counts those before it: by two threads, half of the words each
+          const int mine = tid >> 1, half = tid & 1;
+          word = s.gathered.word[mine];
+          unsigned before = 0;                            // those before it in order, and (upper half) by index
+          for (int j = half * 2; j < n_all; j += 4) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&s.gathered.word[j]);
+            before += (o.x > word ? 1u : 0u) + (o.y > word ? 1u : 0u) + ((unsigned)o.x > (unsigned)word ? 0x10000u : 0u) + ((unsigned)o.y > (unsigned)word ? 0x10000u : 0u);
+          }
+          before += __shfl_xor_sync(0xffffffffu, before, 1);
+          const unsigned before_n = before & 0xffffu, before_at = before >> 16;
+          const bool is = mine < n_all && half == 0;
+          const float x = sa_of_key((unsigned)(word >> 32));
+          // of the first SA_LIST threads: the sum of v up to this one
+          auto upto = [&](u64 v) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+              if (lane >= o) v += up;
+            }
+            __syncthreads();
+            if (lane == 31) s.warp_w[warp] = v;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < SA_LIST / 32; ++k)
+              if (k < warp) v += s.warp_w[k];
+            return v;
+          };
+          // how many of the words in order stay
+          unsigned stay = MASS ? n_all : (unsigned)min(limit - (finish ? 0 : above_n), (u64)n_all);
+          if (MASS || (finish && by_mass)) {
+            if (tid < SA_LIST) s.sorted[tid] = 0;
+            if (tid == 0) s.last_rank = 0;
+            __syncthreads();
+            if (is && before_n < stay) s.sorted[before_n] = mass(x);
+            __syncthreads();
+            const u64 v = tid < SA_LIST ? s.sorted[tid] : 0, end = upto(v);
+            if (!MASS) limit = mass_limit([&] {           // of the mass that top_k has kept
+              u64 all = 0;
+#pragma unroll
+              for (int k = 0; k < SA_LIST / 32; ++k) all += s.warp_w[k];
+              return all;
+            }());
+            const unsigned in = __ballot_sync(0xffffffffu, tid < (int)stay && (finish ? 0 : above_w) + end - v < limit);      // (`end` of a warp's words is that of all)
+            if (lane == 0 && in) atomicAdd(&s.last_rank, __popc(in));
+            __syncthreads();
+            stay = s.last_rank;
+          }
+          if (!finish) {
+            __syncthreads();
+            if (is && before_n == stay - 1) {
+              s.last_key = (unsigned)(word >> 32);
+              s.last_at = (int)~(unsigned)word;
+            }
+            __syncthreads();
+            last_key = s.last_key;
+            last_at = s.last_at;
+            return false;
+          }
+          // all that can be kept is here: the draw
+          if (tid < SA_LIST) s.by_index[tid] = 0;
+          __syncthreads();
+          if (is && before_n < stay) {
+            const u64 w = weight(x);
+            s.by_index[before_at] = w >= w_min ? w : 0;
+            s.sorted[before_at] = ~(unsigned)word;
+          }
+          __syncthreads();
+          const u64 w = tid < SA_LIST ? s.by_index[tid] : 0, end = upto(w);
+          u64 all = 0;
+#pragma unroll
+          for (int k = 0; k < SA_LIST / 32; ++k) all += s.warp_w[k];
+          const u64 d = drawn(all);
+          if (w && d >= end - w && d < end) a.out[row] = (long long)s.sorted[tid];
+          return true;
+        }
+        if (first) {                                      // the range's keys
           auto edge = [&](int b) {                        // the least key whose range is b or one above it
             unsigned l = sa_key(lo), r = sa_key(hi);
             while (l < r) {
@@ -308,134 +515,67 @@ sample_kernel(const __grid_constant__ SampleArgs a, int ctas) {
           };
           key_lo = edge(bin);
           key_hi = bin ? edge(bin - 1) - 1 : sa_key(hi);
-        } else {
-          const u64 top_of = (u64)key_hi - ((u64)bin << shift), low_of = top_of - ((1ULL << shift) - 1);
-          key_lo = (long long)low_of < (long long)key_lo ? key_lo : (unsigned)low_of;
-          key_hi = (unsigned)top_of;
-        }
-        if (in_bin <= SA_LIST) {
-          // few words: each counts those before it
-          SaList& mine = s.list[lists & 1];
-          for (int i = from + lane; i < to; i += 32) {
-            const unsigned k = sa_key(z[i]);
-            if (z[i] > -INFINITY && k >= key_lo && k <= key_hi) {
-              const int at = atomicAdd(&mine.n, 1);       // (below SA_LIST: the range holds in_bin words)
-              mine.key[at] = k;
-              mine.at[at] = v0 + i;
-              mine.w[at] = weight(z[i]);
-            }
-          }
-          if (tid == 0) s.last_rank = 0;
-          sa_cluster(ctas);
-          int base = 0;
-          for (int c = 0; c < ctas; ++c) {
-            const SaList* o = sa_at(&mine, c);
-            const int m = o->n;
-            if (tid < m) {
-              s.gathered.key[base + tid] = o->key[tid];
-              s.gathered.at[base + tid] = o->at[tid];
-              s.gathered.w[base + tid] = o->w[tid];
-            }
-            base += m;
-          }
-          ++lists;
-          __syncthreads();
-          unsigned before_n = 0, key = 0;
-          u64 before_w = 0, w_own = 0;
-          int at = 0;
-          bool keep = false;
-          if (tid < base) {
-            key = s.gathered.key[tid];
-            at = s.gathered.at[tid];
-            w_own = s.gathered.w[tid];
-            for (int j = 0; j < base; ++j) {
-              const unsigned k = s.gathered.key[j];
-              if (k > key || (k == key && s.gathered.at[j] < at)) {
-                ++before_n;
-                before_w += s.gathered.w[j];
-              }
-            }
-            keep = (count_them ? above_n + before_n : above_w + before_w) < limit;
-            if (keep) atomicMax(&s.last_rank, before_n);
-          }
-          __syncthreads();
-          if (keep && before_n == s.last_rank) {
-            s.last_key = key;
-            s.last_at = at;
-            s.last_mass = above_w + before_w + w_own;
-          }
-          __syncthreads();
-          last_key = s.last_key;
-          last_at = s.last_at;
-          mass = s.last_mass;
-          return;
         }
         if (key_lo == key_hi) {
           // equal logits: as many as the limit allows, by their index
-          const u64 w_each = weight(sa_of_key(key_lo));
-          const u64 left = limit - (count_them ? above_n : above_w);      // > 0
-          const u64 take_n = count_them ? left : w_each ? min((left + w_each - 1) / w_each, (u64)in_bin) : (u64)in_bin;
           const float same = sa_of_key(key_lo);
-          const int i = locate([&](int k) -> u64 { return z[k] == same ? 1 : 0; }, [&](u64) { return take_n - 1; });
-          if (i >= 0 && tid < ctas) *sa_at(&s.last_at, tid) = v0 + i;
-          sa_cluster(ctas);
+          const u64 w_each = MASS ? mass(same) : 1, left = limit - (MASS ? above_w : above_n);      // > 0
+          const u64 n_left = w_each ? min((left + w_each - 1) / w_each, (u64)in_bin) : (u64)in_bin;
+          const int i = locate([&](int k, float x) -> u64 { return x == same && (!(MASS && by_count) || kept(x, k)) ? 1 : 0; }, 0, [&](u64) { return n_left - 1; });
+          if (i >= 0 && tid < CTAS) *sa_at(&s.last_at, tid) = v0 + i;
+          sa_cluster<CTAS>();
           last_key = key_lo;
           last_at = s.last_at;
-          mass = above_w + take_n * w_each;
-          return;
+          return false;
         }
-        // the range in 512 parts again
-        SaHist& p = s.part[parts & 1];
-        ++parts;
-        p.n[tid] = 0;
-        p.w[tid] = 0;
-        __syncthreads();
+        // the range in parts again
+        next_hist();
         const unsigned span = key_hi - key_lo;
         shift = 0;
         while (span >> shift >= SA_BINS) ++shift;
-        for (int i = from + lane; i < to; i += 32) {
-          const unsigned k = sa_key(z[i]);
-          if (z[i] > -INFINITY && k >= key_lo && k <= key_hi) {
-            const int b = (key_hi - k) >> shift;
-            const u64 w = weight(z[i]);
-            atomicAdd(&p.n[b], 1u);
-            if (w) atomicAdd(&p.w[b], w);
-          }
-        }
-        sa_cluster(ctas);
-        h = &p;
+        each([&](int i, const float4& x) {
+          const bool a0 = inside(x.x, i), a1 = inside(x.y, i + 1), a2 = inside(x.z, i + 2), a3 = inside(x.w, i + 3);
+          if (a0) count_in((key_hi - sa_key(x.x)) >> shift, MASS ? mass(x.x) : 0);
+          if (a1) count_in((key_hi - sa_key(x.y)) >> shift, MASS ? mass(x.y) : 0);
+          if (a2) count_in((key_hi - sa_key(x.z)) >> shift, MASS ? mass(x.z) : 0);
+          if (a3) count_in((key_hi - sa_key(x.w)) >> shift, MASS ? mass(x.w) : 0);
+        });
+        sa_cluster<CTAS>();
       }
     };
-    auto nothing = [](u64) { return (u64)0; };
-    if (by_count) cut(true, (u64)top_k, nothing);
-    if (by_mass) {
-      auto of = [&](u64 m) -> u64 {
-        const double x = ceil((double)top_p * (double)m);
-        return top_p > 0.f && x >= 1.0 ? (u64)x : 1ULL;
-      };
-      // (the first level has the whole row's mass: what top_k has kept takes its place)
-      const u64 kept = mass;
-      cut(false, 0, [&](u64 m) { return of(by_count ? kept : m); });
+    if ((by_count && cut(SaByCount(), (u64)top_k)) || (by_mass && cut(SaByMass(), 0))) {
+      sa_cluster<CTAS>();                                 // nobody leaves while others may read here
+      return;
     }
   }
   // ---- the draw
-  const float least = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
-  const u64 w_min = least > 0.f ? (u64)ceil((double)least * 8796093022208.0) : 0;
-  const double u = (double)u01;
-  const int i = locate(
-      [&](int k) -> u64 {
-        const float x = z[k];
-        const unsigned key = sa_key(x);
-        if (!(x > -INFINITY) || key < last_key || (key == last_key && v0 + k > last_at)) return 0;
-        const u64 w = weight(x);
-        return w >= w_min ? w : 0;
-      },
-      [&](u64 all) -> u64 {
-        const double x = u > 0.0 ? floor(u * (double)all) : 0.0;
-        return x < (double)all ? min((u64)x, all - 1) : all - 1;
-      });
+  const bool whole = !by_count && !by_mass && w_min == 0;
+  const int i = whole ? locate([&](int, float x) { return weight_bits(x); }, AT_512, drawn)
+                      : locate(
+                            [&](int k, float x) -> u64 {
+                              const bool on = kept(x, k);
+                              if (!__any_sync(__activemask(), on)) return 0;
+                              const u64 w = weight(x);
+                              return on && w >= w_min ? w : 0;
+                            },
+                            0, drawn);
   if (i >= 0 && tid == 0) a.out[row] = v0 + i;
-  sa_cluster(ctas);                                       // nobody leaves while others may read here
+  sa_cluster<CTAS>();                                     // nobody leaves while others may read here
+}
+
+template <typename T, int CTAS>
+static int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
+  const size_t smem = sizeof(SaShared) + (size_t)a.slice * 4;
+  LP_CHECK_CUDA((allow_smem<sample_kernel<T, CTAS>>((int)smem)));
+  LP_CHECK_CUDA(launch_ex(sample_kernel<T, CTAS>, dim3(rows * CTAS), dim3(SA_THREADS), smem, stream, CTAS, false, a));
+  return 0;
+}
+template <typename T>
+static int launch_sample_at(const SampleArgs& a, int rows, int ctas, cudaStream_t stream) {
+  if (ctas == 1) return launch_sample<T, 1>(a, rows, stream);
+  if (ctas == 2) return launch_sample<T, 2>(a, rows, stream);
+  if (ctas == 4) return launch_sample<T, 4>(a, rows, stream);
+  return launch_sample<T, 8>(a, rows, stream);
 }
 
 }  // namespace lp
@@ -454,20 +594,12 @@ extern "C" int lp_sample_tokens(const void* logits, int logits_fp32, long long l
   // CTAs of a row: so that each has 16,384 words at most, and few rows more of them
   int ctas = 1;
   while (ctas < SA_MAX_CTAS && ((V + ctas - 1) / ctas > 16384 || ((long long)rows * ctas < sm_count() && V / ctas > 4096))) ctas *= 2;
-  const int unit = SA_WARPS * 8;
+  const int unit = SA_WARPS * 128;
   SampleArgs a = {logits, rows > 1 ? ld : 0, uniform, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, V, ((V + ctas - 1) / ctas + unit - 1) / unit * unit, false, out};
   const long long size = logits_fp32 ? 4 : 2;
   a.vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && a.ld * size % 16 == 0;
-  const size_t smem = sizeof(SaShared) + (size_t)a.slice * 4;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LP_REQUIRE((long long)rows * ctas <= 2147483647LL, "lp_sample_tokens: %d rows", rows);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   note_launch(1);
-  if (logits_fp32) {
-    LP_CHECK_CUDA((allow_smem<sample_kernel<float>>((int)smem)));
-    LP_CHECK_CUDA(launch_ex(sample_kernel<float>, dim3(rows * ctas), dim3(SA_THREADS), smem, stream, ctas, false, a, ctas));
-  } else {
-    LP_CHECK_CUDA((allow_smem<sample_kernel<bf16>>((int)smem)));
-    LP_CHECK_CUDA(launch_ex(sample_kernel<bf16>, dim3(rows * ctas), dim3(SA_THREADS), smem, stream, ctas, false, a, ctas));
-  }
-  return 0;
+  return logits_fp32 ? launch_sample_at<float>(a, rows, ctas, stream) : launch_sample_at<bf16>(a, rows, ctas, stream);
 }
