@@ -53,7 +53,7 @@ __device__ __forceinline__ unsigned sa_key(float z) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float sa_of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-__constant__ double SA_ROOT[64] = {      // 2^(i / 64)
+__device__ const double SA_ROOT[64] = {      // 2^(i / 64)
     1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284, 1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
     1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418, 1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
     1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687, 1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
@@ -109,6 +109,8 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   const float t = a.temperature ? a.temperature[row] : a.temperature_all;
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all, u01 = a.uniform[row];
+
+  const double root = tid < 64 ? SA_ROOT[tid] : 0.0;
 
   // ---- the row (-inf behind its end), its largest and least logit
   const T* src = reinterpret_cast<const T*>(a.logits) + row * a.ld + v0;
@@ -167,7 +169,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   if (lane == 0) s.warp_top[warp] = make_float2(hi, lo);
   for (int i = tid; i < (int)(sizeof(s.hist) / 4); i += SA_THREADS) reinterpret_cast<unsigned*>(s.hist)[i] = 0;
   if (tid < 2) s.n_list[tid] = 0;
-  if (tid < 64) s.root[tid] = SA_ROOT[tid];
+  if (tid < 64) s.root[tid] = root;
   __syncthreads();
   if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp == 0) {
@@ -237,10 +239,18 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   int turn = 0;                                           // of s.total
   // The word (by index) up to which more than `limit` of value(i, z_i) lies, by all CTAs; limit = choose(the sum of all).  Returns its index in the one CTA that has it, -1 in the others.
   // value(...) is `base` too large.
-  auto locate = [&](auto value, u64 base, auto choose) -> int {
+  // on(i, z_i): whether a word counts at all.
+  auto locate = [&](auto on, auto value_of, u64 base, auto choose) -> int {
     u64 sum = 0;
-    each([&](int i, const float4& x) { sum += (value(i, x.x) + value(i + 1, x.y)) + (value(i + 2, x.z) + value(i + 3, x.w)); });
+    each([&](int i, const float4& x) {
+      const bool a0 = on(i, x.x), a1 = on(i + 1, x.y), a2 = on(i + 2, x.z), a3 = on(i + 3, x.w);
+      if (__any_sync(0xffffffffu, a0 || a1 || a2 || a3)) {
+        const u64 w0 = value_of(x.x), w1 = value_of(x.y), w2 = value_of(x.z), w3 = value_of(x.w);
+        sum += ((a0 ? w0 : base) + (a1 ? w1 : base)) + ((a2 ? w2 : base) + (a3 ? w3 : base));
+      }
+    });
     sum = sa_warp_sum(sum) - base * part;
+    auto value = [&](int i, float x) { return on(i, x) ? value_of(x) : base; };
     if (lane == 0) s.warp_w[warp] = sum;
     __syncthreads();
     u64 mine = 0;
@@ -408,10 +418,12 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           };
           each([&](int i, const float4& x) {
             const bool a0 = inside(x.x, i), a1 = inside(x.y, i + 1), a2 = inside(x.z, i + 2), a3 = inside(x.w, i + 3);
-            if (a0) list(i, x.x);
-            if (a1) list(i + 1, x.y);
-            if (a2) list(i + 2, x.z);
-            if (a3) list(i + 3, x.w);
+            if (__any_sync(0xffffffffu, a0 || a1 || a2 || a3)) {
+              if (a0) list(i, x.x);
+              if (a1) list(i + 1, x.y);
+              if (a2) list(i + 2, x.z);
+              if (a3) list(i + 3, x.w);
+            }
           });
           sa_cluster<CTAS>();
           if (finish && rank != 0) return true;
@@ -521,7 +533,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           const float same = sa_of_key(key_lo);
           const u64 w_each = MASS ? mass(same) : 1, left = limit - (MASS ? above_w : above_n);      // > 0
           const u64 n_left = w_each ? min((left + w_each - 1) / w_each, (u64)in_bin) : (u64)in_bin;
-          const int i = locate([&](int k, float x) -> u64 { return x == same && (!(MASS && by_count) || kept(x, k)) ? 1 : 0; }, 0, [&](u64) { return n_left - 1; });
+          const int i = locate([&](int k, float x) { return x == same && (!(MASS && by_count) || kept(x, k)); }, [](float) -> u64 { return 1; }, 0, [&](u64) { return n_left - 1; });
           if (i >= 0 && tid < CTAS) *sa_at(&s.last_at, tid) = v0 + i;
           sa_cluster<CTAS>();
           last_key = key_lo;
@@ -535,6 +547,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
         while (span >> shift >= SA_BINS) ++shift;
         each([&](int i, const float4& x) {
           const bool a0 = inside(x.x, i), a1 = inside(x.y, i + 1), a2 = inside(x.z, i + 2), a3 = inside(x.w, i + 3);
+          if (!__any_sync(0xffffffffu, a0 || a1 || a2 || a3)) return;
           if (a0) count_in((key_hi - sa_key(x.x)) >> shift, MASS ? mass(x.x) : 0);
           if (a1) count_in((key_hi - sa_key(x.y)) >> shift, MASS ? mass(x.y) : 0);
           if (a2) count_in((key_hi - sa_key(x.z)) >> shift, MASS ? mass(x.z) : 0);
@@ -550,15 +563,13 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   }
   // ---- the draw
   const bool whole = !by_count && !by_mass && w_min == 0;
-  const int i = whole ? locate([&](int, float x) { return weight_bits(x); }, AT_512, drawn)
-                      : locate(
-                            [&](int k, float x) -> u64 {
-                              const bool on = kept(x, k);
-                              if (!__any_sync(__activemask(), on)) return 0;
-                              const u64 w = weight(x);
-                              return on && w >= w_min ? w : 0;
-                            },
-                            0, drawn);
+  const int i = whole ? locate([](int, float) { return true; }, weight_bits, AT_512, drawn)
+                      : locate([&](int k, float x) { return kept(x, k); },
+                               [&](float x) {
+                                 const u64 w = weight(x);
+                                 return w >= w_min ? w : 0;
+                               },
+                               0, drawn);
   if (i >= 0 && tid == 0) a.out[row] = v0 + i;
   sa_cluster<CTAS>();                                     // nobody leaves while others may read here
 }
