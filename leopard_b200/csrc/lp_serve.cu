@@ -9,137 +9,172 @@ namespace lp {
 // ---- step tables ---------------------------------------------------------------------------------------------------
 //   row0[b] = sum of new[0 .. b),  row r of request b:  position lengths[b] + r - row0[b],  slot = page_table[b][position / size] size + position % size
 // Entries of the new rows' pages that are negative get the next pages of the free list, request after request and page after page.
-// One cluster does it all: every CTA adds up rows and missing pages of all requests (a few KB), then each gives pages to its share of them and, when all have, writes its share of
-// the rows.  Bound by latency: the chain lengths -> table -> free list -> table -> slot, two barriers of the cluster.
-constexpr int ST_THREADS = 1024, ST_MAX_BATCH = 8192, ST_FEW = 4;      // a span of more pages than ST_FEW is looked at by a whole warp
+// One cluster does it all.  Its CTAs share the requests, count their rows and missing pages and tell one another; every CTA adds up all of them, gives its requests their pages and, when all have, writes its
+// share of the rows.  Bound by latency: the chain lengths -> table -> sums -> free list -> table -> slot, two barriers of the cluster.
+constexpr int ST_MAX_BATCH = 8192, ST_FEW = 4;      // a span of more pages than ST_FEW is looked at by a whole warp
 
 struct StepTablesArgs {
   const int* lengths; const int* fresh;
   int* table; long long ld; int max_pages, size;
   const int* pages; int n_pages; int* used;
-  int B, rows;
+  int B, rows, each;                      // `each` requests a CTA
   int *row_seq, *row_pos; long long* slots; int* row0;
 };
 // the pages that a request's new rows lie in: [first, last), none where it brings nothing
 __device__ __forceinline__ void st_span(const StepTablesArgs& a, int len, int fresh, int& first, int& last) {
   first = (int)min((unsigned)len / (unsigned)a.size, (unsigned)a.max_pages);
-  last = fresh > 0 ? (int)min(((long long)len + fresh + a.size - 1) / a.size, (long long)a.max_pages) : first;
+  last = fresh > 0 ? (int)min(((unsigned)len + (unsigned)fresh - 1) / (unsigned)a.size + 1, (unsigned)a.max_pages) : first;
 }
-// inclusive sum over the block's threads; `total`: of all of them
-__device__ __forceinline__ long long st_scan(long long v, long long* warps, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += up;
-  }
-  if (lane == 31) warps[warp] = v;
-  __syncthreads();
-  long long w = warps[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += up;
-  }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const long long before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  __syncthreads();
-  return v + (warp ? before : 0);
-}
-__global__ void __launch_bounds__(ST_THREADS)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
 step_tables_kernel(const __grid_constant__ StepTablesArgs a) {
+  constexpr int WARPS = THREADS / 32;
   extern __shared__ int st_smem[];
-  int* row0 = st_smem;                    // [B + 1]
-  int* given = st_smem + a.B + 1;         // [B] pages given to the requests before
-  __shared__ long long warps[32];
-  const int lane = threadIdx.x & 31, cta = blockIdx.x, ctas = gridDim.x;
+  int* row0 = st_smem;                    // [B + 1]: tokens, then their sums
+  int* given = row0 + a.B + 1;            // [B]: missing pages, then those given to the requests before
+  int* past = given + a.B;                // [B]
+  int* wide = past + a.B;                 // [each]: requests of this CTA that want many pages
+  __shared__ long long warps[2][WARPS];
+  __shared__ int n_wide;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x, ctas = gridDim.x;
   const int base = min(max(a.used[0], 0), a.n_pages);
-  long long rows = 0, need = 0;
-  for (int b0 = 0; b0 < a.B; b0 += ST_THREADS) {
-    const int b = b0 + threadIdx.x;
-    int fresh = 0, first = 0, last = 0, missing = 0;
-    if (b < a.B) {
-      fresh = max(a.fresh[b], 0);
-      st_span(a, max(a.lengths[b], 0), fresh, first, last);
-      if (last - first <= ST_FEW)
+  if (threadIdx.x == 0) n_wide = 0;
+  if (ctas > 1) cluster_sync_all();       // (no CTA is written to before it has begun)
+  else __syncthreads();
+  auto tell = [&](int* place, int v) {
+    const uint32_t at = smem_u32(place);
+    if (ctas == 1) *place = v;
+    else
+      for (int c = 0; c < ctas; ++c) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(at, c)), "r"(v) : "memory");
+  };
+  const int b0 = cta * a.each, b1 = min(a.B, b0 + a.each);
+  for (int b = b0 + threadIdx.x; b < b1; b += THREADS) {
+    const int fresh = max(a.fresh[b], 0), len = max(a.lengths[b], 0);
+    int first, last, missing = 0;
+    st_span(a, len, fresh, first, last);
+    if (last - first <= ST_FEW) {
 #pragma unroll
-        for (int i = 0; i < ST_FEW; ++i)
-          if (first + i < last) missing += __ldcg(a.table + b * a.ld + first + i) < 0;
+      for (int i = 0; i < ST_FEW; ++i)
+        if (first + i < last) missing += a.table[b * a.ld + first + i] < 0;
+      tell(&given[b], missing);
+    } else {
+      wide[atomicAdd(&n_wide, 1)] = b;
     }
-    for (unsigned todo = __ballot_sync(0xffffffffu, last - first > ST_FEW); todo; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1, f = __shfl_sync(0xffffffffu, first, src), l = __shfl_sync(0xffffffffu, last, src);
-      const int* entries = a.table + (long long)__shfl_sync(0xffffffffu, b, src) * a.ld;
-      int n = 0;
-      for (int i = f + lane; i < l; i += 32) n += __ldcg(entries + i) < 0;
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == src) missing = n;
+    tell(&row0[b], fresh);
+    tell(&past[b], len);
+  }
+  __syncthreads();
+  for (int i = warp; i < n_wide; i += WARPS) {
+    const int b = wide[i];
+    int first, last, n = 0;
+    st_span(a, max(a.lengths[b], 0), max(a.fresh[b], 0), first, last);
+#pragma unroll 4
+    for (int k = first + lane; k < last; k += 32) n += a.table[b * a.ld + k] < 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) tell(&given[b], n);
+  }
+  if (ctas > 1) cluster_sync_all();       // all counts are here
+  else __syncthreads();
+  // their sums, in place
+  long long rows = 0, need = 0;
+  for (int s0 = 0; s0 < a.B; s0 += THREADS) {
+    const int b = s0 + threadIdx.x;
+    const int fresh = b < a.B ? row0[b] : 0, missing = b < a.B ? given[b] : 0;
+    long long r = fresh, m = missing;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up_r = __shfl_up_sync(0xffffffffu, r, o), up_m = __shfl_up_sync(0xffffffffu, m, o);
+      if (lane >= o) r += up_r, m += up_m;
     }
-    long long all_rows, all_need;
-    const long long r = st_scan(fresh, warps, all_rows), p = st_scan(missing, warps, all_need);
+    if (lane == 31) warps[0][warp] = r, warps[1][warp] = m;
+    __syncthreads();
+    long long wr = lane < WARPS ? warps[0][lane] : 0, wm = lane < WARPS ? warps[1][lane] : 0;
+#pragma unroll
+    for (int o = 1; o < WARPS; o <<= 1) {
+      const long long up_r = __shfl_up_sync(0xffffffffu, wr, o), up_m = __shfl_up_sync(0xffffffffu, wm, o);
+      if (lane >= o) wr += up_r, wm += up_m;
+    }
+    const long long all_r = __shfl_sync(0xffffffffu, wr, WARPS - 1), all_m = __shfl_sync(0xffffffffu, wm, WARPS - 1);
+    wr = __shfl_sync(0xffffffffu, wr, max(warp - 1, 0));
+    wm = __shfl_sync(0xffffffffu, wm, max(warp - 1, 0));
     if (b < a.B) {
-      row0[b] = (int)min(rows + r - fresh, 2147483647LL);
-      given[b] = (int)min(need + p - missing, 2147483647LL);
+      row0[b] = (int)min(rows + r - fresh + (warp ? wr : 0), 2147483647LL);
+      given[b] = (int)min(need + m - missing + (warp ? wm : 0), 2147483647LL);
     }
-    rows += all_rows;
-    need += all_need;
+    rows += all_r;
+    need += all_m;
+    __syncthreads();
   }
   if (threadIdx.x == 0) row0[a.B] = (int)min(rows, 2147483647LL);
   __syncthreads();
-  cluster_sync_all();                     // everybody knows the table as it was
   if (cta == 0 && threadIdx.x == 0) a.used[0] = (int)min((long long)a.n_pages, base + need);
-  for (int b = cta * ST_THREADS + threadIdx.x; b <= a.B; b += ctas * ST_THREADS) a.row0[b] = row0[b];
-  // pages: a warp takes 32 requests
-  const int per = (a.B + ctas * ST_THREADS - 1) / (ctas * ST_THREADS) * ST_THREADS;
-  for (int b0 = cta * per; b0 < min(a.B, (cta + 1) * per); b0 += ST_THREADS) {
-    const int b = b0 + threadIdx.x;
-    int first = 0, last = 0;
-    if (b < a.B) {
-      st_span(a, max(a.lengths[b], 0), max(a.fresh[b], 0), first, last);
-      if (last - first <= ST_FEW) {
-        long long at = (long long)base + given[b];
-        for (int i = first; i < last; ++i)
-          if (__ldcg(a.table + b * a.ld + i) < 0) {
-            if (at < a.n_pages) a.table[b * a.ld + i] = a.pages[at];
-            ++at;
-          }
+  for (int b = cta * THREADS + threadIdx.x; b <= a.B; b += ctas * THREADS) a.row0[b] = row0[b];
+  // pages
+  for (int b = b0 + threadIdx.x; b < b1; b += THREADS) {
+    int first, last;
+    st_span(a, past[b], max(a.fresh[b], 0), first, last);
+    if (last - first > ST_FEW) continue;
+    long long at = (long long)base + given[b];
+#pragma unroll
+    for (int i = 0; i < ST_FEW; ++i)
+      if (first + i < last && a.table[b * a.ld + first + i] < 0) {
+        if (at < a.n_pages) a.table[b * a.ld + first + i] = a.pages[at];
+        ++at;
       }
-    }
-    for (unsigned todo = __ballot_sync(0xffffffffu, last - first > ST_FEW); todo; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1, f = __shfl_sync(0xffffffffu, first, src), l = __shfl_sync(0xffffffffu, last, src), owner = __shfl_sync(0xffffffffu, b, src);
-      int* entries = a.table + (long long)owner * a.ld;
-      long long at = (long long)base + given[owner];
-      for (int i0 = f; i0 < l; i0 += 32) {
-        const bool gap = i0 + lane < l && __ldcg(entries + i0 + lane) < 0;
-        const unsigned gaps = __ballot_sync(0xffffffffu, gap);
-        const long long mine = at + __popc(gaps & ((1u << lane) - 1));
-        if (gap && mine < a.n_pages) entries[i0 + lane] = a.pages[mine];
-        at += __popc(gaps);
-      }
+  }
+  for (int i = warp; i < n_wide; i += WARPS) {
+    const int b = wide[i];
+    int first, last;
+    st_span(a, past[b], max(a.fresh[b], 0), first, last);
+    int* entries = a.table + b * a.ld;
+    long long at = (long long)base + given[b];
+    for (int k = first; k < last; k += 32) {
+      const bool gap = k + lane < last && entries[k + lane] < 0;
+      const unsigned gaps = __ballot_sync(0xffffffffu, gap);
+      const long long mine = at + __popc(gaps & ((1u << lane) - 1));
+      if (gap && mine < a.n_pages) entries[k + lane] = a.pages[mine];
+      at += __popc(gaps);
     }
   }
-  __syncthreads();
-  cluster_sync_all();                     // ... and as it is now
-  for (int r = cta * ST_THREADS + threadIdx.x; r < a.rows; r += ctas * ST_THREADS) {
-    int seq = -1, pos = -1;
-    long long slot = -1;
-    if (r < row0[a.B]) {
-      int lo = 0, hi = a.B - 1;           // the last request that begins at r or before it (those that bring nothing begin where the next one does)
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (row0[mid] <= r) lo = mid; else hi = mid - 1;
+  __threadfence();
+  if (ctas > 1) cluster_sync_all();       // the table is as it will be
+  else __syncthreads();
+  constexpr int AT_ONCE = 4;
+  const int steps = 32 - __clz(a.B);
+  for (int r0 = cta * THREADS + threadIdx.x; r0 < a.rows; r0 += ctas * THREADS * AT_ONCE) {
+    int seq[AT_ONCE], pos[AT_ONCE];
+    long long slot[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) seq[k] = 0;
+    for (int i = steps - 1; i >= 0; --i)  // the last request that begins at the row or before it (those that bring nothing begin where the next one does)
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int next = seq[k] + (1 << i);
+        if (next < a.B && row0[next] <= r0 + k * ctas * THREADS) seq[k] = next;
       }
-      seq = lo;
-      const long long at = (long long)max(a.lengths[lo], 0) + r - row0[lo];
-      pos = (int)min(at, 2147483647LL);
-      const long long logical = at / a.size;
-      if (logical < a.max_pages) {
-        const int page = __ldcg(a.table + lo * a.ld + logical);
-        if (page >= 0) slot = (long long)page * a.size + (at - logical * a.size);
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int r = r0 + k * ctas * THREADS;
+      slot[k] = pos[k] = -1;
+      if (r >= row0[a.B] || r >= a.rows) {
+        seq[k] = -1;
+        continue;
+      }
+      const unsigned at = (unsigned)past[seq[k]] + (unsigned)(r - row0[seq[k]]), logical = at / (unsigned)a.size;
+      pos[k] = (int)min(at, 2147483647u);
+      if (logical < (unsigned)a.max_pages) {
+        const int page = __ldcg(a.table + seq[k] * a.ld + logical);
+        if (page >= 0) slot[k] = (long long)page * a.size + (at - logical * a.size);
       }
     }
-    a.row_seq[r] = seq;
-    a.row_pos[r] = pos;
-    a.slots[r] = slot;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int r = r0 + k * ctas * THREADS;
+      if (r >= a.rows) break;
+      a.row_seq[r] = seq[k];
+      a.row_pos[r] = pos[k];
+      a.slots[r] = slot[k];
+    }
   }
 }
 
@@ -147,7 +182,7 @@ step_tables_kernel(const __grid_constant__ StepTablesArgs a) {
 //   y[i], y[i'] = s (x[i] cos a - x[i'] sin a),  s (x[i'] cos a + x[i] sin a),   a = position f[i],  i' = i + n ("half") or the pairs (2i, 2i + 1) ("interleaved")
 // The inverse (the gradient) turns by -a.  The angle is formed in 64 bits, in turns, of which whole ones are dropped: at position 10^6 a 32-bit angle is off by 0.03.  A CTA knows the angles of a few rows
 // (shared memory) and turns all heads of them, 16 bytes and their partners a thread.  Bound by HBM.
-constexpr int RO_THREADS = 256, RO_MAX_ROWS = 4, RO_MAX_FREQ = 256;
+constexpr int RO_MAX_FREQ = 256;
 
 struct RotarySeg {                        // heads of one tensor: x -> y
   const void* x; long long x_row, x_head;
@@ -179,101 +214,172 @@ template <> struct RotaryVec<bf16> {
   }
   static __device__ __forceinline__ uint4 put(const float* f) { return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])); }
 };
-template <typename T> __device__ __forceinline__ T rotary_as(float x);
-template <> __device__ __forceinline__ float rotary_as<float>(float x) { return x; }
-template <> __device__ __forceinline__ bf16 rotary_as<bf16>(float x) { return __float2bfloat16_rn(x); }
+template <typename T, bool VEC> struct RotaryRaw { typedef uint4 type; };
+template <typename T> struct RotaryRaw<T, false> { typedef T type; };
+template <typename T> __device__ __forceinline__ void rotary_get(const uint4& x, float* f) { RotaryVec<T>::get(x, f); }
+template <typename T> __device__ __forceinline__ void rotary_put(uint4& x, const float* f) { x = RotaryVec<T>::put(f); }
+template <typename T> __device__ __forceinline__ void rotary_get(const T& x, float* f) { f[0] = (float)x; }
+template <typename T> __device__ __forceinline__ void rotary_put(float& x, const float* f) { x = f[0]; }
+template <typename T> __device__ __forceinline__ void rotary_put(bf16& x, const float* f) { x = __float2bfloat16_rn(f[0]); }
 
+// Cosine and sine of frequency f stand at place ro_at(f): 16-byte pieces (two frequencies) change places within fours, so that the eight lanes that one shared-memory access serves, which take pieces
+// 1, 2 or 4 apart, find them in different banks (16,384 rows of 32 heads of 128, bf16: 53.6 us without, 41.9 with).
+__device__ __forceinline__ int ro_piece(int p) { return p ^ ((p >> 3) & 3); }
+__device__ __forceinline__ int ro_at(int f) { return 2 * ro_piece(f >> 1) + (f & 1); }
+__host__ __device__ __forceinline__ int ro_row(int n) { return (n + 7) & ~7; }
 // the angles' cosines and sines of `rows` rows from row0 on
+template <int THREADS>
 __device__ __forceinline__ void rotary_angles(const RotaryArgs& a, int row0, int rows, float2* cs) {
-  for (int i = threadIdx.x; i < rows * a.n; i += RO_THREADS) {
+  for (int i = threadIdx.x; i < rows * a.n; i += THREADS) {
     const int r = i / a.n, f = i - r * a.n;
     const long long pos = a.pos64 ? reinterpret_cast<const long long*>(a.pos)[row0 + r] : reinterpret_cast<const int*>(a.pos)[row0 + r];
     double turns = (double)pos * (double)a.freq[f] * 0.15915494309189533577;      // / 2 pi
     turns -= rint(turns);
     float s, c;
     sincospif(2.f * (float)turns, &s, &c);
-    cs[i] = make_float2(c * a.scale, s * a.sign * a.scale);
+    cs[r * ro_row(a.n) + ro_at(f)] = make_float2(c * a.scale, s * a.sign * a.scale);
   }
 }
-// VEC: 16 bytes at a time (strides, bases and the turned dimensions are multiples of them); else single values
-template <typename T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(RO_THREADS)
-rotary_kernel(const __grid_constant__ RotaryArgs a, int rows_each) {
-  __shared__ float2 cs[RO_MAX_ROWS * RO_MAX_FREQ];
-  constexpr int N = VEC ? RotaryVec<T>::N : 1;
-  const int row0 = blockIdx.x * rows_each, rows = min(rows_each, a.rows - row0);
-  rotary_angles(a, row0, rows, cs);
+// What a thread does of a row: a place of N dimensions and, "half", its partner; or (plain) a place that is copied.
+template <typename T, bool VEC>
+struct RotaryPlace {
+  typedef typename RotaryRaw<T, VEC>::type Raw;
+  static constexpr int N = VEC ? RotaryVec<T>::N : 1;
+  const RotarySeg* g;
+  int h, d, e, c;                         // head, its first dimension, its partner's (-1: none), its first angle (-1: plain)
+};
+// VEC: 16 bytes at a time (strides, bases and the turned dimensions are multiples of them); else single values.  A CTA takes ROWS rows; a thread the same places of all of them, the first ones' loads under
+// way while the angles are formed.
+template <typename T, bool HALF, bool VEC, int ROWS, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  typedef RotaryPlace<T, VEC> Place;
+  typedef typename Place::Raw Raw;
+  constexpr int N = Place::N;
+  constexpr bool PAIRS = VEC && !HALF;    // a place holds its pairs
+  extern __shared__ float4 ro_smem[];     // [ROWS][n, rounded up]
+  __shared__ long2 where[ROWS];           // page and row of a slot (page -1: none)
+  float2* cs = reinterpret_cast<float2*>(ro_smem);
+  const int row0 = blockIdx.x * ROWS, rows = min(ROWS, a.rows - row0);
+  const int turned = PAIRS ? 2 * a.n / N : a.n / N, plain = (a.D - 2 * a.n) / N, whole = a.D / N;
+  int items[3], all = 0;
+#pragma unroll
+  for (int s = 0; s < 3; ++s) {
+    items[s] = s < a.segs ? a.seg[s].heads * (a.seg[s].turned ? turned + (a.copy || a.seg[s].paged ? plain : 0) : whole) : 0;
+    all += items[s];
+  }
+  auto place = [&](int i) {
+    Place p;
+    const int s = i < items[0] ? 0 : i < items[0] + items[1] ? 1 : 2;
+    p.g = &a.seg[s];
+    i -= s > 0 ? items[0] : 0;
+    i -= s > 1 ? items[1] : 0;
+    const int units = items[s] / p.g->heads;
+    p.h = i / units;
+    const int u = i - p.h * units;
+    p.c = p.e = -1;
+    if (p.g->turned && u < turned) {
+      p.c = PAIRS ? u * (N / 2) : u * N;
+      p.d = VEC || HALF ? u * N : 2 * u;
+      if (!PAIRS) p.e = HALF ? p.d + a.n : p.d + 1;
+    } else {
+      p.d = p.g->turned ? 2 * a.n + (u - turned) * N : u * N;
+    }
+    return p;
+  };
+  Raw x[ROWS], w[ROWS];
+  auto load = [&](const Place& p) {
+    const T* at = reinterpret_cast<const T*>(p.g->x) + row0 * p.g->x_row + p.h * p.g->x_head;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (r < rows) {
+        x[r] = *reinterpret_cast<const Raw*>(at + r * p.g->x_row + p.d);
+        if (!PAIRS && p.e >= 0) w[r] = *reinterpret_cast<const Raw*>(at + r * p.g->x_row + p.e);
+      }
+  };
+  auto finish = [&](const Place& p) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (r >= rows) break;
+      T* y = reinterpret_cast<T*>(p.g->y) + p.h * p.g->y_head;
+      if (p.g->paged) {
+        const long2 at = where[r];
+        if (at.x < 0) continue;
+        y += at.x * p.g->y_page + at.y * p.g->y_row;
+      } else {
+        y += (row0 + r) * p.g->y_row;
+      }
+      if (p.c >= 0) {
+        float v[N], q[N];
+        float2 m[PAIRS ? N / 2 : N];
+        constexpr int ANGLES = PAIRS ? N / 2 : N;
+        if constexpr (ANGLES >= 2) {
+#pragma unroll
+          for (int k = 0; k < ANGLES / 2; ++k) {
+            const float4 two = ro_smem[r * (ro_row(a.n) / 2) + ro_piece(p.c / 2 + k)];
+            m[2 * k] = make_float2(two.x, two.y);
+            m[2 * k + 1] = make_float2(two.z, two.w);
+          }
+        } else {
+          m[0] = cs[r * ro_row(a.n) + ro_at(p.c)];
+        }
+        rotary_get<T>(x[r], v);
+        if constexpr (PAIRS) {
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) {
+            const float v0 = v[2 * k], v1 = v[2 * k + 1];
+            v[2 * k] = v0 * m[k].x - v1 * m[k].y;
+            v[2 * k + 1] = v1 * m[k].x + v0 * m[k].y;
+          }
+        } else {
+          rotary_get<T>(w[r], q);
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const float v0 = v[k], q0 = q[k];
+            v[k] = v0 * m[k].x - q0 * m[k].y;
+            q[k] = q0 * m[k].x + v0 * m[k].y;
+          }
+          rotary_put<T>(w[r], q);
+          *reinterpret_cast<Raw*>(y + p.e) = w[r];
+        }
+        rotary_put<T>(x[r], v);
+      }
+      *reinterpret_cast<Raw*>(y + p.d) = x[r];
+    }
+  };
+  Place p = place(min((int)threadIdx.x, all - 1));
+  if ((int)threadIdx.x < all) load(p);
+  if (a.slots && (int)threadIdx.x < rows) {
+    const long long slot = a.slots[row0 + threadIdx.x], page = slot / a.page_size;
+    where[threadIdx.x] = make_long2(slot >= 0 && slot < a.n_slots ? page : -1, slot - page * a.page_size);
+  }
+  rotary_angles<THREADS>(a, row0, rows, cs);
   __syncthreads();
-  // units of a head: pairs (two places of N, or one place of N whose neighbours are pairs), then what is not turned
-  const int turned = VEC && !HALF ? 2 * a.n / N : a.n / N, plain = (a.D - 2 * a.n) / N, whole = a.D / N;
-  for (int s = 0; s < a.segs; ++s) {
-    const RotarySeg& g = a.seg[s];
-    const int units = g.turned ? turned + (a.copy || g.paged ? plain : 0) : whole;
-    const int per_row = g.heads * units;
-    for (int i = threadIdx.x; i < rows * per_row; i += RO_THREADS) {
-      const int r = i / per_row, in = i - r * per_row, h = in / units, u = in - h * units;
-      const T* x = reinterpret_cast<const T*>(g.x) + (row0 + r) * g.x_row + h * g.x_head;
-      T* y = reinterpret_cast<T*>(g.y) + h * g.y_head;
-      if (g.paged) {
-        const long long slot = a.slots[row0 + r];
-        if (slot < 0 || slot >= a.n_slots) continue;
-        const long long page = slot / a.page_size;
-        y += page * g.y_page + (slot - page * a.page_size) * g.y_row;
-      } else {
-        y += (row0 + r) * g.y_row;
-      }
-      if (!g.turned || u >= turned) {
-        const int d = g.turned ? 2 * a.n + (u - turned) * N : u * N;
-        if (VEC) *reinterpret_cast<uint4*>(y + d) = *reinterpret_cast<const uint4*>(x + d);
-        else y[d] = x[d];
-        continue;
-      }
-      const float2* c = cs + r * a.n;
-      if (VEC && !HALF) {
-        float v[N];
-        RotaryVec<T>::get(*reinterpret_cast<const uint4*>(x + u * N), v);
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-          const float2 w = c[(u * N + k) >> 1];
-          const float p = v[k] * w.x - v[k + 1] * w.y, q = v[k + 1] * w.x + v[k] * w.y;
-          v[k] = p;
-          v[k + 1] = q;
-        }
-        *reinterpret_cast<uint4*>(y + u * N) = RotaryVec<T>::put(v);
-      } else if (VEC) {
-        float p[N], q[N];
-        RotaryVec<T>::get(*reinterpret_cast<const uint4*>(x + u * N), p);
-        RotaryVec<T>::get(*reinterpret_cast<const uint4*>(x + a.n + u * N), q);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const float2 w = c[u * N + k];
-          const float p0 = p[k] * w.x - q[k] * w.y, q0 = q[k] * w.x + p[k] * w.y;
-          p[k] = p0;
-          q[k] = q0;
-        }
-        *reinterpret_cast<uint4*>(y + u * N) = RotaryVec<T>::put(p);
-        *reinterpret_cast<uint4*>(y + a.n + u * N) = RotaryVec<T>::put(q);
-      } else {
-        const int i0 = HALF ? u : 2 * u, i1 = HALF ? u + a.n : 2 * u + 1;
-        const float p = (float)x[i0], q = (float)x[i1];
-        const float2 w = c[u];
-        y[i0] = rotary_as<T>(p * w.x - q * w.y);
-        y[i1] = rotary_as<T>(q * w.x + p * w.y);
-      }
+  for (int i = threadIdx.x; i < all;) {
+    finish(p);
+    i += THREADS;
+    if (i < all) {
+      p = place(i);
+      load(p);
     }
   }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-template <typename T, bool HALF>
-static int launch_rotary_as(const RotaryArgs& a, bool vec, cudaStream_t stream) {
-  const int rows = a.rows >= 8 * sm_count() && a.n * RO_MAX_ROWS <= RO_MAX_ROWS * RO_MAX_FREQ ? RO_MAX_ROWS : 1;
-  const dim3 grid((unsigned)((a.rows + rows - 1) / rows));
+template <typename T, bool HALF, bool VEC>
+static int launch_rotary_rows(const RotaryArgs& a, cudaStream_t stream) {
+  // four rows a CTA where there are enough of them to fill the GPU
+  const bool four = a.rows >= 8 * sm_count();
+  const unsigned ctas = four ? (unsigned)((a.rows + 3) / 4) : (unsigned)a.rows;
   note_launch(1);
-  if (vec) rotary_kernel<T, HALF, true><<<grid, RO_THREADS, 0, stream>>>(a, rows);
-  else rotary_kernel<T, HALF, false><<<grid, RO_THREADS, 0, stream>>>(a, rows);
+  if (four) rotary_kernel<T, HALF, VEC, 4, 256><<<ctas, 256, 4 * ro_row(a.n) * sizeof(float2), stream>>>(a);
+  else rotary_kernel<T, HALF, VEC, 1, 512><<<ctas, 512, ro_row(a.n) * sizeof(float2), stream>>>(a);
   LP_CHECK_CUDA(cudaGetLastError());
   return 0;
+}
+template <typename T, bool HALF>
+static int launch_rotary_as(const RotaryArgs& a, bool vec, cudaStream_t stream) {
+  return vec ? launch_rotary_rows<T, HALF, true>(a, stream) : launch_rotary_rows<T, HALF, false>(a, stream);
 }
 static int launch_rotary(RotaryArgs& a, int fp32, int interleaved, cudaStream_t stream) {
   const long long N = fp32 ? 4 : 8;
@@ -297,13 +403,21 @@ extern "C" int lp_step_tables(const int* lengths, const int* fresh, int* page_ta
   LP_REQUIRE(lengths && fresh && page_table && used && row0 && (n_free == 0 || free_pages) && (rows == 0 || (row_seq && row_pos && slots)), "lp_step_tables: null argument");
   LP_REQUIRE(B > 0 && B <= ST_MAX_BATCH, "lp_step_tables: B=%d (1 to %d)", B, ST_MAX_BATCH);
   LP_REQUIRE(page_size > 0 && max_pages > 0 && (B == 1 || ld_table >= max_pages), "lp_step_tables: %d pages of %d rows, ld_table %lld", max_pages, page_size, ld_table);
-  LP_REQUIRE(rows >= 0 && n_free >= 0, "lp_step_tables: rows=%d, %d free pages", rows, n_free);
-  StepTablesArgs a = {lengths, fresh, page_table, B == 1 ? 0 : ld_table, max_pages, page_size, free_pages, n_free, used, B, rows, row_seq, row_pos, slots, row0};
-  const int ctas = rows <= 4 * ST_THREADS && B <= ST_THREADS ? 1 : 8;
-  const size_t smem = (size_t)(2 * B + 1) * 4;
+  LP_REQUIRE((long long)max_pages * page_size <= 1LL << 31, "lp_step_tables: %d pages of %d rows are too many", max_pages, page_size);
+  LP_REQUIRE(rows >= 0 && rows <= 1 << 30 && n_free >= 0, "lp_step_tables: rows=%d, %d free pages", rows, n_free);
+  // one CTA while a thread has a row or two, then eight
+  const bool one = rows <= 2048 && B <= 1024, small = one && rows <= 512 && B <= 256;
+  const int ctas = one ? 1 : 8, each = (B + ctas - 1) / ctas;
+  StepTablesArgs a = {lengths, fresh, page_table, B == 1 ? 0 : ld_table, max_pages, page_size, free_pages, n_free, used, B, rows, each, row_seq, row_pos, slots, row0};
+  const size_t smem = (size_t)(3 * B + 1 + each) * 4;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   note_launch(1);
-  LP_CHECK_CUDA((allow_smem<step_tables_kernel>((int)smem)));
-  LP_CHECK_CUDA(launch_ex(step_tables_kernel, dim3(ctas), dim3(ST_THREADS), smem, reinterpret_cast<cudaStream_t>(stream_), ctas, false, a));
+  if (small) {
+    LP_CHECK_CUDA(launch_ex(step_tables_kernel<256>, dim3(1), dim3(256), smem, stream, 1, false, a));
+    return 0;
+  }
+  LP_CHECK_CUDA((allow_smem<step_tables_kernel<1024>>((int)smem)));
+  LP_CHECK_CUDA(launch_ex(step_tables_kernel<1024>, dim3(ctas), dim3(1024), smem, stream, ctas, false, a));
   return 0;
 }
 
