@@ -18,6 +18,7 @@ struct StepTablesArgs {
   int* table; long long ld; int max_pages, size;
   const int* pages; int n_pages; int* used;
   int B, rows, each;                      // `each` requests a CTA
+  bool wide_stores;                       // the row tables begin on 16 bytes
   int *row_seq, *row_pos; long long* slots; int* row0;
 };
 // the pages that a request's new rows lie in: [first, last), none where it brings nothing
@@ -25,7 +26,61 @@ __device__ __forceinline__ void st_span(const StepTablesArgs& a, int len, int fr
   first = (int)min((unsigned)len / (unsigned)a.size, (unsigned)a.max_pages);
   last = fresh > 0 ? (int)min(((unsigned)len + (unsigned)fresh - 1) / (unsigned)a.size + 1, (unsigned)a.max_pages) : first;
 }
-template <int THREADS>
+// rows: a thread takes PER neighbours
+template <int PER>
+__device__ __forceinline__ void st_rows(const StepTablesArgs& a, const int* row0, const int* past, int thread, int threads) {
+  const int steps = 32 - __clz(a.B), there = min(a.rows, row0[a.B]);
+  for (int r0 = thread * PER; r0 < a.rows; r0 += threads * PER) {
+    int seq[PER], pos[PER], b = -1, end = 0, page = -1;
+    long long slot[PER];
+    unsigned at = 0, logical = 0, in = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int r = r0 + k;
+      seq[k] = pos[k] = -1;
+      slot[k] = -1;
+      if (r >= there) continue;
+      bool look = true;
+      if (b < 0 || r >= end) {            // the last request that begins at the row or before it (those that bring nothing begin where the next one does)
+        b = 0;
+        for (int i = steps - 1; i >= 0; --i) {
+          const int next = b + (1 << i);
+          if (next < a.B && row0[next] <= r) b = next;
+        }
+        end = row0[b + 1];
+        at = (unsigned)max(past[b], 0) + (unsigned)(r - row0[b]);
+        logical = at / (unsigned)a.size;
+        in = at - logical * a.size;
+      } else {
+        ++at;
+        look = ++in == (unsigned)a.size;
+        if (look) ++logical, in = 0;
+      }
+      if (look) page = logical < (unsigned)a.max_pages ? __ldcg(a.table + b * a.ld + logical) : -1;
+      seq[k] = b;
+      pos[k] = (int)min(at, 2147483647u);
+      if (page >= 0) slot[k] = (long long)page * a.size + in;
+    }
+    if (PER % 4 == 0 && a.wide_stores && r0 + PER <= a.rows) {
+#pragma unroll
+      for (int k = 0; k + 3 < PER; k += 4) {
+        *reinterpret_cast<int4*>(a.row_seq + r0 + k) = make_int4(seq[k], seq[k + 1], seq[k + 2], seq[k + 3]);
+        *reinterpret_cast<int4*>(a.row_pos + r0 + k) = make_int4(pos[k], pos[k + 1], pos[k + 2], pos[k + 3]);
+        *reinterpret_cast<longlong2*>(a.slots + r0 + k) = make_longlong2(slot[k], slot[k + 1]);
+        *reinterpret_cast<longlong2*>(a.slots + r0 + k + 2) = make_longlong2(slot[k + 2], slot[k + 3]);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (r0 + k >= a.rows) break;
+      a.row_seq[r0 + k] = seq[k];
+      a.row_pos[r0 + k] = pos[k];
+      a.slots[r0 + k] = slot[k];
+    }
+  }
+}
+template <int THREADS, int PER>
 __global__ void __launch_bounds__(THREADS)
 step_tables_kernel(const __grid_constant__ StepTablesArgs a) {
   constexpr int WARPS = THREADS / 32;
@@ -37,6 +92,7 @@ step_tables_kernel(const __grid_constant__ StepTablesArgs a) {
   __shared__ long long warps[2][WARPS];
   __shared__ int n_wide;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x, ctas = gridDim.x;
+  pdl_launch_dependents();
   const int base = min(max(a.used[0], 0), a.n_pages);
   if (threadIdx.x == 0) n_wide = 0;
   if (ctas > 1) cluster_sync_all();       // (no CTA is written to before it has begun)
@@ -139,43 +195,16 @@ step_tables_kernel(const __grid_constant__ StepTablesArgs a) {
   __threadfence();
   if (ctas > 1) cluster_sync_all();       // the table is as it will be
   else __syncthreads();
-  constexpr int AT_ONCE = 4;
-  const int steps = 32 - __clz(a.B);
-  for (int r0 = cta * THREADS + threadIdx.x; r0 < a.rows; r0 += ctas * THREADS * AT_ONCE) {
-    int seq[AT_ONCE], pos[AT_ONCE];
-    long long slot[AT_ONCE];
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) seq[k] = 0;
-    for (int i = steps - 1; i >= 0; --i)  // the last request that begins at the row or before it (those that bring nothing begin where the next one does)
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {
-        const int next = seq[k] + (1 << i);
-        if (next < a.B && row0[next] <= r0 + k * ctas * THREADS) seq[k] = next;
-      }
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const int r = r0 + k * ctas * THREADS;
-      slot[k] = pos[k] = -1;
-      if (r >= row0[a.B] || r >= a.rows) {
-        seq[k] = -1;
-        continue;
-      }
-      const unsigned at = (unsigned)past[seq[k]] + (unsigned)(r - row0[seq[k]]), logical = at / (unsigned)a.size;
-      pos[k] = (int)min(at, 2147483647u);
-      if (logical < (unsigned)a.max_pages) {
-        const int page = __ldcg(a.table + seq[k] * a.ld + logical);
-        if (page >= 0) slot[k] = (long long)page * a.size + (at - logical * a.size);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const int r = r0 + k * ctas * THREADS;
-      if (r >= a.rows) break;
-      a.row_seq[r] = seq[k];
-      a.row_pos[r] = pos[k];
-      a.slots[r] = slot[k];
-    }
-  }
+  if (PER > 0) st_rows<(PER > 0 ? PER : 1)>(a, row0, past, cta * THREADS + threadIdx.x, ctas * THREADS);
+}
+// many rows: all SMs write them (63,897 of 256 prompts: 7.5 us by the cluster's eight)
+__global__ void __launch_bounds__(256)
+step_rows_kernel(const __grid_constant__ StepTablesArgs a) {
+  extern __shared__ int st_smem[];
+  pdl_wait();
+  for (int b = threadIdx.x; b <= a.B; b += 256) st_smem[b] = __ldcg(a.row0 + b);
+  __syncthreads();
+  st_rows<4>(a, st_smem, a.lengths, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- rotary positions ----------------------------------------------------------------------------------------------
@@ -405,19 +434,25 @@ extern "C" int lp_step_tables(const int* lengths, const int* fresh, int* page_ta
   LP_REQUIRE(page_size > 0 && max_pages > 0 && (B == 1 || ld_table >= max_pages), "lp_step_tables: %d pages of %d rows, ld_table %lld", max_pages, page_size, ld_table);
   LP_REQUIRE((long long)max_pages * page_size <= 1LL << 31, "lp_step_tables: %d pages of %d rows are too many", max_pages, page_size);
   LP_REQUIRE(rows >= 0 && rows <= 1 << 30 && n_free >= 0, "lp_step_tables: rows=%d, %d free pages", rows, n_free);
-  // one CTA while a thread has a row or two, then eight
-  const bool one = rows <= 2048 && B <= 1024, small = one && rows <= 512 && B <= 256;
+  // one CTA while a thread has a row or two, then eight; above 16,384 rows they are a kernel of their own
+  const bool one = rows <= 2048 && B <= 1024, small = rows <= 512 && B <= 256;
   const int ctas = one ? 1 : 8, each = (B + ctas - 1) / ctas;
-  StepTablesArgs a = {lengths, fresh, page_table, B == 1 ? 0 : ld_table, max_pages, page_size, free_pages, n_free, used, B, rows, each, row_seq, row_pos, slots, row0};
+  const bool wide = (reinterpret_cast<uintptr_t>(row_seq) | reinterpret_cast<uintptr_t>(row_pos) | reinterpret_cast<uintptr_t>(slots)) % 16 == 0;
+  StepTablesArgs a = {lengths, fresh, page_table, B == 1 ? 0 : ld_table, max_pages, page_size, free_pages, n_free, used, B, rows, each, wide, row_seq, row_pos, slots, row0};
   const size_t smem = (size_t)(3 * B + 1 + each) * 4;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  note_launch(1);
-  if (small) {
-    LP_CHECK_CUDA(launch_ex(step_tables_kernel<256>, dim3(1), dim3(256), smem, stream, 1, false, a));
-    return 0;
+  note_launch(rows <= 16384 ? 1 : 2);
+#define LP_TABLES(THREADS, PER)                                                                                                        \
+  {                                                                                                                                    \
+    LP_CHECK_CUDA((allow_smem<step_tables_kernel<THREADS, PER>>((int)smem)));                                                          \
+    LP_CHECK_CUDA(launch_ex(step_tables_kernel<THREADS, PER>, dim3(ctas), dim3(THREADS), smem, stream, ctas, false, a));               \
   }
-  LP_CHECK_CUDA((allow_smem<step_tables_kernel<1024>>((int)smem)));
-  LP_CHECK_CUDA(launch_ex(step_tables_kernel<1024>, dim3(ctas), dim3(1024), smem, stream, ctas, false, a));
+  if (small) LP_TABLES(256, 1) else if (rows <= 16384) LP_TABLES(1024, 1) else LP_TABLES(1024, 0)
+#undef LP_TABLES
+  if (rows > 16384) {
+    const int blocks = (rows + 1023) / 1024;
+    LP_CHECK_CUDA(launch_ex(step_rows_kernel, dim3(blocks < 2 * sm_count() ? blocks : 2 * sm_count()), dim3(256), (size_t)(B + 1) * 4, stream, 1, true, a));
+  }
   return 0;
 }
 

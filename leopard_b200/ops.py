@@ -845,7 +845,8 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     rows = int(rows)
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
-    both = torch.empty((2, rows), dtype=_I32, device=dev)
+    ld = -(-rows // 4) * 4
+    both = torch.empty((2, ld), dtype=_I32, device=dev)[:, :rows]
     slots = torch.empty((rows,), dtype=_I64, device=dev)
     if B == 0:
         return both[0].fill_(-1), both[1].fill_(-1), slots.fill_(-1), torch.zeros((1,), dtype=_I32, device=dev)
@@ -853,7 +854,7 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     L = _lib.lib()
     at = both.data_ptr()
     _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), page_table.stride(0), max_pages, int(page_size), free.data_ptr(), free.numel(),
-          used.data_ptr(), B, rows, at, at + 4 * rows, slots.data_ptr(), row0.data_ptr())
+          used.data_ptr(), B, rows, at, at + 4 * ld, slots.data_ptr(), row0.data_ptr())
     return both[0], both[1], slots, row0
 
 
