@@ -8,89 +8,65 @@
 
 namespace lp {
 
-// A CTA takes 16 rows of a key head and a piece of the keys; its four warps take 16 keys of each tile of 64.  mma.sync with nothing in shared memory on the way: a lane loads 16 bytes of each
-// of its keys' rows as they lie.  The products do not mind the order of what they sum over, so the dimensions of a head (and the columns of the values) are dealt to the operands' places as
-// the loads bring them; values of two keys are put side by side by byte permutations.
+// A CTA takes 16 rows of a key head and a piece of the keys; its four warps take 16 keys of each tile of 64.  mma.sync, keys and values straight into registers: a lane loads 16 bytes of each of its keys'
+// rows as they lie.  The products do not mind the order of what they sum over, so the dimensions of a head (and the columns of the values) are dealt to the operands' places as the loads bring them;
+// values of two keys are put side by side by byte permutations.  The queries are in shared memory as the product's first operand takes them, so that four CTAs fit on an SM.
+template <int D>
+constexpr int pa_smem(int B) { return 4 * PA_ROWS * (D + 8) * 4 + (B + 1) * 4; }
 template <int D>
 __global__ void __launch_bounds__(128, 3)
 prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
   constexpr int KC = D / 32, VC = (D + 63) / 64;                  // 16-byte pieces of a key's row a lane loads; of a value's
-  extern __shared__ int pa_first[];                               // [B + 1]
-  __shared__ float obuf[PA_ROWS][D + 4];
+  constexpr int LD = D / 4 + 2;                                   // 16-byte pieces from one row of a warp's sums to the next
+  extern __shared__ float4 pa_sums[];                             // [warp][PA_ROWS][LD]; before, the queries [KC][2][32]; then first
+  int* first = reinterpret_cast<int*>(pa_sums + 4 * PA_ROWS * LD);
+  uint4* queries = reinterpret_cast<uint4*>(pa_sums);
   __shared__ float2 ml[4][PA_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const bool pre = (int)blockIdx.x < pre_ctas;
   pdl_launch_dependents();
-  pa_tokens(a, pa_first);
 
   // ---- the piece
-  int kvh, r0, rows, n_keys, past, t0, t1, owner = 0;
-  const bool pre = (int)blockIdx.x < pre_ctas;
-  const bf16 *kb, *vb;
-  long long k_page, k_row, v_page, v_row;
-  const int* table;
-  int page_size, n_pages, page_of, key_first;
-  long long slot;
-  if (pre) {
-    rows = pa_first[a.d.B] * a.group;
-    const PrefixLine line = pa_line(a, rows);
-    long long u, u_end;
-    pa_range(a, line, blockIdx.x, u, u_end);
-    if (u >= u_end) return;
-    const PrefixPiece p = pa_piece(a, line, u, u_end);            // (the only one: there are as many CTAs as items can be)
-    kvh = p.kvh;
-    r0 = p.r0;
-    t0 = p.t0;
-    t1 = p.t0 + p.n;
-    past = n_keys = a.d.prefix;
-    slot = (long long)p.item + blockIdx.x;
-  } else {
-    int i = blockIdx.x - pre_ctas;
-    const int piece = i % a.own_splits;
-    slot = i;
-    i /= a.own_splits;
-    const int blk = i % a.own_blocks;
-    i /= a.own_blocks;
-    kvh = i % a.d.KVH;
+  int kvh, r0, rows, n_keys, past, t0, t1, owner = 0, slot, length = 0;
+  if (!pre) {
+    const int i = (int)(blockIdx.x - pre_ctas) / a.own_splits / a.own_blocks;
     owner = i / a.d.KVH;
-    r0 = blk * PA_ROWS;
-    const int fresh = pa_first[owner + 1] - pa_first[owner];
+    kvh = i - owner * a.d.KVH;
+    length = a.d.lengths[owner];
+  }
+  pa_tokens(a, first);
+  if (pre) {
+    rows = first[a.d.B] * a.group;
+    const PrefixLine line = pa_line(a, rows);
+    const int item = line.own ? (int)blockIdx.x / line.own : 0;
+    if (item >= line.items) return;
+    const int piece = blockIdx.x - item * line.own;               // (of as many CTAs as items can be, each has at most one)
+    kvh = item / line.blocks;
+    r0 = (item - kvh * line.blocks) * PA_ROWS;
+    t0 = pa_cut(a.pre_tiles, piece, line.own);
+    t1 = pa_cut(a.pre_tiles, piece + 1, line.own);
+    past = n_keys = a.d.prefix;
+    slot = item + blockIdx.x;
+  } else {
+    slot = blockIdx.x - pre_ctas;
+    const int rest = slot / a.own_splits, piece = slot - rest * a.own_splits;
+    r0 = rest % a.own_blocks * PA_ROWS;
+    const int fresh = first[owner + 1] - first[owner];
     rows = fresh * a.group;
-    pa_own(a, owner, fresh, past, n_keys);
-    const int tiles = (n_keys + PA_KEYS - 1) / PA_KEYS, pieces = pa_own_pieces(a, n_keys);
+    pa_own(a, length, fresh, past, n_keys);
+    const int pieces = pa_own_pieces(a, n_keys);
     if (piece >= pieces) return;
-    t0 = (int)((long long)tiles * piece / pieces);
-    t1 = (int)((long long)tiles * (piece + 1) / pieces);
+    const int tiles = (n_keys + PA_KEYS - 1) / PA_KEYS;
+    t0 = pa_cut(tiles, piece, pieces);
+    t1 = pa_cut(tiles, piece + 1, pieces);
   }
   if (r0 >= rows) return;
-  if (pre && a.d.prefix_k) {
-    kb = reinterpret_cast<const bf16*>(a.d.prefix_k) + kvh * a.d.pk_head, vb = reinterpret_cast<const bf16*>(a.d.prefix_v) + kvh * a.d.pv_head;
-    k_page = v_page = 0, k_row = a.d.pk_row, v_row = a.d.pv_row;
-    table = nullptr, page_size = 0, n_pages = 1, page_of = 0, key_first = 0;
-  } else {
-    kb = reinterpret_cast<const bf16*>(a.d.k) + kvh * a.d.k_head, vb = reinterpret_cast<const bf16*>(a.d.v) + kvh * a.d.v_head;
-    k_page = a.d.k_page, v_page = a.d.v_page, k_row = a.d.k_row, v_row = a.d.v_row;
-    table = a.d.page_table ? a.d.page_table + owner * a.d.ld_table : nullptr;
-    page_size = a.d.page_size, n_pages = a.d.n_pages, page_of = owner, key_first = table && !pre ? a.d.prefix : 0;
-  }
-
-  // ---- this lane's two rows
-  uint32_t qa[KC][2][4];
-  int limit[2];                                                   // keys that a row sees
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = r0 + g + 8 * h;
-    const bool there = r < rows;
-    const int i = there ? r / a.group : 0, head = kvh * a.group + (there ? r - i * a.group : 0);
-    const int b = pre ? pa_find(pa_first, a.d.B, i) : owner, t = pre ? i - pa_first[b] : i;
-    const bf16* q = reinterpret_cast<const bf16*>(a.d.q) + b * a.d.q_batch + t * a.d.q_token + head * a.d.q_head + t4 * 8;
-    limit[h] = pre ? n_keys : min(n_keys, past + t + 1);
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const uint4 x = there ? *reinterpret_cast<const uint4*>(q + c * 32) : make_uint4(0, 0, 0, 0);
-      qa[c][h][0] = x.x, qa[c][h][1] = x.y, qa[c][h][2] = x.z, qa[c][h][3] = x.w;
-    }
-  }
-  const int sure = pre ? n_keys : min(n_keys, past + 1);          // keys that all rows see
+  const bool apart = pre && a.d.prefix_k;                         // the prefix has a cache of its own
+  const bf16* kb = apart ? reinterpret_cast<const bf16*>(a.d.prefix_k) + kvh * a.d.pk_head : reinterpret_cast<const bf16*>(a.d.k) + kvh * a.d.k_head;
+  const bf16* vb = apart ? reinterpret_cast<const bf16*>(a.d.prefix_v) + kvh * a.d.pv_head : reinterpret_cast<const bf16*>(a.d.v) + kvh * a.d.v_head;
+  const long long k_row = apart ? a.d.pk_row : a.d.k_row, v_row = apart ? a.d.pv_row : a.d.v_row, k_page = a.d.k_page, v_page = a.d.v_page;
+  const int* table = a.d.page_table && !apart ? a.d.page_table + owner * a.d.ld_table : nullptr;
+  const int page_of = apart ? 0 : owner, key_first = table && !pre ? a.d.prefix : 0;
 
   // where the warp's 16 keys of a tile lie: lane i (and i + 16) knows key i's page and row
   int2 place;
@@ -99,9 +75,9 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     place = make_int2(-1, 0);
     if (tile < t1 && key < n_keys) {
       if (table) {
-        const unsigned at = (unsigned)key + (unsigned)key_first, logical = at / (unsigned)page_size;
+        const unsigned at = (unsigned)key + (unsigned)key_first, logical = at / (unsigned)a.d.page_size;
         const int page = table[logical];
-        place = make_int2(page < n_pages ? page : -1, (int)(at - logical * page_size));
+        place = make_int2(page < a.d.n_pages ? page : -1, (int)(at - logical * a.d.page_size));
       } else {
         place = make_int2(page_of, key);
       }
@@ -113,7 +89,7 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int page = __shfl_sync(0xffffffffu, place.x, j * 8 + g), row = __shfl_sync(0xffffffffu, place.y, j * 8 + g);
-      const bf16* p = kb + page * k_page + row * k_row + t4 * 8;
+      const bf16* p = kb + (apart ? 0 : page * k_page) + row * k_row + t4 * 8;
 #pragma unroll
       for (int c = 0; c < KC; ++c) kr[j][c] = page >= 0 ? ldg_once(p + c * 32) : none;
     }
@@ -123,11 +99,27 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     for (int j = 0; j < 4; ++j) {
       const int key = (j >> 1) * 8 + 2 * t4 + (j & 1);
       const int page = __shfl_sync(0xffffffffu, at.x, key), row = __shfl_sync(0xffffffffu, at.y, key);
-      const bf16* p = vb + page * v_page + row * v_row + g * 8;
+      const bf16* p = vb + (apart ? 0 : page * v_page) + row * v_row + g * 8;
 #pragma unroll
       for (int c = 0; c < VC; ++c) vr[j][c] = page >= 0 && c * 8 + g < D / 8 ? ldg_once(p + c * 64) : none;
     }
   };
+  locate(t0);
+  // ---- this lane's two rows: how many keys they see; their queries
+  int limit[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = r0 + g + 8 * h;
+    const bool there = r < rows;
+    const int i = there ? r / a.group : 0, head = kvh * a.group + (there ? r - i * a.group : 0);
+    const int b = pre ? pa_find(first, a.d.B, i) : owner, t = pre ? i - first[b] : i;
+    limit[h] = pre ? n_keys : min(n_keys, past + t + 1);
+    for (int c = warp; c < KC; c += 4) {
+      const bf16* q = reinterpret_cast<const bf16*>(a.d.q) + b * a.d.q_batch + t * a.d.q_token + head * a.d.q_head + t4 * 8 + c * 32;
+      queries[(c * 2 + h) * 32 + lane] = there ? *reinterpret_cast<const uint4*>(q) : none;
+    }
+  }
+  const int sure = pre ? n_keys : min(n_keys, past + 1);          // keys that all rows see
   float o[VC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < VC; ++c)
@@ -135,21 +127,22 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[c][j][k] = 0.f;
-
-  locate(t0);
   load_k();
   load_v(place);
   int2 here = place;
   locate(t0 + 1);
+  __syncthreads();                                                // the queries are there
   for (int tile = t0; tile < t1; ++tile) {
     float s[2][4] = {};
 #pragma unroll
-    for (int c = 0; c < KC; ++c)
+    for (int c = 0; c < KC; ++c) {
+      const uint4 qa = lds_u4(queries + c * 64 + lane), qb = lds_u4(queries + c * 64 + 32 + lane);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        mma_bf16(s[j], qa[c][0][0], qa[c][1][0], qa[c][0][1], qa[c][1][1], kr[j][c].x, kr[j][c].y);
-        mma_bf16(s[j], qa[c][0][2], qa[c][1][2], qa[c][0][3], qa[c][1][3], kr[j][c].z, kr[j][c].w);
+        mma_bf16(s[j], qa.x, qb.x, qa.y, qb.y, kr[j][c].x, kr[j][c].y);
+        mma_bf16(s[j], qa.z, qb.z, qa.w, qb.w, kr[j][c].z, kr[j][c].w);
       }
+    }
     const int2 next = place;
     load_k();                                                     // (of the next tile)
     locate(tile + 2);
@@ -218,7 +211,7 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
         for (int key = 0; key < 16; ++key) {
           const int page = __shfl_sync(0xffffffffu, here.x, key), row = __shfl_sync(0xffffffffu, here.y, key);
           if (page < 0) continue;
-          const bf16* p = vb + page * v_page + row * v_row;
+          const bf16* p = vb + (apart ? 0 : page * v_page) + row * v_row;
 #pragma unroll
           for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -252,57 +245,58 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     load_v(next);
     here = next;
   }
-  // ---- the warps' rows together
+  // ---- the warps' rows together: 16-byte pieces, of which eights change places so that the eight lanes that one access serves find them in different banks
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     if (t4 == 0) ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
   }
-  __syncthreads();
-  float f[2];
+  __syncthreads();                                                // (the queries are done with)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][g + 8 * h].x);
-    f[h] = m[h] == -INFINITY ? 1.f : pa_ex2(m[h] - top);          // (sums and values of a warp that saw nothing are zeros, or NaN)
+    const float f = m[h] == -INFINITY ? 1.f : pa_ex2(m[h] - top);      // (sums and values of a warp that saw nothing are zeros, or NaN)
+    float4* at = pa_sums + (warp * PA_ROWS + g + 8 * h) * LD;
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int piece = c * 8 + 2 * t4 + x;
+        if (piece < D / 8)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int p4 = piece * 2 + j;
+            at[p4 ^ ((p4 >> 3) & 1)] = make_float4(o[c][4 * j][2 * h + x] * f, o[c][4 * j + 1][2 * h + x] * f, o[c][4 * j + 2][2 * h + x] * f, o[c][4 * j + 3][2 * h + x] * f);
+          }
+      }
   }
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w == warp)
-#pragma unroll
-      for (int c = 0; c < VC; ++c)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int piece = c * 8 + 2 * t4 + x;
-          if (piece < D / 8)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float* at = &obuf[g + 8 * h][piece * 8 + j];
-                const float v = o[c][j][2 * h + x] * f[h];
-                *at = w == 0 ? v : *at + v;
-              }
-        }
-    __syncthreads();
-  }
+  __syncthreads();
   const int mine = min(PA_ROWS, rows - r0);
-  float* po = (pre ? a.pre_o : a.own_o) + slot * (D * PA_ROWS);
-  float2* pm = (pre ? a.pre_ml : a.own_ml) + slot * PA_ROWS;
-  for (int i = threadIdx.x; i < PA_ROWS * (D / 4); i += 128) {
-    const int r = i % PA_ROWS, c4 = i / PA_ROWS;
-    if (r >= mine) continue;
-    *reinterpret_cast<float4*>(po + (c4 * PA_ROWS + r) * 4) = *reinterpret_cast<const float4*>(&obuf[r][c4 * 4]);
-    if (c4 == 0) {
-      float2 x = make_float2(-INFINITY, 0.f);
+  float* po = (pre ? a.pre_o : a.own_o) + (long long)slot * (D * PA_ROWS);
+  float2* pm = (pre ? a.pre_ml : a.own_ml) + (long long)slot * PA_ROWS;
+  const int r = threadIdx.x % PA_ROWS;
+  if (r >= mine) return;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) x.x = fmaxf(x.x, ml[w][r].x);
+  for (int i = 0; i < D / 32; ++i) {
+    const int c4 = i * 8 + threadIdx.x / PA_ROWS, from = r * LD + (c4 ^ ((c4 >> 3) & 1));
+    float4 x = pa_sums[from];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) x.y += ml[w][r].y * (ml[w][r].x == -INFINITY ? 1.f : pa_ex2(ml[w][r].x - x.x));
-      pm[r] = x;
+    for (int w = 1; w < 4; ++w) {
+      const float4 y = pa_sums[w * PA_ROWS * LD + from];
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
+    *reinterpret_cast<float4*>(po + (c4 * PA_ROWS + r) * 4) = x;
+  }
+  if (threadIdx.x < PA_ROWS) {
+    float2 x = make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x.x = fmaxf(x.x, ml[w][r].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x.y += ml[w][r].y * (ml[w][r].x == -INFINITY ? 1.f : pa_ex2(ml[w][r].x - x.x));
+    pm[r] = x;
   }
 }
 
@@ -321,7 +315,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
   if (r0 >= rows) return;
   const int r = min(r0 + in, rows - 1), i = r / a.group, g = r - i * a.group, b = pa_find(pa_first, a.d.B, i), t = i - pa_first[b];
   int past, keys;
-  pa_own(a, b, pa_first[b + 1] - pa_first[b], past, keys);
+  pa_own(a, a.d.lengths[b], pa_first[b + 1] - pa_first[b], past, keys);
   int n_pre = 0, pre_in = 0;
   long long pre_slot = 0;
   if (a.pre_ctas) {
@@ -387,6 +381,7 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   LP_REQUIRE((long long)d->B * d->T * d->H <= 1LL << 24, "lp_prefix_attention: %d requests of %d tokens and %d heads are too many", d->B, d->T, d->H);
   LP_REQUIRE(d->n_pages > 0 && d->page_size > 0 && d->max_pages > 0, "lp_prefix_attention: %d pages of %d rows, %d a request", d->n_pages, d->page_size, d->max_pages);
   LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 256, "lp_prefix_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
+  LP_REQUIRE(d->B * (long long)d->KVH * ((d->T * (d->H / d->KVH) + PA_ROWS - 1) / PA_ROWS) <= 1 << 24, "lp_prefix_attention: %d requests of %d tokens over %d key heads are too many", d->B, d->T, d->KVH);
   LP_REQUIRE(d->prefix >= 0 && d->prefix <= (1LL << 31) - 256, "lp_prefix_attention: prefix %d", d->prefix);
   if (d->prefix_k) LP_REQUIRE(!d->page_table && d->prefix_v, "lp_prefix_attention: a prefix of its own goes with a cache of its own each");
   else if (d->page_table) LP_REQUIRE(d->prefix <= (long long)d->max_pages * d->page_size, "lp_prefix_attention: a prefix of %d rows in %d pages of %d", d->prefix, d->max_pages, d->page_size);
@@ -477,7 +472,8 @@ extern "C" int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* worksp
   note_launch(tc ? 3 : 2);
 #define LP_PREFIX(DD)                                                                                             \
   {                                                                                                               \
-    prefix_rows_kernel<DD><<<(unsigned)ctas, 128, first, stream>>>(a, pre_ctas);                                  \
+    LP_CHECK_CUDA((allow_smem<prefix_rows_kernel<DD>>(pa_smem<DD>(d->B))));                                       \
+    prefix_rows_kernel<DD><<<(unsigned)ctas, 128, pa_smem<DD>(d->B), stream>>>(a, pre_ctas);                      \
     LP_CHECK_CUDA(cudaGetLastError());                                                                            \
     if (tc) { if (const int rc = launch_prefix_tc(a, stream)) return rc; }                                        \
     LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD>, join, dim3(PJ_ROWS * DD / 4), first, stream, 1, true, a));    \

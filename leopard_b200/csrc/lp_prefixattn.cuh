@@ -64,9 +64,9 @@ __device__ __forceinline__ int pa_find(const int* first, int B, int i) {
   }
   return lo;
 }
-// own rows of request b before its new tokens, and with them (as far as there is room for rows)
-__device__ __forceinline__ void pa_own(const PrefixArgs& a, int b, int fresh, int& past, int& keys) {
-  const int own = max(max(a.d.lengths[b], 0) - a.d.prefix, 0);
+// own rows of a request before its new tokens, and with them (as far as there is room for rows)
+__device__ __forceinline__ void pa_own(const PrefixArgs& a, int length, int fresh, int& past, int& keys) {
+  const int own = max(max(length, 0) - a.d.prefix, 0);
   past = min(own, a.own_rows);
   keys = (int)min((long long)own + fresh, (long long)a.own_rows);
 }
@@ -85,9 +85,10 @@ __device__ __forceinline__ PrefixLine pa_line(const PrefixArgs& a, int rows) {
   }
   return l;
 }
-__device__ __forceinline__ long long pa_cut(long long total, int k, int n) {      // the k-th of n equal ranges begins here
-  const long long each = total / n;
-  return each * k + min((long long)k, total - each * n);
+template <typename T>
+__device__ __forceinline__ T pa_cut(T total, int k, int n) {      // the k-th of n equal ranges begins here
+  const T each = total / n, more = total - each * n;
+  return each * k + min((T)k, more);
 }
 __device__ __forceinline__ void pa_range(const PrefixArgs& a, const PrefixLine& l, int cta, long long& from, long long& to) {
   from = to = 0;

@@ -495,6 +495,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
+  pdl_wait();                           // (begun beside the own rows' kernel; the join, which waits for this one, needs that one to be over too)
   if (warp == 3) {
     __syncwarp();
     tmem_dealloc(tmem_base, 512);
@@ -536,12 +537,11 @@ static int launch_tc(const PrefixTc& tc, cudaStream_t stream) {
   const size_t smem = (split ? 7 : 6) * NB * PT_BOX + PT_BARS + (split ? 128 * 8 : 0) + (size_t)(d.B + 1) * 4 + 1024;
   if (split) {
     LP_CHECK_CUDA((allow_smem<prefix_tc_kernel<DH, true>>((int)smem)));
-    prefix_tc_kernel<DH, true><<<tc.a.pre_ctas, PT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+    LP_CHECK_CUDA(launch_ex(prefix_tc_kernel<DH, true>, dim3(tc.a.pre_ctas), dim3(PT_THREADS), smem, stream, 1, true, tm[0], tm[1], tc));
   } else {
     LP_CHECK_CUDA((allow_smem<prefix_tc_kernel<DH, false>>((int)smem)));
-    prefix_tc_kernel<DH, false><<<tc.a.pre_ctas, PT_THREADS, smem, stream>>>(tm[0], tm[1], tc);
+    LP_CHECK_CUDA(launch_ex(prefix_tc_kernel<DH, false>, dim3(tc.a.pre_ctas), dim3(PT_THREADS), smem, stream, 1, true, tm[0], tm[1], tc));
   }
-  LP_CHECK_CUDA(cudaGetLastError());
   return 0;
 }
 
