@@ -8,49 +8,50 @@
 
 namespace lp {
 
-// A CTA takes 16 rows of a key head and a piece of the keys; its four warps take 16 keys of each tile of 64.  mma.sync, keys and values straight into registers: a lane loads 16 bytes of each of its keys'
-// rows as they lie.  The products do not mind the order of what they sum over, so the dimensions of a head (and the columns of the values) are dealt to the operands' places as the loads bring them;
-// values of two keys are put side by side by byte permutations.  The queries are in shared memory as the product's first operand takes them, so that four CTAs fit on an SM.
+// A CTA takes 8 NT rows of a key head and a piece of the keys; its four warps take 16 keys of each tile of 64.  mma.sync, keys and values straight into registers: a lane loads 16 bytes of each of its keys'
+// rows as they lie.  Keys are the products' 16 rows and the queries' rows their 8 columns, since few rows look at the same keys (four of a token with eight key heads of 32).  A product does not mind the order of
+// what it sums over, so the dimensions of a head are dealt to the operands' places as the loads bring them: piece t + 4 c of a key's 16-byte pieces goes to places 2t, 2t + 1 and 2t + 8, 2t + 9 of steps
+// 2c and 2c + 1.  In the second product the dimensions are the rows, values of two keys put side by side by byte permutations.
 template <int D>
-constexpr int pa_smem(int B) { return 4 * PA_ROWS * (D + 8) * 4 + (B + 1) * 4; }
-template <int D>
-__global__ void __launch_bounds__(128, 3)
-prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
-  constexpr int KC = D / 32, VC = (D + 63) / 64;                  // 16-byte pieces of a key's row a lane loads; of a value's
-  constexpr int LD = D / 4 + 2;                                   // 16-byte pieces from one row of a warp's sums to the next
-  extern __shared__ float4 pa_sums[];                             // [warp][PA_ROWS][LD]; before, the queries [KC][2][32]; then first
-  int* first = reinterpret_cast<int*>(pa_sums + 4 * PA_ROWS * LD);
-  uint4* queries = reinterpret_cast<uint4*>(pa_sums);
-  __shared__ float2 ml[4][PA_ROWS];
+constexpr int pa_ld() { return D / 4 + 1; }                       // 16-byte pieces from one row of a warp's sums to the next (eight rows' in eight different banks)
+template <int D, int NT>
+constexpr int pa_smem() { return 4 * 8 * NT * pa_ld<D>() * 16; }
+template <int D, int NT, bool PRE>
+__device__ __forceinline__ void prefix_rows(const PrefixArgs& a, int cta) {
+  constexpr int KC = D / 32, VC = (D + 63) / 64, ROWS = 8 * NT;   // 16-byte pieces of a key's row a lane loads; of a value's
+  constexpr int LD = pa_ld<D>();
+  extern __shared__ float4 pa_sums[];                             // first, and behind it [warp][ROWS][LD]; before, the queries [KC][NT][32]
+  int* first = reinterpret_cast<int*>(pa_sums);
+  float4* sums = pa_sums + (a.d.B + 4) / 4;
+  uint4* queries = reinterpret_cast<uint4*>(sums);
+  __shared__ float2 ml[4][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-  const bool pre = (int)blockIdx.x < pre_ctas;
-  pdl_launch_dependents();
 
   // ---- the piece
   int kvh, r0, rows, n_keys, past, t0, t1, owner = 0, slot, length = 0;
-  if (!pre) {
-    const int i = (int)(blockIdx.x - pre_ctas) / a.own_splits / a.own_blocks;
+  if (!PRE) {
+    const int i = cta / a.own_splits / a.own_blocks;
     owner = i / a.d.KVH;
     kvh = i - owner * a.d.KVH;
     length = a.d.lengths[owner];
   }
   pa_tokens(a, first);
-  if (pre) {
+  if (PRE) {
     rows = first[a.d.B] * a.group;
     const PrefixLine line = pa_line(a, rows);
-    const int item = line.own ? (int)blockIdx.x / line.own : 0;
+    const int item = line.own ? cta / line.own : 0;
     if (item >= line.items) return;
-    const int piece = blockIdx.x - item * line.own;               // (of as many CTAs as items can be, each has at most one)
+    const int piece = cta - item * line.own;                      // (of as many CTAs as items can be, each has at most one)
     kvh = item / line.blocks;
-    r0 = (item - kvh * line.blocks) * PA_ROWS;
+    r0 = (item - kvh * line.blocks) * ROWS;
     t0 = pa_cut(a.pre_tiles, piece, line.own);
     t1 = pa_cut(a.pre_tiles, piece + 1, line.own);
     past = n_keys = a.d.prefix;
-    slot = item + blockIdx.x;
+    slot = item + cta;
   } else {
-    slot = blockIdx.x - pre_ctas;
+    slot = cta;
     const int rest = slot / a.own_splits, piece = slot - rest * a.own_splits;
-    r0 = rest % a.own_blocks * PA_ROWS;
+    r0 = rest % a.own_blocks * ROWS;
     const int fresh = first[owner + 1] - first[owner];
     rows = fresh * a.group;
     pa_own(a, length, fresh, past, n_keys);
@@ -61,12 +62,13 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     t1 = pa_cut(tiles, piece + 1, pieces);
   }
   if (r0 >= rows) return;
-  const bool apart = pre && a.d.prefix_k;                         // the prefix has a cache of its own
+  const bool apart = PRE && a.d.prefix_k;                         // the prefix has a cache of its own
   const bf16* kb = apart ? reinterpret_cast<const bf16*>(a.d.prefix_k) + kvh * a.d.pk_head : reinterpret_cast<const bf16*>(a.d.k) + kvh * a.d.k_head;
   const bf16* vb = apart ? reinterpret_cast<const bf16*>(a.d.prefix_v) + kvh * a.d.pv_head : reinterpret_cast<const bf16*>(a.d.v) + kvh * a.d.v_head;
-  const long long k_row = apart ? a.d.pk_row : a.d.k_row, v_row = apart ? a.d.pv_row : a.d.v_row, k_page = a.d.k_page, v_page = a.d.v_page;
   const int* table = a.d.page_table && !apart ? a.d.page_table + owner * a.d.ld_table : nullptr;
-  const int page_of = apart ? 0 : owner, key_first = table && !pre ? a.d.prefix : 0;
+  const int page_of = apart ? 0 : owner, key_first = !PRE && table ? a.d.prefix : 0;
+  auto key_at = [&](int page, int row) { return kb + (apart ? row * a.d.pk_row : page * a.d.k_page + row * a.d.k_row); };
+  auto value_at = [&](int page, int row) { return vb + (apart ? row * a.d.pv_row : page * a.d.v_page + row * a.d.v_row); };
 
   // where the warp's 16 keys of a tile lie: lane i (and i + 16) knows key i's page and row
   int2 place;
@@ -89,7 +91,7 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int page = __shfl_sync(0xffffffffu, place.x, j * 8 + g), row = __shfl_sync(0xffffffffu, place.y, j * 8 + g);
-      const bf16* p = kb + (apart ? 0 : page * k_page) + row * k_row + t4 * 8;
+      const bf16* p = key_at(page, row) + t4 * 8;
 #pragma unroll
       for (int c = 0; c < KC; ++c) kr[j][c] = page >= 0 ? ldg_once(p + c * 32) : none;
     }
@@ -99,103 +101,115 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     for (int j = 0; j < 4; ++j) {
       const int key = (j >> 1) * 8 + 2 * t4 + (j & 1);
       const int page = __shfl_sync(0xffffffffu, at.x, key), row = __shfl_sync(0xffffffffu, at.y, key);
-      const bf16* p = vb + (apart ? 0 : page * v_page) + row * v_row + g * 8;
+      const bf16* p = value_at(page, row) + g * 8;
 #pragma unroll
       for (int c = 0; c < VC; ++c) vr[j][c] = page >= 0 && c * 8 + g < D / 8 ? ldg_once(p + c * 64) : none;
     }
   };
   locate(t0);
-  // ---- this lane's two rows: how many keys they see; their queries
-  int limit[2];
+  // ---- the queries, a piece a warp: row g (+ 8) as the first product's columns
+  uint4 qx[NT];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = r0 + g + 8 * h;
+  for (int n = 0; n < NT; ++n) {
+    const int r = r0 + 8 * n + g;
     const bool there = r < rows;
     const int i = there ? r / a.group : 0, head = kvh * a.group + (there ? r - i * a.group : 0);
-    const int b = pre ? pa_find(first, a.d.B, i) : owner, t = pre ? i - first[b] : i;
-    limit[h] = pre ? n_keys : min(n_keys, past + t + 1);
-    for (int c = warp; c < KC; c += 4) {
-      const bf16* q = reinterpret_cast<const bf16*>(a.d.q) + b * a.d.q_batch + t * a.d.q_token + head * a.d.q_head + t4 * 8 + c * 32;
-      queries[(c * 2 + h) * 32 + lane] = there ? *reinterpret_cast<const uint4*>(q) : none;
-    }
+    const int b = PRE ? pa_find(first, a.d.B, i) : owner, t = PRE ? i - first[b] : i;
+    const bf16* q = reinterpret_cast<const bf16*>(a.d.q) + b * a.d.q_batch + t * a.d.q_token + head * a.d.q_head + t4 * 8 + warp * 32;
+    qx[n] = there && warp < KC ? *reinterpret_cast<const uint4*>(q) : none;
   }
-  const int sure = pre ? n_keys : min(n_keys, past + 1);          // keys that all rows see
-  float o[VC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < VC; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[c][j][k] = 0.f;
   load_k();
   load_v(place);
   int2 here = place;
   locate(t0 + 1);
-  __syncthreads();                                                // the queries are there
+  // keys that this lane's rows (two of each eight) see, and that all rows see
+  int limit[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) limit[n][h] = PRE ? n_keys : min(n_keys, past + (r0 + 8 * n + 2 * t4 + h) / a.group + 1);
+  const int sure = PRE ? n_keys : min(n_keys, past + 1);
+  if (warp < KC)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) queries[(warp * NT + n) * 32 + lane] = qx[n];
+  __syncthreads();
+
+  int odd = 0;                                                    // values that are not finite were left out
+  float o[NT][VC][4][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[n][c][j][k] = 0.f;
+  }
   for (int tile = t0; tile < t1; ++tile) {
-    float s[2][4] = {};
+    float s[NT][4];                                               // keys g, g (row 2t4, 2t4 + 1), g + 8, g + 8
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const uint4 qa = lds_u4(queries + c * 64 + lane), qb = lds_u4(queries + c * 64 + 32 + lane);
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mma_bf16(s[j], qa.x, qb.x, qa.y, qb.y, kr[j][c].x, kr[j][c].y);
-        mma_bf16(s[j], qa.z, qb.z, qa.w, qb.w, kr[j][c].z, kr[j][c].w);
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 q = lds_u4(queries + (c * NT + n) * 32 + lane);
+        mma_bf16(s[n], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, q.x, q.y);
+        mma_bf16(s[n], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, q.z, q.w);
       }
-    }
     const int2 next = place;
     load_k();                                                     // (of the next tile)
     locate(tile + 2);
     const int key0 = tile * PA_KEYS + warp * 16;
     const unsigned there = __ballot_sync(0xffffffffu, here.x >= 0) & 0xffffu;
     const bool tail = key0 + 16 > sure;
+    bool grow = tile == t0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[j][k] *= a.scale_log2;
-    if (tail || there != 0xffffu) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = j * 8 + 2 * t4 + (k & 1);
-          if (!((there >> key) & 1) || key0 + key >= limit[k >> 1]) s[j][k] = -INFINITY;
+      for (int k = 0; k < 4; ++k) {
+        s[n][k] *= a.scale_log2;
+        if (tail || there != 0xffffu) {
+          const int key = g + 8 * (k >> 1);
+          if (!((there >> key) & 1) || key0 + key >= limit[n][k & 1]) s[n][k] = -INFINITY;
         }
-    }
-    float mx[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(m[h], fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)));
-    }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float f = m[h] == -INFINITY ? 0.f : pa_ex2(m[h] - mx[h]);
-        m[h] = mx[h];
-        l[h] *= f;
-#pragma unroll
-        for (int c = 0; c < VC; ++c)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[c][j][2 * h] *= f, o[c][j][2 * h + 1] *= f;
+        grow |= s[n][k] > m[n][k & 1] + 8.f;
       }
-    }
+    // weights are taken to a maximum that is at most 2^8 too small: sums and values are scaled when one grows past that
+    if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float ref = m[h] == -INFINITY ? 0.f : m[h];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(s[n][h], s[n][2 + h]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          s[j][2 * h + k] = pa_ex2(s[j][2 * h + k] - ref);
-          l[h] += s[j][2 * h + k];
+          for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          mx = fmaxf(mx, m[n][h]);
+          const float f = m[n][h] == -INFINITY ? 0.f : pa_ex2(m[n][h] - mx);
+          m[n][h] = mx;
+          l[n][h] *= f;
+#pragma unroll
+          for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][c][j][h] *= f, o[n][c][j][2 + h] *= f;
         }
     }
-    // weights go into the second product as bf16 (half a step is 2^-8 of a weight); their sum was taken before
-    const uint32_t p0 = pack_bf16x2(s[0][0], s[0][1]), p1 = pack_bf16x2(s[0][2], s[0][3]), p2 = pack_bf16x2(s[1][0], s[1][1]), p3 = pack_bf16x2(s[1][2], s[1][3]);
-    if (tail && a.d.T > 1) {                                      // 0 x NaN: values that are not finite are left out of the product, and reach the rows that see them
-      bool odd = false;
+    uint32_t p[NT][2];                                            // weights as the second product's columns: rows g, keys 2t4, 2t4 + 1 (+ 8)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[k] = pa_ex2(s[n][k] - (m[n][k & 1] == -INFINITY ? 0.f : m[n][k & 1]));
+        l[n][k & 1] += w[k];
+      }
+      // as bf16 (half a step is 2^-8 of a weight); their sum was taken before
+      asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][0]) : "r"(pack_bf16x2(w[0], w[1])));
+      asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][1]) : "r"(pack_bf16x2(w[2], w[3])));
+    }
+    if (!PRE && tail && a.d.T > 1) {                              // 0 x NaN: values that are not finite are left out of the product, and reach the rows that see them at the end
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -203,94 +217,85 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
           uint32_t* w = &vr[j][c].x;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u, odd = true;
-            if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu, odd = true;
+            if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u, odd = 1;
+            if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu, odd = 1;
           }
         }
-      if (__any_sync(0xffffffffu, odd)) {
-        for (int key = 0; key < 16; ++key) {
-          const int page = __shfl_sync(0xffffffffu, here.x, key), row = __shfl_sync(0xffffffffu, here.y, key);
-          if (page < 0) continue;
-          const bf16* p = vb + (apart ? 0 : page * v_page) + row * v_row;
-#pragma unroll
-          for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int piece = c * 8 + 2 * t4 + x;
-              if (piece >= D / 8) continue;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float v = __bfloat162float(p[piece * 8 + j]);
-                if (not_finite(v)) {
-                  if (key0 + key < limit[0]) o[c][j][x] += v;
-                  if (key0 + key < limit[1]) o[c][j][2 + x] += v;
-                }
-              }
-            }
-        }
-      }
     }
 #pragma unroll
     for (int c = 0; c < VC; ++c) {
-      const uint32_t* x0 = &vr[0][c].x;
-      const uint32_t* x1 = &vr[1][c].x;
-      const uint32_t* y0 = &vr[2][c].x;
-      const uint32_t* y1 = &vr[3][c].x;
+      const uint32_t *x0 = &vr[0][c].x, *x1 = &vr[1][c].x, *y0 = &vr[2][c].x, *y1 = &vr[3][c].x;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-        mma_bf16(o[c][j], p0, p1, p2, p3, __byte_perm(x0[j >> 1], x1[j >> 1], sel), __byte_perm(y0[j >> 1], y1[j >> 1], sel));
+      for (int j = 0; j < 4; ++j) {                               // rows g: dimension 8 (8 c + g) + 2 j, rows g + 8: the next one
+        const uint32_t a0 = __byte_perm(x0[j], x1[j], 0x5410), a1 = __byte_perm(x0[j], x1[j], 0x7632), a2 = __byte_perm(y0[j], y1[j], 0x5410), a3 = __byte_perm(y0[j], y1[j], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_bf16(o[n][c][j], a0, a1, a2, a3, p[n][0], p[n][1]);
       }
     }
     load_v(next);
     here = next;
   }
-  // ---- the warps' rows together: 16-byte pieces, of which eights change places so that the eight lanes that one access serves find them in different banks
+  // ---- the warps' rows together.  Of a row's 16-byte pieces the even ones stand first, then the odd ones: eight lanes' stores find different banks.
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (t4 == 0) ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
-  }
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], x);
+      if (g == 0) ml[warp][8 * n + 2 * t4 + h] = make_float2(m[n][h], l[n][h]);
+    }
   __syncthreads();                                                // (the queries are done with)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float top = -INFINITY;
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][g + 8 * h].x);
-    const float f = m[h] == -INFINITY ? 1.f : pa_ex2(m[h] - top);      // (sums and values of a warp that saw nothing are zeros, or NaN)
-    float4* at = pa_sums + (warp * PA_ROWS + g + 8 * h) * LD;
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * n + 2 * t4 + h;
+      float top = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < VC; ++c)
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][r].x);
+      const float f = m[n][h] == -INFINITY ? 1.f : pa_ex2(m[n][h] - top);      // (sums and values of a warp that saw nothing are zeros, or NaN)
+      float4* at = sums + (warp * ROWS + r) * LD;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int piece = c * 8 + 2 * t4 + x;
-        if (piece < D / 8)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int p4 = piece * 2 + j;
-            at[p4 ^ ((p4 >> 3) & 1)] = make_float4(o[c][4 * j][2 * h + x] * f, o[c][4 * j + 1][2 * h + x] * f, o[c][4 * j + 2][2 * h + x] * f, o[c][4 * j + 3][2 * h + x] * f);
-          }
+      for (int c = 0; c < VC; ++c)
+        if (c * 8 + g < D / 8) {
+          const float(&x)[4][4] = o[n][c];
+          at[c * 8 + g] = make_float4(x[0][h] * f, x[0][2 + h] * f, x[1][h] * f, x[1][2 + h] * f);
+          at[D / 8 + c * 8 + g] = make_float4(x[2][h] * f, x[2][2 + h] * f, x[3][h] * f, x[3][2 + h] * f);
+        }
+    }
+  if (__syncthreads_or(odd)) {      // (PRE: never)
+    // the tiles that some rows do not see whole: a thread looks at one dimension of all their keys
+    const int k0 = max(t0 * PA_KEYS, sure & ~15), k1 = min(t1 * PA_KEYS, n_keys);
+    for (int d = threadIdx.x; d < D; d += 128) {
+      float* to = reinterpret_cast<float*>(sums + (d >> 3) + ((d >> 2) & 1) * (D / 8)) + d % 4;
+      for (int key = k0; key < k1; ++key) {
+        const unsigned at = (unsigned)key + (unsigned)key_first, logical = table ? at / (unsigned)a.d.page_size : 0;
+        const int page = table ? table[logical] : page_of;
+        if (page < 0 || page >= a.d.n_pages) continue;
+        const float v = __bfloat162float(value_at(page, table ? (int)(at - logical * a.d.page_size) : key)[d]);
+        if (!not_finite(v)) continue;
+        for (int r = 0; r < min(ROWS, rows - r0); ++r)
+          if (key < past + (r0 + r) / a.group + 1) to[r * LD * 4] += v;
       }
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const int mine = min(PA_ROWS, rows - r0);
-  float* po = (pre ? a.pre_o : a.own_o) + (long long)slot * (D * PA_ROWS);
-  float2* pm = (pre ? a.pre_ml : a.own_ml) + (long long)slot * PA_ROWS;
-  const int r = threadIdx.x % PA_ROWS;
+  const int mine = min(ROWS, rows - r0), r = threadIdx.x % ROWS;
+  float* po = (PRE ? a.pre_o : a.own_o) + (long long)slot * (D * ROWS);
+  float2* pm = (PRE ? a.pre_ml : a.own_ml) + (long long)slot * ROWS;
   if (r >= mine) return;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int c4 = i * 8 + threadIdx.x / PA_ROWS, from = r * LD + (c4 ^ ((c4 >> 3) & 1));
-    float4 x = pa_sums[from];
+  for (int c4 = threadIdx.x / ROWS; c4 < D / 4; c4 += 128 / ROWS) {
+    const int from = r * LD + (c4 >> 1) + (c4 & 1) * (D / 8);
+    float4 x = sums[from];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
-      const float4 y = pa_sums[w * PA_ROWS * LD + from];
+      const float4 y = sums[w * ROWS * LD + from];
       x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    *reinterpret_cast<float4*>(po + (c4 * PA_ROWS + r) * 4) = x;
+    *reinterpret_cast<float4*>(po + (c4 * ROWS + r) * 4) = x;
   }
-  if (threadIdx.x < PA_ROWS) {
+  if (threadIdx.x < ROWS) {
     float2 x = make_float2(-INFINITY, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; ++w) x.x = fmaxf(x.x, ml[w][r].x);
@@ -299,20 +304,40 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
     pm[r] = x;
   }
 }
+// PRE: the prefix's pieces come first, of 8 PRE rows; then the own rows', of 8 OWN
+template <int D, int PRE, int OWN>
+__global__ void __launch_bounds__(128, PRE == 2 || OWN == 2 ? 3 : 4)
+prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
+  pdl_launch_dependents();
+  if constexpr (PRE > 0) {
+    if ((int)blockIdx.x < pre_ctas) {
+      prefix_rows<D, PRE, true>(a, blockIdx.x);
+      return;
+    }
+  }
+  prefix_rows<D, OWN, false>(a, blockIdx.x - pre_ctas);
+}
 
-// The pieces of a row together: a CTA takes 8 rows of a key head, a thread four columns of one; weights follow a running maximum, so that each piece is read once, eight at a time.
+// The pieces of a row together: a CTA takes 8 rows of a key head, a thread four columns of one and, of GROUPS groups, every GROUPS-th eight pieces, which are under way at once; weights follow a running maximum, so
+// that each piece is read once.  Bound by latency, and by the workspace's way through L2.
 constexpr int PJ_ROWS = 8, PJ_AT_ONCE = 8;
-template <int D>
-__global__ void __launch_bounds__(PJ_ROWS * D / 4)
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(PJ_ROWS * D / 4 * GROUPS)
 prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
+  constexpr int THREADS = PJ_ROWS * D / 4;
   extern __shared__ int pa_first[];
   __shared__ __align__(16) bf16 done[PJ_ROWS][D + 8];
   __shared__ long long to[PJ_ROWS];
-  const int kvh = blockIdx.y, in = threadIdx.x % PJ_ROWS, c4 = threadIdx.x / PJ_ROWS;
+  __shared__ float4 more_x[GROUPS > 1 ? GROUPS - 1 : 1][GROUPS > 1 ? THREADS : 1];
+  __shared__ float2 more_ml[GROUPS > 1 ? GROUPS - 1 : 1][GROUPS > 1 ? THREADS : 1];
+  const int group = GROUPS > 1 ? threadIdx.x / THREADS : 0, tid = GROUPS > 1 ? threadIdx.x - group * THREADS : threadIdx.x;
+  const int kvh = blockIdx.y, in = tid % PJ_ROWS, c4 = tid / PJ_ROWS;
   pa_tokens(a, pa_first);
   const int rows = pa_first[a.d.B] * a.group, r0 = blockIdx.x * PJ_ROWS;
-  pdl_wait();
-  if (r0 >= rows) return;
+  if (r0 >= rows) {
+    pdl_wait();
+    return;
+  }
   const int r = min(r0 + in, rows - 1), i = r / a.group, g = r - i * a.group, b = pa_find(pa_first, a.d.B, i), t = i - pa_first[b];
   int past, keys;
   pa_own(a, a.d.lengths[b], pa_first[b + 1] - pa_first[b], past, keys);
@@ -327,12 +352,13 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
     n_pre = c1 - c0 + 1;
     pre_slot = (long long)item + c0;
   }
-  const int own = t * a.group + g, n = n_pre + pa_own_pieces(a, keys), own_blk = own / PA_ROWS, own_in = own - own_blk * PA_ROWS;
+  const int own = t * a.group + g, n = n_pre + pa_own_pieces(a, keys), own_blk = own / a.own_block, own_in = own - own_blk * a.own_block;
   const long long own_slot = (((long long)b * a.d.KVH + kvh) * a.own_blocks + own_blk) * a.own_splits;
-  if (c4 == 0) to[in] = r0 + in < rows ? b * a.d.o_batch + t * a.d.o_token + (kvh * a.group + g) * a.d.o_head : -1;
+  if (tid < PJ_ROWS && group == 0) to[tid] = r0 + tid < rows ? b * a.d.o_batch + t * a.d.o_token + (kvh * a.group + g) * a.d.o_head : -1;
+  pdl_wait();
   float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < n; p0 += PJ_AT_ONCE) {
+  for (int p0 = group * PJ_AT_ONCE; p0 < n; p0 += GROUPS * PJ_AT_ONCE) {
     float2 ml[PJ_AT_ONCE];
     float4 y[PJ_AT_ONCE];
 #pragma unroll
@@ -345,8 +371,8 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
         y[k] = *reinterpret_cast<const float4*>(a.pre_o + (((pre_slot + p) * (D / 4) + c4) * a.pre_rows + pre_in) * 4);
       } else if (p < n) {
         const long long s = own_slot + p - n_pre;
-        ml[k] = a.own_ml[s * PA_ROWS + own_in];
-        y[k] = *reinterpret_cast<const float4*>(a.own_o + ((s * (D / 4) + c4) * PA_ROWS + own_in) * 4);
+        ml[k] = a.own_ml[s * a.own_block + own_in];
+        y[k] = *reinterpret_cast<const float4*>(a.own_o + ((s * (D / 4) + c4) * a.own_block + own_in) * 4);
       }
     }
     float m = top;
@@ -363,8 +389,30 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
       x.x += y[k].x * f; x.y += y[k].y * f; x.z += y[k].z * f; x.w += y[k].w * f;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint2*>(&done[in][c4 * 4]) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  if (GROUPS > 1) {
+    if (group > 0) more_x[group - 1][tid] = x, more_ml[group - 1][tid] = make_float2(top, sum);
+    __syncthreads();
+    if (group == 0) {
+      float m = top;
+#pragma unroll
+      for (int k = 0; k < GROUPS - 1; ++k) m = fmaxf(m, more_ml[k][tid].x);
+      const float old = top == -INFINITY ? 1.f : pa_ex2(top - m);
+      sum *= old;
+      x.x *= old; x.y *= old; x.z *= old; x.w *= old;
+#pragma unroll
+      for (int k = 0; k < GROUPS - 1; ++k) {
+        const float2 ml = more_ml[k][tid];
+        const float4 y = more_x[k][tid];
+        const float f = ml.x == -INFINITY ? 1.f : pa_ex2(ml.x - m);
+        sum += ml.y * f;
+        x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
+      }
+    }
+  }
+  if (group == 0) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(&done[in][c4 * 4]) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  }
   __syncthreads();
   if (threadIdx.x < PJ_ROWS * (D / 8)) {
     const int row = threadIdx.x / (D / 8), col = (threadIdx.x % (D / 8)) * 8;
@@ -381,7 +429,7 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   LP_REQUIRE((long long)d->B * d->T * d->H <= 1LL << 24, "lp_prefix_attention: %d requests of %d tokens and %d heads are too many", d->B, d->T, d->H);
   LP_REQUIRE(d->n_pages > 0 && d->page_size > 0 && d->max_pages > 0, "lp_prefix_attention: %d pages of %d rows, %d a request", d->n_pages, d->page_size, d->max_pages);
   LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 256, "lp_prefix_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
-  LP_REQUIRE(d->B * (long long)d->KVH * ((d->T * (d->H / d->KVH) + PA_ROWS - 1) / PA_ROWS) <= 1 << 24, "lp_prefix_attention: %d requests of %d tokens over %d key heads are too many", d->B, d->T, d->KVH);
+  LP_REQUIRE(d->B * (long long)d->KVH * ((d->T * (d->H / d->KVH) + 7) / 8) <= 1 << 24, "lp_prefix_attention: %d requests of %d tokens over %d key heads are too many", d->B, d->T, d->KVH);
   LP_REQUIRE(d->prefix >= 0 && d->prefix <= (1LL << 31) - 256, "lp_prefix_attention: prefix %d", d->prefix);
   if (d->prefix_k) LP_REQUIRE(!d->page_table && d->prefix_v, "lp_prefix_attention: a prefix of its own goes with a cache of its own each");
   else if (d->page_table) LP_REQUIRE(d->prefix <= (long long)d->max_pages * d->page_size, "lp_prefix_attention: a prefix of %d rows in %d pages of %d", d->prefix, d->max_pages, d->page_size);
@@ -397,14 +445,16 @@ static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
   a.group = d->H / d->KVH;
   const long long own = (long long)d->max_pages * d->page_size - (d->page_table ? d->prefix : 0);
   a.own_rows = (int)own;
-  a.own_blocks = (d->T * a.group + PA_ROWS - 1) / PA_ROWS;
-  const long long items = (long long)d->B * d->KVH * a.own_blocks, tiles = (own + PA_KEYS - 1) / PA_KEYS, room = 4LL * sm_count();
-  long long splits = items >= room ? 1 : room / items;
-  a.own_splits = (int)(splits < tiles ? splits : tiles > 0 ? tiles : 1);
+  a.own_block = d->T * a.group <= 8 ? 8 : 16;
+  a.own_blocks = (d->T * a.group + a.own_block - 1) / a.own_block;
   const long long rows = (long long)d->B * d->T * a.group;
   const bool tc = prefix_tc(d);
+  a.pre_rows = !tc ? (rows <= 8 ? 8 : 16) : rows <= 128 ? 128 : 256;
+  const long long items = (long long)d->B * d->KVH * a.own_blocks, tiles = (own + PA_KEYS - 1) / PA_KEYS, room = ((a.own_block == 16 || (a.pre_rows == 16 && d->prefix > 0)) ? 3LL : 4LL) * sm_count();      // (as many CTAs as run at once)
+  long long splits = items >= room ? 1 : room / items;
+  a.own_splits = (int)(splits < tiles ? splits : tiles > 0 ? tiles : 1);
+  a.own_slots = items * a.own_splits;
   const int keys = tc ? 128 : PA_KEYS;
-  a.pre_rows = !tc ? PA_ROWS : rows <= 128 ? 128 : 256;
   a.pre_tiles = (int)(((long long)d->prefix + keys - 1) / keys);
   a.pre_ctas = 0;
   a.pre_slots = 0;
@@ -414,13 +464,13 @@ static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
       const long long most = pre_items * a.pre_tiles;
       a.pre_ctas = (int)(most < sm_count() ? most : sm_count());
     } else {
-      splits = pre_items >= room ? 1 : room / pre_items;
+      const long long left = a.own_slots < room / 2 ? room - a.own_slots : room / 2;      // (at once with the own rows')
+      splits = pre_items >= left ? 1 : left / pre_items;
       a.pre_ctas = (int)((splits < a.pre_tiles ? splits : a.pre_tiles) * pre_items);
     }
     a.pre_slots = pre_items + a.pre_ctas;
   }
-  a.own_slots = items * a.own_splits;
-  return ((size_t)a.pre_slots * a.pre_rows + (size_t)a.own_slots * PA_ROWS) * (d->D * 4 + 8);
+  return ((size_t)a.pre_slots * a.pre_rows + (size_t)a.own_slots * a.own_block) * (d->D * 4 + 8);
 }
 
 }  // namespace lp
@@ -459,26 +509,38 @@ extern "C" int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* worksp
   LP_REQUIRE(strides_nest(places, 3, d->D), "lp_prefix_attention: rows of out share their memory (strides %lld, %lld, %lld)", d->o_batch, d->o_token, d->o_head);
   LP_REQUIRE(ws_bytes >= need, "lp_prefix_attention: workspace too small");
   a.scale_log2 = d->scale * 1.4426950408889634f;
-  const size_t pre = (size_t)a.pre_slots * a.pre_rows, mine = (size_t)a.own_slots * PA_ROWS;
+  const size_t pre = (size_t)a.pre_slots * a.pre_rows, mine = (size_t)a.own_slots * a.own_block;
   a.pre_o = reinterpret_cast<float*>(workspace);
   a.own_o = a.pre_o + pre * d->D;
   a.pre_ml = reinterpret_cast<float2*>(a.own_o + mine * d->D);
   a.own_ml = a.pre_ml + pre;
-  const bool tc = a.pre_ctas && a.pre_rows != PA_ROWS;
+  const bool tc = a.pre_rows > 16;
   const int pre_ctas = tc ? 0 : a.pre_ctas;
   const long long ctas = pre_ctas + a.own_slots;
   const size_t first = (size_t)(d->B + 1) * 4;
   const dim3 join((unsigned)(((long long)d->B * d->T * a.group + PJ_ROWS - 1) / PJ_ROWS), d->KVH);
   note_launch(tc ? 3 : 2);
-#define LP_PREFIX(DD)                                                                                             \
-  {                                                                                                               \
-    LP_CHECK_CUDA((allow_smem<prefix_rows_kernel<DD>>(pa_smem<DD>(d->B))));                                       \
-    prefix_rows_kernel<DD><<<(unsigned)ctas, 128, pa_smem<DD>(d->B), stream>>>(a, pre_ctas);                      \
-    LP_CHECK_CUDA(cudaGetLastError());                                                                            \
-    if (tc) { if (const int rc = launch_prefix_tc(a, stream)) return rc; }                                        \
-    LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD>, join, dim3(PJ_ROWS * DD / 4), first, stream, 1, true, a));    \
+  const long long pieces = a.pre_ctas ? a.pre_ctas / (a.pre_slots - a.pre_ctas) + a.own_splits : a.own_splits, joins = (long long)join.x * join.y;
+  const int groups = pieces <= PJ_AT_ONCE || joins > 4LL * sm_count() ? 1 : joins > sm_count() ? 2 : 4;
+  const size_t list = ((size_t)d->B + 4) / 4 * 16;
+#define LP_ROWS(DD, PRE, OWN)                                                                                                       \
+  {                                                                                                                                 \
+    const size_t smem = list + pa_smem<DD, (PRE > OWN ? PRE : OWN)>();                                                              \
+    LP_CHECK_CUDA((allow_smem<prefix_rows_kernel<DD, PRE, OWN>>((int)smem)));                                                       \
+    prefix_rows_kernel<DD, PRE, OWN><<<(unsigned)ctas, 128, smem, stream>>>(a, pre_ctas);                                           \
+  }
+#define LP_PREFIX(DD)                                                                                                               \
+  {                                                                                                                                 \
+    if (tc || !pre_ctas) { if (a.own_block == 8) LP_ROWS(DD, 0, 1) else LP_ROWS(DD, 0, 2) }                                         \
+    else if (a.pre_rows == 8) LP_ROWS(DD, 1, 1) else if (a.own_block == 8) LP_ROWS(DD, 2, 1) else LP_ROWS(DD, 2, 2)                 \
+    LP_CHECK_CUDA(cudaGetLastError());                                                                                              \
+    if (tc) { if (const int rc = launch_prefix_tc(a, stream)) return rc; }                                                          \
+    if (groups == 4) LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD, 4>, join, dim3(PJ_ROWS * DD), first, stream, 1, true, a));      \
+    else if (groups == 2) LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD, 2>, join, dim3(PJ_ROWS * DD / 2), first, stream, 1, true, a)); \
+    else LP_CHECK_CUDA(launch_ex(prefix_join_kernel<DD, 1>, join, dim3(PJ_ROWS * DD / 4), first, stream, 1, true, a));              \
   }
   if (d->D == 128) LP_PREFIX(128) else if (d->D == 96) LP_PREFIX(96) else LP_PREFIX(64)
+#undef LP_ROWS
 #undef LP_PREFIX
   return 0;
 }

@@ -12,14 +12,13 @@ namespace lp {
 
 constexpr int PA_MAX_BATCH = 2048;
 constexpr int PA_KEYS = 64;               // keys of a tile of the requests' own rows (and of the prefix, where few rows look at it)
-constexpr int PA_ROWS = 16;               // rows of a block there
 
 struct PrefixArgs {
   lp_prefix_attn_desc d;
   int group;
   float scale_log2;
-  int own_blocks, own_splits, own_rows;   // blocks of a request's rows, pieces of its keys (at most); keys that there may be
-  int pre_rows, pre_tiles, pre_ctas;      // the prefix: rows of a block (PA_ROWS, or the tcgen05 kernel's), tiles of its keys (of PA_KEYS, or 128), CTAs (0: there is none)
+  int own_block, own_blocks, own_splits, own_rows;      // rows of a block (8, 16), blocks of a request's rows, pieces of its keys (at most); keys that there may be
+  int pre_rows, pre_tiles, pre_ctas;      // the prefix: rows of a block (8, 16; 128, 256: the tcgen05 kernel), tiles of its keys (of PA_KEYS, or 128), CTAs (0: there is none)
   long long pre_slots, own_slots;         // partial results' places
   // partial results of the prefix's pieces [item + CTA] and of the own rows' [request][key head][block][piece]: values [D / 4][rows of a block][4], maximum (log2 units) and sum [rows]
   float *pre_o, *own_o;
@@ -81,7 +80,7 @@ __device__ __forceinline__ PrefixLine pa_line(const PrefixArgs& a, int rows) {
   l.own = 0;
   if (l.items > 0 && l.items <= a.pre_ctas) {
     l.own = min(a.pre_ctas / l.items, a.pre_tiles);
-    if (a.pre_rows != PA_ROWS && (a.pre_tiles + l.own - 1) / l.own > (long long)l.items * a.pre_tiles / a.pre_ctas + PA_SLACK) l.own = 0;
+    if (a.pre_rows > 16 && (a.pre_tiles + l.own - 1) / l.own > (long long)l.items * a.pre_tiles / a.pre_ctas + PA_SLACK) l.own = 0;
   }
   return l;
 }
