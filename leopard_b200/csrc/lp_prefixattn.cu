@@ -42,8 +42,9 @@ __device__ __forceinline__ void prefix_rows(const PrefixArgs& a, int cta) {
     const int item = line.own ? cta / line.own : 0;
     if (item >= line.items) return;
     const int piece = cta - item * line.own;                      // (of as many CTAs as items can be, each has at most one)
-    kvh = item / line.blocks;
-    r0 = (item - kvh * line.blocks) * ROWS;
+    const int blk = item / a.d.KVH;
+    kvh = item - blk * a.d.KVH;
+    r0 = blk * ROWS;
     t0 = pa_cut(a.pre_tiles, piece, line.own);
     t1 = pa_cut(a.pre_tiles, piece + 1, line.own);
     past = n_keys = a.d.prefix;
@@ -345,7 +346,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
   long long pre_slot = 0;
   if (a.pre_ctas) {
     const PrefixLine line = pa_line(a, rows);
-    const int blk = r / a.pre_rows, item = kvh * line.blocks + blk;
+    const int blk = r / a.pre_rows, item = pa_item(a, blk, kvh);
     int c0, c1;
     pa_ctas_of(a, line, item, c0, c1);
     pre_in = r - blk * a.pre_rows;

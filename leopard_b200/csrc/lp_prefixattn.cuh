@@ -69,32 +69,52 @@ __device__ __forceinline__ void pa_own(const PrefixArgs& a, int length, int fres
   past = min(own, a.own_rows);
   keys = (int)min((long long)own + fresh, (long long)a.own_rows);
 }
-// The prefix's tiles of all items (key head, block of rows) stand in one line, of which every CTA takes an equal range; or each item has `own` CTAs, where the longest range is then little above an equal
-// share: a range that goes on in another item costs another piece's start and end.  How many rows there are, and so how many items, only the GPU knows.
-struct PrefixLine { int blocks, items, own; };
-constexpr int PA_SLACK = 4;
-__device__ __forceinline__ PrefixLine pa_line(const PrefixArgs& a, int rows) {
-  PrefixLine l;
-  l.blocks = (rows + a.pre_rows - 1) / a.pre_rows;
-  l.items = a.d.KVH * l.blocks;
-  l.own = 0;
-  if (l.items > 0 && l.items <= a.pre_ctas) {
-    l.own = min(a.pre_ctas / l.items, a.pre_tiles);
-    if (a.pre_rows > 16 && (a.pre_tiles + l.own - 1) / l.own > (long long)l.items * a.pre_tiles / a.pre_ctas + PA_SLACK) l.own = 0;
-  }
-  return l;
-}
+// The prefix's tiles of all items (block of rows, key head) stand in one line, of which every CTA takes a range of equal cost; or each item has `own` CTAs, where the longest range is then little above an equal
+// share: a range that goes on in another item costs another piece's start and end.  The last block of each key head comes last in the line; with 128 rows at most (one of the tcgen05 kernel's two
+// streams) its tiles cost PA_HALF of PA_FULL (1.7 and 2.5 us).  How many rows there are, and so how many items, only the GPU knows.
+constexpr int PA_SLACK = 4, PA_FULL = 10, PA_HALF = 7;
+struct PrefixLine {
+  int blocks, items, own, last_cost;      // last_cost: of a tile of the last blocks
+  long long full, cost;                   // tiles of the other blocks; cost of the line
+};
 template <typename T>
 __device__ __forceinline__ T pa_cut(T total, int k, int n) {      // the k-th of n equal ranges begins here
   const T each = total / n, more = total - each * n;
   return each * k + min((T)k, more);
 }
+__device__ __forceinline__ PrefixLine pa_line(const PrefixArgs& a, int rows) {
+  PrefixLine l;
+  l.blocks = (rows + a.pre_rows - 1) / a.pre_rows;
+  l.items = a.d.KVH * l.blocks;
+  l.own = 0;
+  if (a.pre_rows <= 16) {                 // few rows: CTAs of their own
+    if (l.items > 0) l.own = min(a.pre_ctas / l.items, a.pre_tiles);
+    return l;
+  }
+  l.last_cost = a.pre_rows == 256 && rows - (l.blocks - 1) * 256 <= 128 ? PA_HALF : PA_FULL;
+  l.full = (long long)(l.items - a.d.KVH) * a.pre_tiles;
+  l.cost = l.full * PA_FULL + (long long)a.d.KVH * a.pre_tiles * l.last_cost;
+  if (l.items > 0 && l.items <= a.pre_ctas) {
+    l.own = min(a.pre_ctas / l.items, a.pre_tiles);
+    if ((a.pre_tiles + l.own - 1) / l.own * (long long)(l.blocks > 1 ? PA_FULL : l.last_cost) > l.cost / a.pre_ctas + PA_SLACK * PA_FULL) l.own = 0;
+  }
+  return l;
+}
+__device__ __forceinline__ long long pa_begin(const PrefixArgs& a, const PrefixLine& l, int cta) {      // the first tile of a CTA's range of the line
+  const long long c = pa_cut(l.cost, cta, a.pre_ctas), over = c - l.full * PA_FULL;
+  return over <= 0 ? (c + PA_FULL - 1) / PA_FULL : l.full + (over + l.last_cost - 1) / l.last_cost;
+}
+__device__ __forceinline__ int pa_cta_of(const PrefixArgs& a, const PrefixLine& l, long long tile) {      // the CTA in whose range a tile is
+  const long long c = tile <= l.full ? tile * PA_FULL : l.full * PA_FULL + (tile - l.full) * l.last_cost;
+  int cta = (int)min((long long)a.pre_ctas - 1, c * a.pre_ctas / l.cost);
+  while (pa_begin(a, l, cta) > tile) --cta;
+  while (cta + 1 < a.pre_ctas && pa_begin(a, l, cta + 1) <= tile) ++cta;
+  return cta;
+}
 __device__ __forceinline__ void pa_range(const PrefixArgs& a, const PrefixLine& l, int cta, long long& from, long long& to) {
   from = to = 0;
   if (!l.own) {
-    const long long all = (long long)l.items * a.pre_tiles;
-    from = pa_cut(all, cta, a.pre_ctas);
-    to = pa_cut(all, cta + 1, a.pre_ctas);
+    if (l.items) from = pa_begin(a, l, cta), to = pa_begin(a, l, cta + 1);
   } else if (cta < l.items * l.own) {
     const int item = cta / l.own, k = cta - item * l.own;
     from = (long long)item * a.pre_tiles + pa_cut(a.pre_tiles, k, l.own);
@@ -108,20 +128,20 @@ __device__ __forceinline__ void pa_ctas_of(const PrefixArgs& a, const PrefixLine
     c1 = c0 + l.own - 1;
     return;
   }
-  const long long all = (long long)l.items * a.pre_tiles, each = all / a.pre_ctas, more = all - each * a.pre_ctas;      // the first `more` CTAs have one tile more
-  auto cta = [&](long long u) { return (int)(u < (each + 1) * more ? u / (each + 1) : more + (u - (each + 1) * more) / max(each, 1LL)); };
-  c0 = cta((long long)item * a.pre_tiles);
-  c1 = cta((long long)(item + 1) * a.pre_tiles - 1);
+  c0 = pa_cta_of(a, l, (long long)item * a.pre_tiles);
+  c1 = pa_cta_of(a, l, (long long)(item + 1) * a.pre_tiles - 1);
 }
 // a CTA's piece of an item
 struct PrefixPiece { int item, kvh, r0, t0, n; };
-__device__ __forceinline__ PrefixPiece pa_piece(const PrefixArgs& a, const PrefixLine& l, long long u, long long u_end) {
+__device__ __forceinline__ int pa_item(const PrefixArgs& a, int blk, int kvh) { return blk * a.d.KVH + kvh; }
+__device__ __forceinline__ PrefixPiece pa_piece(const PrefixArgs& a, long long u, long long u_end) {
   PrefixPiece p;
   p.item = (int)(u / a.pre_tiles);
   p.t0 = (int)(u - (long long)p.item * a.pre_tiles);
   p.n = (int)min((long long)(a.pre_tiles - p.t0), u_end - u);
-  p.kvh = p.item / l.blocks;
-  p.r0 = (p.item - p.kvh * l.blocks) * a.pre_rows;
+  const int blk = p.item / a.d.KVH;
+  p.kvh = p.item - blk * a.d.KVH;
+  p.r0 = blk * a.pre_rows;
   return p;
 }
 __device__ __forceinline__ int pa_own_pieces(const PrefixArgs& a, int keys) { return min(a.own_splits, (keys + PA_KEYS - 1) / PA_KEYS); }

@@ -136,7 +136,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     const int boxes = PT_KEYS / tc.box;
     int g = 0;
     for (long long u = u_begin; u < u_end;) {
-      const PrefixPiece p = pa_piece(a, line, u, u_end);
+      const PrefixPiece p = pa_piece(a, u, u_end);
       u += p.n;
       int key = lane < boxes ? p.t0 * PT_KEYS + lane * tc.box : 0;      // this lane's box of the tile
       PrefixPlace at(a, key);
@@ -178,7 +178,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     constexpr int STEP = SPLIT ? 2 : 1;
     int g = 0, nt = 0, pieces = 0;      // tiles of the CTA so far; tiles of this stream; pieces whose queries it has waited for
     for (long long u = u_begin; u < u_end;) {
-      const PrefixPiece p = pa_piece(a, line, u, u_end);
+      const PrefixPiece p = pa_piece(a, u, u_end);
       u += p.n;
       const int j0 = SPLIT ? q : 0;
       if (SPLIT && j0 >= p.n) {         // one tile: the other stream's, with nothing to wait for here (a wait that the other stream does not wait for in turn may miss its phase)
@@ -255,7 +255,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     constexpr int STEP = SPLIT ? 2 : 1;
     int g = 0, nt = 0, pieces = 0, joins = 0;      // tiles of the CTA and of this stream so far; pieces that it had tiles of; SPLIT: pieces of both streams
     for (long long u = u_begin; u < u_end;) {
-      const PrefixPiece p = pa_piece(a, line, u, u_end);
+      const PrefixPiece p = pa_piece(a, u, u_end);
       u += p.n;
       const int row_base = p.r0 + (SPLIT ? 0 : q * 128), j0 = SPLIT ? q : 0;
       if (SPLIT ? j0 >= p.n : row_base >= rows) { g += p.n; continue; }
