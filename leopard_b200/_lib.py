@@ -400,7 +400,7 @@ STREAM32_SYMBOLS = ("lp_last_error", "lp_abi_version", "lp_launch_count", "lp_li
 STREAM32_OPTIONAL = ("lp_gemm_bf16", "lp_split_rows", "lp_gemm_split", "lp_latent_expanded_workspace_bytes", "lp_latent_attend_expanded",
                      "lp_latent_route", "lp_window_prompt_count", "lp_gather_rows",
                      "lp_window_prompt_workspace_bytes", "lp_window_attn_prompt", "lp_gemm_grouped", "lp_linear_split", "lp_gemm_linear",
-                     "lp_cache_compact", "lp_cache_copy_pages")      # present in the native libraries, absent from the CPU-emulated build
+                     "lp_cache_compact", "lp_cache_copy_pages", "lp_sample_tokens")      # present in the native libraries, absent from the CPU-emulated build
 _stream32 = None
 
 

@@ -35,7 +35,7 @@ def cmd_generate(args) -> int:
     eng = _load(args)
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in args.prompt]
     outs = generate(eng, prompts, max_new_tokens=args.max_new_tokens, eos=set(args.eos or ()),
-                    sampling=SamplingParams(temperature=args.temperature, top_k=args.top_k, seed=args.seed))
+                    sampling=SamplingParams(temperature=args.temperature, top_k=args.top_k, seed=args.seed, top_p=args.top_p, min_p=args.min_p))
     for p, o in zip(prompts, outs):
         print(json.dumps({"prompt": p, "output": o}))
     return 0
@@ -82,6 +82,8 @@ def main(argv: Optional[List[str]] = None) -> int:
             p.add_argument("--eos", type=int, action="append")
             p.add_argument("--temperature", type=float, default=0.0)
             p.add_argument("--top-k", type=int, default=0)
+            p.add_argument("--top-p", type=float, default=1.0)
+            p.add_argument("--min-p", type=float, default=0.0)
             p.add_argument("--seed", type=int)
         else:
             p.add_argument("--out", required=True)

@@ -15,7 +15,7 @@
 namespace lp {
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2 * SA_THREADS, SA_LIST = 256, SA_MAX_CTAS = 8;
-constexpr int SA_MAX_SLICE = 47 * 1024;      // words that a CTA can hold
+constexpr int SA_MAX_SLICE = 46 * 1024;      // words that a CTA can hold
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -307,7 +307,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     const u64 power_bits = a.slice <= 16384 ? AT_2_17 : AT_2_20;
     auto mass = [&](float x) { return sa_weight_bits(((double)x - top) * unit, power, s.root) - power_bits; };
     // ranges of equal width below the largest logit, as far as weights reach (30 t) or a top_k may look
-    const float reach = fminf(fmaxf(30.f * t, 24.f), hi - lo), fine = reach > 0.f ? (float)(SA_BINS - 1) / reach : 0.f;
+    const float reach = fminf(fmaxf(30.f * t, 24.f), hi - lo), fine = reach > 1e-30f ? (float)(SA_BINS - 1) / reach : 0.f;
     auto bin_of = [&](float x) { return __float_as_int(fminf(__fmaf_rn(hi - x, fine, 12582912.f), 12582912.f + (SA_BINS - 1))) - 0x4b400000; };      // (1.5 2^23: the whole number is in the low bits)
     int hists = 0;
     // The last word before which fewer than `limit` words lie (MASS: less than top_p of the mass): last_key and last_at.  True: the word has been drawn.

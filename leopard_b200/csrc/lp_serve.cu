@@ -297,6 +297,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     items[s] = s < a.segs ? a.seg[s].heads * (a.seg[s].turned ? turned + (a.copy || a.seg[s].paged ? plain : 0) : whole) : 0;
     all += items[s];
   }
+  if (all == 0) return;
   auto place = [&](int i) {
     Place p;
     const int s = i < items[0] ? 0 : i < items[0] + items[1] ? 1 : 2;

@@ -826,36 +826,40 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     before (it grows; when the list is over, entries stay negative); rows: how many rows the step has room for.
     -> (row_seq int32 [rows], row_pos int32 [rows], slots int64 [rows] = page * page_size + row of the page; row0 int32 [B + 1], each request's first row).  Rows that no request has are -1 in all
     three, rows without a page in slots."""
-    B = lengths.shape[0] if isinstance(lengths, torch.Tensor) and lengths.dim() == 1 else -1
-    dev = getattr(lengths, "device", None)
     try:
-        max_pages = page_table.shape[1]
-        fine = (lengths.is_cuda and all(t.dtype is _I32 and t.device == dev for t in (lengths, new, page_table, free, used)) and B >= 0 and lengths.is_contiguous() and new.shape == (B,)
-                and new.is_contiguous() and page_table.shape == (B, max_pages) and (page_table.stride(1) == 1 or max_pages <= 1) and (page_table.stride(0) >= max_pages or B <= 1)
-                and free.dim() == 1 and free.is_contiguous() and used.shape == (1,))
-    except (AttributeError, IndexError):
+        (B,), dev, max_pages = lengths.shape, lengths.device, page_table.shape[1]
+        fine = (lengths.is_cuda and lengths.dtype is _I32 and new.dtype is _I32 and page_table.dtype is _I32 and free.dtype is _I32 and used.dtype is _I32 and new.device == dev
+                and page_table.device == dev and free.device == dev and used.device == dev and new.shape == (B,) and lengths.is_contiguous() and new.is_contiguous()
+                and page_table.shape == (B, max_pages) and (page_table.stride(1) == 1 or max_pages <= 1) and (page_table.stride(0) >= max_pages or B <= 1) and free.dim() == 1 and free.is_contiguous()
+                and used.shape == (1,))
+    except (AttributeError, ValueError, IndexError):
         fine = False
     if not fine:
-        for t, n in ((lengths, "lengths"), (new, "new"), (used, "used"), (free, "free")):
-            _need(t, n, (_I32,), 1, None if n in ("free", "lengths") else (1,) if n == "used" else lengths.shape, lengths.device if n != "lengths" else None, contiguous=True)
-        _need(page_table, "page_table", (_I32,), 2, (B, page_table.shape[-1]), lengths.device, rows=True)
-    for t, n in ((lengths, "lengths"), (new, "new"), (free, "free"), (used, "used")):
-        if _overlaps(page_table, t) or (t is not used and _overlaps(used, t)):
-            raise ValueError(f"{n} must not share memory with what the call changes")
-    rows = int(rows)
+        _need(lengths, "lengths", (_I32,), 1, contiguous=True)
+        for t, n, shape in ((new, "new", lengths.shape), (used, "used", (1,)), (free, "free", None)):
+            _need(t, n, (_I32,), 1, shape, lengths.device, contiguous=True)
+        _need(page_table, "page_table", (_I32,), 2, (lengths.shape[0], page_table.shape[-1]), lengths.device, rows=True)
+        raise ValueError("step_tables: the tables must be contiguous in their rows")
+    rows, n_free, ld = int(rows), free.shape[0], page_table.stride(0)
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
-    ld = -(-rows // 4) * 4
-    both = torch.empty((2, ld), dtype=_I32, device=dev)[:, :rows]
+    p_table, p_used, p_free, p_len, p_new = page_table.data_ptr(), used.data_ptr(), free.data_ptr(), lengths.data_ptr(), new.data_ptr()
+    end = p_table + 4 * ((B - 1) * ld + max_pages)
+    for p, n, name in ((p_used, 1, "used"), (p_free, n_free, "free"), (p_len, B, "lengths"), (p_new, B, "new")):
+        if (p < end and p + 4 * n > p_table) or (p != p_used and p < p_used + 4 and p + 4 * n > p_used) or (p == p_used and name != "used" and n):
+            raise ValueError(f"{name} must not share memory with what the call changes")
+    padded = (rows + 3) & -4
+    seq, pos = torch.empty((2, padded), dtype=_I32, device=dev).unbind(0)
+    if padded != rows:
+        seq, pos = seq[:rows], pos[:rows]
     slots = torch.empty((rows,), dtype=_I64, device=dev)
     if B == 0:
-        return both[0].fill_(-1), both[1].fill_(-1), slots.fill_(-1), torch.zeros((1,), dtype=_I32, device=dev)
+        return seq.fill_(-1), pos.fill_(-1), slots.fill_(-1), torch.zeros((1,), dtype=_I32, device=dev)
     row0 = torch.empty((B + 1,), dtype=_I32, device=dev)
     L = _lib.lib()
-    at = both.data_ptr()
-    _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), page_table.stride(0), max_pages, int(page_size), free.data_ptr(), free.numel(),
-          used.data_ptr(), B, rows, at, at + 4 * ld, slots.data_ptr(), row0.data_ptr())
-    return both[0], both[1], slots, row0
+    _call(dev, L, "lp_step_tables", L.lp_step_tables, p_len, p_new, p_table, ld, max_pages, int(page_size), p_free, n_free, p_used, B, rows, seq.data_ptr(), pos.data_ptr(), slots.data_ptr(),
+          row0.data_ptr())
+    return seq, pos, slots, row0
 
 
 def _apart(a, b):
@@ -874,6 +878,17 @@ def _apart(a, b):
         q, r = divmod(delta, s)
         return (-n < q < m and meet(r, inner)) or (-n < q + 1 < m and meet(r - s, inner))
     return not meet((b.data_ptr() - a.data_ptr()) // a.element_size(), dims)
+
+
+def _shares(a, b):
+    """whether two tensors may share an element: their spans of memory meet, and they are not told apart"""
+    p, q = a.data_ptr(), b.data_ptr()
+    if p <= q:
+        if p + (sum((s - 1) * st for s, st in zip(a.shape, a.stride())) + 1) * a.element_size() <= q:
+            return False
+    elif q + (sum((s - 1) * st for s, st in zip(b.shape, b.stride())) + 1) * b.element_size() <= p:
+        return False
+    return a.numel() > 0 and b.numel() > 0 and not _apart(a, b)
 
 
 def _rotary_check(x, name, dtypes, dim, device=None):
@@ -899,26 +914,38 @@ def rotary(x, positions, inv_freq, layout="half", scale=1.0, inverse=False, out=
     """Rotary positions (lp_rotary): x bf16 or fp32 [rows, heads, D]; positions int32 or int64 [rows]; inv_freq fp32 [n] (seqlm.rotary_table has the scaled ones and their `scale`): the first
     2 n dimensions of each head are turned, pairs (i, i + n) for layout "half" and (2 i, 2 i + 1) for "interleaved", and multiplied by `scale`.  inverse: turned back, which takes the gradient of the result to
     that of x.  Angles are formed in 64 bits from the position.  out: x itself, or memory apart from it.  -> out."""
+    try:
+        rows, heads, D = x.shape
+        dev, kind, n = x.device, x.dtype, inv_freq.shape[0]
+        xs = x.stride()
+        fine = (x.is_cuda and (kind is _BF16 or kind is _F32) and (xs[2] == 1 or D <= 1) and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,)
+                and positions.is_contiguous() and positions.device == dev and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D
+                and out is None)
+    except (AttributeError, ValueError, IndexError):
+        fine = False
     inter = _rotary_layout(layout)
-    _rotary_check(x, "x", (_BF16, _F32), 3)
-    rows, heads, D = x.shape
-    dev = x.device
-    _rotary_rows(positions, inv_freq, rows, D, dev)
+    if not fine:
+        _rotary_check(x, "x", (_BF16, _F32), 3)
+        rows, heads, D = x.shape
+        dev, kind, xs = x.device, x.dtype, x.stride()
+        _rotary_rows(positions, inv_freq, rows, D, dev)
+        n = inv_freq.numel()
+        if out is not None:
+            _rotary_check(out, "out", (kind,), 3, dev)
+            if out.shape != x.shape:
+                raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+            if _shares(out, x) and (out.data_ptr() != x.data_ptr() or out.stride() != xs):
+                raise ValueError("out must be x itself or share no memory with it")
+            if _overlaps(out, positions) or _overlaps(out, inv_freq):
+                raise ValueError("out must not share memory with positions or inv_freq")
     if out is None:
-        out = torch.empty((rows, heads, D), dtype=x.dtype, device=dev)
-    else:
-        _rotary_check(out, "out", (x.dtype,), 3, dev)
-        if out.shape != x.shape:
-            raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
-        if _overlaps(out, x) and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()):
-            raise ValueError("out must be x itself or share no memory with it")
-        if _overlaps(out, positions) or _overlaps(out, inv_freq):
-            raise ValueError("out must not share memory with positions or inv_freq")
-    if x.numel() == 0:
+        out = torch.empty((rows, heads, D), dtype=kind, device=dev)
+    if rows == 0 or heads == 0 or D == 0:
         return out
+    ys = out.stride()
     L = _lib.lib()
-    _call(dev, L, "lp_rotary", L.lp_rotary, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), 1 if x.dtype is _F32 else 0, rows, heads, D,
-          positions.data_ptr(), 1 if positions.dtype is _I64 else 0, inv_freq.data_ptr(), inv_freq.numel(), int(inter), float(scale), int(bool(inverse)))
+    _call(dev, L, "lp_rotary", L.lp_rotary, x.data_ptr(), xs[0], xs[1], out.data_ptr(), ys[0], ys[1], 1 if kind is _F32 else 0, rows, heads, D, positions.data_ptr(),
+          1 if positions.dtype is _I64 else 0, inv_freq.data_ptr(), n, int(inter), float(scale), int(bool(inverse)))
     return out
 
 
@@ -926,38 +953,48 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
     """A step's queries and keys turned as by `rotary`, keys and values written to their cache rows in the same pass (lp_rotary_append): q [rows, H, D], k, v [rows, KVH, D] bf16 or fp32 (views of
     one product, say); k_pool, v_pool of the same type [pages, page_size, KVH, D]; slots int64 [rows] (step_tables): page * page_size + row of the page, rows whose slot is no row of the pool are
     left out; no slot comes twice.  -> q_out (q itself, if given so)."""
+    try:
+        rows, H, D = q.shape
+        dev, kind, n, G = q.device, q.dtype, inv_freq.shape[0], k.shape[1]
+        s, ks, vs, kp, vp = q.stride(), k.stride(), v.stride(), k_pool.stride(), v_pool.stride()
+        fine = (q.is_cuda and (kind is _BF16 or kind is _F32) and k.dtype is kind and v.dtype is kind and k_pool.dtype is kind and v_pool.dtype is kind and s[2] == ks[2] == vs[2] == kp[3] == vp[3] == 1
+                and k.shape == (rows, G, D) and v.shape == (rows, G, D) and k_pool.shape[2:] == (G, D) and v_pool.shape == k_pool.shape and k.device == dev and v.device == dev and k_pool.device == dev
+                and v_pool.device == dev and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,) and positions.is_contiguous() and positions.device == dev
+                and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D and slots.dtype is _I64 and slots.shape == (rows,)
+                and slots.is_contiguous() and slots.device == dev and q_out is None)
+    except (AttributeError, ValueError, IndexError):
+        fine = False
     inter = _rotary_layout(layout)
-    _rotary_check(q, "q", (_BF16, _F32), 3)
-    rows, H, D = q.shape
-    dev = q.device
-    for t, n, dim in ((k, "k", 3), (v, "v", 3), (k_pool, "k_pool", 4), (v_pool, "v_pool", 4)):
-        _rotary_check(t, n, (q.dtype,), dim, dev)
-    G = k.shape[1]
-    if k.shape != (rows, G, D) or v.shape != k.shape or k_pool.shape[2:] != (G, D) or v_pool.shape != k_pool.shape:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, k_pool {tuple(k_pool.shape)} and v_pool {tuple(v_pool.shape)} do not fit together")
-    _rotary_rows(positions, inv_freq, rows, D, dev)
-    _need(slots, "slots", (_I64,), 1, (rows,), dev, contiguous=True)
-    if q_out is None:
-        q_out = torch.empty((rows, H, D), dtype=q.dtype, device=dev)
-    else:
-        _rotary_check(q_out, "q_out", (q.dtype,), 3, dev)
-        if q_out.shape != q.shape:
-            raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-        if _overlaps(q_out, q) and (q_out.data_ptr() != q.data_ptr() or q_out.stride() != q.stride()):
-            raise ValueError("q_out must be q itself or share no memory with it")
-    written = (k_pool, v_pool, q_out)
-    for i, w in enumerate(written):
-        for t in (q, k, v, positions, inv_freq, slots) + written[:i]:
-            if t is q and w is q_out and q_out.data_ptr() == q.data_ptr():
-                continue
-            if _overlaps(w, t) and not _apart(w, t):
+    if not fine:
+        _rotary_check(q, "q", (_BF16, _F32), 3)
+        rows, H, D = q.shape
+        dev, kind = q.device, q.dtype
+        for t, name, dim in ((k, "k", 3), (v, "v", 3), (k_pool, "k_pool", 4), (v_pool, "v_pool", 4)):
+            _rotary_check(t, name, (kind,), dim, dev)
+        G = k.shape[1]
+        if k.shape != (rows, G, D) or v.shape != k.shape or k_pool.shape[2:] != (G, D) or v_pool.shape != k_pool.shape:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, k_pool {tuple(k_pool.shape)} and v_pool {tuple(v_pool.shape)} do not fit together")
+        _rotary_rows(positions, inv_freq, rows, D, dev)
+        _need(slots, "slots", (_I64,), 1, (rows,), dev, contiguous=True)
+        n, s, ks, vs, kp, vp = inv_freq.numel(), q.stride(), k.stride(), v.stride(), k_pool.stride(), v_pool.stride()
+        if q_out is not None:
+            _rotary_check(q_out, "q_out", (kind,), 3, dev)
+            if q_out.shape != q.shape:
+                raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+            if _shares(q_out, q) and (q_out.data_ptr() != q.data_ptr() or q_out.stride() != s):
+                raise ValueError("q_out must be q itself or share no memory with it")
+            if any(_shares(q_out, t) for t in (k, v, k_pool, v_pool, positions, inv_freq, slots)):
                 raise ValueError("k_pool, v_pool and q_out must share no memory with one another nor with what the call reads")
+    if any(_shares(p, t) for p in (k_pool, v_pool) for t in (q, k, v, positions, inv_freq, slots)) or _shares(k_pool, v_pool):
+        raise ValueError("k_pool, v_pool and q_out must share no memory with one another nor with what the call reads")
+    if q_out is None:
+        q_out = torch.empty((rows, H, D), dtype=kind, device=dev)
     if rows == 0 or D == 0 or k_pool.numel() == 0:
         return q_out
-    s, o, ks, vs, kp, vp = q.stride(), q_out.stride(), k.stride(), v.stride(), k_pool.stride(), v_pool.stride()
+    o = q_out.stride()
     d = _lib.RotaryAppendDesc(q.data_ptr(), s[0], s[1], q_out.data_ptr(), o[0], o[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], k_pool.data_ptr(), kp[0], kp[1], kp[2],
-                              v_pool.data_ptr(), vp[0], vp[1], vp[2], positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), 1 if positions.dtype is _I64 else 0, inv_freq.numel(),
-                              int(inter), 1 if q.dtype is _F32 else 0, rows, H, G, D, k_pool.shape[0], k_pool.shape[1], float(scale))
+                              v_pool.data_ptr(), vp[0], vp[1], vp[2], positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), 1 if positions.dtype is _I64 else 0, n,
+                              int(inter), 1 if kind is _F32 else 0, rows, H, G, D, k_pool.shape[0], k_pool.shape[1], float(scale))
     L = _lib.lib()
     _call(dev, L, "lp_rotary_append", L.lp_rotary_append, C.byref(d))
     return q_out
@@ -1027,7 +1064,7 @@ def prefix_attention(q, k, v, lengths, prefix, new=None, page_table=None, prefix
         _prefix_refusals(q, k, v, lengths, prefix, new, page_table, prefix_k, prefix_v, out)
     if out is None:
         out = torch.empty((B, T, H, D), dtype=_BF16, device=dev)
-    elif any(t is not None and _overlaps(out, t) for t in (q, k, v, prefix_k, prefix_v, lengths, new, page_table)):
+    elif any(t is not None and _shares(out, t) for t in (q, k, v, prefix_k, prefix_v, lengths, new, page_table)):
         raise ValueError("out must not share memory with the inputs")
     if B == 0 or T == 0:
         return out
@@ -1056,13 +1093,20 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     """The next token of each row from given random numbers (lp_sample_tokens): logits fp32 or bf16 [rows, V]; uniform fp32 [rows] in [0, 1).  temperature, top_p, min_p (numbers or fp32 [rows]) and
     top_k (a number or int32 [rows]): of the words in the order of their logits, equal ones by index, the first top_k are kept (0: all), of them those before which less than top_p of their mass
     lies, of them those at least min_p times as likely as the likeliest; drawn is the first kept word, by index, up to which more than `uniform` of the kept mass lies.  temperature 0 takes the largest
-    logit, the first of equal ones.  -> int64 [rows]; -1 for a row of -inf and NaN alone, which are never drawn.  V <= 385024."""
-    _need(logits, "logits", (_F32, _BF16), 2, rows=True)
-    R, V = logits.shape
-    dev = logits.device
-    _need(uniform, "uniform", (_F32,), 1, (R,), dev, contiguous=True)
+    logit, the first of equal ones.  -> int64 [rows]; -1 for a row of -inf and NaN alone, which are never drawn.  V <= 376832."""
+    try:
+        R, V = logits.shape
+        dev, kind, ld = logits.device, logits.dtype, logits.stride(0)
+        fine = (logits.is_cuda and (kind is _F32 or kind is _BF16) and (logits.stride(1) == 1 or V <= 1) and (R <= 1 or ld >= V) and uniform.dtype is _F32 and uniform.shape == (R,)
+                and uniform.is_contiguous() and uniform.device == dev)
+    except (AttributeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _need(logits, "logits", (_F32, _BF16), 2, rows=True)
+        _need(uniform, "uniform", (_F32,), 1, logits.shape[:1], logits.device, contiguous=True)
+        raise ValueError("sample_tokens: rows must be contiguous")
     settings = [*_setting(temperature, "temperature", _F32, R, dev), *_setting(top_k, "top_k", _I32, R, dev), *_setting(top_p, "top_p", _F32, R, dev), *_setting(min_p, "min_p", _F32, R, dev)]
     out = torch.empty((R,), dtype=_I64, device=dev)
-    L = _lib.lib()
-    _call(dev, L, "lp_sample_tokens", L.lp_sample_tokens, logits.data_ptr(), 1 if logits.dtype is _F32 else 0, max(logits.stride(0), V), uniform.data_ptr(), *settings, R, V, out.data_ptr())
+    L = _lib.stream32_lib()
+    _call(dev, L, "lp_sample_tokens", L.lp_sample_tokens, logits.data_ptr(), 1 if kind is _F32 else 0, max(ld, V), uniform.data_ptr(), *settings, R, V, out.data_ptr())
     return out

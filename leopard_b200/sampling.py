@@ -1,5 +1,6 @@
 """Token selection from a step's logits.  Greedy arg-max is what the reference's evaluation uses (generate(..., do_sample=False),
-evaluations/models/llava_multiimg_siglip_anyres.py:448-452); temperature / top-k sampling is offered for the language models.
+evaluations/models/llava_multiimg_siglip_anyres.py:448-452); temperature / top-k sampling is offered for the language models,
+with top-p and min-p by the native draw (ops.sample_tokens).
 Selection runs on the device; only the chosen ids come back to the host (the stopping criterion needs them)."""
 from __future__ import annotations
 
@@ -8,12 +9,16 @@ from typing import Optional
 
 import torch
 
+from . import ops
+
 
 @dataclass
 class SamplingParams:
     temperature: float = 0.0       # 0: greedy
     top_k: int = 0                 # 0: the whole vocabulary
     seed: Optional[int] = None
+    top_p: float = 1.0             # the likeliest words, before which less than this share of the mass lies (1: all)
+    min_p: float = 0.0             # words at least this many times as likely as the likeliest (0: all)
 
 
 class Sampler:
@@ -30,6 +35,8 @@ class Sampler:
             self._gen = torch.Generator(device=logits.device)
             if p.seed is not None:
                 self._gen.manual_seed(p.seed)
+        if p.top_p < 1.0 or p.min_p > 0.0:
+            return ops.sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device, generator=self._gen), p.temperature, max(p.top_k, 0), p.top_p, p.min_p)
         z = logits / p.temperature
         if p.top_k > 0 and p.top_k < z.shape[-1]:
             kth = z.topk(p.top_k, -1).values[:, -1:]
