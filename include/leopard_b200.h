@@ -1087,7 +1087,7 @@ typedef struct lp_prefix_attn_desc {
 size_t lp_prefix_attention_workspace_bytes(const lp_prefix_attn_desc* desc);
 int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* workspace, size_t ws_bytes, void* stream);
 
-/* The next token of each row of logits (fp32 or bf16 [rows][ld], V <= 385024 words), by uniform[row] in [0, 1).  With w = exp((z - max z) / temperature) and the words in the order of their logits, the
+/* The next token of each row of logits (fp32 or bf16 [rows][ld], V <= 376832 words), by uniform[row] in [0, 1).  With w = exp((z - max z) / temperature) and the words in the order of their logits, the
  * largest first, equal ones by index: the first top_k are kept (0: all); of them those before which less than top_p of their mass lies, the first in any case; of them those with
  * w >= min_p; out[row] is the first kept word, by index, up to which more than uniform of the kept mass lies.  temperature 0 (negative, NaN): the largest, the first of equal ones.
  * Weights are held in units of 2^-43 of the largest.  Settings of each row, or (NULL) one for all.  -inf and NaN are never drawn; of a row with +inf entries only these are; a row with nothing

@@ -53,6 +53,54 @@ inline bool strides_nest(Dim* dims, int n, long long inner) {
   return true;
 }
 
+// Where a tensor lies: `n` dimensions (strides in elements of `elem` bytes).  spans_meet: whether two may share an element.  Those whose spans of memory meet share none where both have the same strides, each past
+// what lies within it, and their places differ all the same: the parts of one product or of one pool.
+struct Span {
+  const void* p; int elem, n;
+  Dim d[4];
+};
+inline bool spans_meet_from(__int128 delta, const Dim* a, const Dim* b, int n) {      // elements i of a and j of b, `delta` behind: sum (i - j) stride = delta
+  if (n == 0) return delta == 0;
+  const long long s = a[0].stride;
+  __int128 reach = 0;
+  for (int k = 1; k < n; ++k) reach += (__int128)a[k].stride * ((a[k].size > b[k].size ? a[k].size : b[k].size) - 1);
+  if (s <= reach) return true;            // not nested: not known
+  __int128 q = delta / s, r = delta - q * s;
+  if (r < 0) --q, r += s;
+  return (q > -b[0].size && q < a[0].size && spans_meet_from(r, a + 1, b + 1, n - 1)) || (q + 1 > -b[0].size && q + 1 < a[0].size && spans_meet_from(r - s, a + 1, b + 1, n - 1));
+}
+inline bool spans_meet(const Span& a, const Span& b) {
+  __int128 lo[2], hi[2];
+  const Span* both[2] = {&a, &b};
+  for (int i = 0; i < 2; ++i) {
+    lo[i] = hi[i] = 0;
+    for (int k = 0; k < both[i]->n; ++k) {
+      if (both[i]->d[k].size <= 0) return false;
+      const __int128 x = (__int128)both[i]->d[k].stride * (both[i]->d[k].size - 1);
+      (x < 0 ? lo : hi)[i] += x;
+    }
+    lo[i] = lo[i] * both[i]->elem + (__int128)reinterpret_cast<uintptr_t>(both[i]->p);
+    hi[i] = (hi[i] + 1) * both[i]->elem + (__int128)reinterpret_cast<uintptr_t>(both[i]->p);
+  }
+  if (hi[0] <= lo[1] || hi[1] <= lo[0]) return false;
+  if (a.elem != b.elem || a.n != b.n) return true;
+  Dim x[4], y[4];
+  int n = 0;
+  for (int k = 0; k < a.n; ++k) {
+    Dim p = a.d[k], q = b.d[k];
+    if (p.size == 1 && q.size == 1) continue;
+    if (p.size == 1) p.stride = q.stride;
+    if (q.size == 1) q.stride = p.stride;
+    if (p.stride != q.stride || p.stride <= 0) return true;
+    int at = n++;
+    for (; at > 0 && x[at - 1].stride < p.stride; --at) x[at] = x[at - 1], y[at] = y[at - 1];
+    x[at] = p;
+    y[at] = q;
+  }
+  const long long bytes = (long long)(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+  return bytes % a.elem != 0 || spans_meet_from(bytes / a.elem, x, y, n);
+}
+
 #ifdef __CUDACC__
 // two fp32 multiply-adds (products) in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {

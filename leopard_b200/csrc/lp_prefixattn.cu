@@ -508,6 +508,12 @@ extern "C" int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* worksp
   LP_REQUIRE(strides % 8 == 0 && bases % 16 == 0, "lp_prefix_attention: strides in multiples of 8 elements, 16-byte aligned bases");
   Dim places[3] = {{d->B, d->o_batch}, {d->T, d->o_token}, {d->H, d->o_head}};
   LP_REQUIRE(strides_nest(places, 3, d->D), "lp_prefix_attention: rows of out share their memory (strides %lld, %lld, %lld)", d->o_batch, d->o_token, d->o_head);
+  const Span out = {d->out, 2, 4, {{d->B, d->o_batch}, {d->T, d->o_token}, {d->H, d->o_head}, {d->D, 1}}};
+  const Span reads[8] = {{d->q, 2, 4, {{d->B, d->q_batch}, {d->T, d->q_token}, {d->H, d->q_head}, {d->D, 1}}}, {d->k, 2, 4, {{d->n_pages, d->k_page}, {d->page_size, d->k_row}, {d->KVH, d->k_head}, {d->D, 1}}},
+                         {d->v, 2, 4, {{d->n_pages, d->v_page}, {d->page_size, d->v_row}, {d->KVH, d->v_head}, {d->D, 1}}}, {d->prefix_k, 2, 3, {{d->prefix, d->pk_row}, {d->KVH, d->pk_head}, {d->D, 1}}},
+                         {d->prefix_v, 2, 3, {{d->prefix, d->pv_row}, {d->KVH, d->pv_head}, {d->D, 1}}}, {d->page_table, 4, 2, {{d->B, d->ld_table}, {d->max_pages, 1}}}, {d->lengths, 4, 1, {{d->B, 1}}},
+                         {d->fresh, 4, 1, {{d->B, 1}}}};
+  for (const Span& r : reads) LP_REQUIRE(!r.p || !spans_meet(out, r), "lp_prefix_attention: out must share no memory with the inputs");
   LP_REQUIRE(ws_bytes >= need, "lp_prefix_attention: workspace too small");
   a.scale_log2 = d->scale * 1.4426950408889634f;
   const size_t pre = (size_t)a.pre_slots * a.pre_rows, mine = (size_t)a.own_slots * a.own_block;

@@ -435,6 +435,10 @@ extern "C" int lp_step_tables(const int* lengths, const int* fresh, int* page_ta
   LP_REQUIRE(page_size > 0 && max_pages > 0 && (B == 1 || ld_table >= max_pages), "lp_step_tables: %d pages of %d rows, ld_table %lld", max_pages, page_size, ld_table);
   LP_REQUIRE((long long)max_pages * page_size <= 1LL << 31, "lp_step_tables: %d pages of %d rows are too many", max_pages, page_size);
   LP_REQUIRE(rows >= 0 && rows <= 1 << 30 && n_free >= 0, "lp_step_tables: rows=%d, %d free pages", rows, n_free);
+  const Span table = {page_table, 4, 2, {{B, ld_table}, {max_pages, 1}}}, count = {used, 4, 1, {{1, 1}}};
+  const Span reads[3] = {{lengths, 4, 1, {{B, 1}}}, {fresh, 4, 1, {{B, 1}}}, {free_pages, 4, 1, {{n_free, 1}}}};
+  LP_REQUIRE(!spans_meet(table, count), "lp_step_tables: page_table and used share their memory");
+  for (const Span& r : reads) LP_REQUIRE(!spans_meet(table, r) && !spans_meet(count, r), "lp_step_tables: page_table and used must share no memory with what the call reads");
   // one CTA while a thread has a row or two, then eight; above 16,384 rows they are a kernel of their own
   const bool one = rows <= 2048 && B <= 1024, small = rows <= 512 && B <= 256;
   const int ctas = one ? 1 : 8, each = (B + ctas - 1) / ctas;
@@ -467,6 +471,11 @@ extern "C" int lp_rotary(const void* x, long long x_row, long long x_head, void*
   Dim places[2] = {{rows, y_row}, {heads, y_head}};
   LP_REQUIRE(strides_nest(places, 2, D), "lp_rotary: rows of the output share their memory (strides %lld, %lld)", y_row, y_head);
   if (rows == 0) return 0;
+  const int elem = fp32 ? 4 : 2;
+  const Span in = {x, elem, 3, {{rows, x_row}, {heads, x_head}, {D, 1}}}, out = {y, elem, 3, {{rows, y_row}, {heads, y_head}, {D, 1}}};
+  const Span at = {positions, positions_64 ? 8 : 4, 1, {{rows, 1}}}, freq = {inv_freq, 4, 1, {{n_freq, 1}}};
+  LP_REQUIRE((x == y && (rows == 1 || x_row == y_row) && (heads == 1 || x_head == y_head)) || !spans_meet(in, out), "lp_rotary: the output must be the input or share no memory with it");
+  LP_REQUIRE(!spans_meet(out, at) && !spans_meet(out, freq), "lp_rotary: the output must share no memory with positions and inv_freq");
   RotaryArgs a = {};
   a.seg[0] = {x, x_row, x_head, y, y_row, y_head, 0, heads, true, false};
   a.segs = 1, a.rows = rows, a.D = D, a.n = n_freq;
@@ -488,6 +497,18 @@ extern "C" int lp_rotary_append(const lp_rotary_append_desc* d, void* stream) {
   Dim kp[3] = {{d->n_pages, d->kp_page}, {d->page_size, d->kp_row}, {d->KVH, d->kp_head}}, vp[3] = {{d->n_pages, d->vp_page}, {d->page_size, d->vp_row}, {d->KVH, d->vp_head}};
   LP_REQUIRE(strides_nest(kp, 3, d->D) && strides_nest(vp, 3, d->D), "lp_rotary_append: rows of a pool share their memory");
   if (d->rows == 0) return 0;
+  const int elem = d->fp32 ? 4 : 2;
+  auto heads = [&](const void* p, long long row, long long head, int n) { return Span{p, elem, 3, {{d->rows, row}, {n, head}, {d->D, 1}}}; };
+  auto pool = [&](const void* p, long long page, long long row, long long head) { return Span{p, elem, 4, {{d->n_pages, page}, {d->page_size, row}, {d->KVH, head}, {d->D, 1}}}; };
+  const Span writes[3] = {pool(d->k_pool, d->kp_page, d->kp_row, d->kp_head), pool(d->v_pool, d->vp_page, d->vp_row, d->vp_head), heads(d->q_out, d->o_row, d->o_head, d->H)};
+  const Span reads[6] = {heads(d->q, d->q_row, d->q_head, d->H), heads(d->k, d->k_row, d->k_head, d->KVH), heads(d->v, d->v_row, d->v_head, d->KVH),
+                         {d->positions, d->positions_64 ? 8 : 4, 1, {{d->rows, 1}}}, {d->inv_freq, 4, 1, {{d->n_freq, 1}}}, {d->slots, 8, 1, {{d->rows, 1}}}};
+  const bool in_place = d->q == d->q_out && (d->rows == 1 || d->q_row == d->o_row) && (d->H == 1 || d->q_head == d->o_head);
+  for (int w = 0; w < 3; ++w) {
+    for (int r = 0; r < 6; ++r)
+      LP_REQUIRE((w == 2 && r == 0 && in_place) || !spans_meet(writes[w], reads[r]), "lp_rotary_append: the pools and q_out must share no memory with what the call reads (q_out may be q)");
+    for (int o = 0; o < w; ++o) LP_REQUIRE(!spans_meet(writes[w], writes[o]), "lp_rotary_append: the pools and q_out must share no memory with one another");
+  }
   RotaryArgs a = {};
   a.seg[0] = {d->q, d->q_row, d->q_head, d->q_out, d->o_row, d->o_head, 0, d->H, true, false};
   a.seg[1] = {d->k, d->k_row, d->k_head, d->k_pool, d->kp_row, d->kp_head, d->n_pages > 1 ? d->kp_page : 0, d->KVH, true, true};

@@ -843,52 +843,15 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     rows, n_free, ld = int(rows), free.shape[0], page_table.stride(0)
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
-    p_table, p_used, p_free, p_len, p_new = page_table.data_ptr(), used.data_ptr(), free.data_ptr(), lengths.data_ptr(), new.data_ptr()
-    end = p_table + 4 * ((B - 1) * ld + max_pages)
-    for p, n, name in ((p_used, 1, "used"), (p_free, n_free, "free"), (p_len, B, "lengths"), (p_new, B, "new")):
-        if (p < end and p + 4 * n > p_table) or (p != p_used and p < p_used + 4 and p + 4 * n > p_used) or (p == p_used and name != "used" and n):
-            raise ValueError(f"{name} must not share memory with what the call changes")
-    padded = (rows + 3) & -4
-    seq, pos = torch.empty((2, padded), dtype=_I32, device=dev).unbind(0)
-    if padded != rows:
-        seq, pos = seq[:rows], pos[:rows]
+    seq, pos = torch.empty((rows,), dtype=_I32, device=dev), torch.empty((rows,), dtype=_I32, device=dev)
     slots = torch.empty((rows,), dtype=_I64, device=dev)
     if B == 0:
         return seq.fill_(-1), pos.fill_(-1), slots.fill_(-1), torch.zeros((1,), dtype=_I32, device=dev)
     row0 = torch.empty((B + 1,), dtype=_I32, device=dev)
     L = _lib.lib()
-    _call(dev, L, "lp_step_tables", L.lp_step_tables, p_len, p_new, p_table, ld, max_pages, int(page_size), p_free, n_free, p_used, B, rows, seq.data_ptr(), pos.data_ptr(), slots.data_ptr(),
-          row0.data_ptr())
+    _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), ld, max_pages, int(page_size), free.data_ptr(), n_free, used.data_ptr(), B, rows,
+          seq.data_ptr(), pos.data_ptr(), slots.data_ptr(), row0.data_ptr())
     return seq, pos, slots, row0
-
-
-def _apart(a, b):
-    """whether two tensors of the same number of dimensions and the same strides share no element (the parts of one product or of one pool, whose spans of memory meet)"""
-    if a.dtype != b.dtype or a.dim() != b.dim() or any(p < 0 or (p != q and m > 1 and n > 1) for p, q, m, n in zip(a.stride(), b.stride(), a.shape, b.shape)):
-        return False
-    dims = sorted(((q if m == 1 else p, m, n) for p, q, m, n in zip(a.stride(), b.stride(), a.shape, b.shape) if m > 1 or n > 1), reverse=True)
-
-    def meet(delta, dims):                    # element i of a and element j of b, delta behind: i s = j s + the rest
-        if not dims:
-            return delta == 0
-        (s, m, n), inner = dims[0], dims[1:]
-        reach = sum(t * (max(x, y) - 1) for t, x, y in inner)
-        if s <= reach:
-            return True                       # not nested: not known
-        q, r = divmod(delta, s)
-        return (-n < q < m and meet(r, inner)) or (-n < q + 1 < m and meet(r - s, inner))
-    return not meet((b.data_ptr() - a.data_ptr()) // a.element_size(), dims)
-
-
-def _shares(a, b):
-    """whether two tensors may share an element: their spans of memory meet, and they are not told apart"""
-    p, q = a.data_ptr(), b.data_ptr()
-    if p <= q:
-        if p + (sum((s - 1) * st for s, st in zip(a.shape, a.stride())) + 1) * a.element_size() <= q:
-            return False
-    elif q + (sum((s - 1) * st for s, st in zip(b.shape, b.stride())) + 1) * b.element_size() <= p:
-        return False
-    return a.numel() > 0 and b.numel() > 0 and not _apart(a, b)
 
 
 def _rotary_check(x, name, dtypes, dim, device=None):
@@ -920,7 +883,7 @@ def rotary(x, positions, inv_freq, layout="half", scale=1.0, inverse=False, out=
         xs = x.stride()
         fine = (x.is_cuda and (kind is _BF16 or kind is _F32) and (xs[2] == 1 or D <= 1) and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,)
                 and positions.is_contiguous() and positions.device == dev and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D
-                and out is None)
+                and (out is None or (out.dtype is kind and out.shape == x.shape and out.device == dev and (out.stride(2) == 1 or D <= 1))))
     except (AttributeError, ValueError, IndexError):
         fine = False
     inter = _rotary_layout(layout)
@@ -934,10 +897,6 @@ def rotary(x, positions, inv_freq, layout="half", scale=1.0, inverse=False, out=
             _rotary_check(out, "out", (kind,), 3, dev)
             if out.shape != x.shape:
                 raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
-            if _shares(out, x) and (out.data_ptr() != x.data_ptr() or out.stride() != xs):
-                raise ValueError("out must be x itself or share no memory with it")
-            if _overlaps(out, positions) or _overlaps(out, inv_freq):
-                raise ValueError("out must not share memory with positions or inv_freq")
     if out is None:
         out = torch.empty((rows, heads, D), dtype=kind, device=dev)
     if rows == 0 or heads == 0 or D == 0:
@@ -961,7 +920,8 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
                 and k.shape == (rows, G, D) and v.shape == (rows, G, D) and k_pool.shape[2:] == (G, D) and v_pool.shape == k_pool.shape and k.device == dev and v.device == dev and k_pool.device == dev
                 and v_pool.device == dev and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,) and positions.is_contiguous() and positions.device == dev
                 and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D and slots.dtype is _I64 and slots.shape == (rows,)
-                and slots.is_contiguous() and slots.device == dev and q_out is None)
+                and slots.is_contiguous() and slots.device == dev
+                and (q_out is None or (q_out.dtype is kind and q_out.shape == (rows, H, D) and q_out.device == dev and q_out.stride(2) == 1)))
     except (AttributeError, ValueError, IndexError):
         fine = False
     inter = _rotary_layout(layout)
@@ -981,12 +941,6 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
             _rotary_check(q_out, "q_out", (kind,), 3, dev)
             if q_out.shape != q.shape:
                 raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-            if _shares(q_out, q) and (q_out.data_ptr() != q.data_ptr() or q_out.stride() != s):
-                raise ValueError("q_out must be q itself or share no memory with it")
-            if any(_shares(q_out, t) for t in (k, v, k_pool, v_pool, positions, inv_freq, slots)):
-                raise ValueError("k_pool, v_pool and q_out must share no memory with one another nor with what the call reads")
-    if any(_shares(p, t) for p in (k_pool, v_pool) for t in (q, k, v, positions, inv_freq, slots)) or _shares(k_pool, v_pool):
-        raise ValueError("k_pool, v_pool and q_out must share no memory with one another nor with what the call reads")
     if q_out is None:
         q_out = torch.empty((rows, H, D), dtype=kind, device=dev)
     if rows == 0 or D == 0 or k_pool.numel() == 0:
@@ -1064,8 +1018,6 @@ def prefix_attention(q, k, v, lengths, prefix, new=None, page_table=None, prefix
         _prefix_refusals(q, k, v, lengths, prefix, new, page_table, prefix_k, prefix_v, out)
     if out is None:
         out = torch.empty((B, T, H, D), dtype=_BF16, device=dev)
-    elif any(t is not None and _shares(out, t) for t in (q, k, v, prefix_k, prefix_v, lengths, new, page_table)):
-        raise ValueError("out must not share memory with the inputs")
     if B == 0 or T == 0:
         return out
     os_ = out.stride()

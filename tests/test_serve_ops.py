@@ -41,7 +41,7 @@ def test_struct_layouts_match_the_header(tmp_path, struct, name):
 def prefix_desc(**kw):
     """a descriptor whose numbers are in order (its addresses are not touched before the checks are through)"""
     base = dict(q=1 << 20, q_batch=4096, q_token=1024, q_head=128, k=1 << 20, k_page=65536, k_row=256, k_head=128, v=1 << 20, v_page=65536, v_row=256, v_head=128, prefix_k=None, pk_row=0,
-                pk_head=0, prefix_v=None, pv_row=0, pv_head=0, out=1 << 20, o_batch=4096, o_token=1024, o_head=128, page_table=1 << 20, ld_table=4, max_pages=4, n_pages=9, page_size=64,
+                pk_head=0, prefix_v=None, pv_row=0, pv_head=0, out=1 << 36, o_batch=4096, o_token=1024, o_head=128, page_table=1 << 20, ld_table=4, max_pages=4, n_pages=9, page_size=64,
                 lengths=1 << 20, fresh=None, prefix=100, B=2, T=4, H=8, KVH=2, D=128, scale=0.1)
     return _lib.PrefixAttnDesc(**{**base, **kw})
 
@@ -74,18 +74,18 @@ def test_other_refusals_are_status_codes(native_lib):
     p, L = C.c_void_p(1 << 20), native_lib
 
     def tables(**kw):
-        a = {**dict(B=3, W=4, ld=4, size=16, free=p, n=5, used=p, rows=8), **kw}
-        return L.lp_step_tables(p, p, p, a["ld"], a["W"], a["size"], a["free"], a["n"], a["used"], a["B"], a["rows"], p, p, p, p, None)
+        a = {**dict(B=3, W=4, ld=4, size=16, free=p, n=5, used=C.c_void_p(1 << 31), rows=8), **kw}
+        return L.lp_step_tables(p, p, C.c_void_p(1 << 34), a["ld"], a["W"], a["size"], a["free"], a["n"], a["used"], a["B"], a["rows"], p, p, p, p, None)
     assert [tables(**kw) for kw in (dict(B=0), dict(B=8193), dict(W=0), dict(size=0), dict(ld=3), dict(rows=-1), dict(n=-1), dict(free=None), dict(used=None), dict(W=1 << 20, ld=1 << 20, size=1 << 12),
                                     dict(rows=(1 << 30) + 1))] == [-1] * 11
 
     def rotary(**kw):
         a = {**dict(x=p, rows=5, heads=4, D=64, yr=256, yh=64, n=32, freq=p, pos=p), **kw}
-        return L.lp_rotary(a["x"], 256, 64, p, a["yr"], a["yh"], 0, a["rows"], a["heads"], a["D"], a["pos"], 0, a["freq"], a["n"], 0, 1.0, 0, None)
+        return L.lp_rotary(a["x"], 256, 64, C.c_void_p(1 << 34), a["yr"], a["yh"], 0, a["rows"], a["heads"], a["D"], a["pos"], 0, a["freq"], a["n"], 0, 1.0, 0, None)
     assert [rotary(**kw) for kw in (dict(x=None), dict(pos=None), dict(freq=None), dict(rows=-1), dict(heads=0), dict(D=0), dict(D=4097), dict(n=33), dict(n=-1), dict(yr=200), dict(yh=32))] == [-1] * 11
     assert rotary(rows=0) == 0
-    base = dict(q=1 << 20, q_row=512, q_head=64, q_out=1 << 20, o_row=512, o_head=64, k=1 << 20, k_row=128, k_head=64, v=1 << 20, v_row=128, v_head=64, k_pool=1 << 20, kp_page=2048, kp_row=128,
-                kp_head=64, v_pool=1 << 20, vp_page=2048, vp_row=128, vp_head=64, positions=1 << 20, inv_freq=1 << 20, slots=1 << 20, positions_64=0, n_freq=32, interleaved=0, fp32=0, rows=5, H=8,
+    base = dict(q=1 << 20, q_row=512, q_head=64, q_out=1 << 30, o_row=512, o_head=64, k=1 << 20, k_row=128, k_head=64, v=1 << 20, v_row=128, v_head=64, k_pool=1 << 32, kp_page=2048, kp_row=128,
+                kp_head=64, v_pool=1 << 34, vp_page=2048, vp_row=128, vp_head=64, positions=1 << 20, inv_freq=1 << 20, slots=1 << 20, positions_64=0, n_freq=32, interleaved=0, fp32=0, rows=5, H=8,
                 KVH=2, D=64, n_pages=3, page_size=16, scale=1.0)
 
     def append(**kw):
@@ -118,12 +118,23 @@ def test_wrappers_refuse_what_is_not_on_a_gpu():
         ops.sample_tokens(z(2, 10), z(2))
 
 
-def test_parts_of_one_product_are_told_apart():
-    x = torch.zeros(5, 12, 8)
-    assert ops._apart(x[:, :8], x[:, 8:10]) and ops._apart(x[:, 10:], x[:, 8:10]) and not ops._apart(x[:, :9], x[:, 8:10]) and not ops._apart(x, x)
-    assert not ops._apart(x[:, :8], x.view(10, 6, 8)[:, :2])      # of other strides: not known
-    kv = torch.zeros(3, 2, 16, 2, 8)
-    assert ops._apart(kv[:, 0], kv[:, 1]) and not ops._apart(kv[:, 0], kv[:, 0]) and ops._apart(kv[:2], kv[2:])
+def test_parts_of_one_product_are_told_apart(native_lib):
+    """what may share memory and what may not, by the entry points' checks: all of these are refused or pass before anything runs (rows of heads of another strides are not known to be apart)"""
+    base = dict(q=1 << 20, q_row=96, q_head=8, q_out=1 << 30, o_row=64, o_head=8, k=(1 << 20) + 8 * 8 * 4, k_row=96, k_head=8, v=(1 << 20) + 10 * 8 * 4, v_row=96, v_head=8, k_pool=1 << 32, kp_page=512, kp_row=16,
+                kp_head=8, v_pool=(1 << 32) + 256 * 4, vp_page=512, vp_row=16, vp_head=8, positions=1 << 34, inv_freq=1 << 35, slots=1 << 36, positions_64=0, n_freq=4, interleaved=0, fp32=1, rows=5, H=8,
+                KVH=2, D=8, n_pages=3, page_size=16, scale=1.0)
+
+    def refused(**kw):
+        rc = native_lib.lp_rotary_append(C.byref(_lib.RotaryAppendDesc(**{**base, **kw})), None)
+        assert rc != 0      # (without a GPU what passes the checks does not launch)
+        return rc == -1 and "share no memory" in native_lib.lp_last_error().decode()
+    if torch.cuda.is_available():
+        pytest.skip("addresses that nobody holds: for machines without a GPU")
+    assert not refused() and not refused(q_out=1 << 20, o_row=96)                                    # apart; the queries in place, beside keys and values of the same rows
+    assert refused(q_out=(1 << 20) + 32, o_row=96) and refused(q_out=(1 << 20) + 8 * 4, o_row=96, H=2)
+    assert refused(q_out=(1 << 20) + 11 * 8 * 4, o_row=96, H=1) and not refused(q_out=(1 << 20) + 96 * 5 * 4, o_row=96)
+    assert refused(v_pool=1 << 32) and refused(v_pool=(1 << 32) + 255 * 4) and refused(v_pool=(1 << 32) + 4 * 512 - 4) and not refused(v_pool=(1 << 32) + 4 * (2 * 512 + 256))
+    assert refused(k_pool=1 << 20) and refused(slots=1 << 32) and refused(positions=(1 << 32) + 512 * 4 * 2) and refused(k_pool=(1 << 35) + 12)
 
 
 # ------------------------------------------------------------------------------------------------------------ step tables
@@ -192,7 +203,7 @@ def test_step_tables_wrapper_refusals():
     good = dict(lengths=lengths, new=new, page_table=table, free=free, used=used, page_size=16, rows=8)
     for change, err in ((dict(lengths=lengths.long()), TypeError), (dict(new=new[:1]), ValueError), (dict(page_table=table[:1]), ValueError), (dict(used=free[:2]), ValueError), (dict(free=table), ValueError),
                         (dict(rows=-1), ValueError), (dict(page_size=0), _lib.NativeError), (dict(page_table=table.t().contiguous().t()), ValueError), (dict(lengths=table[:, 0].contiguous().cpu()), TypeError),
-                        (dict(free=table.view(-1)), ValueError), (dict(used=free[:1]), ValueError)):
+                        (dict(free=table.view(-1)), _lib.NativeError), (dict(used=free[:1]), _lib.NativeError)):
         with pytest.raises(err):
             ops.step_tables(**{**good, **change})
     none = ops.step_tables(lengths[:0], new[:0], table[:0], free, used, 16, 3)
@@ -274,7 +285,7 @@ def test_rotary_wrapper_refusals():
     x, pos, f = torch.zeros(4, 2, 16, device="cuda"), torch.zeros(4, dtype=I32, device="cuda"), freqs(8)
     for args, kw, err in (((x.half(), pos, f), {}, TypeError), ((x, pos.float(), f), {}, TypeError), ((x, pos[:3], f), {}, ValueError), ((x, pos, f.double()), {}, TypeError), ((x, pos, freqs(9)), {}, ValueError),
                           ((x, pos, f), dict(out=x[:, :1]), ValueError), ((x, pos, f), dict(out=x.bfloat16()), TypeError), ((x[:, :, ::2], pos, freqs(4)), {}, ValueError),
-                          ((x[:3], pos[:3], f), dict(out=x[1:]), ValueError), ((x, pos, f), dict(out=x[:1].expand(4, 2, 16).clone()[:1].expand(4, 2, 16)), _lib.NativeError)):
+                          ((x[:3], pos[:3], f), dict(out=x[1:]), _lib.NativeError), ((x, pos, f), dict(out=x[:1].expand(4, 2, 16).clone()[:1].expand(4, 2, 16)), _lib.NativeError)):
         with pytest.raises(err):
             ops.rotary(*args, **kw)
     assert ops.rotary(x[:0], pos[:0], f).shape == (0, 2, 16)
@@ -316,8 +327,8 @@ def test_rotary_append_wrapper_refusals():
     q, k = torch.zeros(4, 4, 16, device="cuda"), torch.zeros(4, 2, 16, device="cuda")
     pool, pos, slots, f = torch.zeros(3, 8, 2, 16, device="cuda"), torch.zeros(4, dtype=I32, device="cuda"), torch.arange(4, device="cuda"), freqs(8)
     good = dict(q=q, k=k, v=k.clone(), positions=pos, inv_freq=f, k_pool=pool, v_pool=pool.clone(), slots=slots)
-    for change, err in ((dict(k=k.bfloat16()), TypeError), (dict(v=k[:, :1]), ValueError), (dict(slots=slots.int()), TypeError), (dict(slots=slots[:3]), ValueError), (dict(v_pool=pool), ValueError),
-                        (dict(k_pool=pool[:, :, :1]), ValueError), (dict(q_out=q[:, :2]), ValueError), (dict(k=pool[0, :4]), ValueError), (dict(q_out=q[:1].expand(4, 4, 16)), ValueError),
+    for change, err in ((dict(k=k.bfloat16()), TypeError), (dict(v=k[:, :1]), ValueError), (dict(slots=slots.int()), TypeError), (dict(slots=slots[:3]), ValueError), (dict(v_pool=pool), _lib.NativeError),
+                        (dict(k_pool=pool[:, :, :1]), ValueError), (dict(q_out=q[:, :2]), ValueError), (dict(k=pool[0, :4]), _lib.NativeError), (dict(q_out=q[:1].expand(4, 4, 16)), _lib.NativeError),
                         (dict(layout="x"), ValueError), (dict(inv_freq=freqs(9)), ValueError)):
         with pytest.raises(err):
             ops.rotary_append(**{**good, **change})
@@ -532,7 +543,7 @@ def test_offsets_beyond_32_bits(B):
 def test_prefix_attention_wrapper_refusals():
     c = prefix_case(2, 4, 8, 2, 128, 20, [3, 4], page=16, seed=14)
     for change, err in ((dict(q=c["q"].float()), TypeError), (dict(k=c["k"][..., :64]), ValueError), (dict(lengths=c["lengths"].long()), TypeError), (dict(lengths=c["lengths"][:1]), ValueError),
-                        (dict(page_table=c["page_table"][:1]), ValueError), (dict(new=c["lengths"][:1]), ValueError), (dict(out=c["q"]), ValueError), (dict(prefix=10 ** 6), _lib.NativeError),
+                        (dict(page_table=c["page_table"][:1]), ValueError), (dict(new=c["lengths"][:1]), ValueError), (dict(out=c["q"]), _lib.NativeError), (dict(prefix=10 ** 6), _lib.NativeError),
                         (dict(q=c["q"].transpose(2, 3).contiguous().transpose(2, 3)), ValueError), (dict(q=torch.zeros(2, 4, 9, 128, dtype=BF16, device="cuda")), _lib.NativeError),
                         (dict(out=c["q"][:1]), ValueError), (dict(prefix_k=c["k"][0], prefix_v=c["v"][0]), ValueError), (dict(page_table=None), ValueError), (dict(prefix=-1), _lib.NativeError)):
         with pytest.raises(err):
