@@ -437,9 +437,15 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   else LP_REQUIRE(d->prefix == 0, "lp_prefix_attention: a prefix of %d rows that is nowhere", d->prefix);
   return 0;
 }
-// whether the prefix goes to the tcgen05 kernel
-constexpr int PA_TC_ROWS = 16;
-static bool prefix_tc(const lp_prefix_attn_desc* d) { return (long long)d->B * d->T * (d->H / d->KVH) > PA_TC_ROWS && prefix_tc_takes(d); }
+// Whether the prefix goes to the tcgen05 kernel: it costs a launch and 10 us of start and end, the other reads the prefix once for every 16 rows.  Decided by blocks of 16 rows x key heads x keys, of more than 8 rows.
+// mma.sync and tcgen05, us a call, 64 own rows a request, 32 heads over 8 (16 over 16): 16 rows after 4,796 22.5 and 28.7 (26.6, 32.8), after 20,000 34.8 and 36.9 (59.4, 53.2), after 100,003 92 and 86 (233, 150);
+// 32 rows after 512 18.4 and 22.5 (20.5, 26.6), after 4,796 26.6 and 32.8 (36.8, 34.8), after 20,000 49 and 43 (107, 53), after 100,003 182 and 92; 64 rows after 4,796 34.8 both (57, 37), after 20,000 100 and 45.
+// Up to 8 rows read it once in any case: 8 after 100,003 84 and 84 (160, 154).
+constexpr long long PA_TC_WORK = 160000;
+static bool prefix_tc(const lp_prefix_attn_desc* d) {
+  const long long rows = (long long)d->B * d->T * (d->H / d->KVH);
+  return rows > 8 && (rows + 15) / 16 * d->KVH * d->prefix > PA_TC_WORK && prefix_tc_takes(d);
+}
 // how a call is cut: what the descriptor's numbers alone decide
 static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
   a.d = *d;

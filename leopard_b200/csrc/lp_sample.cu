@@ -217,13 +217,10 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     for (int i = from + lane * 4; i < from + part; i += 128) f(i, *reinterpret_cast<const float4*>(z + i));
   };
 
-  // ---- what is kept: keys above last_key, and of those equal to it the ones up to last_at
-  unsigned last_key = 0;
-  int last_at = 0x7fffffff;
-  auto kept = [&](float x, int i) {
-    const unsigned key = sa_key(x);
-    return x > -INFINITY && (key > last_key || (key == last_key && v0 + i <= last_at));
-  };
+  // ---- what is kept: logits above `last`, and of those equal to it the ones up to last_at
+  float last = -INFINITY;
+  int last_at = -1;
+  auto kept = [&](float x, int i) { return x > last || (x == last && v0 + i <= last_at); };
   const bool by_count = top_k > 0 && top_k < a.V, by_mass = top_p < 1.f;
   const float least = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
   const u64 w_min = least > 0.f ? (u64)ceil((double)least * 8796093022208.0) : 0;
@@ -237,6 +234,14 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     return top_p > 0.f && x >= 1.0 ? (u64)x : 1ULL;
   };
   int turn = 0;                                           // of s.total
+  auto upto_lanes = [&](u64 v) {                          // the sum of v up to this lane
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    return v;
+  };
   // The word (by index) up to which more than `limit` of value(i, z_i) lies, by all CTAs; limit = choose(the sum of all).  Returns its index in the one CTA that has it, -1 in the others.
   // value(...) is `base` too large.
   // on(i, z_i): whether a word counts at all.
@@ -253,9 +258,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     auto value = [&](int i, float x) { return on(i, x) ? value_of(x) : base; };
     if (lane == 0) s.warp_w[warp] = sum;
     __syncthreads();
-    u64 mine = 0;
-#pragma unroll
-    for (int w = 0; w < SA_WARPS; ++w) mine += s.warp_w[w];
+    const u64 w_upto = upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0), mine = __shfl_sync(0xffffffffu, w_upto, 31);
     if (tid < CTAS) *sa_at(&s.total[turn][rank], tid) = mine;
     sa_cluster<CTAS>();
     u64 all = 0, before = 0;
@@ -267,29 +270,19 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     turn ^= 1;
     const u64 limit = choose(all);
     if (limit < before || limit >= before + mine) return -1;
-    u64 at = before;
-    int w = 0;
-#pragma unroll
-    for (int k = 0; k < SA_WARPS; ++k)
-      if (k == w && at + s.warp_w[k] <= limit) at += s.warp_w[k], w = k + 1;
+    const int w = __popc(__ballot_sync(0xffffffffu, before + w_upto <= limit));      // the warp in whose words it lies
+    u64 at = before + (w ? __shfl_sync(0xffffffffu, w_upto, max(w - 1, 0)) : 0);
     // that warp's words, a thread some of them side by side
     const int some = (part + SA_THREADS - 1) / SA_THREADS, i0 = min(tid * some, part) + w * part, i1 = min((tid + 1) * some, part) + w * part;
     u64 own = 0;
 #pragma unroll 2
     for (int i = i0; i < i1; ++i) own += value(i, z[i]) - base;
-    u64 run = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-    }
+    const u64 run = upto_lanes(own);
     __syncthreads();                                      // (warp_w has been read)
     if (lane == 31) s.warp_w[warp] = run;
     __syncthreads();
-    at += run - own;
-#pragma unroll
-    for (int k = 0; k < SA_WARPS; ++k)
-      if (k < warp) at += s.warp_w[k];
+    const u64 upto = upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0);
+    at += run - own + (warp ? __shfl_sync(0xffffffffu, upto, max(warp - 1, 0)) : 0);
     if (limit >= at && limit < at + own)
       for (int i = i0; i < i1; ++i) {
         const u64 v = value(i, z[i]) - base;
@@ -308,17 +301,19 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     auto mass = [&](float x) { return sa_weight_bits(((double)x - top) * unit, power, s.root) - power_bits; };
     // ranges of equal width below the largest logit, as far as weights reach (30 t) or a top_k may look
     const float reach = fminf(fmaxf(30.f * t, 24.f), hi - lo), fine = reach > 1e-30f ? (float)(SA_BINS - 1) / reach : 0.f;
-    auto bin_of = [&](float x) { return __float_as_int(fminf(__fmaf_rn(hi - x, fine, 12582912.f), 12582912.f + (SA_BINS - 1))) - 0x4b400000; };      // (1.5 2^23: the whole number is in the low bits)
+    constexpr float WHOLE = 12582912.f;                   // 1.5 2^23: the whole number is in the low bits
+    auto depth = [&](float x) { return fminf(__fmaf_rn(hi - x, fine, WHOLE), WHOLE + (SA_BINS - 1)); };
+    auto bin_of = [&](float x) { return __float_as_int(depth(x)) - 0x4b400000; };
     int hists = 0;
-    // The last word before which fewer than `limit` words lie (MASS: less than top_p of the mass): last_key and last_at.  True: the word has been drawn.
+    // The last word before which fewer than `limit` words lie (MASS: less than top_p of the mass): `last` and last_at.  True: the word has been drawn.
     auto cut = [&](auto by, u64 limit) -> bool {
       constexpr bool MASS = decltype(by)::value;
       SaHist* h;
       auto count_in = [&](int b, u64 w) {
         atomicAdd(&h->n[b], 1u);
         if (MASS) {
-          const unsigned w_lo = (unsigned)w & ((1u << low) - 1), w_hi = (unsigned)(w >> low);
-          if (w_lo) atomicAdd(&h->lo[b], w_lo);
+          const unsigned w_hi = (unsigned)(w >> low);
+          atomicAdd(&h->lo[b], (unsigned)w & ((1u << low) - 1));
           if (w_hi) atomicAdd(&h->hi[b], w_hi);
         }
       };
@@ -402,29 +397,31 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           key_lo = lo_of - key_lo > width ? lo_of - width : key_lo;
         }
         const bool finish = first && !(MASS && by_count) && above_n + in_bin <= SA_LIST;      // few words down to the limit: all of them are listed
-        auto inside = [&](float x, int i) {
-          if (MASS && by_count ? !kept(x, i) : !(x > -INFINITY)) return false;
-          if (first) {
-            const int b = bin_of(x);
-            return finish ? b <= bin : b == bin;
-          }
+        const float from_depth = finish ? 0.f : WHOLE + (float)bin, to_depth = WHOLE + (float)bin;
+        auto on = [&](float x, int i) { return MASS && by_count ? kept(x, i) : x > -INFINITY; };
+        auto inside = [&](float x, int i) {               // of the range (finish: of it and of those above)
+          const float d = depth(x);
           const unsigned k = sa_key(x);
-          return k >= key_lo && k <= key_hi;
+          return on(x, i) && (first ? d >= from_depth && d <= to_depth : k >= key_lo && k <= key_hi);
         };
         if (finish || in_bin <= SA_LIST) {
           auto list = [&](int i, float x) {
             const int at = atomicAdd(&s.n_list[MASS], 1);      // (below SA_LIST: there are no more words)
             s.list[MASS].word[at] = (u64)sa_key(x) << 32 | ~(unsigned)(v0 + i);
           };
-          each([&](int i, const float4& x) {
-            const bool a0 = inside(x.x, i), a1 = inside(x.y, i + 1), a2 = inside(x.z, i + 2), a3 = inside(x.w, i + 3);
-            if (__any_sync(0xffffffffu, a0 || a1 || a2 || a3)) {
-              if (a0) list(i, x.x);
-              if (a1) list(i + 1, x.y);
-              if (a2) list(i + 2, x.z);
-              if (a3) list(i + 3, x.w);
-            }
-          });
+          auto look_through = [&](auto in) {
+            each([&](int i, const float4& x) {
+              const bool a0 = in(x.x, i), a1 = in(x.y, i + 1), a2 = in(x.z, i + 2), a3 = in(x.w, i + 3);
+              if (__any_sync(0xffffffffu, a0 || a1 || a2 || a3)) {
+                if (a0) list(i, x.x);
+                if (a1) list(i + 1, x.y);
+                if (a2) list(i + 2, x.z);
+                if (a3) list(i + 3, x.w);
+              }
+            });
+          };
+          if (first && !(MASS && by_count)) look_through([&](float x, int) { const float d = depth(x); return d >= from_depth && d <= to_depth && x > -INFINITY; });
+          else look_through(inside);
           sa_cluster<CTAS>();
           if (finish && rank != 0) return true;
           int n_all = 0;
@@ -444,10 +441,20 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           // each word counts those before it: by two threads, half of the words each
           const int mine = tid >> 1, half = tid & 1;
           word = s.gathered.word[mine];
-          unsigned before = 0;                            // those before it in order, and (upper half) by index
-          for (int j = half * 2; j < n_all; j += 4) {
-            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&s.gathered.word[j]);
-            before += (o.x > word ? 1u : 0u) + (o.y > word ? 1u : 0u) + ((unsigned)o.x > (unsigned)word ? 0x10000u : 0u) + ((unsigned)o.y > (unsigned)word ? 0x10000u : 0u);
+          unsigned before = 0;                            // those before it in order, and (upper half: where all is drawn from the list) by index
+          if (warp * 16 < n_all) {
+            if (finish)
+#pragma unroll 2
+              for (int j = half * 2; j < n_all; j += 4) {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&s.gathered.word[j]);
+                before += (o.x > word ? 1u : 0u) + (o.y > word ? 1u : 0u) + ((unsigned)o.x > (unsigned)word ? 0x10000u : 0u) + ((unsigned)o.y > (unsigned)word ? 0x10000u : 0u);
+              }
+            else
+#pragma unroll 2
+              for (int j = half * 2; j < n_all; j += 4) {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&s.gathered.word[j]);
+                before += (o.x > word ? 1u : 0u) + (o.y > word ? 1u : 0u);
+              }
           }
           before += __shfl_xor_sync(0xffffffffu, before, 1);
           const unsigned before_n = before & 0xffffu, before_at = before >> 16;
@@ -455,11 +462,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           const float x = sa_of_key((unsigned)(word >> 32));
           // of the first SA_LIST threads: the sum of v up to this one
           auto upto = [&](u64 v) {
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const u64 up = __shfl_up_sync(0xffffffffu, v, o);
-              if (lane >= o) v += up;
-            }
+            v = upto_lanes(v);
             __syncthreads();
             if (lane == 31) s.warp_w[warp] = v;
             __syncthreads();
@@ -495,7 +498,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
               s.last_at = (int)~(unsigned)word;
             }
             __syncthreads();
-            last_key = s.last_key;
+            last = sa_of_key(s.last_key);
             last_at = s.last_at;
             return false;
           }
@@ -536,7 +539,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           const int i = locate([&](int k, float x) { return x == same && (!(MASS && by_count) || kept(x, k)); }, [](float) -> u64 { return 1; }, 0, [&](u64) { return n_left - 1; });
           if (i >= 0 && tid < CTAS) *sa_at(&s.last_at, tid) = v0 + i;
           sa_cluster<CTAS>();
-          last_key = key_lo;
+          last = same;
           last_at = s.last_at;
           return false;
         }
