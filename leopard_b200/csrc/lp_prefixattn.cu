@@ -323,7 +323,7 @@ prefix_rows_kernel(const __grid_constant__ PrefixArgs a, int pre_ctas) {
 // that each piece is read once.  Bound by latency, and by the workspace's way through L2.
 constexpr int PJ_ROWS = 8, PJ_AT_ONCE = 8;
 template <int D, int GROUPS>
-__global__ void __launch_bounds__(PJ_ROWS * D / 4 * GROUPS)
+__global__ void __launch_bounds__(PJ_ROWS * D / 4 * GROUPS, 1024 / (PJ_ROWS * D / 4 * GROUPS))
 prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
   constexpr int THREADS = PJ_ROWS * D / 4;
   extern __shared__ int pa_first[];
@@ -429,9 +429,9 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   LP_REQUIRE(d->D == 64 || d->D == 96 || d->D == 128, "lp_prefix_attention: heads of %d are not built (64, 96, 128)", d->D);
   LP_REQUIRE((long long)d->B * d->T * d->H <= 1LL << 24, "lp_prefix_attention: %d requests of %d tokens and %d heads are too many", d->B, d->T, d->H);
   LP_REQUIRE(d->n_pages > 0 && d->page_size > 0 && d->max_pages > 0, "lp_prefix_attention: %d pages of %d rows, %d a request", d->n_pages, d->page_size, d->max_pages);
-  LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 256, "lp_prefix_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
+  LP_REQUIRE((long long)d->max_pages * d->page_size <= (1LL << 31) - 512, "lp_prefix_attention: %d pages of %d rows are too many", d->max_pages, d->page_size);
   LP_REQUIRE(d->B * (long long)d->KVH * ((d->T * (d->H / d->KVH) + 7) / 8) <= 1 << 24, "lp_prefix_attention: %d requests of %d tokens over %d key heads are too many", d->B, d->T, d->KVH);
-  LP_REQUIRE(d->prefix >= 0 && d->prefix <= (1LL << 31) - 256, "lp_prefix_attention: prefix %d", d->prefix);
+  LP_REQUIRE(d->prefix >= 0 && d->prefix <= (1LL << 31) - 512, "lp_prefix_attention: prefix %d", d->prefix);
   if (d->prefix_k) LP_REQUIRE(!d->page_table && d->prefix_v, "lp_prefix_attention: a prefix of its own goes with a cache of its own each");
   else if (d->page_table) LP_REQUIRE(d->prefix <= (long long)d->max_pages * d->page_size, "lp_prefix_attention: a prefix of %d rows in %d pages of %d", d->prefix, d->max_pages, d->page_size);
   else LP_REQUIRE(d->prefix == 0, "lp_prefix_attention: a prefix of %d rows that is nowhere", d->prefix);

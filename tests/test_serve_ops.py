@@ -405,6 +405,73 @@ def test_prefix_attention(B, T, H, G, D, prefix, own, new, page):
     assert torch.equal(attend(c, out=torch.full_like(out, 7.0)), got)
 
 
+# rows x key heads x keys enough for the tcgen05 kernel: up to 128 rows, a block of 256, a last one of up to 128, more items than CTAs; every head, pages that end inside a tile and whole tiles, few tiles
+MANY = [
+    (20, 1, 32, 8, 128, 4100, [i for i in range(20)], None, 64), (9, 1, 32, 8, 128, 7001, [3] * 9, [1, 1, 0, 1, 1, 1, 1, 1, 0], 16), (32, 1, 32, 8, 128, 2600, [0] * 32, None, 0),
+    (40, 1, 32, 8, 128, 2051, [i % 70 for i in range(40)], [i % 4 > 0 for i in range(40)], 48), (70, 1, 32, 8, 128, 1153, [i for i in range(70)], None, 0), (8, 9, 32, 8, 128, 1280, [5 * i for i in range(8)], [i + 1 for i in range(8)], 128),
+    (50, 1, 12, 4, 64, 4099, [i % 9 for i in range(50)], None, 8), (12, 5, 16, 4, 96, 3001, [64] * 12, [i % 6 for i in range(12)], 48), (13, 3, 8, 1, 128, 9000, [7] * 13, None, 64), (200, 2, 16, 16, 64, 640, [2] * 200, None, 16),
+    (600, 1, 32, 8, 64, 257, [1] * 600, None, 64), (2, 100, 16, 1, 96, 5000, [3, 0], [100, 99], 0), (17, 1, 16, 16, 128, 10001, list(range(17)), None, 1000), (24, 16, 32, 8, 128, 2000, list(range(24)), [i % 17 for i in range(24)], 24),
+]
+
+
+@gpu
+@pytest.mark.parametrize("B, T, H, G, D, prefix, own, new, page", MANY)
+def test_prefix_attention_of_many_rows(B, T, H, G, D, prefix, own, new, page):
+    test_prefix_attention(B, T, H, G, D, prefix, own, new, page)
+
+
+@gpu
+@pytest.mark.parametrize("B, prefix, page", [(20, 4100, 64), (40, 2051, 48), (70, 1153, 8)])
+def test_many_rows_see_no_stale_rows_nor_pages_that_are_not_there(B, prefix, page):
+    c = prefix_case(B, 1, 32, 8, 128, prefix, [b % 5 for b in range(B)], page=page, seed=19)
+    clean = attend(c)
+    held = torch.zeros(c["k"].shape[:2], dtype=torch.bool)
+    for b in range(B):
+        for i in range(prefix + b % 5 + 1) if b == 0 else range(prefix // page * page, prefix + b % 5 + 1):
+            held[int(c["page_table"][b, i // page]), i % page] = True
+    for t in (c["k"], c["v"]):
+        t[~held.cuda()] = float("nan")
+    # (behind the prefix request 0's page holds its own rows: they are no other's)
+    row = (int(c["page_table"][0, prefix // page]), prefix % page)
+    c["k"][row], c["v"][row] = float("nan"), float("inf")
+    again = attend(c)
+    assert torch.equal(again[1:], clean[1:]) and bool(again[0].isnan().any())
+    c["k"][row], c["v"][row] = 0.0, 0.0
+    for i in (0, 3, prefix // page // 2):
+        c["page_table"][:, i] = -1
+    c["page_table"][0, 5] = c["k"].shape[0]
+    c["page_table"][:, 7:9] = -2 ** 31
+    close(attend(c), c)
+    c["page_table"][:, :prefix // page] = -1               # nothing of the prefix's whole pages
+    close(attend(c), c)
+    c["page_table"][:] = -1
+    assert bool((attend(c) == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("B, prefix", [(3, 300), (20, 4100), (70, 1153)])
+def test_values_of_the_prefix_reach_all(B, prefix, bad):
+    c = prefix_case(B, 1, 32, 8, 128, prefix, [b % 5 for b in range(B)], page=64, seed=20)
+    clean = attend(c)
+    c["v"][int(c["page_table"][0, 1]), 9, 3, 17] = bad
+    got = attend(c)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[:, :, 12:16, 17] = True                            # (weights that are 0 in fp32 make inf a NaN, as in the definition: 0 x inf)
+    assert bool((~got[hit].isfinite()).all()) and torch.equal(got[~hit], clean[~hit])
+
+
+@gpu
+def test_weights_far_below_the_first_ones_do_not_count():
+    """scores that grow by hundreds from tile to tile, and fall: maxima that are left behind, in both kernels"""
+    for B, prefix in ((2, 700), (20, 4100), (70, 1153)):
+        c = prefix_case(B, 1, 32, 8, 128, prefix, [40] * B, page=64, seed=21)
+        ramp = torch.linspace(0.05, 6.0, c["k"].shape[0], device="cuda").to(BF16)[:, None, None, None]
+        for k in (c["k"] * ramp, c["k"] * ramp.flip(0)):
+            d = dict(c, k=k.contiguous())
+            close(attend(d), d)
+
+
 @gpu
 @pytest.mark.parametrize("B, T", [(3, 1), (3, 20)])
 def test_prefix_attention_is_attention_over_the_whole_sequence(B, T):
@@ -418,17 +485,17 @@ def test_prefix_attention_is_attention_over_the_whole_sequence(B, T):
 
 @gpu
 @pytest.mark.parametrize("scale", [0.02, -0.07, 0.0])
-@pytest.mark.parametrize("B", [2, 40])
-def test_prefix_attention_takes_any_scale(B, scale):
-    c = prefix_case(B, 2, 8, 2, 128, 200, [31] * B, page=64, seed=5)
+@pytest.mark.parametrize("B, prefix", [(2, 200), (40, 200), (40, 4200)])
+def test_prefix_attention_takes_any_scale(B, prefix, scale):
+    c = prefix_case(B, 2, 8, 2, 128, prefix, [31] * B, page=64, seed=5)
     close(attend(c, scale=scale), c, scale)
 
 
 @gpu
-@pytest.mark.parametrize("B", [2, 30])
-def test_prefix_attention_of_views(B):
+@pytest.mark.parametrize("B, prefix", [(2, 150), (30, 150), (30, 4000)])
+def test_prefix_attention_of_views(B, prefix):
     """heads as columns of a wider projection, keys and values as halves of one pool's rows, the prefix's too"""
-    c = prefix_case(B, 3, 8, 2, 128, 150, [7 + b for b in range(B)], page=32, seed=6)
+    c = prefix_case(B, 3, 8, 2, 128, prefix, [7 + b for b in range(B)], page=32, seed=6)
     qkv = torch.randn(B * 3, 12 * 128 + 8, device="cuda", generator=gen(1)).to(BF16)
     q = qkv[:, :1024].view(B, 3, 8, 128)
     q.copy_(c["q"])
@@ -438,7 +505,7 @@ def test_prefix_attention_of_views(B):
     got = attend(c, q=q, k=pool[:, :, :2], v=pool[:, :, 2:], out=out[:, :, 8:1032].unflatten(2, (8, 128)).transpose(0, 1))
     close(got, c)
     assert torch.equal(got, attend(c)) and bool((out[:, :, :8] == 0).all()) and bool((out[:, :, 1032:] == 0).all())
-    c = prefix_case(B, 3, 8, 2, 128, 150, [7 + b for b in range(B)], seed=7)
+    c = prefix_case(B, 3, 8, 2, 128, prefix, [7 + b for b in range(B)], seed=7)
     both = torch.stack([c["prefix_k"], c["prefix_v"]], 1)
     assert torch.equal(attend(c, prefix_k=both[:, 0], prefix_v=both[:, 1]), attend(c))
     heads_first = c["k"].transpose(1, 2).contiguous().transpose(1, 2)
@@ -528,11 +595,11 @@ def test_the_largest_batches(B, T, H, G, D):
 
 
 @gpu
-@pytest.mark.parametrize("B", [2, 40])
-def test_offsets_beyond_32_bits(B):
+@pytest.mark.parametrize("B, prefix", [(2, 130), (40, 8100)])
+def test_offsets_beyond_32_bits(B, prefix):
     """a pool of 4.5 GB: its last pages lie past 2^32 bytes and 2^31 elements"""
     pages = 70000
-    c = prefix_case(B, 1, 8, 4, 128, 130, [40] * B, page=64, seed=13)
+    c = prefix_case(B, 1, 8, 4, 128, prefix, [40] * B, page=64, seed=13)
     n = c["k"].shape[0]
     k, v = (torch.zeros(pages, 64, 4, 128, dtype=BF16, device="cuda") for _ in range(2))
     k[pages - n:], v[pages - n:] = c["k"], c["v"]
@@ -695,7 +762,7 @@ def test_the_sampler_draws_by_it():
 # ------------------------------------------------------------------------------------------------------------ streams, graphs, devices
 @gpu
 def test_two_streams_and_a_captured_step():
-    cs = [prefix_case(20, 1, 8, 2, 128, 600, [30 + i for i in range(20)], page=64, seed=s) for s in (1, 2)]
+    cs = [prefix_case(20, 1, 32, 8, 128, 4100, [30 + i for i in range(20)], page=64, seed=s) for s in (1, 2)]
     zs = [torch.randn(9, 40000, generator=gen(s), device="cuda") * 2 for s in (3, 4)]
     u = torch.rand(9, generator=gen(5), device="cuda")
     alone = [(attend(c), ops.sample_tokens(z, u, top_p=0.9)) for c, z in zip(cs, zs)]
@@ -712,7 +779,8 @@ def test_two_streams_and_a_captured_step():
     c, z = cs[0], zs[0]
     with torch.cuda.graph(graph):
         out, tokens = attend(c), ops.sample_tokens(z, u, top_p=0.9)
-    for other, oz, want in ((cs[1], zs[1], alone[1]), (prefix_case(20, 1, 8, 2, 128, 600, [30 + i for i in range(20)], page=64, seed=1), zs[0].clone(), alone[0])):
+    first = zs[0].clone()
+    for other, oz, want in ((cs[1], zs[1], alone[1]), (prefix_case(20, 1, 32, 8, 128, 4100, [30 + i for i in range(20)], page=64, seed=1), first, alone[0])):
         for n in ("q", "k", "v", "page_table", "lengths"):
             c[n].copy_(other[n])
         z.copy_(oz)
