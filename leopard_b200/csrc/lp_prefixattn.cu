@@ -28,15 +28,9 @@ __device__ __forceinline__ void prefix_rows(const PrefixArgs& a, int cta) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
 
   // ---- the piece
-  int kvh, r0, rows, n_keys, past, t0, t1, owner = 0, slot, length = 0;
-  if (!PRE) {
-    const int i = cta / a.own_splits / a.own_blocks;
-    owner = i / a.d.KVH;
-    kvh = i - owner * a.d.KVH;
-    length = a.d.lengths[owner];
-  }
-  pa_tokens(a, first);
+  int kvh, r0, rows, n_keys, past, t0, t1, owner = 0, slot;
   if (PRE) {
+    pa_tokens(a, first);
     rows = first[a.d.B] * a.group;
     const PrefixLine line = pa_line(a, rows);
     const int item = line.own ? cta / line.own : 0;
@@ -51,11 +45,13 @@ __device__ __forceinline__ void prefix_rows(const PrefixArgs& a, int cta) {
     slot = item + cta;
   } else {
     slot = cta;
-    const int rest = slot / a.own_splits, piece = slot - rest * a.own_splits;
-    r0 = rest % a.own_blocks * ROWS;
-    const int fresh = first[owner + 1] - first[owner];
+    const int rest = cta / a.own_splits, piece = cta - rest * a.own_splits, i = rest / a.own_blocks;
+    r0 = (rest - i * a.own_blocks) * ROWS;
+    owner = i / a.d.KVH;
+    kvh = i - owner * a.d.KVH;
+    const int fresh = pa_new(a, owner);
     rows = fresh * a.group;
-    pa_own(a, length, fresh, past, n_keys);
+    pa_own(a, a.d.lengths[owner], fresh, past, n_keys);
     const int pieces = pa_own_pieces(a, n_keys);
     if (piece >= pieces) return;
     const int tiles = (n_keys + PA_KEYS - 1) / PA_KEYS;
