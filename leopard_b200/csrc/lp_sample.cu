@@ -423,7 +423,10 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           if (first && !(MASS && by_count)) look_through([&](float x, int) { const float d = depth(x); return d >= from_depth && d <= to_depth && x > -INFINITY; });
           else look_through(inside);
           sa_cluster<CTAS>();
-          if (finish && rank != 0) return true;
+          if (finish && rank != 0) {
+            sa_cluster<CTAS>();                           // (its list has been read)
+            return true;
+          }
           int n_all = 0;
           u64 word = 0;
           {
@@ -437,6 +440,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
             }
           }
           if (tid < SA_LIST) s.gathered.word[tid] = word;      // (0 stands behind all words)
+          if (finish) sa_cluster<CTAS>();
           __syncthreads();
           // each word counts those before it: by two threads, half of the words each
           const int mine = tid >> 1, half = tid & 1;
@@ -559,10 +563,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
         sa_cluster<CTAS>();
       }
     };
-    if ((by_count && cut(SaByCount(), (u64)top_k)) || (by_mass && cut(SaByMass(), 0))) {
-      sa_cluster<CTAS>();                                 // nobody leaves while others may read here
-      return;
-    }
+    if ((by_count && cut(SaByCount(), (u64)top_k)) || (by_mass && cut(SaByMass(), 0))) return;
   }
   // ---- the draw
   const bool whole = !by_count && !by_mass && w_min == 0;
@@ -573,8 +574,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
                                  return w >= w_min ? w : 0;
                                },
                                0, drawn);
-  if (i >= 0 && tid == 0) a.out[row] = v0 + i;
-  sa_cluster<CTAS>();                                     // nobody leaves while others may read here
+  if (i >= 0 && tid == 0) a.out[row] = v0 + i;            // (since the last barrier nobody reads or writes in another CTA)
 }
 
 template <typename T, int CTAS>
