@@ -7,7 +7,7 @@
 // Weights are integers in units of 2^-43 (from a 64-bit exponential): their sums do not depend on the order in which they are taken, and the draw is the one that 64 bits give.
 // A cluster of CTAs holds a row in shared memory, read once.  Nothing is sorted: what top_k and top_p keep ends at one word, which is found by counts and masses of 1,024 ranges of
 // logits, first of all of the row, then of the range where the limit lies, until the few words left in it are put in order one by one.  Where the words down to the limit are few altogether (a top_k of
-// 50, a sure model's top_p), one CTA takes them all and is through.
+// 50 or 200, a sure model's top_p), one CTA takes them all and the others leave.
 // Bound by latency and by passes over shared memory, at two CTAs an SM: one row of 128,256 18 us (a barrier of the cluster takes 0.5 to 1, a load 2.5, counts 2, the few words 5), 64 rows of 128,256 28 (no limit), 36
 // (top_k 40) to 85 (top_p 0.9, when thousands of words are kept), 256 of 32,003 26; their bytes take 5.
 #include "lp_common.cuh"
@@ -17,6 +17,7 @@
 namespace lp {
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32, SA_BINS = 2 * SA_THREADS, SA_LIST = 256, SA_MAX_CTAS = 8;
+constexpr int SA_MORE = SA_THREADS;          // words that one CTA finishes with (a list of them takes the place of a SaHist)
 constexpr int SA_MAX_SLICE = 46 * 1024;      // words that a CTA can hold
 typedef unsigned long long u64;
 
@@ -88,6 +89,81 @@ __device__ __forceinline__ T* sa_at(T* mine, int rank) {
   u64 to;
   asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(mine), "r"(rank));
   return reinterpret_cast<T*>(to);
+}
+// A few hundred words (key and index, as in SaList) of which all that can be kept are: top_k (limit, by_count) or the mass that top_p leaves (limit, if not by_count), top_p, min_p and the draw, by one CTA.  They are sorted
+// by their order, cut by sums over it, sorted by their index and drawn by sums over that.  words: SA_MORE (0 behind the last), and behind them room for as many.
+struct SaDraw {
+  double top, unit, power, u;
+  u64 power_bits, w_min;
+  float top_p;
+};
+constexpr u64 SA_AT_512 = 0x4080000000000000ULL;
+__device__ __forceinline__ u64 sa_drawn(double u, u64 all) {      // the word up to which more than this lies
+  const double x = u > 0.0 ? floor(u * (double)all) : 0.0;
+  return x < (double)all ? min((u64)x, all - 1) : all - 1;
+}
+__device__ __forceinline__ u64 sa_mass_limit(float top_p, u64 m) {
+  const double x = ceil((double)top_p * (double)m);
+  return top_p > 0.f && x >= 1.0 ? (u64)x : 1ULL;
+}
+__device__ __forceinline__ u64 sa_upto_lanes(u64 v) {             // the sum of v up to this lane
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += up;
+  }
+  return v;
+}
+// (a warp's pairs up to 32 apart are its own 64 words)
+__device__ __forceinline__ void sa_sort(u64* a, bool down) {
+  for (int k = 2; k <= SA_MORE; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (threadIdx.x < SA_MORE / 2) {
+        const int i = 2 * threadIdx.x - (threadIdx.x & (j - 1));
+        const u64 x = a[i], y = a[i + j];
+        if ((x > y) == (((i & k) == 0) != down)) a[i] = y, a[i + j] = x;
+      }
+      if (j > 32 || (j > 1 ? j >> 1 : k) > 32) __syncthreads();
+      else __syncwarp();
+    }
+  __syncthreads();
+}
+// sum up to this thread, and of all
+__device__ __forceinline__ u64 sa_upto_threads(SaShared& s, u64 v, u64& all) {
+  v = sa_upto_lanes(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 31) s.warp_w[threadIdx.x >> 5] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int k = 0; k < SA_WARPS; ++k) {
+    if (k < (int)(threadIdx.x >> 5)) v += s.warp_w[k];
+    all += s.warp_w[k];
+  }
+  return v;
+}
+__device__ __noinline__ void sa_finish(SaShared& s, u64* words, int n, bool by_count, u64 limit, bool by_mass, const SaDraw& d, long long* out) {
+  u64* values = words + SA_MORE;
+  const int tid = threadIdx.x;
+  sa_sort(words, true);
+  int stay = by_count ? (int)min(limit, (u64)n) : n;
+  u64 word = words[tid], all;
+  const double x = ((double)sa_of_key((unsigned)(word >> 32)) - d.top) * d.unit;
+  if (by_mass) {
+    const u64 v = tid < stay ? sa_weight_bits(x, d.power, s.root) - d.power_bits : 0, before = sa_upto_threads(s, v, all) - v;
+    if (by_count) limit = sa_mass_limit(d.top_p, all);            // (of what top_k has kept)
+    stay = __syncthreads_count(tid < stay && before < limit);
+  }
+  if (tid < stay) {
+    const u64 w = sa_weight_bits(x, 512.0, s.root) - SA_AT_512;
+    values[tid] = w >= d.w_min ? w : 0;
+  }
+  words[tid] = tid < stay ? (u64)(unsigned)~(unsigned)word << 32 | (unsigned)tid : ~0ULL;
+  __syncthreads();
+  sa_sort(words, false);
+  word = words[tid];
+  const u64 w = word != ~0ULL ? values[(unsigned)word] : 0, end = sa_upto_threads(s, w, all), lies = sa_drawn(d.u, all);
+  if (lies >= end - w && lies < end) *out = (long long)(word >> 32);
 }
 struct SaByCount { static constexpr bool value = false; };
 struct SaByMass { static constexpr bool value = true; };
@@ -185,7 +261,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   for (int c = 0; c < CTAS; ++c) hi = fmaxf(hi, s.top[c].x), lo = fminf(lo, s.top[c].y);
 
   // ---- nothing to draw; the largest
-  if (hi == -INFINITY || !(t > 0.f)) {                    // (the same in all CTAs of the cluster)
+  if (hi == -INFINITY || !(t > 0.f) || top_k == 1) {      // (the same in all CTAs of the cluster)
     int best = 0x7fffffff;
     if (hi > -INFINITY)
       for (int i = tid; i < count; i += SA_THREADS)
@@ -210,7 +286,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     __syncthreads();
   }
   const double unit = fmax(1.4426950408889634074 * 64.0 / (double)t, 1e-300), top = (double)hi;
-  constexpr u64 AT_512 = 0x4080000000000000ULL, AT_2_17 = 0x4100000000000000ULL, AT_2_20 = 0x4130000000000000ULL;      // 512, 2^17, 2^20
+  constexpr u64 AT_512 = SA_AT_512, AT_2_17 = 0x4100000000000000ULL, AT_2_20 = 0x4130000000000000ULL;      // 512, 2^17, 2^20
   auto weight_bits = [&](float x) { return sa_weight_bits(((double)x - top) * unit, 512.0, s.root); };
   auto weight = [&](float x) { return weight_bits(x) - AT_512; };
   // four of the warp's words a lane, at a time
@@ -227,23 +303,8 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
   const float least = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
   const u64 w_min = least > 0.f ? (u64)ceil((double)least * 8796093022208.0) : 0;
   const double u = (double)u01;
-  auto drawn = [&](u64 all) -> u64 {                      // the word up to which more than this lies
-    const double x = u > 0.0 ? floor(u * (double)all) : 0.0;
-    return x < (double)all ? min((u64)x, all - 1) : all - 1;
-  };
-  auto mass_limit = [&](u64 m) -> u64 {
-    const double x = ceil((double)top_p * (double)m);
-    return top_p > 0.f && x >= 1.0 ? (u64)x : 1ULL;
-  };
+  auto drawn = [&](u64 all) { return sa_drawn(u, all); };
   int turn = 0;                                           // of s.total
-  auto upto_lanes = [&](u64 v) {                          // the sum of v up to this lane
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 up = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += up;
-    }
-    return v;
-  };
   // The word (by index) up to which more than `limit` of value(i, z_i) lies, by all CTAs; limit = choose(the sum of all).  Returns its index in the one CTA that has it, -1 in the others.
   // value(...) is `base` too large.
   // on(i, z_i): whether a word counts at all.
@@ -260,7 +321,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     auto value = [&](int i, float x) { return on(i, x) ? value_of(x) : base; };
     if (lane == 0) s.warp_w[warp] = sum;
     __syncthreads();
-    const u64 w_upto = upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0), mine = __shfl_sync(0xffffffffu, w_upto, 31);
+    const u64 w_upto = sa_upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0), mine = __shfl_sync(0xffffffffu, w_upto, 31);
     if (tid < CTAS) *sa_at(&s.total[turn][rank], tid) = mine;
     sa_cluster<CTAS>();
     u64 all = 0, before = 0;
@@ -279,11 +340,11 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
     u64 own = 0;
 #pragma unroll 2
     for (int i = i0; i < i1; ++i) own += value(i, z[i]) - base;
-    const u64 run = upto_lanes(own);
+    const u64 run = sa_upto_lanes(own);
     __syncthreads();                                      // (warp_w has been read)
     if (lane == 31) s.warp_w[warp] = run;
     __syncthreads();
-    const u64 upto = upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0);
+    const u64 upto = sa_upto_lanes(lane < SA_WARPS ? s.warp_w[lane] : 0);
     at += run - own + (warp ? __shfl_sync(0xffffffffu, upto, max(warp - 1, 0)) : 0);
     if (limit >= at && limit < at + own)
       for (int i = i0; i < i1; ++i) {
@@ -380,7 +441,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           if (k < warp) upto_n += s.warp_n[k], upto_w += s.warp_w[k];
           all_w += s.warp_w[k];
         }
-        if (first && MASS) limit = mass_limit(all_w);
+        if (first && MASS) limit = sa_mass_limit(top_p, all_w);
         auto look = [&](int b, unsigned in, u64 mass, u64 n_end, u64 w_end) {
           const u64 end = MASS ? w_end : n_end, begin = end - (MASS ? mass : in);
           if (begin < limit && end >= limit) s.bin = b, s.bin_n = in, s.above_n = n_end - in, s.above_w = w_end - mass;
@@ -398,7 +459,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           key_hi = lo_of;
           key_lo = lo_of - key_lo > width ? lo_of - width : key_lo;
         }
-        const bool finish = first && !(MASS && by_count) && above_n + in_bin <= SA_LIST;      // few words down to the limit: all of them are listed
+        const bool finish = first && !(MASS && by_count) && above_n + in_bin <= SA_MORE;      // few words down to the limit: all of them are listed
         const float from_depth = finish ? 0.f : WHOLE + (float)bin, to_depth = WHOLE + (float)bin;
         auto on = [&](float x, int i) { return MASS && by_count ? kept(x, i) : x > -INFINITY; };
         auto inside = [&](float x, int i) {               // of the range (finish: of it and of those above)
@@ -407,9 +468,10 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           return on(x, i) && (first ? d >= from_depth && d <= to_depth : k >= key_lo && k <= key_hi);
         };
         if (finish || in_bin <= SA_LIST) {
+          u64* list_at = finish ? reinterpret_cast<u64*>(&s.hist[1]) : s.list[MASS].word;      // (of the first cut's first level the other counts are not in use)
           auto list = [&](int i, float x) {
-            const int at = atomicAdd(&s.n_list[MASS], 1);      // (below SA_LIST: there are no more words)
-            s.list[MASS].word[at] = (u64)sa_key(x) << 32 | ~(unsigned)(v0 + i);
+            const int at = atomicAdd(&s.n_list[MASS], 1);      // (below SA_LIST, SA_MORE: there are no more words)
+            list_at[at] = (u64)sa_key(x) << 32 | ~(unsigned)(v0 + i);
           };
           auto look_through = [&](auto in) {
             each([&](int i, const float4& x) {
@@ -429,19 +491,23 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
             sa_cluster<CTAS>();                           // (its list has been read)
             return true;
           }
-          int n_all = 0;
+          int n_all = 0, sizes[CTAS];
           u64 word = 0;
-          {
-            int sizes[CTAS];
 #pragma unroll
-            for (int c = 0; c < CTAS; ++c) sizes[c] = *sa_at(&s.n_list[MASS], c);
+          for (int c = 0; c < CTAS; ++c) sizes[c] = *sa_at(&s.n_list[MASS], c);
 #pragma unroll
-            for (int c = 0; c < CTAS; ++c) {
-              if (tid >= n_all && tid < n_all + sizes[c]) word = sa_at(&s.list[MASS], c)->word[tid - n_all];
-              n_all += sizes[c];
-            }
+          for (int c = 0; c < CTAS; ++c) {
+            if (tid >= n_all && tid < n_all + sizes[c]) word = sa_at(list_at, c)[tid - n_all];
+            n_all += sizes[c];
           }
-          if (tid < SA_LIST) s.gathered.word[tid] = word;      // (0 stands behind all words)
+          if (finish && n_all > SA_LIST) {
+            u64* words = reinterpret_cast<u64*>(z);       // (the logits are done with)
+            words[tid] = word;                            // (0 stands behind all words)
+            sa_cluster<CTAS>();
+            sa_finish(s, words, n_all, !MASS, limit, by_mass, SaDraw{top, unit, power, u, power_bits, w_min, top_p}, a.out + row);
+            return true;
+          }
+          if (tid < SA_LIST) s.gathered.word[tid] = word;
           if (finish) sa_cluster<CTAS>();
           __syncthreads();
           // each word counts those before it: by two threads, half of the words each
@@ -468,7 +534,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
           const float x = sa_of_key((unsigned)(word >> 32));
           // of the first SA_LIST threads: the sum of v up to this one
           auto upto = [&](u64 v) {
-            v = upto_lanes(v);
+            v = sa_upto_lanes(v);
             __syncthreads();
             if (lane == 31) s.warp_w[warp] = v;
             __syncthreads();
@@ -486,7 +552,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
             if (is && before_n < stay) s.sorted[before_n] = mass(x);
             __syncthreads();
             const u64 v = tid < SA_LIST ? s.sorted[tid] : 0, end = upto(v);
-            if (!MASS) limit = mass_limit([&] {           // of the mass that top_k has kept
+            if (!MASS) limit = sa_mass_limit(top_p, [&] {           // of the mass that top_k has kept
               u64 all = 0;
 #pragma unroll
               for (int k = 0; k < SA_LIST / 32; ++k) all += s.warp_w[k];
@@ -581,6 +647,7 @@ sample_kernel(const __grid_constant__ SampleArgs a) {
 
 template <typename T, int CTAS>
 static int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
+  static_assert(SA_WARPS * 128 * 4 >= 2 * SA_MORE * (int)sizeof(u64), "the few words' place is that of the least slice");
   const size_t smem = sizeof(SaShared) + (size_t)a.slice * 4;
   LP_CHECK_CUDA((allow_smem<sample_kernel<T, CTAS>>((int)smem)));
   LP_CHECK_CUDA(launch_ex(sample_kernel<T, CTAS>, dim3(rows * CTAS), dim3(SA_THREADS), smem, stream, CTAS, false, a));
