@@ -1068,7 +1068,8 @@ int lp_rotary_append(const lp_rotary_append_desc* desc, void* stream);
  * All bf16, sums in fp32.  D = 64, 96 or 128; T <= LP_PREFIX_MAX_NEW; B T H <= 2^24.  Two forms:
  *   page_table given: k, v are pages as in lp_tree_attention, row j of request b (the prefix's rows counted) lies in its pages; the prefix is read from request 0's, prefix_k and prefix_v are NULL;
  *   page_table NULL: the prefix is prefix_k, prefix_v [prefix][KVH][D], own rows lie in page b (max_pages 1) from its row 0 on.
- * Strides in elements, multiples of 8, the last dimension contiguous, 16-byte aligned bases.  Rows of pages that are not in [0, n_pages) are not seen, nor are rows behind the request's pages.
+ * Strides in elements, multiples of 8, the last dimension contiguous, 16-byte aligned bases.  Rows of pages that are not in [0, n_pages) are not seen, nor are rows behind the request's pages
+ * (2^31 - 512 rows at most, the prefix too).
  * A row that sees nothing is zeros; what a row does not see has no effect on it, NaN and infinities among it.  Rows t >= fresh[b] of out are not written; its rows share
  * no memory with one another nor with the inputs.  workspace: lp_prefix_attention_workspace_bytes(desc) bytes, 16-byte aligned, for this call alone until it has ended. */
 #define LP_PREFIX_MAX_NEW 256
