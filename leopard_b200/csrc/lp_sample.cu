@@ -4,7 +4,9 @@
 //   the first top_k (0: all),  of them those before which less than top_p of their mass lies (the first in any case),  of them those with w >= min_p,
 // and drawn is the first kept word, by index, up to which more than u of the kept mass lies.  t = 0 takes the largest.
 //
-// Weights are integers in units of 2^-43 (from a 64-bit exponential): their sums do not depend on the order in which they are taken, and the draw is the one that 64 bits give.
+// Weights are integers in units of 2^-43 (from a 64-bit exponential): their sums do not depend on the order in which they are taken, and the draw is the one that 64 bits give, but where a sum lies that near a
+// border.  What top_p sums up is in units of 2^-35 (vocabularies above 131,072: 2^-32): of two equal words and others below 2^-36 it takes the first alone at top_p 0.5, where the others' share would let
+// the second in.
 // A cluster of CTAs holds a row in shared memory, read once.  Nothing is sorted: what top_k and top_p keep ends at one word, which is found by counts and masses of 1,024 ranges of
 // logits, first of all of the row, then of the range where the limit lies, until the few words left in it are put in order one by one.  Where the words down to the limit are few altogether (a top_k of
 // 50 or 200, a sure model's top_p), one CTA takes them all and the others leave.

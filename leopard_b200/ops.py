@@ -1044,7 +1044,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     """The next token of each row from given random numbers (lp_sample_tokens): logits fp32 or bf16 [rows, V]; uniform fp32 [rows] in [0, 1).  temperature, top_p, min_p (numbers or fp32 [rows]) and
     top_k (a number or int32 [rows]): of the words in the order of their logits, equal ones by index, the first top_k are kept (0: all), of them those before which less than top_p of their mass
     lies, of them those at least min_p times as likely as the likeliest; drawn is the first kept word, by index, up to which more than `uniform` of the kept mass lies.  temperature 0 takes the largest
-    logit, the first of equal ones.  -> int64 [rows]; -1 for a row of -inf and NaN alone, which are never drawn.  V <= 376832."""
+    logit, the first of equal ones.  -> int64 [rows]; -1 for a row of -inf and NaN alone, which are never drawn.  Weights are held in units
+    of 2^-43 of the largest, for top_p of 2^-35 (V > 131072: 2^-32).  V <= 376832."""
     try:
         R, V = logits.shape
         dev, kind, ld = logits.device, logits.dtype, logits.stride(0)
