@@ -152,9 +152,22 @@ __device__ __forceinline__ void pa_ctas_of(const PrefixArgs& a, const PrefixLine
   c0 = pa_cta_of(a, l, (long long)item * a.pre_tiles);
   c1 = pa_cta_of(a, l, (long long)(item + 1) * a.pre_tiles - 1);
 }
+__device__ __forceinline__ int pa_item(const PrefixArgs& a, int blk, int kvh) { return blk * a.d.KVH + kvh; }
+// the prefix's pieces for row r of the list: how many, the first one's place, the row's in their block
+__device__ __forceinline__ void pa_pieces_of(const PrefixArgs& a, int rows, int kvh, int r, int& n, long long& slot, int& in) {
+  n = in = 0;
+  slot = 0;
+  if (!a.pre_ctas) return;
+  const PrefixLine line = pa_line(a, rows);
+  const int blk = r / a.pre_rows, item = pa_item(a, blk, kvh);
+  int c0, c1;
+  pa_ctas_of(a, line, item, c0, c1);
+  in = r - blk * a.pre_rows;
+  n = c1 - c0 + 1;
+  slot = (long long)item + c0;
+}
 // a CTA's piece of an item
 struct PrefixPiece { int item, kvh, r0, t0, n; };
-__device__ __forceinline__ int pa_item(const PrefixArgs& a, int blk, int kvh) { return blk * a.d.KVH + kvh; }
 __device__ __forceinline__ PrefixPiece pa_piece(const PrefixArgs& a, long long u, long long u_end) {
   PrefixPiece p;
   p.item = (int)(u / a.pre_tiles);
