@@ -542,6 +542,12 @@ static size_t prefix_plan(const lp_prefix_attn_desc* d, PrefixArgs& a) {
     } else {
       const long long left = a.own_slots < room / 2 ? room - a.own_slots : room / 2;      // (at once with the own rows')
       splits = pre_items >= left ? 1 : left / pre_items;
+      // pieces of more than 12 tiles become such of 8, as long as all of them are half as many again as the CTAs that run at once: the longest piece is what a call waits for (us a call, without and so: 64 samples after
+      // 1,200 rows 45 and 31, two prompts of 32 after 1,000 37 and 25, 16 samples after 4,900 35 and 32; with 600 rows of their own 32 after 2,400 39 and 43, 64 after 1,200 47 both)
+      if ((a.pre_tiles + splits - 1) / splits > 12) {
+        const long long most = room * 3 / 2 / pre_items, fine = (a.pre_tiles + 7) / 8, more = fine < most ? fine : most;
+        if (more > splits) splits = more;
+      }
       a.pre_ctas = (int)((splits < a.pre_tiles ? splits : a.pre_tiles) * pre_items);
     }
     a.pre_slots = pre_items + a.pre_ctas;
