@@ -507,8 +507,8 @@ static int prefix_check(const lp_prefix_attn_desc* d) {
   return 0;
 }
 // Whether the prefix goes to the tcgen05 kernel: it costs a launch and 10 us of start and end, the other reads the prefix once for every 16 rows.  Decided by blocks of 16 rows x key heads x keys, of more than 8 rows.
-// mma.sync and tcgen05, us a call, 64 own rows a request, 32 heads over 8 (16 over 16): 16 rows after 4,796 22.5 and 28.7 (26.6, 32.8), after 20,000 34.8 and 36.9 (59.4, 53.2), after 100,003 92 and 86 (233, 150);
-// 32 rows after 512 18.4 and 22.5 (20.5, 26.6), after 4,796 26.6 and 32.8 (36.8, 34.8), after 20,000 49 and 43 (107, 53), after 100,003 182 and 92; 64 rows after 4,796 34.8 both (57, 37), after 20,000 100 and 45.
+// mma.sync and tcgen05, us a call, 60 own rows a request, at 180,000 of these: 32 rows of 32 heads over 8 after 11,250 34.8 and 32.8, 64 after 5,625 32.8 and 30.7, 256 after 1,406 32.8 and 28.7, 32 of 16 heads over 16 after
+// 5,625 34.9 and 34.8, 256 of 8 over 1 after 5,625 26.6 and 24.6, 192 of 12 over 4 (64 dimensions) after 3,750 20.5 and 24.6; at 270,000 47 - 53 and 31 - 39 (the last one 30.7 and 27.5).  Below 8 x 10^4 tcgen05's is 4 - 6 us behind.
 // Up to 8 rows read it once in any case: 8 after 100,003 84 and 84 (160, 154).
 constexpr long long PA_TC_WORK = 160000;
 static bool prefix_tc(const lp_prefix_attn_desc* d) {
