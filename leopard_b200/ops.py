@@ -942,8 +942,10 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
                 raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
     if q_out is None:
         q_out = torch.empty((rows, H, D), dtype=kind, device=dev)
-    if rows == 0 or D == 0 or k_pool.numel() == 0:
+    if rows == 0 or D == 0:
         return q_out
+    if k_pool.numel() == 0:      # no slot is one of its rows: the queries are turned all the same
+        return rotary(q, positions, inv_freq, layout, scale, out=q_out)
     o = q_out.stride()
     d = _lib.RotaryAppendDesc(q.data_ptr(), s[0], s[1], q_out.data_ptr(), o[0], o[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], k_pool.data_ptr(), kp[0], kp[1], kp[2],
                               v_pool.data_ptr(), vp[0], vp[1], vp[2], positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), 1 if positions.dtype is _I64 else 0, n,
