@@ -1038,7 +1038,9 @@ int lp_distill_fwd_bwd(const void* logits, int logits_fp32, long long ld, const 
 /* Request b has lengths[b] cached rows and brings fresh[b] tokens (0: it waits; negative numbers count as 0), whose rows stand one request after the other: row0[b]
  * [B + 1] is its first.  Entries of its new rows' pages in page_table [B][ld] (int32, max_pages a request) that are negative get free_pages[used[0]], free_pages[used[0] + 1], ... in the order of
  * requests and pages, and used[0] grows by their number; when the list is over they stay as they were.  Row r < `rows`: row_seq[r] its request, row_pos[r] its position, slots[r] =
- * page * page_size + row of the page, -1 where it has no page; all three -1 behind the last row.  Rows that do not fit into `rows` have pages but no entries. */
+ * page * page_size + row of the page, -1 where it has no page; all three -1 behind the last row.  Rows that do not fit into `rows` have pages but no entries.
+ * Entries that are not negative stay, whoever else holds these pages: requests with the same page behind their rows get the same slots in it, so whole pages can be shared, and a page that a shared prompt ends in is
+ * copied for each request before (lp_cache_copy_pages). */
 int lp_step_tables(const int* lengths, const int* fresh, int* page_table, long long ld_table, int max_pages, int page_size, const int* free_pages, int n_free, int* used, int B, int rows,
                    int* row_seq, int* row_pos, long long* slots, int* row0, void* stream);
 

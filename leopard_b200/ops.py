@@ -824,6 +824,8 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     """The index tables of a step whose requests bring tokens, and the cache pages that these need (lp_step_tables): lengths int32 [B], cached rows; new int32 [B], tokens that each
     brings (0: none); page_table int32 [B, max_pages] (negative: no page yet), which gets pages for the new rows, in place, from free int32 [n], of which used int32 [1] have been given
     before (it grows; when the list is over, entries stay negative); rows: how many rows the step has room for.
+    Entries that are pages already stay, whoever else holds them: a page that a shared prompt ends in has to be copied for each request before its first step (cache_copy_pages), or the requests get the
+    same slots.
     -> (row_seq int32 [rows], row_pos int32 [rows], slots int64 [rows] = page * page_size + row of the page; row0 int32 [B + 1], each request's first row).  Rows that no request has are -1 in all
     three, rows without a page in slots."""
     try:
@@ -986,8 +988,8 @@ def _prefix_refusals(q, k, v, lengths, prefix, new, page_table, prefix_k, prefix
 def prefix_attention(q, k, v, lengths, prefix, new=None, page_table=None, prefix_k=None, prefix_v=None, scale=None, out=None):
     """Attention of a batch whose requests share their first `prefix` rows, which are read once for all of them (lp_prefix_attention): q bf16 [B, T, H, D], the requests' new tokens; lengths int32 [B], rows
     of each before these, the prefix among them; new int32 [B] or None (T), tokens that each brings, whose keys and values are the cache's next rows already (rotary_append): token t sees the prefix and its
-    request's rows up to its own.  With page_table int32 [B, max_pages]: k, v bf16 [pages, page_size, KVH, D] and each request's whole sequence in its pages (SequenceCache.fork shares them), the prefix
-    read from those of request 0.  Without: own rows in k, v [B, rows, KVH, D], from row 0 on, the prefix in prefix_k, prefix_v [prefix, KVH, D].  Strides are free but for a contiguous last
+    request's rows up to its own.  With page_table int32 [B, max_pages]: k, v bf16 [pages, page_size, KVH, D] and each request's whole sequence in its pages (tables that begin with the same pages share
+    them; a page that the prefix ends in is each request's own), the prefix read from those of request 0.  Without: own rows in k, v [B, rows, KVH, D], from row 0 on, the prefix in prefix_k, prefix_v [prefix, KVH, D].  Strides are free but for a contiguous last
     dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of tokens that a request does not bring stay as they were (`out` given; its rows share no memory, and its span meets none of the
     inputs) or are unspecified.  A token that sees nothing is zeros.  T <= 256."""
     try:

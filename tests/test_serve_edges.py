@@ -1,9 +1,15 @@
-"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page."""
+"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page."""
+import textwrap
+from pathlib import Path
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from leopard_b200 import _lib, ops
+from leopard_b200 import ops
 from oracle import serve as O
+from test_serve_ops import close
+from test_serve_run import DEFINITIONS
 
 gpu = pytest.mark.gpu
 BF16, F32, I32, I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
@@ -38,3 +44,72 @@ def test_queries_are_turned_though_the_pool_has_no_rows(pages, size, G, dtype, l
     with pytest.raises(ValueError, match="layout"):
         ops.rotary_append(q, k, v, *rest, layout="pairs")
     assert ops.rotary_append(q[:0], k[:0], v[:0], pos[:0], freq, *pools, slots[:0]).shape == (0, H, D)
+
+
+# ------------------------------------------------------------------------------------------------------------ a shared prompt, as the README has it
+def readme_steps():
+    """the README's lines for a shared prompt -> (those of the prompt, those of a step)"""
+    text = (Path(__file__).resolve().parents[1] / "README.md").read_text()
+    text = text[text.index("## Serving many continuations of one prompt"):]
+    code = textwrap.dedent("\n".join(line for line in text.splitlines() if line.startswith("    ")))
+    cut = code.index("# once a step")
+    return code[:cut], code[cut:]
+
+
+def by_readme(device, ops, prefix, page_size):
+    """Requests that share a prompt's pages by their tables bring a few tokens each, some wait: after each step every request's sequence is in its pages, the prompt's rows and then its own, which nobody else has
+    written over, and what it attends to is that sequence."""
+    setup, step = readme_steps()
+    B, H, G, D, max_pages, n_pages = 5, 8, 2, 64, -(-(prefix + 9) // page_size), 90      # (9 tokens at most behind the prompt)
+    g = gen(prefix, "cpu")
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF16).to(device)  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=I32, device=device)  # noqa: E731
+    k_pages, v_pages = (torch.full((n_pages, page_size, G, D), float("nan"), dtype=BF16, device=device) for _ in range(2))
+    order = torch.randperm(n_pages, generator=g).to(I32).to(device)
+    n = -(-prefix // page_size)
+    freq = (10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))).float().to(device)
+    ns = {"torch": torch, "ops": ops, "B": B, "max_pages": max_pages, "prefix": prefix, "page_size": page_size, "prompt_pages": order[:n].clone(), "k_pages": k_pages, "v_pages": v_pages,
+          "free_pages": order[n:].clone(), "used": i32([3]), "inv_freq": freq, "lengths": i32([prefix] * B)}
+    prompt = [rnd(prefix, G, D) for _ in range(2)]
+    for i in range(prefix):
+        for pool, x in zip((k_pages, v_pages), prompt):
+            pool[int(order[i // page_size]), i % page_size] = x[i]
+    seqs = [[(prompt[0][i].double(), 2.0 ** -20, prompt[1][i]) for i in range(prefix)] for _ in range(B)]      # key, what it may be off by, value
+    exec(setup, ns)
+    for new in ([3, 0, 1, 4, 2], [1, 1, 0, 1, 1], [4, 4, 4, 4, 4]):
+        rows, T = -(-sum(new) // 8) * 8, max(new)
+        before = ns["lengths"].clone()
+        k, v = rnd(rows, G, D), rnd(rows, G, D)
+        logits, u = torch.randn(B, 40, generator=g).to(device), torch.rand(B, generator=g).to(device)
+        ns.update(new=i32(new), rows=rows, T=T, q=rnd(rows, H, D), k=k, v=v, logits=logits, uniform=u)
+        exec(step, ns)
+        r = 0
+        for b, t in enumerate(new):
+            for i in range(t):
+                turned, _ = O.rotary(k[r:r + 1], torch.tensor([len(seqs[b])], device=device), freq)
+                seqs[b].append((turned[0], 2.0 ** -8 * turned[0].abs() + 2.0 ** -18 * k[r].double().abs().amax(), v[r]))      # half a step; angles of fp32
+                r += 1
+        slots = ns["slots"][:r].tolist()
+        assert min(slots) >= 0 and len(set(slots)) == r and ns["slots"][r:].tolist() == [-1] * (rows - r)
+        assert ns["lengths"].tolist() == [len(s) for s in seqs]
+        for b, s in enumerate(seqs):
+            at = torch.arange(len(s), device=device)
+            where = (ns["page_table"][b, at // page_size].long(), at % page_size)
+            for i, (key, off, value) in enumerate(s):
+                assert bool(((k_pages[where][i].double() - key).abs() <= off).all()) and torch.equal(v_pages[where][i], value), (b, i)
+        close(ns["out"], {"q": ns["q"][ns["at"]], "k": k_pages.nan_to_num(0.0), "v": v_pages.nan_to_num(0.0), "lengths": before, "prefix": prefix, "new": ns["new"], "page_table": ns["page_table"],
+                          "prefix_k": None, "prefix_v": None})
+        assert ns["token"].tolist() == O.sample_tokens(logits, u, temperature=0.8, top_k=50, top_p=0.95)
+
+
+@pytest.mark.parametrize("prefix, page_size", [(37, 16), (32, 16), (5, 8), (3, 1)])
+def test_the_readme_serves_a_shared_prompt_by_the_definitions(prefix, page_size):
+    tables, append, attend, draw, copy_pages = DEFINITIONS
+    by_readme("cpu", SimpleNamespace(step_tables=tables, rotary_append=append, sample_tokens=draw, cache_copy_pages=copy_pages,
+                                     prefix_attention=lambda q, k, v, lengths, P, new, page_table: attend(q, k, v, lengths, P, new, page_table)), prefix, page_size)
+
+
+@gpu
+@pytest.mark.parametrize("prefix, page_size", [(37, 16), (32, 16), (5, 8), (3, 1), (515, 64)])
+def test_the_readme_serves_a_shared_prompt(prefix, page_size):
+    by_readme("cuda", ops, prefix, page_size)
