@@ -32,10 +32,10 @@ def cmd_models(args) -> int:
 def cmd_generate(args) -> int:
     from .sampling import SamplingParams
     from .scheduler import generate
+    sampling = SamplingParams(temperature=args.temperature, top_k=args.top_k, seed=args.seed, top_p=args.top_p, min_p=args.min_p)
     eng = _load(args)
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in args.prompt]
-    outs = generate(eng, prompts, max_new_tokens=args.max_new_tokens, eos=set(args.eos or ()),
-                    sampling=SamplingParams(temperature=args.temperature, top_k=args.top_k, seed=args.seed, top_p=args.top_p, min_p=args.min_p))
+    outs = generate(eng, prompts, max_new_tokens=args.max_new_tokens, eos=set(args.eos or ()), sampling=sampling)
     for p, o in zip(prompts, outs):
         print(json.dumps({"prompt": p, "output": o}))
     return 0

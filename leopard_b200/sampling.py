@@ -20,6 +20,13 @@ class SamplingParams:
     top_p: float = 1.0             # the likeliest words, before which less than this share of the mass lies (1: all)
     min_p: float = 0.0             # words at least this many times as likely as the likeliest (0: all)
 
+    def __post_init__(self):
+        # before a prompt has run and holds pages (what is not a number fails both)
+        if not 0.0 < self.top_p <= 1.0:
+            raise ValueError(f"top_p must be above 0 and 1 at most, got {self.top_p}")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError(f"min_p must be from 0 to 1, got {self.min_p}")
+
 
 class Sampler:
     def __init__(self, params: Optional[SamplingParams] = None):

@@ -1,4 +1,4 @@
-"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page."""
+"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range."""
 import textwrap
 from pathlib import Path
 from types import SimpleNamespace
@@ -6,7 +6,8 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from leopard_b200 import ops
+from leopard_b200 import cli, ops
+from leopard_b200.sampling import SamplingParams
 from oracle import serve as O
 from test_serve_ops import close
 from test_serve_run import DEFINITIONS
@@ -113,3 +114,20 @@ def test_the_readme_serves_a_shared_prompt_by_the_definitions(prefix, page_size)
 @pytest.mark.parametrize("prefix, page_size", [(37, 16), (32, 16), (5, 8), (3, 1), (515, 64)])
 def test_the_readme_serves_a_shared_prompt(prefix, page_size):
     by_readme("cuda", ops, prefix, page_size)
+
+
+# ------------------------------------------------------------------------------------------------------------ the sampler
+@pytest.mark.parametrize("option, value", [("top_p", 1.5), ("top_p", 0.0), ("top_p", -0.5), ("top_p", float("nan")), ("min_p", 2.0), ("min_p", -0.1), ("min_p", float("nan"))])
+def test_settings_out_of_range_are_refused_before_a_prompt_runs(monkeypatch, option, value):
+    with pytest.raises(ValueError, match=option):
+        SamplingParams(temperature=0.8, **{option: value})
+    with pytest.raises(ValueError, match=option):
+        SamplingParams(temperature=0.8, **{"min_p": 0.1, "top_p": 0.9, option: value})
+    monkeypatch.setattr(cli, "_load", lambda args: pytest.fail("the model was loaded"))
+    with pytest.raises(ValueError, match=option):
+        cli.main(["generate", "--model", "m", "--prompt", "1,2", "--temperature", "0.8", f"--{option.replace('_', '-')}={value}"])
+
+
+def test_settings_at_the_ends_of_their_ranges_are_taken():
+    for kw in (dict(), dict(top_p=1.0, min_p=0.0), dict(top_p=1, min_p=1), dict(top_p=1e-9, min_p=1.0)):
+        assert SamplingParams(temperature=0.8, **kw).min_p == kw.get("min_p", 0.0)
