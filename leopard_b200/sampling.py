@@ -15,10 +15,10 @@ from . import ops
 @dataclass
 class SamplingParams:
     temperature: float = 0.0       # 0: greedy
-    top_k: int = 0                 # 0: the whole vocabulary
+    top_k: int = 0                 # the likeliest words, and all that are equal to the last of them (0: the whole vocabulary)
     seed: Optional[int] = None
-    top_p: float = 1.0             # the likeliest words, before which less than this share of the mass lies (1: all)
-    min_p: float = 0.0             # words at least this many times as likely as the likeliest (0: all)
+    top_p: float = 1.0             # of these the likeliest, before which less than this share of the mass lies (1: all)
+    min_p: float = 0.0             # of these words at least this many times as likely as the likeliest (0: all)
 
     def __post_init__(self):
         # before a prompt has run and holds pages (what is not a number fails both)
@@ -42,10 +42,10 @@ class Sampler:
             self._gen = torch.Generator(device=logits.device)
             if p.seed is not None:
                 self._gen.manual_seed(p.seed)
+        if 0 < p.top_k < logits.shape[-1]:
+            # All words equal to the k-th stay, whatever else is set; ops.sample_tokens takes them by index, exactly top_k (and 20 us for a row of 128,256 where this takes 137, 42 and 270 for 64).
+            z = logits / p.temperature
+            logits = logits.masked_fill(z < z.topk(p.top_k, -1).values[:, -1:], float("-inf"))
         if p.top_p < 1.0 or p.min_p > 0.0:
-            return ops.sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device, generator=self._gen), p.temperature, max(p.top_k, 0), p.top_p, p.min_p)
-        z = logits / p.temperature
-        if p.top_k > 0 and p.top_k < z.shape[-1]:
-            kth = z.topk(p.top_k, -1).values[:, -1:]
-            z = z.masked_fill(z < kth, float("-inf"))
-        return torch.multinomial(torch.softmax(z, -1), 1, generator=self._gen).squeeze(-1)
+            return ops.sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device, generator=self._gen), p.temperature, 0, p.top_p, p.min_p)
+        return torch.multinomial(torch.softmax(logits / p.temperature, -1), 1, generator=self._gen).squeeze(-1)

@@ -1,4 +1,4 @@
-"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range."""
+"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range, words equal to the last that top_k keeps."""
 import textwrap
 from pathlib import Path
 from types import SimpleNamespace
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from leopard_b200 import cli, ops
-from leopard_b200.sampling import SamplingParams
+from leopard_b200.sampling import Sampler, SamplingParams
 from oracle import serve as O
 from test_serve_ops import close
 from test_serve_run import DEFINITIONS
@@ -131,3 +131,17 @@ def test_settings_out_of_range_are_refused_before_a_prompt_runs(monkeypatch, opt
 def test_settings_at_the_ends_of_their_ranges_are_taken():
     for kw in (dict(), dict(top_p=1.0, min_p=0.0), dict(top_p=1, min_p=1), dict(top_p=1e-9, min_p=1.0)):
         assert SamplingParams(temperature=0.8, **kw).min_p == kw.get("min_p", 0.0)
+
+
+def keeps_the_same_words(device):
+    """logits of few steps, so that many words are equal to the k-th: the draws come from the words that top_k alone keeps, and all of these come up"""
+    z = torch.tensor([0.5, 2.0, 1.0, 1.0, 2.0, 0.5, 1.0, -3.0, 1.0], device=device).expand(4000, 9).contiguous()
+    for top_k, words in ((1, {1, 4}), (2, {1, 4}), (3, {1, 2, 3, 4, 6, 8}), (6, {1, 2, 3, 4, 6, 8}), (7, {0, 1, 2, 3, 4, 5, 6, 8}), (8, {0, 1, 2, 3, 4, 5, 6, 8}), (9, set(range(9))), (0, set(range(9)))):
+        for kw in (dict(), dict(top_p=0.999999), dict(min_p=1e-6), dict(top_p=0.999999, min_p=1e-6)):      # (the least likely word has 1.5 % of the mass)
+            drawn = Sampler(SamplingParams(temperature=2.0, top_k=top_k, seed=3, **kw))(z)
+            assert set(drawn.tolist()) == words, (top_k, kw)
+
+
+@gpu
+def test_top_k_keeps_the_same_words_with_other_settings_and_without():
+    keeps_the_same_words("cuda")
