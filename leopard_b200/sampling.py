@@ -28,6 +28,19 @@ class SamplingParams:
             raise ValueError(f"min_p must be from 0 to 1, got {self.min_p}")
 
 
+def _draw(logits, u, temperature, top_p, min_p):
+    """What ops.sample_tokens draws, for logits that are not on a GPU (the engines of the CPU backend): in 64 bits, from the words in their order."""
+    t, top_p, min_p = torch.tensor([temperature, top_p, min_p], dtype=torch.float32).double()      # (settings come in 32 bits)
+    z = logits.double()
+    z = torch.where(z.isnan(), -torch.inf, z)
+    z, order = torch.sort(z, dim=-1, descending=True, stable=True)
+    top = z[:, :1]
+    w = torch.where(z == top, 1.0, torch.exp((z - top) / t)).masked_fill(z == -torch.inf, 0.0)     # (beside an infinite one nothing counts)
+    keep = (w.cumsum(-1) - w < top_p * w.sum(-1, keepdim=True)) & (w >= min_p)
+    upto = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0.0)).cumsum(-1)
+    return torch.where(top[:, 0] > -torch.inf, (upto > u.double()[:, None] * upto[:, -1:]).int().argmax(-1), -1)
+
+
 class Sampler:
     def __init__(self, params: Optional[SamplingParams] = None):
         self.p = params or SamplingParams()
@@ -47,5 +60,7 @@ class Sampler:
             z = logits / p.temperature
             logits = logits.masked_fill(z < z.topk(p.top_k, -1).values[:, -1:], float("-inf"))
         if p.top_p < 1.0 or p.min_p > 0.0:
-            return ops.sample_tokens(logits, torch.rand(logits.shape[0], device=logits.device, generator=self._gen), p.temperature, 0, p.top_p, p.min_p)
+            u = torch.rand(logits.shape[0], device=logits.device, generator=self._gen)
+            draw = ops.sample_tokens if logits.is_cuda else _draw
+            return draw(logits, u, temperature=p.temperature, top_p=p.top_p, min_p=p.min_p)
         return torch.multinomial(torch.softmax(logits / p.temperature, -1), 1, generator=self._gen).squeeze(-1)

@@ -1,4 +1,5 @@
-"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range, words equal to the last that top_k keeps."""
+"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range, words equal to the last that top_k keeps, draws without a GPU."""
+import json
 import textwrap
 from pathlib import Path
 from types import SimpleNamespace
@@ -145,3 +146,48 @@ def keeps_the_same_words(device):
 @gpu
 def test_top_k_keeps_the_same_words_with_other_settings_and_without():
     keeps_the_same_words("cuda")
+
+
+# ------------------------------------------------------------------------------------------------------------ the sampler without a GPU
+def test_top_k_keeps_the_same_words_without_a_gpu():
+    keeps_the_same_words("cpu")
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.8), dict(min_p=0.1), dict(top_p=0.95, min_p=0.02), dict(top_p=1e-6), dict(min_p=1.0), dict(top_p=0.999, temperature=3.0), dict(top_k=20, top_p=0.9)])
+@pytest.mark.parametrize("V", [1, 7, 700])
+def test_the_sampler_draws_by_the_definition_without_a_gpu(kw, V):
+    z = torch.randn(40, V, generator=gen(V, "cpu")) * 2
+    z[3] = -torch.inf
+    z[4, V // 2:] = float("nan")
+    z[5, ::3] = torch.inf
+    z[6, :] = 0.25
+    kw = {"temperature": 0.9, **kw}
+    rows = [r for r in range(40) if "top_k" not in kw or r not in (4, 5, 6)]      # (numbers that are none, and more than 20 equal ones: the sampler's top_k is another than the draw's)
+    got = Sampler(SamplingParams(seed=11, **kw))(z)
+    want = O.sample_tokens(z, torch.rand(40, generator=gen(11, "cpu")), **kw)
+    assert got.dtype == I64 and [got.tolist()[r] for r in rows] == [want[r] for r in rows]
+
+
+class FewWords:
+    """an engine whose logits are numbers of its own"""
+    def __init__(self):
+        self.g = gen(9, "cpu")
+
+    def step(self, entries):
+        return torch.randn(len(entries), 50, generator=self.g)
+
+    def finish(self, key):
+        pass
+
+
+def test_the_command_line_draws_with_its_settings(monkeypatch, capsys):
+    """generate's options reach the draw: the same engine's logits, drawn by the definition"""
+    monkeypatch.setattr(cli, "_load", lambda args: FewWords())
+    assert cli.main(["generate", "--model", "m", "--prompt", "1,2", "--prompt", "3", "--max-new-tokens", "4", "--temperature", "0.8", "--top-p", "0.7", "--min-p", "0.05", "--seed", "5"]) == 0
+    printed = [json.loads(line) for line in capsys.readouterr().out.splitlines()]
+    eng, numbers, want = FewWords(), gen(5, "cpu"), [[], []]
+    for _ in range(4):
+        drawn = O.sample_tokens(eng.step([0, 1]), torch.rand(2, generator=numbers), temperature=0.8, top_p=0.7, min_p=0.05)
+        for o, t in zip(want, drawn):
+            o.append(t)
+    assert printed == [{"prompt": [1, 2], "output": want[0]}, {"prompt": [3], "output": want[1]}]
