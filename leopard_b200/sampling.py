@@ -62,5 +62,5 @@ class Sampler:
         if p.top_p < 1.0 or p.min_p > 0.0:
             u = torch.rand(logits.shape[0], device=logits.device, generator=self._gen)
             draw = ops.sample_tokens if logits.is_cuda else _draw
-            return draw(logits, u, temperature=p.temperature, top_p=p.top_p, min_p=p.min_p)
+            return draw(logits, u, temperature=p.temperature, top_p=max(p.top_p, 1e-30), min_p=p.min_p)      # (top_p goes there in 32 bits)
         return torch.multinomial(torch.softmax(logits / p.temperature, -1), 1, generator=self._gen).squeeze(-1)

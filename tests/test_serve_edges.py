@@ -191,3 +191,19 @@ def test_the_command_line_draws_with_its_settings(monkeypatch, capsys):
         for o, t in zip(want, drawn):
             o.append(t)
     assert printed == [{"prompt": [1, 2], "output": want[0]}, {"prompt": [3], "output": want[1]}]
+
+
+def least_top_p(device):
+    """a top_p that is 0 in 32 bits keeps the likeliest word, as all below its share of the mass do"""
+    z = torch.randn(30, 300, generator=gen(2, "cpu")).to(device)
+    for top_p in (1e-50, 1e-45, 1e-30, 1e-9):
+        assert torch.equal(Sampler(SamplingParams(temperature=1.0, top_p=top_p, seed=1))(z), z.argmax(-1))
+
+
+def test_the_least_top_p_without_a_gpu():
+    least_top_p("cpu")
+
+
+@gpu
+def test_the_least_top_p():
+    least_top_p("cuda")
