@@ -820,6 +820,16 @@ def distill_fwd_bwd(logits, ids, teacher, weight, vocab, temperature=1.0, target
 
 # ---- serving many continuations of one prompt (csrc/lp_serve.cu, lp_sample.cu, lp_prefixattn.cu): a step's tables and pages, rotary positions and cache rows, attention over a prefix
 # that the batch shares, the next tokens ----------------------------------------------------------------------------------------------------------------------------------------------
+_MOST = 2 ** 31 - 1      # the entry points' whole numbers have 32 bits, of which ctypes would take the low ones of a larger one
+
+
+def _whole(x, name):
+    x = int(x)
+    if not -_MOST <= x <= _MOST:
+        raise ValueError(f"{name} must be a whole number of 32 bits, got {x}")
+    return x
+
+
 def step_tables(lengths, new, page_table, free, used, page_size, rows):
     """The index tables of a step whose requests bring tokens, and the cache pages that these need (lp_step_tables): lengths int32 [B], cached rows; new int32 [B], tokens that each
     brings (0: none); page_table int32 [B, max_pages] (negative: no page yet), which gets pages for the new rows, in place, from free int32 [n], of which used int32 [1] have been given
@@ -842,7 +852,7 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
             _need(t, n, (_I32,), 1, shape, lengths.device, contiguous=True)
         _need(page_table, "page_table", (_I32,), 2, (lengths.shape[0], page_table.shape[-1]), lengths.device, rows=True)
         raise ValueError("step_tables: the tables must be contiguous in their rows")
-    rows, n_free, ld = int(rows), free.shape[0], page_table.stride(0)
+    rows, page_size, n_free, ld = _whole(rows, "rows"), _whole(page_size, "page_size"), free.shape[0], page_table.stride(0)
     if rows < 0:
         raise ValueError(f"rows must not be negative, got {rows}")
     slots, seq, pos, row0 = torch.empty((4 * rows + B + 1,), dtype=_I32, device=dev).split((2 * rows, rows, rows, B + 1))      # (one allocation: four take 2.4 us longer)
@@ -850,7 +860,7 @@ def step_tables(lengths, new, page_table, free, used, page_size, rows):
     if B == 0:
         return seq.fill_(-1), pos.fill_(-1), slots.fill_(-1), row0.zero_()
     L = _lib.lib()
-    _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), ld, max_pages, int(page_size), free.data_ptr(), n_free, used.data_ptr(), B, rows,
+    _call(dev, L, "lp_step_tables", L.lp_step_tables, lengths.data_ptr(), new.data_ptr(), page_table.data_ptr(), ld, max_pages, page_size, free.data_ptr(), n_free, used.data_ptr(), B, rows,
           seq.data_ptr(), pos.data_ptr(), slots.data_ptr(), row0.data_ptr())
     return seq, pos, slots, row0
 
@@ -868,6 +878,7 @@ def _rotary_layout(layout):
 
 
 def _rotary_rows(positions, inv_freq, rows, D, dev):
+    _whole(rows, "the number of rows")
     _need(positions, "positions", (_I32, _I64), 1, (rows,), dev, contiguous=True)
     _need(inv_freq, "inv_freq", (_F32,), 1, device=dev, contiguous=True)
     if 2 * inv_freq.numel() > D:
@@ -882,7 +893,7 @@ def rotary(x, positions, inv_freq, layout="half", scale=1.0, inverse=False, out=
         rows, heads, D = x.shape
         dev, kind, n = x.device, x.dtype, inv_freq.shape[0]
         xs = x.stride()
-        fine = (x.is_cuda and (kind is _BF16 or kind is _F32) and (xs[2] == 1 or D <= 1) and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,)
+        fine = (x.is_cuda and rows <= _MOST and (kind is _BF16 or kind is _F32) and (xs[2] == 1 or D <= 1) and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,)
                 and positions.is_contiguous() and positions.device == dev and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D
                 and (out is None or (out.dtype is kind and out.shape == x.shape and out.device == dev and (out.stride(2) == 1 or D <= 1))))
     except (AttributeError, ValueError, IndexError):
@@ -917,7 +928,7 @@ def rotary_append(q, k, v, positions, inv_freq, k_pool, v_pool, slots, layout="h
         rows, H, D = q.shape
         dev, kind, n, G = q.device, q.dtype, inv_freq.shape[0], k.shape[1]
         s, ks, vs, kp, vp = q.stride(), k.stride(), v.stride(), k_pool.stride(), v_pool.stride()
-        fine = (q.is_cuda and (kind is _BF16 or kind is _F32) and k.dtype is kind and v.dtype is kind and k_pool.dtype is kind and v_pool.dtype is kind and s[2] == ks[2] == vs[2] == kp[3] == vp[3] == 1
+        fine = (q.is_cuda and rows <= _MOST and (kind is _BF16 or kind is _F32) and k.dtype is kind and v.dtype is kind and k_pool.dtype is kind and v_pool.dtype is kind and s[2] == ks[2] == vs[2] == kp[3] == vp[3] == 1
                 and k.shape == (rows, G, D) and v.shape == (rows, G, D) and k_pool.shape[2:] == (G, D) and v_pool.shape == k_pool.shape and k.device == dev and v.device == dev and k_pool.device == dev
                 and v_pool.device == dev and (positions.dtype is _I32 or positions.dtype is _I64) and positions.shape == (rows,) and positions.is_contiguous() and positions.device == dev
                 and inv_freq.dtype is _F32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev and 2 * n <= D and slots.dtype is _I64 and slots.shape == (rows,)
@@ -992,10 +1003,11 @@ def prefix_attention(q, k, v, lengths, prefix, new=None, page_table=None, prefix
     them; a page that the prefix ends in is each request's own), the prefix read from those of request 0.  Without: own rows in k, v [B, rows, KVH, D], from row 0 on, the prefix in prefix_k, prefix_v [prefix, KVH, D].  Strides are free but for a contiguous last
     dimension and multiples of 8.  -> out bf16 [B, T, H, D]; rows of tokens that a request does not bring stay as they were (`out` given; its rows share no memory, and its span meets none of the
     inputs) or are unspecified.  A token that sees nothing is zeros.  T <= 256."""
+    prefix = _whole(prefix, "prefix")
     try:
         B, T, H, D = q.shape
         P, S, G, Dk = k.shape
-        dev, prefix = q.device, int(prefix)
+        dev = q.device
         fine = (q.is_cuda and q.dtype is _BF16 and k.dtype is _BF16 and v.dtype is _BF16 and Dk == D and v.shape == k.shape and k.device == dev and v.device == dev
                 and lengths.dtype is _I32 and lengths.device == dev and lengths.shape == (B,) and lengths.is_contiguous())
         qs, ks, vs = q.stride(), k.stride(), v.stride()
@@ -1041,7 +1053,7 @@ def _setting(x, name, dtype, rows, dev):
     if isinstance(x, torch.Tensor):
         _need(x, name, (dtype,), 1, (rows,), dev, contiguous=True)
         return x.data_ptr(), 0
-    return None, int(x) if dtype is _I32 else float(x)
+    return None, max(-1, min(int(x), _MOST)) if dtype is _I32 else float(x)      # (top_k: more words than any row has)
 
 
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -1053,12 +1065,13 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     try:
         R, V = logits.shape
         dev, kind, ld = logits.device, logits.dtype, logits.stride(0)
-        fine = (logits.is_cuda and (kind is _F32 or kind is _BF16) and (logits.stride(1) == 1 or V <= 1) and (R <= 1 or ld >= V) and uniform.dtype is _F32 and uniform.shape == (R,)
+        fine = (logits.is_cuda and max(R, V) <= _MOST and (kind is _F32 or kind is _BF16) and (logits.stride(1) == 1 or V <= 1) and (R <= 1 or ld >= V) and uniform.dtype is _F32 and uniform.shape == (R,)
                 and uniform.is_contiguous() and uniform.device == dev)
     except (AttributeError, ValueError, IndexError):
         fine = False
     if not fine:
         _need(logits, "logits", (_F32, _BF16), 2, rows=True)
+        _whole(max(logits.shape), "a size of logits")
         _need(uniform, "uniform", (_F32,), 1, logits.shape[:1], logits.device, contiguous=True)
         raise ValueError("sample_tokens: rows must be contiguous")
     settings = [*_setting(temperature, "temperature", _F32, R, dev), *_setting(top_k, "top_k", _I32, R, dev), *_setting(top_p, "top_p", _F32, R, dev), *_setting(min_p, "min_p", _F32, R, dev)]

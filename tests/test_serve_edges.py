@@ -1,4 +1,4 @@
-"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range, words equal to the last that top_k keeps, draws without a GPU."""
+"""Calls of the serving operators and of the sampler at the edges of what they say of themselves: pools without a page, prompts that end inside a page, settings out of range, words equal to the last that top_k keeps, draws without a GPU, numbers of more than 32 bits."""
 import json
 import textwrap
 from pathlib import Path
@@ -7,7 +7,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from leopard_b200 import cli, ops
+from leopard_b200 import _lib, cli, ops
 from leopard_b200.sampling import Sampler, SamplingParams
 from oracle import serve as O
 from test_serve_ops import close
@@ -204,6 +204,30 @@ def test_the_least_top_p_without_a_gpu():
     least_top_p("cpu")
 
 
+# ------------------------------------------------------------------------------------------------------------ numbers of more than 32 bits
 @gpu
 def test_the_least_top_p():
     least_top_p("cuda")
+
+
+@gpu
+def test_a_top_k_of_more_than_32_bits_keeps_all():
+    z, u = torch.randn(6, 500, generator=gen(4), device="cuda"), torch.rand(6, generator=gen(5), device="cuda")
+    want = O.sample_tokens(z, u)
+    for top_k in (2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1, 2 ** 32 + 1, 2 ** 40, 2 ** 63 - 1):
+        assert ops.sample_tokens(z, u, top_k=top_k).tolist() == want, top_k
+    for top_k in (-2 ** 32, -2 ** 32 + 1, -2 ** 31):
+        with pytest.raises(_lib.NativeError, match="top_k"):
+            ops.sample_tokens(z, u, top_k=top_k)
+
+
+@gpu
+def test_sizes_of_more_than_32_bits_are_refused():
+    i32 = lambda x: torch.tensor(x, dtype=I32, device="cuda")  # noqa: E731
+    for size, rows in ((2 ** 32 + 16, 8), (2 ** 31, 8), (16, 2 ** 32 + 8), (16, 2 ** 31)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.step_tables(i32([5, 30]), i32([4, 4]), i32([[-1, -1, -1]] * 2), i32([3, 4, 5, 6]), i32([0]), size, rows)
+    q, k = torch.zeros(2, 1, 4, 64, dtype=BF16, device="cuda"), torch.zeros(9, 16, 2, 64, dtype=BF16, device="cuda")
+    for prefix in (2 ** 32 + 20, 2 ** 31, -2 ** 32):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.prefix_attention(q, k, k, i32([25, 25]), prefix, page_table=i32([[0, 1], [0, 2]]))
