@@ -1093,7 +1093,7 @@ int lp_prefix_attention(const lp_prefix_attn_desc* desc, void* workspace, size_t
 /* The next token of each row of logits (fp32 or bf16 [rows][ld], V <= 376832 words), by uniform[row] in [0, 1).  With w = exp((z - max z) / temperature) and the words in the order of their logits, the
  * largest first, equal ones by index: the first top_k are kept (0: all); of them those before which less than top_p of their mass lies, the first in any case; of them those with
  * w >= min_p; out[row] is the first kept word, by index, up to which more than uniform of the kept mass lies.  temperature 0 (negative, NaN): the largest, the first of equal ones.
- * Weights are held in units of 2^-43 of the largest, for top_p in units of 2^-35 (V > 131072: 2^-32).  Settings of each row, or (NULL) one for all.  -inf and NaN are never drawn; of a row with +inf entries only these are; a row with nothing
+ * Weights are held in units of 2^-43 of the largest, each less than one off, for top_p in units of 2^-35 (V > 131072: 2^-32), to nearest.  Settings of each row, or (NULL) one for all.  -inf and NaN are never drawn; of a row with +inf entries only these are; a row with nothing
  * to draw gives -1. */
 int lp_sample_tokens(const void* logits, int logits_fp32, long long ld, const float* uniform, const float* temperature, float temperature_all, const int* top_k, int top_k_all,
                      const float* top_p, float top_p_all, const float* min_p, float min_p_all, int rows, int V, long long* out, void* stream);

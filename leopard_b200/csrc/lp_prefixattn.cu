@@ -13,7 +13,8 @@ namespace lp {
 // what it sums over, so the dimensions of a head are dealt to the operands' places as the loads bring them: piece t + 4 c of a key's 16-byte pieces goes to places 2t, 2t + 1 and 2t + 8, 2t + 9 of steps
 // 2c and 2c + 1.  In the second product the dimensions are the rows, values of two keys put side by side by byte permutations.
 // Bound by HBM for many or long requests (300 own rows of 64, 32 heads over 8: 23 us, of which the tiles take 12, 6.6 TB/s, the first loads' latency 7), by latency else (4 rows a key head after 512 9 us).  Four CTAs an SM with
-// 8 rows, three with 16.
+// 8 rows, three with 16.  At 128 dimensions the former spill 110 to 140 bytes (the join 100).  Fewer CTAs an SM and no spills, in both kernels: 64 samples after 32,771 rows 77 us a call and 76, 16 after 1,000 24.6 and
+// 23.3, two after 4,796 22.5 and 24.6, four others the same.
 template <int D>
 constexpr int pa_ld() { return D / 4 + 1; }                       // 16-byte pieces from one row of a warp's sums to the next (eight rows' in eight different banks)
 template <int D, int NT>

@@ -4,14 +4,14 @@
 //   the first top_k (0: all),  of them those before which less than top_p of their mass lies (the first in any case),  of them those with w >= min_p,
 // and drawn is the first kept word, by index, up to which more than u of the kept mass lies.  t = 0 takes the largest.
 //
-// Weights are integers in units of 2^-43 (from a 64-bit exponential): their sums do not depend on the order in which they are taken, and the draw is the one that 64 bits give, but where a sum lies that near a
-// border.  What top_p sums up is in units of 2^-35 (vocabularies above 131,072: 2^-32): of two equal words and others below 2^-36 it takes the first alone at top_p 0.5, where the others' share would let
-// the second in.
+// Weights are integers in units of 2^-43 (from a 64-bit exponential), each less than one unit off: their sums do not depend on the order in which they are taken and are less than V units off, 4 x 10^-8 of the
+// largest weight for the largest vocabulary.  The draw is the one that 64 bits give, but where a sum lies that near a border.  What top_p sums up is in units of 2^-35 (vocabularies above 131,072:
+// 2^-32): of two equal words and others below 2^-36 it takes the first alone at top_p 0.5, where the others' share would let the second in.
 // A cluster of CTAs holds a row in shared memory, read once.  Nothing is sorted: what top_k and top_p keep ends at one word, which is found by counts and masses of 1,024 ranges of
 // logits, first of all of the row, then of the range where the limit lies, until the few words left in it are put in order one by one.  Where the words down to the limit are few altogether (a top_k of
 // 50 or 200, a sure model's top_p), one CTA takes them all and the others leave.
 // Bound by latency and by passes over shared memory, at two CTAs an SM: one row of 128,256 18 us (a barrier of the cluster takes 0.5 to 1, a load 2.5, counts 2, the few words 5), 64 rows of 128,256 28 (no limit), 36
-// (top_k 40) to 85 (top_p 0.9, when thousands of words are kept), 256 of 32,003 26; their bytes take 5.
+// (top_k 40) to 85 (top_p 0.9, when thousands of words are kept), 256 of 32,003 30, their logits not in L2; the bytes take 5.
 #include "lp_common.cuh"
 #include "lp_host.h"
 #include "../../include/leopard_b200.h"
@@ -67,8 +67,9 @@ __device__ const double SA_ROOT[64] = {      // 2^(i / 64)
     1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267, 1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
     1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062, 1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656, 1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
-// 2^(x / 64), x <= 0, to nearest: x = 64 e + i + r, |r| <= 1/2; 2^(i / 64) from the table, e^y, y = r ln 2 / 64, by its series to y^4 (the next term is 2^-44.6).  Added to a power of two, it is a whole number
-// in the sum's low bits: 512 makes units of 2^-43, 131072 of 2^-35, 2^20 of 2^-32; that power's own bits are left in.  Below x = -2944 (-inf among it) the result is that of about there, less than half a unit.
+// 2^(x / 64), x <= 0: x = 64 e + i + r, |r| <= 1/2; 2^(i / 64) from the table, e^y, y = r ln 2 / 64, by its series to y^4 (the next term is 2^-44.6).  Added to a power of two, it is a whole number
+// in the sum's low bits: 512 makes units of 2^-43 (off by 0.83 of one at most:
+// half for the whole number, a third for the series; 2 % are not the nearest), 131072 of 2^-35, 2^20 of 2^-32 (the nearest); that power's own bits are left in.  Below x = -2944 (-inf among it) the result is that of about there, less than half a unit.
 __device__ __forceinline__ u64 sa_weight_bits(double x, double power, const double* root) {
   x = __hiloint2double((int)min((unsigned)__double2hiint(x), 0xc0a70000u), __double2loint(x));
   const double m = x + 6755399441055744.0;                // 1.5 2^52: the whole number is in the low bits

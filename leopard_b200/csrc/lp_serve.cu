@@ -11,7 +11,8 @@ namespace lp {
 // Entries of the new rows' pages that are negative get the next pages of the free list, request after request and page after page.
 // One cluster does it all.  Its CTAs share the requests, count their rows and missing pages and tell one another; every CTA adds up all of them, gives its requests their pages and, when all have, writes its
 // share of the rows.  Bound by latency: the chain lengths -> table -> sums -> free list -> table -> slot, two barriers of the
-// cluster: one token of 64 requests 5.3 us, 63,897 rows of 256 prompts 9.3 and 5 for the rows.
+// cluster: one token of 64 requests 4 us,
+// 6 where all of them begin a page; 63,897 rows of 256 prompts 9.3 and 5 for the rows, 2 more where 4,385 pages are given out.
 constexpr int ST_MAX_BATCH = 8192, ST_FEW = 4;      // a span of more pages than ST_FEW is looked at by a whole warp
 
 struct StepTablesArgs {
