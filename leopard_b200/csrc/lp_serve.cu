@@ -213,7 +213,7 @@ step_rows_kernel(const __grid_constant__ StepTablesArgs a) {
 //   y[i], y[i'] = s (x[i] cos a - x[i'] sin a),  s (x[i'] cos a + x[i] sin a),   a = position f[i],  i' = i + n ("half") or the pairs (2i, 2i + 1) ("interleaved")
 // The inverse (the gradient) turns by -a.  The angle is formed in 64 bits, in turns, of which whole ones are dropped: at position 10^6 a 32-bit angle is off by 0.03.  A CTA knows the angles of a few rows
 // (shared memory) and turns all heads of them, 16 bytes and their partners a thread.  Bound by HBM: 16,384 rows of 32 heads of 128, bf16, 40 us, 6.7 TB/s; 4,796 of fp32 26.4, 5.9; 4,796 rows of 32 + 8 + 8 heads into
-// a cache 22.9, 5.2.  64 such rows 3.5 us.
+// a cache 22.9, 5.2.  64 such rows 3 us.
 constexpr int RO_MAX_FREQ = 256;
 
 struct RotarySeg {                        // heads of one tensor: x -> y
