@@ -48,9 +48,9 @@ def test_queries_are_turned_though_the_pool_has_no_rows(pages, size, G, dtype, l
     assert ops.rotary_append(q[:0], k[:0], v[:0], pos[:0], freq, *pools, slots[:0]).shape == (0, H, D)
 
 
-# ------------------------------------------------------------------------------------------------------------ a shared prompt, as the README has it
+# ------------------------------------------------------------------------------------------------------------ a shared prompt, as the user documentation has it
 def readme_steps():
-    """the README's lines for a shared prompt -> (those of the prompt, those of a step)"""
+    """the documented lines for a shared prompt -> (those of the prompt, those of a step)"""
     text = (Path(__file__).resolve().parents[1] / "README.md").read_text()
     text = text[text.index("## Serving many continuations of one prompt"):]
     code = textwrap.dedent("\n".join(line for line in text.splitlines() if line.startswith("    ")))
